@@ -62,6 +62,7 @@ class WeightRef(C.Structure):
 SQ_HOOK = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p)
 
 _vp, _i, _i64, _f, _u32, _u64, _d = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_uint32, C.c_uint64, C.c_double
+_sz = C.c_size_t
 
 # name -> (restype, argtypes); every function declared in include/aeth_galore.h
 SIGNATURES = {
@@ -122,6 +123,18 @@ SIGNATURES = {
     "aeth_fc_decode_nf4": (_i, [_vp, _i64, _f, _vp, _vp]),
     "aeth_bf16_sr_update": (_i, [_vp, _vp, _i64, C.POINTER(C.c_uint64), _vp, _vp]),
     "aeth_lomo_update": (_i, [_vp, _i64, _vp, _f, _f, _f, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "aeth_cut_ce_workspace": (_i, [_i64, _i64, _i64, _i, C.POINTER(C.c_size_t)]),
+    "aeth_cut_ce_forward": (_i, [_vp, _i64, _vp, _i64, _i, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "aeth_cut_ce_backward": (_i, [_vp, _i64, _vp, _i64, _i, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _f, _vp, _i64, _vp,
+                                  _i64, _vp, _sz, _vp]),
+    "aeth_rms_norm_checkpoint": (_i, [_vp, _i64, _vp, _i64, _vp, _i, _i, _i64, _i64, _f, _vp, _vp, _vp, _vp, _vp]),
+    "aeth_checkpoint_decode": (_i, [_vp, _vp, _i64, _i64, _vp, _i, _f, _vp, _i64, _i, _vp]),
+    "aeth_rms_norm_checkpoint_backward_workspace": (_i, [_i64, _i64, C.POINTER(C.c_size_t)]),
+    "aeth_rms_norm_checkpoint_backward": (_i, [_vp, _i64, _vp, _vp, _vp, _i, _vp, _i64, _i, _i64, _i64, _f, _vp, _vp,
+                                               _vp, _sz, _vp]),
+    "aeth_checkpoint_weight_grad_workspace": (_i, [_i64, _i64, _i64, C.POINTER(C.c_size_t)]),
+    "aeth_checkpoint_weight_grad": (_i, [_vp, _i64, _vp, _vp, _vp, _i, _f, _i, _i64, _i64, _i64, _vp, _i64, _vp, _sz,
+                                         _vp]),
     "aeth_status_string": (C.c_char_p, [_i]),
     "aeth_last_error": (_i, []),
     "aeth_device_error": (_i, [_i]),

@@ -5,9 +5,10 @@
 Run it as a script (or load it by file path): importing the package itself
 requires the built library.
 
-The library is a single translation unit (csrc/aeth_galore.cu) linked against
-the static CUDA runtime, so it only needs the driver on the machine that loads
-it.  No fast-math: the NF4/INT8 codes and the REF-mode arithmetic must round
+The library is two translation units, compiled side by side: csrc/aeth_galore.cu
+(the optimizer step) and csrc/aeth_train.cu (the training operators around it).
+It is linked against the static CUDA runtime, so it only needs the driver on the
+machine that loads it.  No fast-math: the NF4/INT8 codes and the REF-mode arithmetic must round
 exactly like the CPU definition.
 """
 from __future__ import annotations
@@ -15,6 +16,7 @@ from __future__ import annotations
 import argparse
 import glob
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -22,13 +24,15 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libaeth_galore.so")
+OBJ = os.path.join(HERE, "_obj")  # object files, kept so an unchanged unit is not compiled again
+UNITS = ("aeth_galore", "aeth_train")
 ROOT = os.path.dirname(HERE)
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
     "-Xcompiler", "-fPIC,-O2,-ffp-contract=off",
-    "-shared", "--expt-relaxed-constexpr",
+    "--expt-relaxed-constexpr",
     "-Xptxas", "-warn-spills",
 ]
 
@@ -52,19 +56,48 @@ def needs_build() -> bool:
     return any(os.path.getmtime(s) > t for s in sources())
 
 
+def stale(obj: str, unit: str) -> bool:
+    """Whether `unit`'s object is missing or older than the unit or any file it
+    includes (found by following the quoted includes)."""
+    if not os.path.exists(obj):
+        return True
+    seen, todo = set(), [os.path.join(CSRC, unit + ".cu")]
+    while todo:
+        f = os.path.normpath(todo.pop())
+        if f in seen:
+            continue
+        seen.add(f)
+        with open(f) as h:
+            todo += [os.path.join(os.path.dirname(f), m) for m in re.findall(r'^#include "([^"]+)"', h.read(), re.M)]
+    return any(os.path.getmtime(f) > os.path.getmtime(obj) for f in seen)
+
+
 def build(force: bool = False, verbose: bool = False, extra: list[str] | None = None) -> str:
     if not force and not needs_build():
         return LIB
-    cmd = [nvcc(), *NVCC_FLAGS, *(extra or []), "-I", os.path.join(ROOT, "include"),
-           os.path.join(CSRC, "aeth_galore.cu"), "-o", LIB + ".tmp"]
-    if verbose:
-        print(" ".join(cmd))
+    os.makedirs(OBJ, exist_ok=True)
+    compiles = []
+    for unit in UNITS:
+        obj = os.path.join(OBJ, unit + ".o")
+        src = os.path.join(CSRC, unit + ".cu")
+        if force or extra or stale(obj, unit):
+            cmd = [nvcc(), *NVCC_FLAGS, *(extra or []), "-I", os.path.join(ROOT, "include"), "-c", src, "-o", obj]
+            if verbose:
+                print(" ".join(cmd))
+            compiles.append(subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True))
+    for p in compiles:
+        out = p.communicate()[0]
+        if p.returncode != 0:
+            sys.stderr.write(out)
+        elif verbose and out:
+            print(out)
+    if any(p.returncode != 0 for p in compiles):
+        raise RuntimeError("nvcc failed building libaeth_galore.so")
+    cmd = [nvcc(), *NVCC_FLAGS[:2], "-shared", *[os.path.join(OBJ, u + ".o") for u in UNITS], "-o", LIB + ".tmp"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
-        raise RuntimeError("nvcc failed building libaeth_galore.so")
-    if verbose and (res.stdout or res.stderr):
-        print(res.stdout + res.stderr)
+        raise RuntimeError("nvcc failed linking libaeth_galore.so")
     os.replace(LIB + ".tmp", LIB)
     return LIB
 

@@ -1,0 +1,392 @@
+// aeth_train.cu -- libaeth_galore: the training operators around the optimizer
+// step (section 3b of include/aeth_galore.h): the head's loss and gradient, the
+// RMS norm whose input is kept in 8 bits, and the weight gradient taken from
+// that checkpoint.
+#include <algorithm>
+
+#include "checkpoint.cuh"
+#include "common.cuh"
+#include "head_loss.cuh"
+#include "pair_gemm.cuh"
+
+using namespace aeth;
+
+namespace {
+
+bool is16(int dtype) { return dtype == AETH_DTYPE_BF16 || dtype == AETH_DTYPE_F16; }
+bool known_dtype(int dtype) { return dtype == AETH_DTYPE_F32 || is16(dtype); }
+int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Carves a workspace into 256-byte aligned parts.
+struct Carver {
+    uint8_t* base;
+    size_t used = 0;
+    explicit Carver(void* p) : base(static_cast<uint8_t*>(p)) {}
+    template <typename T>
+    T* take(int64_t count) {
+        T* p = reinterpret_cast<T*>(base + used);
+        used += (size_t)up(count * (int64_t)sizeof(T), 256);
+        return p;
+    }
+};
+
+// ---------------------------------------------------------------------------
+// Head loss
+// ---------------------------------------------------------------------------
+constexpr int64_t kHeadMaxDim = 1ll << 30;       // token, feature and vocabulary counts (tile coordinates are int)
+constexpr int64_t kHeadGradBytes = 256ll << 20;  // G of one piece
+constexpr int kHeadBN = 256;
+
+struct HeadPlan {
+    int64_t n_pad, dp, piece, ldg;
+    int np;      // column ranges of the forward's statistics
+    int splits;  // K splits of a piece's dH product
+
+    HeadPlan(int64_t n, int64_t d, int64_t vocab) {
+        n_pad = up(std::max<int64_t>(n, 1), 256);
+        dp = up(d, 8);
+        np = 2 * (int)((vocab + kHeadBN - 1) / kHeadBN);
+        // pieces of equal size (a multiple of the tile) whose G takes at most kHeadGradBytes
+        int64_t most = std::max<int64_t>(kHeadGradBytes / (2 * n_pad) / kHeadBN * kHeadBN, kHeadBN);
+        const int64_t count = (vocab + most - 1) / most;
+        piece = std::min(up((vocab + count - 1) / count, kHeadBN), up(vocab, 8));
+        ldg = up(piece, 8);
+        // a piece's dH has few tiles where there are few tokens: its K (the piece) is then
+        // split so that every CTA pair has a unit, at least 8 k-blocks each
+        const int64_t tiles = n_pad / 256 * ((d + 255) / 256), kb = (piece + 63) / 64;
+        const int64_t s = std::max<int64_t>(std::min<int64_t>(74 / tiles, kb / 8), 1);
+        const int64_t per = (kb + s - 1) / s;
+        splits = (int)((kb + per - 1) / per);
+    }
+};
+
+struct HeadWork {
+    int *rows, *pos, *lab, *count;
+    uint16_t* h;
+    // forward
+    float* label_logit;
+    float2* part;
+    // backward
+    float *coef, *lse2, *out_scale, *slab;
+    uint16_t* g;
+    size_t bytes;
+
+    HeadWork(const HeadPlan& p, int64_t n, bool backward, void* ws) {
+        Carver c(ws);
+        rows = c.take<int>(p.n_pad);
+        pos = c.take<int>(std::max<int64_t>(n, 1));
+        lab = c.take<int>(p.n_pad);
+        count = c.take<int>(1);
+        h = c.take<uint16_t>(p.n_pad * p.dp);
+        label_logit = nullptr;
+        part = nullptr;
+        coef = lse2 = out_scale = slab = nullptr;
+        g = nullptr;
+        if (!backward) {
+            label_logit = c.take<float>(p.n_pad);
+            part = c.take<float2>((int64_t)p.np * p.n_pad);
+        } else {
+            coef = c.take<float>(p.n_pad);
+            lse2 = c.take<float>(p.n_pad);
+            out_scale = c.take<float>(1);
+            g = c.take<uint16_t>(p.n_pad * p.ldg);
+            slab = c.take<float>(p.splits * p.n_pad * p.dp);
+        }
+        bytes = c.used;
+    }
+};
+
+int head_check(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, int dtype,
+               const int64_t* labels, int64_t n, int64_t d, int64_t vocab) {
+    if (n < 0 || d <= 0 || vocab <= 0 || !weight || ld_weight < d) return AETH_ERR_ARG;
+    if (n > 0 && (!hidden || !labels || ld_hidden < d)) return AETH_ERR_ARG;
+    if (!known_dtype(dtype)) return AETH_ERR_ARG;
+    if (!is16(dtype)) return AETH_ERR_UNSUPPORTED;
+    if (n > kHeadMaxDim || d > kHeadMaxDim || vocab > kHeadMaxDim) return AETH_ERR_UNSUPPORTED;
+    if ((n + 255) / 256 * ((vocab + 255) / 256) > kHeadMaxDim) return AETH_ERR_UNSUPPORTED;
+    if (!aligned16(weight) || ld_weight % 8) return AETH_ERR_UNSUPPORTED;  // TMA reads the weight in place
+    return AETH_OK;
+}
+
+int head_rows(const HeadRows& a, const void* hidden, int64_t ld, int64_t d, const HeadPlan& p, const HeadWork& w,
+              cudaStream_t st) {
+    DeviceRuntime* rt = nullptr;
+    AETH_TRY(runtime_for_current(&rt));
+    head_rows_kernel<<<1, 1024, 0, st>>>(a, rt->err_word);
+    AETH_LAUNCH_CHECK();
+    head_pack_kernel<<<(unsigned)std::min<int64_t>(p.n_pad, 65536), 256, 0, st>>>(
+        static_cast<const uint16_t*>(hidden), ld, (int)d, w.rows, w.count, w.h, p.dp);
+    AETH_LAUNCH_CHECK();
+    return AETH_OK;
+}
+
+template <bool BF16>
+int head_backward(const HeadPlan& p, const HeadWork& w, const void* weight, int64_t ld_weight, int64_t n, int64_t d,
+                  int64_t vocab, void* d_hidden, int64_t ld_dh, void* d_weight, int64_t ld_dw, cudaStream_t st) {
+    const uint16_t* W = static_cast<const uint16_t*>(weight);
+    for (int64_t v0 = 0; v0 < vocab; v0 += p.piece) {
+        const int64_t vp = std::min(p.piece, vocab - v0);
+        const PairOperand H{w.h, p.dp, p.n_pad, d}, Wp{W + v0 * ld_weight, ld_weight, vp, d};
+        const PairOperand G{w.g, p.ldg, p.n_pad, vp};
+        HeadGrad<BF16> eg{w.lab, w.coef, w.lse2, w.g, p.ldg, (int)v0};
+        AETH_TRY((pair_gemm_launch<HeadGrad<BF16>, false, false>(H, Wp, (int)n, (int)vp, (int)d, w.count, PAIR_LIVE_M,
+                                                                 kHeadBN, 1, BF16, eg, st)));
+        if (d_weight) {
+            PairOut16<BF16> ew{static_cast<uint16_t*>(d_weight) + v0 * ld_dw, ld_dw, w.out_scale};
+            AETH_TRY((pair_gemm_launch<PairOut16<BF16>, true, true>(G, H, (int)vp, (int)d, (int)n, w.count, PAIR_LIVE_K,
+                                                                    256, 1, BF16, ew, st)));
+        }
+        if (d_hidden) {
+            const int64_t kb = (vp + 63) / 64, full = (p.piece + 63) / 64;
+            const int64_t per = (full + p.splits - 1) / p.splits;
+            PairSlab es{w.slab, p.dp, p.n_pad * p.dp, v0 == 0};
+            const int splits = (int)((kb + per - 1) / per);  // a shorter last piece fills fewer slabs
+            AETH_TRY((pair_gemm_launch<PairSlab, false, true>(G, Wp, (int)n, (int)d, (int)vp, w.count, PAIR_LIVE_M, 256,
+                                                              splits, BF16, es, st)));
+        }
+    }
+    if (d_hidden && n > 0) {
+        head_dh_kernel<BF16><<<(unsigned)std::min<int64_t>(n, 65536), 256, 0, st>>>(
+            w.slab, p.dp, p.n_pad * p.dp, p.splits, w.pos, n, (int)d, w.out_scale, static_cast<uint16_t*>(d_hidden),
+            ld_dh);
+        AETH_LAUNCH_CHECK();
+    }
+    return AETH_OK;
+}
+
+// ---------------------------------------------------------------------------
+// Checkpoints
+// ---------------------------------------------------------------------------
+constexpr int64_t kCkptMaxDim = 1ll << 30;
+constexpr int kGainRanges = 64;  // row ranges of d_gain's sum
+
+int ckpt_dims(int64_t rows, int64_t d, int dtype) {
+    if (rows < 0 || d <= 0 || !known_dtype(dtype)) return AETH_ERR_ARG;
+    if (rows > kCkptMaxDim || d > kCkptMaxDim) return AETH_ERR_UNSUPPORTED;
+    return AETH_OK;
+}
+
+unsigned row_grid(int64_t rows) { return (unsigned)std::min<int64_t>(rows, 65536); }
+
+template <typename F>
+int by_type(int dtype, F f) {
+    if (dtype == AETH_DTYPE_F32) return f((float*)nullptr);
+    if (dtype == AETH_DTYPE_F16) return f((__half*)nullptr);
+    return f((__nv_bfloat16*)nullptr);
+}
+
+int decode(const int8_t* codes, const float* scales, int64_t rows, int64_t d, const void* gain, int gain_dtype,
+           float eps, void* out, int64_t ld_out, int dtype, cudaStream_t st) {
+    return by_type(dtype, [&](auto* tag) {
+        using T = std::remove_pointer_t<decltype(tag)>;
+        ckpt_decode_kernel<T><<<row_grid(rows), 256, 0, st>>>(codes, scales, rows, (int)d, gain, gain_dtype, eps,
+                                                              static_cast<T*>(out), ld_out);
+        AETH_LAUNCH_CHECK();
+        return (int)AETH_OK;
+    });
+}
+
+}  // namespace
+
+extern "C" {
+
+int aeth_cut_ce_workspace(int64_t n, int64_t d, int64_t vocab, int backward, size_t* bytes) {
+    if (n < 0 || d <= 0 || vocab <= 0 || !bytes) return set_err(AETH_ERR_ARG);
+    if (n > kHeadMaxDim || d > kHeadMaxDim || vocab > kHeadMaxDim) return set_err(AETH_ERR_UNSUPPORTED);
+    *bytes = HeadWork(HeadPlan(n, d, vocab), n, backward != 0, nullptr).bytes;
+    return AETH_OK;
+}
+
+int aeth_cut_ce_forward(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, int dtype,
+                        const int64_t* labels, int64_t n, int64_t d, int64_t vocab, int64_t ignore_index,
+                        float* losses, float* lse, float* loss, void* workspace, size_t workspace_bytes,
+                        aeth_stream_t stream) {
+    AETH_TRY(head_check(hidden, ld_hidden, weight, ld_weight, dtype, labels, n, d, vocab));
+    if (!loss || (n > 0 && (!losses || !lse || !workspace))) return set_err(AETH_ERR_ARG);
+    cudaStream_t st = to_stream(stream);
+    if (n == 0) {
+        AETH_CUDA(cudaMemsetAsync(loss, 0, sizeof(float), st));
+        return AETH_OK;
+    }
+    const HeadPlan p(n, d, vocab);
+    const HeadWork w(p, n, false, workspace);
+    if (workspace_bytes < w.bytes || !aligned16(workspace)) return set_err(AETH_ERR_ARG);
+    HeadRows a = {};
+    a.labels = labels;
+    a.n = n;
+    a.ignore_index = ignore_index;
+    a.vocab = (int)vocab;
+    a.rows = w.rows;
+    a.pos = w.pos;
+    a.lab = w.lab;
+    a.count = w.count;
+    AETH_TRY(head_rows(a, hidden, ld_hidden, d, p, w, st));
+    HeadStats es{w.lab, w.label_logit, w.part, p.n_pad};
+    AETH_TRY((pair_gemm_launch<HeadStats, false, false>({w.h, p.dp, p.n_pad, d}, {weight, ld_weight, vocab, d}, (int)n,
+                                                        (int)vocab, (int)d, w.count, PAIR_LIVE_M, kHeadBN, 1,
+                                                        dtype == AETH_DTYPE_BF16, es, st)));
+    head_loss_kernel<<<(unsigned)std::min<int64_t>((n + 31) / 32, 65536), 256, 0, st>>>(
+        w.part, p.n_pad, p.np, w.label_logit, w.rows, w.count, losses, lse);
+    AETH_LAUNCH_CHECK();
+    head_mean_kernel<<<1, 1024, 0, st>>>(w.pos, n, w.count, losses, lse, loss);
+    AETH_LAUNCH_CHECK();
+    return AETH_OK;
+}
+
+int aeth_cut_ce_backward(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, int dtype,
+                         const int64_t* labels, int64_t n, int64_t d, int64_t vocab, int64_t ignore_index,
+                         const float* lse, const float* grad_losses, float scale, void* d_hidden, int64_t ld_dh,
+                         void* d_weight, int64_t ld_dw, void* workspace, size_t workspace_bytes,
+                         aeth_stream_t stream) {
+    AETH_TRY(head_check(hidden, ld_hidden, weight, ld_weight, dtype, labels, n, d, vocab));
+    if (!d_hidden && !d_weight) return set_err(AETH_ERR_ARG);
+    if ((d_hidden && ld_dh < d) || (d_weight && ld_dw < d)) return set_err(AETH_ERR_ARG);
+    if (n > 0 && (!lse || !workspace)) return set_err(AETH_ERR_ARG);
+    cudaStream_t st = to_stream(stream);
+    if (n == 0) {
+        if (d_weight)
+            AETH_CUDA(cudaMemset2DAsync(d_weight, (size_t)ld_dw * 2, 0, (size_t)d * 2, (size_t)vocab, st));
+        return AETH_OK;
+    }
+    const HeadPlan p(n, d, vocab);
+    const HeadWork w(p, n, true, workspace);
+    if (workspace_bytes < w.bytes || !aligned16(workspace)) return set_err(AETH_ERR_ARG);
+    const bool bf16 = dtype == AETH_DTYPE_BF16;
+    HeadRows a = {};
+    a.labels = labels;
+    a.n = n;
+    a.ignore_index = ignore_index;
+    a.vocab = (int)vocab;
+    a.rows = w.rows;
+    a.pos = w.pos;
+    a.lab = w.lab;
+    a.count = w.count;
+    a.lse = lse;
+    a.grad = grad_losses;
+    a.scale = scale;
+    a.g_bits = head_g_bits(bf16);
+    a.g_scale = head_g_scale(bf16);
+    a.coef = w.coef;
+    a.lse2 = w.lse2;
+    a.out_scale = w.out_scale;
+    AETH_TRY(head_rows(a, hidden, ld_hidden, d, p, w, st));
+    return bf16 ? head_backward<true>(p, w, weight, ld_weight, n, d, vocab, d_hidden, ld_dh, d_weight, ld_dw, st)
+                : head_backward<false>(p, w, weight, ld_weight, n, d, vocab, d_hidden, ld_dh, d_weight, ld_dw, st);
+}
+
+int aeth_rms_norm_checkpoint(const void* x, int64_t ld_x, const void* residual, int64_t ld_residual, const void* gain,
+                             int gain_dtype, int dtype, int64_t rows, int64_t d, float eps, void* sum_out, void* y,
+                             int8_t* codes, float* scales, aeth_stream_t stream) {
+    AETH_TRY(ckpt_dims(rows, d, dtype));
+    if (!gain || !known_dtype(gain_dtype)) return set_err(AETH_ERR_ARG);
+    if (rows == 0) return AETH_OK;
+    if (!x || !y || !codes || !scales || ld_x < d || (residual && (!sum_out || ld_residual < d)))
+        return set_err(AETH_ERR_ARG);
+    cudaStream_t st = to_stream(stream);
+    return by_type(dtype, [&](auto* tag) {
+        using T = std::remove_pointer_t<decltype(tag)>;
+        CkptStore<T> a{static_cast<const T*>(x), ld_x, static_cast<const T*>(residual), ld_residual, gain, gain_dtype,
+                       rows, (int)d, eps, static_cast<T*>(sum_out), static_cast<T*>(y), codes, scales};
+        ckpt_store_kernel<T><<<row_grid(rows), 256, 0, st>>>(a);
+        AETH_LAUNCH_CHECK();
+        return (int)AETH_OK;
+    });
+}
+
+int aeth_checkpoint_decode(const int8_t* codes, const float* scales, int64_t rows, int64_t d, const void* gain,
+                           int gain_dtype, float eps, void* out, int64_t ld_out, int dtype, aeth_stream_t stream) {
+    AETH_TRY(ckpt_dims(rows, d, dtype));
+    if (gain && !known_dtype(gain_dtype)) return set_err(AETH_ERR_ARG);
+    if (rows == 0) return AETH_OK;
+    if (!codes || !scales || !out || ld_out < d) return set_err(AETH_ERR_ARG);
+    return decode(codes, scales, rows, d, gain, gain_dtype, eps, out, ld_out, dtype, to_stream(stream));
+}
+
+int aeth_rms_norm_checkpoint_backward_workspace(int64_t rows, int64_t d, size_t* bytes) {
+    AETH_TRY(ckpt_dims(rows, d, AETH_DTYPE_F32));
+    if (!bytes) return set_err(AETH_ERR_ARG);
+    Carver c(nullptr);
+    c.take<float>(std::max<int64_t>(rows, 1));
+    c.take<float>(kGainRanges * d);
+    *bytes = c.used;
+    return AETH_OK;
+}
+
+int aeth_rms_norm_checkpoint_backward(const void* dy, int64_t ld_dy, const int8_t* codes, const float* scales,
+                                      const void* gain, int gain_dtype, const void* d_residual, int64_t ld_residual,
+                                      int dtype, int64_t rows, int64_t d, float eps, void* dx, float* d_gain,
+                                      void* workspace, size_t workspace_bytes, aeth_stream_t stream) {
+    AETH_TRY(ckpt_dims(rows, d, dtype));
+    if (!gain || !known_dtype(gain_dtype) || !d_gain) return set_err(AETH_ERR_ARG);
+    cudaStream_t st = to_stream(stream);
+    if (rows == 0) {
+        AETH_CUDA(cudaMemsetAsync(d_gain, 0, sizeof(float) * (size_t)d, st));
+        return AETH_OK;
+    }
+    if (!dy || !codes || !scales || !dx || ld_dy < d || (d_residual && ld_residual < d) || !workspace)
+        return set_err(AETH_ERR_ARG);
+    Carver c(workspace);
+    float* rstd = c.take<float>(rows);
+    float* part = c.take<float>(kGainRanges * d);
+    if (workspace_bytes < c.used || !aligned16(workspace)) return set_err(AETH_ERR_ARG);
+    const int64_t per = (rows + kGainRanges - 1) / kGainRanges;
+    const int ranges = (int)((rows + per - 1) / per);
+    return by_type(dtype, [&](auto* tag) {
+        using T = std::remove_pointer_t<decltype(tag)>;
+        CkptBack<T> a{static_cast<const T*>(dy), ld_dy, codes, scales, gain, gain_dtype,
+                      static_cast<const T*>(d_residual), ld_residual, rows, (int)d, eps, static_cast<T*>(dx), rstd};
+        ckpt_back_kernel<T><<<row_grid(rows), 256, 0, st>>>(a);
+        AETH_LAUNCH_CHECK();
+        const unsigned cols = (unsigned)((d + 127) / 128);
+        ckpt_gain_partial_kernel<T><<<dim3(cols, ranges), 128, 0, st>>>(a.dy, ld_dy, codes, scales, rstd, rows, (int)d,
+                                                                        per, part);
+        AETH_LAUNCH_CHECK();
+        ckpt_gain_sum_kernel<<<cols, 128, 0, st>>>(part, ranges, (int)d, d_gain);
+        AETH_LAUNCH_CHECK();
+        return (int)AETH_OK;
+    });
+}
+
+int aeth_checkpoint_weight_grad_workspace(int64_t rows, int64_t m, int64_t d, size_t* bytes) {
+    AETH_TRY(ckpt_dims(rows, d, AETH_DTYPE_F32));
+    if (m <= 0 || !bytes) return set_err(AETH_ERR_ARG);
+    Carver c(nullptr);
+    c.take<uint16_t>(std::max<int64_t>(rows, 1) * up(d, 8));
+    *bytes = c.used;
+    return AETH_OK;
+}
+
+int aeth_checkpoint_weight_grad(const void* dy, int64_t ld_dy, const int8_t* codes, const float* scales,
+                                const void* gain, int gain_dtype, float eps, int dtype, int64_t rows, int64_t m,
+                                int64_t d, void* d_weight, int64_t ld_dw, void* workspace, size_t workspace_bytes,
+                                aeth_stream_t stream) {
+    AETH_TRY(ckpt_dims(rows, d, dtype));
+    if (m <= 0 || !d_weight || ld_dw < d || (gain && !known_dtype(gain_dtype))) return set_err(AETH_ERR_ARG);
+    if (!is16(dtype) || m > kCkptMaxDim) return set_err(AETH_ERR_UNSUPPORTED);
+    if ((m + 255) / 256 * ((d + 255) / 256) > kCkptMaxDim) return set_err(AETH_ERR_UNSUPPORTED);
+    cudaStream_t st = to_stream(stream);
+    if (rows == 0) {
+        AETH_CUDA(cudaMemset2DAsync(d_weight, (size_t)ld_dw * 2, 0, (size_t)d * 2, (size_t)m, st));
+        return AETH_OK;
+    }
+    if (!dy || !codes || !scales || !workspace || ld_dy < m) return set_err(AETH_ERR_ARG);
+    if (!aligned16(dy) || ld_dy % 8) return set_err(AETH_ERR_UNSUPPORTED);  // TMA reads dY in place
+    Carver c(workspace);
+    const int64_t dp = up(d, 8);
+    uint16_t* xr = c.take<uint16_t>(rows * dp);
+    if (workspace_bytes < c.used || !aligned16(workspace)) return set_err(AETH_ERR_ARG);
+    AETH_TRY(decode(codes, scales, rows, d, gain, gain_dtype, eps, xr, dp, dtype, st));
+    const bool bf16 = dtype == AETH_DTYPE_BF16;
+    const PairOperand A{dy, ld_dy, rows, m}, B{xr, dp, rows, d};
+    if (bf16) {
+        PairOut16<true> e{static_cast<uint16_t*>(d_weight), ld_dw, nullptr};
+        return pair_gemm_launch<PairOut16<true>, true, true>(A, B, (int)m, (int)d, (int)rows, nullptr, PAIR_LIVE_NONE,
+                                                             256, 1, true, e, st);
+    }
+    PairOut16<false> e{static_cast<uint16_t*>(d_weight), ld_dw, nullptr};
+    return pair_gemm_launch<PairOut16<false>, true, true>(A, B, (int)m, (int)d, (int)rows, nullptr, PAIR_LIVE_NONE, 256,
+                                                          1, false, e, st);
+}
+
+}  // extern "C"

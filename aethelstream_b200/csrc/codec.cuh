@@ -157,19 +157,6 @@ inline int codec_maps_ensure() {
     return AETH_OK;
 }
 
-// Linear INT8 encode with the reference's rounding (half away from zero).
-__device__ __forceinline__ int8_t lin_encode(float x, float inv) {
-    float q = roundf(__fmul_rn(x, inv));
-    q = fminf(fmaxf(q, -127.0f), 127.0f);
-    return (int8_t)(int)q;
-}
-
-__device__ __forceinline__ float lin_scale_from_absmax(float amax) {
-    return amax <= 0.0f ? 1.0f : __fdiv_rn(amax, 127.0f);
-}
-
-__device__ __forceinline__ float lin_inv(float scale) { return scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f; }
-
 // Nearest entry of a sorted 256-entry map held in shared memory.
 __device__ __forceinline__ uint32_t dmap_encode(const float* __restrict__ map, float xn) {
     int lo = 0;

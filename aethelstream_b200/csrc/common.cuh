@@ -228,6 +228,19 @@ __device__ __forceinline__ void atomic_max_nonneg(float* addr, float v) {
     atomicMax(reinterpret_cast<unsigned int*>(addr), __float_as_uint(v));
 }
 
+// Linear INT8 encode with the reference's rounding (half away from zero).
+__device__ __forceinline__ int8_t lin_encode(float x, float inv) {
+    float q = roundf(__fmul_rn(x, inv));
+    q = fminf(fmaxf(q, -127.0f), 127.0f);
+    return (int8_t)(int)q;
+}
+
+__device__ __forceinline__ float lin_scale_from_absmax(float amax) {
+    return amax <= 0.0f ? 1.0f : __fdiv_rn(amax, 127.0f);
+}
+
+__device__ __forceinline__ float lin_inv(float scale) { return scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f; }
+
 inline int grid_for(int64_t work, int threads, int cap = 148 * 16) {
     int64_t g = (work + threads - 1) / threads;
     if (g < 1) g = 1;

@@ -1,0 +1,383 @@
+// pair_gemm.cuh -- the matrix product of the training operators: a persistent
+// tcgen05 GEMM on CTA pairs, D (M x N) = A (M x K) B (K x N), 16-bit operands,
+// fp32 accumulation in TMEM, the epilogue a functor.
+//
+// Unit = (256 x bn tile of D, K split); each CTA of the pair holds its 128 rows
+// of A and half of the tile's bn columns of B per 64-deep k-block, CTA 0 issues
+// the pair's MMAs (M = 256, N = bn) and its commits reach both CTAs' barriers.
+// 256 x 256 is the largest tile whose accumulator fits TMEM twice (2 x 256
+// columns), so the epilogue of one tile runs under the MMAs of the next; each
+// CTA then loads 32 KB per k-block of 512 MMA cycles.  Warps: 0 = TMEM
+// allocation + TMA producer, 1 = MMA issuer, 2..9 = epilogue (warp w reads TMEM
+// lane quarter w % 4; warps 2-5 take the first half of the columns, 6-9 the
+// second).
+//
+// M or K may be held on the device (`live`): the number of rows that a mask
+// leaves.  Operand rows past it, up to the next multiple of 256, must be zero.
+// Tiles are walked in groups of kGroupM row tiles so that the tiles in flight
+// share their operands in L2.
+#pragma once
+#include "tmap.cuh"
+#include "umma.cuh"
+
+namespace aeth {
+
+constexpr int kPairEpiWarps = 8;
+constexpr int kPairThreads = 64 + 32 * kPairEpiWarps;
+constexpr int kPairStages = 6;
+constexpr int kPairOperand = 128 * 64 * 2;                  // one operand of one stage and CTA
+constexpr int kPairStage = 2 * kPairOperand;
+constexpr int kPairStaging = 32 * 128;                      // per epilogue warp: 32 rows x 128 bytes
+constexpr int kPairBar = 256;
+constexpr int kPairSmem = 1024 + kPairStages * kPairStage + kPairEpiWarps * kPairStaging + kPairBar;
+constexpr int kGroupM = 8;
+
+enum PairLive { PAIR_LIVE_NONE = 0, PAIR_LIVE_M = 1, PAIR_LIVE_K = 2 };
+
+struct PairGemm {
+    CUtensorMap tmA;  // K-major: box 64 (K) x 128; MN-major: box 64 (M) x 64 (K)
+    CUtensorMap tmB;  // K-major: box 64 (K) x bn / 2; MN-major: box 64 (N) x 64 (K)
+    const int* live;  // device count that replaces M or K
+    int live_dim;     // PairLive
+    int M, N, K;
+    int bn;           // columns per tile: a multiple of 32 (128 where B is MN-major), at most 256
+    int splits;       // of K; each split is a unit of its own
+    uint32_t idesc;
+};
+
+// The part of D that an epilogue call covers: this warp's 32 rows, its columns.
+struct PairTile {
+    uint32_t tmem;     // address of (this warp's lane quarter, the tile's first column)
+    int row0;          // first of the warp's 32 rows of D
+    int col0;          // first column of the tile
+    int c_begin, c_end;  // this warp's columns within the tile (multiples of 32)
+    int n_tile, half;
+    int split;
+    int M, N;          // live sizes
+    uint8_t* staging;  // kPairStaging bytes of this warp alone
+    int lane;
+};
+
+struct PairUnit {
+    int m0, n0, n_tile, split, kb0, kb1;
+};
+
+struct PairShape {
+    int M, K, tiles_m, tiles_n, kb, kb_split, total;
+    __device__ explicit PairShape(const PairGemm& g) {
+        M = g.M;
+        K = g.K;
+        if (g.live_dim == PAIR_LIVE_M) M = *g.live;
+        if (g.live_dim == PAIR_LIVE_K) K = *g.live;
+        tiles_m = max((M + 255) / 256, 1);
+        tiles_n = (g.N + g.bn - 1) / g.bn;
+        kb = max((K + 63) / 64, 1);
+        kb_split = (kb + g.splits - 1) / g.splits;
+        total = tiles_m * tiles_n * g.splits;
+    }
+    __device__ PairUnit unit(const PairGemm& g, int u) const {
+        const int per = tiles_m * tiles_n;
+        PairUnit t;
+        t.split = u / per;
+        const int r = u - t.split * per;
+        const int grp = r / (kGroupM * tiles_n);
+        const int first = grp * kGroupM;
+        const int gm = min(kGroupM, tiles_m - first);
+        const int rr = r - grp * kGroupM * tiles_n;
+        t.n_tile = rr / gm;
+        t.m0 = (first + rr - t.n_tile * gm) * 256;
+        t.n0 = t.n_tile * g.bn;
+        t.kb0 = t.split * kb_split;
+        t.kb1 = min(t.kb0 + kb_split, kb);
+        return t;
+    }
+};
+
+template <class Epi, bool A_MN, bool B_MN>
+__global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid_constant__ PairGemm g, const Epi epi,
+                                                                     uint32_t* err) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);  // stays a shared pointer
+    uint8_t* sA = base;
+    uint8_t* sB = base + kPairStages * kPairOperand;
+    uint8_t* staging = base + kPairStages * kPairStage;
+    uint64_t* full = reinterpret_cast<uint64_t*>(staging + kPairEpiWarps * kPairStaging);
+    uint64_t* empty = full + kPairStages;
+    uint64_t* acc_full = empty + kPairStages;
+    uint64_t* acc_empty = acc_full + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    static_assert((2 * kPairStages + 4) * 8 + 8 <= kPairBar, "barriers must fit the barrier area");
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int crank = (int)cluster_ctarank();
+    const int ustart = (int)(blockIdx.x >> 1), ustep = (int)(gridDim.x >> 1);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kPairStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        // acc_empty (CTA 0): one arrival per epilogue warp of both CTAs
+        for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * kPairEpiWarps); }
+        *abort = 0;
+        fence_mbar_init();
+    }
+    if (warp == 0) { tmem_alloc_pair(tmem_slot, 512); tmem_relinquish_pair(); }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const PairShape sh(g);
+
+    if (warp == 0) {
+        if (lane == 0) {
+            const int half_n = g.bn / 2;
+            const uint32_t bytes = 2u * (uint32_t)(kPairOperand + half_n * 64 * 2);  // both CTAs
+            int it = 0;
+            for (int u = ustart; u < sh.total && !*abort; u += ustep) {
+                const PairUnit t = sh.unit(g, u);
+                const int m0 = t.m0 + crank * 128, n0 = t.n0 + crank * half_n;
+                for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
+                    const int s = it % kPairStages;
+                    const uint32_t ph = (uint32_t)(it / kPairStages) & 1u;
+                    if (!mbar_wait(&empty[s], ph ^ 1u, abort, err, DEVERR_TIMEOUT_TMA)) break;
+                    if (crank == 0) mbar_arrive_expect_tx(&full[s], bytes);
+                    uint8_t* a = sA + s * kPairOperand;
+                    uint8_t* b = sB + s * kPairOperand;
+                    if (A_MN) {
+                        tma_load_2d_pair(a, &g.tmA, &full[s], m0, kb * 64);
+                        tma_load_2d_pair(a + 8192, &g.tmA, &full[s], m0 + 64, kb * 64);
+                    } else {
+                        tma_load_2d_pair(a, &g.tmA, &full[s], kb * 64, m0);
+                    }
+                    if (B_MN) {
+                        for (int c = 0; c < half_n; c += 64)
+                            tma_load_2d_pair(b + c * 128, &g.tmB, &full[s], n0 + c, kb * 64);
+                    } else {
+                        tma_load_2d_pair(b, &g.tmB, &full[s], kb * 64, n0);
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && crank == 0) {
+            int it = 0, j = 0;
+            for (int u = ustart; u < sh.total && !*abort; u += ustep, ++j) {
+                const PairUnit t = sh.unit(g, u);
+                const int b = j & 1;
+                if (!mbar_wait(&acc_empty[b], ((uint32_t)(j >> 1) & 1u) ^ 1u, abort, err, DEVERR_TIMEOUT_MMA)) break;
+                tc_fence_after();
+                const uint32_t d = tmem + (uint32_t)(b * 256);
+                for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
+                    const int s = it % kPairStages;
+                    const uint32_t ph = (uint32_t)(it / kPairStages) & 1u;
+                    if (!mbar_wait(&full[s], ph, abort, err, DEVERR_TIMEOUT_MMA)) break;
+                    tc_fence_after();
+                    const uint32_t a_addr = smem_u32(sA + s * kPairOperand);
+                    const uint32_t b_addr = smem_u32(sB + s * kPairOperand);
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {
+                        const uint64_t ad = A_MN ? sdesc_sw128(a_addr + kk * 2048, 8192, 1024)
+                                                 : sdesc_sw128(a_addr + kk * 32, 16, 1024);
+                        const uint64_t bd = B_MN ? sdesc_sw128(b_addr + kk * 2048, 8192, 1024)
+                                                 : sdesc_sw128(b_addr + kk * 32, 16, 1024);
+                        umma_f16_ss_pair(d, ad, bd, g.idesc, (kb > t.kb0 || kk > 0) ? 1u : 0u);
+                    }
+                    umma_commit_pair(&empty[s]);
+                }
+                umma_commit_pair(&acc_full[b]);
+            }
+        }
+    } else {
+        const int ew = warp - 2;
+        const int q = warp & 3;
+        const int mid = (g.bn / 32 + 1) / 2 * 32;  // columns of the first half: a multiple of 32
+        PairTile tile;
+        tile.half = ew >> 2;
+        tile.c_begin = tile.half ? mid : 0;
+        tile.c_end = tile.half ? g.bn : mid;
+        tile.M = sh.M;
+        tile.N = g.N;
+        tile.staging = staging + ew * kPairStaging;
+        tile.lane = lane;
+        int j = 0;
+        for (int u = ustart; u < sh.total; u += ustep, ++j) {
+            const PairUnit t = sh.unit(g, u);
+            const int b = j & 1;
+            if (!mbar_wait(&acc_full[b], (uint32_t)(j >> 1) & 1u, abort, err, DEVERR_TIMEOUT_EPI) || *abort) break;
+            tc_fence_after();
+            tile.tmem = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(b * 256);
+            tile.row0 = t.m0 + crank * 128 + q * 32;
+            tile.col0 = t.n0;
+            tile.n_tile = t.n_tile;
+            tile.split = t.split;
+            epi.tile(tile);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(smem_leader(&acc_empty[b]));
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // the pair's MMAs and both epilogues are done with TMEM
+    if (warp == 0) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem, 512);
+    }
+}
+
+// Writes 32 columns of the warp's 32 rows (thread = row, v = its values, times
+// alpha) as 16-bit values: through the warp's staging area, so that each row's
+// 64 bytes go out as four 16-byte pieces of neighbouring lanes.  ld and out
+// decide the piece: whole pieces where every row starts on 16 bytes, else
+// single values.
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+    uint32_t r;
+    if (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// out16: element (r, c) of a matrix with row pitch ld; rows < rows, columns < cols are written.
+__device__ __forceinline__ void pair_store16(const PairTile& t, const uint32_t (&w)[32], int c, uint16_t* out,
+                                             int64_t ld, int rows, int cols) {
+    // 64 columns: 32 words per row, chunk k (16 bytes) of row r at k ^ (r & 7)
+    const int row = t.lane;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+        *reinterpret_cast<uint4*>(t.staging + row * 128 + ((k ^ (row & 7)) * 16)) =
+            make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+    __syncwarp();
+    const bool whole = (ld % 8) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = i * 4 + (t.lane >> 3), k = t.lane & 7;
+        const int gr = t.row0 + r, gc = t.col0 + c + k * 8;
+        const uint4 v = *reinterpret_cast<const uint4*>(t.staging + r * 128 + ((k ^ (r & 7)) * 16));
+        if (gr < rows && gc < cols) {
+            uint16_t* o = out + (int64_t)gr * ld + gc;
+            if (whole && gc + 8 <= cols) {
+                *reinterpret_cast<uint4*>(o) = v;
+            } else {
+                const uint32_t ww[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (gc + e < cols) o[e] = (uint16_t)(ww[e >> 1] >> (16 * (e & 1)));
+            }
+        }
+    }
+    __syncwarp();
+}
+
+// Epilogue: D times a device scale, in 16 bits.
+template <bool BF16>
+struct PairOut16 {
+    uint16_t* out;
+    int64_t ld;
+    const float* scale;  // device; null: 1
+    __device__ __forceinline__ void tile(const PairTile& t) const {
+        const float a = scale ? *scale : 1.0f;
+        for (int c = t.c_begin; c < t.c_end; c += 64) {
+            if (t.col0 + c >= t.N || t.row0 >= t.M) break;
+            uint32_t w[32];
+            float v[32];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (c + 32 * h < t.c_end) {
+                    tmem_ld32<0>(t.tmem + (uint32_t)(c + 32 * h), v);
+                    tmem_wait_ld();
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) w[16 * h + i] = pack16<BF16>(v[2 * i] * a, v[2 * i + 1] * a);
+            }
+            pair_store16(t, w, c, out, ld, t.M, min(t.N, t.col0 + t.c_end));
+        }
+    }
+};
+
+// Epilogue: D in fp32 into slab[split], stored by the first K range of a sum
+// and added by the later ones.  Each element has one writer per launch, so the
+// order of a sum is the order of the launches.
+struct PairSlab {
+    float* slab;
+    int64_t ld, split_stride;  // ld a multiple of 4
+    int first;
+    __device__ __forceinline__ void tile(const PairTile& t) const {
+        float* base = slab + (int64_t)t.split * split_stride;
+        for (int c = t.c_begin; c < t.c_end; c += 32) {
+            if (t.col0 + c >= t.N || t.row0 >= t.M) break;
+            float v[32];
+            tmem_ld32<0>(t.tmem + (uint32_t)c, v);
+            tmem_wait_ld();
+            const int row = t.lane;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                *reinterpret_cast<float4*>(t.staging + row * 128 + ((k ^ (row & 7)) * 16)) =
+                    make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = i * 4 + (t.lane >> 3), k = t.lane & 7;
+                const int gr = t.row0 + r, gc = t.col0 + c + k * 4;
+                float4 x = *reinterpret_cast<const float4*>(t.staging + r * 128 + ((k ^ (r & 7)) * 16));
+                if (gr < t.M && gc < ld) {
+                    float4* o = reinterpret_cast<float4*>(base + (int64_t)gr * ld + gc);
+                    if (!first) {
+                        const float4 p = *o;
+                        x = make_float4(p.x + x.x, p.y + x.y, p.z + x.z, p.w + x.w);
+                    }
+                    *o = x;
+                }
+            }
+            __syncwarp();
+        }
+    }
+};
+
+// ---- host ----
+struct PairOperand {
+    const void* ptr;
+    int64_t ld;    // row pitch in elements
+    int64_t rows;  // rows that may be read (K rows where MN-major, M or N rows where K-major)
+    int64_t cols;
+};
+
+template <class Epi, bool A_MN, bool B_MN>
+int pair_gemm_launch(PairOperand A, PairOperand B, int M, int N, int K, const int* live, int live_dim, int bn,
+                     int splits, bool bf16, const Epi& epi, cudaStream_t st) {
+    DeviceRuntime* rt = nullptr;
+    AETH_TRY(runtime_for_current(&rt));
+    PairGemm g;
+    AETH_TRY(make_tmap_16b(&g.tmA, A.ptr, (uint64_t)A.cols, (uint64_t)A.rows, A.ld, 64, A_MN ? 64 : 128, bf16));
+    AETH_TRY(make_tmap_16b(&g.tmB, B.ptr, (uint64_t)B.cols, (uint64_t)B.rows, B.ld, 64, B_MN ? 64 : bn / 2, bf16));
+    g.live = live;
+    g.live_dim = live_dim;
+    g.M = M;
+    g.N = N;
+    g.K = K;
+    g.bn = bn;
+    g.splits = splits;
+    g.idesc = idesc_f16(256, bn, bf16, A_MN, B_MN);
+    auto kern = pair_gemm_kernel<Epi, A_MN, B_MN>;
+    static std::atomic<bool> attr_set[kMaxDevices] = {};
+    int dev = 0;
+    AETH_TRY(current_device(&dev));
+    if (!attr_set[dev].load(std::memory_order_acquire)) {
+        AETH_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
+        attr_set[dev].store(true, std::memory_order_release);
+    }
+    const int64_t units = (int64_t)((M + 255) / 256) * ((N + bn - 1) / bn) * splits;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * (unsigned)std::min<int64_t>(units, num_sms() / 2));
+    cfg.blockDim = dim3(kPairThreads);
+    cfg.dynamicSmemBytes = kPairSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim = {2, 1, 1};
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    AETH_CUDA(cudaLaunchKernelEx(&cfg, kern, g, epi, rt->err_word));
+    return AETH_OK;
+}
+
+}  // namespace aeth

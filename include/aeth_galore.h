@@ -504,6 +504,79 @@ int aeth_lomo_update(const void* grad_bf16, int64_t n, const double* sq_dev, flo
                      float* prequant_out, aeth_stream_t stream);
 
 /* ======================================================================
+ * 3b. Training operators around the step: the loss at the head, the norm whose
+ *     input is kept in 8 bits, and the weight gradient taken from that
+ *     checkpoint.  Their outputs are the gradients that section 2 consumes.
+ *     All matrices are row-major device buffers with a row pitch (ld_*) in
+ *     elements; scratch comes from the caller (`workspace`, 16-byte aligned,
+ *     at least the bytes that the *_workspace function gives; its contents
+ *     need not be kept between calls).  Nothing synchronises or allocates, so
+ *     every call can be captured into a CUDA graph.
+ * ====================================================================== */
+
+/* Softmax cross entropy of s = hidden weight^T (streaming_cut_ce,
+ * doublepass/src/loss.rs:83-377) without keeping the logits.
+ *   hidden n x d, weight vocab x d: both F16 or both BF16 (F32:
+ *   AETH_ERR_UNSUPPORTED); weight 16-byte aligned with ld_weight % 8 == 0.
+ *   labels[t]: the vocabulary entry, or ignore_index.  Tokens with ignore_index
+ *   are left out altogether (loss 0, lse 0, gradient 0, whatever their hidden
+ *   state holds).  A label outside the vocabulary sets AETH_DEVERR_BAD_ARG,
+ *   gives that token a NaN loss (so the mean is NaN) and no gradient.
+ *   forward: losses[t] = lse_t - s_t,label (n floats), lse (n floats, for the
+ *   backward), *loss = the mean over the tokens that take part (0 if none).
+ *   backward: with g_t = scale * grad_losses[t], or scale / count where
+ *   grad_losses is NULL (the mean's gradient), and G = g_t (softmax - onehot):
+ *   d_hidden = G weight, d_weight = G^T hidden, in the inputs' type; either may
+ *   be NULL.  G exists for one vocabulary piece at a time, in 16 bits (at most
+ *   256 MiB). */
+int aeth_cut_ce_workspace(int64_t n, int64_t d, int64_t vocab, int backward, size_t* bytes);
+int aeth_cut_ce_forward(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, int dtype,
+                        const int64_t* labels, int64_t n, int64_t d, int64_t vocab, int64_t ignore_index,
+                        float* losses, float* lse, float* loss, void* workspace, size_t workspace_bytes,
+                        aeth_stream_t stream);
+int aeth_cut_ce_backward(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, int dtype,
+                         const int64_t* labels, int64_t n, int64_t d, int64_t vocab, int64_t ignore_index,
+                         const float* lse, const float* grad_losses, float scale, void* d_hidden, int64_t ld_dh,
+                         void* d_weight, int64_t ld_dw, void* workspace, size_t workspace_bytes,
+                         aeth_stream_t stream);
+
+/* RMS norm (doublepass/src/math.rs) with its input kept in 8 bits (the role of
+ * ramflow/kernels/checkpoint_compress.cu, with scales per row and block of 128
+ * features instead of per channel).  s = x, or x + residual rounded to the
+ * activations' type and written to sum_out; y = s / sqrt(mean s^2 + eps) * gain.
+ *   codes rows x d, scales rows x ceil(d / 128): scale = max|s| / 127 of the
+ *   block (1 where that maximum is below 2^-119), code = clamp(round(s *
+ *   (1 / scale)), +-127), halves away from zero.  A block that holds a NaN or
+ *   an infinity gets a NaN scale and restores to NaN.
+ * dtype F32, F16 or BF16 for x, residual, sum_out and y; gain has a type of its
+ * own.  sum_out, y and codes are contiguous. */
+int aeth_rms_norm_checkpoint(const void* x, int64_t ld_x, const void* residual, int64_t ld_residual, const void* gain,
+                             int gain_dtype, int dtype, int64_t rows, int64_t d, float eps, void* sum_out, void* y,
+                             int8_t* codes, float* scales, aeth_stream_t stream);
+/* out = code * scale, or its RMS norm times gain where gain is not NULL (the
+ * second pass's recomputed norm). */
+int aeth_checkpoint_decode(const int8_t* codes, const float* scales, int64_t rows, int64_t d, const void* gain,
+                           int gain_dtype, float eps, void* out, int64_t ld_out, int dtype, aeth_stream_t stream);
+/* The norm's gradient at the restored x: with r = 1 / sqrt(mean x^2 + eps),
+ * dx = r dy gain - x r^3 mean(dy gain x) (+ d_residual), d_gain = sum over rows
+ * of dy x r (F32).  dx is contiguous. */
+int aeth_rms_norm_checkpoint_backward_workspace(int64_t rows, int64_t d, size_t* bytes);
+int aeth_rms_norm_checkpoint_backward(const void* dy, int64_t ld_dy, const int8_t* codes, const float* scales,
+                                      const void* gain, int gain_dtype, const void* d_residual, int64_t ld_residual,
+                                      int dtype, int64_t rows, int64_t d, float eps, void* dx, float* d_gain,
+                                      void* workspace, size_t workspace_bytes, aeth_stream_t stream);
+
+/* Weight gradient of a linear layer whose input is kept in 8 bits:
+ * d_weight (m x d) = dy^T X, dy rows x m, X the restored checkpoint, or its RMS
+ * norm times gain where gain is not NULL.  X is rounded to dtype (F16 or BF16)
+ * for the tensor cores.  dy 16-byte aligned with ld_dy % 8 == 0. */
+int aeth_checkpoint_weight_grad_workspace(int64_t rows, int64_t m, int64_t d, size_t* bytes);
+int aeth_checkpoint_weight_grad(const void* dy, int64_t ld_dy, const int8_t* codes, const float* scales,
+                                const void* gain, int gain_dtype, float eps, int dtype, int64_t rows, int64_t m,
+                                int64_t d, void* d_weight, int64_t ld_dw, void* workspace, size_t workspace_bytes,
+                                aeth_stream_t stream);
+
+/* ======================================================================
  * 4. Errors and build information.
  * ====================================================================== */
 const char* aeth_status_string(int status);
