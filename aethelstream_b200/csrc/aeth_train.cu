@@ -3,6 +3,7 @@
 // RMS norm whose input is kept in 8 bits, and the weight gradient taken from
 // that checkpoint.
 #include <algorithm>
+#include <type_traits>
 
 #include "checkpoint.cuh"
 #include "common.cuh"
@@ -159,7 +160,6 @@ int head_backward(const HeadPlan& p, const HeadWork& w, const void* weight, int6
 // Checkpoints
 // ---------------------------------------------------------------------------
 constexpr int64_t kCkptMaxDim = 1ll << 30;
-constexpr int kGainRanges = 64;  // row ranges of d_gain's sum
 
 int ckpt_dims(int64_t rows, int64_t d, int dtype) {
     if (rows < 0 || d <= 0 || !known_dtype(dtype)) return AETH_ERR_ARG;
@@ -167,7 +167,28 @@ int ckpt_dims(int64_t rows, int64_t d, int dtype) {
     return AETH_OK;
 }
 
-unsigned row_grid(int64_t rows) { return (unsigned)std::min<int64_t>(rows, 65536); }
+// How a kernel that holds rows in registers is laid out: vpt eights of
+// features a thread, tx threads a row, ty rows a CTA.
+struct RowPlan {
+    int vpt, tx, ty;
+    bool wide;
+    unsigned grid;
+
+    // per_sm: CTAs an SM is given (they walk over the rows)
+    RowPlan(int64_t rows, int64_t d, int per_sm, int vpt_many = 4) {
+        const int64_t nv = (d + 7) / 8;
+        wide = nv > 1024;
+        // A row spread over four times the threads has the shorter chain of loads, which
+        // counts when there are too few rows to fill the SMs.
+        vpt = wide || rows > 2 * num_sms() ? vpt_many : 1;
+        const int most = 1024 / vpt;
+        tx = wide ? most : (int)((nv + vpt - 1) / vpt + 31) / 32 * 32;
+        ty = (int)std::max<int64_t>(std::min<int64_t>(256 / tx, rows), 1);
+        grid = (unsigned)std::min<int64_t>((rows + ty - 1) / ty, (int64_t)num_sms() * per_sm);
+    }
+    dim3 block() const { return dim3(tx, ty); }
+};
+constexpr int kStorePerSm = 8, kBackPerSm = 2;
 
 template <typename F>
 int by_type(int dtype, F f) {
@@ -176,12 +197,38 @@ int by_type(int dtype, F f) {
     return f((__nv_bfloat16*)nullptr);
 }
 
-int decode(const int8_t* codes, const float* scales, int64_t rows, int64_t d, const void* gain, int gain_dtype,
-           float eps, void* out, int64_t ld_out, int dtype, cudaStream_t st) {
+template <int V>
+using Int = std::integral_constant<int, V>;
+
+// f(type tag, vpt, vec, wide) with the last three as compile-time constants
+template <int VPT, typename F>
+int by_row(int dtype, const RowPlan& p, bool vec, F f) {
     return by_type(dtype, [&](auto* tag) {
+        if (p.wide) return vec ? f(tag, Int<VPT>(), Int<1>(), Int<1>()) : f(tag, Int<VPT>(), Int<0>(), Int<1>());
+        if (p.vpt > 1) return vec ? f(tag, Int<VPT>(), Int<1>(), Int<0>()) : f(tag, Int<VPT>(), Int<0>(), Int<0>());
+        return vec ? f(tag, Int<1>(), Int<1>(), Int<0>()) : f(tag, Int<1>(), Int<0>(), Int<0>());
+    });
+}
+
+// Whether rows of pitch ld at p can be taken in eights of `size` bytes each
+bool vec_rows(const void* p, int64_t ld, int size) {
+    const int bytes = std::min(8 * size, 16);
+    return reinterpret_cast<uintptr_t>(p) % bytes == 0 && ld * size % bytes == 0;
+}
+int type_size(int dtype) { return dtype == AETH_DTYPE_F32 ? 4 : 2; }
+
+int decode(const CkptRead& a, void* out, int64_t ld_out, int dtype, cudaStream_t st) {
+    const bool vec = a.d % 8 == 0 && vec_rows(a.codes, a.d, 1) && vec_rows(out, ld_out, type_size(dtype));
+    RowPlan p(a.rows, a.d, kStorePerSm);
+    return by_row<4>(dtype, p, vec, [&](auto* tag, auto vpt, auto v, auto wide) {
         using T = std::remove_pointer_t<decltype(tag)>;
-        ckpt_decode_kernel<T><<<row_grid(rows), 256, 0, st>>>(codes, scales, rows, (int)d, gain, gain_dtype, eps,
-                                                              static_cast<T*>(out), ld_out);
+        T* o = static_cast<T*>(out);
+        if (a.gain) {
+            ckpt_norm_kernel<T, vpt.value, v.value, wide.value><<<p.grid, p.block(), 0, st>>>(a, o, ld_out);
+        } else {
+            const unsigned spans = (unsigned)((a.d + 8 * p.vpt * p.tx - 1) / (8 * p.vpt * p.tx));
+            ckpt_decode_kernel<T, vpt.value, v.value><<<dim3(p.grid, spans), p.block(), 0, st>>>(a, o, ld_out);
+        }
         AETH_LAUNCH_CHECK();
         return (int)AETH_OK;
     });
@@ -284,11 +331,15 @@ int aeth_rms_norm_checkpoint(const void* x, int64_t ld_x, const void* residual, 
     if (!x || !y || !codes || !scales || ld_x < d || (residual && (!sum_out || ld_residual < d)))
         return set_err(AETH_ERR_ARG);
     cudaStream_t st = to_stream(stream);
-    return by_type(dtype, [&](auto* tag) {
+    const int sz = type_size(dtype);
+    const bool vec = d % 8 == 0 && vec_rows(x, ld_x, sz) && vec_rows(y, d, sz) && vec_rows(codes, d, 1) &&
+                     (!residual || (vec_rows(residual, ld_residual, sz) && vec_rows(sum_out, d, sz)));
+    const RowPlan p(rows, d, kStorePerSm);
+    return by_row<4>(dtype, p, vec, [&](auto* tag, auto vpt, auto v, auto wide) {
         using T = std::remove_pointer_t<decltype(tag)>;
         CkptStore<T> a{static_cast<const T*>(x), ld_x, static_cast<const T*>(residual), ld_residual, gain, gain_dtype,
                        rows, (int)d, eps, static_cast<T*>(sum_out), static_cast<T*>(y), codes, scales};
-        ckpt_store_kernel<T><<<row_grid(rows), 256, 0, st>>>(a);
+        ckpt_store_kernel<T, vpt.value, v.value, wide.value><<<p.grid, p.block(), 0, st>>>(a);
         AETH_LAUNCH_CHECK();
         return (int)AETH_OK;
     });
@@ -300,15 +351,15 @@ int aeth_checkpoint_decode(const int8_t* codes, const float* scales, int64_t row
     if (gain && !known_dtype(gain_dtype)) return set_err(AETH_ERR_ARG);
     if (rows == 0) return AETH_OK;
     if (!codes || !scales || !out || ld_out < d) return set_err(AETH_ERR_ARG);
-    return decode(codes, scales, rows, d, gain, gain_dtype, eps, out, ld_out, dtype, to_stream(stream));
+    return decode({codes, scales, gain, gain_dtype, rows, (int)d, eps}, out, ld_out, dtype, to_stream(stream));
 }
 
 int aeth_rms_norm_checkpoint_backward_workspace(int64_t rows, int64_t d, size_t* bytes) {
     AETH_TRY(ckpt_dims(rows, d, AETH_DTYPE_F32));
     if (!bytes) return set_err(AETH_ERR_ARG);
+    const RowPlan p(std::max<int64_t>(rows, 1), d, kBackPerSm, 2);
     Carver c(nullptr);
-    c.take<float>(std::max<int64_t>(rows, 1));
-    c.take<float>(kGainRanges * d);
+    c.take<float>((int64_t)p.grid * p.ty * d);
     *bytes = c.used;
     return AETH_OK;
 }
@@ -326,23 +377,20 @@ int aeth_rms_norm_checkpoint_backward(const void* dy, int64_t ld_dy, const int8_
     }
     if (!dy || !codes || !scales || !dx || ld_dy < d || (d_residual && ld_residual < d) || !workspace)
         return set_err(AETH_ERR_ARG);
+    const RowPlan p(rows, d, kBackPerSm, 2);
     Carver c(workspace);
-    float* rstd = c.take<float>(rows);
-    float* part = c.take<float>(kGainRanges * d);
+    float* part = c.take<float>((int64_t)p.grid * p.ty * d);
     if (workspace_bytes < c.used || !aligned16(workspace)) return set_err(AETH_ERR_ARG);
-    const int64_t per = (rows + kGainRanges - 1) / kGainRanges;
-    const int ranges = (int)((rows + per - 1) / per);
-    return by_type(dtype, [&](auto* tag) {
+    const int sz = type_size(dtype);
+    const bool vec = d % 8 == 0 && vec_rows(dy, ld_dy, sz) && vec_rows(dx, d, sz) && vec_rows(codes, d, 1) &&
+                     (!d_residual || vec_rows(d_residual, ld_residual, sz));
+    return by_row<2>(dtype, p, vec, [&](auto* tag, auto vpt, auto v, auto wide) {
         using T = std::remove_pointer_t<decltype(tag)>;
-        CkptBack<T> a{static_cast<const T*>(dy), ld_dy, codes, scales, gain, gain_dtype,
-                      static_cast<const T*>(d_residual), ld_residual, rows, (int)d, eps, static_cast<T*>(dx), rstd};
-        ckpt_back_kernel<T><<<row_grid(rows), 256, 0, st>>>(a);
+        CkptBack<T> a{{codes, scales, gain, gain_dtype, rows, (int)d, eps}, static_cast<const T*>(dy), ld_dy,
+                      static_cast<const T*>(d_residual), ld_residual, static_cast<T*>(dx), part};
+        ckpt_back_kernel<T, vpt.value, v.value, wide.value><<<p.grid, p.block(), 0, st>>>(a);
         AETH_LAUNCH_CHECK();
-        const unsigned cols = (unsigned)((d + 127) / 128);
-        ckpt_gain_partial_kernel<T><<<dim3(cols, ranges), 128, 0, st>>>(a.dy, ld_dy, codes, scales, rstd, rows, (int)d,
-                                                                        per, part);
-        AETH_LAUNCH_CHECK();
-        ckpt_gain_sum_kernel<<<cols, 128, 0, st>>>(part, ranges, (int)d, d_gain);
+        ckpt_gain_sum_kernel<<<(unsigned)((d + 31) / 32), 256, 0, st>>>(part, (int)p.grid * p.ty, (int)d, d_gain);
         AETH_LAUNCH_CHECK();
         return (int)AETH_OK;
     });
@@ -376,7 +424,7 @@ int aeth_checkpoint_weight_grad(const void* dy, int64_t ld_dy, const int8_t* cod
     const int64_t dp = up(d, 8);
     uint16_t* xr = c.take<uint16_t>(rows * dp);
     if (workspace_bytes < c.used || !aligned16(workspace)) return set_err(AETH_ERR_ARG);
-    AETH_TRY(decode(codes, scales, rows, d, gain, gain_dtype, eps, xr, dp, dtype, st));
+    AETH_TRY(decode({codes, scales, gain, gain_dtype, rows, (int)d, eps}, xr, dp, dtype, st));
     const bool bf16 = dtype == AETH_DTYPE_BF16;
     const PairOperand A{dy, ld_dy, rows, m}, B{xr, dp, rows, d};
     if (bf16) {
