@@ -175,20 +175,42 @@ struct RowPlan {
     unsigned grid;
 
     // per_sm: CTAs an SM is given (they walk over the rows)
-    RowPlan(int64_t rows, int64_t d, int per_sm, int vpt_many = 4) {
+    RowPlan(int64_t rows, int64_t d, int per_sm) {
         const int64_t nv = (d + 7) / 8;
         wide = nv > 1024;
         // A row spread over four times the threads has the shorter chain of loads, which
         // counts when there are too few rows to fill the SMs.
-        vpt = wide || rows > 2 * num_sms() ? vpt_many : 1;
+        vpt = wide || rows > 2 * num_sms() ? 4 : 1;
         const int most = 1024 / vpt;
         tx = wide ? most : (int)((nv + vpt - 1) / vpt + 31) / 32 * 32;
         ty = (int)std::max<int64_t>(std::min<int64_t>(256 / tx, rows), 1);
         grid = (unsigned)std::min<int64_t>((rows + ty - 1) / ty, (int64_t)num_sms() * per_sm);
     }
     dim3 block() const { return dim3(tx, ty); }
+    // dynamic shared memory: rows of 4 bytes a feature (gain where it is kept there, and `more`)
+    int shared(int more = 0) const {
+        return ((ck_shared_gain(vpt, wide) ? 1 : 0) + (wide ? 0 : more)) * vpt * tx * 32;
+    }
 };
-constexpr int kStorePerSm = 8, kBackPerSm = 2;
+constexpr int kStorePerSm = 8, kBackPerSm = 3;
+
+// The ring's layout for rows of d features: groups of tx threads that hold a
+// row in four eights each, as many stages as shared memory takes beside gain.
+// Taken for many rows (each SM walks over several) that bulk copies can move.
+CkptRing ring_plan(int64_t d, int size, bool res) {
+    CkptRing r;
+    r.tx = (int)((d + 1023) / 1024) * 32;
+    r.groups = kRingThreads / r.tx;
+    const int row = (int)up(d * size, 128);
+    r.res_at = row;
+    r.codes_at = row * (res ? 2 : 1);
+    r.stage_bytes = r.codes_at + (int)up(d, 128);
+    const int room = 220 * 1024 - 4 * 8 * 4 * r.tx;
+    while (r.groups > 1 && room / r.stage_bytes / r.groups < 2) r.groups /= 2;  // two stages a group at least
+    r.stages = std::min(room / r.stage_bytes / r.groups, kRingMaxStages);
+    return r;
+}
+bool ring_fits(int64_t rows, int64_t d) { return rows > 2 * num_sms() && d % 16 == 0 && d >= 256 && d <= 8192; }
 
 template <typename F>
 int by_type(int dtype, F f) {
@@ -201,11 +223,11 @@ template <int V>
 using Int = std::integral_constant<int, V>;
 
 // f(type tag, vpt, vec, wide) with the last three as compile-time constants
-template <int VPT, typename F>
+template <typename F>
 int by_row(int dtype, const RowPlan& p, bool vec, F f) {
     return by_type(dtype, [&](auto* tag) {
-        if (p.wide) return vec ? f(tag, Int<VPT>(), Int<1>(), Int<1>()) : f(tag, Int<VPT>(), Int<0>(), Int<1>());
-        if (p.vpt > 1) return vec ? f(tag, Int<VPT>(), Int<1>(), Int<0>()) : f(tag, Int<VPT>(), Int<0>(), Int<0>());
+        if (p.wide) return vec ? f(tag, Int<4>(), Int<1>(), Int<1>()) : f(tag, Int<4>(), Int<0>(), Int<1>());
+        if (p.vpt > 1) return vec ? f(tag, Int<4>(), Int<1>(), Int<0>()) : f(tag, Int<4>(), Int<0>(), Int<0>());
         return vec ? f(tag, Int<1>(), Int<1>(), Int<0>()) : f(tag, Int<1>(), Int<0>(), Int<0>());
     });
 }
@@ -218,13 +240,18 @@ bool vec_rows(const void* p, int64_t ld, int size) {
 int type_size(int dtype) { return dtype == AETH_DTYPE_F32 ? 4 : 2; }
 
 int decode(const CkptRead& a, void* out, int64_t ld_out, int dtype, cudaStream_t st) {
-    const bool vec = a.d % 8 == 0 && vec_rows(a.codes, a.d, 1) && vec_rows(out, ld_out, type_size(dtype));
+    const bool vec = a.d % 8 == 0 && vec_rows(a.codes, a.d, 1) && vec_rows(out, ld_out, type_size(dtype)) &&
+                     (!a.gain || aligned16(a.gain));
     RowPlan p(a.rows, a.d, kStorePerSm);
-    return by_row<4>(dtype, p, vec, [&](auto* tag, auto vpt, auto v, auto wide) {
+    return by_row(dtype, p, vec, [&](auto* tag, auto vpt, auto v, auto wide) {
         using T = std::remove_pointer_t<decltype(tag)>;
         T* o = static_cast<T*>(out);
         if (a.gain) {
-            ckpt_norm_kernel<T, vpt.value, v.value, wide.value><<<p.grid, p.block(), 0, st>>>(a, o, ld_out);
+            ckpt_norm_kernel<T, vpt.value, v.value, wide.value><<<p.grid, p.block(), p.shared(), st>>>(a, o, ld_out);
+        } else if (vec && a.d % kCkptBlock == 0 && ld_out == a.d && aligned16(a.codes) && aligned16(out)) {
+            const int64_t n16 = a.rows * a.d / 16;
+            ckpt_decode_flat_kernel<T><<<(unsigned)std::min<int64_t>((n16 + 1023) / 1024, 1 << 20), 256, 0, st>>>(
+                reinterpret_cast<const uint4*>(a.codes), a.scales, n16, o);
         } else {
             const unsigned spans = (unsigned)((a.d + 8 * p.vpt * p.tx - 1) / (8 * p.vpt * p.tx));
             ckpt_decode_kernel<T, vpt.value, v.value><<<dim3(p.grid, spans), p.block(), 0, st>>>(a, o, ld_out);
@@ -332,14 +359,14 @@ int aeth_rms_norm_checkpoint(const void* x, int64_t ld_x, const void* residual, 
         return set_err(AETH_ERR_ARG);
     cudaStream_t st = to_stream(stream);
     const int sz = type_size(dtype);
-    const bool vec = d % 8 == 0 && vec_rows(x, ld_x, sz) && vec_rows(y, d, sz) && vec_rows(codes, d, 1) &&
+    const bool vec = d % 8 == 0 && aligned16(gain) && vec_rows(x, ld_x, sz) && vec_rows(y, d, sz) && vec_rows(codes, d, 1) &&
                      (!residual || (vec_rows(residual, ld_residual, sz) && vec_rows(sum_out, d, sz)));
     const RowPlan p(rows, d, kStorePerSm);
-    return by_row<4>(dtype, p, vec, [&](auto* tag, auto vpt, auto v, auto wide) {
+    return by_row(dtype, p, vec, [&](auto* tag, auto vpt, auto v, auto wide) {
         using T = std::remove_pointer_t<decltype(tag)>;
         CkptStore<T> a{static_cast<const T*>(x), ld_x, static_cast<const T*>(residual), ld_residual, gain, gain_dtype,
                        rows, (int)d, eps, static_cast<T*>(sum_out), static_cast<T*>(y), codes, scales};
-        ckpt_store_kernel<T, vpt.value, v.value, wide.value><<<p.grid, p.block(), 0, st>>>(a);
+        ckpt_store_kernel<T, vpt.value, v.value, wide.value><<<p.grid, p.block(), p.shared(), st>>>(a);
         AETH_LAUNCH_CHECK();
         return (int)AETH_OK;
     });
@@ -357,9 +384,9 @@ int aeth_checkpoint_decode(const int8_t* codes, const float* scales, int64_t row
 int aeth_rms_norm_checkpoint_backward_workspace(int64_t rows, int64_t d, size_t* bytes) {
     AETH_TRY(ckpt_dims(rows, d, AETH_DTYPE_F32));
     if (!bytes) return set_err(AETH_ERR_ARG);
-    const RowPlan p(std::max<int64_t>(rows, 1), d, kBackPerSm, 2);
+    const RowPlan p(std::max<int64_t>(rows, 1), d, kBackPerSm);
     Carver c(nullptr);
-    c.take<float>((int64_t)p.grid * p.ty * d);
+    c.take<float>(std::max<int64_t>((int64_t)p.grid * p.ty, num_sms()) * d);
     *bytes = c.used;
     return AETH_OK;
 }
@@ -377,20 +404,36 @@ int aeth_rms_norm_checkpoint_backward(const void* dy, int64_t ld_dy, const int8_
     }
     if (!dy || !codes || !scales || !dx || ld_dy < d || (d_residual && ld_residual < d) || !workspace)
         return set_err(AETH_ERR_ARG);
-    const RowPlan p(rows, d, kBackPerSm, 2);
+    const RowPlan p(rows, d, kBackPerSm);
     Carver c(workspace);
-    float* part = c.take<float>((int64_t)p.grid * p.ty * d);
+    float* part = c.take<float>(std::max<int64_t>((int64_t)p.grid * p.ty, num_sms()) * d);
     if (workspace_bytes < c.used || !aligned16(workspace)) return set_err(AETH_ERR_ARG);
     const int sz = type_size(dtype);
-    const bool vec = d % 8 == 0 && vec_rows(dy, ld_dy, sz) && vec_rows(dx, d, sz) && vec_rows(codes, d, 1) &&
+    const bool vec = d % 8 == 0 && aligned16(gain) && vec_rows(dy, ld_dy, sz) && vec_rows(dx, d, sz) && vec_rows(codes, d, 1) &&
                      (!d_residual || vec_rows(d_residual, ld_residual, sz));
-    return by_row<2>(dtype, p, vec, [&](auto* tag, auto vpt, auto v, auto wide) {
+    DeviceRuntime* rt = nullptr;
+    AETH_TRY(runtime_for_current(&rt));
+    return by_row(dtype, p, vec, [&](auto* tag, auto vpt, auto v, auto wide) {
         using T = std::remove_pointer_t<decltype(tag)>;
         CkptBack<T> a{{codes, scales, gain, gain_dtype, rows, (int)d, eps}, static_cast<const T*>(dy), ld_dy,
                       static_cast<const T*>(d_residual), ld_residual, static_cast<T*>(dx), part};
-        ckpt_back_kernel<T, vpt.value, v.value, wide.value><<<p.grid, p.block(), 0, st>>>(a);
+        if (vec && ring_fits(rows, d) && aligned16(codes)) {
+            const CkptRing r = ring_plan(d, sz, d_residual != nullptr);
+            const int smem = r.groups * r.stages * r.stage_bytes + 4 * 8 * 4 * r.tx;
+            auto kern = ckpt_back_ring_kernel<T>;
+            AETH_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+            kern<<<num_sms(), r.groups * r.tx, smem, st>>>(a, r, rt->err_word);
+            AETH_LAUNCH_CHECK();
+            ckpt_gain_sum_kernel<<<(unsigned)((d + 31) / 32), 1024, 0, st>>>(part, num_sms(), (int)d, d_gain);
+            AETH_LAUNCH_CHECK();
+            return (int)AETH_OK;
+        }
+        auto kern = ckpt_back_kernel<T, vpt.value, v.value, wide.value>;
+        const int smem = p.shared(p.ty);
+        if (smem > 48 * 1024) AETH_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        kern<<<p.grid, p.block(), smem, st>>>(a);
         AETH_LAUNCH_CHECK();
-        ckpt_gain_sum_kernel<<<(unsigned)((d + 31) / 32), 256, 0, st>>>(part, (int)p.grid * p.ty, (int)d, d_gain);
+        ckpt_gain_sum_kernel<<<(unsigned)((d + 31) / 32), 1024, 0, st>>>(part, (int)p.grid * p.ty, (int)d, d_gain);
         AETH_LAUNCH_CHECK();
         return (int)AETH_OK;
     });

@@ -16,7 +16,7 @@
 //   d_gain = sum over rows of dy x^ r
 // Sums are fp32.
 #pragma once
-#include "common.cuh"
+#include "umma.cuh"
 
 namespace aeth {
 
@@ -76,6 +76,39 @@ __device__ __forceinline__ Pack8<T> ck_pack(const float (&v)[8]) {
     return p;
 }
 
+// Read once: past L1, so that it keeps the gain.
+__device__ __forceinline__ uint4 ck_stream(const uint4* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint2 ck_stream(const uint2* p) {
+    uint2 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+
+// The same from a row in shared memory.
+template <typename T>
+__device__ __forceinline__ Pack8<T> ck_shared8(const uint8_t* row, int c) {
+    Pack8<T> p;
+#pragma unroll
+    for (int k = 0; k < Pack8<T>::kWords; ++k) p.w[k] = reinterpret_cast<const uint4*>(row + (size_t)c * sizeof(T))[k];
+    return p;
+}
+
+// Makes the second pass over a row unpack its values again: kept unpacked
+// across the barrier they would take two to four times the registers.
+__device__ __forceinline__ void ck_opaque(uint2& q) { asm volatile("" : "+r"(q.x), "+r"(q.y)::"memory"); }
+template <typename T>
+__device__ __forceinline__ void ck_opaque(Pack8<T>& p) {
+#pragma unroll
+    for (int k = 0; k < Pack8<T>::kWords; ++k)
+        asm volatile("" : "+r"(p.w[k].x), "+r"(p.w[k].y), "+r"(p.w[k].z), "+r"(p.w[k].w)::"memory");
+}
+
 // Features c .. c + 7 of a row of d (zero past its end).  VEC: every row
 // starts on 16 bytes and d is a multiple of 8; otherwise single elements.
 template <typename T, bool VEC>
@@ -84,7 +117,7 @@ __device__ __forceinline__ Pack8<T> ck_load8(const T* row, int c, int d) {
     if (VEC) {
 #pragma unroll
         for (int k = 0; k < Pack8<T>::kWords; ++k)
-            p.w[k] = c < d ? __ldg(reinterpret_cast<const uint4*>(row + c) + k) : make_uint4(0, 0, 0, 0);
+            p.w[k] = c < d ? ck_stream(reinterpret_cast<const uint4*>(row + c) + k) : make_uint4(0, 0, 0, 0);
     } else {
         float v[8];
 #pragma unroll
@@ -107,7 +140,7 @@ __device__ __forceinline__ void ck_store8(T* row, int c, int d, const Pack8<T>& 
 }
 template <bool VEC>
 __device__ __forceinline__ uint2 ck_load_codes(const int8_t* row, int c, int d) {
-    if (VEC) return c < d ? __ldg(reinterpret_cast<const uint2*>(row + c)) : make_uint2(0, 0);
+    if (VEC) return c < d ? ck_stream(reinterpret_cast<const uint2*>(row + c)) : make_uint2(0, 0);
     uint32_t w[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -124,14 +157,65 @@ __device__ __forceinline__ void ck_store_codes(int8_t* row, int c, int d, uint2 
             if (c + i < d) row[c + i] = (int8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
     }
 }
+// The value of code i (the conversion instruction takes a byte of a register).
 __device__ __forceinline__ float ck_code(uint2 q, int i) {
     return (float)(int8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
 }
 
-// gain has a type of its own
+// gain has a type of its own.
 __device__ __forceinline__ void ck_gain8(const void* gain, int dtype, int c, int d, float (&g)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) g[i] = c + i < d ? load_as_f32(gain, c + i, dtype) : 0.0f;
+}
+
+// Eight floats of a thread in shared memory, [k][half][thread of the row], so
+// that neighbouring lanes take neighbouring 16 bytes.
+__device__ __forceinline__ float4& ck_slot(float4* base, int k, int half) {
+    return base[(2 * k + half) * blockDim.x + threadIdx.x];
+}
+template <int VPT>
+__device__ __forceinline__ void ck_gain_to_shared(float4* sg, const void* gain, int dtype, int d) {
+    if (threadIdx.y == 0)
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            float g[8];
+            ck_gain8(gain, dtype, 8 * (threadIdx.x + k * blockDim.x), d, g);
+            ck_slot(sg, k, 0) = make_float4(g[0], g[1], g[2], g[3]);
+            ck_slot(sg, k, 1) = make_float4(g[4], g[5], g[6], g[7]);
+        }
+    __syncthreads();
+}
+__device__ __forceinline__ void ck_slot8(float4* base, int k, float (&g)[8]) {
+    const float4 a = ck_slot(base, k, 0), b = ck_slot(base, k, 1);
+    g[0] = a.x; g[1] = a.y; g[2] = a.z; g[3] = a.w;
+    g[4] = b.x; g[5] = b.y; g[6] = b.z; g[7] = b.w;
+}
+
+// Two floats in one 64-bit register, for chains of packed arithmetic.
+__device__ __forceinline__ uint64_t f2(float a, float b) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ float2 f2_get(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
 }
 
 // Scale of a block from its maximum magnitude (NaN where the block held one).
@@ -140,50 +224,106 @@ __device__ __forceinline__ float ck_scale(float amax) {
     return amax < 1.504632769e-36f ? 1.0f : __fdiv_rn(amax, 127.0f);
 }
 
-// round_half_away(x / scale's rounded reciprocal): adding a half of x's sign
-// with rounding toward zero never carries a value below k - 1/2 up to k, so the
-// truncation of that sum is the rounding.  |x| <= 127 scale (1 + 2^-22) in a
-// block, so the sum stays below 128 and needs no clamp.
+// round_half_away(x * inv): adding a half of x's sign with rounding toward zero
+// never carries a value below k - 1/2 up to k, so the truncation of that sum is
+// the rounding.  |x * inv| <= 127 (1 + 2^-22) in a block, so the sum stays below
+// 128 and needs no clamp; a NaN (the NaN scale's reciprocal) converts to 0.
 __device__ __forceinline__ int ck_round(float v) {
     return __float2int_rz(__fadd_rz(v, __uint_as_float((__float_as_uint(v) & 0x80000000u) | 0x3f000000u)));
 }
-__device__ __forceinline__ uint2 ck_encode8(const float (&x)[8], float scale) {
-    if (scale != scale) return make_uint2(0, 0);
-    const float inv = __frcp_rn(scale);
+__device__ __forceinline__ uint2 ck_encode8(const float (&x)[8], float inv) {
     int q[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = ck_round(__fmul_rn(x[i], inv));
+    for (int i = 0; i < 8; i += 2) {
+        const float2 v = mul2_rn(make_float2(x[i], x[i + 1]), make_float2(inv, inv));
+        q[i] = ck_round(v.x);
+        q[i + 1] = ck_round(v.y);
+    }
     const uint32_t a = __byte_perm(q[0], q[1], 0x0040), b = __byte_perm(q[2], q[3], 0x0040);
     const uint32_t c = __byte_perm(q[4], q[5], 0x0040), e = __byte_perm(q[6], q[7], 0x0040);
     return make_uint2(__byte_perm(a, b, 0x5410), __byte_perm(c, e, 0x5410));
 }
 
-__device__ __forceinline__ float ck_rstd(float sumsq, int d, float eps) {
-    return __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sumsq, (float)d), eps)));
+// x^ of eight codes
+__device__ __forceinline__ void ck_decode8(uint2 q, float s, float (&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const float2 v = mul2_rn(make_float2(ck_code(q, i), ck_code(q, i + 1)), make_float2(s, s));
+        x[i] = v.x;
+        x[i + 1] = v.y;
+    }
 }
+template <typename T>
+__device__ __forceinline__ void ck_unpack(const Pack8<T>& p, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = ck_value<T>(p, i);
+}
+// acc += a b over eight values, in two chains (even and odd features)
+__device__ __forceinline__ float ck_dot8(const float (&a)[8], const float (&b)[8]) {
+    float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) s = fma2_rn(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]), s);
+    return s.x + s.y;
+}
+
+__device__ __forceinline__ float ck_rstd(float sumsq, float inv_d, float eps) { return rsqrtf(fmaf(sumsq, inv_d, eps)); }
+
+// Joins v[k] of the sixteen lanes that hold a block, for all k at once: with
+// four, the first two exchanges halve the blocks that a lane carries on, five
+// exchanges instead of sixteen.  Lane l ends with block ck_lane_block<VPT>(l);
+// the order of the joins (lanes 8, 4, 2, 1 apart) is the same for every VPT.
+struct CkAdd {
+    __device__ float operator()(float a, float b) const { return a + b; }
+};
+struct CkMaxNan {
+    __device__ float operator()(float a, float b) const { return fmax3_nan(a, a, b); }
+};
+template <int VPT, typename Op>
+__device__ __forceinline__ float ck_block_tree(const float (&v)[VPT], Op op) {
+    const uint32_t all = 0xffffffffu;
+    float c;
+    if constexpr (VPT == 4) {
+        const bool b3 = threadIdx.x & 8, b2 = threadIdx.x & 4;
+        const float a0 = op(b3 ? v[1] : v[0], __shfl_xor_sync(all, b3 ? v[0] : v[1], 8));
+        const float a1 = op(b3 ? v[3] : v[2], __shfl_xor_sync(all, b3 ? v[2] : v[3], 8));
+        c = op(b2 ? a1 : a0, __shfl_xor_sync(all, b2 ? a0 : a1, 4));
+    } else {
+        static_assert(VPT == 1, "one or four blocks a lane");
+        c = op(v[0], __shfl_xor_sync(all, v[0], 8));
+        c = op(c, __shfl_xor_sync(all, c, 4));
+    }
+    c = op(c, __shfl_xor_sync(all, c, 2));
+    return op(c, __shfl_xor_sync(all, c, 1));
+}
+template <int VPT>
+__device__ __forceinline__ int ck_lane_block() {  // the k whose block this lane ends with
+    return VPT == 4 ? (int)((threadIdx.x >> 3) & 1) + (int)((threadIdx.x >> 1) & 2) : 0;
+}
+template <int VPT>
+__device__ __forceinline__ float ck_from_block(float c, int k) {  // that block's value, in all its lanes
+    return VPT == 4 ? __shfl_sync(0xffffffffu, c, (threadIdx.x & 16) | ((k & 1) << 3) | ((k & 2) << 1)) : c;
+}
+template <int VPT>
+__device__ __forceinline__ bool ck_block_writer() { return (threadIdx.x & (VPT == 4 ? 3 : 15)) == 0; }
 
 // Sums of a row, spread over threadIdx.x (threadIdx.y is the row within the
 // CTA).  The order depends on the row's length alone, so a row's result does
-// not change with the number of rows in the call: v[k] is the sum of one
+// not change with the number of rows in the call: v[n][k] is the sum of one
 // thread's eight features, sixteen lanes join to a block's sum, lane l of every
 // warp adds the blocks l and l + 32, and a warp's tree joins the lanes.  One
 // barrier a call: `sh` has two halves that alternate.
 constexpr int kCkptShared = 64;  // blocks that a CTA holds: 8192 features / 128
-template <int N, int VPT>
-__device__ __forceinline__ void ck_row_sum(const float (&v)[VPT][N], float* sh, int parity, float (&sum)[N]) {
-    const int tx = blockDim.x, blocks = VPT * tx / 16;
-    float* s = sh + parity * (N * kCkptShared) + threadIdx.y * blocks * N;
+template <int N, int VPT, typename Barrier>
+__device__ __forceinline__ void ck_row_sum(const float (&v)[N][VPT], float* s, int x0, int tx, float (&sum)[N],
+                                           Barrier barrier) {
+    const int blocks = VPT * tx / 16;
+    const int blk = (x0 >> 4) + ck_lane_block<VPT>() * (tx >> 4);
 #pragma unroll
-    for (int k = 0; k < VPT; ++k)
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            float x = v[k][n];
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-            if ((threadIdx.x & 15) == 0) s[((threadIdx.x + k * tx) >> 4) * N + n] = x;
-        }
-    if (tx == 32) __syncwarp();
-    else __syncthreads();
+    for (int n = 0; n < N; ++n) {
+        const float x = ck_block_tree<VPT>(v[n], CkAdd());
+        if (ck_block_writer<VPT>()) s[blk * N + n] = x;
+    }
+    barrier();
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
@@ -195,19 +335,31 @@ __device__ __forceinline__ void ck_row_sum(const float (&v)[VPT][N], float* sh, 
     }
 }
 
+// The same for the CTA's rows: sh holds two halves that alternate.
+template <int N, int VPT>
+__device__ __forceinline__ void ck_row_sum(const float (&v)[N][VPT], float* sh, int parity, float (&sum)[N]) {
+    const int tx = blockDim.x;
+    ck_row_sum<N, VPT>(v, sh + parity * (N * kCkptShared) + threadIdx.y * (VPT * tx / 16) * N, threadIdx.x, tx, sum,
+                       [=] {
+                           if (tx == 32) __syncwarp();
+                           else __syncthreads();
+                       });
+}
+
 // Every kernel below holds a row in registers: thread x of a row takes the
 // features 8 (x + k blockDim.x) .. + 7, k < VPT, so that sixteen neighbouring
-// lanes hold a block of 128.  A CTA walks over rows; what depends on the
-// feature alone (gain, its gradient's sum) stays in registers meanwhile.
+// lanes hold a block of 128, and waits for one sum over the row before it can
+// write.  What hides that wait is other rows on the SM, so a thread keeps only
+// its row's values as they lie in memory; gain (fp32) and the sums of its
+// gradient sit in shared memory where a CTA walks over many rows.
 // WIDE: rows longer than a CTA holds, taken in spans of 8 VPT blockDim.x
 // features (v then sums a thread's eights over the spans) and read a second
 // time after the row's sums are known.
 #define CK_SPANS(base, d) for (int base = 0; base < (WIDE ? (d) : 1); base += 8 * VPT * (int)blockDim.x)
 #define CK_COLUMN(base, k) ((base) + 8 * (int)(threadIdx.x + (k) * blockDim.x))
 
-// Resident CTAs that the register budget has to allow: two rows of 8192 in
-// flight on an SM (VPT 4), one of 1024 threads otherwise.
-constexpr int ck_min_ctas(int vpt) { return vpt == 4 ? 2 : 1; }
+// CTAs that the register budget has to allow on an SM.
+constexpr int ck_min_ctas(int vpt, int many) { return vpt == 4 ? many : 1; }
 
 template <typename T>
 struct CkptStore {
@@ -236,62 +388,78 @@ __device__ __forceinline__ void ckpt_input(const CkptStore<T>& a, int64_t t, int
         for (int k = 0; k < VPT; ++k) res[k] = ck_load8<T, VEC>(a.residual + t * a.ldr, CK_COLUMN(base, k), d);
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
-            float v[8];
+            float v[8], w[8];
+            ck_unpack(x[k], v);
+            ck_unpack(res[k], w);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = ck_value<T>(x[k], i) + ck_value<T>(res[k], i);
+            for (int i = 0; i < 8; ++i) v[i] += w[i];
             x[k] = ck_pack<T>(v);
         }
     }
 }
 
+// Whether gain is kept in shared memory (dynamic, 4 bytes a feature)
+constexpr bool ck_shared_gain(int vpt, bool wide) { return vpt == 4 && !wide; }
+
 template <typename T, int VPT, bool VEC, bool WIDE>
-__global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT)) ckpt_store_kernel(const __grid_constant__ CkptStore<T> a) {
+__global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, sizeof(T) == 2 ? 4 : 3))
+    ckpt_store_kernel(const __grid_constant__ CkptStore<T> a) {
     __shared__ float sh[2 * kCkptShared];
+    extern __shared__ float4 ck_dyn[];
+    constexpr bool kShared = ck_shared_gain(VPT, WIDE);
     const int nb = (a.d + kCkptBlock - 1) / kCkptBlock;
-    float g[VPT][8];
-    if (!WIDE)
-#pragma unroll
-        for (int k = 0; k < VPT; ++k) ck_gain8(a.gain, a.gain_dtype, CK_COLUMN(0, k), a.d, g[k]);
+    const float inv_d = 1.0f / (float)a.d;
+    if (kShared) ck_gain_to_shared<VPT>(ck_dyn, a.gain, a.gain_dtype, a.d);
     int parity = 0;
     for (int64_t t0 = (int64_t)blockIdx.x * blockDim.y; t0 < a.rows; t0 += (int64_t)gridDim.x * blockDim.y, parity ^= 1) {
         const int64_t t = t0 + threadIdx.y;
         const int d = t < a.rows ? a.d : 0;  // a row past the end holds nothing
         Pack8<T> x[VPT];
-        float ss[VPT][1] = {}, sum[1];
+        float ss[1][VPT] = {}, sum[1];
         CK_SPANS(base, a.d) {
             ckpt_input<T, VPT, VEC>(a, t, base, d, x);
+            float m[VPT];
 #pragma unroll
             for (int k = 0; k < VPT; ++k) {
-                const int c = CK_COLUMN(base, k);
-                if (a.residual) ck_store8<T, VEC>(a.sum + t * a.d, c, d, x[k]);
-                float v[8], m = 0.0f;
+                if (a.residual) ck_store8<T, VEC>(a.sum + t * a.d, CK_COLUMN(base, k), d, x[k]);
+                float v[8];
+                ck_unpack(x[k], v);
+                ss[0][k] += ck_dot8(v, v);
+                m[k] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    v[i] = ck_value<T>(x[k], i);
-                    ss[k][0] = fmaf(v[i], v[i], ss[k][0]);
-                }
-#pragma unroll
-                for (int i = 0; i < 8; i += 2) m = fmax3_nan(m, fabsf(v[i]), fabsf(v[i + 1]));
-#pragma unroll
-                for (int o = 8; o > 0; o >>= 1) m = fmax3_nan(m, m, __shfl_xor_sync(0xffffffffu, m, o));
-                const float s = ck_scale(m);
-                if ((threadIdx.x & 15) == 0 && c < d) a.scales[t * nb + c / kCkptBlock] = s;
-                ck_store_codes<VEC>(a.codes + t * a.d, c, d, ck_encode8(v, s));
+                for (int i = 0; i < 8; i += 2) m[k] = fmax3_nan(m[k], fabsf(v[i]), fabsf(v[i + 1]));
             }
-        }
-        ck_row_sum<1>(ss, sh, parity, sum);
-        const float r = ck_rstd(sum[0], a.d, a.eps);
-        CK_SPANS(base, a.d) {
-            if (WIDE) {
-                ckpt_input<T, VPT, VEC>(a, t, base, d, x);
-#pragma unroll
-                for (int k = 0; k < VPT; ++k) ck_gain8(a.gain, a.gain_dtype, CK_COLUMN(base, k), a.d, g[k]);
-            }
+            // a lane scales one of its blocks
+            const float scale = ck_scale(ck_block_tree<VPT>(m, CkMaxNan()));
+            const float inv = __frcp_rn(scale);
+            const int c0 = CK_COLUMN(base, ck_lane_block<VPT>()) / kCkptBlock * kCkptBlock;
+            if (ck_block_writer<VPT>() && c0 < d) a.scales[t * nb + c0 / kCkptBlock] = scale;
 #pragma unroll
             for (int k = 0; k < VPT; ++k) {
                 float v[8];
+                ck_opaque(x[k]);
+                ck_unpack(x[k], v);
+                ck_store_codes<VEC>(a.codes + t * a.d, CK_COLUMN(base, k), d, ck_encode8(v, ck_from_block<VPT>(inv, k)));
+            }
+        }
+        ck_row_sum<1, VPT>(ss, sh, parity, sum);
+        const float r = ck_rstd(sum[0], inv_d, a.eps);
+        CK_SPANS(base, a.d) {
+            if (WIDE) ckpt_input<T, VPT, VEC>(a, t, base, d, x);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = ck_value<T>(x[k], i) * r * g[k][i];
+            for (int k = 0; k < VPT; ++k) {
+                float v[8], g[8];
+                ck_opaque(x[k]);
+                ck_unpack(x[k], v);
+                if (kShared) ck_slot8(ck_dyn, k, g);
+                else ck_gain8(a.gain, a.gain_dtype, CK_COLUMN(base, k), a.d, g);
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    const float2 y = mul2_rn(mul2_rn(make_float2(v[i], v[i + 1]), make_float2(r, r)),
+                                             make_float2(g[i], g[i + 1]));
+                    v[i] = y.x;
+                    v[i + 1] = y.y;
+                }
                 ck_store8<T, VEC>(a.y + t * a.d, CK_COLUMN(base, k), d, ck_pack<T>(v));
             }
         }
@@ -318,46 +486,79 @@ __device__ __forceinline__ void ck_restore8(const CkptRead& a, int64_t t, int c,
 
 // The norm of x^, in rows of pitch ldo.
 template <typename T, int VPT, bool VEC, bool WIDE>
-__global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT))
+__global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, 4))
     ckpt_norm_kernel(const __grid_constant__ CkptRead a, T* __restrict__ out, int64_t ldo) {
     __shared__ float sh[2 * kCkptShared];
-    float g[VPT][8];
-    if (!WIDE)
-#pragma unroll
-        for (int k = 0; k < VPT; ++k) ck_gain8(a.gain, a.gain_dtype, CK_COLUMN(0, k), a.d, g[k]);
+    extern __shared__ float4 ck_dyn[];
+    constexpr bool kShared = ck_shared_gain(VPT, WIDE);
+    const float inv_d = 1.0f / (float)a.d;
+    if (kShared) ck_gain_to_shared<VPT>(ck_dyn, a.gain, a.gain_dtype, a.d);
     int parity = 0;
     for (int64_t t0 = (int64_t)blockIdx.x * blockDim.y; t0 < a.rows; t0 += (int64_t)gridDim.x * blockDim.y, parity ^= 1) {
         const int64_t t = t0 + threadIdx.y;
         const int d = t < a.rows ? a.d : 0;
         uint2 q[VPT];
-        float s[VPT], ss[VPT][1] = {}, sum[1];
+        float s[VPT], ss[1][VPT] = {}, sum[1];
         CK_SPANS(base, a.d) {
 #pragma unroll
             for (int k = 0; k < VPT; ++k) ck_restore8<VEC>(a, t, CK_COLUMN(base, k), d, q[k], s[k]);
 #pragma unroll
-            for (int k = 0; k < VPT; ++k)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float x = ck_code(q[k], i) * s[k];
-                    ss[k][0] = fmaf(x, x, ss[k][0]);
-                }
+            for (int k = 0; k < VPT; ++k) {
+                float x[8];
+                ck_decode8(q[k], s[k], x);
+                ss[0][k] += ck_dot8(x, x);
+            }
         }
-        ck_row_sum<1>(ss, sh, parity, sum);
-        const float r = ck_rstd(sum[0], a.d, a.eps);
+        ck_row_sum<1, VPT>(ss, sh, parity, sum);
+        const float r = ck_rstd(sum[0], inv_d, a.eps);
         CK_SPANS(base, a.d) {
             if (WIDE)
 #pragma unroll
-                for (int k = 0; k < VPT; ++k) {
-                    ck_restore8<VEC>(a, t, CK_COLUMN(base, k), d, q[k], s[k]);
-                    ck_gain8(a.gain, a.gain_dtype, CK_COLUMN(base, k), a.d, g[k]);
-                }
+                for (int k = 0; k < VPT; ++k) ck_restore8<VEC>(a, t, CK_COLUMN(base, k), d, q[k], s[k]);
 #pragma unroll
             for (int k = 0; k < VPT; ++k) {
-                float v[8];
+                float x[8], g[8];
+                ck_opaque(q[k]);
+                ck_decode8(q[k], s[k], x);
+                if (kShared) ck_slot8(ck_dyn, k, g);
+                else ck_gain8(a.gain, a.gain_dtype, CK_COLUMN(base, k), a.d, g);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = ck_code(q[k], i) * s[k] * r * g[k][i];
-                ck_store8<T, VEC>(out + t * ldo, CK_COLUMN(base, k), d, ck_pack<T>(v));
+                for (int i = 0; i < 8; i += 2) {
+                    const float2 y = mul2_rn(mul2_rn(make_float2(x[i], x[i + 1]), make_float2(r, r)),
+                                             make_float2(g[i], g[i + 1]));
+                    x[i] = y.x;
+                    x[i + 1] = y.y;
+                }
+                ck_store8<T, VEC>(out + t * ldo, CK_COLUMN(base, k), d, ck_pack<T>(x));
             }
+        }
+    }
+}
+
+// x^ of a whole checkpoint whose rows are whole blocks and lie one after the
+// other: sixteen codes (one load) at a time, four in flight.
+template <typename T>
+__global__ void __launch_bounds__(256) ckpt_decode_flat_kernel(const uint4* __restrict__ codes,
+                                                               const float* __restrict__ scales, int64_t n16,
+                                                               T* __restrict__ out) {
+    for (int64_t i0 = (int64_t)blockIdx.x * 1024 + threadIdx.x; i0 < n16; i0 += (int64_t)gridDim.x * 1024) {
+        uint4 q[4];
+        float s[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int64_t i = i0 + k * 256;
+            q[k] = i < n16 ? ck_stream(codes + i) : make_uint4(0, 0, 0, 0);
+            s[k] = i < n16 ? __ldg(scales + i / 8) : 0.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int64_t i = i0 + k * 256;
+            if (i >= n16) break;
+            float v[8];
+            ck_decode8(make_uint2(q[k].x, q[k].y), s[k], v);
+            ck_store8<T, true>(out + 16 * i, 0, 8, ck_pack<T>(v));
+            ck_decode8(make_uint2(q[k].z, q[k].w), s[k], v);
+            ck_store8<T, true>(out + 16 * i, 8, 16, ck_pack<T>(v));
         }
     }
 }
@@ -377,11 +578,44 @@ __global__ void __launch_bounds__(1024 / VPT) ckpt_decode_kernel(const __grid_co
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
             float v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = ck_code(q[k], i) * s[k];
+            ck_decode8(q[k], s[k], v);
             ck_store8<T, VEC>(out + t * ldo, CK_COLUMN(base, k), d, ck_pack<T>(v));
         }
     }
+}
+
+// A row's sums from eight features: of x^ squared, and of x^ dy gain.  The
+// codes' squares are whole numbers; the block's scale goes to the sums.
+template <typename T>
+__device__ __forceinline__ void ck_back_sums(uint2 q, const Pack8<T>& dy, const uint64_t (&g)[4], float s, float& xx,
+                                             float& xd) {
+    uint64_t dot = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        dot = f2_fma(f2_mul(f2(ck_value<T>(dy, 2 * i), ck_value<T>(dy, 2 * i + 1)), g[i]),
+                     f2(ck_code(q, 2 * i), ck_code(q, 2 * i + 1)), dot);
+    const float2 dd = f2_get(dot);
+    xx += (float)__dp4a((int)q.y, (int)q.y, __dp4a((int)q.x, (int)q.x, 0)) * (s * s);
+    xd += (dd.x + dd.y) * s;
+}
+// dx of eight features (dy gain r + x^ f + the residual's) and their addends
+// to d_gain's sums.
+template <typename T>
+__device__ __forceinline__ Pack8<T> ck_back_apply(uint2 q, const Pack8<T>& dy, const Pack8<T>& res, bool with_res,
+                                                  const uint64_t (&g)[4], float s, float r, float f, uint64_t (&dg)[4]) {
+    const uint64_t fs = f2(f * s, f * s), rs = f2(r * s, r * s), rr = f2(r, r);
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint64_t xx = f2(ck_code(q, 2 * i), ck_code(q, 2 * i + 1));
+        const uint64_t ee = f2(ck_value<T>(dy, 2 * i), ck_value<T>(dy, 2 * i + 1));
+        dg[i] = f2_fma(f2_mul(ee, rs), xx, dg[i]);
+        const uint64_t z = with_res ? f2(ck_value<T>(res, 2 * i), ck_value<T>(res, 2 * i + 1)) : 0;
+        const float2 o = f2_get(f2_fma(f2_mul(ee, g[i]), rr, f2_fma(xx, fs, z)));
+        v[2 * i] = o.x;
+        v[2 * i + 1] = o.y;
+    }
+    return ck_pack<T>(v);
 }
 
 template <typename T>
@@ -396,33 +630,30 @@ struct CkptBack {
 };
 
 // dx, and each row group's sum of d_gain (ckpt_gain_sum_kernel adds them in
-// their order).  WIDE keeps that sum in `part` itself: each element has one
-// thread.
+// their order).  A thread's sums lie in shared memory (dynamic, 4 bytes a
+// feature and row of the CTA), those of WIDE in `part` itself; each element has
+// one thread.
 template <typename T, int VPT, bool VEC, bool WIDE>
-__global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT)) ckpt_back_kernel(const __grid_constant__ CkptBack<T> a) {
+__global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, 2))
+    ckpt_back_kernel(const __grid_constant__ CkptBack<T> a) {
     __shared__ float sh[4 * kCkptShared];
+    extern __shared__ float4 ck_dyn[];
+    constexpr bool kShared = ck_shared_gain(VPT, WIDE);
+    const float inv_d = 1.0f / (float)a.in.d;
     float* part = a.part + ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * a.in.d;
-    float g[VPT][8], dg[VPT][8];
-    auto gain_of = [&](int base) {
+    float4* dg = ck_dyn + threadIdx.y * 2 * VPT * blockDim.x;
+    float4* sg = ck_dyn + blockDim.y * 2 * VPT * blockDim.x;
+    if (!WIDE)
 #pragma unroll
-        for (int k = 0; k < VPT; ++k) ck_gain8(a.in.gain, a.in.gain_dtype, CK_COLUMN(base, k), a.in.d, g[k]);
+        for (int k = 0; k < VPT; ++k) ck_slot(dg, k, 0) = ck_slot(dg, k, 1) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (kShared) ck_gain_to_shared<VPT>(sg, a.in.gain, a.in.gain_dtype, a.in.d);
+    auto gain_of = [&](int base, int k, uint64_t (&p)[4]) {
+        float g[8];
+        if (kShared) ck_slot8(sg, k, g);
+        else ck_gain8(a.in.gain, a.in.gain_dtype, CK_COLUMN(base, k), a.in.d, g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = f2(g[2 * i], g[2 * i + 1]);
     };
-    auto sums_to = [&](int base, bool add) {
-#pragma unroll
-        for (int k = 0; k < VPT; ++k) {
-            const int c = CK_COLUMN(base, k);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (c + i < a.in.d) part[c + i] = dg[k][i] + (add ? part[c + i] : 0.0f);
-        }
-    };
-    if (!WIDE) {
-        gain_of(0);
-#pragma unroll
-        for (int k = 0; k < VPT; ++k)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) dg[k][i] = 0.0f;
-    }
     int parity = 0;
     bool first = true;
     for (int64_t t0 = (int64_t)blockIdx.x * blockDim.y; t0 < a.in.rows;
@@ -430,7 +661,7 @@ __global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT)) ckpt_back_kernel
         const int64_t t = t0 + threadIdx.y;
         const int d = t < a.in.rows ? a.in.d : 0;
         uint2 q[VPT];
-        float s[VPT], acc[VPT][2] = {}, sum[2];
+        float s[VPT], acc[2][VPT] = {}, sum[2];
         Pack8<T> dy[VPT], res[VPT];
         auto read = [&](int base) {
 #pragma unroll
@@ -438,63 +669,249 @@ __global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT)) ckpt_back_kernel
                 const int c = CK_COLUMN(base, k);
                 ck_restore8<VEC>(a.in, t, c, d, q[k], s[k]);
                 dy[k] = ck_load8<T, VEC>(a.dy + t * a.ld_dy, c, d);
-                if (a.d_res) res[k] = ck_load8<T, VEC>(a.d_res + t * a.ld_res, c, d);
             }
         };
+        auto read_res = [&](int base) {
+            if (a.d_res)
+#pragma unroll
+                for (int k = 0; k < VPT; ++k) res[k] = ck_load8<T, VEC>(a.d_res + t * a.ld_res, CK_COLUMN(base, k), d);
+        };
         CK_SPANS(base, a.in.d) {
-            if (WIDE) gain_of(base);
             read(base);
 #pragma unroll
-            for (int k = 0; k < VPT; ++k)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float x = ck_code(q[k], i) * s[k];
-                    acc[k][0] = fmaf(x, x, acc[k][0]);
-                    acc[k][1] = fmaf(x, ck_value<T>(dy[k], i) * g[k][i], acc[k][1]);
-                }
+            for (int k = 0; k < VPT; ++k) {
+                uint64_t g[4];
+                gain_of(base, k, g);
+                ck_back_sums<T>(q[k], dy[k], g, s[k], acc[0][k], acc[1][k]);
+            }
         }
-        ck_row_sum<2>(acc, sh, parity, sum);
-        const float r = ck_rstd(sum[0], a.in.d, a.in.eps);
-        const float f = r * r * r * (sum[1] / (float)a.in.d);
+        if (!WIDE) read_res(0);  // arrives during the row's sum
+        ck_row_sum<2, VPT>(acc, sh, parity, sum);
+        const float r = ck_rstd(sum[0], inv_d, a.in.eps);
+        const float f = -(r * r * r * (sum[1] * inv_d));
         CK_SPANS(base, a.in.d) {
             if (WIDE) {
-                gain_of(base);
                 read(base);
+                read_res(base);
             }
 #pragma unroll
             for (int k = 0; k < VPT; ++k) {
-                float v[8];
+                const int c = CK_COLUMN(base, k);
+                uint64_t g[4], w[4];
+                float p[8];
+                ck_opaque(q[k]);
+                ck_opaque(dy[k]);
+                gain_of(base, k, g);
+                if (WIDE) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float x = ck_code(q[k], i) * s[k], e = ck_value<T>(dy[k], i) * r;
-                    dg[k][i] = WIDE ? e * x : fmaf(e, x, dg[k][i]);
-                    v[i] = fmaf(e, g[k][i], -x * f);
-                    if (a.d_res) v[i] += ck_value<T>(res[k], i);
+                    for (int i = 0; i < 8; ++i) p[i] = c + i < a.in.d && !first ? part[c + i] : 0.0f;
+                } else {
+                    ck_slot8(dg, k, p);
                 }
-                ck_store8<T, VEC>(a.dx + t * a.in.d, CK_COLUMN(base, k), d, ck_pack<T>(v));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = f2(p[2 * i], p[2 * i + 1]);
+                ck_store8<T, VEC>(a.dx + t * a.in.d, c, d,
+                                  ck_back_apply<T>(q[k], dy[k], res[k], a.d_res != nullptr, g, s[k], r, f, w));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 x = f2_get(w[i]);
+                    p[2 * i] = x.x;
+                    p[2 * i + 1] = x.y;
+                }
+                if (WIDE) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (c + i < a.in.d) part[c + i] = p[i];
+                } else {
+                    ck_slot(dg, k, 0) = make_float4(p[0], p[1], p[2], p[3]);
+                    ck_slot(dg, k, 1) = make_float4(p[4], p[5], p[6], p[7]);
+                }
             }
-            if (WIDE) sums_to(base, !first);
         }
     }
-    if (!WIDE) sums_to(0, false);
+    if (!WIDE)
+#pragma unroll
+        for (int k = 0; k < VPT; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int c = CK_COLUMN(0, k) + 4 * h;
+                const float4 p = ck_slot(dg, k, h);
+                if (VEC) {
+                    if (c < a.in.d) *reinterpret_cast<float4*>(part + c) = p;
+                } else {
+                    const float w[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (c + i < a.in.d) part[c + i] = w[i];
+                }
+            }
 }
 
-// d_gain: 32 columns a CTA, its eight warps every eighth row group, then the
-// warps in their order.
-__global__ void __launch_bounds__(256) ckpt_gain_sum_kernel(const float* __restrict__ part, int np, int d,
-                                                            float* __restrict__ d_gain) {
-    __shared__ float sh[8][32];
+// The same for many rows of up to 8192 features (d a multiple of 16, every row
+// on 16 bytes): one CTA an SM, whose rows come through shared memory by bulk
+// copies, so that what is in flight does not depend on the registers or on
+// where the row sums stand.  The CTA's threads form groups of tx, each of which
+// takes every n-th row of the CTA through a ring of its own: when all its warps
+// have reached a row's sum, the row before it is done with and its stage is
+// filled again.  A thread's d_gain sums stay in registers; at the end the
+// groups' are added in their order.
+struct CkptRing {
+    int tx, groups, stages;  // stages a group
+    int stage_bytes, res_at, codes_at;  // dy first
+};
+constexpr int kRingThreads = 512, kRingMaxStages = 8;
+
+template <typename T>
+__global__ void __launch_bounds__(kRingThreads, 1)
+    ckpt_back_ring_kernel(const __grid_constant__ CkptBack<T> a, const CkptRing ring, uint32_t* err) {
+    constexpr int VPT = 4;
+    extern __shared__ __align__(128) uint8_t ck_ring[];
+    __shared__ float sh[2 * 2 * VPT * kRingThreads / 16];  // [group][parity][block][2]
+    __shared__ uint64_t full_s[16 * kRingMaxStages];
+    __shared__ int abort_s;
+    volatile int* abort = &abort_s;
+    const int d = a.in.d, nb = (d + kCkptBlock - 1) / kCkptBlock;
+    const int tx = ring.tx, x0 = (int)threadIdx.x % tx, grp = (int)threadIdx.x / tx;
+    uint8_t* stages = ck_ring + (size_t)grp * ring.stages * ring.stage_bytes;
+    uint64_t* full = full_s + grp * kRingMaxStages;
+    // gain: [k][half][thread of the group]
+    ulonglong2* sg = reinterpret_cast<ulonglong2*>(ck_ring + (size_t)ring.groups * ring.stages * ring.stage_bytes);
+    if (threadIdx.x == 0) abort_s = 0;
+    if (x0 == 0) {
+        for (int s = 0; s < ring.stages; ++s) mbar_init(&full[s], 1);
+        fence_mbar_init();
+    }
+    for (int i = threadIdx.x; i < 2 * VPT * tx; i += blockDim.x) {
+        const int c = 8 * (i % tx + i / (2 * tx) * tx) + 4 * (i / tx % 2);
+        float g[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) g[j] = c + j < d ? load_as_f32(a.in.gain, c + j, a.in.gain_dtype) : 0.0f;
+        sg[i] = make_ulonglong2(f2(g[0], g[1]), f2(g[2], g[3]));
+    }
+    __syncthreads();
+    // the group's row j is the CTA's row grp + j * groups, row blockIdx.x + that * gridDim.x of all
+    const int64_t step = (int64_t)gridDim.x * ring.groups, row0 = blockIdx.x + (int64_t)grp * gridDim.x;
+    const int mine = row0 < a.in.rows ? (int)((a.in.rows - row0 + step - 1) / step) : 0;
+    auto copy = [&](int j, int s) {  // row j into stage s, by the group's first thread
+        const int64_t t = row0 + j * step;
+        const uint32_t row16 = (uint32_t)d * (uint32_t)sizeof(T);
+        uint8_t* st = stages + (size_t)s * ring.stage_bytes;
+        mbar_arrive_expect_tx(&full[s], row16 * (a.d_res ? 2 : 1) + (uint32_t)d);
+        bulk_load(st, a.dy + t * a.ld_dy, row16, &full[s]);
+        if (a.d_res) bulk_load(st + ring.res_at, a.d_res + t * a.ld_res, row16, &full[s]);
+        bulk_load(st + ring.codes_at, a.in.codes + t * d, (uint32_t)d, &full[s]);
+    };
+    if (x0 == 0)
+        for (int j = 0; j < min(ring.stages, mine); ++j) copy(j, j);
+    auto scales_of = [&](int j, float (&s)[VPT]) {
+        const int64_t t = row0 + j * step;
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            const int c = 8 * (x0 + k * tx);
+            s[k] = j < mine && c < d ? __ldg(a.in.scales + t * nb + c / kCkptBlock) : 0.0f;
+        }
+    };
+    const float inv_d = 1.0f / (float)d;
+    float s[VPT], next[VPT];
+    uint64_t dg[VPT][4];  // pairs
+#pragma unroll
+    for (int k = 0; k < VPT; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dg[k][i] = 0;
+    scales_of(0, s);
+    int j = 0, stage = 0;
+    uint32_t phase = 0;
+    for (; j < mine; ++j) {
+        scales_of(j + 1, next);  // a row ahead
+        const int64_t t = row0 + j * step;
+        if (!mbar_wait(&full[stage], phase, abort, err, DEVERR_TIMEOUT_TMA)) break;
+        const uint8_t* st = stages + (size_t)stage * ring.stage_bytes;
+        float acc[2][VPT], sum[2];
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            const int c = 8 * (x0 + k * tx);
+            acc[0][k] = acc[1][k] = 0.0f;
+            if (c < d) {
+                const uint2 q = *reinterpret_cast<const uint2*>(st + ring.codes_at + c);
+                const Pack8<T> dy = ck_shared8<T>(st, c);
+                const ulonglong2 g0 = sg[2 * k * tx + x0], g1 = sg[(2 * k + 1) * tx + x0];
+                const uint64_t g[4] = {g0.x, g0.y, g1.x, g1.y};
+                ck_back_sums<T>(q, dy, g, s[k], acc[0][k], acc[1][k]);
+            }
+        }
+        ck_row_sum<2, VPT>(acc, sh + (grp * 2 + (j & 1)) * (VPT * tx / 16) * 2, x0, tx, sum, [=] {
+            if (tx == 32) __syncwarp();
+            else named_bar(1 + grp, tx);
+        });
+        if (x0 == 0 && j > 0 && j - 1 + ring.stages < mine)
+            copy(j - 1 + ring.stages, stage > 0 ? stage - 1 : ring.stages - 1);
+        const float r = ck_rstd(sum[0], inv_d, a.in.eps);
+        const float f = -(r * r * r * (sum[1] * inv_d));
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            const int c = 8 * (x0 + k * tx);
+            if (c < d) {
+                uint2 q = *reinterpret_cast<const uint2*>(st + ring.codes_at + c);
+                Pack8<T> dy = ck_shared8<T>(st, c), res;
+                ck_opaque(q);
+                ck_opaque(dy);
+                if (a.d_res) res = ck_shared8<T>(st + ring.res_at, c);
+                const ulonglong2 g0 = sg[2 * k * tx + x0], g1 = sg[(2 * k + 1) * tx + x0];
+                const uint64_t g[4] = {g0.x, g0.y, g1.x, g1.y};
+                ck_store8<T, true>(a.dx + t * d, c, d,
+                                   ck_back_apply<T>(q, dy, res, a.d_res != nullptr, g, s[k], r, f, dg[k]));
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) s[k] = next[k];
+        if (++stage == ring.stages) {
+            stage = 0;
+            phase ^= 1u;
+        }
+    }
+    // a wait gave up: the copies in flight get a last, bounded chance to land
+    if (j < mine && x0 == 0)
+        for (int i = 0; i < ring.stages && j + i < mine; ++i)
+            for (int n = 0, w = stage + i < ring.stages ? stage + i : stage + i - ring.stages;
+                 n < 1000 && !mbar_try_wait(&full[w], stage + i < ring.stages ? phase : phase ^ 1u); ++n) {}
+    __syncthreads();
+    if (*abort) return;
+    // the groups' sums, added in their order
+    float* all = reinterpret_cast<float*>(ck_ring);
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+        const int c = 8 * (x0 + k * tx);
+        if (c < d) {
+            ulonglong2* o = reinterpret_cast<ulonglong2*>(all + (size_t)grp * d + c);
+            o[0] = make_ulonglong2(dg[k][0], dg[k][1]);
+            o[1] = make_ulonglong2(dg[k][2], dg[k][3]);
+        }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < d; c += blockDim.x) {
+        float v = all[c];
+        for (int g = 1; g < ring.groups; ++g) v += all[(size_t)g * d + c];
+        a.part[(int64_t)blockIdx.x * d + c] = v;
+    }
+}
+
+// d_gain: 32 columns a CTA, its 32 warps every 32nd row group, then the warps
+// in their order.
+__global__ void __launch_bounds__(1024) ckpt_gain_sum_kernel(const float* __restrict__ part, int np, int d,
+                                                             float* __restrict__ d_gain) {
+    __shared__ float sh[32][33];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int c = blockIdx.x * 32 + lane;
     float s = 0.0f;
     if (c < d)
-        for (int p = warp; p < np; p += 8) s += part[(int64_t)p * d + c];
+#pragma unroll 8
+        for (int p = warp; p < np; p += 32) s += part[(int64_t)p * d + c];
     sh[warp][lane] = s;
     __syncthreads();
-    if (warp == 0 && c < d) {
-        for (int w = 1; w < 8; ++w) s += sh[w][lane];
-        d_gain[c] = s;
-    }
+    s = sh[lane][warp];  // column `warp` of the 32, its 32 sums over the lanes
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0 && blockIdx.x * 32 + warp < d) d_gain[blockIdx.x * 32 + warp] = s;
 }
 
 }  // namespace aeth

@@ -18,6 +18,7 @@ ABI raise AethError.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -27,51 +28,66 @@ from .galore import _DTYPES
 
 CHECKPOINT_BLOCK = 128  # features that share a scale
 
+_lib = L.load()
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
-def _addr(t: torch.Tensor | None):
-    return None if t is None else t.data_ptr()
 
-
-def _workspace(fn: str, device, *dims) -> tuple[torch.Tensor, int]:
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(fn: str, *dims: int) -> int:
     size = C.c_size_t()
-    L.check(getattr(L.load(), fn)(*dims, C.byref(size)), fn)
-    return torch.empty(size.value, dtype=torch.uint8, device=device), size.value
+    L.check(getattr(_lib, fn)(*dims, C.byref(size)), fn)
+    return size.value
 
 
-def _device_of(name: str, t: torch.Tensor, *others: torch.Tensor | None) -> torch.device:
-    if not t.is_cuda:
-        raise ValueError(f"{name}: device tensors expected")
-    for o in others:
-        if o is not None and o.device != t.device:
-            raise ValueError(f"{name}: all tensors must be on {t.device}")
-    return t.device
+def _on_device(f):
+    """Runs f(device index, first tensor, ...) with that device current, so that
+    its allocations, its stream and its launch are the tensors'."""
+    first = f.__code__.co_varnames[0]
+
+    @functools.wraps(f)
+    def run(*args, **kw):
+        t = args[0] if args else kw[first]
+        dev = (t.codes if isinstance(t, ActivationCheckpoint) else t).get_device()
+        if dev < 0:
+            raise ValueError(f"{f.__name__}: device tensors expected")
+        if dev == torch.cuda.current_device():
+            return f(*args, **kw)
+        with torch.cuda.device(dev):
+            return f(*args, **kw)
+    return run
 
 
-def _rows2d(t: torch.Tensor) -> torch.Tensor:
-    """`t` as a matrix of rows whose last dimension is contiguous; a view where
-    the strides allow it."""
-    d = t.shape[-1]
+def _same_device(what: str, dev: int, *tensors: torch.Tensor | None) -> None:
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{what}: all tensors must be on cuda:{dev}")
+
+
+def _rows(t: torch.Tensor, d: int) -> tuple[torch.Tensor, int, int]:
+    """`t` (..., d) as rows: (a tensor whose data are those rows, their number,
+    their pitch), a view where the strides allow it."""
+    if t.is_contiguous():
+        return t, t.numel() // d, d
     t = t.reshape(-1, d)
-    return t if t.stride(1) == 1 and _pitch(t) >= d else t.contiguous()
+    if t.stride(1) == 1 and t.size(0) > 1 and t.stride(0) >= d:
+        return t, t.size(0), t.stride(0)
+    return t.contiguous(), t.size(0), d
 
 
-def _pitch(t: torch.Tensor) -> int:
-    """Row pitch of a matrix of rows (a single row's stride says nothing)."""
-    return t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // 8) * 8
-
-
-def _tma_rows(t: torch.Tensor) -> torch.Tensor:
-    """A matrix that TMA can read in place (16-byte aligned rows), else a copy
-    with padded rows."""
-    t = _rows2d(t)
-    if _pitch(t) % 8 == 0 and t.data_ptr() % 16 == 0:
-        return t
-    out = torch.empty(t.shape[0], -(-t.shape[1] // 8) * 8, dtype=t.dtype, device=t.device)[:, :t.shape[1]]
-    return out.copy_(t)
+def _tma_rows(t: torch.Tensor, d: int) -> tuple[torch.Tensor, int, int]:
+    """The same, 16-bit rows that TMA can read in place (16-byte aligned), else a
+    copy with padded rows."""
+    t, n, ld = _rows(t, d)
+    if ld % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t, n, ld
+    ld = -(-d // 8) * 8
+    out = torch.empty(n, ld, dtype=t.dtype, device=t.device)
+    out[:, :d] = t.reshape(-1, d)
+    return out, n, ld
 
 
 # ---- head loss ----
-@dataclass
+@dataclass(slots=True)
 class CutCrossEntropy:
     """Result of ``cut_cross_entropy``: the mean loss (a 0-dimensional tensor),
     every token's loss, and the log-sum-exp that the backward starts from."""
@@ -81,17 +97,18 @@ class CutCrossEntropy:
 
 
 def _head_args(what, hidden, weight, labels):
-    if weight.dim() != 2 or 0 in weight.shape or hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1]:
+    if weight.dim() != 2 or weight.numel() == 0 or hidden.dim() < 1 or hidden.size(-1) != weight.size(1):
         raise ValueError(f"{what}: hidden (..., d) and weight (vocab, d) expected, "
                          f"got {tuple(hidden.shape)} and {tuple(weight.shape)}")
     if hidden.dtype != weight.dtype or hidden.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError(f"{what}: hidden and weight must both be bfloat16 or both float16")
     if labels.shape != hidden.shape[:-1] or labels.dtype.is_floating_point or labels.dtype.is_complex:
         raise ValueError(f"{what}: labels must be whole numbers of shape {tuple(hidden.shape[:-1])}")
-    dev = _device_of(what, hidden, weight, labels)
-    return dev, _rows2d(hidden), _tma_rows(weight), labels.reshape(-1).to(torch.int64).contiguous()
+    _same_device(what, hidden.get_device(), weight, labels)
+    return labels.to(torch.int64).contiguous()
 
 
+@_on_device
 def cut_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
                       ignore_index: int = -100) -> CutCrossEntropy:
     """Cross entropy of softmax(hidden @ weight.T) against `labels`, the logits
@@ -100,20 +117,21 @@ def cut_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.
     take no part: their loss is 0 and whatever their hidden state holds is not
     read.  A label outside the vocabulary makes its token's loss and the mean
     NaN and sets DEVERR_BAD_ARG in the device error word."""
-    dev, h, w, lab = _head_args("cut_cross_entropy", hidden, weight, labels)
-    n, d = h.shape
-    with torch.cuda.device(dev):
-        losses = torch.empty(labels.shape, dtype=torch.float32, device=dev)
-        lse = torch.empty(labels.shape, dtype=torch.float32, device=dev)
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        ws, size = _workspace("aeth_cut_ce_workspace", dev, n, d, w.shape[0], 0)
-        L.check(L.load().aeth_cut_ce_forward(
-            _addr(h), _pitch(h), _addr(w), _pitch(w), _DTYPES[h.dtype], _addr(lab), n, d, w.shape[0],
-            ignore_index, _addr(losses), _addr(lse), _addr(loss), _addr(ws), size,
-            torch.cuda.current_stream().cuda_stream), "aeth_cut_ce_forward")
-    return CutCrossEntropy(loss, losses, lse)
+    lab = _head_args("cut_cross_entropy", hidden, weight, labels)
+    v, d = weight.shape
+    h, n, ld_h = _rows(hidden, d)
+    w, _, ld_w = _tma_rows(weight, d)
+    out = torch.empty(2 * n + 1, dtype=torch.float32, device=h.device)  # losses, lse, loss: one allocation
+    at = out.data_ptr()
+    size = _workspace_bytes("aeth_cut_ce_workspace", n, d, v, 0)
+    ws = torch.empty(size, dtype=torch.uint8, device=h.device)
+    L.check(_lib.aeth_cut_ce_forward(
+        h.data_ptr(), ld_h, w.data_ptr(), ld_w, _DTYPES[h.dtype], lab.data_ptr(), n, d, v, ignore_index, at,
+        at + 4 * n, at + 8 * n, ws.data_ptr(), size, _raw_stream(h.get_device())), "aeth_cut_ce_forward")
+    return CutCrossEntropy(out[2 * n], out[:n].view(labels.shape), out[n:2 * n].view(labels.shape))
 
 
+@_on_device
 def cut_cross_entropy_backward(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, ce: CutCrossEntropy,
                                grad_losses: torch.Tensor | None = None, scale: float = 1.0, ignore_index: int = -100,
                                need_hidden: bool = True, need_weight: bool = True):
@@ -122,30 +140,33 @@ def cut_cross_entropy_backward(hidden: torch.Tensor, weight: torch.Tensor, label
     of scale * mean loss, or of scale * sum(grad_losses * losses) where
     `grad_losses` (float32, the shape of the labels) is given."""
     what = "cut_cross_entropy_backward"
-    dev, h, w, lab = _head_args(what, hidden, weight, labels)
-    n, d = h.shape
+    lab = _head_args(what, hidden, weight, labels)
+    v, d = weight.shape
+    h, n, ld_h = _rows(hidden, d)
     if ce.lse.dtype != torch.float32 or ce.lse.numel() != n:
         raise ValueError(f"{what}: ce must be the result of cut_cross_entropy for these tokens")
     if grad_losses is not None and (grad_losses.dtype != torch.float32 or grad_losses.numel() != n):
         raise ValueError(f"{what}: grad_losses must be float32, one per token")
-    _device_of(what, h, ce.lse, grad_losses)
+    _same_device(what, h.get_device(), ce.lse, grad_losses)
     if not need_hidden and not need_weight:
         return None, None
-    with torch.cuda.device(dev):
-        lse = ce.lse.contiguous()
-        grad = None if grad_losses is None else grad_losses.contiguous()
-        dh = torch.empty(hidden.shape, dtype=h.dtype, device=dev) if need_hidden else None
-        dw = torch.empty(w.shape, dtype=w.dtype, device=dev) if need_weight else None
-        ws, size = _workspace("aeth_cut_ce_workspace", dev, n, d, w.shape[0], 1)
-        L.check(L.load().aeth_cut_ce_backward(
-            _addr(h), _pitch(h), _addr(w), _pitch(w), _DTYPES[h.dtype], _addr(lab), n, d, w.shape[0],
-            ignore_index, _addr(lse), _addr(grad), float(scale), _addr(dh), d, _addr(dw), d, _addr(ws), size,
-            torch.cuda.current_stream().cuda_stream), "aeth_cut_ce_backward")
+    w, _, ld_w = _tma_rows(weight, d)
+    lse = ce.lse.contiguous()
+    grad = None if grad_losses is None else grad_losses.contiguous()
+    dh = torch.empty(hidden.shape, dtype=h.dtype, device=h.device) if need_hidden else None
+    dw = torch.empty(weight.shape, dtype=w.dtype, device=h.device) if need_weight else None
+    size = _workspace_bytes("aeth_cut_ce_workspace", n, d, v, 1)
+    ws = torch.empty(size, dtype=torch.uint8, device=h.device)
+    L.check(_lib.aeth_cut_ce_backward(
+        h.data_ptr(), ld_h, w.data_ptr(), ld_w, _DTYPES[h.dtype], lab.data_ptr(), n, d, v, ignore_index,
+        lse.data_ptr(), None if grad is None else grad.data_ptr(), scale, dh.data_ptr() if need_hidden else None, d,
+        dw.data_ptr() if need_weight else None, d, ws.data_ptr(), size, _raw_stream(h.get_device())),
+        "aeth_cut_ce_backward")
     return dh, dw
 
 
 # ---- checkpointed norm ----
-@dataclass
+@dataclass(slots=True)
 class ActivationCheckpoint:
     """Activations in 8 bits: codes (..., d) int8 and one float32 scale per row
     and block of CHECKPOINT_BLOCK features, (..., ceil(d / 128)); `dtype` is the
@@ -155,68 +176,79 @@ class ActivationCheckpoint:
     dtype: torch.dtype
 
 
-def _gain(what, gain, d):
-    if gain.dim() != 1 or gain.shape[0] != d or gain.dtype not in _DTYPES:
+def _gain(what, gain, d, dev):
+    if gain.dim() != 1 or gain.size(0) != d or gain.dtype not in _DTYPES:
         raise ValueError(f"{what}: weight must be a float vector of {d} features")
-    return gain.contiguous()
+    _same_device(what, dev, gain)
+    return gain.contiguous(), _DTYPES[gain.dtype]
 
 
 def _ckpt_args(what, ckpt):
+    """(codes, scales, rows, d) of a checkpoint, contiguous."""
     codes, scales = ckpt.codes, ckpt.scales
-    d = codes.shape[-1] if codes.dim() else 0
+    d = codes.size(-1) if codes.dim() else 0
     rows = codes.numel() // d if d else 0
     blocks = -(-d // CHECKPOINT_BLOCK)
-    if codes.dtype != torch.int8 or scales.dtype != torch.float32 or d == 0 or scales.numel() != rows * blocks \
-            or scales.shape[-1] != blocks or ckpt.dtype not in _DTYPES:
+    if d == 0 or codes.dtype != torch.int8 or scales.dtype != torch.float32 or scales.numel() != rows * blocks \
+            or scales.size(-1) != blocks or ckpt.dtype not in _DTYPES:
         raise ValueError(f"{what}: an ActivationCheckpoint with int8 codes (..., d) and float32 scales "
                          f"(..., ceil(d / {CHECKPOINT_BLOCK})) expected")
-    return _device_of(what, codes, scales), codes.contiguous(), scales.contiguous(), rows, d
+    _same_device(what, codes.get_device(), scales)
+    return codes.contiguous(), scales.contiguous(), rows, d
 
 
+@_on_device
 def rms_norm_checkpoint(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
                         residual: torch.Tensor | None = None):
     """RMS norm of x (..., d) times `weight`, and x in 8 bits for the second
     pass: (y, checkpoint).  With `residual` the norm's input is x + residual,
     rounded to x's type: (y, checkpoint, sum).  float32, float16 or bfloat16."""
     what = "rms_norm_checkpoint"
-    if x.dtype not in _DTYPES or x.dim() < 1 or x.shape[-1] == 0:
+    dt, dev = _DTYPES.get(x.dtype), x.get_device()
+    d = x.size(-1) if x.dim() else 0
+    if dt is None or d == 0:
         raise ValueError(f"{what}: x must be a float tensor (..., d)")
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
-        raise ValueError(f"{what}: residual must match x")
-    dev = _device_of(what, x, weight, residual)
-    d = x.shape[-1]
-    gain = _gain(what, weight, d)
-    xr = _rows2d(x)
-    rr = None if residual is None else _rows2d(residual)
-    with torch.cuda.device(dev):
-        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        codes = torch.empty(x.shape, dtype=torch.int8, device=dev)
-        scales = torch.empty((*x.shape[:-1], -(-d // CHECKPOINT_BLOCK)), dtype=torch.float32, device=dev)
-        total = None if rr is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
-        L.check(L.load().aeth_rms_norm_checkpoint(
-            _addr(xr), _pitch(xr), _addr(rr), 0 if rr is None else _pitch(rr), _addr(gain), _DTYPES[gain.dtype],
-            _DTYPES[x.dtype], xr.shape[0], d, float(eps), _addr(total), _addr(y), _addr(codes), _addr(scales),
-            torch.cuda.current_stream().cuda_stream), "aeth_rms_norm_checkpoint")
+    gain, gain_dt = _gain(what, weight, d, dev)
+    xr, rows, ld = _rows(x, d)
+    total, rr, ld_r = None, None, 0
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise ValueError(f"{what}: residual must match x")
+        _same_device(what, dev, residual)
+        rr, _, ld_r = _rows(residual, d)
+        total = torch.empty_like(x, memory_format=torch.contiguous_format)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    codes = torch.empty_like(x, dtype=torch.int8, memory_format=torch.contiguous_format)
+    scales = x.new_empty((*x.shape[:-1], -(-d // CHECKPOINT_BLOCK)), dtype=torch.float32)
+    st = _lib.aeth_rms_norm_checkpoint(
+        xr.data_ptr(), ld, None if rr is None else rr.data_ptr(), ld_r, gain.data_ptr(), gain_dt, dt, rows, d, eps,
+        None if total is None else total.data_ptr(), y.data_ptr(), codes.data_ptr(), scales.data_ptr(),
+        _raw_stream(dev))
+    if st:
+        L.check(st, "aeth_rms_norm_checkpoint")
     ckpt = ActivationCheckpoint(codes, scales, x.dtype)
     return (y, ckpt) if residual is None else (y, ckpt, total)
 
 
+@_on_device
 def checkpoint_decode(ckpt: ActivationCheckpoint, norm_weight: torch.Tensor | None = None,
                       eps: float = 1e-6) -> torch.Tensor:
     """The checkpoint's activations restored to their type; with `norm_weight`
     their RMS norm times it (the second pass's recomputed norm)."""
     what = "checkpoint_decode"
-    dev, codes, scales, rows, d = _ckpt_args(what, ckpt)
-    gain = None if norm_weight is None else _gain(what, norm_weight, d)
-    _device_of(what, codes, gain)
-    with torch.cuda.device(dev):
-        out = torch.empty(codes.shape, dtype=ckpt.dtype, device=dev)
-        L.check(L.load().aeth_checkpoint_decode(
-            _addr(codes), _addr(scales), rows, d, _addr(gain), 0 if gain is None else _DTYPES[gain.dtype], float(eps),
-            _addr(out), d, _DTYPES[ckpt.dtype], torch.cuda.current_stream().cuda_stream), "aeth_checkpoint_decode")
+    codes, scales, rows, d = _ckpt_args(what, ckpt)
+    dev = codes.get_device()
+    gain, gain_dt = (None, 0) if norm_weight is None else _gain(what, norm_weight, d, dev)
+    out = torch.empty_like(codes, dtype=ckpt.dtype)
+    st = _lib.aeth_checkpoint_decode(codes.data_ptr(), scales.data_ptr(), rows, d,
+                                     None if gain is None else gain.data_ptr(), gain_dt, eps, out.data_ptr(), d,
+                                     _DTYPES[ckpt.dtype], _raw_stream(dev))
+    if st:
+        L.check(st, "aeth_checkpoint_decode")
     return out
 
 
+@_on_device
 def rms_norm_checkpoint_backward(dy: torch.Tensor, ckpt: ActivationCheckpoint, weight: torch.Tensor, eps: float = 1e-6,
                                  d_residual: torch.Tensor | None = None):
     """(dx, d_weight) of the RMS norm at the restored activations, for the
@@ -224,46 +256,54 @@ def rms_norm_checkpoint_backward(dy: torch.Tensor, ckpt: ActivationCheckpoint, w
     norm's input past it, is added to dx.  dx has dy's type, d_weight is
     float32 (the sum over all rows, in one fixed order)."""
     what = "rms_norm_checkpoint_backward"
-    dev, codes, scales, rows, d = _ckpt_args(what, ckpt)
-    gain = _gain(what, weight, d)
+    codes, scales, rows, d = _ckpt_args(what, ckpt)
+    dev = dy.get_device()
+    gain, gain_dt = _gain(what, weight, d, dev)
     if dy.shape != codes.shape or dy.dtype != ckpt.dtype:
         raise ValueError(f"{what}: dy must have the checkpoint's shape and type")
-    if d_residual is not None and (d_residual.shape != dy.shape or d_residual.dtype != dy.dtype):
-        raise ValueError(f"{what}: d_residual must match dy")
-    _device_of(what, codes, dy, gain, d_residual)
-    g = _rows2d(dy)
-    r = None if d_residual is None else _rows2d(d_residual)
-    with torch.cuda.device(dev):
-        dx = torch.empty(dy.shape, dtype=dy.dtype, device=dev)
-        dw = torch.empty(d, dtype=torch.float32, device=dev)
-        ws, size = _workspace("aeth_rms_norm_checkpoint_backward_workspace", dev, rows, d)
-        L.check(L.load().aeth_rms_norm_checkpoint_backward(
-            _addr(g), _pitch(g), _addr(codes), _addr(scales), _addr(gain), _DTYPES[gain.dtype], _addr(r),
-            0 if r is None else _pitch(r), _DTYPES[dy.dtype], rows, d, float(eps), _addr(dx), _addr(dw), _addr(ws),
-            size, torch.cuda.current_stream().cuda_stream), "aeth_rms_norm_checkpoint_backward")
+    _same_device(what, dev, codes, d_residual)
+    g, _, ld = _rows(dy, d)
+    r, ld_r = None, 0
+    if d_residual is not None:
+        if d_residual.shape != dy.shape or d_residual.dtype != dy.dtype:
+            raise ValueError(f"{what}: d_residual must match dy")
+        r, _, ld_r = _rows(d_residual, d)
+    dx = torch.empty_like(dy, memory_format=torch.contiguous_format)
+    dw = dy.new_empty(d, dtype=torch.float32)
+    size = _workspace_bytes("aeth_rms_norm_checkpoint_backward_workspace", rows, d)
+    ws = dy.new_empty(size, dtype=torch.uint8)
+    st = _lib.aeth_rms_norm_checkpoint_backward(
+        g.data_ptr(), ld, codes.data_ptr(), scales.data_ptr(), gain.data_ptr(), gain_dt,
+        None if r is None else r.data_ptr(), ld_r, _DTYPES[dy.dtype], rows, d, eps, dx.data_ptr(), dw.data_ptr(),
+        ws.data_ptr(), size, _raw_stream(dev))
+    if st:
+        L.check(st, "aeth_rms_norm_checkpoint_backward")
     return dx, dw
 
 
+@_on_device
 def checkpoint_weight_grad(dy: torch.Tensor, ckpt: ActivationCheckpoint, norm_weight: torch.Tensor | None = None,
                            eps: float = 1e-6) -> torch.Tensor:
     """Weight gradient (m, d) = dy^T X of a linear layer, dy (..., m) the gradient
     of its output, X (..., d) its input: the restored checkpoint, or with
     `norm_weight` its RMS norm times that.  bfloat16 or float16."""
     what = "checkpoint_weight_grad"
-    dev, codes, scales, rows, d = _ckpt_args(what, ckpt)
-    gain = None if norm_weight is None else _gain(what, norm_weight, d)
+    codes, scales, rows, d = _ckpt_args(what, ckpt)
+    dev = dy.get_device()
+    gain, gain_dt = (None, 0) if norm_weight is None else _gain(what, norm_weight, d, dev)
     if dy.dtype != ckpt.dtype or dy.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError(f"{what}: dy must be bfloat16 or float16, as the checkpoint")
-    if dy.dim() < 1 or dy.shape[:-1] != codes.shape[:-1] or dy.shape[-1] == 0:
+    m = dy.size(-1) if dy.dim() else 0
+    if m == 0 or dy.shape[:-1] != codes.shape[:-1]:
         raise ValueError(f"{what}: dy must be ({', '.join(map(str, codes.shape[:-1]))}, m)")
-    _device_of(what, codes, dy, gain)
-    g = _tma_rows(dy)
-    m = g.shape[1]
-    with torch.cuda.device(dev):
-        dw = torch.empty(m, d, dtype=dy.dtype, device=dev)
-        ws, size = _workspace("aeth_checkpoint_weight_grad_workspace", dev, rows, m, d)
-        L.check(L.load().aeth_checkpoint_weight_grad(
-            _addr(g), _pitch(g), _addr(codes), _addr(scales), _addr(gain), 0 if gain is None else _DTYPES[gain.dtype],
-            float(eps), _DTYPES[dy.dtype], rows, m, d, _addr(dw), d, _addr(ws), size,
-            torch.cuda.current_stream().cuda_stream), "aeth_checkpoint_weight_grad")
+    _same_device(what, dev, codes)
+    g, _, ld = _tma_rows(dy, m)
+    dw = dy.new_empty((m, d))
+    size = _workspace_bytes("aeth_checkpoint_weight_grad_workspace", rows, m, d)
+    ws = dy.new_empty(size, dtype=torch.uint8)
+    st = _lib.aeth_checkpoint_weight_grad(
+        g.data_ptr(), ld, codes.data_ptr(), scales.data_ptr(), None if gain is None else gain.data_ptr(), gain_dt, eps,
+        _DTYPES[dy.dtype], rows, m, d, dw.data_ptr(), d, ws.data_ptr(), size, _raw_stream(dev))
+    if st:
+        L.check(st, "aeth_checkpoint_weight_grad")
     return dw
