@@ -37,21 +37,40 @@ struct Carver {
 // ---------------------------------------------------------------------------
 constexpr int64_t kHeadMaxDim = 1ll << 30;       // token, feature and vocabulary counts (tile coordinates are int)
 constexpr int64_t kHeadGradBytes = 256ll << 20;  // G of one piece
-constexpr int kHeadBN = 256;
+
+// Columns per tile for a product of `cols` columns (B K-major) with `tiles_m`
+// row tiles: what makes the last wave of tiles over the 74 CTA pairs least
+// wasteful.  A wave lasts about bn columns plus a share that does not shrink
+// with bn (32 columns' worth of time).
+int head_bn(int64_t tiles_m, int64_t cols) {
+    int best = 256;
+    int64_t least = INT64_MAX;
+    for (int bn = 256; bn >= 64; bn -= 32) {
+        const int64_t units = tiles_m * ((cols + bn - 1) / bn), pairs = num_sms() / 2;
+        const int64_t cost = (units + pairs - 1) / pairs * (bn + 32);
+        if (cost < least) {
+            least = cost;
+            best = bn;
+        }
+    }
+    return best;
+}
 
 struct HeadPlan {
     int64_t n_pad, dp, piece, ldg;
+    int bn;      // tile columns of the forward
     int np;      // column ranges of the forward's statistics
     int splits;  // K splits of a piece's dH product
 
     HeadPlan(int64_t n, int64_t d, int64_t vocab) {
         n_pad = up(std::max<int64_t>(n, 1), 256);
         dp = up(d, 8);
-        np = 2 * (int)((vocab + kHeadBN - 1) / kHeadBN);
+        bn = head_bn(n_pad / 256, vocab);
+        np = 2 * (int)((vocab + bn - 1) / bn);
         // pieces of equal size (a multiple of the tile) whose G takes at most kHeadGradBytes
-        int64_t most = std::max<int64_t>(kHeadGradBytes / (2 * n_pad) / kHeadBN * kHeadBN, kHeadBN);
+        int64_t most = std::max<int64_t>(kHeadGradBytes / (2 * n_pad) / 256 * 256, 256);
         const int64_t count = (vocab + most - 1) / most;
-        piece = std::min(up((vocab + count - 1) / count, kHeadBN), up(vocab, 8));
+        piece = std::min(up((vocab + count - 1) / count, 256), up(vocab, 8));
         ldg = up(piece, 8);
         // a piece's dH has few tiles where there are few tokens: its K (the piece) is then
         // split so that every CTA pair has a unit, at least 8 k-blocks each
@@ -110,14 +129,14 @@ int head_check(const void* hidden, int64_t ld_hidden, const void* weight, int64_
     return AETH_OK;
 }
 
-int head_rows(const HeadRows& a, const void* hidden, int64_t ld, int64_t d, const HeadPlan& p, const HeadWork& w,
+int head_rows(const HeadRows& a, const void* hidden, int64_t ld, int64_t n, int64_t d, const HeadPlan& p, const HeadWork& w,
               cudaStream_t st) {
     DeviceRuntime* rt = nullptr;
     AETH_TRY(runtime_for_current(&rt));
     head_rows_kernel<<<1, 1024, 0, st>>>(a, rt->err_word);
     AETH_LAUNCH_CHECK();
     head_pack_kernel<<<(unsigned)std::min<int64_t>(p.n_pad, 65536), 256, 0, st>>>(
-        static_cast<const uint16_t*>(hidden), ld, (int)d, w.rows, w.count, w.h, p.dp);
+        static_cast<const uint16_t*>(hidden), ld, n, (int)d, w.rows, w.count, w.h, p.dp);
     AETH_LAUNCH_CHECK();
     return AETH_OK;
 }
@@ -128,11 +147,11 @@ int head_backward(const HeadPlan& p, const HeadWork& w, const void* weight, int6
     const uint16_t* W = static_cast<const uint16_t*>(weight);
     for (int64_t v0 = 0; v0 < vocab; v0 += p.piece) {
         const int64_t vp = std::min(p.piece, vocab - v0);
-        const PairOperand H{w.h, p.dp, p.n_pad, d}, Wp{W + v0 * ld_weight, ld_weight, vp, d};
-        const PairOperand G{w.g, p.ldg, p.n_pad, vp};
-        HeadGrad<BF16> eg{w.lab, w.coef, w.lse2, w.g, p.ldg, (int)v0};
+        const PairOperand H{w.h, p.dp, n, d}, Wp{W + v0 * ld_weight, ld_weight, vp, d};
+        const PairOperand G{w.g, p.ldg, n, vp};
+        HeadGrad<BF16> eg{w.lab, w.coef, w.lse2, w.g, p.ldg, (int)n, (int)v0};
         AETH_TRY((pair_gemm_launch<HeadGrad<BF16>, false, false>(H, Wp, (int)n, (int)vp, (int)d, w.count, PAIR_LIVE_M,
-                                                                 kHeadBN, 1, BF16, eg, st)));
+                                                                 head_bn(p.n_pad / 256, vp), 1, BF16, eg, st)));
         if (d_weight) {
             PairOut16<BF16> ew{static_cast<uint16_t*>(d_weight) + v0 * ld_dw, ld_dw, w.out_scale};
             AETH_TRY((pair_gemm_launch<PairOut16<BF16>, true, true>(G, H, (int)vp, (int)d, (int)n, w.count, PAIR_LIVE_K,
@@ -295,10 +314,10 @@ int aeth_cut_ce_forward(const void* hidden, int64_t ld_hidden, const void* weigh
     a.pos = w.pos;
     a.lab = w.lab;
     a.count = w.count;
-    AETH_TRY(head_rows(a, hidden, ld_hidden, d, p, w, st));
+    AETH_TRY(head_rows(a, hidden, ld_hidden, n, d, p, w, st));
     HeadStats es{w.lab, w.label_logit, w.part, p.n_pad};
-    AETH_TRY((pair_gemm_launch<HeadStats, false, false>({w.h, p.dp, p.n_pad, d}, {weight, ld_weight, vocab, d}, (int)n,
-                                                        (int)vocab, (int)d, w.count, PAIR_LIVE_M, kHeadBN, 1,
+    AETH_TRY((pair_gemm_launch<HeadStats, false, false>({w.h, p.dp, n, d}, {weight, ld_weight, vocab, d}, (int)n,
+                                                        (int)vocab, (int)d, w.count, PAIR_LIVE_M, p.bn, 1,
                                                         dtype == AETH_DTYPE_BF16, es, st)));
     head_loss_kernel<<<(unsigned)std::min<int64_t>((n + 31) / 32, 65536), 256, 0, st>>>(
         w.part, p.n_pad, p.np, w.label_logit, w.rows, w.count, losses, lse);
@@ -344,7 +363,7 @@ int aeth_cut_ce_backward(const void* hidden, int64_t ld_hidden, const void* weig
     a.coef = w.coef;
     a.lse2 = w.lse2;
     a.out_scale = w.out_scale;
-    AETH_TRY(head_rows(a, hidden, ld_hidden, d, p, w, st));
+    AETH_TRY(head_rows(a, hidden, ld_hidden, n, d, p, w, st));
     return bf16 ? head_backward<true>(p, w, weight, ld_weight, n, d, vocab, d_hidden, ld_dh, d_weight, ld_dw, st)
                 : head_backward<false>(p, w, weight, ld_weight, n, d, vocab, d_hidden, ld_dh, d_weight, ld_dw, st);
 }

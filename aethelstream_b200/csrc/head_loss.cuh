@@ -128,11 +128,13 @@ __global__ void __launch_bounds__(1024) head_rows_kernel(HeadRows a, uint32_t* e
 }
 
 // Live rows of H, gathered to a pitch that TMA takes; rows from the count up
-// to the next multiple of 256 are zero (the products' last tiles read them).
-__global__ void __launch_bounds__(256) head_pack_kernel(const uint16_t* __restrict__ h, int64_t ld, int d,
+// to the next multiple of 256 are zero (the products' last tiles read them;
+// past row n TMA itself fills with zero, without reading).
+__global__ void __launch_bounds__(256) head_pack_kernel(const uint16_t* __restrict__ h, int64_t ld, int64_t n, int d,
                                                         const int* __restrict__ rows, const int* __restrict__ count,
                                                         uint16_t* __restrict__ out, int64_t ldo) {
-    const int live = *count, padded = max((live + 255) / 256 * 256, 256);
+    const int live = *count;
+    const int64_t padded = min((int64_t)max((live + 255) / 256 * 256, 256), n);
     const bool whole = (ld % 8) == 0 && (d % 8) == 0 && (reinterpret_cast<uintptr_t>(h) & 15) == 0;
     for (int64_t i = blockIdx.x; i < padded; i += gridDim.x) {
         const uint16_t* src = h + (i < live ? (int64_t)rows[i] * ld : 0);
@@ -156,45 +158,53 @@ struct HeadStats {
     float* label_logit;
     float2* part;  // [2 * n_tile + half][row]
     int64_t ld_part;
-    __device__ __forceinline__ void tile(const PairTile& t) const {
+    static constexpr int kChunk = 8;  // the loss is an fp32 result: see pair_gemm.cuh
+    __device__ __forceinline__ void finish(const PairTile& t, const float (&acc)[128]) const {
         const int row = t.row0 + t.lane;
         const bool in = row < t.M;
-        const int lab = in ? lab_at(row) - t.col0 : -1;
+        const int at = in ? lab[row] - t.col0 - t.c_begin : -1;
         float mx = -INFINITY, sum = 0.0f;  // mx in units of log2
-        for (int c = t.c_begin; c < t.c_end; c += 32) {
-            float v[32];
-            tmem_ld32<0>(t.tmem + (uint32_t)c, v);
-            tmem_wait_ld();
-            if (t.col0 + c + 32 > t.N) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (t.col0 + c + i >= t.N) v[i] = -INFINITY;
-            }
-            float m = fmaxf(v[0], v[1]);
+        for (int c = 0; c < 4; ++c) {
+            const int left = min(t.c_end, t.N - t.col0) - t.c_begin - 32 * c;  // columns of this chunk that exist
+            if (left > 0) {
+                float m = -INFINITY;
+                if (left >= 32) {
 #pragma unroll
-            for (int i = 2; i < 32; i += 2) m = fmax3(m, v[i], v[i + 1]);
-            const float nm = fmaxf(mx, m * kLog2e);
-            const float off = nm == -INFINITY ? 0.0f : nm;
-            sum *= ex2(mx - off);
-            float s0 = 0.0f, s1 = 0.0f;
+                    for (int i = 0; i < 32; i += 2) m = fmax3(m, acc[32 * c + i], acc[32 * c + i + 1]);
+                } else {
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-                s0 += ex2(fmaf(v[i], kLog2e, -off));
-                s1 += ex2(fmaf(v[i + 1], kLog2e, -off));
-            }
-            sum += s0 + s1;
-            mx = nm;
-            const int k = lab - c;
-            if (__any_sync(0xffffffffu, k >= 0 && k < 32)) {
-                float x = 0.0f;
+                    for (int i = 0; i < 32; ++i)
+                        if (i < left) m = fmaxf(m, acc[32 * c + i]);
+                }
+                const float nm = fmaxf(mx, m * kLog2e);
+                const float off = nm == -INFINITY ? 0.0f : nm;
+                sum *= ex2(mx - off);
+                float s0 = 0.0f, s1 = 0.0f;
+                if (left >= 32) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) x = k == i ? v[i] : x;
-                if (k >= 0 && k < 32) label_logit[row] = x;
+                    for (int i = 0; i < 32; i += 2) {
+                        s0 += ex2(fmaf(acc[32 * c + i], kLog2e, -off));
+                        s1 += ex2(fmaf(acc[32 * c + i + 1], kLog2e, -off));
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (i < left) s0 += ex2(fmaf(acc[32 * c + i], kLog2e, -off));
+                }
+                sum += s0 + s1;
+                mx = nm;
+                const int k = at - 32 * c;
+                if (__any_sync(0xffffffffu, k >= 0 && k < 32)) {
+                    float x = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) x = k == i ? acc[32 * c + i] : x;
+                    if (k >= 0 && k < 32) label_logit[row] = x;
+                }
             }
         }
         if (in) part[(int64_t)(2 * t.n_tile + t.half) * ld_part + row] = make_float2(mx, sum);
     }
-    __device__ __forceinline__ int lab_at(int row) const { return lab[row]; }
 };
 
 // Joins the column ranges' maxima and sums.  A CTA takes 32 live rows (lane =
@@ -259,14 +269,16 @@ __global__ void __launch_bounds__(1024) head_mean_kernel(const int* __restrict__
 }
 
 // Epilogue of the backward's product: G of the piece in 16 bits.  G is rounded
-// once, from fp32; rows past the count (up to the tile's end) become zero.
+// once, from fp32; rows from the count to the tile's end (or n) become zero.
 template <bool BF16>
 struct HeadGrad {
+    static constexpr int kChunk = 0;
     const int* lab;
     const float* coef;
     const float* lse2;
     uint16_t* g;
     int64_t ldg;
+    int n;   // rows of g: the tokens
     int v0;  // first vocabulary entry of the piece
     __device__ __forceinline__ void tile(const PairTile& t) const {
         const int row = t.row0 + t.lane;
@@ -274,7 +286,7 @@ struct HeadGrad {
         const float f = in ? coef[row] : 0.0f, l2 = in ? lse2[row] : 0.0f;
         const int lab_c = in ? lab[row] - v0 - t.col0 : -1;
         for (int c = t.c_begin; c < t.c_end; c += 64) {
-            if (t.col0 + c >= t.N) break;
+            if (t.col0 + c >= t.N || t.row0 >= n) break;
             uint32_t w[32];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -293,7 +305,7 @@ struct HeadGrad {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) w[16 * h + i] = pack16<BF16>(v[2 * i] * f, v[2 * i + 1] * f);
             }
-            pair_store16(t, w, c, g, ldg, t.row0 + 32, min(t.N, t.col0 + t.c_end));
+            pair_store16(t, w, c, g, ldg, n, min(t.N, t.col0 + t.c_end));
         }
     }
 };

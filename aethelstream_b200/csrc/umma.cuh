@@ -253,6 +253,20 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[N]) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[OFF + i] = __uint_as_float(r[i]);
 }
+// 32 lanes x 16 consecutive 32-bit TMEM columns into v[OFF .. OFF+15].
+template <int OFF, int N>
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[N]) {
+    static_assert(OFF + 16 <= N, "tmem_ld16 destination too small");
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[OFF + i] = __uint_as_float(r[i]);
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // wait::ld that also binds the 16 destination registers of an earlier
