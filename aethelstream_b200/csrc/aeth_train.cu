@@ -60,7 +60,8 @@ struct HeadPlan {
     int64_t n_pad, dp, piece, ldg;
     int bn;      // tile columns of the forward
     int np;      // column ranges of the forward's statistics
-    int splits;  // K splits of a piece's dH product
+    int tail_kb;    // k-blocks of a piece's dH product
+    int64_t extra;  // buffers of its tail
 
     HeadPlan(int64_t n, int64_t d, int64_t vocab) {
         n_pad = up(std::max<int64_t>(n, 1), 256);
@@ -72,14 +73,16 @@ struct HeadPlan {
         const int64_t count = (vocab + most - 1) / most;
         piece = std::min(up((vocab + count - 1) / count, 256), up(vocab, 8));
         ldg = up(piece, 8);
-        // a piece's dH has few tiles where there are few tokens: its K (the piece) is then
-        // split so that every CTA pair has a unit, at least 8 k-blocks each
-        const int64_t tiles = n_pad / 256 * ((d + 255) / 256), kb = (piece + 63) / 64;
-        const int64_t s = std::max<int64_t>(std::min<int64_t>(74 / tiles, kb / 8), 1);
-        const int64_t per = (kb + s - 1) / s;
-        splits = (int)((kb + per - 1) / per);
+        tail_kb = (int)((piece + 63) / 64);
+        // buffers that a dH product's tail may need: it has at most this many tiles
+        const int64_t tiles = n_pad / 256 * ((d + 255) / 256);
+        extra = std::min<int64_t>(3 * pair_count(), 15 * std::min<int64_t>(tiles, pair_count()));
     }
 };
+
+// The forward of a few tokens reads the weight by rows (head_vec_kernel).
+constexpr int kHeadVecShared = 96 * 1024;
+bool head_vec_fits(int64_t n, int64_t d) { return n <= kHeadVecTokens && n * up(d, 8) * 2 <= kHeadVecShared; }
 
 struct HeadWork {
     int *rows, *pos, *lab, *count;
@@ -88,7 +91,7 @@ struct HeadWork {
     float* label_logit;
     float2* part;
     // backward
-    float *coef, *lse2, *out_scale, *slab;
+    float *coef, *lse2, *out_scale, *slab, *extra;
     uint16_t* g;
     size_t bytes;
 
@@ -101,17 +104,18 @@ struct HeadWork {
         h = c.take<uint16_t>(p.n_pad * p.dp);
         label_logit = nullptr;
         part = nullptr;
-        coef = lse2 = out_scale = slab = nullptr;
+        coef = lse2 = out_scale = slab = extra = nullptr;
         g = nullptr;
         if (!backward) {
             label_logit = c.take<float>(p.n_pad);
-            part = c.take<float2>((int64_t)p.np * p.n_pad);
+            part = c.take<float2>(std::max<int64_t>((int64_t)p.np * p.n_pad, 2 * num_sms() * kHeadVecTokens));
         } else {
             coef = c.take<float>(p.n_pad);
             lse2 = c.take<float>(p.n_pad);
             out_scale = c.take<float>(1);
             g = c.take<uint16_t>(p.n_pad * p.ldg);
-            slab = c.take<float>(p.splits * p.n_pad * p.dp);
+            slab = c.take<float>(p.n_pad * p.dp);
+            extra = c.take<float>(p.extra * 65536);
         }
         bytes = c.used;
     }
@@ -135,9 +139,24 @@ int head_rows(const HeadRows& a, const void* hidden, int64_t ld, int64_t n, int6
     AETH_TRY(runtime_for_current(&rt));
     head_rows_kernel<<<1, 1024, 0, st>>>(a, rt->err_word);
     AETH_LAUNCH_CHECK();
-    head_pack_kernel<<<(unsigned)std::min<int64_t>(p.n_pad, 65536), 256, 0, st>>>(
-        static_cast<const uint16_t*>(hidden), ld, n, (int)d, w.rows, w.count, w.h, p.dp);
+    AETH_CUDA(launch_after(head_pack_kernel, dim3((unsigned)std::min<int64_t>(n, 65536)), dim3(256), 0, st, 1,
+                           static_cast<const uint16_t*>(hidden), ld, n, (int)d, w.rows, w.count, w.h, p.dp));
+    return AETH_OK;
+}
+
+template <bool BF16>
+int head_vec(const HeadVec& a, int64_t n, int ctas, float* losses, float* lse, float* loss, cudaStream_t st) {
+    DeviceRuntime* rt = nullptr;
+    AETH_TRY(runtime_for_current(&rt));
+    auto kern = n == 1 ? head_vec_kernel<BF16, 1> : n == 2 ? head_vec_kernel<BF16, 2>
+              : n == 3 ? head_vec_kernel<BF16, 3> : head_vec_kernel<BF16, 4>;
+    const int smem = (int)(n * up(a.d, 8) * 2);
+    static std::atomic<bool> allowed[kHeadVecTokens][kMaxDevices] = {};
+    AETH_TRY(allow_shared(kern, kHeadVecShared, allowed[n - 1]));
+    kern<<<ctas, kHeadVecThreads, smem, st>>>(a);
     AETH_LAUNCH_CHECK();
+    AETH_CUDA(launch_after(head_vec_loss_kernel, dim3(1), dim3(32 * (unsigned)n), 0, st, 1, a, (int)n, ctas, losses, lse,
+                           loss, rt->err_word));
     return AETH_OK;
 }
 
@@ -151,26 +170,24 @@ int head_backward(const HeadPlan& p, const HeadWork& w, const void* weight, int6
         const PairOperand G{w.g, p.ldg, n, vp};
         HeadGrad<BF16> eg{w.lab, w.coef, w.lse2, w.g, p.ldg, (int)n, (int)v0};
         AETH_TRY((pair_gemm_launch<HeadGrad<BF16>, false, false>(H, Wp, (int)n, (int)vp, (int)d, w.count, PAIR_LIVE_M,
-                                                                 head_bn(p.n_pad / 256, vp), 1, BF16, eg, st)));
+                                                                 head_bn(p.n_pad / 256, vp), 0, BF16, eg, st)));
         if (d_weight) {
             PairOut16<BF16> ew{static_cast<uint16_t*>(d_weight) + v0 * ld_dw, ld_dw, w.out_scale};
             AETH_TRY((pair_gemm_launch<PairOut16<BF16>, true, true>(G, H, (int)vp, (int)d, (int)n, w.count, PAIR_LIVE_K,
-                                                                    256, 1, BF16, ew, st)));
+                                                                    256, 0, BF16, ew, st)));
         }
         if (d_hidden) {
-            const int64_t kb = (vp + 63) / 64, full = (p.piece + 63) / 64;
-            const int64_t per = (full + p.splits - 1) / p.splits;
-            PairSlab es{w.slab, p.dp, p.n_pad * p.dp, v0 == 0};
-            const int splits = (int)((kb + per - 1) / per);  // a shorter last piece fills fewer slabs
+            PairSlab es{w.slab, p.dp, w.extra, v0 == 0};
             AETH_TRY((pair_gemm_launch<PairSlab, false, true>(G, Wp, (int)n, (int)d, (int)vp, w.count, PAIR_LIVE_M, 256,
-                                                              splits, BF16, es, st)));
+                                                              p.tail_kb, BF16, es, st)));
         }
     }
     if (d_hidden && n > 0) {
-        head_dh_kernel<BF16><<<(unsigned)std::min<int64_t>(n, 65536), 256, 0, st>>>(
-            w.slab, p.dp, p.n_pad * p.dp, p.splits, w.pos, n, (int)d, w.out_scale, static_cast<uint16_t*>(d_hidden),
-            ld_dh);
-        AETH_LAUNCH_CHECK();
+        const HeadDh a{w.slab, p.dp, w.extra, pair_count(), p.tail_kb, w.pos, w.count, n, (int)d, w.out_scale,
+                       static_cast<uint16_t*>(d_hidden), ld_dh};
+        const unsigned cols = (unsigned)((d + 1023) / 1024);
+        const unsigned rows = (unsigned)std::min<int64_t>(n, std::max<int64_t>(8 * num_sms() / cols, 1));
+        AETH_CUDA(launch_after(head_dh_kernel<BF16>, dim3(rows, cols), dim3(256), 0, st, 1, a));
     }
     return AETH_OK;
 }
@@ -216,6 +233,7 @@ constexpr int kStorePerSm = 8, kBackPerSm = 3;
 // The ring's layout for rows of d features: groups of tx threads that hold a
 // row in four eights each, as many stages as shared memory takes beside gain.
 // Taken for many rows (each SM walks over several) that bulk copies can move.
+constexpr int kRingShared = 220 * 1024;
 CkptRing ring_plan(int64_t d, int size, bool res) {
     CkptRing r;
     r.tx = (int)((d + 1023) / 1024) * 32;
@@ -224,7 +242,7 @@ CkptRing ring_plan(int64_t d, int size, bool res) {
     r.res_at = row;
     r.codes_at = row * (res ? 2 : 1);
     r.stage_bytes = r.codes_at + (int)up(d, 128);
-    const int room = 220 * 1024 - 4 * 8 * 4 * r.tx;
+    const int room = kRingShared - 4 * 8 * 4 * r.tx;
     while (r.groups > 1 && room / r.stage_bytes / r.groups < 2) r.groups /= 2;  // two stages a group at least
     r.stages = std::min(room / r.stage_bytes / r.groups, kRingMaxStages);
     return r;
@@ -302,9 +320,16 @@ int aeth_cut_ce_forward(const void* hidden, int64_t ld_hidden, const void* weigh
         AETH_CUDA(cudaMemsetAsync(loss, 0, sizeof(float), st));
         return AETH_OK;
     }
+    const bool bf16 = dtype == AETH_DTYPE_BF16;
     const HeadPlan p(n, d, vocab);
     const HeadWork w(p, n, false, workspace);
     if (workspace_bytes < w.bytes || !aligned16(workspace)) return set_err(AETH_ERR_ARG);
+    if (head_vec_fits(n, d)) {
+        const HeadVec a{static_cast<const uint16_t*>(hidden), ld_hidden, static_cast<const uint16_t*>(weight), ld_weight,
+                        labels, (int)d, (int)vocab, ignore_index, w.label_logit, w.part};
+        const int ctas = (n == 1 ? 2 : 1) * num_sms();
+        return bf16 ? head_vec<true>(a, n, ctas, losses, lse, loss, st) : head_vec<false>(a, n, ctas, losses, lse, loss, st);
+    }
     HeadRows a = {};
     a.labels = labels;
     a.n = n;
@@ -317,13 +342,11 @@ int aeth_cut_ce_forward(const void* hidden, int64_t ld_hidden, const void* weigh
     AETH_TRY(head_rows(a, hidden, ld_hidden, n, d, p, w, st));
     HeadStats es{w.lab, w.label_logit, w.part, p.n_pad};
     AETH_TRY((pair_gemm_launch<HeadStats, false, false>({w.h, p.dp, n, d}, {weight, ld_weight, vocab, d}, (int)n,
-                                                        (int)vocab, (int)d, w.count, PAIR_LIVE_M, p.bn, 1,
-                                                        dtype == AETH_DTYPE_BF16, es, st)));
-    head_loss_kernel<<<(unsigned)std::min<int64_t>((n + 31) / 32, 65536), 256, 0, st>>>(
-        w.part, p.n_pad, p.np, w.label_logit, w.rows, w.count, losses, lse);
-    AETH_LAUNCH_CHECK();
-    head_mean_kernel<<<1, 1024, 0, st>>>(w.pos, n, w.count, losses, lse, loss);
-    AETH_LAUNCH_CHECK();
+                                                        (int)vocab, (int)d, w.count, PAIR_LIVE_M, p.bn, 0,
+                                                        bf16, es, st)));
+    AETH_CUDA(launch_after(head_loss_kernel, dim3((unsigned)std::min<int64_t>((n + 7) / 8, 65536)), dim3(512), 0, st, 1,
+                           w.part, p.n_pad, p.np, w.label_logit, w.rows, w.count, losses, lse));
+    AETH_CUDA(launch_after(head_mean_kernel, dim3(1), dim3(1024), 0, st, 1, w.pos, n, w.count, losses, lse, loss));
     return AETH_OK;
 }
 
@@ -432,6 +455,11 @@ int aeth_rms_norm_checkpoint_backward(const void* dy, int64_t ld_dy, const int8_
                      (!d_residual || vec_rows(d_residual, ld_residual, sz));
     DeviceRuntime* rt = nullptr;
     AETH_TRY(runtime_for_current(&rt));
+    auto gain_sum = [&](int groups) -> int {
+        AETH_CUDA(launch_after(ckpt_gain_sum_kernel, dim3((unsigned)((d + 31) / 32)), dim3(1024), 0, st, 1, part, groups,
+                               (int)d, d_gain));
+        return AETH_OK;
+    };
     return by_row(dtype, p, vec, [&](auto* tag, auto vpt, auto v, auto wide) {
         using T = std::remove_pointer_t<decltype(tag)>;
         CkptBack<T> a{{codes, scales, gain, gain_dtype, rows, (int)d, eps}, static_cast<const T*>(dy), ld_dy,
@@ -439,22 +467,20 @@ int aeth_rms_norm_checkpoint_backward(const void* dy, int64_t ld_dy, const int8_
         if (vec && ring_fits(rows, d) && aligned16(codes)) {
             const CkptRing r = ring_plan(d, sz, d_residual != nullptr);
             const int smem = r.groups * r.stages * r.stage_bytes + 4 * 8 * 4 * r.tx;
+            static std::atomic<bool> allowed[kMaxDevices] = {};
             auto kern = ckpt_back_ring_kernel<T>;
-            AETH_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+            AETH_TRY(allow_shared(kern, kRingShared, allowed));
             kern<<<num_sms(), r.groups * r.tx, smem, st>>>(a, r, rt->err_word);
             AETH_LAUNCH_CHECK();
-            ckpt_gain_sum_kernel<<<(unsigned)((d + 31) / 32), 1024, 0, st>>>(part, num_sms(), (int)d, d_gain);
-            AETH_LAUNCH_CHECK();
-            return (int)AETH_OK;
+            return gain_sum(num_sms());
         }
         auto kern = ckpt_back_kernel<T, vpt.value, v.value, wide.value>;
         const int smem = p.shared(p.ty);
-        if (smem > 48 * 1024) AETH_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        static std::atomic<bool> allowed[kMaxDevices] = {};
+        AETH_TRY(allow_shared(kern, 64 * 1024, allowed));  // 8192 features: their sums and gain
         kern<<<p.grid, p.block(), smem, st>>>(a);
         AETH_LAUNCH_CHECK();
-        ckpt_gain_sum_kernel<<<(unsigned)((d + 31) / 32), 1024, 0, st>>>(part, (int)p.grid * p.ty, (int)d, d_gain);
-        AETH_LAUNCH_CHECK();
-        return (int)AETH_OK;
+        return gain_sum((int)p.grid * p.ty);
     });
 }
 
@@ -492,11 +518,11 @@ int aeth_checkpoint_weight_grad(const void* dy, int64_t ld_dy, const int8_t* cod
     if (bf16) {
         PairOut16<true> e{static_cast<uint16_t*>(d_weight), ld_dw, nullptr};
         return pair_gemm_launch<PairOut16<true>, true, true>(A, B, (int)m, (int)d, (int)rows, nullptr, PAIR_LIVE_NONE,
-                                                             256, 1, true, e, st);
+                                                             256, 0, true, e, st);
     }
     PairOut16<false> e{static_cast<uint16_t*>(d_weight), ld_dw, nullptr};
     return pair_gemm_launch<PairOut16<false>, true, true>(A, B, (int)m, (int)d, (int)rows, nullptr, PAIR_LIVE_NONE, 256,
-                                                          1, false, e, st);
+                                                          0, false, e, st);
 }
 
 }  // extern "C"

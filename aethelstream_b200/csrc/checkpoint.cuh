@@ -492,6 +492,7 @@ __global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, 4))
     extern __shared__ float4 ck_dyn[];
     constexpr bool kShared = ck_shared_gain(VPT, WIDE);
     const float inv_d = 1.0f / (float)a.d;
+    pdl_trigger();
     if (kShared) ck_gain_to_shared<VPT>(ck_dyn, a.gain, a.gain_dtype, a.d);
     int parity = 0;
     for (int64_t t0 = (int64_t)blockIdx.x * blockDim.y; t0 < a.rows; t0 += (int64_t)gridDim.x * blockDim.y, parity ^= 1) {
@@ -541,6 +542,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) ckpt_decode_flat_kernel(const uint4* __restrict__ codes,
                                                                const float* __restrict__ scales, int64_t n16,
                                                                T* __restrict__ out) {
+    pdl_trigger();
     for (int64_t i0 = (int64_t)blockIdx.x * 1024 + threadIdx.x; i0 < n16; i0 += (int64_t)gridDim.x * 1024) {
         uint4 q[4];
         float s[4];
@@ -567,6 +569,7 @@ __global__ void __launch_bounds__(256) ckpt_decode_flat_kernel(const uint4* __re
 template <typename T, int VPT, bool VEC>
 __global__ void __launch_bounds__(1024 / VPT) ckpt_decode_kernel(const __grid_constant__ CkptRead a, T* __restrict__ out,
                                                                  int64_t ldo) {
+    pdl_trigger();
     const int base = blockIdx.y * 8 * VPT * blockDim.x;
     for (int64_t t0 = (int64_t)blockIdx.x * blockDim.y; t0 < a.rows; t0 += (int64_t)gridDim.x * blockDim.y) {
         const int64_t t = t0 + threadIdx.y;
@@ -638,6 +641,7 @@ __global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, 2))
     ckpt_back_kernel(const __grid_constant__ CkptBack<T> a) {
     __shared__ float sh[4 * kCkptShared];
     extern __shared__ float4 ck_dyn[];
+    pdl_trigger();
     constexpr bool kShared = ck_shared_gain(VPT, WIDE);
     const float inv_d = 1.0f / (float)a.in.d;
     float* part = a.part + ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * a.in.d;
@@ -776,6 +780,7 @@ __global__ void __launch_bounds__(kRingThreads, 1)
     uint64_t* full = full_s + grp * kRingMaxStages;
     // gain: [k][half][thread of the group]
     ulonglong2* sg = reinterpret_cast<ulonglong2*>(ck_ring + (size_t)ring.groups * ring.stages * ring.stage_bytes);
+    pdl_trigger();
     if (threadIdx.x == 0) abort_s = 0;
     if (x0 == 0) {
         for (int s = 0; s < ring.stages; ++s) mbar_init(&full[s], 1);
@@ -897,9 +902,9 @@ __global__ void __launch_bounds__(kRingThreads, 1)
 
 // d_gain: 32 columns a CTA, its 32 warps every 32nd row group, then the warps
 // in their order.
-__global__ void __launch_bounds__(1024) ckpt_gain_sum_kernel(const float* __restrict__ part, int np, int d,
-                                                             float* __restrict__ d_gain) {
+__global__ void __launch_bounds__(1024) ckpt_gain_sum_kernel(const float* part, int np, int d, float* d_gain) {
     __shared__ float sh[32][33];
+    pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int c = blockIdx.x * 32 + lane;
     float s = 0.0f;

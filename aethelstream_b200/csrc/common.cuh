@@ -241,6 +241,44 @@ __device__ __forceinline__ float lin_scale_from_absmax(float amax) {
 
 __device__ __forceinline__ float lin_inv(float scale) { return scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f; }
 
+// Programmatic dependent launch: a kernel launched with launch_after() may
+// start its set-up while the kernel before it on the stream drains; it calls
+// pdl_wait() before it touches memory that earlier work writes or reads, and
+// pdl_trigger() once its own successor may start its set-up.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename... P, typename... A>
+cudaError_t launch_after(void (*kern)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, int cluster, A&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim = {(unsigned)cluster, 1, 1};
+    cfg.attrs = at;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kern, P(args)...);
+}
+
+// Raises a kernel's dynamic shared memory limit once per device (`done` is the
+// kernel's own flag array).
+template <typename K>
+inline int allow_shared(K kern, int bytes, std::atomic<bool>* done) {
+    int dev = 0;
+    AETH_TRY(current_device(&dev));
+    if (dev < 0 || dev >= kMaxDevices) return set_err(AETH_ERR_UNSUPPORTED);
+    if (!done[dev].load(std::memory_order_acquire)) {
+        AETH_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        done[dev].store(true, std::memory_order_release);
+    }
+    return AETH_OK;
+}
+
 inline int grid_for(int64_t work, int threads, int cap = 148 * 16) {
     int64_t g = (work + threads - 1) / threads;
     if (g < 1) g = 1;

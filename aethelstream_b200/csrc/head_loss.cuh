@@ -55,54 +55,76 @@ struct HeadRows {
     float* out_scale;  // max|g| / g_scale
 };
 
-// One CTA numbers the live tokens in order (a scan over the labels) and
-// gathers what the epilogues need per live row.
+// One CTA numbers the live tokens in order (a scan over the labels, 8192 at a
+// time, so that their loads are in flight together) and gathers what the
+// epilogues need per live row.
 __global__ void __launch_bounds__(1024) head_rows_kernel(HeadRows a, uint32_t* err) {
-    __shared__ int wsum[32];
+    constexpr int kItems = 8;
+    __shared__ int wsum[kItems * 32];
     __shared__ float wmax[32];
     __shared__ int base_s;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    pdl_trigger();
     int base = 0;
     float gmax = 0.0f;
     bool gnan = false;
-    for (int64_t t0 = 0; t0 < a.n; t0 += 1024) {
-        const int64_t t = t0 + tid;
-        bool live = false, bad = false;
-        int64_t lab = 0;
-        if (t < a.n) {
-            lab = a.labels[t];
-            live = lab != a.ignore_index;
-            bad = live && (lab < 0 || lab >= a.vocab);
-            if (bad) { live = false; report_dev_error(err, DEVERR_BAD_ARG); }
+    for (int64_t t0 = 0; t0 < a.n; t0 += kItems * 1024) {
+        int64_t lab[kItems];
+        float lse[kItems], grad[kItems];
+        uint32_t m[kItems];
+#pragma unroll
+        for (int k = 0; k < kItems; ++k) {
+            const int64_t t = t0 + k * 1024 + tid;
+            lab[k] = t < a.n ? a.labels[t] : a.ignore_index;
+            lse[k] = a.coef && t < a.n ? a.lse[t] : 0.0f;
+            grad[k] = a.coef && a.grad && t < a.n ? a.grad[t] : 0.0f;
         }
-        const uint32_t m = __ballot_sync(0xffffffffu, live);
-        if (lane == 0) wsum[warp] = __popc(m);
+#pragma unroll
+        for (int k = 0; k < kItems; ++k) {
+            const bool live = lab[k] != a.ignore_index && lab[k] >= 0 && lab[k] < a.vocab;
+            m[k] = __ballot_sync(0xffffffffu, live);
+            if (lane == 0) wsum[k * 32 + warp] = __popc(m[k]);
+        }
         __syncthreads();
-        if (warp == 0) {
-            int v = wsum[lane], s = v;
+        if (warp == 0) {  // exclusive scan of the 256 warp counts: eight a lane
+            int v[kItems], s = 0;
+#pragma unroll
+            for (int k = 0; k < kItems; ++k) {
+                v[k] = s;
+                s += wsum[lane * kItems + k];
+            }
+            int x = s;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int x = __shfl_up_sync(0xffffffffu, s, o);
-                if (lane >= o) s += x;
+                const int y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
             }
-            wsum[lane] = s - v;
-            if (lane == 31) base_s = s;
+#pragma unroll
+            for (int k = 0; k < kItems; ++k) wsum[lane * kItems + k] = x - s + v[k];
+            if (lane == 31) base_s = x;
         }
         __syncthreads();
-        if (t < a.n) {
-            const int i = base + wsum[warp] + __popc(m & ((1u << lane) - 1));
-            a.pos[t] = live ? i : bad ? kHeadBad : kHeadIgnored;
-            if (live) {
-                a.rows[i] = (int)t;
-                a.lab[i] = (int)lab;
-                if (a.coef) {
-                    a.lse2[i] = fmaf(a.lse[t], kLog2e, -a.g_bits);
-                    if (a.grad) {
-                        const float g = a.grad[t] * a.scale;
-                        a.coef[i] = g;
-                        gmax = fmaxf(gmax, fabsf(g));
-                        gnan |= g != g;
-                    }
+#pragma unroll
+        for (int k = 0; k < kItems; ++k) {
+            const int64_t t = t0 + k * 1024 + tid;
+            if (t >= a.n) continue;
+            if (!((m[k] >> lane) & 1u)) {
+                const bool bad = lab[k] != a.ignore_index;
+                if (bad) report_dev_error(err, DEVERR_BAD_ARG);
+                a.pos[t] = bad ? kHeadBad : kHeadIgnored;
+                continue;
+            }
+            const int i = base + wsum[k * 32 + warp] + __popc(m[k] & ((1u << lane) - 1));
+            a.pos[t] = i;
+            a.rows[i] = (int)t;
+            a.lab[i] = (int)lab[k];
+            if (a.coef) {
+                a.lse2[i] = fmaf(lse[k], kLog2e, -a.g_bits);
+                if (a.grad) {
+                    const float g = grad[k] * a.scale;
+                    a.coef[i] = g;
+                    gmax = fmaxf(gmax, fabsf(g));
+                    gnan |= g != g;
                 }
             }
         }
@@ -131,8 +153,10 @@ __global__ void __launch_bounds__(1024) head_rows_kernel(HeadRows a, uint32_t* e
 // to the next multiple of 256 are zero (the products' last tiles read them;
 // past row n TMA itself fills with zero, without reading).
 __global__ void __launch_bounds__(256) head_pack_kernel(const uint16_t* __restrict__ h, int64_t ld, int64_t n, int d,
-                                                        const int* __restrict__ rows, const int* __restrict__ count,
+                                                        const int* rows, const int* count,
                                                         uint16_t* __restrict__ out, int64_t ldo) {
+    pdl_wait();
+    pdl_trigger();
     const int live = *count;
     const int64_t padded = min((int64_t)max((live + 255) / 256 * 256, 256), n);
     const bool whole = (ld % 8) == 0 && (d % 8) == 0 && (reinterpret_cast<uintptr_t>(h) & 15) == 0;
@@ -207,37 +231,53 @@ struct HeadStats {
     }
 };
 
-// Joins the column ranges' maxima and sums.  A CTA takes 32 live rows (lane =
-// row), its warps every eighth range.
-__global__ void __launch_bounds__(256) head_loss_kernel(const float2* __restrict__ part, int64_t ld_part, int np,
-                                                        const float* __restrict__ label_logit,
-                                                        const int* __restrict__ rows, const int* __restrict__ count,
-                                                        float* __restrict__ losses, float* __restrict__ lse) {
-    __shared__ float2 sh[8][32];
+// Joins two (maximum, sum) pairs.
+__device__ __forceinline__ float2 head_join(float2 a, float2 b) {
+    const float m = fmaxf(a.x, b.x), off = m == -INFINITY ? 0.0f : m;
+    return make_float2(m, a.y * ex2(a.x - off) + b.y * ex2(b.x - off));
+}
+__device__ __forceinline__ float head_lse(float2 a) {
+    return (a.x == -INFINITY ? 0.0f : a.x) * kLn2 + logf(a.y);
+}
+
+// Joins the column ranges' maxima and sums.  A CTA takes 8 live rows (lane % 8),
+// its 64 quarter-warps every 64th range, four loads in flight; then a tree.
+__global__ void __launch_bounds__(512) head_loss_kernel(const float2* part, int64_t ld_part, int np,
+                                                        const float* label_logit, const int* rows, const int* count,
+                                                        float* losses, float* lse) {
+    __shared__ float2 sh[16][8];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_wait();
+    pdl_trigger();
     const int live = *count;
-    for (int64_t r0 = (int64_t)blockIdx.x * 32; r0 < live; r0 += (int64_t)gridDim.x * 32) {
-        const int64_t row = r0 + lane;
-        float mx = -INFINITY, sum = 0.0f;
-        if (row < live) {
-            for (int p = warp; p < np; p += 8) {
-                const float2 x = part[p * ld_part + row];
-                const float nm = fmaxf(mx, x.x), off = nm == -INFINITY ? 0.0f : nm;
-                sum = sum * ex2(mx - off) + x.y * ex2(x.x - off);
-                mx = nm;
-            }
+    for (int64_t r0 = (int64_t)blockIdx.x * 8; r0 < live; r0 += (int64_t)gridDim.x * 8) {
+        const int64_t row = r0 + (lane & 7);
+        float2 x = make_float2(-INFINITY, 0.0f);
+        for (int p0 = warp * 4 + (lane >> 3); p0 < np; p0 += 256) {
+            float2 v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                v[k] = p0 + 64 * k < np && row < live ? part[(p0 + 64 * k) * ld_part + row] : make_float2(-INFINITY, 0.0f);
+            x = head_join(x, head_join(head_join(v[0], v[1]), head_join(v[2], v[3])));
         }
-        sh[warp][lane] = make_float2(mx, sum);
+#pragma unroll
+        for (int o = 8; o < 32; o <<= 1)
+            x = head_join(x, make_float2(__shfl_xor_sync(0xffffffffu, x.x, o), __shfl_xor_sync(0xffffffffu, x.y, o)));
+        if (lane < 8) sh[warp][lane] = x;
         __syncthreads();
-        if (warp == 0 && row < live) {
-            for (int w = 1; w < 8; ++w) mx = fmaxf(mx, sh[w][lane].x);
-            const float off = mx == -INFINITY ? 0.0f : mx;
-            sum = 0.0f;
-            for (int w = 0; w < 8; ++w) sum += sh[w][lane].y * ex2(sh[w][lane].x - off);
-            const float l = off * kLn2 + logf(sum);
-            const int t = rows[row];
-            lse[t] = l;
-            losses[t] = l - label_logit[row];
+        if (warp == 0) {
+            x = sh[lane >> 3][lane & 7];
+#pragma unroll
+            for (int w = 4; w < 16; w += 4) x = head_join(x, sh[w + (lane >> 3)][lane & 7]);
+#pragma unroll
+            for (int o = 8; o < 32; o <<= 1)
+                x = head_join(x, make_float2(__shfl_xor_sync(0xffffffffu, x.x, o), __shfl_xor_sync(0xffffffffu, x.y, o)));
+            if (lane < 8 && row < live) {
+                const float l = head_lse(x);
+                const int t = rows[row];
+                lse[t] = l;
+                losses[t] = l - label_logit[row];
+            }
         }
         __syncthreads();
     }
@@ -245,10 +285,10 @@ __global__ void __launch_bounds__(256) head_loss_kernel(const float2* __restrict
 
 // Losses of the tokens that take no part (0; NaN for a label outside the
 // vocabulary) and the mean over the live ones, summed in one fixed order.
-__global__ void __launch_bounds__(1024) head_mean_kernel(const int* __restrict__ pos, int64_t n,
-                                                         const int* __restrict__ count, float* __restrict__ losses,
-                                                         float* __restrict__ lse, float* __restrict__ loss) {
+__global__ void __launch_bounds__(1024) head_mean_kernel(const int* pos, int64_t n, const int* count, float* losses,
+                                                         float* lse, float* loss) {
     __shared__ double ws[32];
+    pdl_wait();
     double s = 0.0;
     for (int64_t t = threadIdx.x; t < n; t += 1024) {
         const int p = pos[t];
@@ -265,6 +305,167 @@ __global__ void __launch_bounds__(1024) head_mean_kernel(const int* __restrict__
     if (threadIdx.x < 32) {
         s = warp_sum_d(ws[threadIdx.x]);
         if (threadIdx.x == 0) *loss = (float)(s / (double)max(*count, 1));
+    }
+}
+
+// Forward of one to four tokens: a product that reads the weight once and does
+// little else, so the bytes in flight and their order in DRAM decide.  A warp
+// takes two vocabulary entries at a time, each a row read from its start to its
+// end (512 bytes an instruction, eight in flight), against the tokens' hidden
+// states in shared memory; it keeps their running maximum and sum and leaves
+// one pair per token and CTA.  (The tile product needs the same bytes in
+// 128-byte columns: 70 us at 4096 x 32000 where this takes 46; measured.)
+constexpr int kHeadVecTokens = 4, kHeadVecThreads = 512;
+
+struct HeadVec {
+    const uint16_t* hidden;
+    int64_t ld_h;
+    const uint16_t* weight;
+    int64_t ld_w;
+    const int64_t* labels;
+    int d, vocab;
+    int64_t ignore_index;
+    float* label_logit;  // [token]
+    float2* part;        // [CTA][token]
+};
+
+template <bool BF16>
+__device__ __forceinline__ float2 head_pair(uint32_t w) {
+    if (BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+template <bool BF16, int NT>
+__global__ void __launch_bounds__(kHeadVecThreads, NT == 1 ? 2 : 1) head_vec_kernel(const HeadVec a) {
+    constexpr int R = 2, U = 4;  // entries a warp, loads in flight an entry
+    extern __shared__ uint4 head_sh[];  // [token][eight of features]
+    __shared__ float2 red[kHeadVecThreads / 32][NT];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, eights = (a.d + 7) / 8;
+    const int64_t first = (int64_t)R * (blockIdx.x * (kHeadVecThreads / 32) + warp);
+    // the warp's first entries are on their way to L2 while the hidden states are staged
+    for (int r = 0; r < R; ++r)
+        for (int b = lane * 128; b < 2 * a.d && first + r < a.vocab; b += 4096)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(a.weight + (first + r) * a.ld_w) + b));
+    uint16_t* sh16 = reinterpret_cast<uint16_t*>(head_sh);
+    for (int i = threadIdx.x; i < NT * eights * 8; i += kHeadVecThreads) {
+        const int t = i / (eights * 8), c = i - t * eights * 8;
+        sh16[i] = c < a.d ? a.hidden[t * a.ld_h + c] : (uint16_t)0;
+    }
+    int lab[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int64_t l = a.labels[t];
+        lab[t] = l != a.ignore_index && l >= 0 && l < a.vocab ? (int)l : -1;
+    }
+    __syncthreads();
+    float2 st[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) st[t] = make_float2(-INFINITY, 0.0f);
+    pdl_trigger();
+    const int warps = gridDim.x * (kHeadVecThreads / 32);
+    for (int64_t v0 = first; v0 < a.vocab; v0 += (int64_t)R * warps) {
+        const uint16_t* row[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) row[r] = a.weight + min(v0 + r, (int64_t)a.vocab - 1) * a.ld_w;
+        float2 acc[R][NT];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) acc[r][t] = make_float2(0.0f, 0.0f);
+        for (int e0 = lane; e0 < eights; e0 += 32 * U) {
+            uint4 w[R][U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+                    w[r][u] = e0 + 32 * u < eights ? __ldg(reinterpret_cast<const uint4*>(row[r]) + e0 + 32 * u)
+                                                   : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int e = e0 + 32 * u;
+                if (e >= eights) break;
+                if (8 * e + 8 > a.d) {  // the row's last eight: nothing past its end
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        uint32_t* x = reinterpret_cast<uint32_t*>(&w[r][u]);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (8 * e + i >= a.d) x[i >> 1] &= (i & 1) ? 0x0000ffffu : 0xffff0000u;
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const uint4 h = head_sh[t * eights + e];
+                    const uint32_t hw[4] = {h.x, h.y, h.z, h.w};
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        const uint32_t ww[4] = {w[r][u].x, w[r][u].y, w[r][u].z, w[r][u].w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[r][t] = fma2_rn(head_pair<BF16>(ww[i]), head_pair<BF16>(hw[i]), acc[r][t]);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                float x = acc[r][t].x + acc[r][t].y;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+                if (v0 + r < a.vocab) {
+                    st[t] = head_join(st[t], make_float2(x * kLog2e, 1.0f));
+                    if (lab[t] == v0 + r && lane == 0) a.label_logit[t] = x;
+                }
+            }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+        if (lane == 0) red[warp][t] = st[t];
+    __syncthreads();
+    if (threadIdx.x < NT) {
+        float2 x = red[0][threadIdx.x];
+        for (int w = 1; w < kHeadVecThreads / 32; ++w) x = head_join(x, red[w][threadIdx.x]);
+        a.part[(int64_t)blockIdx.x * NT + threadIdx.x] = x;
+    }
+}
+
+// One warp a token joins the CTAs' pairs; then losses and mean.
+__global__ void __launch_bounds__(32 * kHeadVecTokens)
+    head_vec_loss_kernel(const HeadVec a, int n, int ctas, float* losses, float* lse, float* loss, uint32_t* err) {
+    __shared__ float sl[kHeadVecTokens];
+    __shared__ int sc[kHeadVecTokens];
+    const int t = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_wait();
+    float2 x = make_float2(-INFINITY, 0.0f);
+    for (int p0 = lane; p0 < ctas; p0 += 128) {
+        float2 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            v[k] = p0 + 32 * k < ctas ? a.part[(int64_t)(p0 + 32 * k) * n + t] : make_float2(-INFINITY, 0.0f);
+        x = head_join(x, head_join(head_join(v[0], v[1]), head_join(v[2], v[3])));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        x = head_join(x, make_float2(__shfl_xor_sync(0xffffffffu, x.x, o), __shfl_xor_sync(0xffffffffu, x.y, o)));
+    if (lane == 0) {
+        const int64_t lab = a.labels[t];
+        const bool in = lab != a.ignore_index, bad = in && (lab < 0 || lab >= a.vocab);
+        const float l = in ? head_lse(x) : 0.0f;
+        lse[t] = bad ? __int_as_float(0x7fc00000) : l;
+        losses[t] = sl[t] = bad ? __int_as_float(0x7fc00000) : in ? l - a.label_logit[t] : 0.0f;
+        sc[t] = in && !bad;
+        if (bad) report_dev_error(err, DEVERR_BAD_ARG);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double s = 0.0;
+        int count = 0;
+        for (int i = 0; i < n; ++i) {
+            s += (double)sl[i];
+            count += sc[i];
+        }
+        *loss = (float)(s / (double)max(count, 1));
     }
 }
 
@@ -310,23 +511,67 @@ struct HeadGrad {
     }
 };
 
-// dH of every token from the slabs (in their order), in 16 bits; zero for the
-// tokens that took no part.
+// dH of every token in 16 bits: the slab's row, plus the further K ranges of
+// the tail's tiles in their order; zero for the tokens that took no part.  A
+// CTA takes 1024 columns of tokens.
+struct HeadDh {
+    const float* slab;
+    int64_t ld;
+    const float* extra;
+    int pairs, tail_kb;
+    const int *pos, *count;
+    int64_t n;
+    int d;
+    const float* scale;
+    uint16_t* out;
+    int64_t ldo;
+};
 template <bool BF16>
-__global__ void __launch_bounds__(256) head_dh_kernel(const float* __restrict__ slab, int64_t ld, int64_t split_stride,
-                                                      int splits, const int* __restrict__ pos, int64_t n, int d,
-                                                      const float* __restrict__ scale, uint16_t* __restrict__ out,
-                                                      int64_t ldo) {
-    const float a = *scale;
-    for (int64_t t = blockIdx.x; t < n; t += gridDim.x) {
-        const int p = pos[t];
-        for (int c = threadIdx.x; c < d; c += blockDim.x) {
-            float v = 0.0f;
-            if (p >= 0) {
-                for (int s = 0; s < splits; ++s) v += slab[s * split_stride + p * ld + c];
-                v *= a;
+__global__ void __launch_bounds__(256) head_dh_kernel(const HeadDh a) {
+    __shared__ int sh[4];
+    pdl_wait();
+    const int tiles_n = (a.d + 255) / 256;
+    if (threadIdx.x == 0) {
+        const int tiles_m = max((*a.count + 255) / 256, 1);
+        const PairTail t(tiles_m * tiles_n, a.pairs, a.tail_kb);
+        sh[0] = tiles_m;
+        sh[1] = t.full;
+        sh[2] = t.rest;
+        sh[3] = t.splits;
+    }
+    __syncthreads();
+    const int tiles_m = sh[0], full = sh[1], rest = sh[2], splits = sh[3];
+    const float scale = *a.scale;
+    const int c = (blockIdx.y * 256 + threadIdx.x) * 4;
+    if (c >= a.d) return;
+    const bool whole = (a.ldo % 4) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 7) == 0 && c + 4 <= a.d;
+#pragma unroll 2
+    for (int64_t t = blockIdx.x; t < a.n; t += gridDim.x) {
+        const int p = a.pos[t];
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (p >= 0) {
+            v = *reinterpret_cast<const float4*>(a.slab + p * a.ld + c);  // ld is a multiple of 8: whole fours
+            const int i = pair_tile_index(p / 256, c / 256, tiles_m, tiles_n) - full;
+            if (i >= 0) {
+#pragma unroll 4
+                for (int s = 0; s + 1 < splits; ++s) {
+                    const float4 e = *reinterpret_cast<const float4*>(
+                        a.extra + ((int64_t)(s * rest + i) * 256 + p % 256) * 256 + c % 256);
+                    v = make_float4(v.x + e.x, v.y + e.y, v.z + e.z, v.w + e.w);
+                }
             }
-            out[t * ldo + c] = (uint16_t)pack16<BF16>(v, 0.0f);
+        }
+        const bool live = p >= 0;
+        const uint32_t lo = live ? pack16<BF16>(v.x * scale, v.y * scale) : 0u;
+        const uint32_t hi = live ? pack16<BF16>(v.z * scale, v.w * scale) : 0u;
+        uint16_t* o = a.out + t * a.ldo + c;
+        if (whole) {
+            *reinterpret_cast<uint2*>(o) = make_uint2(lo, hi);
+        } else {
+            const uint32_t w[2] = {lo, hi};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (c + k < a.d) o[k] = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
         }
     }
 }

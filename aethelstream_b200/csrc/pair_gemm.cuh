@@ -2,7 +2,7 @@
 // tcgen05 GEMM on CTA pairs, D (M x N) = A (M x K) B (K x N), 16-bit operands,
 // fp32 accumulation in TMEM, the epilogue a functor.
 //
-// Unit = (256 x bn tile of D, K split); each CTA of the pair holds its 128 rows
+// Unit = 256 x bn tile of D (or a K range of one, see PairTail); each CTA of the pair holds its 128 rows
 // of A and half of the tile's bn columns of B per 64-deep k-block, CTA 0 issues
 // the pair's MMAs (M = 256, N = bn) and its commits reach both CTAs' barriers.
 // 256 x 256 is the largest tile whose accumulator fits TMEM twice (2 x 256
@@ -48,9 +48,41 @@ struct PairGemm {
     int live_dim;     // PairLive
     int M, N, K;
     int bn;           // columns per tile: a multiple of 32 (128 where B is MN-major), at most 256
-    int splits;       // of K; each split is a unit of its own
+    int tail_kb;      // > 0: the last wave's tiles are split along K (PairTail of that many k-blocks)
     uint32_t idesc;
 };
+
+// Tiles that do not fill a wave of CTA pairs.  `full` tiles run whole; the
+// `rest` (fewer than a wave) are split into `splits` K ranges each, as many as
+// make their waves shortest: ceil(rest splits / pairs) / splits of a tile's
+// time, a range being 8 k-blocks at least and its extra output counted as 1 %.
+// The first range of a tile goes where whole tiles go, the others to buffers
+// of their own ((splits - 1) * rest <= 3 pairs of them).
+struct PairTail {
+    int full, rest, splits;
+    __host__ __device__ PairTail(int tiles, int pairs, int kb) {
+        full = tiles / pairs * pairs;
+        rest = tiles - full;
+        splits = 1;
+        float least = 2.0f;
+        for (int s = 1; s <= 16 && rest > 0; ++s) {
+            if (s > 1 && (s * 8 > kb || s * rest > 3 * pairs)) break;
+            const float cost = (float)((rest * s + pairs - 1) / pairs) / (float)s + 0.01f * (float)s;
+            if (cost < least) {
+                least = cost;
+                splits = s;
+            }
+        }
+        const int per = (kb + splits - 1) / splits;
+        splits = (kb + per - 1) / per;  // no empty range
+    }
+};
+// Position of tile (m, n) in the order in which tiles are walked.
+__host__ __device__ inline int pair_tile_index(int m, int n, int tiles_m, int tiles_n) {
+    const int first = m / kGroupM * kGroupM;
+    const int gm = tiles_m - first < kGroupM ? tiles_m - first : kGroupM;
+    return first * tiles_n + n * gm + (m - first);
+}
 
 // The part of D that an epilogue call covers: this warp's 32 rows, its columns.
 struct PairTile {
@@ -59,18 +91,20 @@ struct PairTile {
     int col0;          // first column of the tile
     int c_begin, c_end;  // this warp's columns within the tile (multiples of 32)
     int n_tile, half;
-    int split;
+    int part;          // 0: the tile's own place; k > 0: buffer k - 1 of the tail
+    int tile_row;      // row0 within the tile
     int M, N;          // live sizes
     uint8_t* staging;  // kPairStaging bytes of this warp alone
     int lane;
 };
 
 struct PairUnit {
-    int m0, n0, n_tile, split, kb0, kb1;
+    int m0, n0, n_tile, part, kb0, kb1;
 };
 
 struct PairShape {
-    int M, K, tiles_m, tiles_n, kb, kb_split, total;
+    int M, K, tiles_m, tiles_n, kb, total;
+    int full, rest, splits;
     __device__ explicit PairShape(const PairGemm& g) {
         M = g.M;
         K = g.K;
@@ -79,14 +113,27 @@ struct PairShape {
         tiles_m = max((M + 255) / 256, 1);
         tiles_n = (g.N + g.bn - 1) / g.bn;
         kb = max((K + 63) / 64, 1);
-        kb_split = (kb + g.splits - 1) / g.splits;
-        total = tiles_m * tiles_n * g.splits;
+        full = tiles_m * tiles_n;
+        rest = 0;
+        splits = 1;
+        if (g.tail_kb > 0) {
+            const PairTail t(full, (int)gridDim.x / 2, g.tail_kb);
+            full = t.full;
+            rest = t.rest;
+            splits = t.splits;
+        }
+        total = full + rest * splits;
     }
     __device__ PairUnit unit(const PairGemm& g, int u) const {
-        const int per = tiles_m * tiles_n;
         PairUnit t;
-        t.split = u / per;
-        const int r = u - t.split * per;
+        int r = u, split = 0, per = kb;
+        t.part = 0;
+        if (u >= full) {
+            split = (u - full) / rest;
+            r = u - split * rest;
+            per = (kb + splits - 1) / splits;
+            t.part = split > 0 ? (split - 1) * rest + (r - full) + 1 : 0;
+        }
         const int grp = r / (kGroupM * tiles_n);
         const int first = grp * kGroupM;
         const int gm = min(kGroupM, tiles_m - first);
@@ -94,8 +141,8 @@ struct PairShape {
         t.n_tile = rr / gm;
         t.m0 = (first + rr - t.n_tile * gm) * 256;
         t.n0 = t.n_tile * g.bn;
-        t.kb0 = t.split * kb_split;
-        t.kb1 = min(t.kb0 + kb_split, kb);
+        t.kb0 = min(split * per, kb);  // a K shorter than the tail's plan leaves its last ranges empty
+        t.kb1 = min(t.kb0 + per, kb);
         return t;
     }
 };
@@ -146,6 +193,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
     cluster_sync();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    pdl_wait();
+    pdl_trigger();
     const PairShape sh(g);
     constexpr int kStep = Epi::kChunk > 0 ? Epi::kChunk : 1 << 30;  // k-blocks per accumulator
 
@@ -244,7 +293,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
             tile.row0 = t.m0 + crank * 128 + q * 32;
             tile.col0 = t.n0;
             tile.n_tile = t.n_tile;
-            tile.split = t.split;
+            tile.part = t.part;
+            tile.tile_row = crank * 128 + q * 32;
             if constexpr (Epi::kChunk > 0) {
                 float acc[128];
 #pragma unroll
@@ -255,7 +305,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
                     release(j);
                 }
                 if (ok) epi.finish(tile, acc);
-            } else {
+            } else if (t.kb0 < t.kb1) {
                 if (!(ok = next(j))) break;
                 epi.tile(tile);
                 release(j++);
@@ -342,16 +392,21 @@ struct PairOut16 {
     }
 };
 
-// Epilogue: D in fp32 into slab[split], stored by the first K range of a sum
-// and added by the later ones.  Each element has one writer per launch, so the
-// order of a sum is the order of the launches.
+// Epilogue: D in fp32, stored by the first K range of a sum over launches and
+// added by the later ones; a tail's further ranges go to `extra`, 256 x 256
+// each.  Each element has one writer per launch, so the order of a sum is the
+// order of the launches.
 struct PairSlab {
     static constexpr int kChunk = 0;
     float* slab;
-    int64_t ld, split_stride;  // ld a multiple of 4
+    int64_t ld;  // a multiple of 4
+    float* extra;
     int first;
     __device__ __forceinline__ void tile(const PairTile& t) const {
-        float* base = slab + (int64_t)t.split * split_stride;
+        float* out = t.part ? extra + (int64_t)(t.part - 1) * 65536 + t.tile_row * 256
+                            : slab + (int64_t)t.row0 * ld + t.col0;
+        const int64_t pitch = t.part ? 256 : ld;
+        const int cols = t.part ? 256 : (int)min((int64_t)256, ld - t.col0);
         for (int c = t.c_begin; c < t.c_end; c += 32) {
             if (t.col0 + c >= t.N || t.row0 >= t.M) break;
             float v[32];
@@ -366,10 +421,10 @@ struct PairSlab {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int r = i * 4 + (t.lane >> 3), k = t.lane & 7;
-                const int gr = t.row0 + r, gc = t.col0 + c + k * 4;
+                const int gc = c + k * 4;
                 float4 x = *reinterpret_cast<const float4*>(t.staging + r * 128 + ((k ^ (r & 7)) * 16));
-                if (gr < t.M && gc < ld) {
-                    float4* o = reinterpret_cast<float4*>(base + (int64_t)gr * ld + gc);
+                if (t.row0 + r < t.M && gc < cols) {
+                    float4* o = reinterpret_cast<float4*>(out + r * pitch + gc);
                     if (!first) {
                         const float4 p = *o;
                         x = make_float4(p.x + x.x, p.y + x.y, p.z + x.z, p.w + x.w);
@@ -390,9 +445,11 @@ struct PairOperand {
     int64_t cols;
 };
 
+inline int pair_count() { return num_sms() / 2; }
+
 template <class Epi, bool A_MN, bool B_MN>
 int pair_gemm_launch(PairOperand A, PairOperand B, int M, int N, int K, const int* live, int live_dim, int bn,
-                     int splits, bool bf16, const Epi& epi, cudaStream_t st) {
+                     int tail_kb, bool bf16, const Epi& epi, cudaStream_t st) {
     DeviceRuntime* rt = nullptr;
     AETH_TRY(runtime_for_current(&rt));
     PairGemm g;
@@ -404,28 +461,14 @@ int pair_gemm_launch(PairOperand A, PairOperand B, int M, int N, int K, const in
     g.N = N;
     g.K = K;
     g.bn = bn;
-    g.splits = splits;
+    g.tail_kb = tail_kb;
     g.idesc = idesc_f16(256, bn, bf16, A_MN, B_MN);
     auto kern = pair_gemm_kernel<Epi, A_MN, B_MN>;
-    static std::atomic<bool> attr_set[kMaxDevices] = {};
-    int dev = 0;
-    AETH_TRY(current_device(&dev));
-    if (!attr_set[dev].load(std::memory_order_acquire)) {
-        AETH_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
-        attr_set[dev].store(true, std::memory_order_release);
-    }
-    const int64_t units = (int64_t)((M + 255) / 256) * ((N + bn - 1) / bn) * splits;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(2 * (unsigned)std::min<int64_t>(units, num_sms() / 2));
-    cfg.blockDim = dim3(kPairThreads);
-    cfg.dynamicSmemBytes = kPairSmem;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim = {2, 1, 1};
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    AETH_CUDA(cudaLaunchKernelEx(&cfg, kern, g, epi, rt->err_word));
+    static std::atomic<bool> allowed[kMaxDevices] = {};
+    AETH_TRY(allow_shared(kern, kPairSmem, allowed));
+    const int64_t units = (int64_t)((M + 255) / 256) * ((N + bn - 1) / bn);
+    const unsigned pairs = (unsigned)(tail_kb > 0 ? pair_count() : std::min<int64_t>(units, pair_count()));
+    AETH_CUDA(launch_after(kern, dim3(2 * pairs), dim3(kPairThreads), kPairSmem, st, 2, g, epi, rt->err_word));
     return AETH_OK;
 }
 

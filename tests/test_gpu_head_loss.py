@@ -296,3 +296,32 @@ def test_offsets_beyond_32_bits():
     e = (U[torch.bfloat16] + 2 * e_s.max().item() + 2.0 ** -18)
     close(dw[-500:], G.T @ h.double(), 1.2 * (e + U[torch.bfloat16]) * ((G.abs() + 1e-6).T @ h.double().abs()))
     close(dh, G @ w[-500:].double(), 1.2 * (e + U[torch.bfloat16] + v * 2.0 ** -23) * ((G.abs() + 1e-6) @ w[-500:].double().abs()))
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("d,v", [(64, 100), (1001, 333), (4104, 5000), (12800, 301)])
+def test_few_tokens(dt, n, d, v):
+    """The forward that reads the weight by rows, and the products beside it."""
+    h, w, lab = make(n, d, v, dt, seed=n + d)
+    check(h, w, lab)
+    import aethelstream_b200 as A
+    from aethelstream_b200 import _lib as L
+    if n > 1:
+        lab[1] = IGNORE
+        bad = h.clone()
+        bad[1] = float("nan")
+        check(bad, w, lab, ref_inputs=(h, w, lab))
+    lab[0] = v
+    L.device_error_bits(0)
+    ce = A.cut_cross_entropy(h, w, lab)
+    assert ce.losses[0].isnan() and ce.loss.isnan() and L.device_error_bits(0) == L.DEVERR_BAD_ARG
+    lab[:] = IGNORE
+    ce = A.cut_cross_entropy(h, w, lab)
+    assert ce.loss.item() == 0 and (ce.losses == 0).all() and (ce.lse == 0).all()
+
+
+@pytest.mark.parametrize("n,d,v", [(300, 2304, 5000), (2000, 2560, 3000), (1100, 8192, 1200), (600, 320, 9000)])
+def test_tail_of_the_hidden_states_product(n, d, v):
+    """Tile counts (of 256 x 256) that leave part of a wave, split along the vocabulary."""
+    check(*make(n, d, v, torch.bfloat16, seed=d, masked=0.1))
