@@ -56,9 +56,13 @@ int head_bn(int64_t tiles_m, int64_t cols) {
     return best;
 }
 
+// Up to this many tokens, taken as N: KHEADSWAP_NOTE
+constexpr int64_t kHeadSwap = 1024;
+
 struct HeadPlan {
     int64_t n_pad, dp, piece, ldg;
-    int bn;      // tile columns of the forward
+    bool live_n;  // tokens as the products' columns (see pair_gemm.cuh)
+    int bn;      // tile columns of the forward otherwise
     int np;      // column ranges of the forward's statistics
     int tail_kb;    // k-blocks of a piece's dH product
     int64_t extra;  // buffers of its tail
@@ -66,8 +70,9 @@ struct HeadPlan {
     HeadPlan(int64_t n, int64_t d, int64_t vocab) {
         n_pad = up(std::max<int64_t>(n, 1), 256);
         dp = up(d, 8);
+        live_n = n <= kHeadSwap;
         bn = head_bn(n_pad / 256, vocab);
-        np = 2 * (int)((vocab + bn - 1) / bn);
+        np = 2 * (int)((vocab + (live_n ? 256 : bn) - 1) / (live_n ? 256 : bn));
         // pieces of equal size (a multiple of the tile) whose G takes at most kHeadGradBytes
         int64_t most = std::max<int64_t>(kHeadGradBytes / (2 * n_pad) / 256 * 256, 256);
         const int64_t count = (vocab + most - 1) / most;
@@ -168,22 +173,34 @@ int head_backward(const HeadPlan& p, const HeadWork& w, const void* weight, int6
         const int64_t vp = std::min(p.piece, vocab - v0);
         const PairOperand H{w.h, p.dp, n, d}, Wp{W + v0 * ld_weight, ld_weight, vp, d};
         const PairOperand G{w.g, p.ldg, n, vp};
-        HeadGrad<BF16> eg{w.lab, w.coef, w.lse2, w.g, p.ldg, (int)n, (int)v0};
-        AETH_TRY((pair_gemm_launch<HeadGrad<BF16>, false, false>(H, Wp, (int)n, (int)vp, (int)d, w.count, PAIR_LIVE_M,
-                                                                 head_bn(p.n_pad / 256, vp), 0, BF16, eg, st)));
+        if (p.live_n) {
+            HeadGradT<BF16> eg{w.lab, w.coef, w.lse2, w.g, p.ldg, (int)n, (int)v0};
+            AETH_TRY((pair_gemm_launch<HeadGradT<BF16>, false, false>(Wp, H, (int)vp, (int)n, (int)d, w.count, PAIR_LIVE_N,
+                                                                      256, 0, BF16, eg, st)));
+        } else {
+            HeadGrad<BF16> eg{w.lab, w.coef, w.lse2, w.g, p.ldg, (int)n, (int)v0};
+            AETH_TRY((pair_gemm_launch<HeadGrad<BF16>, false, false>(H, Wp, (int)n, (int)vp, (int)d, w.count, PAIR_LIVE_M,
+                                                                     head_bn(p.n_pad / 256, vp), 0, BF16, eg, st)));
+        }
         if (d_weight) {
             PairOut16<BF16> ew{static_cast<uint16_t*>(d_weight) + v0 * ld_dw, ld_dw, w.out_scale};
             AETH_TRY((pair_gemm_launch<PairOut16<BF16>, true, true>(G, H, (int)vp, (int)d, (int)n, w.count, PAIR_LIVE_K,
                                                                     256, 0, BF16, ew, st)));
         }
         if (d_hidden) {
-            PairSlab es{w.slab, p.dp, w.extra, v0 == 0};
-            AETH_TRY((pair_gemm_launch<PairSlab, false, true>(G, Wp, (int)n, (int)d, (int)vp, w.count, PAIR_LIVE_M, 256,
-                                                              p.tail_kb, BF16, es, st)));
+            if (p.live_n) {
+                PairSlabT es{w.slab, p.dp, w.extra, v0 == 0};
+                AETH_TRY((pair_gemm_launch<PairSlabT, true, false>(Wp, G, (int)d, (int)n, (int)vp, w.count, PAIR_LIVE_N,
+                                                                   256, p.tail_kb, BF16, es, st)));
+            } else {
+                PairSlab es{w.slab, p.dp, w.extra, v0 == 0};
+                AETH_TRY((pair_gemm_launch<PairSlab, false, true>(G, Wp, (int)n, (int)d, (int)vp, w.count, PAIR_LIVE_M,
+                                                                  256, p.tail_kb, BF16, es, st)));
+            }
         }
     }
     if (d_hidden && n > 0) {
-        const HeadDh a{w.slab, p.dp, w.extra, pair_count(), p.tail_kb, w.pos, w.count, n, (int)d, w.out_scale,
+        const HeadDh a{w.slab, p.dp, w.extra, pair_count(), p.tail_kb, p.live_n, w.pos, w.count, n, (int)d, w.out_scale,
                        static_cast<uint16_t*>(d_hidden), ld_dh};
         const unsigned cols = (unsigned)((d + 1023) / 1024);
         const unsigned rows = (unsigned)std::min<int64_t>(n, std::max<int64_t>(8 * num_sms() / cols, 1));
@@ -340,10 +357,16 @@ int aeth_cut_ce_forward(const void* hidden, int64_t ld_hidden, const void* weigh
     a.lab = w.lab;
     a.count = w.count;
     AETH_TRY(head_rows(a, hidden, ld_hidden, n, d, p, w, st));
-    HeadStats es{w.lab, w.label_logit, w.part, p.n_pad};
-    AETH_TRY((pair_gemm_launch<HeadStats, false, false>({w.h, p.dp, n, d}, {weight, ld_weight, vocab, d}, (int)n,
-                                                        (int)vocab, (int)d, w.count, PAIR_LIVE_M, p.bn, 0,
-                                                        bf16, es, st)));
+    const PairOperand H{w.h, p.dp, n, d}, W{weight, ld_weight, vocab, d};
+    if (p.live_n) {
+        HeadStatsT es{w.lab, w.label_logit, w.part, p.n_pad};
+        AETH_TRY((pair_gemm_launch<HeadStatsT, false, false>(W, H, (int)vocab, (int)n, (int)d, w.count, PAIR_LIVE_N, 256, 0,
+                                                             bf16, es, st)));
+    } else {
+        HeadStats es{w.lab, w.label_logit, w.part, p.n_pad};
+        AETH_TRY((pair_gemm_launch<HeadStats, false, false>(H, W, (int)n, (int)vocab, (int)d, w.count, PAIR_LIVE_M, p.bn, 0,
+                                                            bf16, es, st)));
+    }
     AETH_CUDA(launch_after(head_loss_kernel, dim3((unsigned)std::min<int64_t>((n + 7) / 8, 65536)), dim3(512), 0, st, 1,
                            w.part, p.n_pad, p.np, w.label_logit, w.rows, w.count, losses, lse));
     AETH_CUDA(launch_after(head_mean_kernel, dim3(1), dim3(1024), 0, st, 1, w.pos, n, w.count, losses, lse, loss));

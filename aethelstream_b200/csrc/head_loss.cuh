@@ -174,63 +174,6 @@ __global__ void __launch_bounds__(256) head_pack_kernel(const uint16_t* __restri
     }
 }
 
-// Epilogue of the forward product: per row, over this warp's columns, the
-// largest logit (times log2 e) and the sum of 2^(logit log2 e - that), and the
-// label's logit where it lies here.
-struct HeadStats {
-    const int* lab;
-    float* label_logit;
-    float2* part;  // [2 * n_tile + half][row]
-    int64_t ld_part;
-    static constexpr int kChunk = 8;  // the loss is an fp32 result: see pair_gemm.cuh
-    __device__ __forceinline__ void finish(const PairTile& t, const float (&acc)[128]) const {
-        const int row = t.row0 + t.lane;
-        const bool in = row < t.M;
-        const int at = in ? lab[row] - t.col0 - t.c_begin : -1;
-        float mx = -INFINITY, sum = 0.0f;  // mx in units of log2
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const int left = min(t.c_end, t.N - t.col0) - t.c_begin - 32 * c;  // columns of this chunk that exist
-            if (left > 0) {
-                float m = -INFINITY;
-                if (left >= 32) {
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) m = fmax3(m, acc[32 * c + i], acc[32 * c + i + 1]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (i < left) m = fmaxf(m, acc[32 * c + i]);
-                }
-                const float nm = fmaxf(mx, m * kLog2e);
-                const float off = nm == -INFINITY ? 0.0f : nm;
-                sum *= ex2(mx - off);
-                float s0 = 0.0f, s1 = 0.0f;
-                if (left >= 32) {
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        s0 += ex2(fmaf(acc[32 * c + i], kLog2e, -off));
-                        s1 += ex2(fmaf(acc[32 * c + i + 1], kLog2e, -off));
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (i < left) s0 += ex2(fmaf(acc[32 * c + i], kLog2e, -off));
-                }
-                sum += s0 + s1;
-                mx = nm;
-                const int k = at - 32 * c;
-                if (__any_sync(0xffffffffu, k >= 0 && k < 32)) {
-                    float x = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) x = k == i ? acc[32 * c + i] : x;
-                    if (k >= 0 && k < 32) label_logit[row] = x;
-                }
-            }
-        }
-        if (in) part[(int64_t)(2 * t.n_tile + t.half) * ld_part + row] = make_float2(mx, sum);
-    }
-};
-
 // Joins two (maximum, sum) pairs.
 __device__ __forceinline__ float2 head_join(float2 a, float2 b) {
     const float m = fmaxf(a.x, b.x), off = m == -INFINITY ? 0.0f : m;
@@ -239,6 +182,116 @@ __device__ __forceinline__ float2 head_join(float2 a, float2 b) {
 __device__ __forceinline__ float head_lse(float2 a) {
     return (a.x == -INFINITY ? 0.0f : a.x) * kLn2 + logf(a.y);
 }
+
+// Joins 32 logits (the first `left` of them) to a running maximum, in units of
+// log2, and sum of 2^(logit log2 e - maximum).
+__device__ __forceinline__ void head_stats32(const float (&v)[32], int left, float2& st) {
+    float m = -INFINITY;
+    if (left >= 32) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) m = fmax3(m, v[i], v[i + 1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (i < left) m = fmaxf(m, v[i]);
+    }
+    const float nm = fmaxf(st.x, m * kLog2e);
+    const float off = nm == -INFINITY ? 0.0f : nm;
+    float s0 = 0.0f, s1 = 0.0f;
+    if (left >= 32) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+            s0 += ex2(fmaf(v[i], kLog2e, -off));
+            s1 += ex2(fmaf(v[i + 1], kLog2e, -off));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (i < left) s0 += ex2(fmaf(v[i], kLog2e, -off));
+    }
+    st = make_float2(nm, st.y * ex2(st.x - off) + (s0 + s1));
+}
+// v[k] where some lane's k lies in the 32
+__device__ __forceinline__ void head_label32(const float (&v)[32], int k, float* out) {
+    if (!__any_sync(0xffffffffu, k >= 0 && k < 32)) return;
+    float x = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) x = k == i ? v[i] : x;
+    if (k >= 0 && k < 32) *out = x;
+}
+__device__ __forceinline__ void head_slice(const float (&acc)[128], int c, float (&v)[32]) {  // c known when unrolled
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = acc[32 * c + i];
+}
+
+// Epilogue of the forward product: per row, over this warp's columns, the
+// maximum and sum, and the label's logit where it lies here.
+struct HeadStats {
+    static constexpr int kChunk = 8;  // the loss is an fp32 result: see pair_gemm.cuh
+    const int* lab;
+    float* label_logit;
+    float2* part;  // [2 * n_tile + half][row]
+    int64_t ld_part;
+    __device__ __forceinline__ void finish(const PairTile& t, const float (&acc)[128]) const {
+        const int row = t.row0 + t.lane;
+        const bool in = row < t.M;
+        const int at = in ? lab[row] - t.col0 - t.c_begin : -1;
+        float2 st = make_float2(-INFINITY, 0.0f);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int left = min(t.c_end, t.N - t.col0) - t.c_begin - 32 * c;  // columns of this chunk that exist
+            if (left > 0) {
+                float v[32];
+                head_slice(acc, c, v);
+                head_stats32(v, left, st);
+                head_label32(v, at - 32 * c, label_logit + row);
+            }
+        }
+        if (in) part[(int64_t)(2 * t.n_tile + t.half) * ld_part + row] = st;
+    }
+};
+
+// The same with tokens as the tile's columns (few live rows) and vocabulary
+// entries as its rows: a warp has 32 entries; the four warps of a column half
+// join theirs through shared memory.
+struct HeadStatsT {
+    static constexpr int kChunk = 8;
+    const int* lab;
+    float* label_logit;
+    float2* part;  // [2 * m_tile + CTA of the pair][row]
+    int64_t ld_part;
+    __device__ __forceinline__ void finish(const PairTile& t, const float (&acc)[128]) const {
+        const int left = t.M - t.row0;  // entries of this warp that exist
+        float2 st[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            st[c] = make_float2(-INFINITY, 0.0f);
+            const int token = t.col0 + t.c_begin + 32 * c + t.lane;
+            if (t.c_begin + 32 * c < t.c_end && left > 0) {
+                float v[32];
+                head_slice(acc, c, v);
+                pair_transpose(t, v);
+                head_stats32(v, left, st[c]);
+                const int k = token < t.N ? lab[token] - t.row0 : -1;
+                head_label32(v, k < left ? k : -1, label_logit + token);
+            }
+        }
+        float2* mine = reinterpret_cast<float2*>(t.staging);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) mine[32 * c + t.lane] = st[c];
+        named_bar(1 + t.half, 128);
+        // warp `e` of the half takes its 32 columns c = e
+        const int e = t.warp & 3;
+        const float2* all = reinterpret_cast<const float2*>(t.staging - e * kPairStaging);
+        float2 x = all[32 * e + t.lane];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) x = head_join(x, all[w * (kPairStaging / 8) + 32 * e + t.lane]);
+        const int col = t.c_begin + 32 * e + t.lane;
+        if (col < t.c_end && t.col0 + col < t.N)
+            part[(int64_t)(2 * t.m_tile + (t.tile_row >> 7)) * ld_part + t.col0 + col] = x;
+        named_bar(1 + t.half, 128);
+    }
+};
 
 // Joins the column ranges' maxima and sums.  A CTA takes 8 live rows (lane % 8),
 // its 64 quarter-warps every 64th range, four loads in flight; then a tree.
@@ -511,6 +564,67 @@ struct HeadGrad {
     }
 };
 
+// The same with tokens as the tile's columns: each 32 x 32 block is turned over,
+// so that a thread has a token and 32 entries.
+template <bool BF16>
+struct HeadGradT {
+    static constexpr int kChunk = 0;
+    const int* lab;
+    const float* coef;
+    const float* lse2;
+    uint16_t* g;
+    int64_t ldg;
+    int n;
+    int v0;
+    __device__ __forceinline__ void tile(const PairTile& t) const {
+        const bool whole = (ldg % 8) == 0 && (reinterpret_cast<uintptr_t>(g) & 15) == 0;
+        for (int c = t.c_begin; c < t.c_end; c += 32) {
+            if (t.row0 >= t.M || t.col0 + c >= n) break;
+            float v[32];
+            tmem_ld32<0>(t.tmem + (uint32_t)c, v);
+            tmem_wait_ld();
+            pair_transpose(t, v);
+            const int token = t.col0 + c + t.lane;
+            const bool in = token < t.N;
+            const float f = in ? coef[token] : 0.0f, l2 = in ? lse2[token] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = ex2(fmaf(v[i], kLog2e, -l2));
+            const int k = in ? lab[token] - v0 - t.row0 : -1;
+            if (__any_sync(0xffffffffu, k >= 0 && k < 32)) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = k == i ? v[i] - head_g_scale(BF16) : v[i];
+            }
+            uint32_t w[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = pack16<BF16>(v[2 * i] * f, v[2 * i + 1] * f);
+            // 64 bytes a token; piece p (16 bytes) of token r lies at p ^ (r / 2) % 4
+#pragma unroll
+            for (int p = 0; p < 4; ++p)
+                *reinterpret_cast<uint4*>(t.staging + t.lane * 64 + ((p ^ ((t.lane >> 1) & 3)) * 16)) =
+                    make_uint4(w[4 * p], w[4 * p + 1], w[4 * p + 2], w[4 * p + 3]);
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = i * 8 + (t.lane >> 2), p = t.lane & 3;
+                const int gr = t.col0 + c + r, gc = t.row0 + p * 8;
+                const uint4 x = *reinterpret_cast<const uint4*>(t.staging + r * 64 + ((p ^ ((r >> 1) & 3)) * 16));
+                if (gr < n && gc < t.M) {
+                    uint16_t* o = g + (int64_t)gr * ldg + gc;
+                    if (whole && gc + 8 <= t.M) {
+                        *reinterpret_cast<uint4*>(o) = x;
+                    } else {
+                        const uint32_t xx[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                        for (int q = 0; q < 8; ++q)
+                            if (gc + q < t.M) o[q] = (uint16_t)(xx[q >> 1] >> (16 * (q & 1)));
+                    }
+                }
+            }
+            __syncwarp();
+        }
+    }
+};
+
 // dH of every token in 16 bits: the slab's row, plus the further K ranges of
 // the tail's tiles in their order; zero for the tokens that took no part.  A
 // CTA takes 1024 columns of tokens.
@@ -518,7 +632,7 @@ struct HeadDh {
     const float* slab;
     int64_t ld;
     const float* extra;
-    int pairs, tail_kb;
+    int pairs, tail_kb, live_n;  // live_n: tokens were the product's columns
     const int *pos, *count;
     int64_t n;
     int d;
@@ -528,19 +642,20 @@ struct HeadDh {
 };
 template <bool BF16>
 __global__ void __launch_bounds__(256) head_dh_kernel(const HeadDh a) {
-    __shared__ int sh[4];
+    __shared__ int sh[5];
     pdl_wait();
-    const int tiles_n = (a.d + 255) / 256;
     if (threadIdx.x == 0) {
-        const int tiles_m = max((*a.count + 255) / 256, 1);
-        const PairTail t(tiles_m * tiles_n, a.pairs, a.tail_kb);
-        sh[0] = tiles_m;
-        sh[1] = t.full;
-        sh[2] = t.rest;
-        sh[3] = t.splits;
+        const int count = *a.count, tiles_d = (a.d + 255) / 256;
+        const int bt = a.live_n ? pair_live_bn(count) : 256, tiles_t = max((count + bt - 1) / bt, 1);
+        const PairTail t(tiles_t * tiles_d, a.pairs, a.tail_kb);
+        sh[0] = bt;
+        sh[1] = tiles_t;
+        sh[2] = t.full;
+        sh[3] = t.rest;
+        sh[4] = t.splits;
     }
     __syncthreads();
-    const int tiles_m = sh[0], full = sh[1], rest = sh[2], splits = sh[3];
+    const int bt = sh[0], tiles_t = sh[1], full = sh[2], rest = sh[3], splits = sh[4], tiles_d = (a.d + 255) / 256;
     const float scale = *a.scale;
     const int c = (blockIdx.y * 256 + threadIdx.x) * 4;
     if (c >= a.d) return;
@@ -551,12 +666,13 @@ __global__ void __launch_bounds__(256) head_dh_kernel(const HeadDh a) {
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (p >= 0) {
             v = *reinterpret_cast<const float4*>(a.slab + p * a.ld + c);  // ld is a multiple of 8: whole fours
-            const int i = pair_tile_index(p / 256, c / 256, tiles_m, tiles_n) - full;
+            const int i = (a.live_n ? pair_tile_index(c / 256, p / bt, tiles_d, tiles_t)
+                                    : pair_tile_index(p / bt, c / 256, tiles_t, tiles_d)) - full;
             if (i >= 0) {
 #pragma unroll 4
                 for (int s = 0; s + 1 < splits; ++s) {
                     const float4 e = *reinterpret_cast<const float4*>(
-                        a.extra + ((int64_t)(s * rest + i) * 256 + p % 256) * 256 + c % 256);
+                        a.extra + ((int64_t)(s * rest + i) * 256 + p % bt) * 256 + c % 256);
                     v = make_float4(v.x + e.x, v.y + e.y, v.z + e.z, v.w + e.w);
                 }
             }

@@ -10,15 +10,24 @@
 // CTA then loads 32 KB per k-block of 512 MMA cycles.  Warps: 0 = TMEM
 // allocation + TMA producer, 1 = MMA issuer, 2..9 = epilogue (warp w reads TMEM
 // lane quarter w % 4; warps 2-5 take the first half of the columns, 6-9 the
-// second).
+// second), 10 and 11 = TMA producers too.  Three producers share the k-blocks
+// in turn: one thread's wait, expect and two to four copies take 480 to 640
+// cycles (measured, whatever the copies' sizes), which alone would hold a
+// k-block of 512 MMA cycles at about 720.
 //
 // An epilogue may take the accumulator in pieces of kChunk k-blocks and add
 // them up in registers (Epi::kChunk > 0).  The tensor cores cut every partial
 // sum off toward zero, which shrinks a sum of K products by about K * 1e-9 of
 // itself (measured: 3.8e-6 at K = 4096); pieces of 512 keep that at 4e-7.
 //
-// M or K may be held on the device (`live`): the number of rows that a mask
+// M, N or K may be held on the device (`live`): the number of rows that a mask
 // leaves.  Operand rows past it, up to the next multiple of 256, must be zero.
+//
+// Few live rows are taken as N, not M: M comes in tiles of 256 only, N in
+// multiples of 32, so 311 rows cost two tiles of 160 and not two of 256, and a
+// handful of rows leaves a product bound by the other operand's bytes.  The
+// tile's columns are then the rows of the result, and epilogues turn each
+// 32 x 32 block over in shared memory (pair_transpose).
 // Tiles are walked in groups of kGroupM row tiles so that the tiles in flight
 // share their operands in L2.
 #pragma once
@@ -30,7 +39,8 @@
 namespace aeth {
 
 constexpr int kPairEpiWarps = 8;
-constexpr int kPairThreads = 64 + 32 * kPairEpiWarps;
+constexpr int kPairProducers = 3;  // divides the stages, so each has stages of its own
+constexpr int kPairThreads = 32 * (1 + kPairProducers + kPairEpiWarps);
 constexpr int kPairStages = 6;
 constexpr int kPairOperand = 128 * 64 * 2;                  // one operand of one stage and CTA
 constexpr int kPairStage = 2 * kPairOperand;
@@ -38,19 +48,28 @@ constexpr int kPairStaging = 32 * 128;                      // per epilogue warp
 constexpr int kPairBar = 256;
 constexpr int kPairSmem = 1024 + kPairStages * kPairStage + kPairEpiWarps * kPairStaging + kPairBar;
 constexpr int kGroupM = 8;
+constexpr int kLiveBox = 64;  // rows of B a copy with a live N: the last one brings rows that no MMA reads
 
-enum PairLive { PAIR_LIVE_NONE = 0, PAIR_LIVE_M = 1, PAIR_LIVE_K = 2 };
+enum PairLive { PAIR_LIVE_NONE = 0, PAIR_LIVE_M = 1, PAIR_LIVE_K = 2, PAIR_LIVE_N = 3 };
 
 struct PairGemm {
     CUtensorMap tmA;  // K-major: box 64 (K) x 128; MN-major: box 64 (M) x 64 (K)
-    CUtensorMap tmB;  // K-major: box 64 (K) x bn / 2; MN-major: box 64 (N) x 64 (K)
-    const int* live;  // device count that replaces M or K
+    CUtensorMap tmB;  // K-major: box 64 (K) x bn / 2, or x kLiveBox with a live N; MN-major: box 64 (N) x 64 (K)
+    const int* live;  // device count that replaces M, N or K
     int live_dim;     // PairLive
     int M, N, K;
-    int bn;           // columns per tile: a multiple of 32 (128 where B is MN-major), at most 256
+    int bn;           // columns per tile: a multiple of 32 (128 where B is MN-major), at most 256;
+                      // chosen on the device for a live N
     int tail_kb;      // > 0: the last wave's tiles are split along K (PairTail of that many k-blocks)
-    uint32_t idesc;
+    uint32_t idesc;   // without N
 };
+
+// Tile width for a live N: as few tiles as 256 columns allow, of equal width;
+// together they cover N rounded up to 64 (the k-blocks of a product over them).
+__host__ __device__ inline int pair_live_bn(int n) {
+    const int n64 = (n > 1 ? n + 63 : 64) / 64 * 64, tiles = (n64 + 255) / 256;
+    return ((n64 + tiles - 1) / tiles + 31) / 32 * 32;
+}
 
 // Tiles that do not fill a wave of CTA pairs.  `full` tiles run whole; the
 // `rest` (fewer than a wave) are split into `splits` K ranges each, as many as
@@ -90,12 +109,12 @@ struct PairTile {
     int row0;          // first of the warp's 32 rows of D
     int col0;          // first column of the tile
     int c_begin, c_end;  // this warp's columns within the tile (multiples of 32)
-    int n_tile, half;
+    int m_tile, n_tile, half;
     int part;          // 0: the tile's own place; k > 0: buffer k - 1 of the tail
     int tile_row;      // row0 within the tile
     int M, N;          // live sizes
-    uint8_t* staging;  // kPairStaging bytes of this warp alone
-    int lane;
+    uint8_t* staging;  // kPairStaging bytes of this warp alone, the warps' one after the other
+    int lane, warp;    // warp: of the epilogue's
 };
 
 struct PairUnit {
@@ -103,15 +122,21 @@ struct PairUnit {
 };
 
 struct PairShape {
-    int M, K, tiles_m, tiles_n, kb, total;
+    int M, N, K, bn, tiles_m, tiles_n, kb, total;
     int full, rest, splits;
     __device__ explicit PairShape(const PairGemm& g) {
         M = g.M;
+        N = g.N;
         K = g.K;
+        bn = g.bn;
         if (g.live_dim == PAIR_LIVE_M) M = *g.live;
         if (g.live_dim == PAIR_LIVE_K) K = *g.live;
+        if (g.live_dim == PAIR_LIVE_N) {
+            N = *g.live;
+            bn = pair_live_bn(N);
+        }
         tiles_m = max((M + 255) / 256, 1);
-        tiles_n = (g.N + g.bn - 1) / g.bn;
+        tiles_n = max((N + bn - 1) / bn, 1);
         kb = max((K + 63) / 64, 1);
         full = tiles_m * tiles_n;
         rest = 0;
@@ -124,7 +149,7 @@ struct PairShape {
         }
         total = full + rest * splits;
     }
-    __device__ PairUnit unit(const PairGemm& g, int u) const {
+    __device__ PairUnit unit(int u) const {
         PairUnit t;
         int r = u, split = 0, per = kb;
         t.part = 0;
@@ -140,7 +165,7 @@ struct PairShape {
         const int rr = r - grp * kGroupM * tiles_n;
         t.n_tile = rr / gm;
         t.m0 = (first + rr - t.n_tile * gm) * 256;
-        t.n0 = t.n_tile * g.bn;
+        t.n0 = t.n_tile * bn;
         t.kb0 = min(split * per, kb);  // a K shorter than the tail's plan leaves its last ranges empty
         t.kb1 = min(t.kb0 + per, kb);
         return t;
@@ -176,6 +201,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
     static_assert((2 * kPairStages + 4) * 8 + 8 <= kPairBar, "barriers must fit the barrier area");
+    static_assert(kPairStages % kPairProducers == 0, "every stage has one producer");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int crank = (int)cluster_ctarank();
@@ -198,18 +224,20 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
     const PairShape sh(g);
     constexpr int kStep = Epi::kChunk > 0 ? Epi::kChunk : 1 << 30;  // k-blocks per accumulator
 
-    if (warp == 0) {
-        if (lane == 0) {
-            const int half_n = g.bn / 2;
-            const uint32_t bytes = 2u * (uint32_t)(kPairOperand + half_n * 64 * 2);  // both CTAs
-            int it = 0;
+    if (warp == 0 || warp >= 2 + kPairEpiWarps) {
+        if (elect_one()) {
+            const int me = warp == 0 ? 0 : warp - 1 - kPairEpiWarps;
+            const int half_n = sh.bn / 2;
+            const int rows_b = g.live_dim == PAIR_LIVE_N ? (half_n + kLiveBox - 1) / kLiveBox * kLiveBox : half_n;
+            const uint32_t bytes = 2u * (uint32_t)(kPairOperand + rows_b * 64 * 2);  // both CTAs
+            int s = me, lag = me, issued = 0;  // this producer's next stage; k-blocks until its next turn
+            uint32_t ph = 1;
             for (int u = ustart; u < sh.total && !*abort; u += ustep) {
-                const PairUnit t = sh.unit(g, u);
+                const PairUnit t = sh.unit(u);
                 const int m0 = t.m0 + crank * 128, n0 = t.n0 + crank * half_n;
-                for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
-                    const int s = it % kPairStages;
-                    const uint32_t ph = (uint32_t)(it / kPairStages) & 1u;
-                    if (!mbar_wait(&empty[s], ph ^ 1u, abort, err, DEVERR_TIMEOUT_TMA)) break;
+                int kb = t.kb0 + lag;
+                for (; kb < t.kb1; kb += kPairProducers) {
+                    if (!mbar_wait(&empty[s], ph, abort, err, DEVERR_TIMEOUT_TMA)) break;
                     if (crank == 0) mbar_arrive_expect_tx(&full[s], bytes);
                     uint8_t* a = sA + s * kPairOperand;
                     uint8_t* b = sB + s * kPairOperand;
@@ -222,42 +250,56 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
                     if (B_MN) {
                         for (int c = 0; c < half_n; c += 64)
                             tma_load_2d_pair(b + c * 128, &g.tmB, &full[s], n0 + c, kb * 64);
+                    } else if (g.live_dim == PAIR_LIVE_N) {
+                        for (int c = 0; c < half_n; c += kLiveBox) tma_load_2d_pair(b + c * 128, &g.tmB, &full[s], kb * 64, n0 + c);
                     } else {
                         tma_load_2d_pair(b, &g.tmB, &full[s], kb * 64, n0);
                     }
+                    ++issued;
+                    if ((s += kPairProducers) >= kPairStages) {
+                        s = me;
+                        ph ^= 1u;
+                    }
                 }
+                lag = kb - t.kb1;
             }
             // a wait gave up: the loads in flight get a last, bounded chance to land
             if (*abort && crank == 0)
-                for (int i = max(it - kPairStages, 0); i < it; ++i)
-                    for (int n = 0; n < 1000 && !mbar_try_wait(&full[i % kPairStages], (uint32_t)(i / kPairStages) & 1u); ++n) {}
+                for (int i = max(issued - kPairStages / kPairProducers, 0); i < issued; ++i) {
+                    const int w = me + i % (kPairStages / kPairProducers) * kPairProducers;
+                    const uint32_t p = (uint32_t)(i / (kPairStages / kPairProducers)) & 1u;
+                    for (int n = 0; n < 1000 && !mbar_try_wait(&full[w], p); ++n) {}
+                }
         }
     } else if (warp == 1) {
-        if (lane == 0 && crank == 0) {
-            int it = 0, j = 0;
+        if (crank == 0 && elect_one()) {
+            const uint32_t idesc = g.idesc | ((uint32_t)(sh.bn >> 3) << 17);
+            // descriptors of stage 0; a stage and a step of 16 in K are constants further
+            const uint64_t da0 = sdesc_sw128(smem_u32(sA), A_MN ? 8192 : 16, 1024);
+            const uint64_t db0 = sdesc_sw128(smem_u32(sB), B_MN ? 8192 : 16, 1024);
+            constexpr uint64_t kStepA = (A_MN ? 2048 : 32) / 16, kStepB = (B_MN ? 2048 : 32) / 16;
+            int s = 0, j = 0;
+            uint32_t ph = 0;
             for (int u = ustart; u < sh.total && !*abort; u += ustep) {
-                const PairUnit t = sh.unit(g, u);
+                const PairUnit t = sh.unit(u);
                 for (int kb0 = t.kb0; kb0 < t.kb1 && !*abort; kb0 += kStep, ++j) {
                     const int b = j & 1, kb1 = min(kb0 + kStep, t.kb1);
                     if (!mbar_wait(&acc_empty[b], ((uint32_t)(j >> 1) & 1u) ^ 1u, abort, err, DEVERR_TIMEOUT_MMA)) break;
                     tc_fence_after();
                     const uint32_t d = tmem + (uint32_t)(b * 256);
-                    for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                        const int s = it % kPairStages;
-                        const uint32_t ph = (uint32_t)(it / kPairStages) & 1u;
+                    for (int kb = kb0; kb < kb1; ++kb) {
                         if (!mbar_wait(&full[s], ph, abort, err, DEVERR_TIMEOUT_MMA)) break;
                         tc_fence_after();
-                        const uint32_t a_addr = smem_u32(sA + s * kPairOperand);
-                        const uint32_t b_addr = smem_u32(sB + s * kPairOperand);
-    #pragma unroll
-                        for (int kk = 0; kk < 4; ++kk) {
-                            const uint64_t ad = A_MN ? sdesc_sw128(a_addr + kk * 2048, 8192, 1024)
-                                                     : sdesc_sw128(a_addr + kk * 32, 16, 1024);
-                            const uint64_t bd = B_MN ? sdesc_sw128(b_addr + kk * 2048, 8192, 1024)
-                                                     : sdesc_sw128(b_addr + kk * 32, 16, 1024);
-                            umma_f16_ss_pair(d, ad, bd, g.idesc, (kb > kb0 || kk > 0) ? 1u : 0u);
-                        }
+                        const uint64_t da = da0 + (uint64_t)(s * (kPairOperand / 16));
+                        const uint64_t db = db0 + (uint64_t)(s * (kPairOperand / 16));
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+                            umma_f16_ss_pair(d, da + kk * kStepA, db + kk * kStepB, idesc, (kb > kb0 || kk > 0) ? 1u : 0u);
                         umma_commit_pair(&empty[s]);
+                        if (++s == kPairStages) {
+                            s = 0;
+                            ph ^= 1u;
+                        }
                     }
                     umma_commit_pair(&acc_full[b]);
                 }
@@ -266,15 +308,16 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
     } else {
         const int ew = warp - 2;
         const int q = warp & 3;
-        const int mid = (g.bn / 32 + 1) / 2 * 32;  // columns of the first half: a multiple of 32
+        const int mid = (sh.bn / 32 + 1) / 2 * 32;  // columns of the first half: a multiple of 32
         PairTile tile;
         tile.half = ew >> 2;
         tile.c_begin = tile.half ? mid : 0;
-        tile.c_end = tile.half ? g.bn : mid;
+        tile.c_end = tile.half ? sh.bn : mid;
         tile.M = sh.M;
-        tile.N = g.N;
+        tile.N = sh.N;
         tile.staging = staging + ew * kPairStaging;
         tile.lane = lane;
+        tile.warp = ew;
         auto next = [&](int j) {  // waits for accumulator j
             if (!mbar_wait(&acc_full[j & 1], (uint32_t)(j >> 1) & 1u, abort, err, DEVERR_TIMEOUT_EPI) || *abort) return false;
             tc_fence_after();
@@ -289,9 +332,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
         int j = 0;
         bool ok = true;
         for (int u = ustart; u < sh.total && ok; u += ustep) {
-            const PairUnit t = sh.unit(g, u);
+            const PairUnit t = sh.unit(u);
             tile.row0 = t.m0 + crank * 128 + q * 32;
             tile.col0 = t.n0;
+            tile.m_tile = t.m0 / 256;
             tile.n_tile = t.n_tile;
             tile.part = t.part;
             tile.tile_row = crank * 128 + q * 32;
@@ -319,6 +363,19 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
         tc_fence_after();
         tmem_dealloc_pair(tmem, 512);
     }
+}
+
+// Turns a 32 x 32 block over: in, thread = row, v = its 32 columns; out, thread
+// = column, v = its 32 rows.  Word j of row r lies at j ^ r, so both ways are
+// free of bank conflicts.
+__device__ __forceinline__ void pair_transpose(const PairTile& t, float (&v)[32]) {
+    float* s = reinterpret_cast<float*>(t.staging);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) s[t.lane * 32 + (j ^ t.lane)] = v[j];
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = s[j * 32 + (t.lane ^ j)];
+    __syncwarp();
 }
 
 // Writes 32 columns of the warp's 32 rows (thread = row, v = its values, times
@@ -437,6 +494,35 @@ struct PairSlab {
     }
 };
 
+// The same where the tile's columns are the rows of the result (live N): slab
+// row = column of D.  A tail's further ranges go to `extra`, 256 columns of D
+// by 256 rows each.
+struct PairSlabT {
+    static constexpr int kChunk = 0;
+    float* slab;
+    int64_t ld;  // at least M
+    float* extra;
+    int first;
+    __device__ __forceinline__ void tile(const PairTile& t) const {
+        float* out = t.part ? extra + (int64_t)(t.part - 1) * 65536 : slab + (int64_t)t.col0 * ld + t.row0 - t.tile_row;
+        const int64_t pitch = t.part ? 256 : ld;
+        const bool in = t.row0 + t.lane < t.M;
+        for (int c = t.c_begin; c < t.c_end; c += 32) {
+            if (t.col0 + c >= t.N || t.row0 >= t.M) break;
+            float v[32];
+            tmem_ld32<0>(t.tmem + (uint32_t)c, v);
+            tmem_wait_ld();
+            // a column's 32 rows (the warp's lanes) are 128 bytes of a slab row
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                if (in && t.col0 + c + j < t.N) {
+                    float* o = out + (int64_t)(c + j) * pitch + t.tile_row + t.lane;
+                    *o = first ? v[j] : *o + v[j];
+                }
+        }
+    }
+};
+
 // ---- host ----
 struct PairOperand {
     const void* ptr;
@@ -454,7 +540,9 @@ int pair_gemm_launch(PairOperand A, PairOperand B, int M, int N, int K, const in
     AETH_TRY(runtime_for_current(&rt));
     PairGemm g;
     AETH_TRY(make_tmap_16b(&g.tmA, A.ptr, (uint64_t)A.cols, (uint64_t)A.rows, A.ld, 64, A_MN ? 64 : 128, bf16));
-    AETH_TRY(make_tmap_16b(&g.tmB, B.ptr, (uint64_t)B.cols, (uint64_t)B.rows, B.ld, 64, B_MN ? 64 : bn / 2, bf16));
+    const bool live_n = live_dim == PAIR_LIVE_N;
+    AETH_TRY(make_tmap_16b(&g.tmB, B.ptr, (uint64_t)B.cols, (uint64_t)B.rows, B.ld, 64,
+                           B_MN ? 64 : live_n ? kLiveBox : bn / 2, bf16));
     g.live = live;
     g.live_dim = live_dim;
     g.M = M;
@@ -462,11 +550,11 @@ int pair_gemm_launch(PairOperand A, PairOperand B, int M, int N, int K, const in
     g.K = K;
     g.bn = bn;
     g.tail_kb = tail_kb;
-    g.idesc = idesc_f16(256, bn, bf16, A_MN, B_MN);
+    g.idesc = idesc_f16(256, 0, bf16, A_MN, B_MN);
     auto kern = pair_gemm_kernel<Epi, A_MN, B_MN>;
     static std::atomic<bool> allowed[kMaxDevices] = {};
     AETH_TRY(allow_shared(kern, kPairSmem, allowed));
-    const int64_t units = (int64_t)((M + 255) / 256) * ((N + bn - 1) / bn);
+    const int64_t units = (int64_t)((M + 255) / 256) * (live_n ? (N + 63) / 64 : (N + bn - 1) / bn);
     const unsigned pairs = (unsigned)(tail_kb > 0 ? pair_count() : std::min<int64_t>(units, pair_count()));
     AETH_CUDA(launch_after(kern, dim3(2 * pairs), dim3(kPairThreads), kPairSmem, st, 2, g, epi, rt->err_word));
     return AETH_OK;
