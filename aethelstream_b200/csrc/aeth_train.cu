@@ -36,7 +36,7 @@ struct Carver {
 // Head loss
 // ---------------------------------------------------------------------------
 constexpr int64_t kHeadMaxDim = 1ll << 30;       // token, feature and vocabulary counts (tile coordinates are int)
-constexpr int64_t kHeadGradBytes = 256ll << 20;  // G of one piece
+constexpr int64_t kHeadPieceBytes = 256ll << 20;  // scratch of a vocabulary piece: G, and the buffers of dH's tail
 
 // Columns per tile for a product of `cols` columns (B K-major) with `tiles_m`
 // row tiles: what makes the last wave of tiles over the 74 CTA pairs least
@@ -56,8 +56,17 @@ int head_bn(int64_t tiles_m, int64_t cols) {
     return best;
 }
 
-// Up to this many tokens, taken as N: KHEADSWAP_NOTE
-constexpr int64_t kHeadSwap = 1024;
+// Whether the tokens are the products' columns (pair_gemm.cuh): where tiles of
+// 256 rows would be a tenth larger than the columns that cover the tokens, and
+// masks may leave fewer still.  Measured at d 4096, vocabulary 32000, forward
+// and backward, rows against columns: 16 tokens 70.6 + 187.5 and 65.6 + 180.8
+// us; 300: 101 + 284 and 93 + 259; but 256: 72 + 216 and 75 + 220 (the blocks
+// are turned over in the epilogue), 512: 108 + 325 and 118 + 329.
+bool head_tokens_as_columns(int64_t n) {
+    if (n > 1024) return false;
+    const int64_t bn = pair_live_bn((int)n);
+    return 10 * up(n, 256) >= 11 * ((n + bn - 1) / bn * bn);
+}
 
 struct HeadPlan {
     int64_t n_pad, dp, piece, ldg;
@@ -70,18 +79,28 @@ struct HeadPlan {
     HeadPlan(int64_t n, int64_t d, int64_t vocab) {
         n_pad = up(std::max<int64_t>(n, 1), 256);
         dp = up(d, 8);
-        live_n = n <= kHeadSwap;
+        live_n = head_tokens_as_columns(n);
         bn = head_bn(n_pad / 256, vocab);
         np = 2 * (int)((vocab + (live_n ? 256 : bn) - 1) / (live_n ? 256 : bn));
-        // pieces of equal size (a multiple of the tile) whose G takes at most kHeadGradBytes
-        int64_t most = std::max<int64_t>(kHeadGradBytes / (2 * n_pad) / 256 * 256, 256);
-        const int64_t count = (vocab + most - 1) / most;
-        piece = std::min(up((vocab + count - 1) / count, 256), up(vocab, 8));
+        // buffers that a dH product's tail may need: two waves of tiles at most
+        const int64_t pairs = pair_count(), tiles_m = n_pad / 256;
+        extra = std::min<int64_t>(2 * pairs, 15 * std::min<int64_t>(tiles_m * ((d + 255) / 256), pairs));
+        // a piece is a number of 256-entry tiles whose G fits beside them; of those, from the
+        // largest down to half of it (64 are looked at), the one with the fewest waves of tiles over all pieces
+        const int64_t all = (vocab + 255) / 256;
+        const int64_t most = std::max<int64_t>((kHeadPieceBytes - extra * 262144) / (512 * n_pad), 1);
+        int64_t best = most, least = INT64_MAX;
+        auto waves = [&](int64_t tiles) { return (tiles * tiles_m + pairs - 1) / pairs; };
+        for (int64_t p = most; p >= std::max((most + 1) / 2, most - 64) && most < all; --p) {
+            const int64_t cost = all / p * waves(p) + waves(all % p);
+            if (cost < least) {
+                least = cost;
+                best = p;
+            }
+        }
+        piece = std::min(256 * best, up(vocab, 8));
         ldg = up(piece, 8);
         tail_kb = (int)((piece + 63) / 64);
-        // buffers that a dH product's tail may need: it has at most this many tiles
-        const int64_t tiles = n_pad / 256 * ((d + 255) / 256);
-        extra = std::min<int64_t>(3 * pair_count(), 15 * std::min<int64_t>(tiles, pair_count()));
     }
 };
 

@@ -76,7 +76,7 @@ __host__ __device__ inline int pair_live_bn(int n) {
 // make their waves shortest: ceil(rest splits / pairs) / splits of a tile's
 // time, a range being 8 k-blocks at least and its extra output counted as 1 %.
 // The first range of a tile goes where whole tiles go, the others to buffers
-// of their own ((splits - 1) * rest <= 3 pairs of them).
+// of their own ((splits - 1) * rest <= 2 pairs of them).
 struct PairTail {
     int full, rest, splits;
     __host__ __device__ PairTail(int tiles, int pairs, int kb) {
@@ -85,7 +85,7 @@ struct PairTail {
         splits = 1;
         float least = 2.0f;
         for (int s = 1; s <= 16 && rest > 0; ++s) {
-            if (s > 1 && (s * 8 > kb || s * rest > 3 * pairs)) break;
+            if (s > 1 && (s * 8 > kb || (s - 1) * rest > 2 * pairs)) break;
             const float cost = (float)((rest * s + pairs - 1) / pairs) / (float)s + 0.01f * (float)s;
             if (cost < least) {
                 least = cost;

@@ -81,7 +81,7 @@ def _tma_rows(t: torch.Tensor, d: int) -> tuple[torch.Tensor, int, int]:
     if ld % 8 == 0 and t.data_ptr() % 16 == 0:
         return t, n, ld
     ld = -(-d // 8) * 8
-    out = torch.empty(n, ld, dtype=t.dtype, device=t.device)
+    out = t.new_empty((n, ld))
     out[:, :d] = t.reshape(-1, d)
     return out, n, ld
 
@@ -121,14 +121,16 @@ def cut_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.
     v, d = weight.shape
     h, n, ld_h = _rows(hidden, d)
     w, _, ld_w = _tma_rows(weight, d)
-    out = torch.empty(2 * n + 1, dtype=torch.float32, device=h.device)  # losses, lse, loss: one allocation
-    at = out.data_ptr()
+    losses, lse = (lab.new_empty(labels.shape, dtype=torch.float32) for _ in range(2))
+    loss = lab.new_empty((), dtype=torch.float32)
     size = _workspace_bytes("aeth_cut_ce_workspace", n, d, v, 0)
-    ws = torch.empty(size, dtype=torch.uint8, device=h.device)
-    L.check(_lib.aeth_cut_ce_forward(
-        h.data_ptr(), ld_h, w.data_ptr(), ld_w, _DTYPES[h.dtype], lab.data_ptr(), n, d, v, ignore_index, at,
-        at + 4 * n, at + 8 * n, ws.data_ptr(), size, _raw_stream(h.get_device())), "aeth_cut_ce_forward")
-    return CutCrossEntropy(out[2 * n], out[:n].view(labels.shape), out[n:2 * n].view(labels.shape))
+    ws = lab.new_empty(size, dtype=torch.uint8)
+    st = _lib.aeth_cut_ce_forward(
+        h.data_ptr(), ld_h, w.data_ptr(), ld_w, _DTYPES[h.dtype], lab.data_ptr(), n, d, v, ignore_index,
+        losses.data_ptr(), lse.data_ptr(), loss.data_ptr(), ws.data_ptr(), size, _raw_stream(h.get_device()))
+    if st:
+        L.check(st, "aeth_cut_ce_forward")
+    return CutCrossEntropy(loss, losses, lse)
 
 
 @_on_device
@@ -153,15 +155,16 @@ def cut_cross_entropy_backward(hidden: torch.Tensor, weight: torch.Tensor, label
     w, _, ld_w = _tma_rows(weight, d)
     lse = ce.lse.contiguous()
     grad = None if grad_losses is None else grad_losses.contiguous()
-    dh = torch.empty(hidden.shape, dtype=h.dtype, device=h.device) if need_hidden else None
-    dw = torch.empty(weight.shape, dtype=w.dtype, device=h.device) if need_weight else None
+    dh = h.new_empty(hidden.shape) if need_hidden else None
+    dw = h.new_empty(weight.shape) if need_weight else None
     size = _workspace_bytes("aeth_cut_ce_workspace", n, d, v, 1)
-    ws = torch.empty(size, dtype=torch.uint8, device=h.device)
-    L.check(_lib.aeth_cut_ce_backward(
+    ws = lab.new_empty(size, dtype=torch.uint8)
+    st = _lib.aeth_cut_ce_backward(
         h.data_ptr(), ld_h, w.data_ptr(), ld_w, _DTYPES[h.dtype], lab.data_ptr(), n, d, v, ignore_index,
         lse.data_ptr(), None if grad is None else grad.data_ptr(), scale, dh.data_ptr() if need_hidden else None, d,
-        dw.data_ptr() if need_weight else None, d, ws.data_ptr(), size, _raw_stream(h.get_device())),
-        "aeth_cut_ce_backward")
+        dw.data_ptr() if need_weight else None, d, ws.data_ptr(), size, _raw_stream(h.get_device()))
+    if st:
+        L.check(st, "aeth_cut_ce_backward")
     return dh, dw
 
 
