@@ -132,7 +132,7 @@ struct HeadWork {
         g = nullptr;
         if (!backward) {
             label_logit = c.take<float>(p.n_pad);
-            part = c.take<float2>(std::max<int64_t>((int64_t)p.np * p.n_pad, 2 * num_sms() * kHeadVecTokens));
+            part = c.take<float2>(std::max<int64_t>((int64_t)p.np * p.n_pad, num_sms() * kHeadVecTokens));
         } else {
             coef = c.take<float>(p.n_pad);
             lse2 = c.take<float>(p.n_pad);
@@ -363,7 +363,7 @@ int aeth_cut_ce_forward(const void* hidden, int64_t ld_hidden, const void* weigh
     if (head_vec_fits(n, d)) {
         const HeadVec a{static_cast<const uint16_t*>(hidden), ld_hidden, static_cast<const uint16_t*>(weight), ld_weight,
                         labels, (int)d, (int)vocab, ignore_index, w.label_logit, w.part};
-        const int ctas = (n == 1 ? 2 : 1) * num_sms();
+        const int ctas = num_sms();
         return bf16 ? head_vec<true>(a, n, ctas, losses, lse, loss, st) : head_vec<false>(a, n, ctas, losses, lse, loss, st);
     }
     HeadRows a = {};

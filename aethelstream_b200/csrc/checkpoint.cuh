@@ -162,10 +162,31 @@ __device__ __forceinline__ float ck_code(uint2 q, int i) {
     return (float)(int8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
 }
 
-// gain has a type of its own.
-__device__ __forceinline__ void ck_gain8(const void* gain, int dtype, int c, int d, float (&g)[8]) {
+// Four features of gain, which has a type of its own.  VEC: it starts on 16
+// bytes and d is a multiple of 8.
+template <bool VEC>
+__device__ __forceinline__ float4 ck_gain4(const void* gain, int dtype, int c, int d) {
+    if (VEC) {
+        if (c >= d) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (dtype == AETH_DTYPE_F32) return __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(gain) + c));
+        const uint2 q = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(gain) + c));
+        if (dtype == AETH_DTYPE_BF16)
+            return make_float4(__uint_as_float(q.x << 16), __uint_as_float(q.x & 0xffff0000u), __uint_as_float(q.y << 16),
+                               __uint_as_float(q.y & 0xffff0000u));
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&q.x));
+        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&q.y));
+        return make_float4(a.x, a.y, b.x, b.y);
+    }
+    float g[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) g[i] = c + i < d ? load_as_f32(gain, c + i, dtype) : 0.0f;
+    for (int i = 0; i < 4; ++i) g[i] = c + i < d ? load_as_f32(gain, c + i, dtype) : 0.0f;
+    return make_float4(g[0], g[1], g[2], g[3]);
+}
+template <bool VEC>
+__device__ __forceinline__ void ck_gain8(const void* gain, int dtype, int c, int d, float (&g)[8]) {
+    const float4 a = ck_gain4<VEC>(gain, dtype, c, d), b = ck_gain4<VEC>(gain, dtype, c + 4, d);
+    g[0] = a.x; g[1] = a.y; g[2] = a.z; g[3] = a.w;
+    g[4] = b.x; g[5] = b.y; g[6] = b.z; g[7] = b.w;
 }
 
 // Eight floats of a thread in shared memory, [k][half][thread of the row], so
@@ -173,15 +194,14 @@ __device__ __forceinline__ void ck_gain8(const void* gain, int dtype, int c, int
 __device__ __forceinline__ float4& ck_slot(float4* base, int k, int half) {
     return base[(2 * k + half) * blockDim.x + threadIdx.x];
 }
-template <int VPT>
+template <int VPT, bool VEC>
 __device__ __forceinline__ void ck_gain_to_shared(float4* sg, const void* gain, int dtype, int d) {
     if (threadIdx.y == 0)
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
-            float g[8];
-            ck_gain8(gain, dtype, 8 * (threadIdx.x + k * blockDim.x), d, g);
-            ck_slot(sg, k, 0) = make_float4(g[0], g[1], g[2], g[3]);
-            ck_slot(sg, k, 1) = make_float4(g[4], g[5], g[6], g[7]);
+            const int c = 8 * (threadIdx.x + k * blockDim.x);
+            ck_slot(sg, k, 0) = ck_gain4<VEC>(gain, dtype, c, d);
+            ck_slot(sg, k, 1) = ck_gain4<VEC>(gain, dtype, c + 4, d);
         }
     __syncthreads();
 }
@@ -409,7 +429,7 @@ __global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, sizeof(T) == 2 ? 
     constexpr bool kShared = ck_shared_gain(VPT, WIDE);
     const int nb = (a.d + kCkptBlock - 1) / kCkptBlock;
     const float inv_d = 1.0f / (float)a.d;
-    if (kShared) ck_gain_to_shared<VPT>(ck_dyn, a.gain, a.gain_dtype, a.d);
+    if (kShared) ck_gain_to_shared<VPT, VEC>(ck_dyn, a.gain, a.gain_dtype, a.d);
     int parity = 0;
     for (int64_t t0 = (int64_t)blockIdx.x * blockDim.y; t0 < a.rows; t0 += (int64_t)gridDim.x * blockDim.y, parity ^= 1) {
         const int64_t t = t0 + threadIdx.y;
@@ -452,7 +472,7 @@ __global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, sizeof(T) == 2 ? 
                 ck_opaque(x[k]);
                 ck_unpack(x[k], v);
                 if (kShared) ck_slot8(ck_dyn, k, g);
-                else ck_gain8(a.gain, a.gain_dtype, CK_COLUMN(base, k), a.d, g);
+                else ck_gain8<VEC>(a.gain, a.gain_dtype, CK_COLUMN(base, k), a.d, g);
 #pragma unroll
                 for (int i = 0; i < 8; i += 2) {
                     const float2 y = mul2_rn(mul2_rn(make_float2(v[i], v[i + 1]), make_float2(r, r)),
@@ -493,7 +513,7 @@ __global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, 4))
     constexpr bool kShared = ck_shared_gain(VPT, WIDE);
     const float inv_d = 1.0f / (float)a.d;
     pdl_trigger();
-    if (kShared) ck_gain_to_shared<VPT>(ck_dyn, a.gain, a.gain_dtype, a.d);
+    if (kShared) ck_gain_to_shared<VPT, VEC>(ck_dyn, a.gain, a.gain_dtype, a.d);
     int parity = 0;
     for (int64_t t0 = (int64_t)blockIdx.x * blockDim.y; t0 < a.rows; t0 += (int64_t)gridDim.x * blockDim.y, parity ^= 1) {
         const int64_t t = t0 + threadIdx.y;
@@ -522,7 +542,7 @@ __global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, 4))
                 ck_opaque(q[k]);
                 ck_decode8(q[k], s[k], x);
                 if (kShared) ck_slot8(ck_dyn, k, g);
-                else ck_gain8(a.gain, a.gain_dtype, CK_COLUMN(base, k), a.d, g);
+                else ck_gain8<VEC>(a.gain, a.gain_dtype, CK_COLUMN(base, k), a.d, g);
 #pragma unroll
                 for (int i = 0; i < 8; i += 2) {
                     const float2 y = mul2_rn(mul2_rn(make_float2(x[i], x[i + 1]), make_float2(r, r)),
@@ -650,11 +670,11 @@ __global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, 2))
     if (!WIDE)
 #pragma unroll
         for (int k = 0; k < VPT; ++k) ck_slot(dg, k, 0) = ck_slot(dg, k, 1) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (kShared) ck_gain_to_shared<VPT>(sg, a.in.gain, a.in.gain_dtype, a.in.d);
+    if (kShared) ck_gain_to_shared<VPT, VEC>(sg, a.in.gain, a.in.gain_dtype, a.in.d);
     auto gain_of = [&](int base, int k, uint64_t (&p)[4]) {
         float g[8];
         if (kShared) ck_slot8(sg, k, g);
-        else ck_gain8(a.in.gain, a.in.gain_dtype, CK_COLUMN(base, k), a.in.d, g);
+        else ck_gain8<VEC>(a.in.gain, a.in.gain_dtype, CK_COLUMN(base, k), a.in.d, g);
 #pragma unroll
         for (int i = 0; i < 4; ++i) p[i] = f2(g[2 * i], g[2 * i + 1]);
     };
@@ -788,10 +808,8 @@ __global__ void __launch_bounds__(kRingThreads, 1)
     }
     for (int i = threadIdx.x; i < 2 * VPT * tx; i += blockDim.x) {
         const int c = 8 * (i % tx + i / (2 * tx) * tx) + 4 * (i / tx % 2);
-        float g[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) g[j] = c + j < d ? load_as_f32(a.in.gain, c + j, a.in.gain_dtype) : 0.0f;
-        sg[i] = make_ulonglong2(f2(g[0], g[1]), f2(g[2], g[3]));
+        const float4 g = ck_gain4<true>(a.in.gain, a.in.gain_dtype, c, d);
+        sg[i] = make_ulonglong2(f2(g.x, g.y), f2(g.z, g.w));
     }
     __syncthreads();
     // the group's row j is the CTA's row grp + j * groups, row blockIdx.x + that * gridDim.x of all
