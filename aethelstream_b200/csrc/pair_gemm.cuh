@@ -28,7 +28,7 @@
 // handful of rows leaves a product bound by the other operand's bytes.  The
 // tile's columns are then the rows of the result, and epilogues turn each
 // 32 x 32 block over in shared memory (pair_transpose).
-// Tiles are walked in groups of kGroupM row tiles so that the tiles in flight
+// Tiles are walked in groups of row tiles so that the tiles in flight
 // share their operands in L2.
 #pragma once
 #include <algorithm>
@@ -47,7 +47,12 @@ constexpr int kPairStage = 2 * kPairOperand;
 constexpr int kPairStaging = 32 * 128;                      // per epilogue warp: 32 rows x 128 bytes
 constexpr int kPairBar = 256;
 constexpr int kPairSmem = 1024 + kPairStages * kPairStage + kPairEpiWarps * kPairStaging + kPairBar;
-constexpr int kGroupM = 8;
+// Row tiles of a group.  A group reads all of B once; few row tiles are one
+// group.  Head forward + backward under the power cap, 14 row tiles (3584 x 4096
+// x 32000): one group 665 + 2056 us, groups of 8 687 + 2072, of 4 723 + 2119;
+// 32 row tiles (8192 x 8192 x 32000): of 8 3215 + 9481, of 16 3248 + 9841, of 4
+// 3361 + 9764.
+__host__ __device__ inline int pair_group(int tiles_m) { return tiles_m <= 16 ? tiles_m : 8; }
 constexpr int kLiveBox = 64;  // rows of B a copy with a live N: the last one brings rows that no MMA reads
 
 enum PairLive { PAIR_LIVE_NONE = 0, PAIR_LIVE_M = 1, PAIR_LIVE_K = 2, PAIR_LIVE_N = 3 };
@@ -98,8 +103,8 @@ struct PairTail {
 };
 // Position of tile (m, n) in the order in which tiles are walked.
 __host__ __device__ inline int pair_tile_index(int m, int n, int tiles_m, int tiles_n) {
-    const int first = m / kGroupM * kGroupM;
-    const int gm = tiles_m - first < kGroupM ? tiles_m - first : kGroupM;
+    const int group = pair_group(tiles_m), first = m / group * group;
+    const int gm = tiles_m - first < group ? tiles_m - first : group;
     return first * tiles_n + n * gm + (m - first);
 }
 
@@ -123,7 +128,7 @@ struct PairUnit {
 
 struct PairShape {
     int M, N, K, bn, tiles_m, tiles_n, kb, total;
-    int full, rest, splits;
+    int full, rest, splits, group;
     __device__ explicit PairShape(const PairGemm& g) {
         M = g.M;
         N = g.N;
@@ -138,6 +143,7 @@ struct PairShape {
         tiles_m = max((M + 255) / 256, 1);
         tiles_n = max((N + bn - 1) / bn, 1);
         kb = max((K + 63) / 64, 1);
+        group = pair_group(tiles_m);
         full = tiles_m * tiles_n;
         rest = 0;
         splits = 1;
@@ -159,10 +165,10 @@ struct PairShape {
             per = (kb + splits - 1) / splits;
             t.part = split > 0 ? (split - 1) * rest + (r - full) + 1 : 0;
         }
-        const int grp = r / (kGroupM * tiles_n);
-        const int first = grp * kGroupM;
-        const int gm = min(kGroupM, tiles_m - first);
-        const int rr = r - grp * kGroupM * tiles_n;
+        const int grp = r / (group * tiles_n);
+        const int first = grp * group;
+        const int gm = min(group, tiles_m - first);
+        const int rr = r - grp * group * tiles_n;
         t.n_tile = rr / gm;
         t.m0 = (first + rr - t.n_tile * gm) * 256;
         t.n0 = t.n_tile * bn;
