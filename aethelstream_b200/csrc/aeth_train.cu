@@ -152,7 +152,8 @@ int head_check(const void* hidden, int64_t ld_hidden, const void* weight, int64_
     if (!known_dtype(dtype)) return AETH_ERR_ARG;
     if (!is16(dtype)) return AETH_ERR_UNSUPPORTED;
     if (n > kHeadMaxDim || d > kHeadMaxDim || vocab > kHeadMaxDim) return AETH_ERR_UNSUPPORTED;
-    if ((n + 255) / 256 * ((vocab + 255) / 256) > kHeadMaxDim) return AETH_ERR_UNSUPPORTED;
+    const int64_t tn = (n + 255) / 256, tv = (vocab + 63) / 64, td = (d + 255) / 256;  // tiles of the products
+    if (tn * tv > kHeadMaxDim || tn * td > kHeadMaxDim || tv * td > kHeadMaxDim) return AETH_ERR_UNSUPPORTED;
     if (!aligned16(weight) || ld_weight % 8) return AETH_ERR_UNSUPPORTED;  // TMA reads the weight in place
     return AETH_OK;
 }

@@ -232,12 +232,6 @@ __device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
     return d;
 }
-__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-
 // Scale of a block from its maximum magnitude (NaN where the block held one).
 __device__ __forceinline__ float ck_scale(float amax) {
     if (!(amax <= 3.402823466e38f)) return __int_as_float(0x7fc00000);
@@ -711,7 +705,7 @@ __global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, 2))
         }
         if (!WIDE) read_res(0);  // arrives during the row's sum
         ck_row_sum<2, VPT>(acc, sh, parity, sum);
-        const float r = ck_rstd(sum[0], inv_d, a.in.eps);
+        const float r = t < a.in.rows ? ck_rstd(sum[0], inv_d, a.in.eps) : 0.0f;  // no row: nothing for d_gain, at eps 0 too
         const float f = -(r * r * r * (sum[1] * inv_d));
         CK_SPANS(base, a.in.d) {
             if (WIDE) {
@@ -726,7 +720,13 @@ __global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, 2))
                 ck_opaque(q[k]);
                 ck_opaque(dy[k]);
                 gain_of(base, k, g);
-                if (WIDE) {
+                if (WIDE && VEC) {
+                    const float4 z = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    const float4* o = reinterpret_cast<const float4*>(part + c);
+                    const float4 p0 = c < a.in.d && !first ? o[0] : z, p1 = c < a.in.d && !first ? o[1] : z;
+                    p[0] = p0.x; p[1] = p0.y; p[2] = p0.z; p[3] = p0.w;
+                    p[4] = p1.x; p[5] = p1.y; p[6] = p1.z; p[7] = p1.w;
+                } else if (WIDE) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) p[i] = c + i < a.in.d && !first ? part[c + i] : 0.0f;
                 } else {
@@ -742,7 +742,13 @@ __global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, 2))
                     p[2 * i] = x.x;
                     p[2 * i + 1] = x.y;
                 }
-                if (WIDE) {
+                if (WIDE && VEC) {
+                    if (c < a.in.d) {
+                        float4* o = reinterpret_cast<float4*>(part + c);
+                        o[0] = make_float4(p[0], p[1], p[2], p[3]);
+                        o[1] = make_float4(p[4], p[5], p[6], p[7]);
+                    }
+                } else if (WIDE) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
                         if (c + i < a.in.d) part[c + i] = p[i];
@@ -847,7 +853,11 @@ __global__ void __launch_bounds__(kRingThreads, 1)
     for (; j < mine; ++j) {
         scales_of(j + 1, next);  // a row ahead
         const int64_t t = row0 + j * step;
-        if (!mbar_wait(&full[stage], phase, abort, err, DEVERR_TIMEOUT_TMA)) break;
+        const bool here = mbar_wait(&full[stage], phase, abort, err, DEVERR_TIMEOUT_TMA) && !*abort;
+        if (!__all_sync(0xffffffffu, here)) {
+            if (tx > 32) named_bar_arrive(1 + grp, tx);  // the group may wait for this warp at the row's sum
+            break;
+        }
         const uint8_t* st = stages + (size_t)stage * ring.stage_bytes;
         float acc[2][VPT], sum[2];
 #pragma unroll

@@ -67,7 +67,6 @@ __global__ void __launch_bounds__(1024) head_rows_kernel(HeadRows a, uint32_t* e
     pdl_trigger();
     int base = 0;
     float gmax = 0.0f;
-    bool gnan = false;
     for (int64_t t0 = 0; t0 < a.n; t0 += kItems * 1024) {
         int64_t lab[kItems];
         float lse[kItems], grad[kItems];
@@ -123,8 +122,7 @@ __global__ void __launch_bounds__(1024) head_rows_kernel(HeadRows a, uint32_t* e
                 if (a.grad) {
                     const float g = grad[k] * a.scale;
                     a.coef[i] = g;
-                    gmax = fmaxf(gmax, fabsf(g));
-                    gnan |= g != g;
+                    if (fabsf(g) <= 3.402823466e38f) gmax = fmaxf(gmax, fabsf(g));  // what is not finite stays its token's
                 }
             }
         }
@@ -135,16 +133,17 @@ __global__ void __launch_bounds__(1024) head_rows_kernel(HeadRows a, uint32_t* e
     if (!a.coef) return;
     if (a.grad) {
         gmax = warp_max(gmax);
-        gnan = __any_sync(0xffffffffu, gnan);
-        if (lane == 0) wmax[warp] = gnan ? __int_as_float(0x7fc00000) : gmax;
+        if (lane == 0) wmax[warp] = gmax;
         __syncthreads();
-        gmax = 0.0f;
-        for (int w = 0; w < 32; ++w) gmax = wmax[w] != wmax[w] || gmax != gmax ? __int_as_float(0x7fc00000) : fmaxf(gmax, wmax[w]);
-        for (int i = tid; i < base; i += 1024) a.coef[i] = gmax == 0.0f ? 0.0f : a.coef[i] / gmax;
+        gmax = warp_max(wmax[lane]);
+        for (int i = tid; i < base; i += 1024) {
+            const float g = a.coef[i];
+            a.coef[i] = g == 0.0f ? 0.0f : g / gmax;
+        }
     } else {
         const float g = a.scale / (float)max(base, 1);
         gmax = fabsf(g);
-        for (int i = tid; i < base; i += 1024) a.coef[i] = gmax == 0.0f ? 0.0f : g / gmax;
+        for (int i = tid; i < base; i += 1024) a.coef[i] = g == 0.0f ? 0.0f : g / gmax;
     }
     if (tid == 0) *a.out_scale = gmax / a.g_scale;
 }
@@ -232,6 +231,7 @@ struct HeadStats {
     float* label_logit;
     float2* part;  // [2 * n_tile + half][row]
     int64_t ld_part;
+    __device__ static void give_up(const PairTile&) {}
     __device__ __forceinline__ void finish(const PairTile& t, const float (&acc)[128]) const {
         const int row = t.row0 + t.lane;
         const bool in = row < t.M;
@@ -260,6 +260,10 @@ struct HeadStatsT {
     float* label_logit;
     float2* part;  // [2 * m_tile + CTA of the pair][row]
     int64_t ld_part;
+    __device__ static void give_up(const PairTile& t) {  // the two barriers of finish()
+        named_bar_arrive(1 + t.half, 128);
+        named_bar_arrive(1 + t.half, 128);
+    }
     __device__ __forceinline__ void finish(const PairTile& t, const float (&acc)[128]) const {
         const int left = t.M - t.row0;  // entries of this warp that exist
         float2 st[4];

@@ -15,6 +15,9 @@
 // cycles (measured, whatever the copies' sizes), which alone would hold a
 // k-block of 512 MMA cycles at about 720.
 //
+// Every wait on a barrier is bounded (mbar_wait); an epilogue with barriers of
+// its own says in give_up() how a warp that leaves settles them.
+//
 // An epilogue may take the accumulator in pieces of kChunk k-blocks and add
 // them up in registers (Epi::kChunk > 0).  The tensor cores cut every partial
 // sum off toward zero, which shrinks a sum of K products by about K * 1e-9 of
@@ -325,7 +328,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
         tile.lane = lane;
         tile.warp = ew;
         auto next = [&](int j) {  // waits for accumulator j
-            if (!mbar_wait(&acc_full[j & 1], (uint32_t)(j >> 1) & 1u, abort, err, DEVERR_TIMEOUT_EPI) || *abort) return false;
+            const bool here = mbar_wait(&acc_full[j & 1], (uint32_t)(j >> 1) & 1u, abort, err, DEVERR_TIMEOUT_EPI) && !*abort;
+            if (!__all_sync(0xffffffffu, here)) return false;
             tc_fence_after();
             tile.tmem = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)((j & 1) * 256);
             return true;
@@ -355,6 +359,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
                     release(j);
                 }
                 if (ok) epi.finish(tile, acc);
+                // a warp that gave up arrives where the others may wait for it; they see
+                // `abort` before their next tile
+                else Epi::give_up(tile);
             } else if (t.kb0 < t.kb1) {
                 if (!(ok = next(j))) break;
                 epi.tile(tile);

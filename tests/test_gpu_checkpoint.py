@@ -279,3 +279,17 @@ def test_offsets_beyond_32_bits():
     assert torch.equal(dx[-40:], dx1)
     assert ((dw - dw1).abs() <= 1e-4 * (1 + dw1.abs())).all()
     assert torch.equal(A.checkpoint_decode(ck)[-40:], A.checkpoint_decode(ck1))
+
+
+@pytest.mark.parametrize("rows,d", [(9, 64), (333, 64), (701, 200), (5, 9000)])
+def test_backward_without_eps(rows, d):
+    """eps = 0: rows that a CTA holds past the last one add nothing to d_weight."""
+    import aethelstream_b200 as A
+    x, gain, gen = acts(rows, d, torch.float32, 8)
+    _, ck = A.rms_norm_checkpoint(x, gain, eps=0.0)
+    dy = torch.randn(rows, d, generator=gen, device="cuda")
+    dx, dw = A.rms_norm_checkpoint_backward(dy, ck, gain, eps=0.0)
+    v = values64(ck)
+    want = (dy.double() * v / torch.sqrt((v * v).mean(1, keepdim=True)))
+    close(dw, want.sum(0), want.abs().sum(0) * (d / 16 + 16 + rows) * E + 1e-37)
+    assert dx.isfinite().all()

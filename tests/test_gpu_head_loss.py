@@ -325,3 +325,18 @@ def test_few_tokens(dt, n, d, v):
 def test_tail_of_the_hidden_states_product(n, d, v):
     """Tile counts (of 256 x 256) that leave part of a wave, split along the vocabulary."""
     check(*make(n, d, v, torch.bfloat16, seed=d, masked=0.1))
+
+
+def test_a_token_weight_that_is_not_finite():
+    """It reaches its own token's gradient and d_weight, not the other tokens."""
+    import aethelstream_b200 as A
+    h, w, lab = make(50, 64, 300, torch.bfloat16, seed=14)
+    ce = A.cut_cross_entropy(h, w, lab)
+    grad = torch.rand(50, device="cuda")
+    good, _ = A.cut_cross_entropy_backward(h, w, lab, ce, grad_losses=grad)
+    grad[9] = 0.25 * grad.max()  # not the largest: the others' common factor stays
+    good, _ = A.cut_cross_entropy_backward(h, w, lab, ce, grad_losses=grad)
+    grad[9] = float("nan")
+    dh, dw = A.cut_cross_entropy_backward(h, w, lab, ce, grad_losses=grad)
+    others = torch.arange(50, device="cuda") != 9
+    assert dh[9].isnan().all() and torch.equal(dh[others], good[others]) and dw.isnan().all()
