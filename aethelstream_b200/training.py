@@ -30,6 +30,7 @@ CHECKPOINT_BLOCK = 128  # features that share a scale
 
 _lib = L.load()
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
 @functools.lru_cache(maxsize=4096)
@@ -39,22 +40,13 @@ def _workspace_bytes(fn: str, *dims: int) -> int:
     return size.value
 
 
-def _on_device(f):
-    """Runs f(device index, first tensor, ...) with that device current, so that
-    its allocations, its stream and its launch are the tensors'."""
-    first = f.__code__.co_varnames[0]
-
-    @functools.wraps(f)
-    def run(*args, **kw):
-        t = args[0] if args else kw[first]
-        dev = (t.codes if isinstance(t, ActivationCheckpoint) else t).get_device()
-        if dev < 0:
-            raise ValueError(f"{f.__name__}: device tensors expected")
-        if dev == torch.cuda.current_device():
-            return f(*args, **kw)
-        with torch.cuda.device(dev):
-            return f(*args, **kw)
-    return run
+def _elsewhere(what: str, dev: int, f, *args):
+    """f(*args) with the tensors' device current, so that its allocations, its
+    stream and its launch are theirs."""
+    if dev < 0:
+        raise ValueError(f"{what}: device tensors expected")
+    with torch.cuda.device(dev):
+        return f(*args)
 
 
 def _same_device(what: str, dev: int, *tensors: torch.Tensor | None) -> None:
@@ -108,7 +100,6 @@ def _head_args(what, hidden, weight, labels):
     return labels.to(torch.int64).contiguous()
 
 
-@_on_device
 def cut_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
                       ignore_index: int = -100) -> CutCrossEntropy:
     """Cross entropy of softmax(hidden @ weight.T) against `labels`, the logits
@@ -117,6 +108,9 @@ def cut_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.
     take no part: their loss is 0 and whatever their hidden state holds is not
     read.  A label outside the vocabulary makes its token's loss and the mean
     NaN and sets DEVERR_BAD_ARG in the device error word."""
+    dev = hidden.get_device()
+    if dev < 0 or dev != _current_device():
+        return _elsewhere("cut_cross_entropy", dev, cut_cross_entropy, hidden, weight, labels, ignore_index)
     lab = _head_args("cut_cross_entropy", hidden, weight, labels)
     v, d = weight.shape
     h, n, ld_h = _rows(hidden, d)
@@ -127,13 +121,12 @@ def cut_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.
     ws = lab.new_empty(size, dtype=torch.uint8)
     st = _lib.aeth_cut_ce_forward(
         h.data_ptr(), ld_h, w.data_ptr(), ld_w, _DTYPES[h.dtype], lab.data_ptr(), n, d, v, ignore_index,
-        losses.data_ptr(), lse.data_ptr(), loss.data_ptr(), ws.data_ptr(), size, _raw_stream(h.get_device()))
+        losses.data_ptr(), lse.data_ptr(), loss.data_ptr(), ws.data_ptr(), size, _raw_stream(dev))
     if st:
         L.check(st, "aeth_cut_ce_forward")
     return CutCrossEntropy(loss, losses, lse)
 
 
-@_on_device
 def cut_cross_entropy_backward(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, ce: CutCrossEntropy,
                                grad_losses: torch.Tensor | None = None, scale: float = 1.0, ignore_index: int = -100,
                                need_hidden: bool = True, need_weight: bool = True):
@@ -141,7 +134,10 @@ def cut_cross_entropy_backward(hidden: torch.Tensor, weight: torch.Tensor, label
     where not needed (a frozen head: need_weight=False).  The gradient is that
     of scale * mean loss, or of scale * sum(grad_losses * losses) where
     `grad_losses` (float32, the shape of the labels) is given."""
-    what = "cut_cross_entropy_backward"
+    what, dev = "cut_cross_entropy_backward", hidden.get_device()
+    if dev < 0 or dev != _current_device():
+        return _elsewhere(what, dev, cut_cross_entropy_backward, hidden, weight, labels, ce, grad_losses, scale,
+                          ignore_index, need_hidden, need_weight)
     lab = _head_args(what, hidden, weight, labels)
     v, d = weight.shape
     h, n, ld_h = _rows(hidden, d)
@@ -149,7 +145,7 @@ def cut_cross_entropy_backward(hidden: torch.Tensor, weight: torch.Tensor, label
         raise ValueError(f"{what}: ce must be the result of cut_cross_entropy for these tokens")
     if grad_losses is not None and (grad_losses.dtype != torch.float32 or grad_losses.numel() != n):
         raise ValueError(f"{what}: grad_losses must be float32, one per token")
-    _same_device(what, h.get_device(), ce.lse, grad_losses)
+    _same_device(what, dev, ce.lse, grad_losses)
     if not need_hidden and not need_weight:
         return None, None
     w, _, ld_w = _tma_rows(weight, d)
@@ -162,7 +158,7 @@ def cut_cross_entropy_backward(hidden: torch.Tensor, weight: torch.Tensor, label
     st = _lib.aeth_cut_ce_backward(
         h.data_ptr(), ld_h, w.data_ptr(), ld_w, _DTYPES[h.dtype], lab.data_ptr(), n, d, v, ignore_index,
         lse.data_ptr(), None if grad is None else grad.data_ptr(), scale, dh.data_ptr() if need_hidden else None, d,
-        dw.data_ptr() if need_weight else None, d, ws.data_ptr(), size, _raw_stream(h.get_device()))
+        dw.data_ptr() if need_weight else None, d, ws.data_ptr(), size, _raw_stream(dev))
     if st:
         L.check(st, "aeth_cut_ce_backward")
     return dh, dw
@@ -180,13 +176,15 @@ class ActivationCheckpoint:
 
 
 def _gain(what, gain, d, dev):
-    if gain.dim() != 1 or gain.size(0) != d or gain.dtype not in _DTYPES:
+    dt = _DTYPES.get(gain.dtype)
+    if dt is None or gain.dim() != 1 or gain.size(0) != d:
         raise ValueError(f"{what}: weight must be a float vector of {d} features")
-    _same_device(what, dev, gain)
-    return gain.contiguous(), _DTYPES[gain.dtype]
+    if gain.get_device() != dev:
+        raise ValueError(f"{what}: all tensors must be on cuda:{dev}")
+    return gain.contiguous(), dt
 
 
-def _ckpt_args(what, ckpt):
+def _ckpt_args(what, ckpt, dev):
     """(codes, scales, rows, d) of a checkpoint, contiguous."""
     codes, scales = ckpt.codes, ckpt.scales
     d = codes.size(-1) if codes.dim() else 0
@@ -196,18 +194,20 @@ def _ckpt_args(what, ckpt):
             or scales.size(-1) != blocks or ckpt.dtype not in _DTYPES:
         raise ValueError(f"{what}: an ActivationCheckpoint with int8 codes (..., d) and float32 scales "
                          f"(..., ceil(d / {CHECKPOINT_BLOCK})) expected")
-    _same_device(what, codes.get_device(), scales)
+    if codes.get_device() != dev or scales.get_device() != dev:
+        raise ValueError(f"{what}: all tensors must be on cuda:{dev}")
     return codes.contiguous(), scales.contiguous(), rows, d
 
 
-@_on_device
 def rms_norm_checkpoint(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
                         residual: torch.Tensor | None = None):
     """RMS norm of x (..., d) times `weight`, and x in 8 bits for the second
     pass: (y, checkpoint).  With `residual` the norm's input is x + residual,
     rounded to x's type: (y, checkpoint, sum).  float32, float16 or bfloat16."""
-    what = "rms_norm_checkpoint"
-    dt, dev = _DTYPES.get(x.dtype), x.get_device()
+    what, dev = "rms_norm_checkpoint", x.get_device()
+    if dev < 0 or dev != _current_device():
+        return _elsewhere(what, dev, rms_norm_checkpoint, x, weight, eps, residual)
+    dt = _DTYPES.get(x.dtype)
     d = x.size(-1) if x.dim() else 0
     if dt is None or d == 0:
         raise ValueError(f"{what}: x must be a float tensor (..., d)")
@@ -222,7 +222,8 @@ def rms_norm_checkpoint(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6
         total = torch.empty_like(x, memory_format=torch.contiguous_format)
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
     codes = torch.empty_like(x, dtype=torch.int8, memory_format=torch.contiguous_format)
-    scales = x.new_empty((*x.shape[:-1], -(-d // CHECKPOINT_BLOCK)), dtype=torch.float32)
+    blocks = -(-d // CHECKPOINT_BLOCK)
+    scales = x.new_empty((rows, blocks) if x.dim() == 2 else (*x.shape[:-1], blocks), dtype=torch.float32)
     st = _lib.aeth_rms_norm_checkpoint(
         xr.data_ptr(), ld, None if rr is None else rr.data_ptr(), ld_r, gain.data_ptr(), gain_dt, dt, rows, d, eps,
         None if total is None else total.data_ptr(), y.data_ptr(), codes.data_ptr(), scales.data_ptr(),
@@ -233,14 +234,14 @@ def rms_norm_checkpoint(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6
     return (y, ckpt) if residual is None else (y, ckpt, total)
 
 
-@_on_device
 def checkpoint_decode(ckpt: ActivationCheckpoint, norm_weight: torch.Tensor | None = None,
                       eps: float = 1e-6) -> torch.Tensor:
     """The checkpoint's activations restored to their type; with `norm_weight`
     their RMS norm times it (the second pass's recomputed norm)."""
-    what = "checkpoint_decode"
-    codes, scales, rows, d = _ckpt_args(what, ckpt)
-    dev = codes.get_device()
+    what, dev = "checkpoint_decode", ckpt.codes.get_device()
+    if dev < 0 or dev != _current_device():
+        return _elsewhere(what, dev, checkpoint_decode, ckpt, norm_weight, eps)
+    codes, scales, rows, d = _ckpt_args(what, ckpt, dev)
     gain, gain_dt = (None, 0) if norm_weight is None else _gain(what, norm_weight, d, dev)
     out = torch.empty_like(codes, dtype=ckpt.dtype)
     st = _lib.aeth_checkpoint_decode(codes.data_ptr(), scales.data_ptr(), rows, d,
@@ -251,20 +252,21 @@ def checkpoint_decode(ckpt: ActivationCheckpoint, norm_weight: torch.Tensor | No
     return out
 
 
-@_on_device
 def rms_norm_checkpoint_backward(dy: torch.Tensor, ckpt: ActivationCheckpoint, weight: torch.Tensor, eps: float = 1e-6,
                                  d_residual: torch.Tensor | None = None):
     """(dx, d_weight) of the RMS norm at the restored activations, for the
     gradient dy of its output.  `d_residual`, the gradient that reaches the
     norm's input past it, is added to dx.  dx has dy's type, d_weight is
     float32 (the sum over all rows, in one fixed order)."""
-    what = "rms_norm_checkpoint_backward"
-    codes, scales, rows, d = _ckpt_args(what, ckpt)
-    dev = dy.get_device()
+    what, dev = "rms_norm_checkpoint_backward", dy.get_device()
+    if dev < 0 or dev != _current_device():
+        return _elsewhere(what, dev, rms_norm_checkpoint_backward, dy, ckpt, weight, eps, d_residual)
+    codes, scales, rows, d = _ckpt_args(what, ckpt, dev)
     gain, gain_dt = _gain(what, weight, d, dev)
     if dy.shape != codes.shape or dy.dtype != ckpt.dtype:
         raise ValueError(f"{what}: dy must have the checkpoint's shape and type")
-    _same_device(what, dev, codes, d_residual)
+    if d_residual is not None:
+        _same_device(what, dev, d_residual)
     g, _, ld = _rows(dy, d)
     r, ld_r = None, 0
     if d_residual is not None:
@@ -284,22 +286,21 @@ def rms_norm_checkpoint_backward(dy: torch.Tensor, ckpt: ActivationCheckpoint, w
     return dx, dw
 
 
-@_on_device
 def checkpoint_weight_grad(dy: torch.Tensor, ckpt: ActivationCheckpoint, norm_weight: torch.Tensor | None = None,
                            eps: float = 1e-6) -> torch.Tensor:
     """Weight gradient (m, d) = dy^T X of a linear layer, dy (..., m) the gradient
     of its output, X (..., d) its input: the restored checkpoint, or with
     `norm_weight` its RMS norm times that.  bfloat16 or float16."""
-    what = "checkpoint_weight_grad"
-    codes, scales, rows, d = _ckpt_args(what, ckpt)
-    dev = dy.get_device()
+    what, dev = "checkpoint_weight_grad", dy.get_device()
+    if dev < 0 or dev != _current_device():
+        return _elsewhere(what, dev, checkpoint_weight_grad, dy, ckpt, norm_weight, eps)
+    codes, scales, rows, d = _ckpt_args(what, ckpt, dev)
     gain, gain_dt = (None, 0) if norm_weight is None else _gain(what, norm_weight, d, dev)
     if dy.dtype != ckpt.dtype or dy.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError(f"{what}: dy must be bfloat16 or float16, as the checkpoint")
     m = dy.size(-1) if dy.dim() else 0
     if m == 0 or dy.shape[:-1] != codes.shape[:-1]:
         raise ValueError(f"{what}: dy must be ({', '.join(map(str, codes.shape[:-1]))}, m)")
-    _same_device(what, dev, codes)
     g, _, ld = _tma_rows(dy, m)
     dw = dy.new_empty((m, d))
     size = _workspace_bytes("aeth_checkpoint_weight_grad_workspace", rows, m, d)
