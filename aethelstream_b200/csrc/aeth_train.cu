@@ -110,6 +110,7 @@ bool head_vec_fits(int64_t n, int64_t d) { return n <= kHeadVecTokens && n * up(
 
 struct HeadWork {
     int *rows, *pos, *lab, *count;
+    unsigned* done;
     uint16_t* h;
     // forward
     float* label_logit;
@@ -125,6 +126,7 @@ struct HeadWork {
         pos = c.take<int>(std::max<int64_t>(n, 1));
         lab = c.take<int>(p.n_pad);
         count = c.take<int>(1);
+        done = c.take<unsigned>(1);
         h = c.take<uint16_t>(p.n_pad * p.dp);
         label_logit = nullptr;
         part = nullptr;
@@ -158,14 +160,34 @@ int head_check(const void* hidden, int64_t ld_hidden, const void* weight, int64_
     return AETH_OK;
 }
 
-int head_rows(const HeadRows& a, const void* hidden, int64_t ld, int64_t n, int64_t d, const HeadPlan& p, const HeadWork& w,
-              cudaStream_t st) {
+// Fills in what every call gives, numbers the live tokens and gathers their rows.
+int head_rows(HeadRows a, const int64_t* labels, int64_t n, int64_t d, int64_t vocab, int64_t ignore_index,
+              const void* hidden, int64_t ld, const HeadPlan& p, const HeadWork& w, cudaStream_t st) {
     DeviceRuntime* rt = nullptr;
     AETH_TRY(runtime_for_current(&rt));
-    head_rows_kernel<<<1, 1024, 0, st>>>(a, rt->err_word);
-    AETH_LAUNCH_CHECK();
-    AETH_CUDA(launch_after(head_pack_kernel, dim3((unsigned)std::min<int64_t>(n, 65536)), dim3(256), 0, st, 1,
-                           static_cast<const uint16_t*>(hidden), ld, n, (int)d, w.rows, w.count, w.h, p.dp));
+    a.labels = labels;
+    a.n = n;
+    a.ignore_index = ignore_index;
+    a.vocab = (int)vocab;
+    a.rows = w.rows;
+    a.pos = w.pos;
+    a.lab = w.lab;
+    a.count = w.count;
+    a.done = w.done;
+    a.h = static_cast<const uint16_t*>(hidden);
+    a.ld = ld;
+    a.d = (int)d;
+    a.out = w.h;
+    a.ldo = p.dp;
+    const unsigned ctas = (unsigned)std::min<int64_t>(n, num_sms());
+    if (n <= kHeadScan) {
+        head_rows_kernel<true><<<ctas, 1024, 0, st>>>(a, rt->err_word);
+        AETH_LAUNCH_CHECK();
+    } else {
+        head_rows_kernel<false><<<1, 1024, 0, st>>>(a, rt->err_word);
+        AETH_LAUNCH_CHECK();
+        AETH_CUDA(launch_after(head_pack_kernel, dim3(ctas), dim3(1024), 0, st, 1, a));
+    }
     return AETH_OK;
 }
 
@@ -367,16 +389,7 @@ int aeth_cut_ce_forward(const void* hidden, int64_t ld_hidden, const void* weigh
         const int ctas = num_sms();
         return bf16 ? head_vec<true>(a, n, ctas, losses, lse, loss, st) : head_vec<false>(a, n, ctas, losses, lse, loss, st);
     }
-    HeadRows a = {};
-    a.labels = labels;
-    a.n = n;
-    a.ignore_index = ignore_index;
-    a.vocab = (int)vocab;
-    a.rows = w.rows;
-    a.pos = w.pos;
-    a.lab = w.lab;
-    a.count = w.count;
-    AETH_TRY(head_rows(a, hidden, ld_hidden, n, d, p, w, st));
+    AETH_TRY(head_rows({}, labels, n, d, vocab, ignore_index, hidden, ld_hidden, p, w, st));
     const PairOperand H{w.h, p.dp, n, d}, W{weight, ld_weight, vocab, d};
     if (p.live_n) {
         HeadStatsT es{w.lab, w.label_logit, w.part, p.n_pad};
@@ -387,9 +400,9 @@ int aeth_cut_ce_forward(const void* hidden, int64_t ld_hidden, const void* weigh
         AETH_TRY((pair_gemm_launch<HeadStats, false, false>(H, W, (int)n, (int)vocab, (int)d, w.count, PAIR_LIVE_M, p.bn, 0,
                                                             bf16, es, st)));
     }
-    AETH_CUDA(launch_after(head_loss_kernel, dim3((unsigned)std::min<int64_t>((n + 7) / 8, 65536)), dim3(512), 0, st, 1,
-                           w.part, p.n_pad, p.np, w.label_logit, w.rows, w.count, losses, lse));
-    AETH_CUDA(launch_after(head_mean_kernel, dim3(1), dim3(1024), 0, st, 1, w.pos, n, w.count, losses, lse, loss));
+    const HeadLoss l{w.part, p.n_pad, p.np, w.label_logit, w.rows, w.pos, w.count, w.done, n, losses, lse, loss};
+    AETH_CUDA(launch_after(head_loss_kernel, dim3((unsigned)std::min<int64_t>((n + 7) / 8, 4 * num_sms())), dim3(512), 0, st,
+                           1, l));
     return AETH_OK;
 }
 
@@ -413,14 +426,6 @@ int aeth_cut_ce_backward(const void* hidden, int64_t ld_hidden, const void* weig
     if (workspace_bytes < w.bytes || !aligned16(workspace)) return set_err(AETH_ERR_ARG);
     const bool bf16 = dtype == AETH_DTYPE_BF16;
     HeadRows a = {};
-    a.labels = labels;
-    a.n = n;
-    a.ignore_index = ignore_index;
-    a.vocab = (int)vocab;
-    a.rows = w.rows;
-    a.pos = w.pos;
-    a.lab = w.lab;
-    a.count = w.count;
     a.lse = lse;
     a.grad = grad_losses;
     a.scale = scale;
@@ -429,7 +434,7 @@ int aeth_cut_ce_backward(const void* hidden, int64_t ld_hidden, const void* weig
     a.coef = w.coef;
     a.lse2 = w.lse2;
     a.out_scale = w.out_scale;
-    AETH_TRY(head_rows(a, hidden, ld_hidden, n, d, p, w, st));
+    AETH_TRY(head_rows(a, labels, n, d, vocab, ignore_index, hidden, ld_hidden, p, w, st));
     return bf16 ? head_backward<true>(p, w, weight, ld_weight, n, d, vocab, d_hidden, ld_dh, d_weight, ld_dw, st)
                 : head_backward<false>(p, w, weight, ld_weight, n, d, vocab, d_hidden, ld_dh, d_weight, ld_dw, st);
 }

@@ -46,6 +46,7 @@ struct HeadRows {
     int* pos;    // token -> live row, kHeadIgnored or kHeadBad
     int* lab;    // live row -> label
     int* count;  // live rows
+    unsigned* done;  // zeroed: CTAs of head_loss_kernel that have finished
     // backward only (coef != null)
     const float* lse;   // per token
     const float* grad;  // per token, or null: 1 / count
@@ -53,30 +54,83 @@ struct HeadRows {
     float* coef;       // live row -> g_t / max|g|
     float* lse2;       // live row -> lse * log2(e) - g_bits
     float* out_scale;  // max|g| / g_scale
+    // the live rows of H, gathered to a pitch that TMA takes
+    const uint16_t* h;
+    int64_t ld;
+    int d;
+    uint16_t* out;
+    int64_t ldo;
 };
 
-// One CTA numbers the live tokens in order (a scan over the labels, 8192 at a
-// time, so that their loads are in flight together) and gathers what the
-// epilogues need per live row.
-__global__ void __launch_bounds__(1024) head_rows_kernel(HeadRows a, uint32_t* err) {
-    constexpr int kItems = 8;
+// Copies rows of H (row r of the caller's list from `from(r)` to `to(r)`, zeros
+// where from(r) < 0) with all threads of the CTA, four loads in flight.
+template <typename From, typename To>
+__device__ __forceinline__ void head_copy_rows(const HeadRows& a, int64_t nrows, From from, To to) {
+    const bool whole = (a.ld % 8) == 0 && (a.d % 8) == 0 && (reinterpret_cast<uintptr_t>(a.h) & 15) == 0;
+    if (whole) {
+        const int nv = a.d / 8;
+        for (int64_t i0 = threadIdx.x; i0 < nrows * nv; i0 += 4 * blockDim.x) {
+            uint4 v[4];
+            uint4* o[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int64_t i = i0 + (int64_t)k * blockDim.x;
+                o[k] = nullptr;
+                if (i < nrows * nv) {
+                    const int64_t r = i / nv;
+                    const int c = (int)(i - r * nv);
+                    const int64_t src = from(r), dst = to(r);
+                    v[k] = src >= 0 ? __ldg(reinterpret_cast<const uint4*>(a.h + src * a.ld) + c) : make_uint4(0, 0, 0, 0);
+                    if (dst >= 0) o[k] = reinterpret_cast<uint4*>(a.out + dst * a.ldo) + c;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (o[k]) *o[k] = v[k];
+        }
+    } else {
+        for (int64_t i = threadIdx.x; i < nrows * a.d; i += blockDim.x) {
+            const int64_t r = i / a.d, src = from(r), dst = to(r);
+            const int c = (int)(i - r * a.d);
+            if (dst >= 0) a.out[dst * a.ldo + c] = src >= 0 ? a.h[src * a.ld + c] : (uint16_t)0;
+        }
+    }
+}
+// The products' last tiles read rows from the count up to the next multiple of
+// 256: they are zero (past row n TMA itself fills with zero, without reading).
+__device__ __forceinline__ int64_t head_padded(int live, int64_t n) {
+    return min((int64_t)max((live + 255) / 256 * 256, 256), n);
+}
+
+// Numbers the live tokens in order (a scan over the labels, 8192 at a time, so
+// that their loads are in flight together) and gathers what the epilogues need
+// per live row.  CTA 0 writes that.  PACK (up to 8192 tokens): every CTA makes
+// the scan for itself and then gathers its share of H's rows; more tokens take
+// one CTA and head_pack_kernel behind it.
+constexpr int kHeadScan = 8192;
+template <bool PACK>
+__global__ void __launch_bounds__(1024) head_rows_kernel(const __grid_constant__ HeadRows a, uint32_t* err) {
+    constexpr int kItems = kHeadScan / 1024;
     __shared__ int wsum[kItems * 32];
     __shared__ float wmax[32];
     __shared__ int base_s;
+    __shared__ int spos[PACK ? kHeadScan : 1];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const bool writes = blockIdx.x == 0;
     pdl_trigger();
     int base = 0;
     float gmax = 0.0f;
-    for (int64_t t0 = 0; t0 < a.n; t0 += kItems * 1024) {
+    for (int64_t t0 = 0; t0 < a.n; t0 += kHeadScan) {
         int64_t lab[kItems];
         float lse[kItems], grad[kItems];
         uint32_t m[kItems];
+        const bool per_row = writes && a.coef;
 #pragma unroll
         for (int k = 0; k < kItems; ++k) {
             const int64_t t = t0 + k * 1024 + tid;
             lab[k] = t < a.n ? a.labels[t] : a.ignore_index;
-            lse[k] = a.coef && t < a.n ? a.lse[t] : 0.0f;
-            grad[k] = a.coef && a.grad && t < a.n ? a.grad[t] : 0.0f;
+            lse[k] = per_row && t < a.n ? a.lse[t] : 0.0f;
+            grad[k] = per_row && a.grad && t < a.n ? a.grad[t] : 0.0f;
         }
 #pragma unroll
         for (int k = 0; k < kItems; ++k) {
@@ -107,13 +161,16 @@ __global__ void __launch_bounds__(1024) head_rows_kernel(HeadRows a, uint32_t* e
         for (int k = 0; k < kItems; ++k) {
             const int64_t t = t0 + k * 1024 + tid;
             if (t >= a.n) continue;
-            if (!((m[k] >> lane) & 1u)) {
+            const bool live = (m[k] >> lane) & 1u;
+            const int i = base + wsum[k * 32 + warp] + __popc(m[k] & ((1u << lane) - 1));
+            if (PACK) spos[k * 1024 + tid] = live ? i : kHeadIgnored;
+            if (!writes) continue;
+            if (!live) {
                 const bool bad = lab[k] != a.ignore_index;
                 if (bad) report_dev_error(err, DEVERR_BAD_ARG);
                 a.pos[t] = bad ? kHeadBad : kHeadIgnored;
                 continue;
             }
-            const int i = base + wsum[k * 32 + warp] + __popc(m[k] & ((1u << lane) - 1));
             a.pos[t] = i;
             a.rows[i] = (int)t;
             a.lab[i] = (int)lab[k];
@@ -129,7 +186,20 @@ __global__ void __launch_bounds__(1024) head_rows_kernel(HeadRows a, uint32_t* e
         base += base_s;
         __syncthreads();
     }
-    if (tid == 0) *a.count = base;
+    if (PACK) {
+        const int64_t g = gridDim.x, b = blockIdx.x, first = base + b;
+        head_copy_rows(a, (a.n - b + g - 1) / g, [&](int64_t r) { return b + r * g; },
+                       [&](int64_t r) { return (int64_t)spos[b + r * g]; });
+        const int64_t padded = head_padded(base, a.n);
+        if (first < padded)
+            head_copy_rows(a, (padded - first + g - 1) / g, [](int64_t) { return (int64_t)-1; },
+                           [&](int64_t r) { return first + r * g; });
+    }
+    if (!writes) return;
+    if (tid == 0) {
+        *a.count = base;
+        *a.done = 0;
+    }
     if (!a.coef) return;
     if (a.grad) {
         gmax = warp_max(gmax);
@@ -148,29 +218,16 @@ __global__ void __launch_bounds__(1024) head_rows_kernel(HeadRows a, uint32_t* e
     if (tid == 0) *a.out_scale = gmax / a.g_scale;
 }
 
-// Live rows of H, gathered to a pitch that TMA takes; rows from the count up
-// to the next multiple of 256 are zero (the products' last tiles read them;
-// past row n TMA itself fills with zero, without reading).
-__global__ void __launch_bounds__(256) head_pack_kernel(const uint16_t* __restrict__ h, int64_t ld, int64_t n, int d,
-                                                        const int* rows, const int* count,
-                                                        uint16_t* __restrict__ out, int64_t ldo) {
+// The gathering alone, after the scan (more than kHeadScan tokens).
+__global__ void __launch_bounds__(1024) head_pack_kernel(const __grid_constant__ HeadRows a) {
     pdl_wait();
     pdl_trigger();
-    const int live = *count;
-    const int64_t padded = min((int64_t)max((live + 255) / 256 * 256, 256), n);
-    const bool whole = (ld % 8) == 0 && (d % 8) == 0 && (reinterpret_cast<uintptr_t>(h) & 15) == 0;
-    for (int64_t i = blockIdx.x; i < padded; i += gridDim.x) {
-        const uint16_t* src = h + (i < live ? (int64_t)rows[i] * ld : 0);
-        uint16_t* dst = out + i * ldo;
-        if (i >= live) {
-            for (int c = threadIdx.x; c < d; c += blockDim.x) dst[c] = 0;
-        } else if (whole) {
-            for (int c = threadIdx.x; c < d / 8; c += blockDim.x)
-                reinterpret_cast<uint4*>(dst)[c] = reinterpret_cast<const uint4*>(src)[c];
-        } else {
-            for (int c = threadIdx.x; c < d; c += blockDim.x) dst[c] = src[c];
-        }
-    }
+    const int live = *a.count;
+    const int64_t padded = head_padded(live, a.n), g = gridDim.x, b = blockIdx.x;
+    if (b < padded)
+        head_copy_rows(a, (padded - b + g - 1) / g,
+                       [&](int64_t r) { return b + r * g < live ? (int64_t)a.rows[b + r * g] : -1; },
+                       [&](int64_t r) { return b + r * g; });
 }
 
 // Joins two (maximum, sum) pairs.
@@ -299,22 +356,35 @@ struct HeadStatsT {
 
 // Joins the column ranges' maxima and sums.  A CTA takes 8 live rows (lane % 8),
 // its 64 quarter-warps every 64th range, four loads in flight; then a tree.
-__global__ void __launch_bounds__(512) head_loss_kernel(const float2* part, int64_t ld_part, int np,
-                                                        const float* label_logit, const int* rows, const int* count,
-                                                        float* losses, float* lse) {
+// The CTA that finishes last settles the tokens that take no part (loss 0; NaN
+// for a label outside the vocabulary) and the mean over the live ones, summed
+// in one fixed order.
+struct HeadLoss {
+    const float2* part;
+    int64_t ld_part;
+    int np;
+    const float* label_logit;
+    const int *rows, *pos, *count;
+    unsigned* done;
+    int64_t n;
+    float *losses, *lse, *loss;
+};
+__global__ void __launch_bounds__(512) head_loss_kernel(const HeadLoss a) {
     __shared__ float2 sh[16][8];
+    __shared__ double ws[16];
+    __shared__ bool last;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_wait();
-    pdl_trigger();
-    const int live = *count;
+    const int live = *a.count;
     for (int64_t r0 = (int64_t)blockIdx.x * 8; r0 < live; r0 += (int64_t)gridDim.x * 8) {
         const int64_t row = r0 + (lane & 7);
         float2 x = make_float2(-INFINITY, 0.0f);
-        for (int p0 = warp * 4 + (lane >> 3); p0 < np; p0 += 256) {
+        for (int p0 = warp * 4 + (lane >> 3); p0 < a.np; p0 += 256) {
             float2 v[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                v[k] = p0 + 64 * k < np && row < live ? part[(p0 + 64 * k) * ld_part + row] : make_float2(-INFINITY, 0.0f);
+                v[k] = p0 + 64 * k < a.np && row < live ? a.part[(p0 + 64 * k) * a.ld_part + row]
+                                                        : make_float2(-INFINITY, 0.0f);
             x = head_join(x, head_join(head_join(v[0], v[1]), head_join(v[2], v[3])));
         }
 #pragma unroll
@@ -331,37 +401,36 @@ __global__ void __launch_bounds__(512) head_loss_kernel(const float2* part, int6
                 x = head_join(x, make_float2(__shfl_xor_sync(0xffffffffu, x.x, o), __shfl_xor_sync(0xffffffffu, x.y, o)));
             if (lane < 8 && row < live) {
                 const float l = head_lse(x);
-                const int t = rows[row];
-                lse[t] = l;
-                losses[t] = l - label_logit[row];
+                const int t = a.rows[row];
+                a.lse[t] = l;
+                a.losses[t] = l - a.label_logit[row];
             }
         }
         __syncthreads();
     }
-}
-
-// Losses of the tokens that take no part (0; NaN for a label outside the
-// vocabulary) and the mean over the live ones, summed in one fixed order.
-__global__ void __launch_bounds__(1024) head_mean_kernel(const int* pos, int64_t n, const int* count, float* losses,
-                                                         float* lse, float* loss) {
-    __shared__ double ws[32];
-    pdl_wait();
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) last = atomicAdd(a.done, 1u) == gridDim.x - 1;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
     double s = 0.0;
-    for (int64_t t = threadIdx.x; t < n; t += 1024) {
-        const int p = pos[t];
+    for (int64_t t = threadIdx.x; t < a.n; t += 512) {
+        const int p = a.pos[t];
         if (p < 0) {
-            losses[t] = lse[t] = p == kHeadBad ? __int_as_float(0x7fc00000) : 0.0f;
-            if (p == kHeadBad) s += (double)__int_as_float(0x7fc00000);
+            const float v = p == kHeadBad ? __int_as_float(0x7fc00000) : 0.0f;
+            a.losses[t] = a.lse[t] = v;
+            s += (double)v;
         } else {
-            s += (double)losses[t];
+            s += (double)__ldcg(a.losses + t);
         }
     }
     s = warp_sum_d(s);
-    if ((threadIdx.x & 31) == 0) ws[threadIdx.x >> 5] = s;
+    if (lane == 0) ws[warp] = s;
     __syncthreads();
     if (threadIdx.x < 32) {
-        s = warp_sum_d(ws[threadIdx.x]);
-        if (threadIdx.x == 0) *loss = (float)(s / (double)max(*count, 1));
+        s = warp_sum_d(threadIdx.x < 16 ? ws[threadIdx.x] : 0.0);
+        if (threadIdx.x == 0) *a.loss = (float)(s / (double)max(live, 1));
     }
 }
 

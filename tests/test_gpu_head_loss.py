@@ -340,3 +340,9 @@ def test_a_token_weight_that_is_not_finite():
     dh, dw = A.cut_cross_entropy_backward(h, w, lab, ce, grad_losses=grad)
     others = torch.arange(50, device="cuda") != 9
     assert dh[9].isnan().all() and torch.equal(dh[others], good[others]) and dw.isnan().all()
+
+
+@pytest.mark.parametrize("n", [8191, 8192, 8193, 20000])
+def test_many_tokens(n):
+    """Around the number of labels that one scan takes."""
+    check(*make(n, 64, 300, torch.bfloat16, seed=15, masked=0.3))
