@@ -1,6 +1,7 @@
 // aeth_galore.cu -- libaeth_galore: the C ABI of include/aeth_galore.h.
 //
-// One translation unit (the kernels live in the included .cuh files) so the
+// The translation unit of the optimizer step (its kernels live in the included
+// .cuh files; aeth_train.cu is the other one), so the
 // __constant__ tables exist once per library.  Reference paths are relative
 // to the reference project's aethelStream/ directory.
 #include <math.h>
