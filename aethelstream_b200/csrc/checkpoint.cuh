@@ -415,6 +415,9 @@ __device__ __forceinline__ void ckpt_input(const CkptStore<T>& a, int64_t t, int
 // Whether gain is kept in shared memory (dynamic, 4 bytes a feature)
 constexpr bool ck_shared_gain(int vpt, bool wide) { return vpt == 4 && !wide; }
 
+// Bound by its writes: 8192 x 8192 bf16 with residual 107 us, 5.7 TB/s in all and
+// 3.2 TB/s written, where a copy writes 3.3.  Five of nine bytes an element are
+// written (sum, y, code).
 template <typename T, int VPT, bool VEC, bool WIDE>
 __global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, sizeof(T) == 2 ? 4 : 3))
     ckpt_store_kernel(const __grid_constant__ CkptStore<T> a) {
@@ -498,7 +501,8 @@ __device__ __forceinline__ void ck_restore8(const CkptRead& a, int64_t t, int c,
     s = c < d ? __ldg(a.scales + t * nb + c / kCkptBlock) : 0.0f;
 }
 
-// The norm of x^, in rows of pitch ldo.
+// The norm of x^, in rows of pitch ldo.  8192 x 8192 to bf16: 46 us (writing
+// alone takes 41).
 template <typename T, int VPT, bool VEC, bool WIDE>
 __global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, 4))
     ckpt_norm_kernel(const __grid_constant__ CkptRead a, T* __restrict__ out, int64_t ldo) {
@@ -551,7 +555,8 @@ __global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, 4))
 }
 
 // x^ of a whole checkpoint whose rows are whole blocks and lie one after the
-// other: sixteen codes (one load) at a time, four in flight.
+// other: sixteen codes (one load) at a time, four in flight.  8192 x 8192 to
+// bf16: 42 us, 3.2 TB/s written: the write rate bounds it.
 template <typename T>
 __global__ void __launch_bounds__(256) ckpt_decode_flat_kernel(const uint4* __restrict__ codes,
                                                                const float* __restrict__ scales, int64_t n16,
@@ -784,7 +789,10 @@ __global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, 2))
 // takes every n-th row of the CTA through a ring of its own: when all its warps
 // have reached a row's sum, the row before it is done with and its stage is
 // filled again.  A thread's d_gain sums stay in registers; at the end the
-// groups' are added in their order.
+// groups' are added in their order.  8192 x 8192 bf16 with the residual's
+// gradient: 94 us with the sum over the CTAs, 5.0 TB/s (rows through registers
+// instead: 133).  Sixteen warps an SM issue 55 % of the time; what is left is the
+// wait between a row's two passes.
 struct CkptRing {
     int tx, groups, stages;  // stages a group
     int stage_bytes, res_at, codes_at;  // dy first

@@ -23,6 +23,10 @@
 // sum off toward zero, which shrinks a sum of K products by about K * 1e-9 of
 // itself (measured: 3.8e-6 at K = 4096); pieces of 512 keep that at 4e-7.
 //
+// Measured, 3584 x 4096 x 32000 bf16: 561-591 us a product (1.59-1.68 PF/s at the
+// 1.5 GHz that the power cap leaves), tensor pipe 97-98 % active: the clock
+// bounds it.  With the issuer and one producer behind `lane == 0` 688 us, 71 %.
+//
 // M, N or K may be held on the device (`live`): the number of rows that a mask
 // leaves.  Operand rows past it, up to the next multiple of 256, must be zero.
 //
