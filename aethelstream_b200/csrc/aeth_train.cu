@@ -245,8 +245,8 @@ int head_backward(const HeadPlan& p, const HeadWork& w, const void* weight, int6
         const HeadDh a{w.slab, p.dp, w.extra, pair_count(), p.tail_kb, p.live_n, w.pos, w.count, n, (int)d, w.out_scale,
                        static_cast<uint16_t*>(d_hidden), ld_dh};
         const unsigned cols = (unsigned)((d + 1023) / 1024);
-        const unsigned rows = (unsigned)std::min<int64_t>(n, std::max<int64_t>(8 * num_sms() / cols, 1));
-        AETH_CUDA(launch_after(head_dh_kernel<BF16>, dim3(rows, cols), dim3(256), 0, st, 1, a));
+        const unsigned rows = (unsigned)std::min<int64_t>((n + 3) / 4, std::max<int64_t>(16 * num_sms() / cols, 1));
+        AETH_CUDA(launch_after(head_dh_kernel<BF16>, dim3(rows, cols), dim3(128), 0, st, 1, a));
     }
     return AETH_OK;
 }

@@ -715,7 +715,7 @@ struct HeadGradT {
 
 // dH of every token in 16 bits: the slab's row, plus the further K ranges of
 // the tail's tiles in their order; zero for the tokens that took no part.  A
-// CTA takes 1024 columns of tokens.
+// CTA takes 1024 columns of tokens, four of them in flight.
 struct HeadDh {
     const float* slab;
     int64_t ld;
@@ -729,7 +729,7 @@ struct HeadDh {
     int64_t ldo;
 };
 template <bool BF16>
-__global__ void __launch_bounds__(256) head_dh_kernel(const HeadDh a) {
+__global__ void __launch_bounds__(128) head_dh_kernel(const HeadDh a) {
     __shared__ int sh[5];
     pdl_wait();
     if (threadIdx.x == 0) {
@@ -745,37 +745,54 @@ __global__ void __launch_bounds__(256) head_dh_kernel(const HeadDh a) {
     __syncthreads();
     const int bt = sh[0], tiles_t = sh[1], full = sh[2], rest = sh[3], splits = sh[4], tiles_d = (a.d + 255) / 256;
     const float scale = *a.scale;
-    const int c = (blockIdx.y * 256 + threadIdx.x) * 4;
+    const int c = (blockIdx.y * 128 + threadIdx.x) * 8;
     if (c >= a.d) return;
-    const bool whole = (a.ldo % 4) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 7) == 0 && c + 4 <= a.d;
-#pragma unroll 2
-    for (int64_t t = blockIdx.x; t < a.n; t += gridDim.x) {
-        const int p = a.pos[t];
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (p >= 0) {
-            v = *reinterpret_cast<const float4*>(a.slab + p * a.ld + c);  // ld is a multiple of 8: whole fours
-            const int i = (a.live_n ? pair_tile_index(c / 256, p / bt, tiles_d, tiles_t)
-                                    : pair_tile_index(p / bt, c / 256, tiles_t, tiles_d)) - full;
-            if (i >= 0) {
+    const bool whole = (a.ldo % 8) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && c + 8 <= a.d;
+    for (int64_t t0 = blockIdx.x; t0 < a.n; t0 += 4 * (int64_t)gridDim.x) {
+        float4 v[4][2];
+        int p[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int64_t t = t0 + (int64_t)k * gridDim.x;
+            p[k] = t < a.n ? a.pos[t] : kHeadIgnored;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)  // ld is a multiple of 8
+                v[k][h] = p[k] >= 0 ? *reinterpret_cast<const float4*>(a.slab + p[k] * a.ld + c + 4 * h)
+                                    : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int64_t t = t0 + (int64_t)k * gridDim.x;
+            if (t >= a.n) break;
+            if (p[k] >= 0) {
+                const int i = (a.live_n ? pair_tile_index(c / 256, p[k] / bt, tiles_d, tiles_t)
+                                        : pair_tile_index(p[k] / bt, c / 256, tiles_t, tiles_d)) - full;
+                if (i >= 0) {
+                    const float* e = a.extra + ((int64_t)i * 256 + p[k] % bt) * 256 + c % 256;
 #pragma unroll 4
-                for (int s = 0; s + 1 < splits; ++s) {
-                    const float4 e = *reinterpret_cast<const float4*>(
-                        a.extra + ((int64_t)(s * rest + i) * 256 + p % bt) * 256 + c % 256);
-                    v = make_float4(v.x + e.x, v.y + e.y, v.z + e.z, v.w + e.w);
+                    for (int s = 0; s + 1 < splits; ++s)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float4 x = *reinterpret_cast<const float4*>(e + (int64_t)s * rest * 65536 + 4 * h);
+                            v[k][h] = make_float4(v[k][h].x + x.x, v[k][h].y + x.y, v[k][h].z + x.z, v[k][h].w + x.w);
+                        }
                 }
             }
-        }
-        const bool live = p >= 0;
-        const uint32_t lo = live ? pack16<BF16>(v.x * scale, v.y * scale) : 0u;
-        const uint32_t hi = live ? pack16<BF16>(v.z * scale, v.w * scale) : 0u;
-        uint16_t* o = a.out + t * a.ldo + c;
-        if (whole) {
-            *reinterpret_cast<uint2*>(o) = make_uint2(lo, hi);
-        } else {
-            const uint32_t w[2] = {lo, hi};
+            uint32_t w[4] = {0, 0, 0, 0};
+            if (p[k] >= 0)
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (c + k < a.d) o[k] = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
+                for (int h = 0; h < 2; ++h) {
+                    w[2 * h] = pack16<BF16>(v[k][h].x * scale, v[k][h].y * scale);
+                    w[2 * h + 1] = pack16<BF16>(v[k][h].z * scale, v[k][h].w * scale);
+                }
+            uint16_t* o = a.out + t * a.ldo + c;
+            if (whole) {
+                *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
+            } else {
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (c + q < a.d) o[q] = (uint16_t)(w[q >> 1] >> (16 * (q & 1)));
+            }
         }
     }
 }
