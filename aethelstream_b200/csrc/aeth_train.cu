@@ -291,22 +291,27 @@ constexpr int kStorePerSm = 8, kBackPerSm = 3;
 
 // The ring's layout for rows of d features: groups of tx threads that hold a
 // row in four eights each, as many stages as shared memory takes beside gain.
-// Taken for many rows (each SM walks over several) that bulk copies can move.
+// Taken for many rows (each SM walks over several) that bulk copies can move
+// and of which a group has room for two (f32: up to 15968 features).
 constexpr int kRingShared = 220 * 1024;
 CkptRing ring_plan(int64_t d, int size, bool res) {
     CkptRing r;
-    r.tx = (int)((d + 1023) / 1024) * 32;
+    const bool wide = d > 8192;
+    r.tx = wide ? kRingThreads : (int)((d + 1023) / 1024) * 32;
+    r.eights = (int)((d + 8 * r.tx - 1) / (8 * r.tx));
     r.groups = kRingThreads / r.tx;
     const int row = (int)up(d * size, 128);
     r.res_at = row;
-    r.codes_at = row * (res ? 2 : 1);
+    r.codes_at = row * (res && !wide ? 2 : 1);
     r.stage_bytes = r.codes_at + (int)up(d, 128);
-    const int room = kRingShared - 4 * 8 * 4 * r.tx;
+    const int room = kRingShared - r.gain_bytes();
     while (r.groups > 1 && room / r.stage_bytes / r.groups < 2) r.groups /= 2;  // two stages a group at least
     r.stages = std::min(room / r.stage_bytes / r.groups, kRingMaxStages);
     return r;
 }
-bool ring_fits(int64_t rows, int64_t d) { return rows > 2 * num_sms() && d % 16 == 0 && d >= 256 && d <= 8192; }
+bool ring_fits(int64_t rows, int64_t d, int size, bool res) {
+    return rows > 2 * num_sms() && d % 16 == 0 && d >= 256 && d <= 16384 && ring_plan(d, size, res).stages >= 2;
+}
 
 template <typename F>
 int by_type(int dtype, F f) {
@@ -512,11 +517,11 @@ int aeth_rms_norm_checkpoint_backward(const void* dy, int64_t ld_dy, const int8_
         using T = std::remove_pointer_t<decltype(tag)>;
         CkptBack<T> a{{codes, scales, gain, gain_dtype, rows, (int)d, eps}, static_cast<const T*>(dy), ld_dy,
                       static_cast<const T*>(d_residual), ld_residual, static_cast<T*>(dx), part};
-        if (vec && ring_fits(rows, d) && aligned16(codes)) {
+        if (vec && ring_fits(rows, d, sz, d_residual != nullptr) && aligned16(codes)) {
             const CkptRing r = ring_plan(d, sz, d_residual != nullptr);
-            const int smem = r.groups * r.stages * r.stage_bytes + 4 * 8 * 4 * r.tx;
+            const int smem = r.groups * r.stages * r.stage_bytes + r.gain_bytes();
             static std::atomic<bool> allowed[kMaxDevices] = {};
-            auto kern = ckpt_back_ring_kernel<T>;
+            auto kern = ckpt_back_ring_kernel<T, wide.value>;
             AETH_TRY(allow_shared(kern, kRingShared, allowed));
             kern<<<num_sms(), r.groups * r.tx, smem, st>>>(a, r, rt->err_word);
             AETH_LAUNCH_CHECK();

@@ -301,8 +301,12 @@ __device__ __forceinline__ float ck_block_tree(const float (&v)[VPT], Op op) {
         const float a0 = op(b3 ? v[1] : v[0], __shfl_xor_sync(all, b3 ? v[0] : v[1], 8));
         const float a1 = op(b3 ? v[3] : v[2], __shfl_xor_sync(all, b3 ? v[2] : v[3], 8));
         c = op(b2 ? a1 : a0, __shfl_xor_sync(all, b2 ? a0 : a1, 4));
+    } else if constexpr (VPT == 2) {
+        const bool b3 = threadIdx.x & 8;
+        c = op(b3 ? v[1] : v[0], __shfl_xor_sync(all, b3 ? v[0] : v[1], 8));
+        c = op(c, __shfl_xor_sync(all, c, 4));
     } else {
-        static_assert(VPT == 1, "one or four blocks a lane");
+        static_assert(VPT == 1, "one, two or four blocks a lane");
         c = op(v[0], __shfl_xor_sync(all, v[0], 8));
         c = op(c, __shfl_xor_sync(all, c, 4));
     }
@@ -311,14 +315,16 @@ __device__ __forceinline__ float ck_block_tree(const float (&v)[VPT], Op op) {
 }
 template <int VPT>
 __device__ __forceinline__ int ck_lane_block() {  // the k whose block this lane ends with
-    return VPT == 4 ? (int)((threadIdx.x >> 3) & 1) + (int)((threadIdx.x >> 1) & 2) : 0;
+    const int b3 = (threadIdx.x >> 3) & 1, b2 = (threadIdx.x >> 2) & 1;
+    return VPT == 4 ? b3 + 2 * b2 : VPT == 2 ? b3 : 0;
 }
 template <int VPT>
 __device__ __forceinline__ float ck_from_block(float c, int k) {  // that block's value, in all its lanes
+    static_assert(VPT != 2, "the kernels that need it hold one or four");
     return VPT == 4 ? __shfl_sync(0xffffffffu, c, (threadIdx.x & 16) | ((k & 1) << 3) | ((k & 2) << 1)) : c;
 }
 template <int VPT>
-__device__ __forceinline__ bool ck_block_writer() { return (threadIdx.x & (VPT == 4 ? 3 : 15)) == 0; }
+__device__ __forceinline__ bool ck_block_writer() { return (threadIdx.x & (16 / VPT - 1)) == 0; }
 
 // Sums of a row, spread over threadIdx.x (threadIdx.y is the row within the
 // CTA).  The order depends on the row's length alone, so a row's result does
@@ -782,7 +788,7 @@ __global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, 2))
             }
 }
 
-// The same for many rows of up to 8192 features (d a multiple of 16, every row
+// The same for many rows of up to 16384 features (d a multiple of 16, every row
 // on 16 bytes): one CTA an SM, whose rows come through shared memory by bulk
 // copies, so that what is in flight does not depend on the registers or on
 // where the row sums stand.  The CTA's threads form groups of tx, each of which
@@ -792,17 +798,25 @@ __global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, 2))
 // groups' are added in their order.  8192 x 8192 bf16 with the residual's
 // gradient: 94 us with the sum over the CTAs, 5.0 TB/s (rows through registers
 // instead: 133).  Sixteen warps an SM issue 55 % of the time; what is left is the
-// wait between a row's two passes.
+// wait between a row's two passes.  (A row ahead, its sums taken before the last
+// row's dx is written, costs more in registers and barriers than it hides: 109.)
+// WIDE: more than 8192 features, one group.  The residual's gradient goes
+// through registers, which leaves the ring room for more rows (for shorter rows
+// it costs 4 to 15 %), and a thread's eights join 8192 features apart as the
+// spans of ckpt_back_kernel do, so that the row's sums are the same.  4096 x
+// 12288 bf16 with it: 85 us (in spans: 164).
 struct CkptRing {
     int tx, groups, stages;  // stages a group
+    int eights;              // of features a thread holds, 4 at most
     int stage_bytes, res_at, codes_at;  // dy first
+    __host__ __device__ int gain_bytes() const { return eights * tx * 8 * 4; }
 };
 constexpr int kRingThreads = 512, kRingMaxStages = 8;
 
-template <typename T>
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kRingThreads, 1)
     ckpt_back_ring_kernel(const __grid_constant__ CkptBack<T> a, const CkptRing ring, uint32_t* err) {
-    constexpr int VPT = 4;
+    constexpr int VPT = 4, SUMS = WIDE ? 2 : VPT;
     extern __shared__ __align__(128) uint8_t ck_ring[];
     __shared__ float sh[2 * 2 * VPT * kRingThreads / 16];  // [group][parity][block][2]
     __shared__ uint64_t full_s[16 * kRingMaxStages];
@@ -820,7 +834,7 @@ __global__ void __launch_bounds__(kRingThreads, 1)
         for (int s = 0; s < ring.stages; ++s) mbar_init(&full[s], 1);
         fence_mbar_init();
     }
-    for (int i = threadIdx.x; i < 2 * VPT * tx; i += blockDim.x) {
+    for (int i = threadIdx.x; i < 2 * ring.eights * tx; i += blockDim.x) {
         const int c = 8 * (i % tx + i / (2 * tx) * tx) + 4 * (i / tx % 2);
         const float4 g = ck_gain4<true>(a.in.gain, a.in.gain_dtype, c, d);
         sg[i] = make_ulonglong2(f2(g.x, g.y), f2(g.z, g.w));
@@ -833,9 +847,9 @@ __global__ void __launch_bounds__(kRingThreads, 1)
         const int64_t t = row0 + j * step;
         const uint32_t row16 = (uint32_t)d * (uint32_t)sizeof(T);
         uint8_t* st = stages + (size_t)s * ring.stage_bytes;
-        mbar_arrive_expect_tx(&full[s], row16 * (a.d_res ? 2 : 1) + (uint32_t)d);
+        mbar_arrive_expect_tx(&full[s], row16 * (a.d_res && !WIDE ? 2 : 1) + (uint32_t)d);
         bulk_load(st, a.dy + t * a.ld_dy, row16, &full[s]);
-        if (a.d_res) bulk_load(st + ring.res_at, a.d_res + t * a.ld_res, row16, &full[s]);
+        if (a.d_res && !WIDE) bulk_load(st + ring.res_at, a.d_res + t * a.ld_res, row16, &full[s]);
         bulk_load(st + ring.codes_at, a.in.codes + t * d, (uint32_t)d, &full[s]);
     };
     if (x0 == 0)
@@ -867,20 +881,23 @@ __global__ void __launch_bounds__(kRingThreads, 1)
             break;
         }
         const uint8_t* st = stages + (size_t)stage * ring.stage_bytes;
-        float acc[2][VPT], sum[2];
+        float acc[2][SUMS] = {}, sum[2];
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
             const int c = 8 * (x0 + k * tx);
-            acc[0][k] = acc[1][k] = 0.0f;
             if (c < d) {
                 const uint2 q = *reinterpret_cast<const uint2*>(st + ring.codes_at + c);
                 const Pack8<T> dy = ck_shared8<T>(st, c);
                 const ulonglong2 g0 = sg[2 * k * tx + x0], g1 = sg[(2 * k + 1) * tx + x0];
                 const uint64_t g[4] = {g0.x, g0.y, g1.x, g1.y};
-                ck_back_sums<T>(q, dy, g, s[k], acc[0][k], acc[1][k]);
+                ck_back_sums<T>(q, dy, g, s[k], acc[0][k % SUMS], acc[1][k % SUMS]);
             }
         }
-        ck_row_sum<2, VPT>(acc, sh + (grp * 2 + (j & 1)) * (VPT * tx / 16) * 2, x0, tx, sum, [=] {
+        Pack8<T> held[WIDE ? VPT : 1];
+        if (WIDE && a.d_res)  // arrives during the row's sum
+#pragma unroll
+            for (int k = 0; k < (WIDE ? VPT : 1); ++k) held[k] = ck_load8<T, true>(a.d_res + t * a.ld_res, 8 * (x0 + k * tx), d);
+        ck_row_sum<2, SUMS>(acc, sh + (grp * 2 + (j & 1)) * (SUMS * tx / 16) * 2, x0, tx, sum, [=] {
             if (tx == 32) __syncwarp();
             else named_bar(1 + grp, tx);
         });
@@ -896,7 +913,8 @@ __global__ void __launch_bounds__(kRingThreads, 1)
                 Pack8<T> dy = ck_shared8<T>(st, c), res;
                 ck_opaque(q);
                 ck_opaque(dy);
-                if (a.d_res) res = ck_shared8<T>(st + ring.res_at, c);
+                if (WIDE) res = held[WIDE ? k : 0];
+                else if (a.d_res) res = ck_shared8<T>(st + ring.res_at, c);
                 const ulonglong2 g0 = sg[2 * k * tx + x0], g1 = sg[(2 * k + 1) * tx + x0];
                 const uint64_t g[4] = {g0.x, g0.y, g1.x, g1.y};
                 ck_store8<T, true>(a.dx + t * d, c, d,

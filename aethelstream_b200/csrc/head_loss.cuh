@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(512) head_loss_kernel(const HeadLoss a) {
 // states in shared memory; it keeps their running maximum and sum and leaves
 // one pair per token and CTA.  One token x 4096 x 32000: 46 us a call, 5.7 TB/s
 // (6.3 at 2048 x 131071); the tile product takes 64, its columns of 128 bytes
-// and four launches included.
+// and its launches included.
 constexpr int kHeadVecTokens = 4, kHeadVecThreads = 512;
 
 struct HeadVec {

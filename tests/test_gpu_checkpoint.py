@@ -293,3 +293,22 @@ def test_backward_without_eps(rows, d):
     want = (dy.double() * v / torch.sqrt((v * v).mean(1, keepdim=True)))
     close(dw, want.sum(0), want.abs().sum(0) * (d / 16 + 16 + rows) * E + 1e-37)
     assert dx.isfinite().all()
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("rows,d", [(333, 8208), (700, 12288), (301, 16384), (1200, 1008), (900, 5120)])
+@pytest.mark.parametrize("with_res", [False, True])
+def test_backward_of_many_rows(dt, rows, d, with_res):
+    """Against the formula, and bit for bit what the first rows give by themselves."""
+    import aethelstream_b200 as A
+    x, gain, gen = acts(rows, d, dt, rows + d)
+    _, ck = A.rms_norm_checkpoint(x, gain.to(dt), eps=EPS)
+    dy = torch.randn(rows, d, generator=gen, device="cuda").to(dt)
+    res = torch.randn(rows, d, generator=gen, device="cuda").to(dt) if with_res else None
+    dx, dw = A.rms_norm_checkpoint_backward(dy, ck, gain, eps=EPS, d_residual=res)
+    want, bound, want_w, bound_w = back64(values64(ck), dy.double(), gain.double(), None if res is None else res.double())
+    close(dx, want, 1.1 * (bound + U[dt] * want.abs()) + TINY[dt])
+    close(dw, want_w, bound_w + 1e-37)
+    few = A.rms_norm_checkpoint(x[:9], gain.to(dt), eps=EPS)[1]
+    assert torch.equal(A.rms_norm_checkpoint_backward(dy[:9], few, gain, eps=EPS,
+                                                      d_residual=None if res is None else res[:9])[0], dx[:9])
