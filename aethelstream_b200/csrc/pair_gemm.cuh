@@ -95,11 +95,11 @@ struct PairTail {
         full = tiles / pairs * pairs;
         rest = tiles - full;
         splits = 1;
-        float least = 2.0f;
-        for (int s = 1; s <= 16 && rest > 0; ++s) {
-            if (s > 1 && (s * 8 > kb || (s - 1) * rest > 2 * pairs)) break;
-            const float cost = (float)((rest * s + pairs - 1) / pairs) / (float)s + 0.01f * (float)s;
-            if (cost < least) {
+        int least = 101;  // (waves / s + s / 100) * 100 s, in whole numbers: host and device agree
+        for (int s = 2; s <= 16 && rest > 0; ++s) {
+            if (s * 8 > kb || (s - 1) * rest > 2 * pairs) break;
+            const int cost = 100 * ((rest * s + pairs - 1) / pairs) + s * s;
+            if (cost * splits < least * s) {
                 least = cost;
                 splits = s;
             }
@@ -108,7 +108,16 @@ struct PairTail {
         splits = (kb + per - 1) / per;  // no empty range
     }
 };
-// Position of tile (m, n) in the order in which tiles are walked.
+// Tile r in the order in which tiles are walked.
+__device__ __forceinline__ void pair_tile_at(int r, int tiles_m, int tiles_n, int group, int& m, int& n) {
+    const int grp = r / (group * tiles_n);
+    const int first = grp * group;
+    const int gm = min(group, tiles_m - first);
+    const int rr = r - grp * group * tiles_n;
+    n = rr / gm;
+    m = first + rr - n * gm;
+}
+// Position of tile (m, n) in that order.
 __host__ __device__ inline int pair_tile_index(int m, int n, int tiles_m, int tiles_n) {
     const int group = pair_group(tiles_m), first = m / group * group;
     const int gm = tiles_m - first < group ? tiles_m - first : group;
@@ -123,6 +132,7 @@ struct PairTile {
     int c_begin, c_end;  // this warp's columns within the tile (multiples of 32)
     int m_tile, n_tile, half;
     int part;          // 0: the tile's own place; k > 0: buffer k - 1 of the tail
+    int rest;          // of a split tile: its number among them, else -1
     int tile_row;      // row0 within the tile
     int M, N;          // live sizes
     uint8_t* staging;  // kPairStaging bytes of this warp alone, the warps' one after the other
@@ -130,7 +140,7 @@ struct PairTile {
 };
 
 struct PairUnit {
-    int m0, n0, n_tile, part, kb0, kb1;
+    int m0, n0, n_tile, part, rest, kb0, kb1;
 };
 
 struct PairShape {
@@ -166,18 +176,17 @@ struct PairShape {
         PairUnit t;
         int r = u, split = 0, per = kb;
         t.part = 0;
+        t.rest = -1;
         if (u >= full) {
             split = (u - full) / rest;
             r = u - split * rest;
             per = (kb + splits - 1) / splits;
+            if (splits > 1) t.rest = r - full;
             t.part = split > 0 ? (split - 1) * rest + (r - full) + 1 : 0;
         }
-        const int grp = r / (group * tiles_n);
-        const int first = grp * group;
-        const int gm = min(group, tiles_m - first);
-        const int rr = r - grp * group * tiles_n;
-        t.n_tile = rr / gm;
-        t.m0 = (first + rr - t.n_tile * gm) * 256;
+        int m;
+        pair_tile_at(r, tiles_m, tiles_n, group, m, t.n_tile);
+        t.m0 = m * 256;
         t.n0 = t.n_tile * bn;
         t.kb0 = min(split * per, kb);  // a K shorter than the tail's plan leaves its last ranges empty
         t.kb1 = min(t.kb0 + per, kb);
@@ -352,6 +361,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
             tile.m_tile = t.m0 / 256;
             tile.n_tile = t.n_tile;
             tile.part = t.part;
+            tile.rest = t.rest;
             tile.tile_row = crank * 128 + q * 32;
             if constexpr (Epi::kChunk > 0) {
                 float acc[128];
@@ -466,6 +476,98 @@ struct PairOut16 {
     }
 };
 
+// Writes 32 columns of the warp's 32 rows (thread = row) in fp32 to out, whose
+// row 0 is the warp's first: rows below `rows`, columns c .. below `cols` (both a
+// multiple of 4), over what is there or added to it.
+__device__ __forceinline__ void pair_store32(const PairTile& t, const float (&v)[32], int c, float* out, int64_t pitch,
+                                             int rows, int cols, bool over) {
+    const int row = t.lane;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+        *reinterpret_cast<float4*>(t.staging + row * 128 + ((k ^ (row & 7)) * 16)) =
+            make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = i * 4 + (t.lane >> 3), k = t.lane & 7;
+        const int gc = c + k * 4;
+        float4 x = *reinterpret_cast<const float4*>(t.staging + r * 128 + ((k ^ (r & 7)) * 16));
+        if (r < rows && gc < cols) {
+            float4* o = reinterpret_cast<float4*>(out + r * pitch + gc);
+            if (!over) {
+                const float4 p = *o;
+                x = make_float4(p.x + x.x, p.y + x.y, p.z + x.z, p.w + x.w);
+            }
+            *o = x;
+        }
+    }
+    __syncwarp();
+}
+
+// Epilogue: D in 16 bits; the ranges of a split tile in fp32, each to a buffer
+// of 256 x 256 of its own, for pair_join_kernel.
+template <bool BF16>
+struct PairSplit16 {
+    static constexpr int kChunk = 0;
+    PairOut16<BF16> whole;
+    float* buffers;  // range s of split tile i: s * rest + i
+    int rest;
+    __device__ __forceinline__ void tile(const PairTile& t) const {
+        if (t.rest < 0) {
+            whole.tile(t);
+            return;
+        }
+        float* out = buffers + (int64_t)(t.part ? t.part - 1 + rest : t.rest) * 65536 + t.tile_row * 256;
+        for (int c = t.c_begin; c < t.c_end; c += 32) {
+            if (t.col0 + c >= t.N || t.row0 >= t.M) break;
+            float v[32];
+            tmem_ld32<0>(t.tmem + (uint32_t)c, v);
+            tmem_wait_ld();
+            pair_store32(t, v, c, out, 256, t.M - t.row0, 256, true);
+        }
+    }
+};
+
+// Adds up a split tile's ranges in their order: 8 rows a CTA, a warp a row.
+struct PairJoin {
+    const float* buffers;
+    int full, rest, splits;  // PairTail's
+    int M, N;
+    uint16_t* out;
+    int64_t ld;
+};
+template <bool BF16>
+__global__ void __launch_bounds__(256) pair_join_kernel(const PairJoin a) {
+    pdl_wait();
+    const int i = (int)blockIdx.x >> 5, row = ((int)blockIdx.x & 31) * 8 + ((int)threadIdx.x >> 5);
+    const int col = ((int)threadIdx.x & 31) * 8;
+    const int tiles_m = (a.M + 255) / 256, tiles_n = (a.N + 255) / 256;
+    int m, n;
+    pair_tile_at(a.full + i, tiles_m, tiles_n, pair_group(tiles_m), m, n);
+    const int gr = m * 256 + row, gc = n * 256 + col;
+    if (gr >= a.M || gc >= a.N) return;
+    const float* p = a.buffers + (int64_t)i * 65536 + row * 256 + col;
+    float v[8] = {};
+#pragma unroll 8
+    for (int s = 0; s < a.splits; ++s) {
+        const float4* q = reinterpret_cast<const float4*>(p + (int64_t)s * a.rest * 65536);
+        const float4 x = q[0], y = q[1];
+        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+        v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+    }
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = pack16<BF16>(v[2 * k], v[2 * k + 1]);
+    uint16_t* o = a.out + (int64_t)gr * a.ld + gc;
+    if (a.ld % 8 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && gc + 8 <= a.N) {
+        *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (gc + k < a.N) o[k] = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
+    }
+}
+
 // Epilogue: D in fp32, stored by the first K range of a sum over launches and
 // added by the later ones; a tail's further ranges go to `extra`, 256 x 256
 // each.  Each element has one writer per launch, so the order of a sum is the
@@ -486,27 +588,7 @@ struct PairSlab {
             float v[32];
             tmem_ld32<0>(t.tmem + (uint32_t)c, v);
             tmem_wait_ld();
-            const int row = t.lane;
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                *reinterpret_cast<float4*>(t.staging + row * 128 + ((k ^ (row & 7)) * 16)) =
-                    make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = i * 4 + (t.lane >> 3), k = t.lane & 7;
-                const int gc = c + k * 4;
-                float4 x = *reinterpret_cast<const float4*>(t.staging + r * 128 + ((k ^ (r & 7)) * 16));
-                if (t.row0 + r < t.M && gc < cols) {
-                    float4* o = reinterpret_cast<float4*>(out + r * pitch + gc);
-                    if (!first) {
-                        const float4 p = *o;
-                        x = make_float4(p.x + x.x, p.y + x.y, p.z + x.z, p.w + x.w);
-                    }
-                    *o = x;
-                }
-            }
-            __syncwarp();
+            pair_store32(t, v, c, out, pitch, t.M - t.row0, cols, first);
         }
     }
 };

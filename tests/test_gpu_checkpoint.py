@@ -312,3 +312,55 @@ def test_backward_of_many_rows(dt, rows, d, with_res):
     few = A.rms_norm_checkpoint(x[:9], gain.to(dt), eps=EPS)[1]
     assert torch.equal(A.rms_norm_checkpoint_backward(dy[:9], few, gain, eps=EPS,
                                                       d_residual=None if res is None else res[:9])[0], dx[:9])
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,m,d", [(8170, 216, 952), (5000, 64, 64), (8000, 33, 1001), (8191, 1032, 1040), (8192, 4608, 4360)])
+def test_weight_grad_split_along_the_tokens(dt, rows, m, d):
+    """Tiles that leave CTA pairs idle, alone and after whole waves."""
+    import aethelstream_b200 as A
+    x, gain, gen = acts(rows, d, dt, rows + m + d)
+    _, ck = A.rms_norm_checkpoint(x, gain.to(dt), eps=EPS)
+    dy = torch.randn(rows, m, generator=gen, device="cuda").to(dt)
+    dw = A.checkpoint_weight_grad(dy, ck)
+    v = values64(ck)
+    want = dy.double().T @ v
+    mag = dy.double().abs().T @ v.abs()
+    close(dw, want, (1.1 * U[dt] + 2.0 ** -22 + 2 * rows * E) * mag + 1.1 * U[dt] * want.abs()
+          + TINY[dt] * (1 + dy.double().abs().sum(0)[:, None]))
+    assert torch.equal(dw, A.checkpoint_weight_grad(dy, ck))
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("rows,d", [(5, 1), (40, 7), (3, 8), (9, 255), (9, 257), (33, 263), (700, 513), (400, 2276), (350, 8191), (4, 9001)])
+def test_rows_off_alignment(dt, rows, d):
+    """Every width and address gives bit for bit what aligned rows give."""
+    import aethelstream_b200 as A
+    x, gain, gen = acts(rows, d, dt, rows + d)
+    g = gain.to(dt)
+    dy = torch.randn(rows, d, generator=gen, device="cuda").to(dt)
+    p = -(-d // 16) * 16  # the same rows with zeros up to a multiple of 16: the same blocks and codes
+
+    def padded(t):
+        o = torch.zeros(t.shape[:-1] + (p,), dtype=t.dtype, device="cuda")
+        o[..., :d] = t
+        return o
+
+    ck, ck_p = A.rms_norm_checkpoint(x, g, residual=dy)[1], A.rms_norm_checkpoint(padded(x), padded(g), residual=padded(dy))[1]
+    assert torch.equal(ck.codes, ck_p.codes[:, :d]) and torch.equal(ck.scales, ck_p.scales)
+    plain = A.checkpoint_decode(ck)
+    assert torch.equal(plain, A.checkpoint_decode(ck_p)[:, :d])
+    total = A.rms_norm_checkpoint(x, g, residual=dy)[2]
+    assert torch.equal(total, (x.float() + dy.float()).to(dt))
+    first = A.rms_norm_checkpoint(x, g, eps=EPS), A.checkpoint_decode(ck, g, eps=EPS)
+    dx, dw = A.rms_norm_checkpoint_backward(dy, ck, g, eps=EPS, d_residual=x)
+    for shift in range(1, 9):
+        wide = torch.zeros(rows, d + 19, dtype=dt, device="cuda")
+        wide[:, shift:shift + d] = x
+        dwide = torch.zeros(rows, d + 13, dtype=dt, device="cuda")
+        dwide[:, shift:shift + d] = dy
+        xs, ds = wide[:, shift:shift + d], dwide[:, shift:shift + d]
+        y, c = A.rms_norm_checkpoint(xs, g, eps=EPS)
+        assert torch.equal(y, first[0][0]) and torch.equal(c.codes, first[0][1].codes) and torch.equal(c.scales, first[0][1].scales)
+        dxs, dws = A.rms_norm_checkpoint_backward(ds, ck, g, eps=EPS, d_residual=xs)
+        assert torch.equal(dxs, dx) and torch.equal(dws, dw)
