@@ -109,8 +109,92 @@ __device__ __forceinline__ void ck_opaque(Pack8<T>& p) {
         asm volatile("" : "+r"(p.w[k].x), "+r"(p.w[k].y), "+r"(p.w[k].z), "+r"(p.w[k].w)::"memory");
 }
 
+// Rows that do not start on 16 bytes (odd widths, views): a thread's eight
+// elements lie `ck_off` elements into a 16-byte granule, the same for the whole
+// row.  They are read as whole granules, one more than they fill, and shifted
+// into place; they are written as whole granules too, each lane the one that
+// holds the last elements of the lane before it and all but the last of its own.
+// A write never leaves the row: its ends, and a warp's, go element by element.
+// A read of the row's first or last granule takes in bytes of the rows beside
+// it, which are dropped; the matrix's own first and last row (ck_inner) are read
+// element by element.  8192 x 8191 bf16, single elements against granules: store
+// with residual 435 and 200 us, restored 183 and 70, norm 188 and 89, gradient
+// 378 and 224; what is left is each granule's second load, the shifts and the
+// registers that these take (8192 x 8184, without them: 108, 43, 47 and 110).
+template <typename E>
+__device__ __forceinline__ int ck_off(const E* p) {
+    constexpr int kGranule = sizeof(E) == 1 ? 8 : 16;
+    return (int)((reinterpret_cast<uintptr_t>(p) & (kGranule - 1)) / sizeof(E));
+}
+// out = the bytes of `in` from m on; G words are a granule, m below its bytes.
+template <int W, int G>
+__device__ __forceinline__ void ck_shift(uint32_t (&in)[W + G], uint32_t m, uint32_t (&out)[W]) {
+    if (G == 4)
+#pragma unroll
+        for (int i = 0; i < W + 2; ++i) in[i] = m & 8 ? in[(i + 2) % (W + G)] : in[i];
+#pragma unroll
+    for (int i = 0; i < W + 1; ++i) in[i] = m & 4 ? in[i + 1] : in[i];
+#pragma unroll
+    for (int i = 0; i < W; ++i) out[i] = __funnelshift_r(in[i], in[i + 1], (m & 3) * 8);
+}
+template <typename E>  // E: int8_t (eight bytes, granules of 8) or a float type
+struct CkAny {
+    static constexpr int kWords = 2 * sizeof(E), kGranule = sizeof(E) == 1 ? 2 : 4, kElems = 4 * kGranule / sizeof(E);
+    using V = std::conditional_t<sizeof(E) == 1, uint2, uint4>;
+
+    // The granules that hold the row's elements c .. c + 7.
+    static __device__ __forceinline__ void load(const E* row, int c, int d, uint32_t (&in)[kWords + kGranule]) {
+        const int off = ck_off(row + c);
+        const V* q = reinterpret_cast<const V*>(row + c - off);
+        constexpr int n = kWords / kGranule;
+#pragma unroll
+        for (int i = 0; i <= n; ++i) {
+            V v = {};
+            if (c + i * kElems < d + (i > 0 ? off : 0) && (i < n || off)) v = __ldg(q + i);
+            *reinterpret_cast<V*>(in + i * kGranule) = v;
+        }
+    }
+    // Those elements, zero past the row's end.
+    static __device__ __forceinline__ void place(const E* row, int c, int d, uint32_t (&in)[kWords + kGranule],
+                                                 uint32_t (&w)[kWords]) {
+        ck_shift<kWords, kGranule>(in, (uint32_t)ck_off(row + c) * sizeof(E), w);
+        constexpr int per = 4 / sizeof(E);
+        if (c + 8 > d)
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+                const int have = d - c - i * per;  // elements of this word
+                w[i] = have >= per ? w[i] : have <= 0 ? 0u : w[i] & ((1u << (8 * sizeof(E) * have % 32)) - 1u);
+            }
+    }
+    // By all lanes of a warp, whose c are neighbours.  Bit i of the result: the
+    // lane still has to write its element i.
+    static __device__ __forceinline__ uint32_t store(E* row, int c, int d, const uint32_t (&w)[kWords]) {
+        const int off = ck_off(row + c), lane = threadIdx.x & 31;
+        alignas(16) uint32_t in[kWords + kGranule], o[kWords];
+#pragma unroll
+        for (int i = 0; i < kGranule; ++i) in[i] = __shfl_up_sync(0xffffffffu, w[kWords - kGranule + i], 1);
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) in[kGranule + i] = w[i];
+        const bool mine = (off == 0 || lane > 0) && c - off + 8 <= d;
+        const bool next = off > 0 && lane < 31 && c - off + 16 <= d;
+        if (off) {
+            ck_shift<kWords, kGranule>(in, (uint32_t)(kElems - off) * sizeof(E), o);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) o[i] = w[i];
+        }
+        if (mine) {
+            V* q = reinterpret_cast<V*>(row + c - off);
+#pragma unroll
+            for (int i = 0; i < kWords / kGranule; ++i) q[i] = *reinterpret_cast<const V*>(o + i * kGranule);
+        }
+        const uint32_t head = 0xffu >> off, exist = c >= d ? 0 : c + 8 <= d ? 0xffu : 0xffu >> (8 - (d - c));
+        return exist & ~((mine ? head : 0) | (next ? 0xffu & ~head : 0));
+    }
+};
+
 // Features c .. c + 7 of a row of d (zero past its end).  VEC: every row
-// starts on 16 bytes and d is a multiple of 8; otherwise single elements.
+// starts on 16 bytes and d is a multiple of 8.  Stores by whole warps.
 template <typename T, bool VEC>
 __device__ __forceinline__ Pack8<T> ck_load8(const T* row, int c, int d) {
     Pack8<T> p;
@@ -133,9 +217,18 @@ __device__ __forceinline__ void ck_store8(T* row, int c, int d, const Pack8<T>& 
 #pragma unroll
             for (int k = 0; k < Pack8<T>::kWords; ++k) reinterpret_cast<uint4*>(row + c)[k] = p.w[k];
     } else {
+        uint32_t w[CkAny<T>::kWords];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (c + i < d) row[c + i] = (T)ck_value<T>(p, i);
+        for (int k = 0; k < Pack8<T>::kWords; ++k) {
+            w[4 * k] = p.w[k].x;
+            w[4 * k + 1] = p.w[k].y;
+            w[4 * k + 2] = p.w[k].z;
+            w[4 * k + 3] = p.w[k].w;
+        }
+        if (const uint32_t left = CkAny<T>::store(row, c, d, w))
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (left >> i & 1) row[c + i] = (T)ck_value<T>(p, i);
     }
 }
 template <bool VEC>
@@ -152,9 +245,11 @@ __device__ __forceinline__ void ck_store_codes(int8_t* row, int c, int d, uint2 
     if (VEC) {
         if (c < d) *reinterpret_cast<uint2*>(row + c) = q;
     } else {
+        const uint32_t w[2] = {q.x, q.y};
+        if (const uint32_t left = CkAny<int8_t>::store(row, c, d, w))
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (c + i < d) row[c + i] = (int8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
+            for (int i = 0; i < 8; ++i)
+                if (left >> i & 1) row[c + i] = (int8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
     }
 }
 // The value of code i (the conversion instruction takes a byte of a register).
@@ -378,6 +473,50 @@ __device__ __forceinline__ void ck_row_sum(const float (&v)[N][VPT], float* sh, 
 #define CK_SPANS(base, d) for (int base = 0; base < (WIDE ? (d) : 1); base += 8 * VPT * (int)blockDim.x)
 #define CK_COLUMN(base, k) ((base) + 8 * (int)(threadIdx.x + (k) * blockDim.x))
 
+// A thread's VPT eights of a row.  inner: the matrix goes on before and after
+// the row, whose first and last granule may then be read whole.
+template <typename T, int VPT, bool VEC>
+__device__ __forceinline__ void ck_load_row(const T* row, int base, int d, bool inner, Pack8<T> (&x)[VPT]) {
+    if (!VEC && inner) {
+        alignas(16) uint32_t in[VPT][CkAny<T>::kWords + CkAny<T>::kGranule];
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) CkAny<T>::load(row, CK_COLUMN(base, k), d, in[k]);
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            uint32_t w[CkAny<T>::kWords];
+            CkAny<T>::place(row, CK_COLUMN(base, k), d, in[k], w);
+#pragma unroll
+            for (int i = 0; i < Pack8<T>::kWords; ++i)
+                x[k].w[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) x[k] = ck_load8<T, VEC>(row, CK_COLUMN(base, k), d);
+    }
+}
+template <int VPT, bool VEC>
+__device__ __forceinline__ void ck_codes_row(const int8_t* row, int base, int d, bool inner, uint2 (&q)[VPT]) {
+    if (!VEC && inner) {
+        alignas(16) uint32_t in[VPT][4];
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) CkAny<int8_t>::load(row, CK_COLUMN(base, k), d, in[k]);
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            uint32_t w[2];
+            CkAny<int8_t>::place(row, CK_COLUMN(base, k), d, in[k], w);
+            q[k] = make_uint2(w[0], w[1]);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) q[k] = ck_load_codes<VEC>(row, CK_COLUMN(base, k), d);
+    }
+}
+// Whether 16 bytes of the matrix lie before row t, and 16 after it.
+__device__ __forceinline__ bool ck_inner(int64_t t, int64_t rows, int d) {
+    const int n = d < 16 ? 16 : 1;
+    return t >= n && t + n < rows;
+}
+
 // CTAs that the register budget has to allow on an SM.
 constexpr int ck_min_ctas(int vpt, int many) { return vpt == 4 ? many : 1; }
 
@@ -400,12 +539,11 @@ struct CkptStore {
 
 template <typename T, int VPT, bool VEC>
 __device__ __forceinline__ void ckpt_input(const CkptStore<T>& a, int64_t t, int base, int d, Pack8<T> (&x)[VPT]) {
-#pragma unroll
-    for (int k = 0; k < VPT; ++k) x[k] = ck_load8<T, VEC>(a.x + t * a.ldx, CK_COLUMN(base, k), d);
+    const bool inner = ck_inner(t, a.rows, a.d);
+    ck_load_row<T, VPT, VEC>(a.x + t * a.ldx, base, d, inner, x);
     if (a.residual) {
         Pack8<T> res[VPT];
-#pragma unroll
-        for (int k = 0; k < VPT; ++k) res[k] = ck_load8<T, VEC>(a.residual + t * a.ldr, CK_COLUMN(base, k), d);
+        ck_load_row<T, VPT, VEC>(a.residual + t * a.ldr, base, d, inner, res);
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
             float v[8], w[8];
@@ -425,7 +563,7 @@ constexpr bool ck_shared_gain(int vpt, bool wide) { return vpt == 4 && !wide; }
 // 3.2 TB/s written, where a copy writes 3.3.  Five of nine bytes an element are
 // written (sum, y, code).
 template <typename T, int VPT, bool VEC, bool WIDE>
-__global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, sizeof(T) == 2 ? 4 : 3))
+__global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, VEC && sizeof(T) == 2 ? 4 : 3))
     ckpt_store_kernel(const __grid_constant__ CkptStore<T> a) {
     __shared__ float sh[2 * kCkptShared];
     extern __shared__ float4 ck_dyn[];
@@ -499,18 +637,27 @@ struct CkptRead {
     float eps;
 };
 
-// x^ of eight features: the block's scale and the codes.
-template <bool VEC>
-__device__ __forceinline__ void ck_restore8(const CkptRead& a, int64_t t, int c, int d, uint2& q, float& s) {
+// x^ of a thread's eights: their blocks' scales and the codes.
+template <int VPT, bool VEC>
+__device__ __forceinline__ void ck_restore_row(const CkptRead& a, int64_t t, int base, int d, uint2 (&q)[VPT],
+                                               float (&s)[VPT]) {
     const int nb = (a.d + kCkptBlock - 1) / kCkptBlock;
-    q = ck_load_codes<VEC>(a.codes + t * a.d, c, d);
-    s = c < d ? __ldg(a.scales + t * nb + c / kCkptBlock) : 0.0f;
+    auto scales = [&] {
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            const int c = CK_COLUMN(base, k);
+            s[k] = c < d ? __ldg(a.scales + t * nb + c / kCkptBlock) : 0.0f;
+        }
+    };
+    if (!VEC) scales();  // before the codes are waited for
+    ck_codes_row<VPT, VEC>(a.codes + t * a.d, base, d, ck_inner(t, a.rows, a.d), q);
+    if (VEC) scales();
 }
 
 // The norm of x^, in rows of pitch ldo.  8192 x 8192 to bf16: 46 us (writing
 // alone takes 41).
 template <typename T, int VPT, bool VEC, bool WIDE>
-__global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, 4))
+__global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, VEC || sizeof(T) == 4 ? 4 : 2))
     ckpt_norm_kernel(const __grid_constant__ CkptRead a, T* __restrict__ out, int64_t ldo) {
     __shared__ float sh[2 * kCkptShared];
     extern __shared__ float4 ck_dyn[];
@@ -525,8 +672,7 @@ __global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, 4))
         uint2 q[VPT];
         float s[VPT], ss[1][VPT] = {}, sum[1];
         CK_SPANS(base, a.d) {
-#pragma unroll
-            for (int k = 0; k < VPT; ++k) ck_restore8<VEC>(a, t, CK_COLUMN(base, k), d, q[k], s[k]);
+            ck_restore_row<VPT, VEC>(a, t, base, d, q, s);
 #pragma unroll
             for (int k = 0; k < VPT; ++k) {
                 float x[8];
@@ -537,9 +683,7 @@ __global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, 4))
         ck_row_sum<1, VPT>(ss, sh, parity, sum);
         const float r = ck_rstd(sum[0], inv_d, a.eps);
         CK_SPANS(base, a.d) {
-            if (WIDE)
-#pragma unroll
-                for (int k = 0; k < VPT; ++k) ck_restore8<VEC>(a, t, CK_COLUMN(base, k), d, q[k], s[k]);
+            if (WIDE) ck_restore_row<VPT, VEC>(a, t, base, d, q, s);
 #pragma unroll
             for (int k = 0; k < VPT; ++k) {
                 float x[8], g[8];
@@ -601,8 +745,7 @@ __global__ void __launch_bounds__(1024 / VPT) ckpt_decode_kernel(const __grid_co
         const int d = t < a.rows ? a.d : 0;
         uint2 q[VPT];
         float s[VPT];
-#pragma unroll
-        for (int k = 0; k < VPT; ++k) ck_restore8<VEC>(a, t, CK_COLUMN(base, k), d, q[k], s[k]);
+        ck_restore_row<VPT, VEC>(a, t, base, d, q, s);
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
             float v[8];
@@ -654,11 +797,11 @@ struct CkptBack {
     const T* d_res;  // or null
     int64_t ld_res;
     T* dx;
-    float* part;  // d_gain of each row group: gridDim.x * blockDim.y rows of d
+    float* part;  // d_gain of each CTA: gridDim.x rows of d
 };
 
-// dx, and each row group's sum of d_gain (ckpt_gain_sum_kernel adds them in
-// their order).  A thread's sums lie in shared memory (dynamic, 4 bytes a
+// dx, and each CTA's sum of d_gain (ckpt_gain_sum_kernel adds them in their
+// order).  A thread's sums lie in shared memory (dynamic, 4 bytes a
 // feature and row of the CTA), those of WIDE in `part` itself; each element has
 // one thread.
 template <typename T, int VPT, bool VEC, bool WIDE>
@@ -669,7 +812,7 @@ __global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, 2))
     pdl_trigger();
     constexpr bool kShared = ck_shared_gain(VPT, WIDE);
     const float inv_d = 1.0f / (float)a.in.d;
-    float* part = a.part + ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * a.in.d;
+    float* part = a.part + (int64_t)blockIdx.x * a.in.d;
     float4* dg = ck_dyn + threadIdx.y * 2 * VPT * blockDim.x;
     float4* sg = ck_dyn + blockDim.y * 2 * VPT * blockDim.x;
     if (!WIDE)
@@ -693,17 +836,11 @@ __global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, 2))
         float s[VPT], acc[2][VPT] = {}, sum[2];
         Pack8<T> dy[VPT], res[VPT];
         auto read = [&](int base) {
-#pragma unroll
-            for (int k = 0; k < VPT; ++k) {
-                const int c = CK_COLUMN(base, k);
-                ck_restore8<VEC>(a.in, t, c, d, q[k], s[k]);
-                dy[k] = ck_load8<T, VEC>(a.dy + t * a.ld_dy, c, d);
-            }
+            ck_restore_row<VPT, VEC>(a.in, t, base, d, q, s);
+            ck_load_row<T, VPT, VEC>(a.dy + t * a.ld_dy, base, d, ck_inner(t, a.in.rows, a.in.d), dy);
         };
         auto read_res = [&](int base) {
-            if (a.d_res)
-#pragma unroll
-                for (int k = 0; k < VPT; ++k) res[k] = ck_load8<T, VEC>(a.d_res + t * a.ld_res, CK_COLUMN(base, k), d);
+            if (a.d_res) ck_load_row<T, VPT, VEC>(a.d_res + t * a.ld_res, base, d, ck_inner(t, a.in.rows, a.in.d), res);
         };
         CK_SPANS(base, a.in.d) {
             read(base);
@@ -770,22 +907,25 @@ __global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, 2))
             }
         }
     }
-    if (!WIDE)
+    if (WIDE) return;
+    __syncthreads();
+    for (int i = threadIdx.y * blockDim.x + threadIdx.x; i < 2 * VPT * (int)blockDim.x; i += blockDim.x * blockDim.y) {
+        const int x = i % (int)blockDim.x, kh = i / (int)blockDim.x;
+        const int c = 8 * (x + (kh >> 1) * (int)blockDim.x) + 4 * (kh & 1);
+        float4 p = ck_dyn[i];
+        for (int y = 1; y < (int)blockDim.y; ++y) {  // the rows of the CTA in their order
+            const float4 v = ck_dyn[y * 2 * VPT * blockDim.x + i];
+            p = make_float4(p.x + v.x, p.y + v.y, p.z + v.z, p.w + v.w);
+        }
+        if (VEC) {
+            if (c < a.in.d) *reinterpret_cast<float4*>(part + c) = p;
+        } else {
+            const float w[4] = {p.x, p.y, p.z, p.w};
 #pragma unroll
-        for (int k = 0; k < VPT; ++k)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int c = CK_COLUMN(0, k) + 4 * h;
-                const float4 p = ck_slot(dg, k, h);
-                if (VEC) {
-                    if (c < a.in.d) *reinterpret_cast<float4*>(part + c) = p;
-                } else {
-                    const float w[4] = {p.x, p.y, p.z, p.w};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (c + i < a.in.d) part[c + i] = w[i];
-                }
-            }
+            for (int e = 0; e < 4; ++e)
+                if (c + e < a.in.d) part[c + e] = w[e];
+        }
+    }
 }
 
 // The same for many rows of up to 16384 features (d a multiple of 16, every row
@@ -797,7 +937,7 @@ __global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, 2))
 // filled again.  A thread's d_gain sums stay in registers; at the end the
 // groups' are added in their order.  8192 x 8192 bf16 with the residual's
 // gradient: 94 us with the sum over the CTAs, 5.0 TB/s (rows through registers
-// instead: 133).  Sixteen warps an SM issue 55 % of the time; what is left is the
+// instead: 110).  Sixteen warps an SM issue 55 % of the time; what is left is the
 // wait between a row's two passes.  (A row ahead, its sums taken before the last
 // row's dx is written, costs more in registers and barriers than it hides: 109.)
 // WIDE: more than 8192 features, one group.  The residual's gradient goes
@@ -954,7 +1094,7 @@ __global__ void __launch_bounds__(kRingThreads, 1)
     }
 }
 
-// d_gain: 32 columns a CTA, its 32 warps every 32nd row group, then the warps
+// d_gain: 32 columns a CTA, its 32 warps every 32nd of the sums, then the warps
 // in their order.
 __global__ void __launch_bounds__(1024) ckpt_gain_sum_kernel(const float* part, int np, int d, float* d_gain) {
     __shared__ float sh[32][33];
