@@ -84,14 +84,15 @@ struct HeadPlan {
         np = 2 * (int)((vocab + (live_n ? 256 : bn) - 1) / (live_n ? 256 : bn));
         // buffers that a dH product's tail may need: two waves of tiles at most
         const int64_t pairs = pair_count(), tiles_m = n_pad / 256;
-        extra = std::min<int64_t>(2 * pairs, 15 * std::min<int64_t>(tiles_m * ((d + 255) / 256), pairs));
+        const int64_t most = std::min<int64_t>(pairs, (vocab + 511) / 512) - 1;  // ranges of 8 k-blocks past the first
+        extra = std::min<int64_t>(2 * pairs, most * std::min<int64_t>(tiles_m * ((d + 255) / 256), pairs));
         // a piece is a number of 256-entry tiles whose G fits beside them; of those, from the
         // largest down to half of it (64 are looked at), the one with the fewest waves of tiles over all pieces
         const int64_t all = (vocab + 255) / 256;
-        const int64_t most = std::max<int64_t>((kHeadPieceBytes - extra * 262144) / (512 * n_pad), 1);
-        int64_t best = most, least = INT64_MAX;
+        const int64_t fit = std::max<int64_t>((kHeadPieceBytes - extra * 262144) / (512 * n_pad), 1);
+        int64_t best = fit, least = INT64_MAX;
         auto waves = [&](int64_t tiles) { return (tiles * tiles_m + pairs - 1) / pairs; };
-        for (int64_t p = most; p >= std::max((most + 1) / 2, most - 64) && most < all; --p) {
+        for (int64_t p = fit; p >= std::max((fit + 1) / 2, fit - 64) && fit < all; --p) {
             const int64_t cost = all / p * waves(p) + waves(all % p);
             if (cost < least) {
                 least = cost;
@@ -245,8 +246,11 @@ int head_backward(const HeadPlan& p, const HeadWork& w, const void* weight, int6
         const HeadDh a{w.slab, p.dp, w.extra, pair_count(), p.tail_kb, p.live_n, w.pos, w.count, n, (int)d, w.out_scale,
                        static_cast<uint16_t*>(d_hidden), ld_dh};
         const unsigned cols = (unsigned)((d + 1023) / 1024);
-        const unsigned rows = (unsigned)std::min<int64_t>((n + 3) / 4, std::max<int64_t>(16 * num_sms() / cols, 1));
-        AETH_CUDA(launch_after(head_dh_kernel<BF16>, dim3(rows, cols), dim3(128), 0, st, 1, a));
+        const int64_t rows = std::max<int64_t>(16 * num_sms() / cols, 1);
+        // few tokens: one at a time, and more of its parts
+        if (n <= rows) AETH_CUDA(launch_after(head_dh_kernel<BF16, 1>, dim3((unsigned)n, cols), dim3(128), 0, st, 1, a));
+        else AETH_CUDA(launch_after(head_dh_kernel<BF16, 4>, dim3((unsigned)std::min((n + 3) / 4, rows), cols), dim3(128), 0,
+                                    st, 1, a));
     }
     return AETH_OK;
 }

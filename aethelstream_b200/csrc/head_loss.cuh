@@ -715,7 +715,7 @@ struct HeadGradT {
 
 // dH of every token in 16 bits: the slab's row, plus the further K ranges of
 // the tail's tiles in their order; zero for the tokens that took no part.  A
-// CTA takes 1024 columns of tokens, four of them in flight.
+// CTA takes 1024 columns of tokens, TOKENS of them in flight.
 struct HeadDh {
     const float* slab;
     int64_t ld;
@@ -728,11 +728,11 @@ struct HeadDh {
     uint16_t* out;
     int64_t ldo;
 };
-template <bool BF16>
+template <bool BF16, int TOKENS>
 __global__ void __launch_bounds__(128) head_dh_kernel(const HeadDh a) {
     __shared__ int sh[5];
     pdl_wait();
-    if (threadIdx.x == 0) {
+    if (threadIdx.x < 32) {
         const int count = *a.count, tiles_d = (a.d + 255) / 256;
         const int bt = a.live_n ? pair_live_bn(count) : 256, tiles_t = max((count + bt - 1) / bt, 1);
         const PairTail t(tiles_t * tiles_d, a.pairs, a.tail_kb);
@@ -748,11 +748,11 @@ __global__ void __launch_bounds__(128) head_dh_kernel(const HeadDh a) {
     const int c = (blockIdx.y * 128 + threadIdx.x) * 8;
     if (c >= a.d) return;
     const bool whole = (a.ldo % 8) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && c + 8 <= a.d;
-    for (int64_t t0 = blockIdx.x; t0 < a.n; t0 += 4 * (int64_t)gridDim.x) {
-        float4 v[4][2];
-        int p[4];
+    for (int64_t t0 = blockIdx.x; t0 < a.n; t0 += TOKENS * (int64_t)gridDim.x) {
+        float4 v[TOKENS][2];
+        int p[TOKENS];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < TOKENS; ++k) {
             const int64_t t = t0 + (int64_t)k * gridDim.x;
             p[k] = t < a.n ? a.pos[t] : kHeadIgnored;
 #pragma unroll
@@ -761,7 +761,7 @@ __global__ void __launch_bounds__(128) head_dh_kernel(const HeadDh a) {
                                     : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < TOKENS; ++k) {
             const int64_t t = t0 + (int64_t)k * gridDim.x;
             if (t >= a.n) break;
             if (p[k] >= 0) {
@@ -769,7 +769,7 @@ __global__ void __launch_bounds__(128) head_dh_kernel(const HeadDh a) {
                                         : pair_tile_index(p[k] / bt, c / 256, tiles_t, tiles_d)) - full;
                 if (i >= 0) {
                     const float* e = a.extra + ((int64_t)i * 256 + p[k] % bt) * 256 + c % 256;
-#pragma unroll 4
+#pragma unroll(TOKENS == 1 ? 12 : 4)
                     for (int s = 0; s + 1 < splits; ++s)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {

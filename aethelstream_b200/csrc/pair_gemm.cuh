@@ -84,25 +84,33 @@ __host__ __device__ inline int pair_live_bn(int n) {
 }
 
 // Tiles that do not fill a wave of CTA pairs.  `full` tiles run whole; the
-// `rest` (fewer than a wave) are split into `splits` K ranges each, as many as
-// make their waves shortest: ceil(rest splits / pairs) / splits of a tile's
-// time, a range being 8 k-blocks at least and its extra output counted as 1 %.
-// The first range of a tile goes where whole tiles go, the others to buffers
-// of their own ((splits - 1) * rest <= 2 pairs of them).
+// `rest` (fewer than a wave) are split into `splits` K ranges each, what makes
+// their time least: in k-blocks, waves * ceil(kb / splits), and a fifth of one
+// for each range's output, which is written and added up.  A range is 8 k-blocks
+// at least.  The first range of a tile goes where whole tiles go, the others to
+// buffers of their own ((splits - 1) * rest <= 2 pairs of them).  In whole
+// numbers, so that host and device agree; on the device by whole warps.
 struct PairTail {
     int full, rest, splits;
+    __host__ __device__ static uint32_t cost(int s, int rest, int pairs, int kb) {  // and s in the low 8 bits
+        if (s > 1 && (s * 8 > kb || (s - 1) * rest > 2 * pairs)) return 0xffffffffu;
+        const int per = ((kb < 1 << 19 ? kb : 1 << 19) + s - 1) / s;
+        return (uint32_t)(5 * ((rest * s + pairs - 1) / pairs) * per + s * rest) * 256u + (uint32_t)s;
+    }
+    __host__ __device__ static int most(int pairs) { return pairs < 255 ? pairs : 255; }
     __host__ __device__ PairTail(int tiles, int pairs, int kb) {
         full = tiles / pairs * pairs;
         rest = tiles - full;
         splits = 1;
-        int least = 101;  // (waves / s + s / 100) * 100 s, in whole numbers: host and device agree
-        for (int s = 2; s <= 16 && rest > 0; ++s) {
-            if (s * 8 > kb || (s - 1) * rest > 2 * pairs) break;
-            const int cost = 100 * ((rest * s + pairs - 1) / pairs) + s * s;
-            if (cost * splits < least * s) {
-                least = cost;
-                splits = s;
-            }
+        if (rest > 0) {
+            uint32_t least = 0xffffffffu;
+#ifdef __CUDA_ARCH__
+            for (int s = 1 + (int)(threadIdx.x & 31); s <= most(pairs); s += 32) least = min(least, cost(s, rest, pairs, kb));
+            least = __reduce_min_sync(0xffffffffu, least);
+#else
+            for (int s = 1; s <= most(pairs) && (s == 1 || s * 8 <= kb); ++s) least = std::min(least, cost(s, rest, pairs, kb));
+#endif
+            splits = (int)(least & 255u);
         }
         const int per = (kb + splits - 1) / splits;
         splits = (kb + per - 1) / per;  // no empty range
