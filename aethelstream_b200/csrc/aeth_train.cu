@@ -59,8 +59,8 @@ int head_bn(int64_t tiles_m, int64_t cols) {
 // Whether the tokens are the products' columns (pair_gemm.cuh): where tiles of
 // 256 rows would be a tenth larger than the columns that cover the tokens, and
 // masks may leave fewer still.  Measured at d 4096, vocabulary 32000, forward
-// and backward, rows against columns: 16 tokens 70.6 + 187.5 and 65.6 + 180.8
-// us; 300: 101 + 284 and 93 + 259; but 256: 72 + 216 and 75 + 220 (the blocks
+// and backward, rows against columns: 16 tokens 70.6 + 187.5 and 58 + 170
+// us; 300: 101 + 284 and 89 + 257; but 256: 72 + 216 and 75 + 220 (the blocks
 // are turned over in the epilogue), 512: 108 + 325 and 118 + 329.
 bool head_tokens_as_columns(int64_t n) {
     if (n > 1024) return false;

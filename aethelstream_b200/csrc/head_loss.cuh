@@ -289,6 +289,7 @@ __device__ __forceinline__ void head_slice(const float (&acc)[128], int c, float
 // maximum and sum, and the label's logit where it lies here.
 struct HeadStats {
     static constexpr int kChunk = 8;  // the loss is an fp32 result: see pair_gemm.cuh
+    static constexpr bool kLiveN = false;
     const int* lab;
     float* label_logit;
     float2* part;  // [2 * n_tile + half][row]
@@ -318,6 +319,7 @@ struct HeadStats {
 // join theirs through shared memory.
 struct HeadStatsT {
     static constexpr int kChunk = 8;
+    static constexpr bool kLiveN = true;
     const int* lab;
     float* label_logit;
     float2* part;  // [2 * m_tile + CTA of the pair][row]
@@ -445,7 +447,7 @@ __global__ void __launch_bounds__(512) head_loss_kernel(const HeadLoss a) {
 // end (512 bytes an instruction, sixteen in flight), against the tokens' hidden
 // states in shared memory; it keeps their running maximum and sum and leaves
 // one pair per token and CTA.  One token x 4096 x 32000: 46 us a call, 5.7 TB/s
-// (6.3 at 2048 x 131071); the tile product takes 64, its columns of 128 bytes
+// (6.3 at 2048 x 131071); the tile product takes 57, its columns of 128 bytes
 // and its launches included.
 constexpr int kHeadVecTokens = 4, kHeadVecThreads = 512;
 
@@ -615,6 +617,7 @@ __global__ void __launch_bounds__(32 * kHeadVecTokens)
 template <bool BF16>
 struct HeadGrad {
     static constexpr int kChunk = 0;
+    static constexpr bool kLiveN = false;
     const int* lab;
     const float* coef;
     const float* lse2;
@@ -657,6 +660,7 @@ struct HeadGrad {
 template <bool BF16>
 struct HeadGradT {
     static constexpr int kChunk = 0;
+    static constexpr bool kLiveN = true;
     const int* lab;
     const float* coef;
     const float* lse2;

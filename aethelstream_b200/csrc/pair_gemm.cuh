@@ -32,7 +32,12 @@
 //
 // Few live rows are taken as N, not M: M comes in tiles of 256 only, N in
 // multiples of 32, so 311 rows cost two tiles of 160 and not two of 256, and a
-// handful of rows leaves a product bound by the other operand's bytes.  The
+// handful of rows leaves a product bound by the other operand's bytes.  Their
+// smaller stages make up to ten of six: a k-block of 320 MMA cycles (N = 160)
+// took 530 with six stages, whose copies were not far enough ahead of the MMAs
+// (tensor pipe 52 % active, DRAM 44 %; 300 x 4096 x 32000, forward and backward:
+// 95 + 274 us with six, 89 + 257 with seven; 16 tokens, ten: 63 + 176 and 58 +
+// 170).  The
 // tile's columns are then the rows of the result, and epilogues turn each
 // 32 x 32 block over in shared memory (pair_transpose).
 // Tiles are walked in groups of row tiles so that the tiles in flight
@@ -51,6 +56,7 @@ constexpr int kPairThreads = 32 * (1 + kPairProducers + kPairEpiWarps);
 constexpr int kPairStages = 6;
 constexpr int kPairOperand = 128 * 64 * 2;                  // one operand of one stage and CTA
 constexpr int kPairStage = 2 * kPairOperand;
+constexpr int kPairMaxStages = 10;  // of narrow tiles, whose B takes less
 constexpr int kPairStaging = 32 * 128;                      // per epilogue warp: 32 rows x 128 bytes
 constexpr int kPairBar = 256;
 constexpr int kPairSmem = 1024 + kPairStages * kPairStage + kPairEpiWarps * kPairStaging + kPairBar;
@@ -60,13 +66,14 @@ constexpr int kPairSmem = 1024 + kPairStages * kPairStage + kPairEpiWarps * kPai
 // 32 row tiles (8192 x 8192 x 32000): of 8 3215 + 9481, of 16 3248 + 9841, of 4
 // 3361 + 9764.
 __host__ __device__ inline int pair_group(int tiles_m) { return tiles_m <= 16 ? tiles_m : 8; }
-constexpr int kLiveBox = 64;  // rows of B a copy with a live N: the last one brings rows that no MMA reads
+constexpr int kLiveBox = 64;  // rows of B a copy with a live N (boxes of 16 alone took 20 to 40 % longer)
 
 enum PairLive { PAIR_LIVE_NONE = 0, PAIR_LIVE_M = 1, PAIR_LIVE_K = 2, PAIR_LIVE_N = 3 };
 
 struct PairGemm {
     CUtensorMap tmA;  // K-major: box 64 (K) x 128; MN-major: box 64 (M) x 64 (K)
     CUtensorMap tmB;  // K-major: box 64 (K) x bn / 2, or x kLiveBox with a live N; MN-major: box 64 (N) x 64 (K)
+    CUtensorMap tmB16;  // with a live N: box 64 (K) x 16
     const int* live;  // device count that replaces M, N or K
     int live_dim;     // PairLive
     int M, N, K;
@@ -222,22 +229,20 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);  // stays a shared pointer
     uint8_t* sA = base;
-    uint8_t* sB = base + kPairStages * kPairOperand;
     uint8_t* staging = base + kPairStages * kPairStage;
     uint64_t* full = reinterpret_cast<uint64_t*>(staging + kPairEpiWarps * kPairStaging);
-    uint64_t* empty = full + kPairStages;
-    uint64_t* acc_full = empty + kPairStages;
+    uint64_t* empty = full + kPairMaxStages;
+    uint64_t* acc_full = empty + kPairMaxStages;
     uint64_t* acc_empty = acc_full + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    static_assert((2 * kPairStages + 4) * 8 + 8 <= kPairBar, "barriers must fit the barrier area");
-    static_assert(kPairStages % kPairProducers == 0, "every stage has one producer");
+    static_assert((2 * kPairMaxStages + 4) * 8 + 8 <= kPairBar, "barriers must fit the barrier area");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int crank = (int)cluster_ctarank();
     const int ustart = (int)(blockIdx.x >> 1), ustep = (int)(gridDim.x >> 1);
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kPairStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < kPairMaxStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         // acc_empty (CTA 0): one arrival per epilogue warp of both CTAs
         for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * kPairEpiWarps); }
         *abort = 0;
@@ -253,12 +258,18 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
     pdl_trigger();
     const PairShape sh(g);
     constexpr int kStep = Epi::kChunk > 0 ? Epi::kChunk : 1 << 30;  // k-blocks per accumulator
+    // Rows of B a stage: with a live N in boxes of 64 (a rest of 48 too) and of 16;
+    // what they leave free makes more stages.
+    constexpr bool kLive = Epi::kLiveN;
+    const int half_n = sh.bn / 2;
+    const int rows64 = kLive ? (half_n + 16) / kLiveBox * kLiveBox : half_n, rows_b = max(rows64, half_n);
+    const int b_bytes = kLive ? rows_b * 128 : kPairOperand;
+    const int stages = kLive ? min(kPairStages * kPairStage / (kPairOperand + b_bytes), kPairMaxStages) : kPairStages;
+    uint8_t* sB = base + stages * kPairOperand;
 
     if (warp == 0 || warp >= 2 + kPairEpiWarps) {
         if (elect_one()) {
             const int me = warp == 0 ? 0 : warp - 1 - kPairEpiWarps;
-            const int half_n = sh.bn / 2;
-            const int rows_b = g.live_dim == PAIR_LIVE_N ? (half_n + kLiveBox - 1) / kLiveBox * kLiveBox : half_n;
             const uint32_t bytes = 2u * (uint32_t)(kPairOperand + rows_b * 64 * 2);  // both CTAs
             int s = me, lag = me, issued = 0;  // this producer's next stage; k-blocks until its next turn
             uint32_t ph = 1;
@@ -270,7 +281,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
                     if (!mbar_wait(&empty[s], ph, abort, err, DEVERR_TIMEOUT_TMA)) break;
                     if (crank == 0) mbar_arrive_expect_tx(&full[s], bytes);
                     uint8_t* a = sA + s * kPairOperand;
-                    uint8_t* b = sB + s * kPairOperand;
+                    uint8_t* b = sB + s * b_bytes;
                     if (A_MN) {
                         tma_load_2d_pair(a, &g.tmA, &full[s], m0, kb * 64);
                         tma_load_2d_pair(a + 8192, &g.tmA, &full[s], m0 + 64, kb * 64);
@@ -280,14 +291,15 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
                     if (B_MN) {
                         for (int c = 0; c < half_n; c += 64)
                             tma_load_2d_pair(b + c * 128, &g.tmB, &full[s], n0 + c, kb * 64);
-                    } else if (g.live_dim == PAIR_LIVE_N) {
-                        for (int c = 0; c < half_n; c += kLiveBox) tma_load_2d_pair(b + c * 128, &g.tmB, &full[s], kb * 64, n0 + c);
+                    } else if (kLive) {
+                        for (int c = 0; c < rows64; c += kLiveBox) tma_load_2d_pair(b + c * 128, &g.tmB, &full[s], kb * 64, n0 + c);
+                        for (int c = rows64; c < half_n; c += 16) tma_load_2d_pair(b + c * 128, &g.tmB16, &full[s], kb * 64, n0 + c);
                     } else {
                         tma_load_2d_pair(b, &g.tmB, &full[s], kb * 64, n0);
                     }
                     ++issued;
-                    if ((s += kPairProducers) >= kPairStages) {
-                        s = me;
+                    if ((s += kPairProducers) >= stages) {
+                        s -= stages;
                         ph ^= 1u;
                     }
                 }
@@ -295,10 +307,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
             }
             // a wait gave up: the loads in flight get a last, bounded chance to land
             if (*abort && crank == 0)
-                for (int i = max(issued - kPairStages / kPairProducers, 0); i < issued; ++i) {
-                    const int w = me + i % (kPairStages / kPairProducers) * kPairProducers;
-                    const uint32_t p = (uint32_t)(i / (kPairStages / kPairProducers)) & 1u;
-                    for (int n = 0; n < 1000 && !mbar_try_wait(&full[w], p); ++n) {}
+                for (int i = max(issued - (stages + kPairProducers - 1) / kPairProducers, 0); i < issued; ++i) {
+                    const int kb = me + i * kPairProducers;  // of all that this pair went through
+                    for (int n = 0; n < 1000 && !mbar_try_wait(&full[kb % stages], (uint32_t)(kb / stages) & 1u); ++n) {}
                 }
         }
     } else if (warp == 1) {
@@ -321,12 +332,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
                         if (!mbar_wait(&full[s], ph, abort, err, DEVERR_TIMEOUT_MMA)) break;
                         tc_fence_after();
                         const uint64_t da = da0 + (uint64_t)(s * (kPairOperand / 16));
-                        const uint64_t db = db0 + (uint64_t)(s * (kPairOperand / 16));
+                        const uint64_t db = db0 + (uint64_t)(s * (b_bytes / 16));
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
                             umma_f16_ss_pair(d, da + kk * kStepA, db + kk * kStepB, idesc, (kb > kb0 || kk > 0) ? 1u : 0u);
                         umma_commit_pair(&empty[s]);
-                        if (++s == kPairStages) {
+                        if (++s == stages) {
                             s = 0;
                             ph ^= 1u;
                         }
@@ -461,6 +472,7 @@ __device__ __forceinline__ void pair_store16(const PairTile& t, const uint32_t (
 template <bool BF16>
 struct PairOut16 {
     static constexpr int kChunk = 0;
+    static constexpr bool kLiveN = false;
     uint16_t* out;
     int64_t ld;
     const float* scale;  // device; null: 1
@@ -517,6 +529,7 @@ __device__ __forceinline__ void pair_store32(const PairTile& t, const float (&v)
 template <bool BF16>
 struct PairSplit16 {
     static constexpr int kChunk = 0;
+    static constexpr bool kLiveN = false;
     PairOut16<BF16> whole;
     float* buffers;  // range s of split tile i: s * rest + i
     int rest;
@@ -582,6 +595,7 @@ __global__ void __launch_bounds__(256) pair_join_kernel(const PairJoin a) {
 // order of the launches.
 struct PairSlab {
     static constexpr int kChunk = 0;
+    static constexpr bool kLiveN = false;
     float* slab;
     int64_t ld;  // a multiple of 4
     float* extra;
@@ -606,6 +620,7 @@ struct PairSlab {
 // by 256 rows each.
 struct PairSlabT {
     static constexpr int kChunk = 0;
+    static constexpr bool kLiveN = true;
     float* slab;
     int64_t ld;  // at least M
     float* extra;
@@ -647,9 +662,11 @@ int pair_gemm_launch(PairOperand A, PairOperand B, int M, int N, int K, const in
     AETH_TRY(runtime_for_current(&rt));
     PairGemm g;
     AETH_TRY(make_tmap_16b(&g.tmA, A.ptr, (uint64_t)A.cols, (uint64_t)A.rows, A.ld, 64, A_MN ? 64 : 128, bf16));
-    const bool live_n = live_dim == PAIR_LIVE_N;
+    constexpr bool live_n = Epi::kLiveN;
+    if (live_n != (live_dim == PAIR_LIVE_N)) return AETH_ERR_ARG;
     AETH_TRY(make_tmap_16b(&g.tmB, B.ptr, (uint64_t)B.cols, (uint64_t)B.rows, B.ld, 64,
                            B_MN ? 64 : live_n ? kLiveBox : bn / 2, bf16));
+    if (live_n) AETH_TRY(make_tmap_16b(&g.tmB16, B.ptr, (uint64_t)B.cols, (uint64_t)B.rows, B.ld, 64, 16, bf16));
     g.live = live;
     g.live_dim = live_dim;
     g.M = M;
