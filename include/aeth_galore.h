@@ -569,7 +569,9 @@ int aeth_rms_norm_checkpoint_backward(const void* dy, int64_t ld_dy, const int8_
 /* Weight gradient of a linear layer whose input is kept in 8 bits:
  * d_weight (m x d) = dy^T X, dy rows x m, X the restored checkpoint, or its RMS
  * norm times gain where gain is not NULL.  X is rounded to dtype (F16 or BF16)
- * for the tensor cores.  dy 16-byte aligned with ld_dy % 8 == 0. */
+ * for the tensor cores.  dy 16-byte aligned with ld_dy % 8 == 0.  The workspace
+ * holds X in 16 bits and, where few tiles are split along the rows, at most
+ * 56 MiB of partial sums. */
 int aeth_checkpoint_weight_grad_workspace(int64_t rows, int64_t m, int64_t d, size_t* bytes);
 int aeth_checkpoint_weight_grad(const void* dy, int64_t ld_dy, const int8_t* codes, const float* scales,
                                 const void* gain, int gain_dtype, float eps, int dtype, int64_t rows, int64_t m,
