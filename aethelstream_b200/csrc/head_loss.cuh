@@ -324,9 +324,12 @@ struct HeadStatsT {
     float* label_logit;
     float2* part;  // [2 * m_tile + CTA of the pair][row]
     int64_t ld_part;
-    __device__ static void give_up(const PairTile& t) {  // the two barriers of finish()
+    // The two barriers of finish(), each with an id of its own: a barrier counts
+    // arrivals, so two at one id could both fall into its first wait.  A warp that
+    // leaves waits for nobody, since the others may never come to its next tile's.
+    __device__ static void give_up(const PairTile& t) {
         named_bar_arrive(1 + t.half, 128);
-        named_bar_arrive(1 + t.half, 128);
+        named_bar_arrive(3 + t.half, 128);
     }
     __device__ __forceinline__ void finish(const PairTile& t, const float (&acc)[128]) const {
         const int left = t.M - t.row0;  // entries of this warp that exist
@@ -357,7 +360,7 @@ struct HeadStatsT {
         const int col = t.c_begin + 32 * e + t.lane;
         if (col < t.c_end && t.col0 + col < t.N)
             part[(int64_t)(2 * t.m_tile + (t.tile_row >> 7)) * ld_part + t.col0 + col] = x;
-        named_bar(1 + t.half, 128);
+        named_bar(3 + t.half, 128);
     }
 };
 
