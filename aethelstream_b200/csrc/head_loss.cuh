@@ -616,10 +616,15 @@ __global__ void __launch_bounds__(32 * kHeadVecTokens)
 }
 
 // Epilogue of the backward's product: G of the piece in 16 bits.  G is rounded
-// once, from fp32; rows from the count to the tile's end (or n) become zero.
+// once, from fp32; rows from the count to the tile's end (or n) become zero.  The
+// logits are added up as in the forward, so that they are those that lse came
+// from: taken whole, one of 30 made of 8192 products is 2.3e-4 too small, which
+// is all of p - 1 for a label known with p = 0.9998.  That costs 1.4 to 2.4 % of a
+// large backward (8192 x 8192 x 32000: 10.03 -> 10.18 ms, power-capped; 3584 x 4096
+// x 32000: 2.13 -> 2.19) and 6 to 13 us of one of 130 to 311 tokens (160 to 260 us).
 template <bool BF16>
 struct HeadGrad {
-    static constexpr int kChunk = 0;
+    static constexpr int kChunk = 8;
     static constexpr bool kLiveN = false;
     const int* lab;
     const float* coef;
@@ -628,32 +633,33 @@ struct HeadGrad {
     int64_t ldg;
     int n;   // rows of g: the tokens
     int v0;  // first vocabulary entry of the piece
-    __device__ __forceinline__ void tile(const PairTile& t) const {
+    __device__ static void give_up(const PairTile&) {}
+    __device__ __forceinline__ void finish(const PairTile& t, const float (&acc)[128]) const {
         const int row = t.row0 + t.lane;
         const bool in = row < t.M;
         const float f = in ? coef[row] : 0.0f, l2 = in ? lse2[row] : 0.0f;
-        const int lab_c = in ? lab[row] - v0 - t.col0 : -1;
-        for (int c = t.c_begin; c < t.c_end; c += 64) {
-            if (t.col0 + c >= t.N || t.row0 >= n) break;
-            uint32_t w[32];
+        const int lab_c = in ? lab[row] - v0 - t.col0 - t.c_begin : -1;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float v[32];
-                if (c + 32 * h < t.c_end) {
-                    tmem_ld32<0>(t.tmem + (uint32_t)(c + 32 * h), v);
-                    tmem_wait_ld();
+        for (int b = 0; b < 2; ++b) {
+            const int c = t.c_begin + 64 * b;
+            if (c < t.c_end && t.col0 + c < t.N && t.row0 < n) {
+                uint32_t w[32];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float v[32];
+                    head_slice(acc, 2 * b + h, v);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = ex2(fmaf(v[i], kLog2e, -l2));
+                    const int k = lab_c - 64 * b - 32 * h;
+                    if (__any_sync(0xffffffffu, k >= 0 && k < 32)) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = k == i ? v[i] - head_g_scale(BF16) : v[i];
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) w[16 * h + i] = pack16<BF16>(v[2 * i] * f, v[2 * i + 1] * f);
                 }
-#pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = ex2(fmaf(v[i], kLog2e, -l2));
-                const int k = lab_c - c - 32 * h;
-                if (__any_sync(0xffffffffu, k >= 0 && k < 32)) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = k == i ? v[i] - head_g_scale(BF16) : v[i];
-                }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) w[16 * h + i] = pack16<BF16>(v[2 * i] * f, v[2 * i + 1] * f);
+                pair_store16(t, w, c, g, ldg, n, min(t.N, t.col0 + t.c_end));
             }
-            pair_store16(t, w, c, g, ldg, n, min(t.N, t.col0 + t.c_end));
         }
     }
 };
@@ -662,7 +668,7 @@ struct HeadGrad {
 // so that a thread has a token and 32 entries.
 template <bool BF16>
 struct HeadGradT {
-    static constexpr int kChunk = 0;
+    static constexpr int kChunk = 8;
     static constexpr bool kLiveN = true;
     const int* lab;
     const float* coef;
@@ -671,13 +677,15 @@ struct HeadGradT {
     int64_t ldg;
     int n;
     int v0;
-    __device__ __forceinline__ void tile(const PairTile& t) const {
+    __device__ static void give_up(const PairTile&) {}
+    __device__ __forceinline__ void finish(const PairTile& t, const float (&acc)[128]) const {
         const bool whole = (ldg % 8) == 0 && (reinterpret_cast<uintptr_t>(g) & 15) == 0;
-        for (int c = t.c_begin; c < t.c_end; c += 32) {
-            if (t.row0 >= t.M || t.col0 + c >= n) break;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int c = t.c_begin + 32 * b;
+            if (c >= t.c_end || t.row0 >= t.M || t.col0 + c >= n) continue;
             float v[32];
-            tmem_ld32<0>(t.tmem + (uint32_t)c, v);
-            tmem_wait_ld();
+            head_slice(acc, b, v);
             pair_transpose(t, v);
             const int token = t.col0 + c + t.lane;
             const bool in = token < t.N;

@@ -21,7 +21,10 @@
 // An epilogue may take the accumulator in pieces of kChunk k-blocks and add
 // them up in registers (Epi::kChunk > 0).  The tensor cores cut every partial
 // sum off toward zero, which shrinks a sum of K products by about K * 1e-9 of
-// itself (measured: 3.8e-6 at K = 4096); pieces of 512 keep that at 4e-7.
+// itself (measured: 3.8e-6 at K = 4096); pieces of 512 keep that at 4e-7.  Tiles
+// of at most 160 columns have TMEM for three or four accumulators instead of two,
+// so that the MMAs go on while the epilogue ends a tile (300 and 512 tokens x 4096
+// x 32000, forward: 88.5 -> 86 and 117 -> 109 us).
 //
 // Measured, 3584 x 4096 x 32000 bf16: 561-591 us a product (1.59-1.68 PF/s at the
 // 1.5 GHz that the power cap leaves), tensor pipe 97-98 % active: the clock
@@ -57,6 +60,7 @@ constexpr int kPairStages = 6;
 constexpr int kPairOperand = 128 * 64 * 2;                  // one operand of one stage and CTA
 constexpr int kPairStage = 2 * kPairOperand;
 constexpr int kPairMaxStages = 10;  // of narrow tiles, whose B takes less
+constexpr int kPairMaxAcc = 4;  // accumulators in TMEM
 constexpr int kPairStaging = 32 * 128;                      // per epilogue warp: 32 rows x 128 bytes
 constexpr int kPairBar = 256;
 constexpr int kPairSmem = 1024 + kPairStages * kPairStage + kPairEpiWarps * kPairStaging + kPairBar;
@@ -233,10 +237,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
     uint64_t* full = reinterpret_cast<uint64_t*>(staging + kPairEpiWarps * kPairStaging);
     uint64_t* empty = full + kPairMaxStages;
     uint64_t* acc_full = empty + kPairMaxStages;
-    uint64_t* acc_empty = acc_full + 2;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    uint64_t* acc_empty = acc_full + kPairMaxAcc;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + kPairMaxAcc);
     volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    static_assert((2 * kPairMaxStages + 4) * 8 + 8 <= kPairBar, "barriers must fit the barrier area");
+    static_assert((2 * kPairMaxStages + 2 * kPairMaxAcc) * 8 + 8 <= kPairBar, "barriers must fit the barrier area");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int crank = (int)cluster_ctarank();
@@ -244,7 +248,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
     if (threadIdx.x == 0) {
         for (int s = 0; s < kPairMaxStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         // acc_empty (CTA 0): one arrival per epilogue warp of both CTAs
-        for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * kPairEpiWarps); }
+        for (int b = 0; b < kPairMaxAcc; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * kPairEpiWarps); }
         *abort = 0;
         fence_mbar_init();
     }
@@ -266,6 +270,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
     const int b_bytes = kLive ? rows_b * 128 : kPairOperand;
     const int stages = kLive ? min(kPairStages * kPairStage / (kPairOperand + b_bytes), kPairMaxStages) : kPairStages;
     uint8_t* sB = base + stages * kPairOperand;
+    const int acc_cols = kLive ? sh.bn : 256, accs = kLive ? min(512 / acc_cols, kPairMaxAcc) : 2;
 
     if (warp == 0 || warp >= 2 + kPairEpiWarps) {
         if (elect_one()) {
@@ -319,15 +324,15 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
             const uint64_t da0 = sdesc_sw128(smem_u32(sA), A_MN ? 8192 : 16, 1024);
             const uint64_t db0 = sdesc_sw128(smem_u32(sB), B_MN ? 8192 : 16, 1024);
             constexpr uint64_t kStepA = (A_MN ? 2048 : 32) / 16, kStepB = (B_MN ? 2048 : 32) / 16;
-            int s = 0, j = 0;
-            uint32_t ph = 0;
+            int s = 0, b = 0;
+            uint32_t ph = 0, acc_ph = 1;
             for (int u = ustart; u < sh.total && !*abort; u += ustep) {
                 const PairUnit t = sh.unit(u);
-                for (int kb0 = t.kb0; kb0 < t.kb1 && !*abort; kb0 += kStep, ++j) {
-                    const int b = j & 1, kb1 = min(kb0 + kStep, t.kb1);
-                    if (!mbar_wait(&acc_empty[b], ((uint32_t)(j >> 1) & 1u) ^ 1u, abort, err, DEVERR_TIMEOUT_MMA)) break;
+                for (int kb0 = t.kb0; kb0 < t.kb1 && !*abort; kb0 += kStep) {
+                    const int kb1 = min(kb0 + kStep, t.kb1);
+                    if (!mbar_wait(&acc_empty[b], acc_ph, abort, err, DEVERR_TIMEOUT_MMA)) break;
                     tc_fence_after();
-                    const uint32_t d = tmem + (uint32_t)(b * 256);
+                    const uint32_t d = tmem + (uint32_t)(b * acc_cols);
                     for (int kb = kb0; kb < kb1; ++kb) {
                         if (!mbar_wait(&full[s], ph, abort, err, DEVERR_TIMEOUT_MMA)) break;
                         tc_fence_after();
@@ -343,6 +348,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
                         }
                     }
                     umma_commit_pair(&acc_full[b]);
+                    if (++b == accs) {
+                        b = 0;
+                        acc_ph ^= 1u;
+                    }
                 }
             }
         }
@@ -359,19 +368,24 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
         tile.staging = staging + ew * kPairStaging;
         tile.lane = lane;
         tile.warp = ew;
-        auto next = [&](int j) {  // waits for accumulator j
-            const bool here = mbar_wait(&acc_full[j & 1], (uint32_t)(j >> 1) & 1u, abort, err, DEVERR_TIMEOUT_EPI) && !*abort;
+        int b = 0;
+        uint32_t acc_ph = 0;
+        auto next = [&] {  // waits for the next accumulator
+            const bool here = mbar_wait(&acc_full[b], acc_ph, abort, err, DEVERR_TIMEOUT_EPI) && !*abort;
             if (!__all_sync(0xffffffffu, here)) return false;
             tc_fence_after();
-            tile.tmem = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)((j & 1) * 256);
+            tile.tmem = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(b * acc_cols);
             return true;
         };
-        auto release = [&](int j) {
+        auto release = [&] {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(smem_leader(&acc_empty[j & 1]));
+            if (lane == 0) mbar_arrive_cluster(smem_leader(&acc_empty[b]));
+            if (++b == accs) {
+                b = 0;
+                acc_ph ^= 1u;
+            }
         };
-        int j = 0;
         bool ok = true;
         for (int u = ustart; u < sh.total && ok; u += ustep) {
             const PairUnit t = sh.unit(u);
@@ -386,19 +400,19 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
                 float acc[128];
 #pragma unroll
                 for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
-                for (int kb0 = t.kb0; kb0 < t.kb1; kb0 += kStep, ++j) {
-                    if (!(ok = next(j))) break;
+                for (int kb0 = t.kb0; kb0 < t.kb1; kb0 += kStep) {
+                    if (!(ok = next())) break;
                     pair_accumulate(tile, acc);
-                    release(j);
+                    release();
                 }
                 if (ok) epi.finish(tile, acc);
                 // a warp that gave up arrives where the others may wait for it; they see
                 // `abort` before their next tile
                 else Epi::give_up(tile);
             } else if (t.kb0 < t.kb1) {
-                if (!(ok = next(j))) break;
+                if (!(ok = next())) break;
                 epi.tile(tile);
-                release(j++);
+                release();
             }
         }
     }

@@ -346,3 +346,48 @@ def test_a_token_weight_that_is_not_finite():
 def test_many_tokens(n):
     """Around the number of labels that one scan takes."""
     check(*make(n, 64, 300, torch.bfloat16, seed=15, masked=0.3))
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [5, 40, 256, 700])
+def test_gradient_of_tokens_that_are_known(n, dt):
+    """Logits of 30 made of 8192 products of one sign, labels known with p = 0.999
+    (a second entry close behind) or p = 1 to ten digits: G's label entry is p - 1,
+    and its row adds up to zero.  A constant feature of the weight shows that sum
+    in d_hidden.
+
+    Bounds: loss and gradient make the same sums, in fp32 pieces of 512 products,
+    each within c = 2e-6 of sum |h w| = S (the tensor cores' 512 * 1e-9, and 16
+    additions); p of such logits is within p (1 - p) 2 c S.  lse is rounded at four
+    places, and the exponentials and the logarithm are within 2^-20: p e_x.  G and
+    the output are rounded once."""
+    import aethelstream_b200 as A
+    d, v = 8192, 600
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    w = torch.randn(v, d, generator=gen, device="cuda") * (2.0 / d ** 0.5)
+    w[250:500] = 0.77 * w[:250]
+    w[:, 0] = 1.0
+    w = w.to(dt)
+    lab = torch.randint(0, 350, (n,), generator=gen, device="cuda")
+    lab = torch.where(lab < 250, lab, lab + 250)
+    h = 7.5 * w[lab].float()
+    h[:, 0] = 0.0
+    h = h.to(dt)
+    ce = A.cut_cross_entropy(h, w, lab)
+    dh, dw = A.cut_cross_entropy_backward(h, w, lab, ce, scale=float(n))  # every token's weight is 1
+    hd, wd = h.double(), w.double()
+    s = hd @ wd.T
+    lse = torch.logsumexp(s, 1)
+    p = torch.softmax(s, 1)
+    at = lab[:, None]
+    G = p.scatter_add(1, at, torch.full_like(at, -1.0, dtype=torch.float64))
+    G[torch.arange(n), lab] = -(p.scatter(1, at, 0.0)).sum(1)  # p - 1 without its cancellation
+    S = (hd.abs() @ wd.abs().T).amax(1, keepdim=True)
+    e_x = 4 * 2.0 ** -24 * (1 + lse.abs()[:, None]) + 2.0 ** -20
+    e_g = p * (1 - p) * 4e-6 * S + p * e_x + 1.1 * U[dt] * G.abs() + (2.0 ** -40 if dt is torch.float16 else 0.0)
+    tiny = 2.0 ** -24 if dt is torch.float16 else 1e-38
+    acc = 2 * 2.0 ** -24
+    want = G @ wd
+    close(dh, want, 1.1 * (e_g @ wd.abs()) + acc * v * (G.abs() @ wd.abs()) + 1.1 * U[dt] * want.abs() + tiny)
+    want = G.T @ hd
+    close(dw, want, 1.1 * (e_g.T @ hd.abs()) + acc * n * (G.abs().T @ hd.abs()) + 1.1 * U[dt] * want.abs() + tiny)
