@@ -69,6 +69,27 @@ inline std::mutex g_rt_mu;
 
 inline int current_device(int* dev) { return cuda_status(cudaGetDevice(dev)); }
 
+// A zeroed device word.  The call may come while a stream is being captured, by
+// this thread or another: the thread leaves the capture's checks for as long as
+// it allocates, and the zeroing goes to a stream of its own, which depends on no
+// other and no capture sees.
+inline int alloc_zeroed_word(uint32_t** out) {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    AETH_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+    uint32_t* w = nullptr;
+    cudaStream_t st = nullptr;
+    cudaError_t e = cudaMalloc(&w, sizeof(uint32_t));
+    if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking);
+    if (e == cudaSuccess) e = cudaMemsetAsync(w, 0, sizeof(uint32_t), st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    if (st) cudaStreamDestroy(st);
+    if (e != cudaSuccess && w) cudaFree(w);
+    cudaThreadExchangeStreamCaptureMode(&mode);  // as it was
+    if (e != cudaSuccess) return set_err((int)e);
+    *out = w;
+    return AETH_OK;
+}
+
 inline int runtime_for_current(DeviceRuntime** out) {
     int dev = 0;
     AETH_TRY(current_device(&dev));
@@ -78,12 +99,7 @@ inline int runtime_for_current(DeviceRuntime** out) {
         std::lock_guard<std::mutex> lock(g_rt_mu);
         if (!rt.init.load(std::memory_order_relaxed)) {
             uint32_t* w = nullptr;
-            AETH_CUDA(cudaMalloc(&w, sizeof(uint32_t)));
-            cudaError_t e = cudaMemset(w, 0, sizeof(uint32_t));
-            if (e != cudaSuccess) {
-                cudaFree(w);
-                return set_err((int)e);
-            }
+            AETH_TRY(alloc_zeroed_word(&w));
             rt.err_word = w;
             rt.init.store(true, std::memory_order_release);
         }

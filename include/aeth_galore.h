@@ -510,8 +510,10 @@ int aeth_lomo_update(const void* grad_bf16, int64_t n, const double* sq_dev, flo
  *     All matrices are row-major device buffers with a row pitch (ld_*) in
  *     elements; scratch comes from the caller (`workspace`, 16-byte aligned,
  *     at least the bytes that the *_workspace function gives; its contents
- *     need not be kept between calls).  Nothing synchronises or allocates, so
- *     every call can be captured into a CUDA graph.
+ *     need not be kept between calls).  Nothing synchronises with the caller's
+ *     streams or allocates (but the library's first call on a device, which sets
+ *     up its error word on a stream of its own), so every call can be captured
+ *     into a CUDA graph, the first one too.
  * ====================================================================== */
 
 /* Softmax cross entropy of s = hidden weight^T (streaming_cut_ce,
