@@ -34,7 +34,8 @@ _current_device = torch._C._cuda_getDevice
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_bytes(fn: str, *dims: int) -> int:
+def _workspace_bytes(fn: str, dev: int, *dims: int) -> int:
+    """What `fn` asks for on `dev`, the current device: it depends on the SMs."""
     size = C.c_size_t()
     L.check(getattr(_lib, fn)(*dims, C.byref(size)), fn)
     return size.value
@@ -117,7 +118,7 @@ def cut_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.
     w, _, ld_w = _tma_rows(weight, d)
     losses, lse = (lab.new_empty(labels.shape, dtype=torch.float32) for _ in range(2))
     loss = lab.new_empty((), dtype=torch.float32)
-    size = _workspace_bytes("aeth_cut_ce_workspace", n, d, v, 0)
+    size = _workspace_bytes("aeth_cut_ce_workspace", dev, n, d, v, 0)
     ws = lab.new_empty(size, dtype=torch.uint8)
     st = _lib.aeth_cut_ce_forward(
         h.data_ptr(), ld_h, w.data_ptr(), ld_w, _DTYPES[h.dtype], lab.data_ptr(), n, d, v, ignore_index,
@@ -153,7 +154,7 @@ def cut_cross_entropy_backward(hidden: torch.Tensor, weight: torch.Tensor, label
     grad = None if grad_losses is None else grad_losses.contiguous()
     dh = h.new_empty(hidden.shape) if need_hidden else None
     dw = h.new_empty(weight.shape) if need_weight else None
-    size = _workspace_bytes("aeth_cut_ce_workspace", n, d, v, 1)
+    size = _workspace_bytes("aeth_cut_ce_workspace", dev, n, d, v, 1)
     ws = lab.new_empty(size, dtype=torch.uint8)
     st = _lib.aeth_cut_ce_backward(
         h.data_ptr(), ld_h, w.data_ptr(), ld_w, _DTYPES[h.dtype], lab.data_ptr(), n, d, v, ignore_index,
@@ -275,7 +276,7 @@ def rms_norm_checkpoint_backward(dy: torch.Tensor, ckpt: ActivationCheckpoint, w
         r, _, ld_r = _rows(d_residual, d)
     dx = torch.empty_like(dy, memory_format=torch.contiguous_format)
     dw = dy.new_empty(d, dtype=torch.float32)
-    size = _workspace_bytes("aeth_rms_norm_checkpoint_backward_workspace", rows, d)
+    size = _workspace_bytes("aeth_rms_norm_checkpoint_backward_workspace", dev, rows, d)
     ws = dy.new_empty(size, dtype=torch.uint8)
     st = _lib.aeth_rms_norm_checkpoint_backward(
         g.data_ptr(), ld, codes.data_ptr(), scales.data_ptr(), gain.data_ptr(), gain_dt,
@@ -303,7 +304,7 @@ def checkpoint_weight_grad(dy: torch.Tensor, ckpt: ActivationCheckpoint, norm_we
         raise ValueError(f"{what}: dy must be ({', '.join(map(str, codes.shape[:-1]))}, m)")
     g, _, ld = _tma_rows(dy, m)
     dw = dy.new_empty((m, d))
-    size = _workspace_bytes("aeth_checkpoint_weight_grad_workspace", rows, m, d)
+    size = _workspace_bytes("aeth_checkpoint_weight_grad_workspace", dev, rows, m, d)
     ws = dy.new_empty(size, dtype=torch.uint8)
     st = _lib.aeth_checkpoint_weight_grad(
         g.data_ptr(), ld, codes.data_ptr(), scales.data_ptr(), None if gain is None else gain.data_ptr(), gain_dt, eps,
