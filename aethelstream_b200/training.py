@@ -192,7 +192,7 @@ def _ckpt_args(what, ckpt, dev):
     rows = codes.numel() // d if d else 0
     blocks = -(-d // CHECKPOINT_BLOCK)
     if d == 0 or codes.dtype != torch.int8 or scales.dtype != torch.float32 or scales.numel() != rows * blocks \
-            or scales.size(-1) != blocks or ckpt.dtype not in _DTYPES:
+            or scales.dim() == 0 or scales.size(-1) != blocks or ckpt.dtype not in _DTYPES:
         raise ValueError(f"{what}: an ActivationCheckpoint with int8 codes (..., d) and float32 scales "
                          f"(..., ceil(d / {CHECKPOINT_BLOCK})) expected")
     if codes.get_device() != dev or scales.get_device() != dev:

@@ -30,3 +30,11 @@ def test_workspace_sizes_are_kept_per_device(training, monkeypatch):
         assert asked == [(10, 64, 100, 0)] * 2
     finally:
         training._workspace_bytes.cache_clear()
+
+
+def test_scales_without_dimensions_are_refused(training):
+    """One row of one block: as many scales as are due, but not in the checkpoint's shape."""
+    import torch
+    ck = training.ActivationCheckpoint(torch.zeros(1, 64, dtype=torch.int8), torch.ones(()), torch.bfloat16)
+    with pytest.raises(ValueError, match="ActivationCheckpoint"):
+        training._ckpt_args("checkpoint_decode", ck, -1)
