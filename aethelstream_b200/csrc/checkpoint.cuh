@@ -766,9 +766,13 @@ __device__ __forceinline__ void ck_back_sums(uint2 q, const Pack8<T>& dy, const 
         dot = f2_fma(f2_mul(f2(ck_value<T>(dy, 2 * i), ck_value<T>(dy, 2 * i + 1)), g[i]),
                      f2(ck_code(q, 2 * i), ck_code(q, 2 * i + 1)), dot);
     const float2 dd = f2_get(dot);
-    xx += (float)__dp4a((int)q.y, (int)q.y, __dp4a((int)q.x, (int)q.x, 0)) * (s * s);
+    xx += (float)__dp4a((int)q.y, (int)q.y, __dp4a((int)q.x, (int)q.x, 0)) * s * s;  // in this order: s * s may leave fp32's range
     xd += (dd.x + dd.y) * s;
 }
+// -r^3 mean(dy gain x^), what x^ is taken times in dx.  r |mean| is at most the root
+// mean square of dy gain, so that one factor of r at a time stays in fp32's range as long
+// as r^2 does (r^3 leaves it where activations reach 1e13, or 1e-13 without eps).
+__device__ __forceinline__ float ck_back_factor(float r, float mean) { return -(r * (r * (r * mean))); }
 // dx of eight features (dy gain r + x^ f + the residual's) and their addends
 // to d_gain's sums.
 template <typename T>
@@ -854,7 +858,7 @@ __global__ void __launch_bounds__(1024 / VPT, ck_min_ctas(VPT, 2))
         if (!WIDE) read_res(0);  // arrives during the row's sum
         ck_row_sum<2, VPT>(acc, sh, parity, sum);
         const float r = t < a.in.rows ? ck_rstd(sum[0], inv_d, a.in.eps) : 0.0f;  // no row: nothing for d_gain, at eps 0 too
-        const float f = -(r * r * r * (sum[1] * inv_d));
+        const float f = ck_back_factor(r, sum[1] * inv_d);
         CK_SPANS(base, a.in.d) {
             if (WIDE) {
                 read(base);
@@ -1044,7 +1048,7 @@ __global__ void __launch_bounds__(kRingThreads, 1)
         if (x0 == 0 && j > 0 && j - 1 + ring.stages < mine)
             copy(j - 1 + ring.stages, stage > 0 ? stage - 1 : ring.stages - 1);
         const float r = ck_rstd(sum[0], inv_d, a.in.eps);
-        const float f = -(r * r * r * (sum[1] * inv_d));
+        const float f = ck_back_factor(r, sum[1] * inv_d);
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
             const int c = 8 * (x0 + k * tx);

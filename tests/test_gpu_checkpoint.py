@@ -364,3 +364,23 @@ def test_rows_off_alignment(dt, rows, d):
         assert torch.equal(y, first[0][0]) and torch.equal(c.codes, first[0][1].codes) and torch.equal(c.scales, first[0][1].scales)
         dxs, dws = A.rms_norm_checkpoint_backward(ds, ck, g, eps=EPS, d_residual=xs)
         assert torch.equal(dxs, dx) and torch.equal(dws, dw)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,d", [(9, 1000), (500, 257), (700, 1008), (400, 12288), (3, 20000)])
+@pytest.mark.parametrize("size,eps", [(1e15, EPS), (1e-18, 0.0)])
+def test_backward_of_large_and_small_activations(dt, rows, d, size, eps):
+    """Activations whose squares fp32 holds, though not the factor's third power."""
+    import aethelstream_b200 as A
+    x, gain, gen = acts(rows, d, torch.float32, rows + d)
+    x = (x * size).to(dt)
+    _, ck = A.rms_norm_checkpoint(x, gain.to(dt), eps=eps)
+    dy = torch.randn(rows, d, generator=gen, device="cuda").to(dt)
+    dx, dw = A.rms_norm_checkpoint_backward(dy, ck, gain, eps=eps)
+    v, dyw = values64(ck), dy.double() * gain.double()
+    r = 1 / torch.sqrt((v * v).mean(1, keepdim=True) + eps)
+    want = r * dyw - v * r ** 3 * (dyw * v).mean(1, keepdim=True)
+    bound = (d / 8 + 24) * E * (r * dyw.abs() + v.abs() * r ** 3 * (dyw * v).abs().mean(1, keepdim=True) * 2)
+    close(dx, want, 1.1 * (bound + U[dt] * want.abs()) + TINY[dt])
+    t = dy.double() * v * r
+    close(dw, t.sum(0), t.abs().sum(0) * ((d / 16 + 16) + rows) * E + 1e-37)
