@@ -36,7 +36,7 @@ struct Carver {
 // Head loss
 // ---------------------------------------------------------------------------
 constexpr int64_t kHeadMaxDim = 1ll << 30;       // token, feature and vocabulary counts (tile coordinates are int)
-constexpr int64_t kHeadPieceBytes = 256ll << 20;  // scratch of a vocabulary piece: G, and the buffers of dH's tail
+constexpr int64_t kHeadPieceBytes = 256ll << 20;  // scratch of a vocabulary piece: its G's, and the buffers of dH's tail
 
 // Columns per tile for a product of `cols` columns (B K-major) with `tiles_m`
 // row tiles: what makes the last wave of tiles over the 74 CTA pairs least
@@ -75,8 +75,9 @@ struct HeadPlan {
     int np;      // column ranges of the forward's statistics
     int tail_kb;    // k-blocks of a piece's dH product
     int64_t extra;  // buffers of its tail
+    int gs;         // G's of a piece: a second one without the token weights (head_loss.cuh)
 
-    HeadPlan(int64_t n, int64_t d, int64_t vocab) {
+    HeadPlan(int64_t n, int64_t d, int64_t vocab, int gs_ = 1) : gs(gs_) {
         n_pad = up(std::max<int64_t>(n, 1), 256);
         dp = up(d, 8);
         live_n = head_tokens_as_columns(n);
@@ -86,10 +87,10 @@ struct HeadPlan {
         const int64_t pairs = pair_count(), tiles_m = n_pad / 256;
         const int64_t most = std::min<int64_t>(pairs, (vocab + 511) / 512) - 1;  // ranges of 8 k-blocks past the first
         extra = std::min<int64_t>(2 * pairs, most * std::min<int64_t>(tiles_m * ((d + 255) / 256), pairs));
-        // a piece is a number of 256-entry tiles whose G fits beside them; of those, from the
+        // a piece is a number of 256-entry tiles whose G's fit beside them; of those, from the
         // largest down to half of it (64 are looked at), the one with the fewest waves of tiles over all pieces
         const int64_t all = (vocab + 255) / 256;
-        const int64_t fit = std::max<int64_t>((kHeadPieceBytes - extra * 262144) / (512 * n_pad), 1);
+        const int64_t fit = std::max<int64_t>((kHeadPieceBytes - extra * 262144) / (512 * n_pad * gs), 1);
         int64_t best = fit, least = INT64_MAX;
         auto waves = [&](int64_t tiles) { return (tiles * tiles_m + pairs - 1) / pairs; };
         for (int64_t p = fit; p >= std::max((fit + 1) / 2, fit - 64) && fit < all; --p) {
@@ -117,8 +118,8 @@ struct HeadWork {
     float* label_logit;
     float2* part;
     // backward
-    float *coef, *lse2, *out_scale, *slab, *extra;
-    uint16_t* g;
+    float *coef, *lse2, *out_scale, *row_scale, *slab, *extra;
+    uint16_t *g, *g_unit;
     size_t bytes;
 
     HeadWork(const HeadPlan& p, int64_t n, bool backward, void* ws) {
@@ -131,16 +132,18 @@ struct HeadWork {
         h = c.take<uint16_t>(p.n_pad * p.dp);
         label_logit = nullptr;
         part = nullptr;
-        coef = lse2 = out_scale = slab = extra = nullptr;
-        g = nullptr;
+        coef = lse2 = out_scale = row_scale = slab = extra = nullptr;
+        g = g_unit = nullptr;
         if (!backward) {
             label_logit = c.take<float>(p.n_pad);
             part = c.take<float2>(std::max<int64_t>((int64_t)p.np * p.n_pad, num_sms() * kHeadVecTokens));
         } else {
             coef = c.take<float>(p.n_pad);
             lse2 = c.take<float>(p.n_pad);
+            row_scale = c.take<float>(p.n_pad);
             out_scale = c.take<float>(1);
             g = c.take<uint16_t>(p.n_pad * p.ldg);
+            g_unit = p.gs > 1 ? c.take<uint16_t>(p.n_pad * p.ldg) : g;
             slab = c.take<float>(p.n_pad * p.dp);
             extra = c.take<float>(p.extra * 65536);
         }
@@ -208,22 +211,24 @@ int head_vec(const HeadVec& a, int64_t n, int ctas, float* losses, float* lse, f
     return AETH_OK;
 }
 
-template <bool BF16>
+// UNIT: d_hidden comes from a G without the token weights
+template <bool BF16, bool UNIT>
 int head_backward(const HeadPlan& p, const HeadWork& w, const void* weight, int64_t ld_weight, int64_t n, int64_t d,
                   int64_t vocab, void* d_hidden, int64_t ld_dh, void* d_weight, int64_t ld_dw, cudaStream_t st) {
     const uint16_t* W = static_cast<const uint16_t*>(weight);
+    uint16_t *g = UNIT && !d_weight ? nullptr : w.g, *g_unit = UNIT ? w.g_unit : nullptr;
     for (int64_t v0 = 0; v0 < vocab; v0 += p.piece) {
         const int64_t vp = std::min(p.piece, vocab - v0);
         const PairOperand H{w.h, p.dp, n, d}, Wp{W + v0 * ld_weight, ld_weight, vp, d};
-        const PairOperand G{w.g, p.ldg, n, vp};
+        const PairOperand G{w.g, p.ldg, n, vp}, Gh{UNIT ? w.g_unit : w.g, p.ldg, n, vp};
         if (p.live_n) {
-            HeadGradT<BF16> eg{w.lab, w.coef, w.lse2, w.g, p.ldg, (int)n, (int)v0};
-            AETH_TRY((pair_gemm_launch<HeadGradT<BF16>, false, false>(Wp, H, (int)vp, (int)n, (int)d, w.count, PAIR_LIVE_N,
-                                                                      256, 0, BF16, eg, st)));
+            HeadGradT<BF16, UNIT> eg{w.lab, w.coef, w.lse2, g, g_unit, p.ldg, (int)n, (int)v0};
+            AETH_TRY((pair_gemm_launch<HeadGradT<BF16, UNIT>, false, false>(Wp, H, (int)vp, (int)n, (int)d, w.count,
+                                                                            PAIR_LIVE_N, 256, 0, BF16, eg, st)));
         } else {
-            HeadGrad<BF16> eg{w.lab, w.coef, w.lse2, w.g, p.ldg, (int)n, (int)v0};
-            AETH_TRY((pair_gemm_launch<HeadGrad<BF16>, false, false>(H, Wp, (int)n, (int)vp, (int)d, w.count, PAIR_LIVE_M,
-                                                                     head_bn(p.n_pad / 256, vp), 0, BF16, eg, st)));
+            HeadGrad<BF16, UNIT> eg{w.lab, w.coef, w.lse2, g, g_unit, p.ldg, (int)n, (int)v0};
+            AETH_TRY((pair_gemm_launch<HeadGrad<BF16, UNIT>, false, false>(H, Wp, (int)n, (int)vp, (int)d, w.count, PAIR_LIVE_M,
+                                                                           head_bn(p.n_pad / 256, vp), 0, BF16, eg, st)));
         }
         if (d_weight) {
             PairOut16<BF16> ew{static_cast<uint16_t*>(d_weight) + v0 * ld_dw, ld_dw, w.out_scale};
@@ -233,18 +238,18 @@ int head_backward(const HeadPlan& p, const HeadWork& w, const void* weight, int6
         if (d_hidden) {
             if (p.live_n) {
                 PairSlabT es{w.slab, p.dp, w.extra, v0 == 0};
-                AETH_TRY((pair_gemm_launch<PairSlabT, true, false>(Wp, G, (int)d, (int)n, (int)vp, w.count, PAIR_LIVE_N,
+                AETH_TRY((pair_gemm_launch<PairSlabT, true, false>(Wp, Gh, (int)d, (int)n, (int)vp, w.count, PAIR_LIVE_N,
                                                                    256, p.tail_kb, BF16, es, st)));
             } else {
                 PairSlab es{w.slab, p.dp, w.extra, v0 == 0};
-                AETH_TRY((pair_gemm_launch<PairSlab, false, true>(G, Wp, (int)n, (int)d, (int)vp, w.count, PAIR_LIVE_M,
+                AETH_TRY((pair_gemm_launch<PairSlab, false, true>(Gh, Wp, (int)n, (int)d, (int)vp, w.count, PAIR_LIVE_M,
                                                                   256, p.tail_kb, BF16, es, st)));
             }
         }
     }
     if (d_hidden && n > 0) {
-        const HeadDh a{w.slab, p.dp, w.extra, pair_count(), p.tail_kb, p.live_n, w.pos, w.count, n, (int)d, w.out_scale,
-                       static_cast<uint16_t*>(d_hidden), ld_dh};
+        const HeadDh a{w.slab, p.dp, w.extra, pair_count(), p.tail_kb, p.live_n, w.pos, w.count, n, (int)d,
+                       UNIT ? nullptr : w.out_scale, w.row_scale, static_cast<uint16_t*>(d_hidden), ld_dh};
         const unsigned cols = (unsigned)((d + 1023) / 1024);
         const int64_t rows = std::max<int64_t>(16 * num_sms() / cols, 1);
         // few tokens: one at a time, and more of its parts
@@ -414,6 +419,7 @@ int aeth_cut_ce_workspace(int64_t n, int64_t d, int64_t vocab, int backward, siz
     if (n < 0 || d <= 0 || vocab <= 0 || !bytes) return set_err(AETH_ERR_ARG);
     if (n > kHeadMaxDim || d > kHeadMaxDim || vocab > kHeadMaxDim) return set_err(AETH_ERR_UNSUPPORTED);
     *bytes = HeadWork(HeadPlan(n, d, vocab), n, backward != 0, nullptr).bytes;
+    if (backward) *bytes = std::max(*bytes, HeadWork(HeadPlan(n, d, vocab, 2), n, true, nullptr).bytes);
     return AETH_OK;
 }
 
@@ -470,10 +476,11 @@ int aeth_cut_ce_backward(const void* hidden, int64_t ld_hidden, const void* weig
             AETH_CUDA(cudaMemset2DAsync(d_weight, (size_t)ld_dw * 2, 0, (size_t)d * 2, (size_t)vocab, st));
         return AETH_OK;
     }
-    const HeadPlan p(n, d, vocab);
+    const bool bf16 = dtype == AETH_DTYPE_BF16;
+    const bool unit = !bf16 && grad_losses && d_hidden;
+    const HeadPlan p(n, d, vocab, unit ? 2 : 1);
     const HeadWork w(p, n, true, workspace);
     if (workspace_bytes < w.bytes || !aligned16(workspace)) return set_err(AETH_ERR_ARG);
-    const bool bf16 = dtype == AETH_DTYPE_BF16;
     HeadRows a = {};
     a.lse = lse;
     a.grad = grad_losses;
@@ -483,9 +490,10 @@ int aeth_cut_ce_backward(const void* hidden, int64_t ld_hidden, const void* weig
     a.coef = w.coef;
     a.lse2 = w.lse2;
     a.out_scale = w.out_scale;
+    a.row_scale = w.row_scale;
     AETH_TRY(head_rows(a, labels, n, d, vocab, ignore_index, hidden, ld_hidden, p, w, st));
-    return bf16 ? head_backward<true>(p, w, weight, ld_weight, n, d, vocab, d_hidden, ld_dh, d_weight, ld_dw, st)
-                : head_backward<false>(p, w, weight, ld_weight, n, d, vocab, d_hidden, ld_dh, d_weight, ld_dw, st);
+    auto run = bf16 ? head_backward<true, false> : unit ? head_backward<false, true> : head_backward<false, false>;
+    return run(p, w, weight, ld_weight, n, d, vocab, d_hidden, ld_dh, d_weight, ld_dw, st);
 }
 
 int aeth_rms_norm_checkpoint(const void* x, int64_t ld_x, const void* residual, int64_t ld_residual, const void* gain,

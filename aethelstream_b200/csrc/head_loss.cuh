@@ -31,8 +31,13 @@ constexpr int kHeadIgnored = -1, kHeadBad = -2;  // pos[] of a token that takes 
 
 // G is held relative to the largest token weight (|G| <= 1) and times 2^k, the
 // power folded into the exponent of p: with k = 15 f16 keeps eleven bits down
-// to p = 2e-9 (6e-5 without); with k = 32 what fp32's and bf16's range cuts off
-// is p < 2^-158, not 2^-126.
+// to p = 2e-9 of the largest weight (6e-5 without); with k = 32 what fp32's and
+// bf16's range cuts off is p < 2^-158, not 2^-126.
+// f16 with token weights: what a token of 1e-6 of the largest weight has in G is
+// cut off at p = 1e-6, which its row of dH may need.  dH is then taken from a
+// second G without the weights, which multiply dH's rows at the end; dW, where
+// the tokens are added up, keeps the first (each entry within 2^-40 of the
+// largest weight).
 __host__ __device__ constexpr float head_g_bits(bool bf16) { return bf16 ? 32.0f : 15.0f; }
 __host__ __device__ constexpr float head_g_scale(bool bf16) { return bf16 ? 4294967296.0f : 32768.0f; }
 
@@ -59,6 +64,7 @@ struct HeadRows {
     float* coef;       // live row -> g_t / max|g|
     float* lse2;       // live row -> lse * log2(e) - g_bits
     float* out_scale;  // max|g| / g_scale
+    float* row_scale;  // live row -> |g_t| / g_scale
     // the live rows of H, gathered to a pitch that TMA takes
     const uint16_t* h;
     int64_t ld;
@@ -184,6 +190,7 @@ __global__ void __launch_bounds__(1024) head_rows_kernel(const __grid_constant__
                 if (a.grad) {
                     const float g = grad[k] * a.scale;
                     a.coef[i] = g;
+                    a.row_scale[i] = fabsf(g) / a.g_scale;
                     if (fabsf(g) <= 3.402823466e38f) gmax = fmaxf(gmax, fabsf(g));  // what is not finite stays its token's
                 }
             }
@@ -615,6 +622,9 @@ __global__ void __launch_bounds__(32 * kHeadVecTokens)
     }
 }
 
+// A token weight's part in the G without weights: its sign (NaN and 0 stay).
+__device__ __forceinline__ float head_unit(float f) { return f > 0.0f ? 1.0f : f < 0.0f ? -1.0f : f; }
+
 // Epilogue of the backward's product: G of the piece in 16 bits.  G is rounded
 // once, from fp32; rows from the count to the tile's end (or n) become zero.  The
 // logits are added up as in the forward, so that they are those that lse came
@@ -622,14 +632,17 @@ __global__ void __launch_bounds__(32 * kHeadVecTokens)
 // is all of p - 1 for a label known with p = 0.9998.  That costs 1.4 to 2.4 % of a
 // large backward (8192 x 8192 x 32000: 10.03 -> 10.18 ms, power-capped; 3584 x 4096
 // x 32000: 2.13 -> 2.19) and 6 to 13 us of one of 130 to 311 tokens (160 to 260 us).
-template <bool BF16>
+// UNIT (f16): the G without token weights, beside the other where that is wanted
+// (3584 x 4096 x 32000 with weights: 2.26 -> 2.42 ms, 64 tokens 178 -> 183 us).
+template <bool BF16, bool UNIT>
 struct HeadGrad {
     static constexpr int kChunk = 8;
     static constexpr bool kLiveN = false;
     const int* lab;
     const float* coef;
     const float* lse2;
-    uint16_t* g;
+    uint16_t* g;       // with UNIT: or null
+    uint16_t* g_unit;  // with UNIT
     int64_t ldg;
     int n;   // rows of g: the tokens
     int v0;  // first vocabulary entry of the piece
@@ -637,13 +650,13 @@ struct HeadGrad {
     __device__ __forceinline__ void finish(const PairTile& t, const float (&acc)[128]) const {
         const int row = t.row0 + t.lane;
         const bool in = row < t.M;
-        const float f = in ? coef[row] : 0.0f, l2 = in ? lse2[row] : 0.0f;
+        const float f = in ? coef[row] : 0.0f, u = head_unit(f), l2 = in ? lse2[row] : 0.0f;
         const int lab_c = in ? lab[row] - v0 - t.col0 - t.c_begin : -1;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const int c = t.c_begin + 64 * b;
             if (c < t.c_end && t.col0 + c < t.N && t.row0 < n) {
-                uint32_t w[32];
+                uint32_t w[32], w1[32];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     float v[32];
@@ -656,9 +669,14 @@ struct HeadGrad {
                         for (int i = 0; i < 32; ++i) v[i] = k == i ? v[i] - head_g_scale(BF16) : v[i];
                     }
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) w[16 * h + i] = pack16<BF16>(v[2 * i] * f, v[2 * i + 1] * f);
+                    for (int i = 0; i < 16; ++i) {
+                        w[16 * h + i] = pack16<BF16>(v[2 * i] * f, v[2 * i + 1] * f);
+                        if (UNIT) w1[16 * h + i] = pack16<BF16>(v[2 * i] * u, v[2 * i + 1] * u);
+                    }
                 }
-                pair_store16(t, w, c, g, ldg, n, min(t.N, t.col0 + t.c_end));
+                const int cols = min(t.N, t.col0 + t.c_end);
+                if (!UNIT || g) pair_store16(t, w, c, g, ldg, n, cols);
+                if (UNIT) pair_store16(t, w1, c, g_unit, ldg, n, cols);
             }
         }
     }
@@ -666,7 +684,7 @@ struct HeadGrad {
 
 // The same with tokens as the tile's columns: each 32 x 32 block is turned over,
 // so that a thread has a token and 32 entries.
-template <bool BF16>
+template <bool BF16, bool UNIT>
 struct HeadGradT {
     static constexpr int kChunk = 8;
     static constexpr bool kLiveN = true;
@@ -674,12 +692,12 @@ struct HeadGradT {
     const float* coef;
     const float* lse2;
     uint16_t* g;
+    uint16_t* g_unit;
     int64_t ldg;
     int n;
     int v0;
     __device__ static void give_up(const PairTile&) {}
     __device__ __forceinline__ void finish(const PairTile& t, const float (&acc)[128]) const {
-        const bool whole = (ldg % 8) == 0 && (reinterpret_cast<uintptr_t>(g) & 15) == 0;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
             const int c = t.c_begin + 32 * b;
@@ -689,7 +707,7 @@ struct HeadGradT {
             pair_transpose(t, v);
             const int token = t.col0 + c + t.lane;
             const bool in = token < t.N;
-            const float f = in ? coef[token] : 0.0f, l2 = in ? lse2[token] : 0.0f;
+            const float f = in ? coef[token] : 0.0f, u = head_unit(f), l2 = in ? lse2[token] : 0.0f;
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = ex2(fmaf(v[i], kLog2e, -l2));
             const int k = in ? lab[token] - v0 - t.row0 : -1;
@@ -697,34 +715,43 @@ struct HeadGradT {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) v[i] = k == i ? v[i] - head_g_scale(BF16) : v[i];
             }
-            uint32_t w[16];
+            uint32_t w[16], w1[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = pack16<BF16>(v[2 * i] * f, v[2 * i + 1] * f);
-            // 64 bytes a token; piece p (16 bytes) of token r lies at p ^ (r / 2) % 4
+            for (int i = 0; i < 16; ++i) {
+                w[i] = pack16<BF16>(v[2 * i] * f, v[2 * i + 1] * f);
+                if (UNIT) w1[i] = pack16<BF16>(v[2 * i] * u, v[2 * i + 1] * u);
+            }
+            if (!UNIT || g) store(t, w, c, g);
+            if (UNIT) store(t, w1, c, g_unit);
+        }
+    }
+    // 32 tokens (columns c .. of the tile) x 32 entries, thread = token
+    __device__ __forceinline__ void store(const PairTile& t, const uint32_t (&w)[16], int c, uint16_t* out) const {
+        const bool whole = (ldg % 8) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+        // 64 bytes a token; piece p (16 bytes) of token r lies at p ^ (r / 2) % 4
 #pragma unroll
-            for (int p = 0; p < 4; ++p)
-                *reinterpret_cast<uint4*>(t.staging + t.lane * 64 + ((p ^ ((t.lane >> 1) & 3)) * 16)) =
-                    make_uint4(w[4 * p], w[4 * p + 1], w[4 * p + 2], w[4 * p + 3]);
-            __syncwarp();
+        for (int p = 0; p < 4; ++p)
+            *reinterpret_cast<uint4*>(t.staging + t.lane * 64 + ((p ^ ((t.lane >> 1) & 3)) * 16)) =
+                make_uint4(w[4 * p], w[4 * p + 1], w[4 * p + 2], w[4 * p + 3]);
+        __syncwarp();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = i * 8 + (t.lane >> 2), p = t.lane & 3;
-                const int gr = t.col0 + c + r, gc = t.row0 + p * 8;
-                const uint4 x = *reinterpret_cast<const uint4*>(t.staging + r * 64 + ((p ^ ((r >> 1) & 3)) * 16));
-                if (gr < n && gc < t.M) {
-                    uint16_t* o = g + (int64_t)gr * ldg + gc;
-                    if (whole && gc + 8 <= t.M) {
-                        *reinterpret_cast<uint4*>(o) = x;
-                    } else {
-                        const uint32_t xx[4] = {x.x, x.y, x.z, x.w};
+        for (int i = 0; i < 4; ++i) {
+            const int r = i * 8 + (t.lane >> 2), p = t.lane & 3;
+            const int gr = t.col0 + c + r, gc = t.row0 + p * 8;
+            const uint4 x = *reinterpret_cast<const uint4*>(t.staging + r * 64 + ((p ^ ((r >> 1) & 3)) * 16));
+            if (gr < n && gc < t.M) {
+                uint16_t* o = out + (int64_t)gr * ldg + gc;
+                if (whole && gc + 8 <= t.M) {
+                    *reinterpret_cast<uint4*>(o) = x;
+                } else {
+                    const uint32_t xx[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                        for (int q = 0; q < 8; ++q)
-                            if (gc + q < t.M) o[q] = (uint16_t)(xx[q >> 1] >> (16 * (q & 1)));
-                    }
+                    for (int q = 0; q < 8; ++q)
+                        if (gc + q < t.M) o[q] = (uint16_t)(xx[q >> 1] >> (16 * (q & 1)));
                 }
             }
-            __syncwarp();
         }
+        __syncwarp();
     }
 };
 
@@ -739,7 +766,8 @@ struct HeadDh {
     const int *pos, *count;
     int64_t n;
     int d;
-    const float* scale;
+    const float* scale;      // one for all, or null
+    const float* row_scale;  // else a live row's
     uint16_t* out;
     int64_t ldo;
 };
@@ -759,7 +787,7 @@ __global__ void __launch_bounds__(128) head_dh_kernel(const HeadDh a) {
     }
     __syncthreads();
     const int bt = sh[0], tiles_t = sh[1], full = sh[2], rest = sh[3], splits = sh[4], tiles_d = (a.d + 255) / 256;
-    const float scale = *a.scale;
+    const float scale_all = a.scale ? *a.scale : 0.0f;
     const int c = (blockIdx.y * 128 + threadIdx.x) * 8;
     if (c >= a.d) return;
     const bool whole = (a.ldo % 8) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && c + 8 <= a.d;
@@ -794,6 +822,7 @@ __global__ void __launch_bounds__(128) head_dh_kernel(const HeadDh a) {
                 }
             }
             uint32_t w[4] = {0, 0, 0, 0};
+            const float scale = a.scale || p[k] < 0 ? scale_all : a.row_scale[p[k]];
             if (p[k] >= 0)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {

@@ -529,8 +529,10 @@ int aeth_lomo_update(const void* grad_bf16, int64_t n, const double* sq_dev, flo
  *   backward: with g_t = scale * grad_losses[t], or scale / count where
  *   grad_losses is NULL (the mean's gradient), and G = g_t (softmax - onehot):
  *   d_hidden = G weight, d_weight = G^T hidden, in the inputs' type; either may
- *   be NULL.  G exists for one vocabulary piece at a time, in 16 bits (at most
- *   256 MiB). */
+ *   be NULL.  G exists for one vocabulary piece at a time, in 16 bits; in F16 with
+ *   grad_losses there are two, d_hidden's without the token weights, so that a
+ *   token's row keeps its bits whatever the others weigh.  They take at most 256
+ *   MiB, or 256 entries of the vocabulary where these take more. */
 int aeth_cut_ce_workspace(int64_t n, int64_t d, int64_t vocab, int backward, size_t* bytes);
 int aeth_cut_ce_forward(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, int dtype,
                         const int64_t* labels, int64_t n, int64_t d, int64_t vocab, int64_t ignore_index,

@@ -391,3 +391,46 @@ def test_gradient_of_tokens_that_are_known(n, dt):
     close(dh, want, 1.1 * (e_g @ wd.abs()) + acc * v * (G.abs() @ wd.abs()) + 1.1 * U[dt] * want.abs() + tiny)
     want = G.T @ hd
     close(dw, want, 1.1 * (e_g.T @ hd.abs()) + acc * n * (G.abs().T @ hd.abs()) + 1.1 * U[dt] * want.abs() + tiny)
+
+
+def hidden_bound(h, w, lab, grad, scale):
+    """d_hidden in 64 bits and its bound, every token judged by its own weight (see reference())."""
+    dt = h.dtype
+    hd, wd = h.double(), w.double()
+    s = hd @ wd.T
+    g = scale * grad.double()[:, None]
+    p = torch.softmax(s, 1)
+    lse = torch.logsumexp(s, 1)
+    e_s = (hd.abs() @ wd.abs().T).amax(1) * (2 * h.shape[1] * 2.0 ** -24)
+    G = p.scatter_add(1, lab[:, None], torch.full_like(lab[:, None], -1.0, dtype=torch.float64)) * g
+    e_g = G.abs() * (U[dt] + 2.0 ** -20) + (p * g.abs()) * (2 * e_s + 2.0 ** -18 * (1 + lse.abs() / 16))[:, None] + 2.0 ** -40 * g.abs()
+    want = G @ wd
+    return want, 1.1 * (e_g @ wd.abs()) + 2 * 2.0 ** -24 * w.shape[0] * (G.abs() @ wd.abs()) + 1.1 * U[dt] * want.abs() + 2.0 ** -24
+
+
+@pytest.mark.parametrize("n,d,v", [(3, 64, 131071), (40, 64, 131071), (256, 64, 60001), (4200, 64, 40001)])
+def test_token_weights_over_six_decades(n, d, v):
+    """f16: a token's d_hidden has its bits whatever the other tokens weigh.  Most
+    vocabulary entries are alike and their probabilities small, so that cutting
+    them off would show; a constant feature shows the sum of G's row."""
+    import aethelstream_b200 as A
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    w = torch.zeros(v, d, device="cuda")
+    w[:300] = torch.randn(300, d, generator=gen, device="cuda") * 0.25
+    w[:, 0] = 1.0
+    w = w.half()
+    lab = torch.randint(0, 300, (n,), generator=gen, device="cuda")
+    h = torch.randn(n, d, generator=gen, device="cuda").half()
+    h[:, 0] = 0.0
+    grad = torch.logspace(-6, 0, n, device="cuda")
+    grad[1::2] *= -1
+    scale = 2.0 ** 13
+    ce = A.cut_cross_entropy(h, w, lab)
+    dh, dw = A.cut_cross_entropy_backward(h, w, lab, ce, grad_losses=grad, scale=scale)
+    for at in torch.arange(n, device="cuda").split(64):
+        close(dh[at], *hidden_bound(h[at], w, lab[at], grad[at], scale))
+    assert torch.equal(A.cut_cross_entropy_backward(h, w, lab, ce, grad_losses=grad, scale=scale, need_weight=False)[0], dh)
+    assert torch.equal(A.cut_cross_entropy_backward(h, w, lab, ce, grad_losses=grad, scale=scale, need_hidden=False)[1], dw)
+    if n <= 256:
+        r = reference(h, w, lab, grad=grad, scale=scale)
+        close(dw, r["dw"], r["b_w"])
