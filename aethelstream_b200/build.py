@@ -76,24 +76,27 @@ def build(force: bool = False, verbose: bool = False, extra: list[str] | None = 
     if not force and not needs_build():
         return LIB
     os.makedirs(OBJ, exist_ok=True)
+    suffix = ".extra.o" if extra else ".o"  # objects with flags of their own serve this build alone
+    objects = [os.path.join(OBJ, unit + suffix) for unit in UNITS]
     compiles = []
-    for unit in UNITS:
-        obj = os.path.join(OBJ, unit + ".o")
+    for unit, obj in zip(UNITS, objects):
         src = os.path.join(CSRC, unit + ".cu")
         if force or extra or stale(obj, unit):
-            cmd = [nvcc(), *NVCC_FLAGS, *(extra or []), "-I", os.path.join(ROOT, "include"), "-c", src, "-o", obj]
+            cmd = [nvcc(), *NVCC_FLAGS, *(extra or []), "-I", os.path.join(ROOT, "include"), "-c", src, "-o", obj + ".tmp"]
             if verbose:
                 print(" ".join(cmd))
-            compiles.append(subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True))
-    for p in compiles:
+            compiles.append((obj, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+    for obj, p in compiles:
         out = p.communicate()[0]
         if p.returncode != 0:
             sys.stderr.write(out)
-        elif verbose and out:
-            print(out)
-    if any(p.returncode != 0 for p in compiles):
+        else:
+            os.replace(obj + ".tmp", obj)  # whole, or not at all
+            if verbose and out:
+                print(out)
+    if any(p.returncode != 0 for _, p in compiles):
         raise RuntimeError("nvcc failed building libaeth_galore.so")
-    cmd = [nvcc(), *NVCC_FLAGS[:2], "-shared", *[os.path.join(OBJ, u + ".o") for u in UNITS], "-o", LIB + ".tmp"]
+    cmd = [nvcc(), *NVCC_FLAGS[:2], "-shared", *objects, "-o", LIB + ".tmp"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
