@@ -234,11 +234,16 @@ __global__ void __launch_bounds__(kApplyThreads, 1)
         for (int u = ustart; u < total; u += ustep, ++j) {
             const int b = j & 1;
             const int wb = j % kApplyWSlots;
-            if (!mbar_wait(&w_full[wb], (uint32_t)(j / kApplyWSlots) & 1u, abort, err, DEVERR_TIMEOUT_EPI)) break;
+            const bool w_here = mbar_wait(&w_full[wb], (uint32_t)(j / kApplyWSlots) & 1u, abort, err, DEVERR_TIMEOUT_EPI);
             const int4 info = winfo[wb];
             const ApplyProblem& pr = args.p[info.x];
             const int m0 = info.y, n0 = info.z;
-            if (!mbar_wait(&acc_full[b], (uint32_t)(j >> 1) & 1u, abort, err, DEVERR_TIMEOUT_EPI) || *abort) break;
+            const bool here =
+                w_here && mbar_wait(&acc_full[b], (uint32_t)(j >> 1) & 1u, abort, err, DEVERR_TIMEOUT_EPI) && !*abort;
+            if (!__all_sync(0xffffffffu, here)) {
+                named_bar_arrive(1 + q, 128);  // this unit's, which the row group's others may wait at
+                break;
+            }
             tc_fence_after();
             uint8_t* wp = wslot + wb * L::kWSlot;
             if (n0 + cl < pr.n) {  // warp-uniform

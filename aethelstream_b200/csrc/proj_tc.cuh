@@ -162,7 +162,8 @@ __global__ void __launch_bounds__(192, 1) proj_grouped_kernel(const __grid_const
             const int local = u - pr.unit_begin;
             const int m0 = (local / pr.splits) * 128;
             const int b = j & 1;
-            if (!mbar_wait(&acc_full[b], (uint32_t)(j >> 1) & 1u, abort, err, DEVERR_TIMEOUT_EPI) || *abort) break;
+            const bool here = mbar_wait(&acc_full[b], (uint32_t)(j >> 1) & 1u, abort, err, DEVERR_TIMEOUT_EPI) && !*abort;
+            if (!named_bar_and(1, 128, here)) break;
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < nchunks; ++c, ++cc) {
@@ -339,7 +340,8 @@ __global__ void __launch_bounds__(192, 1) proj_pair_kernel(const __grid_constant
             const int m0 = (local / pr.splits) * 256 + crank * 128;
             const int b = NB == 2 ? (j & 1) : 0;
             const uint32_t use = NB == 2 ? (uint32_t)(j >> 1) : (uint32_t)j;
-            if (!mbar_wait(&acc_full[b], use & 1u, abort, err, DEVERR_TIMEOUT_EPI) || *abort) break;
+            const bool here = mbar_wait(&acc_full[b], use & 1u, abort, err, DEVERR_TIMEOUT_EPI) && !*abort;
+            if (!named_bar_and(1, 128, here)) break;
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < nchunks; ++c, ++cc) {

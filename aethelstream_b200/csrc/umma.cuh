@@ -155,6 +155,20 @@ __device__ __forceinline__ void named_bar(int id, int count) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(count) : "memory");
 }
 
+// The same barrier, and whether `p` held for all of its threads.  Warps that meet
+// at barriers vote so on a bounded wait's outcome before they act on it: if one
+// left by itself, the others would wait for it at the next barrier for good.
+__device__ __forceinline__ bool named_bar_and(int id, int count, bool p) {
+    uint32_t all;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\t"
+        "barrier.cta.red.and.pred q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(all)
+        : "r"(id), "r"(count), "r"((uint32_t)p)
+        : "memory");
+    return all != 0;
+}
+
 // An arrival that does not wait: what a warp that gave up still owes the others.
 __device__ __forceinline__ void named_bar_arrive(int id, int count) {
     asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(count) : "memory");

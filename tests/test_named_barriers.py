@@ -108,3 +108,33 @@ def test_epilogues_with_barriers_are_found():
 def test_a_warp_that_gives_up_leaves_nobody_waiting(name):
     finish, give_up = epilogues()[name]
     assert stuck(finish, give_up) is None
+
+
+def loops():
+    """(file, text) of every `for` loop in the kernels that waits at a named barrier."""
+    out = []
+    for name in sorted(os.listdir(CSRC)):
+        with open(os.path.join(CSRC, name)) as f:
+            text = re.sub(r"//[^\n]*", "", f.read())
+        for m in re.finditer(r"\bfor \(", text):
+            depth, i = 1, m.end()
+            while depth:
+                depth += {"(": 1, ")": -1}.get(text[i], 0)
+                i += 1
+            if not text[i:].lstrip().startswith("{"):
+                continue
+            b = body(text, i)
+            if re.search(r"named_bar\(", b):
+                out.append((name, b))
+    return out
+
+
+def test_no_warp_leaves_such_a_loop_by_itself():
+    """After a bounded wait the warps vote, or the one that leaves settles the barrier."""
+    waits = 0
+    for name, b in loops():
+        for m in re.finditer(r"mbar_wait\(", b):
+            waits += 1
+            leave = b.find("break;", m.end())
+            assert leave < 0 or re.search(r"named_bar_and\(|named_bar_arrive\(", b[m.end():leave]), (name, b[m.start():leave + 6])
+    assert waits >= 4  # both projections, the weight write's, the ring's
