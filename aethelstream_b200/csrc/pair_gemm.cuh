@@ -36,10 +36,10 @@
 // Few live rows are taken as N, not M: M comes in tiles of 256 only, N in
 // multiples of 32, so 311 rows cost two tiles of 160 and not two of 256, and a
 // handful of rows leaves a product bound by the other operand's bytes.  Their
-// smaller stages make up to ten of six: a k-block of 320 MMA cycles (N = 160)
+// smaller stages make up to nine of six: a k-block of 320 MMA cycles (N = 160)
 // took 530 with six stages, whose copies were not far enough ahead of the MMAs
 // (tensor pipe 52 % active, DRAM 44 %; 300 x 4096 x 32000, forward and backward:
-// 95 + 274 us with six, 89 + 257 with seven; 16 tokens, ten: 63 + 176 and 58 +
+// 95 + 274 us with six, 89 + 257 with seven; 16 tokens, nine: 63 + 176 and 58 +
 // 170).  The
 // tile's columns are then the rows of the result, and epilogues turn each
 // 32 x 32 block over in shared memory (pair_transpose).
@@ -54,12 +54,20 @@
 namespace aeth {
 
 constexpr int kPairEpiWarps = 8;
-constexpr int kPairProducers = 3;  // divides the stages, so each has stages of its own
+constexpr int kPairProducers = 3;
 constexpr int kPairThreads = 32 * (1 + kPairProducers + kPairEpiWarps);
 constexpr int kPairStages = 6;
 constexpr int kPairOperand = 128 * 64 * 2;                  // one operand of one stage and CTA
 constexpr int kPairStage = 2 * kPairOperand;
-constexpr int kPairMaxStages = 10;  // of narrow tiles, whose B takes less
+// Of narrow tiles, whose B takes less: 64 columns at least (pair_live_bn).
+constexpr int kPairMaxStages = kPairStages * kPairStage / (kPairOperand + 32 * 128);
+static_assert(kPairMaxStages == 9, "stages of a tile of 64 columns");
+// The producers take the k-blocks in turn, whatever the number of stages S (6 to
+// 9), so a stage has k-blocks of several producers.  A wait looks at a barrier's
+// parity alone: before its k-block i a producer waits for the end of k-block i - S,
+// and must not take that of i - 2 S for it.  It cannot, having waited for the end
+// of k-block i - 3 - S, which comes after i - 2 S.
+static_assert(kPairProducers < kPairStages, "a producer's last wait covers the stage's use before last");
 constexpr int kPairMaxAcc = 4;  // accumulators in TMEM
 constexpr int kPairStaging = 32 * 128;                      // per epilogue warp: 32 rows x 128 bytes
 constexpr int kPairBar = 256;
@@ -268,7 +276,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) pair_gemm_kernel(const __grid
     const int half_n = sh.bn / 2;
     const int rows64 = kLive ? (half_n + 16) / kLiveBox * kLiveBox : half_n, rows_b = max(rows64, half_n);
     const int b_bytes = kLive ? rows_b * 128 : kPairOperand;
-    const int stages = kLive ? min(kPairStages * kPairStage / (kPairOperand + b_bytes), kPairMaxStages) : kPairStages;
+    const int stages = kLive ? kPairStages * kPairStage / (kPairOperand + b_bytes) : kPairStages;
     uint8_t* sB = base + stages * kPairOperand;
     const int acc_cols = kLive ? sh.bn : 256, accs = kLive ? min(512 / acc_cols, kPairMaxAcc) : 2;
 
