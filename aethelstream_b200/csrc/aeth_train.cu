@@ -59,9 +59,9 @@ int head_bn(int64_t tiles_m, int64_t cols) {
 // Whether the tokens are the products' columns (pair_gemm.cuh): where tiles of
 // 256 rows would be a tenth larger than the columns that cover the tokens, and
 // masks may leave fewer still.  Measured at d 4096, vocabulary 32000, forward
-// and backward, rows against columns: 16 tokens 70.6 + 187.5 and 58 + 170
-// us; 300: 101 + 284 and 89 + 257; but 256: 72 + 216 and 75 + 220 (the blocks
-// are turned over in the epilogue), 512: 108 + 325 and 118 + 329.
+// and backward, rows against columns: 16 tokens 66.5 + 189 and 58.5 + 173
+// us; 300: 104 + 309 and 91 + 273; but 256: 69 + 237 and 72 + 250 (the blocks
+// are turned over in the epilogue), 512: 117 + 410 and 137 + 397.
 bool head_tokens_as_columns(int64_t n) {
     if (n > 1024) return false;
     const int64_t bn = pair_live_bn((int)n);
@@ -376,8 +376,8 @@ int decode(const CkptRead& a, void* out, int64_t ld_out, int dtype, cudaStream_t
 // The weight gradient's tiles that do not fill a wave are split along the tokens
 // where that takes 32 k-blocks or more (8 us) off the product; a kernel of its
 // own then adds up the ranges, for 5 us and a launch.  A call without and with
-// the split: 8170 x (216 x 952) 69 and 45 us (4 tiles), 8192 x (1024 x 1024) 54
-// and 43, 8192 x (5120 x 5120) 320 and 314; with 24 k-blocks less 2048 x (512 x
+// the split: 8170 x (216 x 952) 65 and 26 us (4 tiles), 8192 x (1024 x 1024) 51
+// and 31, 8192 x (5120 x 5120) 321 and 316; with 24 k-blocks less 2048 x (512 x
 // 2048) 22 and 28.
 struct GradTail {
     int full = 0, rest = 0, splits = 1;

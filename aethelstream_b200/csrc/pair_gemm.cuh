@@ -21,14 +21,18 @@
 // An epilogue may take the accumulator in pieces of kChunk k-blocks and add
 // them up in registers (Epi::kChunk > 0).  The tensor cores cut every partial
 // sum off toward zero, which shrinks a sum of K products by about K * 1e-9 of
-// itself (measured: 3.8e-6 at K = 4096); pieces of 512 keep that at 4e-7.  Tiles
+// itself (measured in bf16: 3.8e-6 at K = 4096); pieces of 512 keep that at 4e-7 to
+// 7e-7 (2.6e-6 in f16, whose products have more bits to cut).  The
+// logits are taken so, in the loss and in its gradient; sums that end in 16 bits
+// (over tokens or the vocabulary) are taken whole: 8e-6 at 8192 terms.  Tiles
 // of at most 160 columns have TMEM for three or four accumulators instead of two,
 // so that the MMAs go on while the epilogue ends a tile (300 and 512 tokens x 4096
 // x 32000, forward: 88.5 -> 86 and 117 -> 109 us).
 //
-// Measured, 3584 x 4096 x 32000 bf16: 561-591 us a product (1.59-1.68 PF/s at the
+// Measured, 3584 x 4096 x 32000 bf16: 568-608 us a product (1.54-1.65 PF/s at the
 // 1.5 GHz that the power cap leaves), tensor pipe 97-98 % active: the clock
-// bounds it.  With the issuer and one producer behind `lane == 0` 688 us, 71 %.
+// bounds it (92 % where G is written: its epilogue outlasts the two accumulators
+// that the MMAs are ahead).  With the issuer and one producer behind `lane == 0` 688 us, 71 %.
 //
 // M, N or K may be held on the device (`live`): the number of rows that a mask
 // leaves.  Operand rows past it, up to the next multiple of 256, must be zero.
@@ -40,7 +44,7 @@
 // took 530 with six stages, whose copies were not far enough ahead of the MMAs
 // (tensor pipe 52 % active, DRAM 44 %; 300 x 4096 x 32000, forward and backward:
 // 95 + 274 us with six, 89 + 257 with seven; 16 tokens, nine: 63 + 176 and 58 +
-// 170).  The
+// 170; before the gradient took its logits in pieces).  The
 // tile's columns are then the rows of the result, and epilogues turn each
 // 32 x 32 block over in shared memory (pair_transpose).
 // Tiles are walked in groups of row tiles so that the tiles in flight

@@ -76,10 +76,8 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
     }
 }
 
-// One lane of a converged warp.  The compiler knows that a branch on it leaves
-// one thread, and keeps the operands of copies and MMAs in uniform registers
-// there: a step of four MMAs, a wait and a commit takes 214 cycles to issue,
-// 444 behind `lane == 0` (measured).
+// One lane of a converged warp.  Behind it a step of four MMAs, a wait and a
+// commit takes 214 cycles to issue, behind `lane == 0` 444 (measured).
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
     asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(p));

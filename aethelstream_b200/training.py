@@ -106,8 +106,8 @@ def cut_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.
     """Cross entropy of softmax(hidden @ weight.T) against `labels`, the logits
     never stored.  hidden (..., d) and weight (vocab, d) are bfloat16 or
     float16; labels (...) are whole numbers.  Tokens labelled `ignore_index`
-    take no part: their loss is 0 and whatever their hidden state holds is not
-    read.  A label outside the vocabulary makes its token's loss and the mean
+    take no part: their loss is 0 and whatever their hidden state holds (NaN
+    too) reaches nothing.  A label outside the vocabulary makes its token's loss and the mean
     NaN and sets DEVERR_BAD_ARG in the device error word."""
     dev = hidden.get_device()
     if dev < 0 or dev != _current_device():
