@@ -357,8 +357,8 @@ def test_gradient_of_tokens_that_are_known(n, dt):
     in d_hidden.
 
     Bounds: loss and gradient make the same sums, in fp32 pieces of 512 products,
-    each within c = 2e-6 of sum |h w| = S (the tensor cores' 512 * 1e-9, and 16
-    additions); p of such logits is within p (1 - p) 2 c S.  lse is rounded at four
+    each within c = 4e-6 of sum |h w| = S (the tensor cores' cut, up to 2.6e-6 in
+    f16, and 16 additions); p of such logits is within p (1 - p) 2 c S.  lse is rounded at four
     places, and the exponentials and the logarithm are within 2^-20: p e_x.  G and
     the output are rounded once."""
     import aethelstream_b200 as A
@@ -384,7 +384,7 @@ def test_gradient_of_tokens_that_are_known(n, dt):
     G[torch.arange(n), lab] = -(p.scatter(1, at, 0.0)).sum(1)  # p - 1 without its cancellation
     S = (hd.abs() @ wd.abs().T).amax(1, keepdim=True)
     e_x = 4 * 2.0 ** -24 * (1 + lse.abs()[:, None]) + 2.0 ** -20
-    e_g = p * (1 - p) * 4e-6 * S + p * e_x + 1.1 * U[dt] * G.abs() + (2.0 ** -40 if dt is torch.float16 else 0.0)
+    e_g = p * (1 - p) * 8e-6 * S + p * e_x + 1.1 * U[dt] * G.abs() + (2.0 ** -40 if dt is torch.float16 else 0.0)
     tiny = 2.0 ** -24 if dt is torch.float16 else 1e-38
     acc = 2 * 2.0 ** -24
     want = G @ wd
