@@ -82,7 +82,7 @@ def build(force: bool = False, verbose: bool = False, extra: list[str] | None = 
     for unit, obj in zip(UNITS, objects):
         src = os.path.join(CSRC, unit + ".cu")
         if force or extra or stale(obj, unit):
-            cmd = [nvcc(), *NVCC_FLAGS, *(extra or []), "-I", os.path.join(ROOT, "include"), "-c", src, "-o", obj + ".tmp"]
+            cmd = [nvcc(), *NVCC_FLAGS, *(extra or []), "-I", os.path.join(ROOT, "include"), "-c", src, "-o", obj[:-2] + ".part.o"]
             if verbose:
                 print(" ".join(cmd))
             compiles.append((obj, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
@@ -91,7 +91,7 @@ def build(force: bool = False, verbose: bool = False, extra: list[str] | None = 
         if p.returncode != 0:
             sys.stderr.write(out)
         else:
-            os.replace(obj + ".tmp", obj)  # whole, or not at all
+            os.replace(obj[:-2] + ".part.o", obj)  # whole, or not at all
             if verbose and out:
                 print(out)
     if any(p.returncode != 0 for _, p in compiles):
