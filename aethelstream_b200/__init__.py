@@ -2,9 +2,10 @@
 
 NF4 weight dequantisation, GaLore projection (tcgen05 tensor cores), INT8
 low-rank Adam, back-projection with a fused NF4 weight write, and a LOMO fused
-full-rank update, and the training operators that make the step's gradients
-(head loss, 8-bit activation checkpoints), behind the C ABI in
-include/aeth_galore.h.  Importing this
+full-rank update, AdamW over many tensors for what the low-rank step leaves, and the
+training operators that make the step's gradients (head loss, 8-bit activation
+checkpoints, rotary positions and per-head norms of queries and keys), behind the
+C ABI in include/aeth_galore.h.  Importing this
 package loads libaeth_galore.so and raises ImportError if it is missing: there
 is no CPU fallback.
 """
@@ -34,6 +35,8 @@ from .galore import (  # noqa: E402
     randomized_svd_fast,
     randomized_svd_sketch,
 )
+from .adamw import AdamWState, adamw_moments, adamw_step  # noqa: E402
+from .qk import RotaryPlan, qk_norm_rotary, qk_norm_rotary_backward, rotary, rotary_backward  # noqa: E402
 from .training import (  # noqa: E402
     ActivationCheckpoint,
     CutCrossEntropy,
@@ -50,5 +53,6 @@ __all__ = [
     "ProjectorKind", "deferred_apply_with_clip", "load", "lomo_sqnorm", "lomo_update", "nf4_dequantize", "nf4_quantize", "randomized_svd", "randomized_svd_fast", "randomized_svd_sketch",
     "ActivationCheckpoint", "CutCrossEntropy", "checkpoint_decode", "checkpoint_weight_grad", "cut_cross_entropy",
     "cut_cross_entropy_backward", "rms_norm_checkpoint", "rms_norm_checkpoint_backward",
-    "_lib",
+    "AdamWState", "adamw_moments", "adamw_step", "RotaryPlan", "qk_norm_rotary", "qk_norm_rotary_backward", "rotary",
+    "rotary_backward", "_lib",
 ]

@@ -5,8 +5,9 @@
 Run it as a script (or load it by file path): importing the package itself
 requires the built library.
 
-The library is two translation units, compiled side by side: csrc/aeth_galore.cu
-(the optimizer step) and csrc/aeth_train.cu (the training operators around it).
+The library is three translation units, compiled side by side: csrc/aeth_galore.cu
+(the optimizer step), csrc/aeth_train.cu (the training operators around it) and
+csrc/aeth_rotary.cu (queries and keys).
 It is linked against the static CUDA runtime, so it only needs the driver on the
 machine that loads it.  No fast-math: the NF4/INT8 codes and the REF-mode arithmetic must round
 exactly like the CPU definition.
@@ -25,7 +26,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libaeth_galore.so")
 OBJ = os.path.join(HERE, "_obj")  # object files, kept so an unchanged unit is not compiled again
-UNITS = ("aeth_galore", "aeth_train")
+UNITS = ("aeth_galore", "aeth_train", "aeth_rotary")
 ROOT = os.path.dirname(HERE)
 
 NVCC_FLAGS = [

@@ -14,6 +14,7 @@
 #include <vector>
 
 #include "adam.cuh"
+#include "adamw.cuh"
 #include "codec.cuh"
 #include "common.cuh"
 #include "gemm_simt.cuh"
@@ -2419,6 +2420,154 @@ int aeth_lomo_update(const void* grad_bf16, int64_t n, const double* sq_dev, flo
                                             (int64_t)num_sms() * std::max(per_sm, 1));
     kern<<<grid, kLomoThreads, kLomoSmem, to_stream(stream)>>>(gb, n, sq_dev, max_norm, lr, beta, mom8, mom_scales,
                                                                w_packed, w_absmax, prequant_out, 1u);
+    AETH_LAUNCH_CHECK();
+    return AETH_OK;
+}
+
+// ---------------------------------------------------------------------------
+// AdamW over many tensors
+// ---------------------------------------------------------------------------
+}  // extern "C"
+
+namespace {
+
+template <int CAP, bool MASTER>
+int adamw_launch(const AdamwArgs<CAP>& a, int bits, cudaStream_t st) {
+    if (bits == 8) {
+        auto kern = adamw8_kernel<CAP, MASTER>;
+        static std::atomic<bool> allowed[kMaxDevices] = {};
+        AETH_TRY(allow_shared(kern, kAdamw8Shared, allowed));
+        kern<<<std::max(std::min((a.blocks + 3) / 4, num_sms()), 1), kAdamw8Threads, kAdamw8Shared, st>>>(a);
+    } else {
+        adamw_kernel<CAP, MASTER><<<std::max(std::min(a.blocks, 6 * num_sms()), 1), 256, 0, st>>>(a);
+    }
+    AETH_LAUNCH_CHECK();
+    return AETH_OK;
+}
+
+struct AdamwList {
+    void* const* p;
+    const void* const* g;
+    const int64_t* n;
+    const uint8_t *p_dtype, *g_dtype, *decay;
+    int count;
+};
+// Launches for the tensors from `i` on that have a gradient: as many as a table
+// takes.  `block`: the first block of tensor i's moments.
+template <int CAP>
+int adamw_some(const AdamwList& l, int& i, int64_t& block, AdamwArgs<CAP>& a, int bits, cudaStream_t st) {
+    a.count = 0;
+    int64_t blocks = 0;
+    for (; i < l.count && a.count < CAP; ++i) {
+        const int64_t nb = (l.n[i] + kAdamwBlock - 1) / kAdamwBlock;
+        if (l.g[i] && nb > 0) {
+            if (blocks + nb > (1 << 30)) break;  // one tensor alone has fewer (aeth_adamw_step)
+            AdamwTensor& t = a.t[a.count];
+            t.p = l.p[i];
+            t.g = l.g[i];
+            t.n = l.n[i];
+            t.first = (int)blocks;
+            t.p_dtype = l.p_dtype[i];
+            t.g_dtype = l.g_dtype[i];
+            t.whole = ((reinterpret_cast<uintptr_t>(t.p) | reinterpret_cast<uintptr_t>(t.g)) & 15) == 0;
+            t.decay = !l.decay || l.decay[i];
+            a.at[a.count++] = (int)block;
+            blocks += nb;
+        }
+        block += nb;
+    }
+    a.blocks = (int)blocks;
+    a.last = i == l.count;
+    return a.master ? adamw_launch<CAP, true>(a, bits, st) : adamw_launch<CAP, false>(a, bits, st);
+}
+template <int CAP>
+int adamw_all(const AdamwList& l, const AethAdamwState& s, double b1, double b2, float eps, float lr, const float* lr_dev,
+              float decay, const float* clip, cudaStream_t st) {
+    AdamwArgs<CAP> a;
+    a.m = s.m;
+    a.v = s.v;
+    a.m_scales = s.m_scales;
+    a.v_scales = s.v_scales;
+    a.master = s.master;
+    a.step = s.step;
+    a.clip = clip;
+    a.lr_dev = lr_dev;
+    a.lr = lr;
+    a.eps = eps;
+    a.decay = decay;
+    a.beta1 = b1;
+    a.beta2 = b2;
+    a.one = 1u;
+    int i = 0;
+    int64_t block = 0;
+    do AETH_TRY(adamw_some<CAP>(l, i, block, a, s.bits, st));
+    while (i < l.count);
+    return AETH_OK;
+}
+
+int adamw_state_check(const AethAdamwState* s) {
+    if (!s || (s->bits != 32 && s->bits != 8) || s->blocks < 0 || !s->step) return AETH_ERR_ARG;
+    if (s->blocks > 0 && (!s->m || !s->v || (s->bits == 8 && (!s->m_scales || !s->v_scales)))) return AETH_ERR_ARG;
+    if ((reinterpret_cast<uintptr_t>(s->m) | reinterpret_cast<uintptr_t>(s->v) | reinterpret_cast<uintptr_t>(s->master)) & 15)
+        return AETH_ERR_UNSUPPORTED;
+    if (s->blocks > (1 << 30)) return AETH_ERR_UNSUPPORTED;
+    return AETH_OK;
+}
+
+// Whether two tensors that the step writes share memory
+bool adamw_overlap(const AdamwList& l) {
+    std::vector<std::pair<uintptr_t, uintptr_t>> r;
+    r.reserve((size_t)l.count);
+    for (int i = 0; i < l.count; ++i)
+        if (l.n[i] > 0) {
+            const uintptr_t a = reinterpret_cast<uintptr_t>(l.p[i]);
+            r.emplace_back(a, a + (uintptr_t)l.n[i] * (l.p_dtype[i] == AETH_DTYPE_F32 ? 4 : 2));
+        }
+    std::sort(r.begin(), r.end());
+    for (size_t i = 1; i < r.size(); ++i)
+        if (r[i].first < r[i - 1].second) return true;
+    return false;
+}
+
+}  // namespace
+
+extern "C" {
+
+int aeth_adamw_step(void* const* p, const void* const* g, const int64_t* n, const uint8_t* p_dtype, const uint8_t* g_dtype,
+                    const uint8_t* decay, int count, const AethAdamwState* state, double beta1, double beta2, float eps,
+                    float lr, const float* lr_dev, float weight_decay, const float* clip_dev, aeth_stream_t stream) {
+    if (count < 0 || (count > 0 && (!p || !g || !n || !p_dtype || !g_dtype))) return set_err(AETH_ERR_ARG);
+    AETH_TRY(adamw_state_check(state));
+    int64_t blocks = 0;
+    for (int i = 0; i < count; ++i) {
+        if (n[i] < 0 || p_dtype[i] > AETH_DTYPE_BF16 || g_dtype[i] > AETH_DTYPE_BF16 || (n[i] > 0 && !p[i]))
+            return set_err(AETH_ERR_ARG);
+        if (n[i] > (int64_t)kAdamwBlock << 30) return set_err(AETH_ERR_UNSUPPORTED);
+        blocks += (n[i] + kAdamwBlock - 1) / kAdamwBlock;
+    }
+    if (blocks > state->blocks) return set_err(AETH_ERR_ARG);
+    const AdamwList l{p, g, n, p_dtype, g_dtype, decay, count};
+    try {
+        if (adamw_overlap(l)) return set_err(AETH_ERR_ARG);
+    } catch (...) {
+        return set_err((int)cudaErrorMemoryAllocation);
+    }
+    if (state->bits == 8) AETH_TRY(codec_maps_ensure());
+    cudaStream_t st = to_stream(stream);
+    return count <= kAdamwFew ? adamw_all<kAdamwFew>(l, *state, beta1, beta2, eps, lr, lr_dev, weight_decay, clip_dev, st)
+                              : adamw_all<kAdamwTensors>(l, *state, beta1, beta2, eps, lr, lr_dev, weight_decay, clip_dev, st);
+}
+
+int aeth_adamw_moments(const AethAdamwState* state, float* m_out, float* v_out, aeth_stream_t stream) {
+    AETH_TRY(adamw_state_check(state));
+    if (state->bits != 8 || (state->blocks > 0 && (!m_out || !v_out))) return set_err(AETH_ERR_ARG);
+    if ((reinterpret_cast<uintptr_t>(m_out) | reinterpret_cast<uintptr_t>(v_out)) & 15) return set_err(AETH_ERR_UNSUPPORTED);
+    if (state->blocks == 0) return AETH_OK;
+    AETH_TRY(codec_maps_ensure());
+    const int64_t n16 = state->blocks * (kAdamwBlock / 16);
+    adamw_decode_kernel<<<(unsigned)std::min<int64_t>((n16 + 255) / 256, 8 * num_sms()), 256, 0, to_stream(stream)>>>(
+        static_cast<const int8_t*>(state->m), static_cast<const int8_t*>(state->v), state->m_scales, state->v_scales, n16,
+        m_out, v_out);
     AETH_LAUNCH_CHECK();
     return AETH_OK;
 }

@@ -1,0 +1,219 @@
+// aeth_rotary.cu -- libaeth_galore: rotary positions of queries and keys, and
+// their per-head norms with the rotation in the same pass (section 3c of
+// include/aeth_galore.h).
+#include <algorithm>
+
+#include "rotary.cuh"
+#include "tmap.cuh"
+
+using namespace aeth;
+
+namespace {
+
+constexpr int64_t kRotMaxRows = 1ll << 40;
+
+bool rot_dtype(int dtype) { return dtype == AETH_DTYPE_F32 || dtype == AETH_DTYPE_F16 || dtype == AETH_DTYPE_BF16; }
+int rot_size(int dtype) { return dtype == AETH_DTYPE_F32 ? 4 : 2; }
+int64_t rot_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+
+int rot_check(const AethRotaryPlan* p, int64_t tokens, int head_dim, int hq, int hk, int dtype) {
+    if (!p || tokens < 0 || head_dim <= 0 || hq < 0 || hk < 0 || hq + hk == 0 || !rot_dtype(dtype)) return AETH_ERR_ARG;
+    if (p->rotary_dim < 2 || p->rotary_dim % 2 || p->rotary_dim > head_dim) return AETH_ERR_ARG;
+    if (!p->freq || p->position_bits != 32 && p->position_bits != 64) return AETH_ERR_ARG;
+    if (tokens > 0 && (!p->positions || p->period <= 0)) return AETH_ERR_ARG;
+    if (head_dim > kRotMaxHead || tokens > kRotMaxRows || hq > (1 << 20) || hk > (1 << 20)) return AETH_ERR_UNSUPPORTED;
+    if (tokens * ((int64_t)hq + hk) > kRotMaxRows) return AETH_ERR_UNSUPPORTED;
+    return AETH_OK;
+}
+int rot_heads(const AethHeads& h, int64_t tokens, const void* out) {
+    if (h.heads == 0 || tokens == 0) return AETH_OK;
+    return h.data && out && h.ld_token >= 0 && h.ld_head >= 0 ? AETH_OK : AETH_ERR_ARG;
+}
+
+// Whether every head row can be taken in 16-byte pieces
+bool rot_whole(const AethHeads& h, int64_t tokens, int size) {
+    if (h.heads == 0) return true;
+    return reinterpret_cast<uintptr_t>(h.data) % 16 == 0 && (tokens == 1 || h.ld_token * size % 16 == 0) &&
+           (h.heads == 1 || h.ld_head * size % 16 == 0);
+}
+
+// Rows of a stretch and CTAs of the grid.  A stretch is what gives every SM six
+// CTAs, 512 rows at most and what the table of its tokens holds; `most`: CTAs
+// that q and k may have together (0: one for each stretch).
+void rot_grid(RotaryArgs& a, int64_t tokens, int step, int most) {
+    const int held = kRotTableBytes / (4 * a.R);  // tokens; 8 at least
+    const int64_t all = a.s[0].rows + a.s[1].rows;
+    int64_t rows = rot_up((all + 6 * num_sms() - 1) / (6 * num_sms()), step);
+    rows = std::min<int64_t>(rows, 512);
+    int64_t table = 0;
+    for (RotaryRows& s : a.s) {
+        if (s.rows == 0) {
+            s.stretch = 1;
+            s.ctas = 0;
+            continue;
+        }
+        s.stretch = (int)std::min<int64_t>(rows, (int64_t)(held - 2) * s.heads + 1);
+        int64_t n = (s.rows + s.stretch - 1) / s.stretch;
+        if (most > 0) n = std::min<int64_t>(n, std::max<int64_t>(s.rows * most / all, 1));
+        s.ctas = (unsigned)std::min<int64_t>(n, 1 << 30);
+        table = std::max<int64_t>(table, std::min<int64_t>((s.stretch + s.heads - 2) / s.heads + 1, tokens) * a.R * 4);
+    }
+    a.table_bytes = (int)rot_up(table, 16);
+}
+
+constexpr int kRotBackPerSm = 4;  // CTAs of the norm's gradient, each of which leaves sums of the gain's
+int rot_back_ctas() { return kRotBackPerSm * num_sms(); }
+
+template <typename T, bool INTER, int OP>
+int rot_launch(RotaryArgs& a, int64_t tokens, bool whole, cudaStream_t st) {
+    constexpr int U = sizeof(T) == 4 ? (OP == ROT_NORM_BACK ? 1 : 2) : (OP == ROT_NORM_BACK ? 2 : 4);
+    const int most = OP == ROT_NORM_BACK ? rot_back_ctas() : 0;
+    if (whole && a.D % 16 == 0 && a.R % 16 == 0 && a.D <= 512) {
+        int lanes = 1;
+        while (lanes < a.D / 16) lanes *= 2;
+        const int groups = kRotThreads / lanes;
+        rot_grid(a, tokens, groups * U, most);
+        if (OP == ROT_NORM_BACK) a.table_bytes = std::max(a.table_bytes, groups * a.D * 4);
+        const int smem = a.table_bytes + (OP == ROT_TURN ? 0 : a.D * 4);
+        rotary_kernel<T, INTER, OP, U><<<a.s[0].ctas + a.s[1].ctas, kRotThreads, smem, st>>>(a, lanes);
+    } else {
+        rot_grid(a, tokens, kRotThreads / 32, most);
+        const int smem = a.table_bytes + (OP == ROT_NORM_BACK ? kRotThreads / 32 * a.D * 4 : 0);
+        auto kern = rotary_any_kernel<T, INTER, OP>;
+        static std::atomic<bool> allowed[kMaxDevices] = {};
+        AETH_TRY(allow_shared(kern, 2 * kRotTableBytes, allowed));
+        kern<<<a.s[0].ctas + a.s[1].ctas, kRotThreads, smem, st>>>(a);
+    }
+    AETH_LAUNCH_CHECK();
+    return AETH_OK;
+}
+
+template <int OP>
+int rot_typed(RotaryArgs& a, int64_t tokens, int dtype, bool inter, bool whole, cudaStream_t st) {
+    if (dtype == AETH_DTYPE_F32)
+        return inter ? rot_launch<float, true, OP>(a, tokens, whole, st) : rot_launch<float, false, OP>(a, tokens, whole, st);
+    if (dtype == AETH_DTYPE_F16)
+        return inter ? rot_launch<__half, true, OP>(a, tokens, whole, st) : rot_launch<__half, false, OP>(a, tokens, whole, st);
+    return inter ? rot_launch<__nv_bfloat16, true, OP>(a, tokens, whole, st)
+                 : rot_launch<__nv_bfloat16, false, OP>(a, tokens, whole, st);
+}
+
+RotaryArgs rot_args(const AethRotaryPlan& p, const AethHeads& q, const AethHeads& k, int64_t tokens, int head_dim, void* q_out,
+                    void* k_out, bool flip) {
+    RotaryArgs a = {};
+    const AethHeads* h[2] = {&q, &k};
+    void* out[2] = {q_out, k_out};
+    for (int i = 0; i < 2; ++i) {
+        a.s[i].x = h[i]->data;
+        a.s[i].ld_t = h[i]->ld_token;
+        a.s[i].ld_h = h[i]->ld_head;
+        a.s[i].out = out[i];
+        a.s[i].heads = std::max(h[i]->heads, 1);
+        a.s[i].rows = tokens * h[i]->heads;
+    }
+    a.pos = p.positions;
+    a.pos32 = p.position_bits == 32;
+    a.period = p.period;
+    a.freq = p.freq;
+    a.amp = p.amplitude;
+    a.flip = flip;
+    a.D = head_dim;
+    a.R = p.rotary_dim;
+    return a;
+}
+bool rot_out_whole(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }  // rows of D, whose bytes 16 divides
+
+}  // namespace
+
+extern "C" {
+
+int aeth_rotary(const AethRotaryPlan* plan, const AethHeads* q, const AethHeads* k, int64_t tokens, int head_dim, int dtype,
+                int inverse, void* q_out, void* k_out, aeth_stream_t stream) {
+    if (!q || !k) return set_err(AETH_ERR_ARG);
+    AETH_TRY(rot_check(plan, tokens, head_dim, q->heads, k->heads, dtype));
+    AETH_TRY(rot_heads(*q, tokens, q_out));
+    AETH_TRY(rot_heads(*k, tokens, k_out));
+    if (tokens == 0) return AETH_OK;
+    RotaryArgs a = rot_args(*plan, *q, *k, tokens, head_dim, q_out, k_out, inverse != 0);
+    const int size = rot_size(dtype);
+    const bool whole = rot_whole(*q, tokens, size) && rot_whole(*k, tokens, size) && rot_out_whole(q_out) && rot_out_whole(k_out);
+    return rot_typed<ROT_TURN>(a, tokens, dtype, plan->interleaved != 0, whole, to_stream(stream));
+}
+
+int aeth_qk_norm_rotary(const AethRotaryPlan* plan, const AethHeads* q, const AethHeads* k, const void* q_gain,
+                        const void* k_gain, int gain_dtype, float eps, int64_t tokens, int head_dim, int dtype, void* q_out,
+                        void* k_out, aeth_stream_t stream) {
+    if (!q || !k) return set_err(AETH_ERR_ARG);
+    AETH_TRY(rot_check(plan, tokens, head_dim, q->heads, k->heads, dtype));
+    AETH_TRY(rot_heads(*q, tokens, q_out));
+    AETH_TRY(rot_heads(*k, tokens, k_out));
+    if (!rot_dtype(gain_dtype) || (q->heads && !q_gain) || (k->heads && !k_gain)) return set_err(AETH_ERR_ARG);
+    if (tokens == 0) return AETH_OK;
+    RotaryArgs a = rot_args(*plan, *q, *k, tokens, head_dim, q_out, k_out, false);
+    a.s[0].gain = q_gain;
+    a.s[1].gain = k_gain;
+    a.gain_dtype = gain_dtype;
+    a.eps = eps;
+    const int size = rot_size(dtype);
+    const bool whole = rot_whole(*q, tokens, size) && rot_whole(*k, tokens, size) && rot_out_whole(q_out) && rot_out_whole(k_out);
+    return rot_typed<ROT_NORM>(a, tokens, dtype, plan->interleaved != 0, whole, to_stream(stream));
+}
+
+int aeth_qk_norm_rotary_backward_workspace(int head_dim, size_t* bytes) {
+    if (head_dim <= 0 || !bytes) return set_err(AETH_ERR_ARG);
+    if (head_dim > kRotMaxHead) return set_err(AETH_ERR_UNSUPPORTED);
+    *bytes = (size_t)(rot_back_ctas() + 2) * (size_t)head_dim * sizeof(float);
+    return AETH_OK;
+}
+
+int aeth_qk_norm_rotary_backward(const AethRotaryPlan* plan, const AethHeads* dq, const AethHeads* dk, const AethHeads* q,
+                                 const AethHeads* k, const void* q_gain, const void* k_gain, int gain_dtype, float eps,
+                                 int64_t tokens, int head_dim, int dtype, void* dq_out, void* dk_out, float* d_q_gain,
+                                 float* d_k_gain, void* workspace, size_t workspace_bytes, aeth_stream_t stream) {
+    if (!q || !k || !dq || !dk || dq->heads != q->heads || dk->heads != k->heads) return set_err(AETH_ERR_ARG);
+    AETH_TRY(rot_check(plan, tokens, head_dim, q->heads, k->heads, dtype));
+    for (const AethHeads* h : {q, dq}) AETH_TRY(rot_heads(*h, tokens, dq_out));
+    for (const AethHeads* h : {k, dk}) AETH_TRY(rot_heads(*h, tokens, dk_out));
+    if (!rot_dtype(gain_dtype) || (q->heads && (!q_gain || !d_q_gain)) || (k->heads && (!k_gain || !d_k_gain)))
+        return set_err(AETH_ERR_ARG);
+    cudaStream_t st = to_stream(stream);
+    if (tokens == 0) {
+        if (q->heads) AETH_CUDA(cudaMemsetAsync(d_q_gain, 0, sizeof(float) * (size_t)head_dim, st));
+        if (k->heads) AETH_CUDA(cudaMemsetAsync(d_k_gain, 0, sizeof(float) * (size_t)head_dim, st));
+        return AETH_OK;
+    }
+    size_t need = 0;
+    AETH_TRY(aeth_qk_norm_rotary_backward_workspace(head_dim, &need));
+    if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16) return set_err(AETH_ERR_ARG);
+    RotaryArgs a = rot_args(*plan, *q, *k, tokens, head_dim, dq_out, dk_out, true);
+    const AethHeads* dy[2] = {dq, dk};
+    for (int i = 0; i < 2; ++i) {
+        a.s[i].dy = dy[i]->data;
+        a.s[i].ld_dt = dy[i]->ld_token;
+        a.s[i].ld_dh = dy[i]->ld_head;
+    }
+    a.s[0].gain = q_gain;
+    a.s[1].gain = k_gain;
+    a.gain_dtype = gain_dtype;
+    a.eps = eps;
+    // q's CTAs and k's together: rot_back_ctas(), or one more of either for the share that rounds down to none
+    a.s[0].part = static_cast<float*>(workspace);
+    const int size = rot_size(dtype);
+    bool whole = rot_out_whole(dq_out) && rot_out_whole(dk_out);
+    for (const AethHeads* h : {q, k, dq, dk}) whole = whole && rot_whole(*h, tokens, size);
+    const int64_t all = a.s[0].rows + a.s[1].rows;
+    a.s[1].part = a.s[0].part + (std::max<int64_t>(a.s[0].rows * rot_back_ctas() / all, 1)) * head_dim;
+    AETH_TRY(rot_typed<ROT_NORM_BACK>(a, tokens, dtype, plan->interleaved != 0, whole, st));
+    const RotaryGain g{{a.s[0].part, a.s[1].part}, {d_q_gain, d_k_gain}, {(int)a.s[0].ctas, (int)a.s[1].ctas}, head_dim};
+    const bool both = q->heads && k->heads;
+    RotaryGain only = g;
+    if (!q->heads) {
+        only.part[0] = g.part[1];
+        only.out[0] = g.out[1];
+        only.groups[0] = g.groups[1];
+    }
+    AETH_CUDA(launch_after(rotary_gain_kernel, dim3((unsigned)(head_dim + 31) / 32, both ? 2 : 1), dim3(1024), 0, st, 1, only));
+    return AETH_OK;
+}
+
+}  // extern "C"

@@ -130,30 +130,48 @@ inline void build_dmap_lut4(const uint2* lut8, int halves, int log2p, uint32_t* 
     }
 }
 
-inline bool g_maps_uploaded[kMaxDevices] = {};
+inline std::atomic<bool> g_maps_uploaded[kMaxDevices] = {};
 
+inline cudaError_t codec_maps_upload(cudaStream_t st) {
+    static float s[256], u[256];
+    static uint2 lut_s[2 * kDmapLutEntries], lut_u[kDmapLutUEntries];
+    static uint32_t lut4_s[2 * kDmapLutEntries], lut4_u[kDmapLutUEntries];
+    build_dynamic_map(1, s);
+    build_dynamic_map(0, u);
+    build_dmap_lut(s, 2, kDmapLutLog2P, lut_s);
+    build_dmap_lut(u, 1, kDmapLutULog2P, lut_u);
+    build_dmap_lut4(lut_s, 2, kDmapLutLog2P, lut4_s);
+    build_dmap_lut4(lut_u, 1, kDmapLutULog2P, lut4_u);
+    cudaError_t e = cudaMemcpyToSymbolAsync(c_dmap_signed, s, sizeof(s), 0, cudaMemcpyHostToDevice, st);
+    auto next = [&](auto& symbol, const auto& from) {
+        if (e == cudaSuccess) e = cudaMemcpyToSymbolAsync(symbol, from, sizeof(from), 0, cudaMemcpyHostToDevice, st);
+    };
+    next(c_dmap_unsigned, u);
+    next(g_dmap_lut_s, lut_s);
+    next(g_dmap_lut_u, lut_u);
+    next(g_dmap_lut4_s, lut4_s);
+    next(g_dmap_lut4_u, lut4_u);
+    return e == cudaSuccess ? cudaStreamSynchronize(st) : e;
+}
+
+// As alloc_zeroed_word, the upload may come while a stream is being captured:
+// it goes to a stream of its own that no capture sees.
 inline int codec_maps_ensure() {
     int dev = 0;
     AETH_TRY(current_device(&dev));
     if (dev < 0 || dev >= kMaxDevices) return set_err(AETH_ERR_UNSUPPORTED);
-    if (!g_maps_uploaded[dev]) {
-        float s[256], u[256];
-        build_dynamic_map(1, s);
-        build_dynamic_map(0, u);
-        AETH_CUDA(cudaMemcpyToSymbol(c_dmap_signed, s, sizeof(s)));
-        AETH_CUDA(cudaMemcpyToSymbol(c_dmap_unsigned, u, sizeof(u)));
-        static uint2 lut_s[2 * kDmapLutEntries], lut_u[kDmapLutUEntries];
-        build_dmap_lut(s, 2, kDmapLutLog2P, lut_s);
-        build_dmap_lut(u, 1, kDmapLutULog2P, lut_u);
-        AETH_CUDA(cudaMemcpyToSymbol(g_dmap_lut_s, lut_s, sizeof(lut_s)));
-        AETH_CUDA(cudaMemcpyToSymbol(g_dmap_lut_u, lut_u, sizeof(lut_u)));
-        static uint32_t lut4_s[2 * kDmapLutEntries], lut4_u[kDmapLutUEntries];
-        build_dmap_lut4(lut_s, 2, kDmapLutLog2P, lut4_s);
-        build_dmap_lut4(lut_u, 1, kDmapLutULog2P, lut4_u);
-        AETH_CUDA(cudaMemcpyToSymbol(g_dmap_lut4_s, lut4_s, sizeof(lut4_s)));
-        AETH_CUDA(cudaMemcpyToSymbol(g_dmap_lut4_u, lut4_u, sizeof(lut4_u)));
-        g_maps_uploaded[dev] = true;
-    }
+    if (g_maps_uploaded[dev].load(std::memory_order_acquire)) return AETH_OK;
+    std::lock_guard<std::mutex> lock(g_rt_mu);
+    if (g_maps_uploaded[dev].load(std::memory_order_relaxed)) return AETH_OK;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    AETH_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+    cudaStream_t st = nullptr;
+    cudaError_t e = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking);
+    if (e == cudaSuccess) e = codec_maps_upload(st);
+    if (st) cudaStreamDestroy(st);
+    cudaThreadExchangeStreamCaptureMode(&mode);  // as it was
+    AETH_CUDA(e);
+    g_maps_uploaded[dev].store(true, std::memory_order_release);
     return AETH_OK;
 }
 

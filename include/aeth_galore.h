@@ -583,6 +583,85 @@ int aeth_checkpoint_weight_grad(const void* dy, int64_t ld_dy, const int8_t* cod
                                 aeth_stream_t stream);
 
 /* ======================================================================
+ * 3c. Rotary positions of queries and keys, and per-head norms with the rotation
+ *     in the same pass.  Of a head's D features the first rotary_dim turn in
+ *     pairs (u, v), (x_p, x_{p + rotary_dim / 2}) or, interleaved, (x_2p,
+ *     x_{2p+1}): at position t by the angle t f_p,
+ *       u' = a (u cos - v sin), v' = a (v cos + u sin).
+ *     Frequencies are whole numbers: freq[p] = 2^64 times the turns that pair p
+ *     makes from one position to the next, modulo 2^64; the angle t freq[p] is
+ *     then exact at any position, negative ones too.
+ *     Rows: head h of token i lies at data + i * ld_token + h * ld_head
+ *     (elements), its features side by side; outputs are contiguous (token, head,
+ *     feature) and must not overlap an input.  F32, F16 or BF16; arithmetic in
+ *     fp32.  Any head_dim up to 1024; heads of whole sixteens up to 512 whose rows
+ *     start on 16 bytes are the fast ones.  A side with heads = 0 is left out.
+ *     Nothing synchronises or allocates.
+ * ====================================================================== */
+typedef struct {
+    const void* positions; /* device: of token i, positions[i % period] */
+    int position_bits;     /* 64 or 32 */
+    int64_t period;
+    const uint64_t* freq;  /* device: rotary_dim / 2 */
+    int rotary_dim;        /* even */
+    int interleaved;
+    float amplitude;       /* a */
+} AethRotaryPlan;
+typedef struct {
+    const void* data;
+    int64_t ld_token, ld_head;
+    int heads;
+} AethHeads;
+/* inverse: turns the other way (with the same amplitude): the gradient. */
+int aeth_rotary(const AethRotaryPlan* plan, const AethHeads* q, const AethHeads* k, int64_t tokens, int head_dim, int dtype,
+                int inverse, void* q_out, void* k_out, aeth_stream_t stream);
+/* y = turned(x r gain), r = 1 / sqrt(mean x^2 + eps) over the head's features;
+ * gains of head_dim, of a type of their own. */
+int aeth_qk_norm_rotary(const AethRotaryPlan* plan, const AethHeads* q, const AethHeads* k, const void* q_gain,
+                        const void* k_gain, int gain_dtype, float eps, int64_t tokens, int head_dim, int dtype, void* q_out,
+                        void* k_out, aeth_stream_t stream);
+/* Its gradient at q and k: with g the turned-back dq, dq_out = r (gain g) -
+ * q r^3 mean(gain g q) and d_q_gain = sum of g q r over tokens and heads (F32,
+ * in an order that the sizes alone decide); k's the same. */
+int aeth_qk_norm_rotary_backward_workspace(int head_dim, size_t* bytes);
+int aeth_qk_norm_rotary_backward(const AethRotaryPlan* plan, const AethHeads* dq, const AethHeads* dk, const AethHeads* q,
+                                 const AethHeads* k, const void* q_gain, const void* k_gain, int gain_dtype, float eps,
+                                 int64_t tokens, int head_dim, int dtype, void* dq_out, void* dk_out, float* d_q_gain,
+                                 float* d_k_gain, void* workspace, size_t workspace_bytes, aeth_stream_t stream);
+
+/* ======================================================================
+ * 3d. AdamW over many tensors at once: what the low-rank step leaves out.
+ *       g = clip g; m = beta1 m + (1 - beta1) g; v = beta2 v + (1 - beta2) g^2;
+ *       p -= lr (m / (1 - beta1^t) / (sqrt(v / (1 - beta2^t)) + eps) + weight_decay p)
+ *     in fp32, t the step counted on the device (*step + 1; the call leaves t).
+ *     Tensor i has n[i] elements of p_dtype[i] at p[i] and a gradient of
+ *     g_dtype[i] at g[i] (NULL: left out of this step), both contiguous, and decays
+ *     where decay[i] is not 0 (decay NULL: all do).  Its moments lie in m and v
+ *     from block sum_{j<i} ceil(n[j] / 2048) on, blocks of 2048 elements: floats
+ *     (bits 32), or the dynamic map's codes (bits 8) with one scale per block, the
+ *     block's largest magnitude (0 where that is below 2^-126; NaN where the block
+ *     holds a NaN or an infinity).  master (or NULL): fp32 parameters laid out as
+ *     the moments, which the step is taken on; p gets their rounding.
+ *     m, v and master 16-byte aligned.  Parameters that overlap one another:
+ *     AETH_ERR_ARG.  Nothing synchronises; with bits 32 nothing allocates, with
+ *     bits 8 the library's first call on a device uploads its maps.
+ * ====================================================================== */
+typedef struct {
+    int bits; /* 32 or 8 */
+    void *m, *v;
+    float *m_scales, *v_scales; /* bits 8 */
+    float* master;
+    int64_t* step;  /* device */
+    int64_t blocks; /* that m and v have room for */
+} AethAdamwState;
+int aeth_adamw_step(void* const* p, const void* const* g, const int64_t* n, const uint8_t* p_dtype, const uint8_t* g_dtype,
+                    const uint8_t* decay, int count, const AethAdamwState* state, double beta1, double beta2, float eps,
+                    float lr, const float* lr_dev /* or NULL: lr */, float weight_decay, const float* clip_dev /* or NULL: 1 */,
+                    aeth_stream_t stream);
+/* 8-bit moments as the values that they stand for: blocks x 2048 floats each. */
+int aeth_adamw_moments(const AethAdamwState* state, float* m_out, float* v_out, aeth_stream_t stream);
+
+/* ======================================================================
  * 4. Errors and build information.
  * ====================================================================== */
 const char* aeth_status_string(int status);
