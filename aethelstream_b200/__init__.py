@@ -40,12 +40,15 @@ from .qk import RotaryPlan, qk_norm_rotary, qk_norm_rotary_backward, rotary, rot
 from .training import (  # noqa: E402
     ActivationCheckpoint,
     CutCrossEntropy,
+    TokenLogProbs,
     checkpoint_decode,
     checkpoint_weight_grad,
     cut_cross_entropy,
     cut_cross_entropy_backward,
     rms_norm_checkpoint,
     rms_norm_checkpoint_backward,
+    token_log_probs,
+    token_log_probs_backward,
 )
 
 __all__ = [
@@ -54,5 +57,5 @@ __all__ = [
     "ActivationCheckpoint", "CutCrossEntropy", "checkpoint_decode", "checkpoint_weight_grad", "cut_cross_entropy",
     "cut_cross_entropy_backward", "rms_norm_checkpoint", "rms_norm_checkpoint_backward",
     "AdamWState", "adamw_moments", "adamw_step", "RotaryPlan", "qk_norm_rotary", "qk_norm_rotary_backward", "rotary",
-    "rotary_backward", "_lib",
+    "rotary_backward", "TokenLogProbs", "token_log_probs", "token_log_probs_backward", "_lib",
 ]

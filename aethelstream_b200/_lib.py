@@ -142,6 +142,11 @@ SIGNATURES = {
     "aeth_cut_ce_forward": (_i, [_vp, _i64, _vp, _i64, _i, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _sz, _vp]),
     "aeth_cut_ce_backward": (_i, [_vp, _i64, _vp, _i64, _i, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _f, _vp, _i64, _vp,
                                   _i64, _vp, _sz, _vp]),
+    "aeth_token_log_probs_workspace": (_i, [_i64, _i64, _i64, _i, _i, C.POINTER(C.c_size_t)]),
+    "aeth_token_log_probs": (_i, [_vp, _i64, _vp, _i64, _i, _vp, _i64, _i64, _i64, _i64, _i, _vp, _vp, _vp, _vp, _vp, _vp,
+                                  _sz, _vp]),
+    "aeth_token_log_probs_backward": (_i, [_vp, _i64, _vp, _i64, _i, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp,
+                                           _i64, _vp, _i64, _vp, _sz, _vp]),
     "aeth_rms_norm_checkpoint": (_i, [_vp, _i64, _vp, _i64, _vp, _i, _i, _i64, _i64, _f, _vp, _vp, _vp, _vp, _vp]),
     "aeth_checkpoint_decode": (_i, [_vp, _vp, _i64, _i64, _vp, _i, _f, _vp, _i64, _i, _vp]),
     "aeth_rms_norm_checkpoint_backward_workspace": (_i, [_i64, _i64, C.POINTER(C.c_size_t)]),

@@ -2,12 +2,15 @@
 // step (section 3b of include/aeth_galore.h): the head's loss and gradient, the
 // RMS norm whose input is kept in 8 bits, and the weight gradient taken from
 // that checkpoint.
+#include <math.h>
+
 #include <algorithm>
 #include <type_traits>
 
 #include "checkpoint.cuh"
 #include "common.cuh"
 #include "head_loss.cuh"
+#include "head_probs.cuh"
 #include "pair_gemm.cuh"
 
 using namespace aeth;
@@ -211,10 +214,12 @@ int head_vec(const HeadVec& a, int64_t n, int ctas, float* losses, float* lse, f
     return AETH_OK;
 }
 
-// UNIT: d_hidden comes from a G without the token weights
-template <bool BF16, bool UNIT>
+// UNIT: d_hidden comes from a G without the token weights.  PROBS: the gradient of
+// log probabilities and entropies, its rows' coefficients in `row`
+template <bool BF16, bool UNIT, bool PROBS = false>
 int head_backward(const HeadPlan& p, const HeadWork& w, const void* weight, int64_t ld_weight, int64_t n, int64_t d,
-                  int64_t vocab, void* d_hidden, int64_t ld_dh, void* d_weight, int64_t ld_dw, cudaStream_t st) {
+                  int64_t vocab, const float4* row, void* d_hidden, int64_t ld_dh, void* d_weight, int64_t ld_dw,
+                  cudaStream_t st) {
     const uint16_t* W = static_cast<const uint16_t*>(weight);
     uint16_t *g = UNIT && !d_weight ? nullptr : w.g, *g_unit = UNIT ? w.g_unit : nullptr;
     for (int64_t v0 = 0; v0 < vocab; v0 += p.piece) {
@@ -222,13 +227,15 @@ int head_backward(const HeadPlan& p, const HeadWork& w, const void* weight, int6
         const PairOperand H{w.h, p.dp, n, d}, Wp{W + v0 * ld_weight, ld_weight, vp, d};
         const PairOperand G{w.g, p.ldg, n, vp}, Gh{UNIT ? w.g_unit : w.g, p.ldg, n, vp};
         if (p.live_n) {
-            HeadGradT<BF16, UNIT> eg{w.lab, w.coef, w.lse2, g, g_unit, p.ldg, (int)n, (int)v0};
-            AETH_TRY((pair_gemm_launch<HeadGradT<BF16, UNIT>, false, false>(Wp, H, (int)vp, (int)n, (int)d, w.count,
-                                                                            PAIR_LIVE_N, 256, 0, BF16, eg, st)));
+            using Epi = HeadGradT<BF16, UNIT, PROBS>;
+            const Epi eg{w.lab, w.coef, w.lse2, g, g_unit, p.ldg, (int)n, (int)v0, row};
+            AETH_TRY((pair_gemm_launch<Epi, false, false>(Wp, H, (int)vp, (int)n, (int)d, w.count, PAIR_LIVE_N, 256, 0, BF16,
+                                                          eg, st)));
         } else {
-            HeadGrad<BF16, UNIT> eg{w.lab, w.coef, w.lse2, g, g_unit, p.ldg, (int)n, (int)v0};
-            AETH_TRY((pair_gemm_launch<HeadGrad<BF16, UNIT>, false, false>(H, Wp, (int)n, (int)vp, (int)d, w.count, PAIR_LIVE_M,
-                                                                           head_bn(p.n_pad / 256, vp), 0, BF16, eg, st)));
+            using Epi = HeadGrad<BF16, UNIT, PROBS>;
+            const Epi eg{w.lab, w.coef, w.lse2, g, g_unit, p.ldg, (int)n, (int)v0, row};
+            AETH_TRY((pair_gemm_launch<Epi, false, false>(H, Wp, (int)n, (int)vp, (int)d, w.count, PAIR_LIVE_M,
+                                                          head_bn(p.n_pad / 256, vp), 0, BF16, eg, st)));
         }
         if (d_weight) {
             PairOut16<BF16> ew{static_cast<uint16_t*>(d_weight) + v0 * ld_dw, ld_dw, w.out_scale};
@@ -256,6 +263,110 @@ int head_backward(const HeadPlan& p, const HeadWork& w, const void* weight, int6
         if (n <= rows) AETH_CUDA(launch_after(head_dh_kernel<BF16, 1>, dim3((unsigned)n, cols), dim3(128), 0, st, 1, a));
         else AETH_CUDA(launch_after(head_dh_kernel<BF16, 4>, dim3((unsigned)std::min((n + 3) / 4, rows), cols), dim3(128), 0,
                                     st, 1, a));
+    }
+    return AETH_OK;
+}
+
+// ---------------------------------------------------------------------------
+// Log probabilities at the head
+// ---------------------------------------------------------------------------
+// Where alternatives are wanted, a piece of the vocabulary whose logits (fp32)
+// fit beside one another: as many equal pieces as it takes.
+struct ProbsPlan {
+    HeadPlan head;
+    int top, ranges;  // ranges: of the whole vocabulary
+    int64_t piece, ld;
+
+    ProbsPlan(int64_t n, int64_t d, int64_t vocab, int top_) : head(n, d, vocab), top(top_) {
+        if (top == 0) {
+            ranges = head.np;
+            piece = vocab;
+            ld = 0;
+            return;
+        }
+        const int64_t tiles = (vocab + 255) / 256, fit = std::max<int64_t>(kHeadPieceBytes / (1024 * head.n_pad), 1);
+        const int64_t pieces = (tiles + fit - 1) / fit;
+        piece = std::min(256 * ((tiles + pieces - 1) / pieces), vocab);
+        ld = up(piece, 4);
+        ranges = 2 * (int)tiles;
+    }
+};
+
+// A CTA's logits beside the hidden states in shared memory.
+constexpr int kVecLogitShared = 96 * 1024;
+int vec_slots(int64_t vocab) {
+    const int each = 2 * kHeadVecThreads / 32;
+    return (int)((vocab + each * num_sms() - 1) / (each * num_sms())) * each;
+}
+bool vec_probs_fits(int64_t n, int64_t d, int64_t vocab) {
+    return head_vec_fits(n, d) && vocab <= (int64_t)num_sms() * (kVecLogitShared / (4 * kHeadVecTokens)) &&
+           n * vec_slots(vocab) * 4 <= kVecLogitShared;
+}
+
+struct ProbsWork {
+    HeadWork head;
+    HeadSums* part;
+    float *label_logit, *logits;
+    float2 *best, *cand;
+    size_t bytes;
+
+    // of the head's workspace only what every call needs: rows, positions, labels, the gathered states
+    ProbsWork(const ProbsPlan& p, int64_t n, int64_t d, int64_t vocab, void* ws) : head(p.head, n, false, ws) {
+        Carver c(ws);
+        c.used = (size_t)(reinterpret_cast<uint8_t*>(head.label_logit) - static_cast<uint8_t*>(ws));
+        const bool vec = vec_probs_fits(n, d, vocab);
+        label_logit = c.take<float>(p.head.n_pad);
+        part = c.take<HeadSums>(vec ? (int64_t)num_sms() * n : p.head.n_pad * p.ranges);
+        cand = c.take<float2>(vec ? (int64_t)num_sms() * n * p.top : 0);
+        best = c.take<float2>(p.top > 0 ? p.head.n_pad * 32 : 0);
+        logits = c.take<float>(p.top > 0 ? p.head.n_pad * p.ld : 0);
+        bytes = c.used;
+    }
+};
+
+template <bool BF16>
+int vec_probs(const HeadVecProbs& a, int64_t n, int ctas, const HeadProbsOut& out, cudaStream_t st) {
+    DeviceRuntime* rt = nullptr;
+    AETH_TRY(runtime_for_current(&rt));
+    auto kern = n == 1 ? head_vec_probs_kernel<BF16, 1> : n == 2 ? head_vec_probs_kernel<BF16, 2>
+              : n == 3 ? head_vec_probs_kernel<BF16, 3> : head_vec_probs_kernel<BF16, 4>;
+    const int smem = (int)(n * (up(a.v.d, 8) * 2 + a.slots * 4));
+    static std::atomic<bool> allowed[kHeadVecTokens][kMaxDevices] = {};
+    AETH_TRY(allow_shared(kern, kHeadVecShared + kVecLogitShared, allowed[n - 1]));
+    kern<<<ctas, kHeadVecThreads, smem, st>>>(a);
+    AETH_LAUNCH_CHECK();
+    AETH_CUDA(launch_after(head_vec_probs_join_kernel, dim3((unsigned)n), dim3(32), 0, st, 1, a, ctas, out, rt->err_word));
+    return AETH_OK;
+}
+
+template <bool TOP>
+int probs_tiles(const ProbsPlan& p, const ProbsWork& w, HeadProbsOut out, const void* weight, int64_t ld_weight, int64_t n,
+                int64_t d, int64_t vocab, bool bf16, cudaStream_t st) {
+    const PairOperand H{w.head.h, p.head.dp, n, d};
+    const unsigned ctas = (unsigned)std::min<int64_t>((n + 7) / 8, 8 * num_sms());
+    for (int64_t v0 = 0; v0 < vocab; v0 += p.piece) {
+        const int64_t vp = std::min(p.piece, vocab - v0);
+        const PairOperand W{static_cast<const uint16_t*>(weight) + v0 * ld_weight, ld_weight, vp, d};
+        const int first = (int)(v0 / kHeadRange);
+        const HeadProbsSums<TOP> sums{w.part, p.ranges, first, w.logits, p.ld};
+        if (p.head.live_n) {
+            using Epi = HeadStatsT<HeadProbsSums<TOP>>;
+            const Epi e{w.head.lab, w.label_logit, (int)v0, sums};
+            AETH_TRY((pair_gemm_launch<Epi, false, false>(W, H, (int)vp, (int)n, (int)d, w.head.count, PAIR_LIVE_N, 256, 0, bf16,
+                                                          e, st)));
+        } else {
+            using Epi = HeadStats<HeadProbsSums<TOP>>;
+            const Epi e{w.head.lab, w.label_logit, (int)v0, sums};
+            AETH_TRY((pair_gemm_launch<Epi, false, false>(H, W, (int)n, (int)vp, (int)d, w.head.count, PAIR_LIVE_M,
+                                                          TOP ? 256 : p.head.bn, 0, bf16, e, st)));
+        }
+        out.first = first;
+        out.count = (int)((vp + kHeadRange - 1) / kHeadRange);
+        out.v0 = (int)v0;
+        out.vp = (int)vp;
+        out.is_first = v0 == 0;
+        out.is_last = v0 + vp == vocab;
+        AETH_CUDA(launch_after(head_probs_kernel<TOP>, dim3(ctas), dim3(256), 0, st, 1, out));
     }
     return AETH_OK;
 }
@@ -447,13 +558,13 @@ int aeth_cut_ce_forward(const void* hidden, int64_t ld_hidden, const void* weigh
     AETH_TRY(head_rows({}, labels, n, d, vocab, ignore_index, hidden, ld_hidden, p, w, st));
     const PairOperand H{w.h, p.dp, n, d}, W{weight, ld_weight, vocab, d};
     if (p.live_n) {
-        HeadStatsT es{w.lab, w.label_logit, w.part, p.n_pad};
-        AETH_TRY((pair_gemm_launch<HeadStatsT, false, false>(W, H, (int)vocab, (int)n, (int)d, w.count, PAIR_LIVE_N, 256, 0,
-                                                             bf16, es, st)));
+        const HeadStatsT<HeadLossSums> es{w.lab, w.label_logit, 0, {w.part, p.n_pad}};
+        AETH_TRY((pair_gemm_launch<HeadStatsT<HeadLossSums>, false, false>(W, H, (int)vocab, (int)n, (int)d, w.count,
+                                                                           PAIR_LIVE_N, 256, 0, bf16, es, st)));
     } else {
-        HeadStats es{w.lab, w.label_logit, w.part, p.n_pad};
-        AETH_TRY((pair_gemm_launch<HeadStats, false, false>(H, W, (int)n, (int)vocab, (int)d, w.count, PAIR_LIVE_M, p.bn, 0,
-                                                            bf16, es, st)));
+        const HeadStats<HeadLossSums> es{w.lab, w.label_logit, 0, {w.part, p.n_pad}};
+        AETH_TRY((pair_gemm_launch<HeadStats<HeadLossSums>, false, false>(H, W, (int)n, (int)vocab, (int)d, w.count,
+                                                                          PAIR_LIVE_M, p.bn, 0, bf16, es, st)));
     }
     const HeadLoss l{w.part, p.n_pad, p.np, w.label_logit, w.rows, w.pos, w.count, w.done, n, losses, lse, loss};
     AETH_CUDA(launch_after(head_loss_kernel, dim3((unsigned)std::min<int64_t>((n + 7) / 8, 4 * num_sms())), dim3(512), 0, st,
@@ -493,7 +604,88 @@ int aeth_cut_ce_backward(const void* hidden, int64_t ld_hidden, const void* weig
     a.row_scale = w.row_scale;
     AETH_TRY(head_rows(a, labels, n, d, vocab, ignore_index, hidden, ld_hidden, p, w, st));
     auto run = bf16 ? head_backward<true, false> : unit ? head_backward<false, true> : head_backward<false, false>;
-    return run(p, w, weight, ld_weight, n, d, vocab, d_hidden, ld_dh, d_weight, ld_dw, st);
+    return run(p, w, weight, ld_weight, n, d, vocab, nullptr, d_hidden, ld_dh, d_weight, ld_dw, st);
+}
+
+int aeth_token_log_probs_workspace(int64_t n, int64_t d, int64_t vocab, int top, int backward, size_t* bytes) {
+    if (n < 0 || d <= 0 || vocab <= 0 || top < 0 || !bytes) return set_err(AETH_ERR_ARG);
+    if (n > kHeadMaxDim || d > kHeadMaxDim || vocab > kHeadMaxDim || top > kHeadTop) return set_err(AETH_ERR_UNSUPPORTED);
+    if (backward) {
+        AETH_TRY(aeth_cut_ce_workspace(n, d, vocab, 1, bytes));
+        *bytes += (size_t)up(HeadPlan(n, d, vocab).n_pad * (int64_t)sizeof(float4), 256);
+    } else {
+        *bytes = ProbsWork(ProbsPlan(n, d, vocab, top), n, d, vocab, nullptr).bytes;
+    }
+    return AETH_OK;
+}
+
+int aeth_token_log_probs(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, int dtype,
+                         const int64_t* labels, int64_t n, int64_t d, int64_t vocab, int64_t ignore_index, int top,
+                         float* log_probs, float* entropy, float* lse, float* top_log_probs, int64_t* top_ids, void* workspace,
+                         size_t workspace_bytes, aeth_stream_t stream) {
+    AETH_TRY(head_check(hidden, ld_hidden, weight, ld_weight, dtype, labels, n, d, vocab));
+    if (top < 0 || top > vocab || (n > 0 && (!log_probs || !entropy || !lse || !workspace))) return set_err(AETH_ERR_ARG);
+    if (top > kHeadTop) return set_err(AETH_ERR_UNSUPPORTED);
+    if (top > 0 && n > 0 && (!top_log_probs || !top_ids)) return set_err(AETH_ERR_ARG);
+    if (n == 0) return AETH_OK;
+    cudaStream_t st = to_stream(stream);
+    const bool bf16 = dtype == AETH_DTYPE_BF16;
+    const ProbsPlan p(n, d, vocab, top);
+    const ProbsWork w(p, n, d, vocab, workspace);
+    if (workspace_bytes < w.bytes || !aligned16(workspace)) return set_err(AETH_ERR_ARG);
+    HeadProbsOut out = {};
+    out.part = w.part;
+    out.ranges = p.ranges;
+    out.label_logit = w.label_logit;
+    out.pos = w.head.pos;
+    out.n = n;
+    out.log_probs = log_probs;
+    out.entropy = entropy;
+    out.lse = lse;
+    out.top = top;
+    out.logits = w.logits;
+    out.ld = p.ld;
+    out.best = w.best;
+    out.top_log_probs = top_log_probs;
+    out.top_ids = top_ids;
+    if (vec_probs_fits(n, d, vocab)) {
+        const HeadVec v{static_cast<const uint16_t*>(hidden), ld_hidden, static_cast<const uint16_t*>(weight), ld_weight, labels,
+                        (int)d, (int)vocab, ignore_index, w.label_logit, nullptr};
+        const HeadVecProbs a{v, w.part, w.cand, top, vec_slots(vocab)};
+        return bf16 ? vec_probs<true>(a, n, num_sms(), out, st) : vec_probs<false>(a, n, num_sms(), out, st);
+    }
+    AETH_TRY(head_rows({}, labels, n, d, vocab, ignore_index, hidden, ld_hidden, p.head, w.head, st));
+    return top > 0 ? probs_tiles<true>(p, w, out, weight, ld_weight, n, d, vocab, bf16, st)
+                   : probs_tiles<false>(p, w, out, weight, ld_weight, n, d, vocab, bf16, st);
+}
+
+int aeth_token_log_probs_backward(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, int dtype,
+                                  const int64_t* labels, int64_t n, int64_t d, int64_t vocab, int64_t ignore_index,
+                                  const float* lse, const float* entropy, const float* grad_log_probs,
+                                  const float* grad_entropy, void* d_hidden, int64_t ld_dh, void* d_weight, int64_t ld_dw,
+                                  void* workspace, size_t workspace_bytes, aeth_stream_t stream) {
+    AETH_TRY(head_check(hidden, ld_hidden, weight, ld_weight, dtype, labels, n, d, vocab));
+    if (!d_hidden && !d_weight) return set_err(AETH_ERR_ARG);
+    if ((d_hidden && ld_dh < d) || (d_weight && ld_dw < d)) return set_err(AETH_ERR_ARG);
+    if (n > 0 && (!lse || !entropy || !workspace)) return set_err(AETH_ERR_ARG);
+    cudaStream_t st = to_stream(stream);
+    if (n == 0) {
+        if (d_weight) AETH_CUDA(cudaMemset2DAsync(d_weight, (size_t)ld_dw * 2, 0, (size_t)d * 2, (size_t)vocab, st));
+        return AETH_OK;
+    }
+    const bool bf16 = dtype == AETH_DTYPE_BF16, unit = !bf16 && d_hidden;
+    const HeadPlan p(n, d, vocab, unit ? 2 : 1);
+    const HeadWork w(p, n, true, workspace);
+    Carver c(workspace);
+    c.used = w.bytes;
+    float4* row = c.take<float4>(p.n_pad);
+    if (workspace_bytes < c.used || !aligned16(workspace)) return set_err(AETH_ERR_ARG);
+    AETH_TRY(head_rows({}, labels, n, d, vocab, ignore_index, hidden, ld_hidden, p, w, st));
+    const HeadProbsRows a{w.rows, w.count, lse, entropy, grad_log_probs, grad_entropy, 0.25f * logf((float)vocab) + 0.5f,
+                          head_g_bits(bf16), head_g_scale(bf16), w.lse2, w.out_scale, w.row_scale, row};
+    AETH_CUDA(launch_after(head_probs_rows_kernel, dim3(1), dim3(1024), 0, st, 1, a));
+    auto run = bf16 ? head_backward<true, false, true> : unit ? head_backward<false, true, true> : head_backward<false, false, true>;
+    return run(p, w, weight, ld_weight, n, d, vocab, row, d_hidden, ld_dh, d_weight, ld_dw, st);
 }
 
 int aeth_rms_norm_checkpoint(const void* x, int64_t ld_x, const void* residual, int64_t ld_residual, const void* gain,

@@ -292,45 +292,63 @@ __device__ __forceinline__ void head_slice(const float (&acc)[128], int c, float
     for (int i = 0; i < 32; ++i) v[i] = acc[32 * c + i];
 }
 
+// What the forward's epilogues keep of a row and range: the loss's maximum and sum
+// of exponentials.  `Sums` of the epilogues; head_probs.cuh has another.
+struct HeadLossSums {
+    using Sum = float2;
+    float2* part;  // [range][row]
+    int64_t ld_part;
+    __device__ static Sum none() { return make_float2(-INFINITY, 0.0f); }
+    __device__ static Sum join(Sum a, Sum b) { return head_join(a, b); }
+    __device__ __forceinline__ static void add32(const float (&v)[32], int left, Sum& st) { head_stats32(v, left, st); }
+    __device__ __forceinline__ void put(int range, int row, Sum x) const { part[(int64_t)range * ld_part + row] = x; }
+    // 32 columns of the warp's rows, and 32 entries of a token (none of them kept)
+    __device__ __forceinline__ void rows(const PairTile&, const float (&)[32], int) const {}
+    __device__ __forceinline__ void token(int, int, int, const float (&)[32]) const {}
+};
+
 // Epilogue of the forward product: per row, over this warp's columns, the
 // maximum and sum, and the label's logit where it lies here.
+template <class Sums>
 struct HeadStats {
     static constexpr int kChunk = 8;  // the loss is an fp32 result: see pair_gemm.cuh
     static constexpr bool kLiveN = false;
     const int* lab;
     float* label_logit;
-    float2* part;  // [2 * n_tile + half][row]
-    int64_t ld_part;
+    int v0;  // first entry of the product's columns
+    Sums sums;  // range: 2 * n_tile + half
     __device__ static void give_up(const PairTile&) {}
     __device__ __forceinline__ void finish(const PairTile& t, const float (&acc)[128]) const {
         const int row = t.row0 + t.lane;
         const bool in = row < t.M;
-        const int at = in ? lab[row] - t.col0 - t.c_begin : -1;
-        float2 st = make_float2(-INFINITY, 0.0f);
+        const int at = in ? lab[row] - v0 - t.col0 - t.c_begin : -1;
+        typename Sums::Sum st = Sums::none();
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             const int left = min(t.c_end, t.N - t.col0) - t.c_begin - 32 * c;  // columns of this chunk that exist
             if (left > 0) {
                 float v[32];
                 head_slice(acc, c, v);
-                head_stats32(v, left, st);
+                Sums::add32(v, left, st);
                 head_label32(v, at - 32 * c, label_logit + row);
+                sums.rows(t, v, t.c_begin + 32 * c);
             }
         }
-        if (in) part[(int64_t)(2 * t.n_tile + t.half) * ld_part + row] = st;
+        if (in) sums.put(2 * t.n_tile + t.half, row, st);
     }
 };
 
 // The same with tokens as the tile's columns (few live rows) and vocabulary
 // entries as its rows: a warp has 32 entries; the four warps of a column half
 // join theirs through shared memory.
+template <class Sums>
 struct HeadStatsT {
     static constexpr int kChunk = 8;
     static constexpr bool kLiveN = true;
     const int* lab;
     float* label_logit;
-    float2* part;  // [2 * m_tile + CTA of the pair][row]
-    int64_t ld_part;
+    int v0;
+    Sums sums;  // range: 2 * m_tile + CTA of the pair
     // The two barriers of finish(), each with an id of its own: a barrier counts
     // arrivals, so two at one id could both fall into its first wait.  A warp that
     // leaves waits for nobody, since the others may never come to its next tile's.
@@ -339,34 +357,35 @@ struct HeadStatsT {
         named_bar_arrive(3 + t.half, 128);
     }
     __device__ __forceinline__ void finish(const PairTile& t, const float (&acc)[128]) const {
+        using Sum = typename Sums::Sum;
         const int left = t.M - t.row0;  // entries of this warp that exist
-        float2 st[4];
+        Sum st[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            st[c] = make_float2(-INFINITY, 0.0f);
+            st[c] = Sums::none();
             const int token = t.col0 + t.c_begin + 32 * c + t.lane;
             if (t.c_begin + 32 * c < t.c_end && left > 0) {
                 float v[32];
                 head_slice(acc, c, v);
                 pair_transpose(t, v);
-                head_stats32(v, left, st[c]);
-                const int k = token < t.N ? lab[token] - t.row0 : -1;
+                Sums::add32(v, left, st[c]);
+                const int k = token < t.N ? lab[token] - v0 - t.row0 : -1;
                 head_label32(v, k < left ? k : -1, label_logit + token);
+                if (token < t.N) sums.token(token, t.row0, left, v);
             }
         }
-        float2* mine = reinterpret_cast<float2*>(t.staging);
+        Sum* mine = reinterpret_cast<Sum*>(t.staging);
 #pragma unroll
         for (int c = 0; c < 4; ++c) mine[32 * c + t.lane] = st[c];
         named_bar(1 + t.half, 128);
         // warp `e` of the half takes its 32 columns c = e
         const int e = t.warp & 3;
-        const float2* all = reinterpret_cast<const float2*>(t.staging - e * kPairStaging);
-        float2 x = all[32 * e + t.lane];
+        const Sum* all = reinterpret_cast<const Sum*>(t.staging - e * kPairStaging);
+        Sum x = all[32 * e + t.lane];
 #pragma unroll
-        for (int w = 1; w < 4; ++w) x = head_join(x, all[w * (kPairStaging / 8) + 32 * e + t.lane]);
+        for (int w = 1; w < 4; ++w) x = Sums::join(x, all[w * (kPairStaging / (int)sizeof(Sum)) + 32 * e + t.lane]);
         const int col = t.c_begin + 32 * e + t.lane;
-        if (col < t.c_end && t.col0 + col < t.N)
-            part[(int64_t)(2 * t.m_tile + (t.tile_row >> 7)) * ld_part + t.col0 + col] = x;
+        if (col < t.c_end && t.col0 + col < t.N) sums.put(2 * t.m_tile + (t.tile_row >> 7), t.col0 + col, x);
         named_bar(3 + t.half, 128);
     }
 };
@@ -488,11 +507,12 @@ __device__ __forceinline__ float2 head_pair(uint32_t w) {
     return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
-template <bool BF16, int NT>
-__global__ void __launch_bounds__(kHeadVecThreads, 1) head_vec_kernel(const HeadVec a) {
+// Stages the hidden states ([token][eight of features]), calls begin() behind a
+// barrier and then logit(token, entry, its logit) with all lanes of a warp, for
+// the entries that are the warp's: two in turn, from 2 (CTA's warps + warp) on.
+template <bool BF16, int NT, typename Begin, typename Logit>
+__device__ __forceinline__ void head_vec_walk(const HeadVec& a, uint4* head_sh, Begin begin, Logit logit) {
     constexpr int R = 2, U = 8;  // entries a warp, loads in flight an entry
-    extern __shared__ uint4 head_sh[];  // [token][eight of features]
-    __shared__ float2 red[kHeadVecThreads / 32][NT];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, eights = (a.d + 7) / 8;
     const int64_t first = (int64_t)R * (blockIdx.x * (kHeadVecThreads / 32) + warp);
     // the warp's first entries are on their way to L2 while the hidden states are staged
@@ -504,16 +524,8 @@ __global__ void __launch_bounds__(kHeadVecThreads, 1) head_vec_kernel(const Head
         const int t = i / (eights * 8), c = i - t * eights * 8;
         sh16[i] = c < a.d ? a.hidden[t * a.ld_h + c] : (uint16_t)0;
     }
-    int lab[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int64_t l = a.labels[t];
-        lab[t] = l != a.ignore_index && l >= 0 && l < a.vocab ? (int)l : -1;
-    }
+    begin();
     __syncthreads();
-    float2 st[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) st[t] = make_float2(-INFINITY, 0.0f);
     pdl_trigger();
     const int warps = gridDim.x * (kHeadVecThreads / 32);
     for (int64_t v0 = first; v0 < a.vocab; v0 += (int64_t)R * warps) {
@@ -566,12 +578,36 @@ __global__ void __launch_bounds__(kHeadVecThreads, 1) head_vec_kernel(const Head
                 float x = acc[r][t].x + acc[r][t].y;
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-                if (v0 + r < a.vocab) {
-                    st[t] = head_join(st[t], make_float2(x * kLog2e, 1.0f));
-                    if (lab[t] == v0 + r && lane == 0) a.label_logit[t] = x;
-                }
+                if (v0 + r < a.vocab) logit(t, (int)(v0 + r), x);
             }
     }
+}
+// The label of token t where it takes part, else -1.
+__device__ __forceinline__ int head_vec_label(const HeadVec& a, int t) {
+    const int64_t l = a.labels[t];
+    return l != a.ignore_index && l >= 0 && l < a.vocab ? (int)l : -1;
+}
+
+template <bool BF16, int NT>
+__global__ void __launch_bounds__(kHeadVecThreads, 1) head_vec_kernel(const HeadVec a) {
+    extern __shared__ uint4 head_sh[];
+    __shared__ float2 red[kHeadVecThreads / 32][NT];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int lab[NT];
+    float2 st[NT];
+    head_vec_walk<BF16, NT>(
+        a, head_sh,
+        [&] {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                lab[t] = head_vec_label(a, t);
+                st[t] = make_float2(-INFINITY, 0.0f);
+            }
+        },
+        [&](int t, int entry, float x) {
+            st[t] = head_join(st[t], make_float2(x * kLog2e, 1.0f));
+            if (lab[t] == entry && lane == 0) a.label_logit[t] = x;
+        });
 #pragma unroll
     for (int t = 0; t < NT; ++t)
         if (lane == 0) red[warp][t] = st[t];
@@ -582,6 +618,7 @@ __global__ void __launch_bounds__(kHeadVecThreads, 1) head_vec_kernel(const Head
         a.part[(int64_t)blockIdx.x * NT + threadIdx.x] = x;
     }
 }
+
 
 // One warp a token joins the CTAs' pairs; then losses and mean.
 __global__ void __launch_bounds__(32 * kHeadVecTokens)
@@ -625,6 +662,46 @@ __global__ void __launch_bounds__(32 * kHeadVecTokens)
 // A token weight's part in the G without weights: its sign (NaN and 0 stay).
 __device__ __forceinline__ float head_unit(float f) { return f > 0.0f ? 1.0f : f < 0.0f ? -1.0f : f; }
 
+// A row of G before the token's weight, from 32 logits of it: 2^k (p - 1[label]),
+// or with PROBS 2^k (alpha 1[label] - p (beta + gamma x)), x = log2 p.
+template <bool BF16, bool PROBS>
+struct HeadRowGrad {
+    // the token's weight, that of the G without weights, and the log-sum-exp: in units of log2 and - k, PROBS as it is
+    float f, u, l2;
+    float alpha, beta, gamma;
+    __device__ __forceinline__ HeadRowGrad(bool in, int r, const float* coef, const float* lse2, const float4* row) {
+        l2 = in ? lse2[r] : 0.0f;
+        if (PROBS) {
+            const float4 x = in ? row[r] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            f = x.w;
+            u = 1.0f;
+            alpha = x.x;
+            beta = x.y;
+            gamma = x.z;
+        } else {
+            f = in ? coef[r] : 0.0f;
+            u = head_unit(f);
+        }
+    }
+    // k: the label's place among the 32
+    __device__ __forceinline__ void values(float (&v)[32], int k) const {
+        constexpr float kBits = head_g_bits(BF16);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            if (PROBS) {
+                const float x = fmax3_nan(fmaf(v[i] - l2, kLog2e, kBits), -300.0f, -300.0f);  // finite where p is 0
+                v[i] = -(ex2(x) * fmaf(gamma, x, beta));
+            } else {
+                v[i] = ex2(fmaf(v[i], kLog2e, -l2));
+            }
+        }
+        if (__any_sync(0xffffffffu, k >= 0 && k < 32)) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = k == i ? v[i] + (PROBS ? alpha : -head_g_scale(BF16)) : v[i];
+        }
+    }
+};
+
 // Epilogue of the backward's product: G of the piece in 16 bits, as the tensor
 // cores take it for dW and dH.  G is rounded once, from fp32, which a sum over many
 // tokens or entries evens out (against 64 bits 1.9e-3 in bf16, 1.7e-3 of it the
@@ -637,7 +714,9 @@ __device__ __forceinline__ float head_unit(float f) { return f > 0.0f ? 1.0f : f
 // x 32000: 2.13 -> 2.19) and 6 to 13 us of one of 130 to 311 tokens (160 to 260 us).
 // UNIT (f16): the G without token weights, beside the other where that is wanted
 // (3584 x 4096 x 32000 with weights: 2.26 -> 2.42 ms, 64 tokens 178 -> 183 us).
-template <bool BF16, bool UNIT>
+// PROBS: the gradient of log probability and entropy (head_probs.cuh), whose rows
+// have coefficients of their own in `row`.
+template <bool BF16, bool UNIT, bool PROBS>
 struct HeadGrad {
     static constexpr int kChunk = 8;
     static constexpr bool kLiveN = false;
@@ -649,12 +728,13 @@ struct HeadGrad {
     int64_t ldg;
     int n;   // rows of g: the tokens
     int v0;  // first vocabulary entry of the piece
+    const float4* row;  // with PROBS
     __device__ static void give_up(const PairTile&) {}
     __device__ __forceinline__ void finish(const PairTile& t, const float (&acc)[128]) const {
-        const int row = t.row0 + t.lane;
-        const bool in = row < t.M;
-        const float f = in ? coef[row] : 0.0f, u = head_unit(f), l2 = in ? lse2[row] : 0.0f;
-        const int lab_c = in ? lab[row] - v0 - t.col0 - t.c_begin : -1;
+        const int r = t.row0 + t.lane;
+        const bool in = r < t.M;
+        const HeadRowGrad<BF16, PROBS> a(in, r, coef, lse2, row);
+        const int lab_c = in ? lab[r] - v0 - t.col0 - t.c_begin : -1;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const int c = t.c_begin + 64 * b;
@@ -664,17 +744,11 @@ struct HeadGrad {
                 for (int h = 0; h < 2; ++h) {
                     float v[32];
                     head_slice(acc, 2 * b + h, v);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = ex2(fmaf(v[i], kLog2e, -l2));
-                    const int k = lab_c - 64 * b - 32 * h;
-                    if (__any_sync(0xffffffffu, k >= 0 && k < 32)) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = k == i ? v[i] - head_g_scale(BF16) : v[i];
-                    }
+                    a.values(v, lab_c - 64 * b - 32 * h);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        w[16 * h + i] = pack16<BF16>(v[2 * i] * f, v[2 * i + 1] * f);
-                        if (UNIT) w1[16 * h + i] = pack16<BF16>(v[2 * i] * u, v[2 * i + 1] * u);
+                        w[16 * h + i] = pack16<BF16>(v[2 * i] * a.f, v[2 * i + 1] * a.f);
+                        if (UNIT) w1[16 * h + i] = pack16<BF16>(v[2 * i] * a.u, v[2 * i + 1] * a.u);
                     }
                 }
                 const int cols = min(t.N, t.col0 + t.c_end);
@@ -687,7 +761,7 @@ struct HeadGrad {
 
 // The same with tokens as the tile's columns: each 32 x 32 block is turned over,
 // so that a thread has a token and 32 entries.
-template <bool BF16, bool UNIT>
+template <bool BF16, bool UNIT, bool PROBS>
 struct HeadGradT {
     static constexpr int kChunk = 8;
     static constexpr bool kLiveN = true;
@@ -699,6 +773,7 @@ struct HeadGradT {
     int64_t ldg;
     int n;
     int v0;
+    const float4* row;
     __device__ static void give_up(const PairTile&) {}
     __device__ __forceinline__ void finish(const PairTile& t, const float (&acc)[128]) const {
 #pragma unroll
@@ -710,19 +785,13 @@ struct HeadGradT {
             pair_transpose(t, v);
             const int token = t.col0 + c + t.lane;
             const bool in = token < t.N;
-            const float f = in ? coef[token] : 0.0f, u = head_unit(f), l2 = in ? lse2[token] : 0.0f;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = ex2(fmaf(v[i], kLog2e, -l2));
-            const int k = in ? lab[token] - v0 - t.row0 : -1;
-            if (__any_sync(0xffffffffu, k >= 0 && k < 32)) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = k == i ? v[i] - head_g_scale(BF16) : v[i];
-            }
+            const HeadRowGrad<BF16, PROBS> a(in, token, coef, lse2, row);
+            a.values(v, in ? lab[token] - v0 - t.row0 : -1);
             uint32_t w[16], w1[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                w[i] = pack16<BF16>(v[2 * i] * f, v[2 * i + 1] * f);
-                if (UNIT) w1[i] = pack16<BF16>(v[2 * i] * u, v[2 * i + 1] * u);
+                w[i] = pack16<BF16>(v[2 * i] * a.f, v[2 * i + 1] * a.f);
+                if (UNIT) w1[i] = pack16<BF16>(v[2 * i] * a.u, v[2 * i + 1] * a.u);
             }
             if (!UNIT || g) store(t, w, c, g);
             if (UNIT) store(t, w1, c, g_unit);

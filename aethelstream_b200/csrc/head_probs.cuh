@@ -1,0 +1,375 @@
+// head_probs.cuh -- log probabilities of given tokens at the language model's
+// head, with the entropy of their distribution and the likeliest alternatives,
+// the logits kept for a piece of the vocabulary at most.
+//
+//   s = H W^T    lse = log sum_v exp s_v    log p_y = s_y - lse
+//   entropy = lse - sum_v p_v s_v           alternatives: the largest s_v - lse
+//
+// One pass of the head's product (head_loss.cuh: rows that take no part are left
+// out before it).  A range of the vocabulary leaves its maximum m, the sum s of
+// 2^x and u, the sum of 2^x x, of x = (logit - m) log2 e; two ranges join as sums
+// do after both are taken to the larger maximum, and
+//   lse = m + ln s     entropy = ln s - ln 2 u / s.
+//
+// Alternatives: of a row's k best entries none lies outside the k ranges (128
+// entries each) whose maxima are the best, the lower range before the other on
+// equal ones: each of these holds an entry before any of another range.  The
+// product therefore leaves its logits in fp32, a piece of the vocabulary at a time
+// (256 MiB), and a warp a row reads the maxima of a piece and then those ranges
+// alone.  It keeps the best so far in its lanes, one each, which bounds k by 32.
+// Equal logits: the lower entry first.
+//
+// Gradient of a log p_y + b entropy, with q = log p:
+//   G_v = a 1[v = y] - p_v (a + b (q_v + entropy))
+// taken as the loss's is (head_loss.cuh), whose weight is one number a token, here
+// w = |a| + c |b|: c = ln(vocab) / 4 + 1/2 bounds |p (q + entropy)|.
+#pragma once
+#include "head_loss.cuh"
+
+namespace aeth {
+
+constexpr int kHeadTop = 32;         // alternatives, at most
+constexpr int kHeadRange = 128;      // entries of a range where alternatives are wanted
+constexpr float kHeadNone = -200.0f;  // of log2: 2^-200 is 0, and finite times 0 too
+
+// (maximum, s, u) of a range
+struct alignas(16) HeadSums {
+    float m, s, u, unused;
+};
+__device__ __forceinline__ HeadSums head_no_sums() { return {-INFINITY, 0.0f, 0.0f, 0.0f}; }
+// What logits are taken against: a maximum, or 0 where there is none.  They are
+// subtracted before they are scaled, so that no finite logit overflows.
+__device__ __forceinline__ float head_base(float m) { return m == -INFINITY ? 0.0f : m; }
+__device__ __forceinline__ float head_log2(float v, float base) { return fmax3_nan((v - base) * kLog2e, kHeadNone, kHeadNone); }
+// a's sums against a larger base
+__device__ __forceinline__ void head_rebase(const HeadSums& a, float base, float& s, float& u) {
+    const float d = head_log2(a.m, base), w = ex2(d);
+    s += a.s * w;
+    u += fmaf(a.s, d, a.u) * w;
+}
+__device__ __forceinline__ HeadSums head_join3(const HeadSums& a, const HeadSums& b) {
+    HeadSums r{fmaxf(a.m, b.m), 0.0f, 0.0f, 0.0f};
+    const float base = head_base(r.m);
+    head_rebase(a, base, r.s, r.u);
+    head_rebase(b, base, r.s, r.u);
+    return r;
+}
+__device__ __forceinline__ HeadSums head_shuffle(const HeadSums& a, int o) {
+    return {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.u, o), 0.0f};
+}
+__device__ __forceinline__ float head_lse3(const HeadSums& a) { return head_base(a.m) + logf(a.s); }
+__device__ __forceinline__ float head_entropy(const HeadSums& a) { return logf(a.s) - kLn2 * (a.u / a.s); }
+
+// Joins 32 logits, the first `left` of them.
+__device__ __forceinline__ void head_sums32(const float (&v)[32], int left, HeadSums& st) {
+    float m = st.m;
+#pragma unroll
+    for (int i = 0; i < 32; i += 2)
+        m = left >= 32 ? fmax3(m, v[i], v[i + 1]) : fmaxf(i < left ? fmaxf(m, v[i]) : m, i + 1 < left ? v[i + 1] : m);
+    const float base = head_base(m);
+    float s0 = 0.0f, s1 = 0.0f, u0 = 0.0f, u1 = 0.0f;
+    head_rebase(st, base, s0, u0);
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+        const float x0 = head_log2(v[i], base), x1 = head_log2(v[i + 1], base);
+        const float e0 = left >= 32 || i < left ? ex2(x0) : 0.0f, e1 = left >= 32 || i + 1 < left ? ex2(x1) : 0.0f;
+        if (left >= 32 || i < left) {
+            s0 += e0;
+            u0 = fmaf(e0, x0, u0);
+        }
+        if (left >= 32 || i + 1 < left) {
+            s1 += e1;
+            u1 = fmaf(e1, x1, u1);
+        }
+    }
+    st = {m, s0 + s1, u0 + u1, 0.0f};
+}
+
+// What the product's epilogues (HeadStats, HeadStatsT) keep: the sums and, with
+// TOP, the logits.
+template <bool TOP>
+struct HeadProbsSums {
+    using Sum = HeadSums;
+    HeadSums* part;  // [row][range]; TOP: ranges of 128 entries, of all pieces
+    int ranges, first;
+    float* logits;  // [row][entry of the piece], a multiple of 4 of them
+    int64_t ld;
+    __device__ static Sum none() { return head_no_sums(); }
+    __device__ static Sum join(const Sum& a, const Sum& b) { return head_join3(a, b); }
+    __device__ __forceinline__ static void add32(const float (&v)[32], int left, Sum& st) { head_sums32(v, left, st); }
+    __device__ __forceinline__ void put(int range, int row, const Sum& x) const { part[(int64_t)row * ranges + first + range] = x; }
+    __device__ __forceinline__ void rows(const PairTile& t, const float (&v)[32], int c) const {
+        if (TOP && t.row0 < t.M)
+            pair_store32(t, v, c, logits + (int64_t)t.row0 * ld + t.col0, ld, t.M - t.row0, (int)min((int64_t)256, ld - t.col0), true);
+    }
+    __device__ __forceinline__ void token(int token, int entry, int left, const float (&v)[32]) const {
+        if (!TOP) return;
+        float4* o = reinterpret_cast<float4*>(logits + (int64_t)token * ld + entry);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (4 * i < left) o[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    }
+};
+
+// The best entries so far, lane i the i-th: larger logits first, the lower entry
+// first among equal ones.
+struct HeadBest {
+    float v;
+    int i;
+    __device__ static bool before(float a, int i, float b, int j) { return a > b || (a == b && i < j); }
+    // Takes (x, j) in; all lanes with the same arguments.
+    __device__ __forceinline__ void insert(float x, int j) {
+        const int lane = threadIdx.x & 31;
+        const int at = __popc(__ballot_sync(0xffffffffu, before(v, i, x, j)));
+        const float up = __shfl_up_sync(0xffffffffu, v, 1);
+        const int ui = __shfl_up_sync(0xffffffffu, i, 1);
+        if (lane > at) {
+            v = up;
+            i = ui;
+        } else if (lane == at) {
+            v = x;
+            i = j;
+        }
+    }
+    // Takes in what the lanes hold, where it comes before the k-th.
+    __device__ __forceinline__ void offer(float x, int j, int k) {
+        uint32_t left = __ballot_sync(0xffffffffu,
+                                      before(x, j, __shfl_sync(0xffffffffu, v, k - 1), __shfl_sync(0xffffffffu, i, k - 1)));
+        while (left) {
+            const int from = __ffs(left) - 1;
+            left &= left - 1;
+            const float y = __shfl_sync(0xffffffffu, x, from);
+            const int l = __shfl_sync(0xffffffffu, j, from);
+            if (before(y, l, __shfl_sync(0xffffffffu, v, k - 1), __shfl_sync(0xffffffffu, i, k - 1))) insert(y, l);
+        }
+    }
+    __device__ static HeadBest none() { return {-INFINITY, 0x7fffffff}; }
+};
+
+// What a token gets; warps of a CTA take tokens.  With alternatives one launch
+// for each piece of the vocabulary, the last of which joins the ranges.
+struct HeadProbsOut {
+    const HeadSums* part;
+    int ranges;              // of the whole vocabulary
+    const float* label_logit;
+    const int* pos;
+    int64_t n;
+    float *log_probs, *entropy, *lse;
+    // alternatives
+    int top;
+    const float* logits;
+    int64_t ld;
+    int first, count, v0, vp;  // the piece's ranges, first entry and entries
+    int is_first, is_last;
+    float2* best;              // [row][32], between pieces: (value, index's bits)
+    float* top_log_probs;      // [token][top]
+    int64_t* top_ids;
+};
+
+__device__ __forceinline__ void head_probs_write(const HeadProbsOut& a, int64_t t, int lane, bool bad, bool live, HeadSums x,
+                                                 float label_logit, const HeadBest& best) {
+    const float nan = __int_as_float(0x7fc00000);
+    // one lane's: in the others the same sums were added the other way round
+    const float lse = __shfl_sync(0xffffffffu, bad ? nan : live ? head_lse3(x) : 0.0f, 0);
+    if (lane == 0) {
+        a.lse[t] = lse;
+        a.log_probs[t] = bad ? nan : live ? label_logit - lse : 0.0f;
+        a.entropy[t] = bad ? nan : live ? head_entropy(x) : 0.0f;
+    }
+    if (lane < a.top) {
+        const bool known = live && !isnan(lse) && best.i != 0x7fffffff;
+        a.top_log_probs[t * a.top + lane] = known ? best.v - lse : bad || live ? nan : 0.0f;
+        a.top_ids[t * a.top + lane] = known ? best.i : -1;
+    }
+}
+
+template <bool TOP>
+__global__ void __launch_bounds__(256) head_probs_kernel(const HeadProbsOut a) {
+    const int lane = threadIdx.x & 31;
+    pdl_wait();
+    pdl_trigger();
+    for (int64_t t = blockIdx.x * 8ll + (threadIdx.x >> 5); t < a.n; t += gridDim.x * 8ll) {
+        const int row = a.pos[t];
+        HeadBest best = HeadBest::none();
+        if (TOP && row >= 0) {
+            if (!a.is_first) {
+                const float2 b = a.best[(int64_t)row * 32 + lane];
+                best = {b.x, __float_as_int(b.y)};
+            }
+            // the ranges whose maxima are the best, and then their entries
+            HeadBest at = HeadBest::none();
+            const HeadSums* p = a.part + (int64_t)row * a.ranges + a.first;
+            for (int r0 = 0; r0 < a.count; r0 += 32) {
+                const int r = r0 + lane;
+                const float m = r < a.count ? p[r].m : -INFINITY;
+                at.offer(m, r < a.count ? r : 0x7fffffff, a.top);
+            }
+            const float* s = a.logits + (int64_t)row * a.ld;
+            for (int k = 0; k < a.top; ++k) {
+                const float m = __shfl_sync(0xffffffffu, at.v, k);
+                const int r = __shfl_sync(0xffffffffu, at.i, k);
+                const float worst = __shfl_sync(0xffffffffu, best.v, a.top - 1);
+                const int worst_at = __shfl_sync(0xffffffffu, best.i, a.top - 1);
+                if (r == 0x7fffffff || !HeadBest::before(m, a.v0 + r * kHeadRange, worst, worst_at)) break;
+                const int e0 = r * kHeadRange + 4 * lane;
+                const float4 v = e0 < a.vp ? *reinterpret_cast<const float4*>(s + e0) : make_float4(0, 0, 0, 0);
+                const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    best.offer(e0 + i < a.vp ? x[i] : -INFINITY, e0 + i < a.vp ? a.v0 + e0 + i : 0x7fffffff, a.top);
+            }
+            if (!a.is_last) a.best[(int64_t)row * 32 + lane] = make_float2(best.v, __int_as_float(best.i));
+        }
+        if (TOP && !a.is_last) continue;
+        HeadSums x = head_no_sums();
+        if (row >= 0) {
+            const HeadSums* p = a.part + (int64_t)row * a.ranges;
+            for (int r = lane; r < a.ranges; r += 32) x = head_join3(x, p[r]);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) x = head_join3(x, head_shuffle(x, o));
+        }
+        head_probs_write(a, t, lane, row == kHeadBad, row >= 0, x, row >= 0 ? a.label_logit[row] : 0.0f, best);
+    }
+}
+
+// One to four tokens: the weight by rows, as head_vec_kernel.  A CTA keeps its
+// logits in shared memory and leaves its sums and, sorted, its best entries: an
+// entry's place is the number of those before it.
+struct HeadVecProbs {
+    HeadVec v;
+    HeadSums* part;  // [token][CTA]
+    float2* cand;  // [token][CTA][top]: (logit, entry's bits)
+    int top, slots;  // logits that a CTA has for a token, at most
+};
+template <bool BF16, int NT>
+__global__ void __launch_bounds__(kHeadVecThreads, 1) head_vec_probs_kernel(const HeadVecProbs a) {
+    extern __shared__ uint4 head_sh[];
+    __shared__ HeadSums red[kHeadVecThreads / 32][NT];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, each = 2 * kHeadVecThreads / 32;  // entries of a round
+    float* logits = reinterpret_cast<float*>(head_sh + NT * ((a.v.d + 7) / 8));  // [token][slot]
+    int lab[NT];
+    HeadSums st[NT];
+    const int round = each * gridDim.x, mine = each * blockIdx.x;  // entry = round's first + mine + place in the CTA
+    head_vec_walk<BF16, NT>(
+        a.v, head_sh,
+        [&] {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                lab[t] = head_vec_label(a.v, t);
+                st[t] = head_no_sums();
+            }
+        },
+        [&](int t, int entry, float x) {
+            st[t] = head_join3(st[t], {x, 1.0f, 0.0f, 0.0f});
+            if (lane == 0) {
+                if (lab[t] == entry) a.v.label_logit[t] = x;
+                const int n = entry / round;
+                logits[t * a.slots + n * each + (entry - n * round - mine)] = x;
+            }
+        });
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+        if (lane == 0) red[warp][t] = st[t];
+    __syncthreads();
+    if (threadIdx.x < NT) {
+        HeadSums x = head_no_sums();
+        for (int w = 0; w < kHeadVecThreads / 32; ++w) x = head_join3(x, red[w][threadIdx.x]);
+        a.part[(int64_t)threadIdx.x * gridDim.x + blockIdx.x] = x;
+    }
+    if (a.top == 0) return;
+    // whole rounds, and what the last one has here
+    const int last = a.v.vocab / round, have = last * each + max(min(a.v.vocab - last * round - mine, each), 0);
+    // none, where there are fewer entries than alternatives, or NaN (which has no place) takes others' places
+    for (int i = threadIdx.x; i < NT * a.top; i += kHeadVecThreads)
+        a.cand[((int64_t)(i / a.top) * gridDim.x + blockIdx.x) * a.top + i % a.top] =
+            make_float2(-INFINITY, __int_as_float(0x7fffffff));
+    __syncthreads();
+#pragma unroll 1
+    for (int t = 0; t < NT; ++t)
+        for (int i = threadIdx.x; i < have; i += kHeadVecThreads) {
+            const float* l = logits + t * a.slots;
+            const float x = l[i];
+            int place = 0;
+            for (int j = 0; j < have; ++j) place += HeadBest::before(l[j], j, x, i);
+            if (place < a.top)
+                a.cand[((int64_t)t * gridDim.x + blockIdx.x) * a.top + place] =
+                    make_float2(x, __int_as_float(i / each * round + mine + i % each));
+        }
+}
+
+// A warp a token: joins the CTAs' sums and takes the best of their best.
+__global__ void __launch_bounds__(32)
+    head_vec_probs_join_kernel(const HeadVecProbs a, int ctas, const HeadProbsOut o, uint32_t* err) {
+    const int t = blockIdx.x, lane = threadIdx.x;
+    pdl_wait();
+    const int64_t lab = a.v.labels[t];
+    const bool in = lab != a.v.ignore_index, bad = in && (lab < 0 || lab >= a.v.vocab);
+    HeadSums x = head_no_sums();
+    for (int r = lane; r < ctas; r += 32) x = head_join3(x, a.part[(int64_t)t * ctas + r]);
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) x = head_join3(x, head_shuffle(x, s));
+    HeadBest best = HeadBest::none();
+    if (a.top > 0) {
+        // the CTAs whose best entries are the best: no other has one of the first `top`
+        HeadBest at = HeadBest::none();  // its entry in place of the CTA, so that equal ones order as entries do
+        for (int r0 = 0; r0 < ctas; r0 += 32) {
+            const float2 c = r0 + lane < ctas ? a.cand[((int64_t)t * ctas + r0 + lane) * a.top]
+                                              : make_float2(-INFINITY, __int_as_float(0x7fffffff));
+            at.offer(c.x, __float_as_int(c.y), a.top);
+        }
+        const int each = 2 * kHeadVecThreads / 32;
+        for (int k = 0; k < a.top; ++k) {
+            const int entry = __shfl_sync(0xffffffffu, at.i, k);
+            const float m = __shfl_sync(0xffffffffu, at.v, k);
+            if (entry == 0x7fffffff || !HeadBest::before(m, entry, __shfl_sync(0xffffffffu, best.v, a.top - 1),
+                                                         __shfl_sync(0xffffffffu, best.i, a.top - 1)))
+                break;
+            const int cta = entry / each % ctas;
+            const float2 c = lane < a.top ? a.cand[((int64_t)t * ctas + cta) * a.top + lane]
+                                          : make_float2(-INFINITY, __int_as_float(0x7fffffff));
+            best.offer(c.x, __float_as_int(c.y), a.top);
+        }
+    }
+    if (bad && lane == 0) report_dev_error(err, DEVERR_BAD_ARG);
+    head_probs_write(o, t, lane, bad, in && !bad, x, in && !bad ? a.v.label_logit[t] : 0.0f, best);
+}
+
+// The gradient's rows: a token's weight w = |a| + c |b| and, of a / w and b / w,
+// what an entry of its row takes (HeadRowGrad).  One CTA; what is not finite
+// stays its token's.
+struct HeadProbsRows {
+    const int *rows, *count;
+    const float *lse, *entropy, *grad, *grad_entropy;  // per token; the gradients may be null: 0
+    float c, g_bits, g_scale;
+    float *lse_row, *out_scale, *row_scale;
+    float4* row;
+};
+__global__ void __launch_bounds__(1024) head_probs_rows_kernel(const HeadProbsRows a) {
+    __shared__ float wmax[32];
+    pdl_wait();
+    pdl_trigger();
+    const int live = *a.count, lane = threadIdx.x & 31;
+    float top = 0.0f;
+    for (int i = threadIdx.x; i < live; i += 1024) {
+        const int t = a.rows[i];
+        const float ga = a.grad ? a.grad[t] : 0.0f, gb = a.grad_entropy ? a.grad_entropy[t] : 0.0f;
+        const float w = fmaf(a.c, fabsf(gb), fabsf(ga));
+        if (w <= 3.402823466e38f) top = fmaxf(top, w);
+    }
+    top = warp_max(top);
+    if (lane == 0) wmax[threadIdx.x >> 5] = top;
+    __syncthreads();
+    top = warp_max(wmax[lane]);
+    for (int i = threadIdx.x; i < live; i += 1024) {
+        const int t = a.rows[i];
+        const float ga = a.grad ? a.grad[t] : 0.0f, gb = a.grad_entropy ? a.grad_entropy[t] : 0.0f;
+        const float w = fmaf(a.c, fabsf(gb), fabsf(ga));
+        const float ua = w == 0.0f ? 0.0f : ga / w, ub = w == 0.0f ? 0.0f : gb / w, gamma = ub * kLn2;
+        a.lse_row[i] = a.lse[t];
+        a.row_scale[i] = w / a.g_scale;
+        a.row[i] = make_float4(ua * a.g_scale, fmaf(-gamma, a.g_bits, fmaf(ub, a.entropy[t], ua)), gamma, w == 0.0f ? 0.0f : w / top);
+    }
+    if (threadIdx.x == 0) *a.out_scale = top / a.g_scale;
+}
+
+}  // namespace aeth

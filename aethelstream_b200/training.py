@@ -4,6 +4,9 @@
 * ``cut_cross_entropy`` / ``cut_cross_entropy_backward``: the loss at the
   language model's head and its gradient, a vocabulary piece at a time, without
   keeping the logits (streaming_cut_ce, doublepass/src/loss.rs:83-377).
+* ``token_log_probs`` / ``token_log_probs_backward``: log probabilities of given
+  tokens at the head, with the entropy and the likeliest alternatives, and the
+  gradient of the first two.
 * ``rms_norm_checkpoint``: RMS norm that keeps its input in 8 bits, as the first
   pass leaves it for the second; ``checkpoint_decode`` restores it (or its
   norm), ``rms_norm_checkpoint_backward`` takes the norm's gradient at it.
@@ -162,6 +165,97 @@ def cut_cross_entropy_backward(hidden: torch.Tensor, weight: torch.Tensor, label
         dw.data_ptr() if need_weight else None, d, ws.data_ptr(), size, _raw_stream(dev))
     if st:
         L.check(st, "aeth_cut_ce_backward")
+    return dh, dw
+
+
+# ---- log probabilities ----
+MAX_ALTERNATIVES = 32
+
+
+@dataclass(slots=True)
+class TokenLogProbs:
+    """Result of ``token_log_probs``, float32 of the labels' shape: log
+    probabilities, entropies and log-sum-exps (the backward needs the last two).
+    top_log_probs and top_ids (int64) have top_k entries more in a last dimension;
+    None without alternatives."""
+    log_probs: torch.Tensor
+    entropy: torch.Tensor
+    lse: torch.Tensor
+    top_log_probs: torch.Tensor | None
+    top_ids: torch.Tensor | None
+
+
+def token_log_probs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, top_k: int = 0,
+                    ignore_index: int = -100) -> TokenLogProbs:
+    """Log probabilities of `labels` under softmax(hidden @ weight.T), the entropies
+    (natural logarithm) of those distributions, and with `top_k` (up to 32) the
+    likeliest entries: log probabilities, the largest first, and indices, the lower
+    first among equal logits.  hidden (..., d) and weight (vocab, d) are bfloat16 or
+    float16.  Tokens labelled `ignore_index` take no part: they get 0, and indices
+    -1.  A label outside the vocabulary gets NaN and -1 and sets DEVERR_BAD_ARG in
+    the device error word; a token whose logits hold a NaN or +infinity gets NaN
+    and -1 too."""
+    what, dev = "token_log_probs", hidden.get_device()
+    if dev < 0 or dev != _current_device():
+        return _elsewhere(what, dev, token_log_probs, hidden, weight, labels, top_k, ignore_index)
+    lab = _head_args(what, hidden, weight, labels)
+    v, d = weight.shape
+    if not 0 <= top_k <= min(MAX_ALTERNATIVES, v):
+        raise ValueError(f"{what}: top_k must be 0 to {min(MAX_ALTERNATIVES, v)}, got {top_k}")
+    h, n, ld_h = _rows(hidden, d)
+    w, _, ld_w = _tma_rows(weight, d)
+    lp, entropy, lse = (lab.new_empty(labels.shape, dtype=torch.float32) for _ in range(3))
+    top = ids = None
+    if top_k:
+        top, ids = (lab.new_empty((*labels.shape, top_k), dtype=t) for t in (torch.float32, torch.int64))
+    size = _workspace_bytes("aeth_token_log_probs_workspace", dev, n, d, v, top_k, 0)
+    ws = lab.new_empty(size, dtype=torch.uint8)
+    st = _lib.aeth_token_log_probs(
+        h.data_ptr(), ld_h, w.data_ptr(), ld_w, _DTYPES[h.dtype], lab.data_ptr(), n, d, v, ignore_index, top_k,
+        lp.data_ptr(), entropy.data_ptr(), lse.data_ptr(), top.data_ptr() if top_k else None,
+        ids.data_ptr() if top_k else None, ws.data_ptr(), size, _raw_stream(dev))
+    if st:
+        L.check(st, "aeth_token_log_probs")
+    return TokenLogProbs(lp, entropy, lse, top, ids)
+
+
+def token_log_probs_backward(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, result: TokenLogProbs,
+                             grad_log_probs: torch.Tensor | None = None, grad_entropy: torch.Tensor | None = None,
+                             ignore_index: int = -100, need_hidden: bool = True, need_weight: bool = True):
+    """(d_hidden, d_weight) of sum(grad_log_probs * log_probs) + sum(grad_entropy *
+    entropy) in the inputs' type; None where not needed.  The gradients of the
+    results are float32, one per token; None counts as zeros.  `result` is what
+    ``token_log_probs`` gave for these inputs."""
+    what, dev = "token_log_probs_backward", hidden.get_device()
+    if dev < 0 or dev != _current_device():
+        return _elsewhere(what, dev, token_log_probs_backward, hidden, weight, labels, result, grad_log_probs, grad_entropy,
+                          ignore_index, need_hidden, need_weight)
+    lab = _head_args(what, hidden, weight, labels)
+    v, d = weight.shape
+    h, n, ld_h = _rows(hidden, d)
+    for t in (result.lse, result.entropy):
+        if t.dtype != torch.float32 or t.numel() != n:
+            raise ValueError(f"{what}: result must be that of token_log_probs for these tokens")
+    for t in (grad_log_probs, grad_entropy):
+        if t is not None and (t.dtype != torch.float32 or t.numel() != n):
+            raise ValueError(f"{what}: gradients must be float32, one per token")
+    _same_device(what, dev, result.lse, result.entropy, grad_log_probs, grad_entropy)
+    if not need_hidden and not need_weight:
+        return None, None
+    w, _, ld_w = _tma_rows(weight, d)
+    lse, entropy = result.lse.contiguous(), result.entropy.contiguous()
+    ga, gb = (None if t is None else t.contiguous() for t in (grad_log_probs, grad_entropy))
+    dh = h.new_empty(hidden.shape) if need_hidden else None
+    dw = h.new_empty(weight.shape) if need_weight else None
+    size = _workspace_bytes("aeth_token_log_probs_workspace", dev, n, d, v, 0, 1)
+    ws = lab.new_empty(size, dtype=torch.uint8)
+    st = _lib.aeth_token_log_probs_backward(
+        h.data_ptr(), ld_h, w.data_ptr(), ld_w, _DTYPES[h.dtype], lab.data_ptr(), n, d, v, ignore_index, lse.data_ptr(),
+        entropy.data_ptr(), None if ga is None else ga.data_ptr(), None if gb is None else gb.data_ptr(),
+        dh.data_ptr() if need_hidden else None, d, dw.data_ptr() if need_weight else None, d, ws.data_ptr(), size,
+        _raw_stream(dev))
+    if st:
+        L.check(st, "aeth_token_log_probs_backward")
     return dh, dw
 
 

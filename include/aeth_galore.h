@@ -544,6 +544,31 @@ int aeth_cut_ce_backward(const void* hidden, int64_t ld_hidden, const void* weig
                          void* d_weight, int64_t ld_dw, void* workspace, size_t workspace_bytes,
                          aeth_stream_t stream);
 
+/* Log probabilities of given tokens under softmax(hidden weight^T), with the
+ * distributions' entropies and the likeliest entries; arguments as above.
+ *   log_probs[t] = s_t,label - lse_t, entropy[t] = lse_t - sum_v p_tv s_tv (n
+ *   floats each; lse too, for the backward).  top: the number of likeliest entries
+ *   wanted, 0 to 32 and at most vocab: their log probabilities, the largest first,
+ *   and their indices (n x top; the lower index first among equal logits).
+ *   Tokens with ignore_index get 0, and indices -1.  A label outside the vocabulary
+ *   sets AETH_DEVERR_BAD_ARG and gets NaN, and indices -1; so does a token whose
+ *   logits hold a NaN or +infinity (without the bit).
+ *   The logits are kept for a piece of the vocabulary where top > 0 (256 MiB, or
+ *   256 entries where these take more), else not at all.
+ *   backward: of sum_t grad_log_probs[t] log_probs[t] + grad_entropy[t] entropy[t]
+ *   (either may be NULL: 0), lse and entropy being the forward's; G as the loss's,
+ *   in F16 twice where d_hidden is wanted. */
+int aeth_token_log_probs_workspace(int64_t n, int64_t d, int64_t vocab, int top, int backward, size_t* bytes);
+int aeth_token_log_probs(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, int dtype,
+                         const int64_t* labels, int64_t n, int64_t d, int64_t vocab, int64_t ignore_index, int top,
+                         float* log_probs, float* entropy, float* lse, float* top_log_probs, int64_t* top_ids, void* workspace,
+                         size_t workspace_bytes, aeth_stream_t stream);
+int aeth_token_log_probs_backward(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, int dtype,
+                                  const int64_t* labels, int64_t n, int64_t d, int64_t vocab, int64_t ignore_index,
+                                  const float* lse, const float* entropy, const float* grad_log_probs,
+                                  const float* grad_entropy, void* d_hidden, int64_t ld_dh, void* d_weight, int64_t ld_dw,
+                                  void* workspace, size_t workspace_bytes, aeth_stream_t stream);
+
 /* RMS norm (doublepass/src/math.rs) with its input kept in 8 bits (the role of
  * ramflow/kernels/checkpoint_compress.cu, with scales per row and block of 128
  * features instead of per channel).  s = x, or x + residual rounded to the
