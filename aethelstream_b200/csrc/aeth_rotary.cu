@@ -10,7 +10,7 @@ using namespace aeth;
 
 namespace {
 
-constexpr int64_t kRotMaxRows = 1ll << 40;
+constexpr int64_t kRotMaxRows = 1ll << 38;
 
 bool rot_dtype(int dtype) { return dtype == AETH_DTYPE_F32 || dtype == AETH_DTYPE_F16 || dtype == AETH_DTYPE_BF16; }
 int rot_size(int dtype) { return dtype == AETH_DTYPE_F32 ? 4 : 2; }
@@ -37,9 +37,9 @@ bool rot_whole(const AethHeads& h, int64_t tokens, int size) {
            (h.heads == 1 || h.ld_head * size % 16 == 0);
 }
 
-// Rows of a stretch and CTAs of the grid.  A stretch is what gives every SM six
-// CTAs, 512 rows at most and what the table of its tokens holds; `most`: CTAs
-// that q and k may have together (0: one for each stretch).
+// Rows of a stretch and CTAs of rotary_any_kernel's grid.  A stretch is what gives
+// every SM six CTAs, 512 rows at most and what the table of its tokens holds;
+// `most`: CTAs that q and k may have together (0: one for each stretch).
 void rot_grid(RotaryArgs& a, int64_t tokens, int step, int most) {
     const int held = kRotTableBytes / (4 * a.R);  // tokens; 8 at least
     const int64_t all = a.s[0].rows + a.s[1].rows;
@@ -61,27 +61,41 @@ void rot_grid(RotaryArgs& a, int64_t tokens, int step, int most) {
     a.table_bytes = (int)rot_up(table, 16);
 }
 
-constexpr int kRotBackPerSm = 4;  // CTAs of the norm's gradient, each of which leaves sums of the gain's
-int rot_back_ctas() { return kRotBackPerSm * num_sms(); }
+// CTAs of an SM, and how many waves of them.  A CTA's start (its table, the first
+// rows' way) is hidden behind the others' rows where they start apart, and costs
+// issue slots: the rotation, which has these to spare, 63, 58, 56 and 60 us in one, two,
+// three and four waves of three, the norm 62.7, 62.1, 67 and the gradient (two of an
+// SM: 126 registers) 92, 102 and 110 in one, two and three.
+template <int OP>
+constexpr int rot_per_sm() { return OP == ROT_NORM_BACK ? 2 : 3; }
+template <int OP>
+constexpr int rot_waves() { return OP == ROT_TURN ? 3 : OP == ROT_NORM ? 2 : 1; }
+int rot_back_ctas() { return rot_per_sm<ROT_NORM_BACK>() * num_sms(); }  // each leaves sums of the gains'
 
 template <typename T, bool INTER, int OP>
 int rot_launch(RotaryArgs& a, int64_t tokens, bool whole, cudaStream_t st) {
-    constexpr int U = sizeof(T) == 4 ? (OP == ROT_NORM_BACK ? 1 : 2) : (OP == ROT_NORM_BACK ? 2 : 4);
-    const int most = OP == ROT_NORM_BACK ? rot_back_ctas() : 0;
+    static std::atomic<bool> allowed[2][kMaxDevices] = {};
     if (whole && a.D % 16 == 0 && a.R % 16 == 0 && a.D <= 512) {
         int lanes = 1;
         while (lanes < a.D / 16) lanes *= 2;
-        const int groups = kRotThreads / lanes;
-        rot_grid(a, tokens, groups * U, most);
-        if (OP == ROT_NORM_BACK) a.table_bytes = std::max(a.table_bytes, groups * a.D * 4);
-        const int smem = a.table_bytes + (OP == ROT_TURN ? 0 : a.D * 4);
-        rotary_kernel<T, INTER, OP, U><<<a.s[0].ctas + a.s[1].ctas, kRotThreads, smem, st>>>(a, lanes);
+        const int groups = kRotThreads / lanes, held = kRotTableBytes / (4 * a.R);
+        const int64_t rows = std::max(a.s[0].rows, a.s[1].rows);
+        const unsigned ctas = (unsigned)std::min<int64_t>((rows + groups - 1) / groups, (int64_t)rot_waves<OP>() * rot_per_sm<OP>() * num_sms());
+        int64_t most = 0;  // tokens that a CTA's rows have, and one more
+        for (RotaryRows& s : a.s) {
+            s.ctas = s.rows > 0 ? ctas : 0;
+            most = std::max<int64_t>(most, ((s.rows + ctas - 1) / ctas + s.heads - 2) / s.heads + 2);
+        }
+        const int sums = rot_ring_bytes<T, OP>() + (OP == ROT_TURN ? 0 : a.D * 8) + (int)std::min<int64_t>(most, held) * a.R * 4;
+        const int smem = sums + (OP == ROT_NORM_BACK ? groups * a.D * 4 : 0);
+        auto kern = rotary_kernel<T, INTER, OP, rot_per_sm<OP>()>;
+        AETH_TRY(allow_shared(kern, rot_ring_bytes<T, OP>() + 512 * 8 + kRotTableBytes + 16 * kRotThreads * 4, allowed[0]));
+        kern<<<ctas, kRotThreads, smem, st>>>(a, lanes, held, sums / 4);
     } else {
-        rot_grid(a, tokens, kRotThreads / 32, most);
+        rot_grid(a, tokens, kRotThreads / 32, OP == ROT_NORM_BACK ? rot_back_ctas() : 0);
         const int smem = a.table_bytes + (OP == ROT_NORM_BACK ? kRotThreads / 32 * a.D * 4 : 0);
         auto kern = rotary_any_kernel<T, INTER, OP>;
-        static std::atomic<bool> allowed[kMaxDevices] = {};
-        AETH_TRY(allow_shared(kern, 2 * kRotTableBytes, allowed));
+        AETH_TRY(allow_shared(kern, 2 * kRotTableBytes, allowed[1]));
         kern<<<a.s[0].ctas + a.s[1].ctas, kRotThreads, smem, st>>>(a);
     }
     AETH_LAUNCH_CHECK();
@@ -109,6 +123,7 @@ RotaryArgs rot_args(const AethRotaryPlan& p, const AethHeads& q, const AethHeads
         a.s[i].ld_h = h[i]->ld_head;
         a.s[i].out = out[i];
         a.s[i].heads = std::max(h[i]->heads, 1);
+        a.s[i].magic = (uint32_t)(((1ull << 32) + a.s[i].heads - 1) / a.s[i].heads);
         a.s[i].rows = tokens * h[i]->heads;
     }
     a.pos = p.positions;
@@ -162,7 +177,7 @@ int aeth_qk_norm_rotary(const AethRotaryPlan* plan, const AethHeads* q, const Ae
 int aeth_qk_norm_rotary_backward_workspace(int head_dim, size_t* bytes) {
     if (head_dim <= 0 || !bytes) return set_err(AETH_ERR_ARG);
     if (head_dim > kRotMaxHead) return set_err(AETH_ERR_UNSUPPORTED);
-    *bytes = (size_t)(rot_back_ctas() + 2) * (size_t)head_dim * sizeof(float);
+    *bytes = (size_t)(rot_back_ctas() + 1) * 2 * (size_t)head_dim * sizeof(float);
     return AETH_OK;
 }
 
@@ -196,13 +211,11 @@ int aeth_qk_norm_rotary_backward(const AethRotaryPlan* plan, const AethHeads* dq
     a.s[1].gain = k_gain;
     a.gain_dtype = gain_dtype;
     a.eps = eps;
-    // q's CTAs and k's together: rot_back_ctas(), or one more of either for the share that rounds down to none
     a.s[0].part = static_cast<float*>(workspace);
     const int size = rot_size(dtype);
     bool whole = rot_out_whole(dq_out) && rot_out_whole(dk_out);
     for (const AethHeads* h : {q, k, dq, dk}) whole = whole && rot_whole(*h, tokens, size);
-    const int64_t all = a.s[0].rows + a.s[1].rows;
-    a.s[1].part = a.s[0].part + (std::max<int64_t>(a.s[0].rows * rot_back_ctas() / all, 1)) * head_dim;
+    a.s[1].part = a.s[0].part + (int64_t)(rot_back_ctas() + 1) * head_dim;
     AETH_TRY(rot_typed<ROT_NORM_BACK>(a, tokens, dtype, plan->interleaved != 0, whole, st));
     const RotaryGain g{{a.s[0].part, a.s[1].part}, {d_q_gain, d_k_gain}, {(int)a.s[0].ctas, (int)a.s[1].ctas}, head_dim};
     const bool both = q->heads && k->heads;

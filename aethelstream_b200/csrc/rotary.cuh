@@ -19,9 +19,18 @@
 // D / 16 lanes (a power of two; lanes past it idle): a lane holds eight features
 // at 8 c and the eight R / 2 further on, which are eight pairs in either layout,
 // so a row needs no exchange but the norm's sums.  A CTA takes a stretch of the
-// (token, head) rows; its tokens' cosines go to shared memory first, each for
-// all the heads.
+// (token, head) rows, all SMs one wave of them; its tokens' cosines go to shared
+// memory first, each for all the heads of q and k.  A lane's rows to come are on
+// their way to shared memory by asynchronous copies of its own, which it alone
+// reads: bytes in flight without registers, and no barrier.  8192 tokens x (64 + 8)
+// heads x 128 bf16: rotation 56 us (5.4 TB/s), with the norm 62 (4.9), the gradient
+// 92 (4.9), where a copy of as many bytes takes 50, 50 and 73.  What is left is
+// the instructions of a row (issue slots half taken) and a CTA's first microsecond,
+// its table; with rows straight from global memory to registers it took 66, 82 and
+// 162 us, with q's rows and k's in CTAs of their own 72, 78 and 123.
 #pragma once
+#include <type_traits>
+
 #include "pack8.cuh"
 
 namespace aeth {
@@ -39,9 +48,10 @@ struct RotaryRows {  // one of q and k
     const void* gain;
     float* part;     // the norm's gradient: D sums for each of the CTAs
     int heads;
+    uint32_t magic;  // of rot_quotient
     int64_t rows;    // tokens x heads
-    int stretch;     // rows of a CTA's stretch; a CTA takes every ctas-th stretch
-    unsigned ctas;   // of the grid
+    int stretch;     // rotary_any_kernel: rows of a stretch, of which a CTA takes every ctas-th
+    unsigned ctas;   // CTAs that have rows of it (rotary_any_kernel: for it alone)
 };
 struct RotaryArgs {
     RotaryRows s[2];  // q, k
@@ -53,7 +63,7 @@ struct RotaryArgs {
     int flip;              // the other way round
     int D, R, gain_dtype;
     float eps;
-    int table_bytes;  // shared memory before the gain (any: before the sums)
+    int table_bytes;  // rotary_any_kernel: shared memory before the sums
 };
 
 __device__ __forceinline__ float2 rot_angle(uint64_t t, float amp, bool flip) {
@@ -66,69 +76,104 @@ __device__ __forceinline__ float2 rot_angle(uint64_t t, float amp, bool flip) {
     const float cs = quarter & 2 ? -x : x, sn = quarter & 2 ? -y : y;
     return make_float2(cs * amp, (flip ? -sn : sn) * amp);
 }
+// n / heads for n below heads + a stretch (512): a product with 2^32 / heads, rounded
+// up, is exact there up to 32768 heads; with more the quotient is 0 or 1.
+__device__ __forceinline__ int rot_quotient(int n, int heads, uint32_t magic) {
+    return heads == 1 ? n : heads > 32768 ? (n >= heads ? 1 : 0) : (int)__umulhi((uint32_t)n, magic);
+}
 __device__ __forceinline__ int64_t rot_position(const RotaryArgs& a, int64_t token) {
     const int64_t i = a.period == 1 ? 0 : token % a.period;
     return a.pos32 ? (int64_t)static_cast<const int*>(a.pos)[i] : static_cast<const int64_t*>(a.pos)[i];
 }
 
 // The cosines and sines of tokens t0 .. t0 + count - 1: place(p) is where pair
-// p's cosine lies among a token's R / 2; the sines follow.
+// p's cosine lies among a token's R / 2; the sines follow.  A thread keeps its pair.
 template <typename Place>
 __device__ __forceinline__ void rot_table(const RotaryArgs& a, float* table, int64_t t0, int count, Place place) {
-    const int half = a.R / 2;
-    for (int i = threadIdx.x; i < count * half; i += kRotThreads) {
-        const int tok = i / half, p = i - tok * half;
-        const float2 cs = rot_angle((uint64_t)rot_position(a, t0 + tok) * a.freq[p], a.amp, a.flip);
-        float* o = table + tok * a.R + place(p);
-        o[0] = cs.x;
-        o[half] = cs.y;
+    const int half = a.R / 2, side = half < kRotThreads ? kRotThreads / half : 1;  // tokens side by side
+    const int mine = half < kRotThreads ? threadIdx.x / half : 0;
+    if (mine >= side) return;
+    for (int p = threadIdx.x - mine * half; p < half; p += kRotThreads) {
+        const uint64_t f = a.freq[p];
+        float* o = table + place(p);
+#pragma unroll 2
+        for (int tok = mine; tok < count; tok += side) {
+            const float2 cs = rot_angle((uint64_t)rot_position(a, t0 + tok) * f, a.amp, a.flip);
+            o[tok * a.R] = cs.x;
+            o[tok * a.R + half] = cs.y;
+        }
     }
 }
 
-// Turns a lane's sixteen features by its eight pairs' cosines and sines.
-template <bool INTER>
-__device__ __forceinline__ void rot_turn(float (&lo)[8], float (&hi)[8], const float (&c)[8], const float (&s)[8]) {
-    if (INTER) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float u = lo[2 * e], v = lo[2 * e + 1], x = hi[2 * e], y = hi[2 * e + 1];
-            lo[2 * e] = u * c[e] - v * s[e];
-            lo[2 * e + 1] = v * c[e] + u * s[e];
-            hi[2 * e] = x * c[4 + e] - y * s[4 + e];
-            hi[2 * e + 1] = y * c[4 + e] + x * s[4 + e];
-        }
+// Eight features of a row and the eight beside them, from shared or to global memory.
+template <typename T>
+__device__ __forceinline__ void rot_get(const uint4* p, int pitch, float2 (&v)[4]) {
+    if constexpr (sizeof(T) == 4) {
+        const uint4 a = p[0], b = p[pitch];
+        v[0] = make_float2(__uint_as_float(a.x), __uint_as_float(a.y));
+        v[1] = make_float2(__uint_as_float(a.z), __uint_as_float(a.w));
+        v[2] = make_float2(__uint_as_float(b.x), __uint_as_float(b.y));
+        v[3] = make_float2(__uint_as_float(b.z), __uint_as_float(b.w));
     } else {
+        const uint4 a = p[0];
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float u = lo[e], v = hi[e];
-            lo[e] = u * c[e] - v * s[e];
-            hi[e] = v * c[e] + u * s[e];
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (std::is_same_v<T, __nv_bfloat16>)
+                v[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+            else
+                v[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
         }
     }
 }
 template <typename T>
-__device__ __forceinline__ void rot_unpack(const Pack8<T>& p, float (&v)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = ck_value<T>(p, i);
+__device__ __forceinline__ void rot_put(T* p, const float2 (&v)[4]) {
+    if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<float4*>(p)[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+        reinterpret_cast<float4*>(p)[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+    } else {
+        *reinterpret_cast<uint4*>(p) = make_uint4(ck_pack2<T>(v[0].x, v[0].y), ck_pack2<T>(v[1].x, v[1].y),
+                                                  ck_pack2<T>(v[2].x, v[2].y), ck_pack2<T>(v[3].x, v[3].y));
+    }
 }
-template <typename T>
-__device__ __forceinline__ Pack8<T> rot_load(const T* p) {
-    Pack8<T> v;
-#pragma unroll
-    for (int k = 0; k < Pack8<T>::kWords; ++k) v.w[k] = ck_stream(reinterpret_cast<const uint4*>(p) + k);
-    return v;
+__device__ __forceinline__ void rot_copy(uint4* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32_addr(to)), "l"(from) : "memory");
 }
-template <typename T>
-__device__ __forceinline__ void rot_store(T* p, const Pack8<T>& v) {
-#pragma unroll
-    for (int k = 0; k < Pack8<T>::kWords; ++k) reinterpret_cast<uint4*>(p)[k] = v.w[k];
-}
-__device__ __forceinline__ void rot_four(const float4* p, float* v) {
+__device__ __forceinline__ void rot_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void rot_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Four values of a table [four of a lane][lane], as two pairs.
+__device__ __forceinline__ void rot_four(const float4* p, float2& a, float2& b) {
     const float4 x = *p;
-    v[0] = x.x;
-    v[1] = x.y;
-    v[2] = x.z;
-    v[3] = x.w;
+    a = make_float2(x.x, x.y);
+    b = make_float2(x.z, x.w);
+}
+// Turns a lane's eight low and eight high features by its eight pairs' cosines
+// and sines ([cosines 0-3, 4-7, sines 0-3, 4-7][lane]).
+template <bool INTER>
+__device__ __forceinline__ void rot_turn(float2 (&lo)[4], float2 (&hi)[4], const float4* t, int pitch) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        float2 c[2], s[2];
+        rot_four(t + k * pitch, c[0], c[1]);
+        rot_four(t + (k + 2) * pitch, s[0], s[1]);
+        if (INTER) {  // a pair of features is a pair
+            float2(&x)[4] = k ? hi : lo;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float ci = i & 1 ? c[i / 2].y : c[i / 2].x, si = i & 1 ? s[i / 2].y : s[i / 2].x;
+                x[i] = make_float2(x[i].x * ci - x[i].y * si, x[i].y * ci + x[i].x * si);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float2 u = lo[2 * k + i], v = hi[2 * k + i], ns = make_float2(-s[i].x, -s[i].y);
+                lo[2 * k + i] = fma2_rn(v, ns, mul2_rn(u, c[i]));
+                hi[2 * k + i] = fma2_rn(u, s[i], mul2_rn(v, c[i]));
+            }
+        }
+    }
 }
 __device__ __forceinline__ float rot_sum(float v, int lanes) {
     for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -137,149 +182,205 @@ __device__ __forceinline__ float rot_sum(float v, int lanes) {
 
 enum RotaryOp { ROT_TURN = 0, ROT_NORM = 1, ROT_NORM_BACK = 2 };
 
-// lanes: of a row, the power of two from D / 16 on.  U: rows that a lane has in flight.
-template <typename T, bool INTER, int OP, int U>
-__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_constant__ RotaryArgs a, int lanes) {
-    extern __shared__ float4 rot_sh[];  // a token's table: [cos 0-3, cos 4-7, sin 0-3, sin 4-7 of the lane][lane]; gain; sums
-    const int which = blockIdx.x >= a.s[0].ctas ? 1 : 0;
-    const RotaryRows& s = a.s[which];
-    const unsigned cta = blockIdx.x - (which ? a.s[0].ctas : 0);
+// What a lane copies of its rows to come: 16-byte pieces of the low features, the
+// high ones, and those of dy.
+template <typename T, int OP>
+constexpr int rot_pieces() { return (int)sizeof(T) / 2 * (OP == ROT_NORM_BACK ? 4 : 2); }
+// Stages of the ring: 32 KB a CTA, 48 KB of the gradient's (at 8192 x (64 + 8) x 128
+// bf16, rotation 56 to 58 us with 4 to 8 stages, gradient 96, 92 and 93 with 2, 3 and 4).
+template <typename T, int OP>
+constexpr int rot_stages() {
+    constexpr int s = (OP == ROT_NORM_BACK ? 12 : 8) / rot_pieces<T, OP>();
+    return s > 2 ? s : 2;
+}
+template <typename T, int OP>
+constexpr int rot_ring_bytes() { return rot_pieces<T, OP>() * rot_stages<T, OP>() * kRotThreads * 16; }
+
+// r / heads
+__device__ __forceinline__ int64_t rot_token(int64_t r, int heads) {
+    return r <= 0xffffffffll ? (int64_t)((uint32_t)r / (uint32_t)heads) : r / heads;
+}
+
+// lanes: of a row, the power of two from D / 16 on.  held: tokens of the table, at
+// most.  sums_at: where the gradient's groups x D sums lie in shared memory.
+// Of q's rows and of k's a CTA takes the same share, so that its table serves both.
+template <typename T, bool INTER, int OP, int CTAS>
+__global__ void __launch_bounds__(kRotThreads, CTAS) rotary_kernel(const __grid_constant__ RotaryArgs a, int lanes, int held, int sums_at) {
+    constexpr int P = rot_pieces<T, OP>(), S = rot_stages<T, OP>(), Q = (int)sizeof(T) / 2;  // Q: pieces of eight features
+    extern __shared__ float4 rot_sh[];  // ring [stage][piece][thread]; q's and k's gain [low 0-3, 4-7, high 0-3, 4-7][lane]; table
+    uint4* ring = reinterpret_cast<uint4*>(rot_sh) + threadIdx.x;
+    float4* gains = rot_sh + rot_ring_bytes<T, OP>() / 16;
+    float4* table = gains + (OP == ROT_TURN ? 0 : a.D / 2);
     const int c = threadIdx.x & (lanes - 1), turning = a.R / 16, all = a.D / 16;
     const int group = threadIdx.x / lanes, groups = kRotThreads / lanes;
     const bool turns = c < turning, mine = c < all;
     const int lo = turns ? 8 * c : a.R + 16 * (c - turning), hi = turns ? a.R / 2 + 8 * c : lo + 8;
-    float4* gain = rot_sh + a.table_bytes / 16;  // [lo 0-3, lo 4-7, hi 0-3, hi 4-7][lane]
-    float wl[8], wh[8];                           // gradient: the sums of the gain's
-    if (OP == ROT_NORM_BACK)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) wl[i] = wh[i] = 0.0f;
-    if (OP != ROT_TURN && group == 0 && mine)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int at = (i < 2 ? lo : hi) + 4 * (i & 1);
-            gain[i * all + c] = make_float4(load_as_f32(s.gain, at, a.gain_dtype), load_as_f32(s.gain, at + 1, a.gain_dtype),
-                                            load_as_f32(s.gain, at + 2, a.gain_dtype), load_as_f32(s.gain, at + 3, a.gain_dtype));
+    if (OP != ROT_TURN)
+        for (int i = threadIdx.x; i < 2 * a.D; i += kRotThreads) {
+            const int which = i >= a.D ? 1 : 0, d = i - which * a.D, half = a.R / 2;
+            // feature d: of lane l its e-th, low or high
+            const bool high = d < a.R ? d >= half : (d - a.R) & 8;
+            const int l = d < a.R ? (high ? d - half : d) / 8 : turning + (d - a.R) / 16, e = (d < a.R && high ? d - half : d) & 7;
+            if (a.s[which].rows > 0)
+                reinterpret_cast<float*>(gains)[which * a.D + (((high ? 2 : 0) + (e >> 2)) * all + l) * 4 + (e & 3)] =
+                    load_as_f32(a.s[which].gain, d, a.gain_dtype);
         }
-    const T *x = static_cast<const T*>(s.x), *dy = static_cast<const T*>(s.dy);
-    T* out = static_cast<T*>(s.out);
-    for (int64_t r0 = (int64_t)cta * s.stretch; r0 < s.rows; r0 += (int64_t)s.ctas * s.stretch) {
-        const int64_t t0 = r0 / s.heads;
-        const int h0 = (int)(r0 - t0 * s.heads), count = (int)min((int64_t)s.stretch, s.rows - r0);
-        __syncthreads();
-        rot_table(a, reinterpret_cast<float*>(rot_sh), t0, (h0 + count - 1) / s.heads + 1, [&](int p) {
-            // a lane's pairs: eight in a row, or four at its low and four at its high features
-            const int q = a.R / 4, l = INTER ? (p < q ? p : p - q) / 4 : p / 8;
-            const int e = INTER ? (p & 3) + (p < q ? 0 : 4) : p & 7;
-            return ((e >> 2) * turning + l) * 4 + (e & 3);
-        });
-        __syncthreads();
-        for (int i0 = group; i0 - group < count; i0 += U * groups) {  // the same for all lanes of a warp
-            Pack8<T> xl[U], xh[U], gl[U], gh[U];
-            int tok[U];
+    auto begin_of = [&](int which, unsigned cta) { return a.s[which].rows * cta / gridDim.x; };
+    int64_t base = 0, until = 0;  // the table's first token, and the one past its last
+#pragma unroll 1
+    for (int which = 0; which < 2; ++which) {
+        const RotaryRows& s = a.s[which];
+        const int64_t begin = begin_of(which, blockIdx.x), end = begin_of(which, blockIdx.x + 1);
+        // this lane's first row; a step of `groups` rows is step_t tokens and step_h heads
+        const int step_t = groups / s.heads, step_h = groups - step_t * s.heads;
+        const int64_t first = begin + group, token = rot_token(first, s.heads);
+        int h = (int)(first - token * s.heads), tok = 0;
+        // rows on their way to the ring: how many are left, the next one's head and place
+        int left = (int)(end - first), ahead_h = h, fill = 0, use = 0;
+        const T* px = static_cast<const T*>(s.x) + token * s.ld_t + h * s.ld_h;
+        const T* pd = OP == ROT_NORM_BACK ? static_cast<const T*>(s.dy) + token * s.ld_dt + h * s.ld_dh : nullptr;
+        const int64_t move = step_t * s.ld_t + step_h * s.ld_h, wrap = s.ld_t - s.heads * s.ld_h;
+        const int64_t move_d = step_t * s.ld_dt + step_h * s.ld_dh, wrap_d = s.ld_dt - s.heads * s.ld_dh;
+        auto fetch = [&] {
+            if (left > 0 && mine) {
+                uint4* r = ring + fill * P * kRotThreads;
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int i = i0 + u * groups;
-                tok[u] = (h0 + i) / s.heads;
-                if (i < count && mine) {
-                    const int64_t t = t0 + tok[u];
-                    const int h = h0 + i - tok[u] * s.heads;
-                    const T* p = x + t * s.ld_t + h * s.ld_h;
-                    xl[u] = rot_load(p + lo);
-                    xh[u] = rot_load(p + hi);
+                for (int k = 0; k < Q; ++k) {
+                    rot_copy(r + k * kRotThreads, px + lo + k * 4);
+                    rot_copy(r + (Q + k) * kRotThreads, px + hi + k * 4);
                     if (OP == ROT_NORM_BACK) {
-                        const T* q = dy + t * s.ld_dt + h * s.ld_dh;
-                        gl[u] = rot_load(q + lo);
-                        gh[u] = rot_load(q + hi);
+                        rot_copy(r + (2 * Q + k) * kRotThreads, pd + lo + k * 4);
+                        rot_copy(r + (3 * Q + k) * kRotThreads, pd + hi + k * 4);
                     }
                 }
             }
+            rot_commit();
+            left -= groups;
+            fill = fill + 1 == S ? 0 : fill + 1;
+            ahead_h += step_h;
+            const bool over = ahead_h >= s.heads;
+            if (over) ahead_h -= s.heads;
+            px += move + (over ? wrap : 0);
+            if (OP == ROT_NORM_BACK) pd += move_d + (over ? wrap_d : 0);
+        };
+#pragma unroll 1
+        for (int i = 0; i < S - 1; ++i) fetch();
+        const float4* gain = gains + (which ? a.D / 4 : 0);
+        float2 wl[4], wh[4];  // gradient: the sums of the gain's
+        if (OP == ROT_NORM_BACK)
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int i = i0 + u * groups;
-                const bool here = i < count && mine;
-                float l[8], h[8], cs[8], sn[8];
-                if (here) {
-                    rot_unpack(xl[u], l);
-                    rot_unpack(xh[u], h);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) l[e] = h[e] = 0.0f;
+            for (int i = 0; i < 4; ++i) wl[i] = wh[i] = make_float2(0.0f, 0.0f);
+        T* out = static_cast<T*>(s.out) + first * a.D;
+        int64_t row_until = begin;  // rows whose tokens the table holds
+        for (int64_t r = begin; r < end; r += groups) {  // the same for all lanes of the CTA
+            if (min(r + groups, end) > row_until) {
+                const int64_t from = rot_token(r, s.heads), to = rot_token(end - 1, s.heads) + 1;
+                if (from < base || min(to, from + held) > until) {
+                    base = from;
+                    until = min(to, from + held);
+                    if (which == 0 && until - base < held && a.s[1].rows > 0)  // k's rows may reach one token further
+                        until = min(until + 1, a.s[1].rows / a.s[1].heads);
+                    __syncthreads();
+                    rot_table(a, reinterpret_cast<float*>(table), base, (int)(until - base), [&](int p) {
+                        // a lane's pairs: eight in a row, or four at its low and four at its high features
+                        const int q = a.R / 4, l = INTER ? (p < q ? p : p - q) / 4 : p / 8;
+                        const int e = INTER ? (p & 3) + (p < q ? 0 : 4) : p & 7;
+                        return ((e >> 2) * turning + l) * 4 + (e & 3);
+                    });
+                    __syncthreads();
                 }
-                if (here && turns) {
-                    const float4* t = rot_sh + tok[u] * (a.R / 4) + c;
-                    rot_four(t, cs);
-                    rot_four(t + turning, cs + 4);
-                    rot_four(t + 2 * turning, sn);
-                    rot_four(t + 3 * turning, sn + 4);
-                }
-                T* o = out + (r0 + i) * a.D;
-                if (OP == ROT_TURN) {
-                    if (here && turns) rot_turn<INTER>(l, h, cs, sn);
-                } else {
-                    float sq = 0.0f;
+                row_until = until * s.heads;
+                tok = (int)(rot_token(r + group, s.heads) - base);
+            }
+            fetch();  // into the stage that the row before took
+            rot_wait<S - 1>();
+            const uint4* in = ring + use * P * kRotThreads;
+            if (++use == S) use = 0;
+            const bool here = r + group < end && mine;
+            const float4* t = table + tok * (a.R / 4) + c;
+            float2 l[4], u[4];
+            rot_get<T>(in, kRotThreads, l);
+            rot_get<T>(in + Q * kRotThreads, kRotThreads, u);
+            if (!here)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) sq += l[e] * l[e] + h[e] * h[e];
-                    const float r = rsqrtf(rot_sum(sq, lanes) / (float)a.D + a.eps);
-                    float gnl[8], gnh[8];
-                    if (here) {
-                        rot_four(gain + c, gnl);
-                        rot_four(gain + all + c, gnl + 4);
-                        rot_four(gain + 2 * all + c, gnh);
-                        rot_four(gain + 3 * all + c, gnh + 4);
+                for (int e = 0; e < 4; ++e) l[e] = u[e] = make_float2(0.0f, 0.0f);
+            float rinv = 1.0f;
+            if (OP != ROT_TURN) {
+                float2 sq = make_float2(0.0f, 0.0f);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sq = fma2_rn(u[e], u[e], fma2_rn(l[e], l[e], sq));
+                rinv = rsqrtf(rot_sum(sq.x + sq.y, lanes) / (float)a.D + a.eps);
+            }
+            if (OP == ROT_NORM && here) {
+                const float2 rr = make_float2(rinv, rinv);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    float2 g[4];
+                    rot_four(gain + k * all + c, g[0], g[1]);
+                    rot_four(gain + (k + 2) * all + c, g[2], g[3]);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        l[2 * k + e] = mul2_rn(mul2_rn(l[2 * k + e], rr), g[e]);
+                        u[2 * k + e] = mul2_rn(mul2_rn(u[2 * k + e], rr), g[2 + e]);
                     }
-                    if (OP == ROT_NORM) {
-                        if (here) {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                l[e] = l[e] * r * gnl[e];
-                                h[e] = h[e] * r * gnh[e];
-                            }
-                            if (turns) rot_turn<INTER>(l, h, cs, sn);
-                        }
-                    } else {
-                        float dl[8], dh[8], dot = 0.0f;
-                        if (here) {
-                            rot_unpack(gl[u], dl);
-                            rot_unpack(gh[u], dh);
-                            if (turns) rot_turn<INTER>(dl, dh, cs, sn);
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                wl[e] += dl[e] * (l[e] * r);
-                                wh[e] += dh[e] * (h[e] * r);
-                                dl[e] *= gnl[e];
-                                dh[e] *= gnh[e];
-                                dot += dl[e] * l[e] + dh[e] * h[e];
-                            }
-                        }
-                        dot = rot_sum(dot, lanes) / (float)a.D * (r * r * r);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            l[e] = r * dl[e] - l[e] * dot;
-                            h[e] = r * dh[e] - h[e] * dot;
-                        }
-                    }
-                }
-                if (here) {
-                    rot_store(o + lo, ck_pack<T>(l));
-                    rot_store(o + hi, ck_pack<T>(h));
                 }
             }
+            if (OP != ROT_NORM_BACK && here && turns) rot_turn<INTER>(l, u, t, turning);
+            if (OP == ROT_NORM_BACK) {
+                float2 dl[4], dh[4], dot2 = make_float2(0.0f, 0.0f);
+                const float2 rr = make_float2(rinv, rinv);
+                rot_get<T>(in + 2 * Q * kRotThreads, kRotThreads, dl);
+                rot_get<T>(in + 3 * Q * kRotThreads, kRotThreads, dh);
+                if (here) {
+                    if (turns) rot_turn<INTER>(dl, dh, t, turning);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        float2 g[4];
+                        rot_four(gain + k * all + c, g[0], g[1]);
+                        rot_four(gain + (k + 2) * all + c, g[2], g[3]);
+#pragma unroll
+                        for (int e = 2 * k; e < 2 * k + 2; ++e) {
+                            wl[e] = fma2_rn(dl[e], mul2_rn(l[e], rr), wl[e]);
+                            wh[e] = fma2_rn(dh[e], mul2_rn(u[e], rr), wh[e]);
+                            dl[e] = mul2_rn(dl[e], g[e - 2 * k]);
+                            dh[e] = mul2_rn(dh[e], g[2 + e - 2 * k]);
+                            dot2 = fma2_rn(dh[e], u[e], fma2_rn(dl[e], l[e], dot2));
+                        }
+                    }
+                }
+                const float dot = -(rot_sum(dot2.x + dot2.y, lanes) / (float)a.D * (rinv * rinv * rinv));
+                const float2 nd = make_float2(dot, dot);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    l[e] = fma2_rn(l[e], nd, mul2_rn(dl[e], rr));
+                    u[e] = fma2_rn(u[e], nd, mul2_rn(dh[e], rr));
+                }
+            }
+            if (here) {
+                rot_put<T>(out + lo, l);
+                rot_put<T>(out + hi, u);
+            }
+            out += (int64_t)groups * a.D;
+            h += step_h;
+            tok += step_t + (h >= s.heads ? 1 : 0);
+            if (h >= s.heads) h -= s.heads;
         }
-    }
-    if (OP == ROT_NORM_BACK) {  // the groups' sums, one after the other
-        float* sums = reinterpret_cast<float*>(rot_sh);
-        __syncthreads();
-        if (mine)
+        rot_wait<0>();
+        if (OP == ROT_NORM_BACK && s.rows > 0) {  // the groups' sums, one after the other
+            float* sums = reinterpret_cast<float*>(rot_sh) + sums_at;
+            __syncthreads();
+            if (mine)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                sums[group * a.D + lo + e] = wl[e];
-                sums[group * a.D + hi + e] = wh[e];
+                for (int e = 0; e < 4; ++e) {
+                    *reinterpret_cast<float2*>(sums + group * a.D + lo + 2 * e) = wl[e];
+                    *reinterpret_cast<float2*>(sums + group * a.D + hi + 2 * e) = wh[e];
+                }
+            __syncthreads();
+            for (int d = threadIdx.x; d < a.D; d += kRotThreads) {
+                float t = 0.0f;
+                for (int g = 0; g < groups; ++g) t += sums[g * a.D + d];
+                s.part[(int64_t)blockIdx.x * a.D + d] = t;
             }
-        __syncthreads();
-        for (int d = threadIdx.x; d < a.D; d += kRotThreads) {
-            float t = 0.0f;
-            for (int g = 0; g < groups; ++g) t += sums[g * a.D + d];
-            s.part[(int64_t)cta * a.D + d] = t;
         }
     }
 }
@@ -306,7 +407,7 @@ __global__ void __launch_bounds__(kRotThreads) rotary_any_kernel(const __grid_co
         rot_table(a, table, t0, (h0 + count - 1) / s.heads + 1, [](int p) { return p; });
         __syncthreads();
         for (int i = warp; i < count; i += kWarps) {
-            const int tok = (h0 + i) / s.heads, h = h0 + i - tok * s.heads;
+            const int tok = rot_quotient(h0 + i, s.heads, s.magic), h = h0 + i - tok * s.heads;
             const T* x = static_cast<const T*>(s.x) + (t0 + tok) * s.ld_t + h * s.ld_h;
             const T* dy = OP == ROT_NORM_BACK ? static_cast<const T*>(s.dy) + (t0 + tok) * s.ld_dt + h * s.ld_dh : nullptr;
             T* o = static_cast<T*>(s.out) + (r0 + i) * a.D;
