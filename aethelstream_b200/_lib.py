@@ -60,12 +60,7 @@ class WeightRef(C.Structure):
 
 
 class RotaryPlan(C.Structure):
-    _fields_ = [("positions", C.c_void_p), ("position_bits", C.c_int), ("period", C.c_int64), ("freq", C.c_void_p),
-                ("rotary_dim", C.c_int), ("interleaved", C.c_int), ("amplitude", C.c_float)]
-
-
-class Heads(C.Structure):
-    _fields_ = [("data", C.c_void_p), ("ld_token", C.c_int64), ("ld_head", C.c_int64), ("heads", C.c_int)]
+    _fields_ = [("freq", C.c_void_p), ("rotary_dim", C.c_int), ("interleaved", C.c_int), ("amplitude", C.c_float)]
 
 
 class AdamwState(C.Structure):
@@ -77,7 +72,7 @@ SQ_HOOK = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p)
 
 _vp, _i, _i64, _f, _u32, _u64, _d = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_uint32, C.c_uint64, C.c_double
 _sz = C.c_size_t
-_plan, _heads = C.POINTER(RotaryPlan), C.POINTER(Heads)
+_at = [C.POINTER(RotaryPlan), _vp, _i, _i64]  # a rotation: plan and positions
 
 # name -> (restype, argtypes); every function declared in include/aeth_galore.h
 SIGNATURES = {
@@ -155,11 +150,12 @@ SIGNATURES = {
     "aeth_checkpoint_weight_grad_workspace": (_i, [_i64, _i64, _i64, C.POINTER(C.c_size_t)]),
     "aeth_checkpoint_weight_grad": (_i, [_vp, _i64, _vp, _vp, _vp, _i, _f, _i, _i64, _i64, _i64, _vp, _i64, _vp, _sz,
                                          _vp]),
-    "aeth_rotary": (_i, [_plan, _heads, _heads, _i64, _i, _i, _i, _vp, _vp, _vp]),
-    "aeth_qk_norm_rotary": (_i, [_plan, _heads, _heads, _vp, _vp, _i, _f, _i64, _i, _i, _vp, _vp, _vp]),
+    "aeth_rotary": (_i, [*_at, _vp, _i64, _i64, _i, _vp, _i64, _i64, _i, _i64, _i, _i, _i, _vp, _vp, _vp]),
+    "aeth_qk_norm_rotary": (_i, [*_at, _vp, _i64, _i64, _i, _vp, _i64, _i64, _i, _vp, _vp, _i, _f, _i64, _i, _i, _vp, _vp,
+                                 _vp]),
     "aeth_qk_norm_rotary_backward_workspace": (_i, [_i, C.POINTER(C.c_size_t)]),
-    "aeth_qk_norm_rotary_backward": (_i, [_plan, _heads, _heads, _heads, _heads, _vp, _vp, _i, _f, _i64, _i, _i, _vp, _vp,
-                                          _vp, _vp, _vp, _sz, _vp]),
+    "aeth_qk_norm_rotary_backward": (_i, [*_at, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i, _vp, _i64, _i64, _i,
+                                          _vp, _vp, _i, _f, _i64, _i, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "aeth_adamw_step": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, C.POINTER(AdamwState), _d, _d, _f, _f, _vp, _f, _vp, _vp]),
     "aeth_adamw_moments": (_i, [C.POINTER(AdamwState), _vp, _vp, _vp]),
     "aeth_status_string": (C.c_char_p, [_i]),

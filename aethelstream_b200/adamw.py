@@ -2,7 +2,7 @@
 out (norm gains, biases, embeddings, the head).
 
 ``AdamWState`` holds the moments of a list of tensors, in 32 or in 8 bits, and
-the step's count; ``adamw_step`` updates all of them in one launch (896 tensors
+the step's count; ``adamw_step`` updates all of them in one launch (768 tensors
 a launch), on the current stream of their device, without synchronising.  Count,
 clip and, where wanted, learning rate lie on the device, so a captured step may be
 replayed.  Wrong shapes, types and devices raise ValueError; statuses of the C ABI
@@ -12,6 +12,7 @@ from __future__ import annotations
 
 from array import array
 from dataclasses import dataclass
+from operator import attrgetter
 
 import torch
 
@@ -22,6 +23,21 @@ from .training import _current_device, _elsewhere, _raw_stream
 ADAMW_BLOCK = 2048  # elements that share a scale; a tensor's moments start on a whole block
 
 _lib = L.load()
+
+
+_numel, _data_ptr, _contiguous = torch.Tensor.numel, torch.Tensor.data_ptr, torch.Tensor.is_contiguous
+_inference, _get_device, _shape, _dtype = torch.Tensor.is_inference, torch.Tensor.get_device, attrgetter("shape"), attrgetter("dtype")
+
+
+def _kinds(what: str, tensors, dev: int) -> bytes:
+    """The types of float tensors on `dev`."""
+    try:
+        kinds = bytes(map(_DTYPES.__getitem__, map(_dtype, tensors)))
+    except KeyError:
+        raise ValueError(f"{what}: float32, float16 or bfloat16 tensors expected") from None
+    if not {dev}.issuperset(map(_get_device, tensors)):
+        raise ValueError(f"{what}: all tensors must be on cuda:{dev}")
+    return kinds
 
 
 def _blocks(n: int) -> int:
@@ -107,38 +123,40 @@ def adamw_step(params, grads, state: AdamWState, config: AdamWConfig | None = No
         raise ValueError(f"{what}: a gradient (or None) and, where given, a decay for each of {count} tensors expected")
     if config.scale_lr_by_rank:
         raise ValueError(f"{what}: scale_lr_by_rank is for low-rank parameters")
-    blocks = 0
-    sizes, kinds, gkinds = array("q"), bytearray(count), bytearray(count)
-    for i, p in enumerate(params):
-        kind, n = _DTYPES.get(p.dtype), p.numel()
-        if kind is None or not p.is_contiguous() or p.get_device() != dev:
-            raise ValueError(f"{what}: tensor {i} must be a contiguous float tensor on cuda:{dev}")
-        g = grads[i]
-        if g is not None:
-            gkind = _DTYPES.get(g.dtype)
-            if gkind is None or g.shape != p.shape or g.get_device() != dev:
-                raise ValueError(f"{what}: gradient {i} must be a float tensor of shape {tuple(p.shape)} on cuda:{dev}")
-            if not g.is_contiguous():
-                grads[i] = g.contiguous()
-            gkinds[i] = gkind
-        kinds[i] = kind
-        sizes.append(n)
-        blocks += -(-n // ADAMW_BLOCK)
+    # by whole lists: a step of hundreds of tensors spends its host time here
+    kinds = _kinds(what, params, dev)
+    here, there = params, [g for g in grads if g is not None]
+    some = len(there) != count
+    if some:
+        here = [p for p, g in zip(params, grads) if g is not None]
+    gkinds = _kinds(what, there, dev)
+    if not all(map(_contiguous, params)):
+        raise ValueError(f"{what}: the tensors must be contiguous")
+    if list(map(_shape, here)) != list(map(_shape, there)):
+        raise ValueError(f"{what}: a gradient must have its tensor's shape")
+    if not all(map(_contiguous, there)):
+        there = [g.contiguous() for g in there]
+    g_ptr = array("Q", map(_data_ptr, there))
+    if some:
+        left = iter(zip(g_ptr, gkinds))
+        each = [(0, 0) if g is None else next(left) for g in grads]
+        g_ptr, gkinds = array("Q", [x for x, _ in each]), bytes(k for _, k in each)
+    p_ptr, sizes = array("Q", map(_data_ptr, params)), array("q", map(_numel, params))
+    blocks = sum([-(-n // ADAMW_BLOCK) for n in sizes])
     c = _state(what, state, dev)
     if blocks != c.blocks:
         raise ValueError(f"{what}: the state is for {c.blocks} blocks of {ADAMW_BLOCK} elements, the tensors have {blocks}")
     clip_ptr, lr_ptr = _scalar(what, "clip", clip, dev), _scalar(what, "lr", lr, dev)
-    p_ptr = array("Q", [p.data_ptr() for p in params])
-    g_ptr = array("Q", [0 if g is None else g.data_ptr() for g in grads])
     st = _lib.aeth_adamw_step(
-        p_ptr.buffer_info()[0], g_ptr.buffer_info()[0], sizes.buffer_info()[0], bytes(kinds), bytes(gkinds),
+        p_ptr.buffer_info()[0], g_ptr.buffer_info()[0], sizes.buffer_info()[0], kinds, gkinds,
         None if decay is None else bytes(map(bool, decay)), count, c, config.beta1, config.beta2, config.eps, config.lr,
         lr_ptr, config.weight_decay, clip_ptr, _raw_stream(dev))
     if st == L.AETH_ERR_ARG:
         raise ValueError(f"{what}: tensors that the step writes share memory")
     if st:
         L.check(st, "aeth_adamw_step")
-    torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])
+    torch.autograd.graph.increment_version(params if not any(map(_inference, params)) else
+                                           [p for p in params if not p.is_inference()])
 
 
 def adamw_moments(state: AdamWState) -> tuple[torch.Tensor, torch.Tensor]:

@@ -20,6 +20,8 @@
 // lie elsewhere in every step and a captured step needs no memory of its own.
 // Bound by its bytes: parameters, gradients and moments pass through once.
 #pragma once
+#include <type_traits>
+
 #include "adam.cuh"
 #include "codec.cuh"
 #include "pack8.cuh"
@@ -27,9 +29,11 @@
 namespace aeth {
 
 constexpr int kAdamwBlock = 2048;
-// Tensors of one launch: the parameters of a launch take 32764 bytes.  A short
-// list has a table of its own, which costs less to hand over.
-constexpr int kAdamwTensors = 896, kAdamwFew = 64;
+// Tensors of one launch, whose parameters take 32764 bytes at most.  Handing a table
+// over costs the host 0.5 us a kilobyte (a launch of 161 gains 22.7 us with 29 KB, 7 with 2),
+// so short lists have shorter ones.
+constexpr int kAdamwTensors = 768, kAdamwSome = 256, kAdamwFew = 64;
+constexpr int kAdamwStarts = 888;  // walkers over the blocks (CTAs, or groups of them), at most
 constexpr int64_t kAdamwStepBits = 40;  // of the step's word that count steps; above them, CTAs that have finished
 
 struct AdamwTensor {
@@ -45,6 +49,7 @@ template <int CAP>
 struct AdamwArgs {
     AdamwTensor t[CAP];
     int at[CAP];  // first of its blocks among all moments
+    uint16_t start[kAdamwStarts];  // the tensor of each walker's first block
     int count, blocks;
     void *m, *v;
     float *m_scales, *v_scales;
@@ -59,68 +64,80 @@ struct AdamwArgs {
 };
 static_assert(sizeof(AdamwArgs<kAdamwTensors>) <= 32764, "a launch's parameters");
 
-// Eight elements of any type.  The first `have` exist; whole: 16-byte aligned.
-__device__ __forceinline__ void adamw_load8(const void* p, int dtype, bool whole, int64_t i, int have, float (&v)[8]) {
+// N elements (4 or 8) of any type, the first `have` of which exist; whole: they
+// start on as many bytes as they take, 16 at most.
+template <int N>
+__device__ __forceinline__ void adamw_load(const void* p, int dtype, bool whole, int64_t i, int have, float (&v)[N]) {
     if (dtype == AETH_DTYPE_F32) {
         const float* q = static_cast<const float*>(p) + i;
-        if (whole && have >= 8) {
-            const float4 a = *reinterpret_cast<const float4*>(q), b = *reinterpret_cast<const float4*>(q + 4);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        if (whole && have >= N) {
+#pragma unroll
+            for (int k = 0; k < N; k += 4) {
+                const float4 a = *reinterpret_cast<const float4*>(q + k);
+                v[k] = a.x; v[k + 1] = a.y; v[k + 2] = a.z; v[k + 3] = a.w;
+            }
         } else {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = k < have ? q[k] : 0.0f;
+            for (int k = 0; k < N; ++k) v[k] = k < have ? q[k] : 0.0f;
         }
         return;
     }
     const uint16_t* q = static_cast<const uint16_t*>(p) + i;
-    Pack8<__half> h;
-    if (whole && have >= 8) {
-        h.w[0] = *reinterpret_cast<const uint4*>(q);
+    uint32_t w[N / 2];
+    if (whole && have >= N) {
+        if constexpr (N == 8) {
+            const uint4 x = *reinterpret_cast<const uint4*>(q);
+            w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+        } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(q);
+            w[0] = x.x; w[1] = x.y;
+        }
     } else {
-        uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (k < have) w[k >> 1] |= (uint32_t)q[k] << (16 * (k & 1));
-        h.w[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int k = 0; k < N; k += 2)
+            w[k / 2] = (k < have ? (uint32_t)q[k] : 0u) | (k + 1 < have ? (uint32_t)q[k + 1] << 16 : 0u);
     }
-    if (dtype == AETH_DTYPE_F16) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = ck_value<__half>(h, k);
-    } else {
-        const Pack8<__nv_bfloat16> b{{h.w[0]}};
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = ck_value<__nv_bfloat16>(b, k);
+    for (int k = 0; k < N; k += 2) {
+        const float2 x = dtype == AETH_DTYPE_F16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[k / 2]))
+                                                 : make_float2(__uint_as_float(w[k / 2] << 16), __uint_as_float(w[k / 2] & 0xffff0000u));
+        v[k] = x.x;
+        v[k + 1] = x.y;
     }
 }
-__device__ __forceinline__ void adamw_store8(void* p, int dtype, bool whole, int64_t i, int have, const float (&v)[8]) {
+template <int N>
+__device__ __forceinline__ void adamw_store(void* p, int dtype, bool whole, int64_t i, int have, const float (&v)[N]) {
     if (dtype == AETH_DTYPE_F32) {
         float* q = static_cast<float*>(p) + i;
-        if (whole && have >= 8) {
-            *reinterpret_cast<float4*>(q) = make_float4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<float4*>(q + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        if (whole && have >= N) {
+#pragma unroll
+            for (int k = 0; k < N; k += 4) *reinterpret_cast<float4*>(q + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
         } else {
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
+            for (int k = 0; k < N; ++k)
                 if (k < have) q[k] = v[k];
         }
         return;
     }
-    const uint4 w = dtype == AETH_DTYPE_F16 ? ck_pack<__half>(v).w[0] : ck_pack<__nv_bfloat16>(v).w[0];
-    uint16_t* q = static_cast<uint16_t*>(p) + i;
-    if (whole && have >= 8) {
-        *reinterpret_cast<uint4*>(q) = w;
-    } else {
-        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+    uint32_t w[N / 2];
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (k < have) q[k] = (uint16_t)(x[k >> 1] >> (16 * (k & 1)));
+    for (int k = 0; k < N; k += 2)
+        w[k / 2] = dtype == AETH_DTYPE_F16 ? ck_pack2<__half>(v[k], v[k + 1]) : ck_pack2<__nv_bfloat16>(v[k], v[k + 1]);
+    uint16_t* q = static_cast<uint16_t*>(p) + i;
+    if (whole && have >= N) {
+        if constexpr (N == 8) *reinterpret_cast<uint4*>(q) = make_uint4(w[0], w[1], w[2], w[3]);
+        else *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (k < have) q[k] = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
     }
 }
 
 // What a step's elements share.
 struct AdamwScalars {
     float clip, lr, b1, b2, omb1, omb2, first, second, eps, decay;
+    bool flush;  // eps is so large that a root below 2^-63 does not count beside it (2^-20 of it)
 };
 // 1 / (1 - b^t), b^t by squaring
 __device__ __forceinline__ float adamw_correction(double b, int64_t t) {
@@ -145,6 +162,7 @@ __device__ __forceinline__ AdamwScalars adamw_scalars(const AdamwArgs<CAP>& a, f
     s.omb2 = (float)(1.0 - a.beta2);
     s.eps = a.eps;
     s.decay = a.decay;
+    s.flush = a.eps >= 1e-12f;
     __syncthreads();
     s.first = shared2[0];
     s.second = shared2[1];
@@ -160,10 +178,12 @@ __device__ __forceinline__ void adamw_count(const AdamwArgs<CAP>& a) {
     if ((was >> kAdamwStepBits) == gridDim.x - 1)
         *(volatile int64_t*)a.step = (int64_t)(was & ((1ull << kAdamwStepBits) - 1)) + 1;
 }
-// The tensor of a block of the launch: the last that starts at or before it.
+// The tensor of a block of the launch: the last that starts at or before it.  `i`:
+// that of an earlier block, and often of this one too.
 template <int CAP>
-__device__ __forceinline__ int adamw_tensor(const AdamwArgs<CAP>& a, int block) {
-    int lo = 0, hi = a.count - 1;
+__device__ __forceinline__ int adamw_tensor(const AdamwArgs<CAP>& a, int block, int i) {
+    if (i + 1 >= a.count || a.t[i + 1].first > block) return i;
+    int lo = i + 1, hi = a.count - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (a.t[mid].first <= block) lo = mid;
@@ -172,54 +192,87 @@ __device__ __forceinline__ int adamw_tensor(const AdamwArgs<CAP>& a, int block) 
     return lo;
 }
 
-__device__ __forceinline__ float adamw_sqrt(float x) {
+// 1 / (sqrt(x) + eps), subnormal numbers flushed to 0 or not
+template <bool FLUSH>
+__device__ __forceinline__ float adamw_scale(float x, float eps) {
     float r;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    if (FLUSH) {
+        asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+        r += eps;
+        asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(r));
+    } else {
+        asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+        r += eps;
+        asm("rcp.approx.f32 %0, %0;" : "+f"(r));
+    }
     return r;
 }
-__device__ __forceinline__ float adamw_rcp(float x) {
-    float r;
-    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-__device__ __forceinline__ void adamw_moments(const AdamwScalars& s, float g, float& m, float& v) {
-    g = __fmul_rn(g, s.clip);
-    m = __fadd_rn(__fmul_rn(s.b1, m), __fmul_rn(s.omb1, g));
-    v = __fadd_rn(__fmul_rn(s.b2, v), __fmul_rn(__fmul_rn(s.omb2, g), g));
-}
-__device__ __forceinline__ float adamw_param(const AdamwScalars& s, float decay, float p, float m, float v) {
-    const float u = m * s.first * adamw_rcp(adamw_sqrt(v * s.second) + s.eps);
-    return p - s.lr * (u + decay * p);
+// New moments from the old ones, and the parameters, of N elements in pairs: the
+// products of two in one instruction, the sums one by one (common.cuh, add2_sep).
+template <int N>
+__device__ __forceinline__ void adamw_update(const AdamwScalars& s, float decay, const float (&g)[N], float (&p)[N], float (&m)[N],
+                                             float (&v)[N]) {
+    const float2 clip = make_float2(s.clip, s.clip), b1 = make_float2(s.b1, s.b1), b2 = make_float2(s.b2, s.b2);
+    const float2 omb1 = make_float2(s.omb1, s.omb1), omb2 = make_float2(s.omb2, s.omb2);
+    const float2 first = make_float2(s.first, s.first), second = make_float2(s.second, s.second);
+#pragma unroll
+    for (int k = 0; k < N; k += 2) {
+        const float2 gg = mul2_rn(make_float2(g[k], g[k + 1]), clip);
+        const float2 mm = add2_sep(mul2_rn(b1, make_float2(m[k], m[k + 1])), mul2_rn(omb1, gg));
+        const float2 vv = add2_sep(mul2_rn(b2, make_float2(v[k], v[k + 1])), mul2_rn(mul2_rn(omb2, gg), gg));
+        m[k] = mm.x;
+        m[k + 1] = mm.y;
+        v[k] = vv.x;
+        v[k + 1] = vv.y;
+    }
+    auto params = [&](auto flush) {
+#pragma unroll
+        for (int k = 0; k < N; k += 2) {
+            const float2 mm = mul2_rn(make_float2(m[k], m[k + 1]), first), vv = mul2_rn(make_float2(v[k], v[k + 1]), second);
+            p[k] -= s.lr * fmaf(mm.x, adamw_scale<flush.value>(vv.x, s.eps), decay * p[k]);
+            p[k + 1] -= s.lr * fmaf(mm.y, adamw_scale<flush.value>(vv.y, s.eps), decay * p[k + 1]);
+        }
+    };
+    if (s.flush) params(std::true_type());
+    else params(std::false_type());
 }
 
-// Moments in 32 bits: a CTA takes blocks, a thread eight elements of one.
-template <int CAP, bool MASTER>
+// Moments in 32 bits: a CTA takes blocks, a thread four elements of each half of
+// one, so that a warp's accesses of any type are whole.
+template <int CAP>
 __global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ AdamwArgs<CAP> a) {
     __shared__ float corr[2];
     const AdamwScalars s = adamw_scalars(a, corr);
+    int i = a.start[blockIdx.x];
     for (int b = blockIdx.x; b < a.blocks; b += gridDim.x) {
-        const int i = adamw_tensor(a, b);
+        if (b != (int)blockIdx.x) i = adamw_tensor(a, b, i);
         const AdamwTensor& t = a.t[i];
-        const int64_t e = (int64_t)(b - t.first) * kAdamwBlock + threadIdx.x * 8;
-        const int64_t o = ((int64_t)a.at[i] + (b - t.first)) * kAdamwBlock + threadIdx.x * 8;
-        const int have = (int)min(t.n - e, (int64_t)8);
-        if (have <= 0) continue;
-        float p[8], g[8], m[8], v[8];
-        adamw_load8(t.g, t.g_dtype, t.whole, e, have, g);
-        if (MASTER) adamw_load8(a.master, AETH_DTYPE_F32, true, o, 8, p);
-        else adamw_load8(t.p, t.p_dtype, t.whole, e, have, p);
-        adamw_load8(a.m, AETH_DTYPE_F32, true, o, 8, m);
-        adamw_load8(a.v, AETH_DTYPE_F32, true, o, 8, v);
+        const int64_t e0 = (int64_t)(b - t.first) * kAdamwBlock + threadIdx.x * 4;
+        const int64_t o0 = ((int64_t)a.at[i] + (b - t.first)) * kAdamwBlock + threadIdx.x * 4;
+        float p[2][4], g[2][4], m[2][4], v[2][4];
+        int have[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const int64_t e = e0 + q * (kAdamwBlock / 2), o = o0 + q * (kAdamwBlock / 2);
+            have[q] = (int)min(t.n - e, (int64_t)4);
+            if (have[q] <= 0) continue;
+            adamw_load<4>(a.m, AETH_DTYPE_F32, true, o, 4, m[q]);
+            adamw_load<4>(a.v, AETH_DTYPE_F32, true, o, 4, v[q]);
+            if (a.master) adamw_load<4>(a.master, AETH_DTYPE_F32, true, o, 4, p[q]);
+            else adamw_load<4>(t.p, t.p_dtype, t.whole, e, have[q], p[q]);
+            adamw_load<4>(t.g, t.g_dtype, t.whole, e, have[q], g[q]);
+        }
         const float decay = t.decay ? s.decay : 0.0f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            adamw_moments(s, g[k], m[k], v[k]);
-            p[k] = adamw_param(s, decay, p[k], m[k], v[k]);
+        for (int q = 0; q < 2; ++q) {
+            const int64_t e = e0 + q * (kAdamwBlock / 2), o = o0 + q * (kAdamwBlock / 2);
+            if (have[q] <= 0) continue;
+            adamw_update<4>(s, decay, g[q], p[q], m[q], v[q]);
+            if (a.master) adamw_store<4>(a.master, AETH_DTYPE_F32, true, o, have[q], p[q]);
+            adamw_store<4>(t.p, t.p_dtype, t.whole, e, have[q], p[q]);
+            adamw_store<4>(a.m, AETH_DTYPE_F32, true, o, have[q], m[q]);
+            adamw_store<4>(a.v, AETH_DTYPE_F32, true, o, have[q], v[q]);
         }
-        if (MASTER) adamw_store8(a.master, AETH_DTYPE_F32, true, o, have, p);
-        adamw_store8(t.p, t.p_dtype, t.whole, e, have, p);
-        adamw_store8(a.m, AETH_DTYPE_F32, true, o, have, m);
-        adamw_store8(a.v, AETH_DTYPE_F32, true, o, have, v);
     }
     adamw_count(a);
 }
@@ -232,7 +285,7 @@ constexpr int kAdamw8Threads = 1024;
 constexpr int kAdamw8Dec = 256 * 256;
 constexpr int kAdamw8Shared = kAdamw8Dec + (2 * kDmapLutEntries + kDmapLutUEntries) * 4;
 
-template <int CAP, bool MASTER>
+template <int CAP>
 __global__ void __launch_bounds__(kAdamw8Threads, 1) adamw8_kernel(const __grid_constant__ AdamwArgs<CAP> a) {
     extern __shared__ __align__(16) uint8_t adamw_smem[];
     float* dec = reinterpret_cast<float*>(adamw_smem);
@@ -251,9 +304,10 @@ __global__ void __launch_bounds__(kAdamw8Threads, 1) adamw8_kernel(const __grid_
     const uint32_t adj_s = smem_u32_addr(lut_s) - (uint32_t)(kDmapLutExpLo << kDmapLutLog2P) * 4u;
     const uint32_t adj_u = smem_u32_addr(lut_u) - (uint32_t)(kDmapLutExpLo << kDmapLutULog2P) * 4u;
     int8_t *m_all = static_cast<int8_t*>(a.m), *v_all = static_cast<int8_t*>(a.v);
-    int par = 0;
-    for (int b = blockIdx.x * 4 + grp; b < a.blocks; b += gridDim.x * 4, par ^= 1) {
-        const int i = adamw_tensor(a, b);
+    const int walker = blockIdx.x * 4 + grp;
+    int par = 0, i = a.start[walker];
+    for (int b = walker; b < a.blocks; b += gridDim.x * 4, par ^= 1) {
+        if (b != walker) i = adamw_tensor(a, b, i);
         const AdamwTensor& t = a.t[i];
         const int64_t blk = (int64_t)a.at[i] + (b - t.first);
         const int64_t e = (int64_t)(b - t.first) * kAdamwBlock + tid * 8, o = blk * kAdamwBlock + tid * 8;
@@ -261,23 +315,34 @@ __global__ void __launch_bounds__(kAdamw8Threads, 1) adamw8_kernel(const __grid_
         const float sm = a.m_scales[blk], sv = a.v_scales[blk];
         const uint2 qm = *reinterpret_cast<const uint2*>(m_all + o), qv = *reinterpret_cast<const uint2*>(v_all + o);
         float p[8], g[8], m[8], v[8], am = 0.0f, av = 0.0f;
-        adamw_load8(t.g, t.g_dtype, t.whole, e, have, g);
-        if (MASTER) adamw_load8(a.master, AETH_DTYPE_F32, true, o, 8, p);
-        else adamw_load8(t.p, t.p_dtype, t.whole, e, have, p);
-        const float decay = t.decay ? s.decay : 0.0f;
+        adamw_load<8>(t.g, t.g_dtype, t.whole, e, have, g);
+        if (a.master) adamw_load<8>(a.master, AETH_DTYPE_F32, true, o, 8, p);
+        else adamw_load<8>(t.p, t.p_dtype, t.whole, e, have, p);
+        const float2 sm2 = make_float2(sm, sm), sv2 = make_float2(sv, sv);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const uint32_t sel = 0x5504u | ((uint32_t)(k & 3) << 4);
-            m[k] = __fmul_rn(__uint_as_float(lds_u32(dec_base + prmt(k < 4 ? qm.x : qm.y, off_m, sel))), sm);
-            v[k] = __fmul_rn(__uint_as_float(lds_u32(dec_base + prmt(k < 4 ? qv.x : qv.y, off_v, sel))), sv);
-            adamw_moments(s, g[k], m[k], v[k]);
-            p[k] = adamw_param(s, decay, p[k], m[k], v[k]);
-            if (k >= have) m[k] = v[k] = 0.0f;  // past the tensor's end: codes of zero
-            am = fmax3_nan(am, fabsf(m[k]), 0.0f);
-            av = fmax3_nan(av, v[k], 0.0f);
+        for (int k = 0; k < 8; k += 2) {
+            const uint32_t sel = 0x5504u | ((uint32_t)(k & 3) << 4), wm = k < 4 ? qm.x : qm.y, wv = k < 4 ? qv.x : qv.y;
+            const float2 mm = mul2_rn(make_float2(__uint_as_float(lds_u32(dec_base + prmt(wm, off_m, sel))),
+                                                  __uint_as_float(lds_u32(dec_base + prmt(wm, off_m, sel + 0x10u)))), sm2);
+            const float2 vv = mul2_rn(make_float2(__uint_as_float(lds_u32(dec_base + prmt(wv, off_v, sel))),
+                                                  __uint_as_float(lds_u32(dec_base + prmt(wv, off_v, sel + 0x10u)))), sv2);
+            m[k] = mm.x;
+            m[k + 1] = mm.y;
+            v[k] = vv.x;
+            v[k + 1] = vv.y;
         }
-        if (MASTER) adamw_store8(a.master, AETH_DTYPE_F32, true, o, have, p);
-        adamw_store8(t.p, t.p_dtype, t.whole, e, have, p);
+        adamw_update<8>(s, t.decay ? s.decay : 0.0f, g, p, m, v);
+        if (a.master) adamw_store<8>(a.master, AETH_DTYPE_F32, true, o, have, p);
+        adamw_store<8>(t.p, t.p_dtype, t.whole, e, have, p);
+        if (have < 8)  // past the tensor's end: codes of zero
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (k >= have) m[k] = v[k] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; k += 2) {
+            am = fmax3_nan(am, fabsf(m[k]), fabsf(m[k + 1]));
+            av = fmax3_nan(av, v[k], v[k + 1]);
+        }
         // non-negative or NaN (0x7fffffff): their bits order as they do
         const uint32_t wm = __reduce_max_sync(0xffffffffu, __float_as_uint(am));
         const uint32_t wv = __reduce_max_sync(0xffffffffu, __float_as_uint(av));
@@ -292,11 +357,16 @@ __global__ void __launch_bounds__(kAdamw8Threads, 1) adamw8_kernel(const __grid_
         const float nm = bad_m || bm < 0x00800000u ? 0.0f : __uint_as_float(bm);
         const float nv = bad_v || bv < 0x00800000u ? 0.0f : __uint_as_float(bv);
         const float im = dyn_inv(nm), iv = dyn_inv(nv);
+        // im = 0: codes of zero (of NaN too: the scale says NaN)
         uint32_t cm[8], cv[8];
+        const float2 im2 = make_float2(im, im), iv2 = make_float2(iv, iv);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            cm[k] = dmap_enc4_s(adj_s, nm > 0.0f ? dyn_xn(m[k], im) : 0.0f, m1, m8, m15);
-            cv[k] = dmap_enc4_u(adj_u, nv > 0.0f ? dyn_xn(v[k], iv) : 0.0f, m8, m16);
+        for (int k = 0; k < 8; k += 2) {
+            const float2 mm = mul2_rn(make_float2(m[k], m[k + 1]), im2), vv = mul2_rn(make_float2(v[k], v[k + 1]), iv2);
+            cm[k] = dmap_enc4_s(adj_s, mm.x, m1, m8, m15);
+            cm[k + 1] = dmap_enc4_s(adj_s, mm.y, m1, m8, m15);
+            cv[k] = dmap_enc4_u(adj_u, vv.x, m8, m16);
+            cv[k + 1] = dmap_enc4_u(adj_u, vv.y, m8, m16);
         }
         uint2 om, ov;
         om.x = prmt(prmt(cm[0], cm[1], 0x3340u), prmt(cm[2], cm[3], 0x3340u), 0x5410u);
@@ -313,27 +383,36 @@ __global__ void __launch_bounds__(kAdamw8Threads, 1) adamw8_kernel(const __grid_
     adamw_count(a);
 }
 
-// 8-bit moments as the values that they stand for: a thread takes 16 codes.
+// 8-bit moments as the values that they stand for, m's and v's by CTAs of their
+// own: a thread takes four codes and sixteen bytes of values, eight times.  Each
+// map entry in eight copies (32 would leave no conflict, and cost the CTAs' start).
+constexpr int kAdamwDecode = 8;
 __global__ void __launch_bounds__(256) adamw_decode_kernel(const int8_t* __restrict__ m, const int8_t* __restrict__ v,
                                                            const float* __restrict__ ms, const float* __restrict__ vs,
-                                                           int64_t n16, float* __restrict__ m_out, float* __restrict__ v_out) {
-    __shared__ float dec[2][256];
-    for (int i = threadIdx.x; i < 256; i += 256) {
-        dec[0][i] = c_dmap_signed[i];
-        dec[1][i] = c_dmap_unsigned[i];
-    }
+                                                           int64_t n4, float* __restrict__ m_out, float* __restrict__ v_out) {
+    __shared__ float dec[256 * 8];
+    const bool second = blockIdx.y != 0;
+    for (int i = threadIdx.x; i < 256 * 8; i += 256) dec[i] = second ? c_dmap_unsigned[i >> 3] : c_dmap_signed[i >> 3];
     __syncthreads();
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n16; i += gridDim.x * 256ll) {
+    const uint32_t* codes = reinterpret_cast<const uint32_t*>(second ? v : m);
+    const float* scales = second ? vs : ms;
+    float4* out = reinterpret_cast<float4*>(second ? v_out : m_out);
+    const float* mine = dec + (threadIdx.x & 7);
+    for (int64_t i0 = blockIdx.x * 256ll * kAdamwDecode + threadIdx.x; i0 < n4; i0 += gridDim.x * 256ll * kAdamwDecode) {
+        uint32_t c[kAdamwDecode];
+        float s[kAdamwDecode];
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-            const uint4 q = ck_stream(reinterpret_cast<const uint4*>(w ? v : m) + i);
-            const float s = (w ? vs : ms)[i / (kAdamwBlock / 16)];
-            const uint32_t c[4] = {q.x, q.y, q.z, q.w};
-            float4* o = reinterpret_cast<float4*>(w ? v_out : m_out) + i * 4;
+        for (int k = 0; k < kAdamwDecode; ++k) {  // n4 is a multiple of 512
+            const int64_t i = i0 + 256 * k;
+            c[k] = i < n4 ? __ldcs(codes + i) : 0u;
+            s[k] = i < n4 ? __ldg(scales + i / (kAdamwBlock / 4)) : 0.0f;
+        }
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                o[k] = make_float4(__fmul_rn(dec[w][c[k] & 255u], s), __fmul_rn(dec[w][c[k] >> 8 & 255u], s),
-                                   __fmul_rn(dec[w][c[k] >> 16 & 255u], s), __fmul_rn(dec[w][c[k] >> 24], s));
+        for (int k = 0; k < kAdamwDecode; ++k) {
+            const int64_t i = i0 + 256 * k;
+            if (i < n4)
+                out[i] = make_float4(__fmul_rn(mine[(c[k] & 255u) * 8], s[k]), __fmul_rn(mine[(c[k] >> 8 & 255u) * 8], s[k]),
+                                     __fmul_rn(mine[(c[k] >> 16 & 255u) * 8], s[k]), __fmul_rn(mine[(c[k] >> 24) * 8], s[k]));
         }
     }
 }

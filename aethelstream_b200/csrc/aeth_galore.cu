@@ -2431,15 +2431,21 @@ int aeth_lomo_update(const void* grad_bf16, int64_t n, const double* sq_dev, flo
 
 namespace {
 
-template <int CAP, bool MASTER>
-int adamw_launch(const AdamwArgs<CAP>& a, int bits, cudaStream_t st) {
+template <int CAP>
+int adamw_launch(AdamwArgs<CAP>& a, int bits, cudaStream_t st) {
+    const int ctas = std::max(bits == 8 ? std::min((a.blocks + 3) / 4, std::min(num_sms(), kAdamwStarts / 4))
+                                        : std::min(a.blocks, std::min(6 * num_sms(), kAdamwStarts)), 1);
+    for (int w = 0, i = 0; w < ctas * (bits == 8 ? 4 : 1); ++w) {
+        while (i + 1 < a.count && a.t[i + 1].first <= w) ++i;
+        a.start[w] = (uint16_t)i;
+    }
     if (bits == 8) {
-        auto kern = adamw8_kernel<CAP, MASTER>;
+        auto kern = adamw8_kernel<CAP>;
         static std::atomic<bool> allowed[kMaxDevices] = {};
         AETH_TRY(allow_shared(kern, kAdamw8Shared, allowed));
-        kern<<<std::max(std::min((a.blocks + 3) / 4, num_sms()), 1), kAdamw8Threads, kAdamw8Shared, st>>>(a);
+        kern<<<ctas, kAdamw8Threads, kAdamw8Shared, st>>>(a);
     } else {
-        adamw_kernel<CAP, MASTER><<<std::max(std::min(a.blocks, 6 * num_sms()), 1), 256, 0, st>>>(a);
+        adamw_kernel<CAP><<<ctas, 256, 0, st>>>(a);
     }
     AETH_LAUNCH_CHECK();
     return AETH_OK;
@@ -2478,7 +2484,7 @@ int adamw_some(const AdamwList& l, int& i, int64_t& block, AdamwArgs<CAP>& a, in
     }
     a.blocks = (int)blocks;
     a.last = i == l.count;
-    return a.master ? adamw_launch<CAP, true>(a, bits, st) : adamw_launch<CAP, false>(a, bits, st);
+    return adamw_launch(a, bits, st);
 }
 template <int CAP>
 int adamw_all(const AdamwList& l, const AethAdamwState& s, double b1, double b2, float eps, float lr, const float* lr_dev,
@@ -2554,8 +2560,8 @@ int aeth_adamw_step(void* const* p, const void* const* g, const int64_t* n, cons
     }
     if (state->bits == 8) AETH_TRY(codec_maps_ensure());
     cudaStream_t st = to_stream(stream);
-    return count <= kAdamwFew ? adamw_all<kAdamwFew>(l, *state, beta1, beta2, eps, lr, lr_dev, weight_decay, clip_dev, st)
-                              : adamw_all<kAdamwTensors>(l, *state, beta1, beta2, eps, lr, lr_dev, weight_decay, clip_dev, st);
+    auto run = count <= kAdamwFew ? adamw_all<kAdamwFew> : count <= kAdamwSome ? adamw_all<kAdamwSome> : adamw_all<kAdamwTensors>;
+    return run(l, *state, beta1, beta2, eps, lr, lr_dev, weight_decay, clip_dev, st);
 }
 
 int aeth_adamw_moments(const AethAdamwState* state, float* m_out, float* v_out, aeth_stream_t stream) {
@@ -2564,9 +2570,9 @@ int aeth_adamw_moments(const AethAdamwState* state, float* m_out, float* v_out, 
     if ((reinterpret_cast<uintptr_t>(m_out) | reinterpret_cast<uintptr_t>(v_out)) & 15) return set_err(AETH_ERR_UNSUPPORTED);
     if (state->blocks == 0) return AETH_OK;
     AETH_TRY(codec_maps_ensure());
-    const int64_t n16 = state->blocks * (kAdamwBlock / 16);
-    adamw_decode_kernel<<<(unsigned)std::min<int64_t>((n16 + 255) / 256, 8 * num_sms()), 256, 0, to_stream(stream)>>>(
-        static_cast<const int8_t*>(state->m), static_cast<const int8_t*>(state->v), state->m_scales, state->v_scales, n16,
+    const int64_t n4 = state->blocks * (kAdamwBlock / 4), per = 256 * kAdamwDecode;
+    adamw_decode_kernel<<<dim3((unsigned)std::min<int64_t>((n4 + per - 1) / per, 4 * num_sms()), 2), 256, 0, to_stream(stream)>>>(
+        static_cast<const int8_t*>(state->m), static_cast<const int8_t*>(state->v), state->m_scales, state->v_scales, n4,
         m_out, v_out);
     AETH_LAUNCH_CHECK();
     return AETH_OK;

@@ -16,25 +16,48 @@ bool rot_dtype(int dtype) { return dtype == AETH_DTYPE_F32 || dtype == AETH_DTYP
 int rot_size(int dtype) { return dtype == AETH_DTYPE_F32 ? 4 : 2; }
 int64_t rot_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
-int rot_check(const AethRotaryPlan* p, int64_t tokens, int head_dim, int hq, int hk, int dtype) {
-    if (!p || tokens < 0 || head_dim <= 0 || hq < 0 || hk < 0 || hq + hk == 0 || !rot_dtype(dtype)) return AETH_ERR_ARG;
-    if (p->rotary_dim < 2 || p->rotary_dim % 2 || p->rotary_dim > head_dim) return AETH_ERR_ARG;
-    if (!p->freq || p->position_bits != 32 && p->position_bits != 64) return AETH_ERR_ARG;
-    if (tokens > 0 && (!p->positions || p->period <= 0)) return AETH_ERR_ARG;
-    if (head_dim > kRotMaxHead || tokens > kRotMaxRows || hq > (1 << 20) || hk > (1 << 20)) return AETH_ERR_UNSUPPORTED;
-    if (tokens * ((int64_t)hq + hk) > kRotMaxRows) return AETH_ERR_UNSUPPORTED;
-    return AETH_OK;
-}
-int rot_heads(const AethHeads& h, int64_t tokens, const void* out) {
+struct RotaryIn {
+    const void* data;
+    int64_t ld_t, ld_h;
+    int heads;
+};
+struct RotaryCall {  // what every entry point has
+    const AethRotaryPlan* plan;
+    const void* positions;
+    int bits;
+    int64_t period;
+    RotaryIn q, k;
+    int64_t tokens;
+    int head_dim, dtype;
+    void *q_out, *k_out;
+};
+
+int rot_heads(const RotaryIn& h, int64_t tokens, const void* out) {
     if (h.heads == 0 || tokens == 0) return AETH_OK;
-    return h.data && out && h.ld_token >= 0 && h.ld_head >= 0 ? AETH_OK : AETH_ERR_ARG;
+    return h.data && out && h.ld_t >= 0 && h.ld_h >= 0 ? AETH_OK : AETH_ERR_ARG;
+}
+int rot_check(const RotaryCall& c) {
+    const AethRotaryPlan* p = c.plan;
+    const int hq = c.q.heads, hk = c.k.heads;
+    if (!p || c.tokens < 0 || c.head_dim <= 0 || hq < 0 || hk < 0 || (hq == 0 && hk == 0) || !rot_dtype(c.dtype)) return AETH_ERR_ARG;
+    if (p->rotary_dim < 2 || p->rotary_dim % 2 || p->rotary_dim > c.head_dim || !p->freq) return AETH_ERR_ARG;
+    if ((c.bits != 32 && c.bits != 64) || (c.tokens > 0 && (!c.positions || c.period <= 0))) return AETH_ERR_ARG;
+    if (c.head_dim > kRotMaxHead || c.tokens > kRotMaxRows || hq > (1 << 20) || hk > (1 << 20)) return AETH_ERR_UNSUPPORTED;
+    if (c.tokens > kRotMaxRows / ((int64_t)hq + hk)) return AETH_ERR_UNSUPPORTED;
+    AETH_TRY(rot_heads(c.q, c.tokens, c.q_out));
+    return rot_heads(c.k, c.tokens, c.k_out);
 }
 
 // Whether every head row can be taken in 16-byte pieces
-bool rot_whole(const AethHeads& h, int64_t tokens, int size) {
+bool rot_whole(const RotaryIn& h, int64_t tokens, int size) {
     if (h.heads == 0) return true;
-    return reinterpret_cast<uintptr_t>(h.data) % 16 == 0 && (tokens == 1 || h.ld_token * size % 16 == 0) &&
-           (h.heads == 1 || h.ld_head * size % 16 == 0);
+    return reinterpret_cast<uintptr_t>(h.data) % 16 == 0 && (tokens == 1 || h.ld_t * size % 16 == 0) &&
+           (h.heads == 1 || h.ld_h * size % 16 == 0);
+}
+bool rot_whole(const RotaryCall& c) {
+    const int size = rot_size(c.dtype);
+    return rot_whole(c.q, c.tokens, size) && rot_whole(c.k, c.tokens, size) && reinterpret_cast<uintptr_t>(c.q_out) % 16 == 0 &&
+           reinterpret_cast<uintptr_t>(c.k_out) % 16 == 0;
 }
 
 // Rows of a stretch and CTAs of rotary_any_kernel's grid.  A stretch is what gives
@@ -112,66 +135,66 @@ int rot_typed(RotaryArgs& a, int64_t tokens, int dtype, bool inter, bool whole, 
                  : rot_launch<__nv_bfloat16, false, OP>(a, tokens, whole, st);
 }
 
-RotaryArgs rot_args(const AethRotaryPlan& p, const AethHeads& q, const AethHeads& k, int64_t tokens, int head_dim, void* q_out,
-                    void* k_out, bool flip) {
+RotaryArgs rot_args(const RotaryCall& c, bool flip) {
     RotaryArgs a = {};
-    const AethHeads* h[2] = {&q, &k};
-    void* out[2] = {q_out, k_out};
+    const RotaryIn* h[2] = {&c.q, &c.k};
+    void* out[2] = {c.q_out, c.k_out};
     for (int i = 0; i < 2; ++i) {
-        a.s[i].x = h[i]->data;
-        a.s[i].ld_t = h[i]->ld_token;
-        a.s[i].ld_h = h[i]->ld_head;
-        a.s[i].out = out[i];
-        a.s[i].heads = std::max(h[i]->heads, 1);
-        a.s[i].magic = (uint32_t)(((1ull << 32) + a.s[i].heads - 1) / a.s[i].heads);
-        a.s[i].rows = tokens * h[i]->heads;
+        RotaryRows& s = a.s[i];
+        s.x = h[i]->data;
+        s.ld_t = h[i]->ld_t;
+        s.ld_h = h[i]->ld_h;
+        s.out = out[i];
+        s.heads = std::max(h[i]->heads, 1);
+        s.magic = (uint32_t)(((1ull << 32) + s.heads - 1) / s.heads);
+        s.rows = c.tokens * h[i]->heads;
     }
-    a.pos = p.positions;
-    a.pos32 = p.position_bits == 32;
-    a.period = p.period;
-    a.freq = p.freq;
-    a.amp = p.amplitude;
+    a.pos = c.positions;
+    a.pos32 = c.bits == 32;
+    a.period = c.period;
+    a.freq = c.plan->freq;
+    a.amp = c.plan->amplitude;
     a.flip = flip;
-    a.D = head_dim;
-    a.R = p.rotary_dim;
+    a.D = c.head_dim;
+    a.R = c.plan->rotary_dim;
     return a;
 }
-bool rot_out_whole(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }  // rows of D, whose bytes 16 divides
+template <int OP>
+int rot_run(RotaryArgs& a, const RotaryCall& c, bool whole, cudaStream_t st) {
+    return rot_typed<OP>(a, c.tokens, c.dtype, c.plan->interleaved != 0, whole, st);
+}
 
 }  // namespace
 
 extern "C" {
 
-int aeth_rotary(const AethRotaryPlan* plan, const AethHeads* q, const AethHeads* k, int64_t tokens, int head_dim, int dtype,
-                int inverse, void* q_out, void* k_out, aeth_stream_t stream) {
-    if (!q || !k) return set_err(AETH_ERR_ARG);
-    AETH_TRY(rot_check(plan, tokens, head_dim, q->heads, k->heads, dtype));
-    AETH_TRY(rot_heads(*q, tokens, q_out));
-    AETH_TRY(rot_heads(*k, tokens, k_out));
+int aeth_rotary(const AethRotaryPlan* plan, const void* positions, int position_bits, int64_t period, const void* q,
+                int64_t ld_q_token, int64_t ld_q_head, int q_heads, const void* k, int64_t ld_k_token, int64_t ld_k_head,
+                int k_heads, int64_t tokens, int head_dim, int dtype, int inverse, void* q_out, void* k_out,
+                aeth_stream_t stream) {
+    const RotaryCall c{plan, positions, position_bits, period, {q, ld_q_token, ld_q_head, q_heads},
+                       {k, ld_k_token, ld_k_head, k_heads}, tokens, head_dim, dtype, q_out, k_out};
+    AETH_TRY(rot_check(c));
     if (tokens == 0) return AETH_OK;
-    RotaryArgs a = rot_args(*plan, *q, *k, tokens, head_dim, q_out, k_out, inverse != 0);
-    const int size = rot_size(dtype);
-    const bool whole = rot_whole(*q, tokens, size) && rot_whole(*k, tokens, size) && rot_out_whole(q_out) && rot_out_whole(k_out);
-    return rot_typed<ROT_TURN>(a, tokens, dtype, plan->interleaved != 0, whole, to_stream(stream));
+    RotaryArgs a = rot_args(c, inverse != 0);
+    return rot_run<ROT_TURN>(a, c, rot_whole(c), to_stream(stream));
 }
 
-int aeth_qk_norm_rotary(const AethRotaryPlan* plan, const AethHeads* q, const AethHeads* k, const void* q_gain,
-                        const void* k_gain, int gain_dtype, float eps, int64_t tokens, int head_dim, int dtype, void* q_out,
-                        void* k_out, aeth_stream_t stream) {
-    if (!q || !k) return set_err(AETH_ERR_ARG);
-    AETH_TRY(rot_check(plan, tokens, head_dim, q->heads, k->heads, dtype));
-    AETH_TRY(rot_heads(*q, tokens, q_out));
-    AETH_TRY(rot_heads(*k, tokens, k_out));
-    if (!rot_dtype(gain_dtype) || (q->heads && !q_gain) || (k->heads && !k_gain)) return set_err(AETH_ERR_ARG);
+int aeth_qk_norm_rotary(const AethRotaryPlan* plan, const void* positions, int position_bits, int64_t period, const void* q,
+                        int64_t ld_q_token, int64_t ld_q_head, int q_heads, const void* k, int64_t ld_k_token,
+                        int64_t ld_k_head, int k_heads, const void* q_gain, const void* k_gain, int gain_dtype, float eps,
+                        int64_t tokens, int head_dim, int dtype, void* q_out, void* k_out, aeth_stream_t stream) {
+    const RotaryCall c{plan, positions, position_bits, period, {q, ld_q_token, ld_q_head, q_heads},
+                       {k, ld_k_token, ld_k_head, k_heads}, tokens, head_dim, dtype, q_out, k_out};
+    AETH_TRY(rot_check(c));
+    if (!rot_dtype(gain_dtype) || (q_heads && !q_gain) || (k_heads && !k_gain)) return set_err(AETH_ERR_ARG);
     if (tokens == 0) return AETH_OK;
-    RotaryArgs a = rot_args(*plan, *q, *k, tokens, head_dim, q_out, k_out, false);
+    RotaryArgs a = rot_args(c, false);
     a.s[0].gain = q_gain;
     a.s[1].gain = k_gain;
     a.gain_dtype = gain_dtype;
     a.eps = eps;
-    const int size = rot_size(dtype);
-    const bool whole = rot_whole(*q, tokens, size) && rot_whole(*k, tokens, size) && rot_out_whole(q_out) && rot_out_whole(k_out);
-    return rot_typed<ROT_NORM>(a, tokens, dtype, plan->interleaved != 0, whole, to_stream(stream));
+    return rot_run<ROT_NORM>(a, c, rot_whole(c), to_stream(stream));
 }
 
 int aeth_qk_norm_rotary_backward_workspace(int head_dim, size_t* bytes) {
@@ -181,51 +204,51 @@ int aeth_qk_norm_rotary_backward_workspace(int head_dim, size_t* bytes) {
     return AETH_OK;
 }
 
-int aeth_qk_norm_rotary_backward(const AethRotaryPlan* plan, const AethHeads* dq, const AethHeads* dk, const AethHeads* q,
-                                 const AethHeads* k, const void* q_gain, const void* k_gain, int gain_dtype, float eps,
+int aeth_qk_norm_rotary_backward(const AethRotaryPlan* plan, const void* positions, int position_bits, int64_t period,
+                                 const void* dq, int64_t ld_dq_token, int64_t ld_dq_head, const void* dk,
+                                 int64_t ld_dk_token, int64_t ld_dk_head, const void* q, int64_t ld_q_token,
+                                 int64_t ld_q_head, int q_heads, const void* k, int64_t ld_k_token, int64_t ld_k_head,
+                                 int k_heads, const void* q_gain, const void* k_gain, int gain_dtype, float eps,
                                  int64_t tokens, int head_dim, int dtype, void* dq_out, void* dk_out, float* d_q_gain,
                                  float* d_k_gain, void* workspace, size_t workspace_bytes, aeth_stream_t stream) {
-    if (!q || !k || !dq || !dk || dq->heads != q->heads || dk->heads != k->heads) return set_err(AETH_ERR_ARG);
-    AETH_TRY(rot_check(plan, tokens, head_dim, q->heads, k->heads, dtype));
-    for (const AethHeads* h : {q, dq}) AETH_TRY(rot_heads(*h, tokens, dq_out));
-    for (const AethHeads* h : {k, dk}) AETH_TRY(rot_heads(*h, tokens, dk_out));
-    if (!rot_dtype(gain_dtype) || (q->heads && (!q_gain || !d_q_gain)) || (k->heads && (!k_gain || !d_k_gain)))
+    const RotaryCall c{plan, positions, position_bits, period, {q, ld_q_token, ld_q_head, q_heads},
+                       {k, ld_k_token, ld_k_head, k_heads}, tokens, head_dim, dtype, dq_out, dk_out};
+    AETH_TRY(rot_check(c));
+    const RotaryIn dy[2] = {{dq, ld_dq_token, ld_dq_head, q_heads}, {dk, ld_dk_token, ld_dk_head, k_heads}};
+    AETH_TRY(rot_heads(dy[0], tokens, dq_out));
+    AETH_TRY(rot_heads(dy[1], tokens, dk_out));
+    if (!rot_dtype(gain_dtype) || (q_heads && (!q_gain || !d_q_gain)) || (k_heads && (!k_gain || !d_k_gain)))
         return set_err(AETH_ERR_ARG);
     cudaStream_t st = to_stream(stream);
     if (tokens == 0) {
-        if (q->heads) AETH_CUDA(cudaMemsetAsync(d_q_gain, 0, sizeof(float) * (size_t)head_dim, st));
-        if (k->heads) AETH_CUDA(cudaMemsetAsync(d_k_gain, 0, sizeof(float) * (size_t)head_dim, st));
+        if (q_heads) AETH_CUDA(cudaMemsetAsync(d_q_gain, 0, sizeof(float) * (size_t)head_dim, st));
+        if (k_heads) AETH_CUDA(cudaMemsetAsync(d_k_gain, 0, sizeof(float) * (size_t)head_dim, st));
         return AETH_OK;
     }
     size_t need = 0;
     AETH_TRY(aeth_qk_norm_rotary_backward_workspace(head_dim, &need));
     if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16) return set_err(AETH_ERR_ARG);
-    RotaryArgs a = rot_args(*plan, *q, *k, tokens, head_dim, dq_out, dk_out, true);
-    const AethHeads* dy[2] = {dq, dk};
+    RotaryArgs a = rot_args(c, true);
     for (int i = 0; i < 2; ++i) {
-        a.s[i].dy = dy[i]->data;
-        a.s[i].ld_dt = dy[i]->ld_token;
-        a.s[i].ld_dh = dy[i]->ld_head;
+        a.s[i].dy = dy[i].data;
+        a.s[i].ld_dt = dy[i].ld_t;
+        a.s[i].ld_dh = dy[i].ld_h;
+        a.s[i].part = static_cast<float*>(workspace) + (int64_t)i * (rot_back_ctas() + 1) * head_dim;
     }
     a.s[0].gain = q_gain;
     a.s[1].gain = k_gain;
     a.gain_dtype = gain_dtype;
     a.eps = eps;
-    a.s[0].part = static_cast<float*>(workspace);
     const int size = rot_size(dtype);
-    bool whole = rot_out_whole(dq_out) && rot_out_whole(dk_out);
-    for (const AethHeads* h : {q, k, dq, dk}) whole = whole && rot_whole(*h, tokens, size);
-    a.s[1].part = a.s[0].part + (int64_t)(rot_back_ctas() + 1) * head_dim;
-    AETH_TRY(rot_typed<ROT_NORM_BACK>(a, tokens, dtype, plan->interleaved != 0, whole, st));
-    const RotaryGain g{{a.s[0].part, a.s[1].part}, {d_q_gain, d_k_gain}, {(int)a.s[0].ctas, (int)a.s[1].ctas}, head_dim};
-    const bool both = q->heads && k->heads;
-    RotaryGain only = g;
-    if (!q->heads) {
-        only.part[0] = g.part[1];
-        only.out[0] = g.out[1];
-        only.groups[0] = g.groups[1];
+    AETH_TRY(rot_run<ROT_NORM_BACK>(a, c, rot_whole(c) && rot_whole(dy[0], tokens, size) && rot_whole(dy[1], tokens, size), st));
+    RotaryGain g{{a.s[0].part, a.s[1].part}, {d_q_gain, d_k_gain}, {(int)a.s[0].ctas, (int)a.s[1].ctas}, head_dim};
+    if (!q_heads) {  // k's alone
+        g.part[0] = g.part[1];
+        g.out[0] = g.out[1];
+        g.groups[0] = g.groups[1];
     }
-    AETH_CUDA(launch_after(rotary_gain_kernel, dim3((unsigned)(head_dim + 31) / 32, both ? 2 : 1), dim3(1024), 0, st, 1, only));
+    AETH_CUDA(launch_after(rotary_gain_kernel, dim3((unsigned)(head_dim + 31) / 32, q_heads && k_heads ? 2 : 1), dim3(1024), 0, st,
+                           1, g));
     return AETH_OK;
 }
 

@@ -84,19 +84,23 @@ class RotaryPlan:
         self.rotary_dim, self.layout, self.amplitude, self.inv_freq = rotary_dim, layout, float(amplitude), tuple(f)
         turns = [round(x / math.tau * 2.0 ** 64) % 2 ** 64 for x in f]  # of 2^64 a position
         self.freq = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns], dtype=torch.int64, device=device)
+        self._c = L.RotaryPlan(self.freq.data_ptr(), rotary_dim, layout == "interleaved", self.amplitude)
+        self._device = self.freq.get_device()
 
 
-def _heads(t: torch.Tensor, d: int) -> tuple[torch.Tensor, int, int]:
+def _heads(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
     """(a tensor whose data are t's head rows, the tokens' pitch, the heads'), `t`
     itself where its strides allow it."""
-    if t.stride(-1) != 1 and d > 1:
+    shape, stride = t.shape, t.stride()
+    if stride[-1] != 1 and shape[-1] > 1:
         t = t.contiguous()
-    if t.dim() == 3:
-        return t, t.stride(0), t.stride(1)
-    if t.dim() == 2:
-        return t, 0, t.stride(0)
-    shape, stride, ld = t.shape, t.stride(), None
-    for i in range(t.dim() - 3, -1, -1):  # the tokens' dimensions as one, the last first
+        stride = t.stride()
+    if len(shape) == 3:
+        return t, stride[0], stride[1]
+    if len(shape) == 2:
+        return t, 0, stride[0]
+    ld = span = None
+    for i in range(len(shape) - 3, -1, -1):  # the tokens' dimensions as one, the last first
         if shape[i] == 1:
             continue
         if ld is None:
@@ -109,75 +113,76 @@ def _heads(t: torch.Tensor, d: int) -> tuple[torch.Tensor, int, int]:
     return t, ld or 0, stride[-2]
 
 
-class _Call:
-    """The checked arguments of a call: q and k beside further pairs of their shapes."""
-
-    def __init__(self, what, dev, positions, plan, *pairs):
-        q, k = pairs[0]
-        if not isinstance(plan, RotaryPlan):
-            raise ValueError(f"{what}: plan must be a RotaryPlan")
-        d = q.size(-1) if q.dim() >= 2 else 0
-        self.dtype = _DTYPES.get(q.dtype)
-        if self.dtype is None or d == 0 or q.size(-2) == 0 or plan.rotary_dim > d or d > MAX_HEAD_DIM:
-            raise ValueError(f"{what}: q must be a float tensor (..., heads, head_dim) with {plan.rotary_dim} to "
-                             f"{MAX_HEAD_DIM} features a head, got {tuple(q.shape)}")
-        lead = q.shape[:-2]
-        if k is not None and (k.dim() != q.dim() or k.shape[:-2] != lead or k.size(-1) != d or k.dtype != q.dtype
-                              or k.size(-2) == 0):
-            raise ValueError(f"{what}: k must be (..., key heads, {d}) of q's type and tokens, got {tuple(k.shape)}")
-        for a, b in pairs[1:]:
-            for x, y in ((a, q), (b, k)):
-                if (x is None) != (y is None) or x is not None and (x.shape != y.shape or x.dtype != y.dtype):
-                    raise ValueError(f"{what}: gradients must have the shapes and types of q and k")
-        if positions.dtype.is_floating_point or positions.dtype.is_complex or positions.dtype == torch.bool:
+def _checked(what, dev, plan, positions, q, k):
+    """The arguments that every call has: ((plan, positions, bits, period), (q, its
+    pitches and heads), (k, ...), (tokens, head_dim, dtype), what the pointers
+    point at)."""
+    if not isinstance(plan, RotaryPlan):
+        raise ValueError(f"{what}: plan must be a RotaryPlan")
+    shape, kind = q.shape, q.dtype
+    dtype = _DTYPES.get(kind)
+    if dtype is None or len(shape) < 2 or not plan.rotary_dim <= shape[-1] <= MAX_HEAD_DIM or shape[-2] == 0:
+        raise ValueError(f"{what}: q must be a float tensor (..., heads, head_dim) with {plan.rotary_dim} to {MAX_HEAD_DIM} "
+                         f"features a head, got {tuple(shape)}")
+    lead, heads, d = shape[:-2], shape[-2], shape[-1]
+    pshape, pkind = positions.shape, positions.dtype
+    if pkind is not torch.int64 and pkind is not torch.int32:
+        if pkind.is_floating_point or pkind.is_complex or pkind is torch.bool:
             raise ValueError(f"{what}: positions must be whole numbers")
-        if positions.dim() > len(lead) or lead[len(lead) - positions.dim():] != positions.shape:
-            raise ValueError(f"{what}: positions must be {tuple(lead)} or its last dimensions, got {tuple(positions.shape)}")
-        for t in (positions, plan.freq, *(t for p in pairs for t in p)):
-            if t is not None and t.get_device() != dev:
-                raise ValueError(f"{what}: all tensors must be on cuda:{dev}")
-        if positions.dtype not in (torch.int64, torch.int32):
-            positions = positions.to(torch.int64)
-        self.d = d
-        self.tokens = q.numel() // (q.size(-2) * d)
-        self.keep = [positions.contiguous()]  # what the pointers point at
-        self.plan = L.RotaryPlan(self.keep[0].data_ptr(), 64 if positions.dtype == torch.int64 else 32,
-                                 max(positions.numel(), 1), plan.freq.data_ptr(), plan.rotary_dim,
-                                 plan.layout == "interleaved", plan.amplitude)
-        self.sides = []
-        for p in pairs:
-            for t in p:
-                if t is None:
-                    self.sides.append(L.Heads(None, 0, 0, 0))
-                    continue
-                r, ld_t, ld_h = _heads(t, d)
-                self.keep.append(r)
-                self.sides.append(L.Heads(r.data_ptr(), ld_t, ld_h, t.size(-2)))
-        self.out = [None if t is None else t.new_empty(t.shape) for t in pairs[0]]
-        self.out_ptr = [None if t is None else t.data_ptr() for t in self.out]
+        positions = positions.to(torch.int64)
+        pkind = torch.int64
+    if pshape != lead and (len(pshape) > len(lead) or lead[len(lead) - len(pshape):] != pshape):
+        raise ValueError(f"{what}: positions must be {tuple(lead)} or its last dimensions, got {tuple(pshape)}")
+    if plan._device != dev or positions.get_device() != dev or k is not None and k.get_device() != dev:
+        raise ValueError(f"{what}: all tensors must be on cuda:{dev}")
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
+    qr, q_t, q_h = _heads(q)
+    if k is None:
+        kr, side = None, (None, 0, 0, 0)
+    else:
+        kshape = k.shape
+        if len(kshape) != len(shape) or kshape[:-2] != lead or kshape[-1] != d or kshape[-2] == 0 or k.dtype is not kind:
+            raise ValueError(f"{what}: k must be (..., key heads, {d}) of q's type and tokens, got {tuple(kshape)}")
+        kr, k_t, k_h = _heads(k)
+        side = (kr.data_ptr(), k_t, k_h, kshape[-2])
+    return ((plan._c, positions.data_ptr(), 64 if pkind is torch.int64 else 32, positions.numel() or 1),
+            (qr.data_ptr(), q_t, q_h, heads), side, (q.numel() // (heads * d), d, dtype), (positions, qr, kr))
 
-    def gains(self, what, dev, q_weight, k_weight):
-        for w, o in ((q_weight, self.out[0]), (k_weight, self.out[1])):
-            if (w is None) != (o is None):
-                raise ValueError(f"{what}: a weight for each of q and k expected")
-            if w is not None and (w.dim() != 1 or w.size(0) != self.d or w.dtype not in _DTYPES or w.dtype != q_weight.dtype):
-                raise ValueError(f"{what}: weights must be float vectors of {self.d} features, of one type")
-            if w is not None and w.get_device() != dev:
-                raise ValueError(f"{what}: all tensors must be on cuda:{dev}")
-        ws = [None if w is None else w.contiguous() for w in (q_weight, k_weight)]
-        self.keep += ws
-        return [None if w is None else w.data_ptr() for w in ws] + [_DTYPES[q_weight.dtype]]
+
+def _gains(what, dev, d, q_weight, k_weight, k):
+    """(pointers and type of the weights, what they point at)"""
+    if q_weight is None or (k_weight is None) != (k is None):
+        raise ValueError(f"{what}: a weight for each of q and k expected")
+    kind = q_weight.dtype
+    for w in (q_weight, k_weight):
+        if w is not None and (w.dim() != 1 or w.size(0) != d or w.dtype is not kind or kind not in _DTYPES):
+            raise ValueError(f"{what}: weights must be float vectors of {d} features, of one type")
+        if w is not None and w.get_device() != dev:
+            raise ValueError(f"{what}: all tensors must be on cuda:{dev}")
+    qw, kw = q_weight.contiguous(), None if k_weight is None else k_weight.contiguous()
+    return (qw.data_ptr(), None if kw is None else kw.data_ptr(), _DTYPES[kind]), (qw, kw)
+
+
+def _results(q, k):
+    """New contiguous tensors of q's and k's shapes, and where they are."""
+    a = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if k is None:
+        return (a, None), (a.data_ptr(), None)
+    b = torch.empty_like(k, memory_format=torch.contiguous_format)
+    return (a, b), (a.data_ptr(), b.data_ptr())
 
 
 def _turn(what, q, k, positions, plan, inverse):
     dev = q.get_device()
     if dev < 0 or dev != _current_device():
         return _elsewhere(what, dev, _turn, what, q, k, positions, plan, inverse)
-    c = _Call(what, dev, positions, plan, (q, k))
-    st = _lib.aeth_rotary(c.plan, c.sides[0], c.sides[1], c.tokens, c.d, c.dtype, inverse, *c.out_ptr, _raw_stream(dev))
+    at, qs, ks, size, keep = _checked(what, dev, plan, positions, q, k)  # noqa: F841 - keep: alive until the launch
+    out, ptr = _results(q, k)
+    st = _lib.aeth_rotary(*at, *qs, *ks, *size, inverse, *ptr, _raw_stream(dev))
     if st:
         L.check(st, "aeth_rotary")
-    return tuple(c.out)
+    return out
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, plan: RotaryPlan):
@@ -199,12 +204,13 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tens
     what, dev = "qk_norm_rotary", q.get_device()
     if dev < 0 or dev != _current_device():
         return _elsewhere(what, dev, qk_norm_rotary, q, k, q_weight, k_weight, positions, plan, eps)
-    c = _Call(what, dev, positions, plan, (q, k))
-    st = _lib.aeth_qk_norm_rotary(c.plan, c.sides[0], c.sides[1], *c.gains(what, dev, q_weight, k_weight), eps, c.tokens,
-                                  c.d, c.dtype, *c.out_ptr, _raw_stream(dev))
+    at, qs, ks, size, keep = _checked(what, dev, plan, positions, q, k)  # noqa: F841
+    gains, weights = _gains(what, dev, size[1], q_weight, k_weight, k)  # noqa: F841
+    out, ptr = _results(q, k)
+    st = _lib.aeth_qk_norm_rotary(*at, *qs, *ks, *gains, eps, *size, *ptr, _raw_stream(dev))
     if st:
         L.check(st, "aeth_qk_norm_rotary")
-    return tuple(c.out)
+    return out
 
 
 def qk_norm_rotary_backward(dq: torch.Tensor, dk: torch.Tensor | None, q: torch.Tensor, k: torch.Tensor | None,
@@ -216,14 +222,23 @@ def qk_norm_rotary_backward(dq: torch.Tensor, dk: torch.Tensor | None, q: torch.
     what, dev = "qk_norm_rotary_backward", q.get_device()
     if dev < 0 or dev != _current_device():
         return _elsewhere(what, dev, qk_norm_rotary_backward, dq, dk, q, k, q_weight, k_weight, positions, plan, eps)
-    c = _Call(what, dev, positions, plan, (q, k), (dq, dk))
-    gains = c.gains(what, dev, q_weight, k_weight)
-    dw = [None if o is None else q.new_empty(c.d, dtype=torch.float32) for o in c.out]
-    size = _workspace_bytes("aeth_qk_norm_rotary_backward_workspace", dev, c.d)
-    ws = q.new_empty(size, dtype=torch.uint8)
+    at, qs, ks, size, keep = _checked(what, dev, plan, positions, q, k)  # noqa: F841
+    gains, weights = _gains(what, dev, size[1], q_weight, k_weight, k)  # noqa: F841
+    for g, x in ((dq, q), (dk, k)):
+        if (g is None) != (x is None) or g is not None and (g.shape != x.shape or g.dtype is not x.dtype):
+            raise ValueError(f"{what}: gradients must have the shapes and types of q and k")
+        if g is not None and g.get_device() != dev:
+            raise ValueError(f"{what}: all tensors must be on cuda:{dev}")
+    gq, gq_t, gq_h = _heads(dq)
+    gk, gk_t, gk_h = (None, 0, 0) if dk is None else _heads(dk)
+    out, ptr = _results(q, k)
+    dw_q = q.new_empty(size[1], dtype=torch.float32)
+    dw_k = None if k is None else q.new_empty(size[1], dtype=torch.float32)
+    room = _workspace_bytes("aeth_qk_norm_rotary_backward_workspace", dev, size[1])
+    ws = q.new_empty(room, dtype=torch.uint8)
     st = _lib.aeth_qk_norm_rotary_backward(
-        c.plan, c.sides[2], c.sides[3], c.sides[0], c.sides[1], *gains, eps, c.tokens, c.d, c.dtype, *c.out_ptr,
-        dw[0].data_ptr(), None if dw[1] is None else dw[1].data_ptr(), ws.data_ptr(), size, _raw_stream(dev))
+        *at, gq.data_ptr(), gq_t, gq_h, None if gk is None else gk.data_ptr(), gk_t, gk_h, *qs, *ks, *gains, eps, *size, *ptr,
+        dw_q.data_ptr(), None if dw_k is None else dw_k.data_ptr(), ws.data_ptr(), room, _raw_stream(dev))
     if st:
         L.check(st, "aeth_qk_norm_rotary_backward")
-    return (*c.out, *dw)
+    return (*out, dw_q, dw_k)

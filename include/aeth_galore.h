@@ -616,7 +616,7 @@ int aeth_checkpoint_weight_grad(const void* dy, int64_t ld_dy, const int8_t* cod
  *     Frequencies are whole numbers: freq[p] = 2^64 times the turns that pair p
  *     makes from one position to the next, modulo 2^64; the angle t freq[p] is
  *     then exact at any position, negative ones too.
- *     Rows: head h of token i lies at data + i * ld_token + h * ld_head
+ *     Rows: head h of token i lies at i * ld_token + h * ld_head
  *     (elements), its features side by side; outputs are contiguous (token, head,
  *     feature) and must not overlap an input.  F32, F16 or BF16; arithmetic in
  *     fp32.  Any head_dim up to 1024; heads of whole sixteens up to 512 whose rows
@@ -624,33 +624,32 @@ int aeth_checkpoint_weight_grad(const void* dy, int64_t ld_dy, const int8_t* cod
  *     Nothing synchronises or allocates.
  * ====================================================================== */
 typedef struct {
-    const void* positions; /* device: of token i, positions[i % period] */
-    int position_bits;     /* 64 or 32 */
-    int64_t period;
-    const uint64_t* freq;  /* device: rotary_dim / 2 */
-    int rotary_dim;        /* even */
+    const uint64_t* freq; /* device: rotary_dim / 2 */
+    int rotary_dim;       /* even */
     int interleaved;
-    float amplitude;       /* a */
+    float amplitude;      /* a */
 } AethRotaryPlan;
-typedef struct {
-    const void* data;
-    int64_t ld_token, ld_head;
-    int heads;
-} AethHeads;
-/* inverse: turns the other way (with the same amplitude): the gradient. */
-int aeth_rotary(const AethRotaryPlan* plan, const AethHeads* q, const AethHeads* k, int64_t tokens, int head_dim, int dtype,
-                int inverse, void* q_out, void* k_out, aeth_stream_t stream);
+/* positions: device, of position_bits (64 or 32); token i is at positions[i %
+ * period].  inverse: turns the other way (with the same amplitude): the gradient. */
+int aeth_rotary(const AethRotaryPlan* plan, const void* positions, int position_bits, int64_t period, const void* q,
+                int64_t ld_q_token, int64_t ld_q_head, int q_heads, const void* k, int64_t ld_k_token, int64_t ld_k_head,
+                int k_heads, int64_t tokens, int head_dim, int dtype, int inverse, void* q_out, void* k_out,
+                aeth_stream_t stream);
 /* y = turned(x r gain), r = 1 / sqrt(mean x^2 + eps) over the head's features;
  * gains of head_dim, of a type of their own. */
-int aeth_qk_norm_rotary(const AethRotaryPlan* plan, const AethHeads* q, const AethHeads* k, const void* q_gain,
-                        const void* k_gain, int gain_dtype, float eps, int64_t tokens, int head_dim, int dtype, void* q_out,
-                        void* k_out, aeth_stream_t stream);
+int aeth_qk_norm_rotary(const AethRotaryPlan* plan, const void* positions, int position_bits, int64_t period, const void* q,
+                        int64_t ld_q_token, int64_t ld_q_head, int q_heads, const void* k, int64_t ld_k_token,
+                        int64_t ld_k_head, int k_heads, const void* q_gain, const void* k_gain, int gain_dtype, float eps,
+                        int64_t tokens, int head_dim, int dtype, void* q_out, void* k_out, aeth_stream_t stream);
 /* Its gradient at q and k: with g the turned-back dq, dq_out = r (gain g) -
  * q r^3 mean(gain g q) and d_q_gain = sum of g q r over tokens and heads (F32,
  * in an order that the sizes alone decide); k's the same. */
 int aeth_qk_norm_rotary_backward_workspace(int head_dim, size_t* bytes);
-int aeth_qk_norm_rotary_backward(const AethRotaryPlan* plan, const AethHeads* dq, const AethHeads* dk, const AethHeads* q,
-                                 const AethHeads* k, const void* q_gain, const void* k_gain, int gain_dtype, float eps,
+int aeth_qk_norm_rotary_backward(const AethRotaryPlan* plan, const void* positions, int position_bits, int64_t period,
+                                 const void* dq, int64_t ld_dq_token, int64_t ld_dq_head, const void* dk,
+                                 int64_t ld_dk_token, int64_t ld_dk_head, const void* q, int64_t ld_q_token,
+                                 int64_t ld_q_head, int q_heads, const void* k, int64_t ld_k_token, int64_t ld_k_head,
+                                 int k_heads, const void* q_gain, const void* k_gain, int gain_dtype, float eps,
                                  int64_t tokens, int head_dim, int dtype, void* dq_out, void* dk_out, float* d_q_gain,
                                  float* d_k_gain, void* workspace, size_t workspace_bytes, aeth_stream_t stream);
 

@@ -170,7 +170,7 @@ def test_mixed_types_views_and_left_out(A, maps, bits):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
-@pytest.mark.parametrize("count", [64, 65, 896, 897, 1900])
+@pytest.mark.parametrize("count", [64, 65, 256, 257, 768, 769, 1900])
 def test_long_lists(A, maps, bits, count):
     """Tables of both sizes, and several launches that count one step."""
     gen = torch.Generator(device="cuda").manual_seed(3)

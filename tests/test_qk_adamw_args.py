@@ -18,59 +18,51 @@ P = 4096  # a non-null, aligned address that no refused call reads
 ARG, UNSUPPORTED = -1, -4
 
 
-def plan(L, **kw):
-    a = dict(positions=P, position_bits=64, period=4, freq=P, rotary_dim=64, interleaved=0, amplitude=1.0)
+def rotary(lib, which="turn", **kw):
+    """A call whose arguments are right but for those of kw."""
+    a = dict(freq=P, rotary_dim=64, positions=P, bits=64, period=4, q=P, qt=256, qh=64, hq=4, k=P, kt=256, kh=64, hk=1, tokens=4,
+             d=64, dtype=2, qg=P, kg=P, gain_dtype=2, qo=P, ko=P, dq=P, dqt=256, dk=P, dwq=P, dwk=P, ws=P, size=1 << 30, plan=True)
     a.update(kw)
-    return L.RotaryPlan(*a.values())
-
-
-def heads(L, **kw):
-    a = dict(data=P, ld_token=256, ld_head=64, heads=4)
-    a.update(kw)
-    return L.Heads(*a.values())
-
-
-CASES = [(dict(rotary_dim=63), {}, {}, ARG), (dict(rotary_dim=0), {}, {}, ARG), (dict(rotary_dim=66), {}, {}, ARG),
-         (dict(freq=None), {}, {}, ARG), (dict(positions=None), {}, {}, ARG), (dict(period=0), {}, {}, ARG),
-         (dict(position_bits=16), {}, {}, ARG), ({}, dict(data=None), {}, ARG), ({}, dict(heads=-1), {}, ARG),
-         ({}, dict(ld_head=-64), {}, ARG), ({}, {}, dict(tokens=-1), ARG), ({}, {}, dict(head_dim=0), ARG),
-         ({}, {}, dict(dtype=5), ARG), ({}, {}, dict(head_dim=1025), UNSUPPORTED), ({}, {}, dict(tokens=1 << 39), UNSUPPORTED),
-         ({}, dict(heads=0), dict(k_heads=0), ARG), ({}, {}, dict(out=None), ARG)]
-
-
-@pytest.mark.parametrize("pl,qs,more,status", CASES)
-def test_rotary_refusals(lib, pl, qs, more, status):
-    a = dict(tokens=4, head_dim=64, dtype=2, k_heads=1, out=P)
-    a.update(more)
-    q, k, p = heads(lib, **qs), heads(lib, heads=a["k_heads"]), plan(lib, **pl)
     L = lib.load()
-    assert L.aeth_rotary(p, q, k, a["tokens"], a["head_dim"], a["dtype"], 0, a["out"], P, None) == status
-    assert L.aeth_qk_norm_rotary(p, q, k, P, P, 2, 1e-6, a["tokens"], a["head_dim"], a["dtype"], a["out"], P, None) == status
-    assert L.aeth_qk_norm_rotary_backward(p, q, k, q, k, P, P, 2, 1e-6, a["tokens"], a["head_dim"], a["dtype"], a["out"], P, P, P,
-                                          P, 1 << 30, None) == status
+    at = (lib.RotaryPlan(a["freq"], a["rotary_dim"], 0, 1.0) if a["plan"] else None, a["positions"], a["bits"], a["period"])
+    qk = (a["q"], a["qt"], a["qh"], a["hq"], a["k"], a["kt"], a["kh"], a["hk"])
+    size, gains = (a["tokens"], a["d"], a["dtype"]), (a["qg"], a["kg"], a["gain_dtype"], 1e-6)
+    if which == "turn":
+        return L.aeth_rotary(*at, *qk, *size, 0, a["qo"], a["ko"], None)
+    if which == "norm":
+        return L.aeth_qk_norm_rotary(*at, *qk, *gains, *size, a["qo"], a["ko"], None)
+    return L.aeth_qk_norm_rotary_backward(*at, a["dq"], a["dqt"], 64, a["dk"], 256, 64, *qk, *gains, *size, a["qo"], a["ko"],
+                                          a["dwq"], a["dwk"], a["ws"], a["size"], None)
+
+
+@pytest.mark.parametrize("which", ["turn", "norm", "back"])
+@pytest.mark.parametrize("kw,status", [
+    (dict(rotary_dim=63), ARG), (dict(rotary_dim=0), ARG), (dict(rotary_dim=66), ARG), (dict(freq=None), ARG), (dict(plan=False), ARG),
+    (dict(positions=None), ARG), (dict(period=0), ARG), (dict(bits=16), ARG), (dict(q=None), ARG), (dict(k=None), ARG),
+    (dict(hq=-1), ARG), (dict(hk=-1), ARG), (dict(hq=0, hk=0), ARG), (dict(qh=-64), ARG), (dict(kt=-1), ARG), (dict(qo=None), ARG),
+    (dict(ko=None), ARG), (dict(tokens=-1), ARG), (dict(d=0), ARG), (dict(dtype=5), ARG), (dict(d=1025), UNSUPPORTED),
+    (dict(tokens=1 << 37), UNSUPPORTED), (dict(hq=1 << 21), UNSUPPORTED)])
+def test_rotary_refusals(lib, which, kw, status):
+    assert rotary(lib, which, **kw) == status
+    assert lib.load().aeth_last_error() == status
 
 
 def test_norm_refusals(lib):
-    L, p, q, k = lib.load(), plan(lib), heads(lib), heads(lib, heads=1)
-    assert L.aeth_qk_norm_rotary(p, q, k, None, P, 2, 1e-6, 4, 64, 2, P, P, None) == ARG
-    assert L.aeth_qk_norm_rotary(p, q, k, P, None, 2, 1e-6, 4, 64, 2, P, P, None) == ARG
-    assert L.aeth_qk_norm_rotary(p, q, k, P, P, 9, 1e-6, 4, 64, 2, P, P, None) == ARG
-    size = C.c_size_t()
+    L, size = lib.load(), C.c_size_t()
+    for which in ("norm", "back"):
+        for kw in (dict(qg=None), dict(kg=None), dict(gain_dtype=9)):
+            assert rotary(lib, which, **kw) == ARG, (which, kw)
+    for kw in (dict(dq=None), dict(dk=None), dict(dqt=-1), dict(dwq=None), dict(dwk=None), dict(ws=None), dict(size=64), dict(ws=P + 8)):
+        assert rotary(lib, "back", **kw) == ARG, kw
     assert L.aeth_qk_norm_rotary_backward_workspace(64, C.byref(size)) == 0 and size.value >= 64 * 4
     assert L.aeth_qk_norm_rotary_backward_workspace(0, C.byref(size)) == ARG
     assert L.aeth_qk_norm_rotary_backward_workspace(64, None) == ARG
     assert L.aeth_qk_norm_rotary_backward_workspace(2000, C.byref(size)) == UNSUPPORTED
-    back = lambda **a: L.aeth_qk_norm_rotary_backward(p, a.get("dq", q), k, q, k, P, P, 2, 1e-6, 4, 64, 2, P, P, a.get("dw", P), P,  # noqa: E731
-                                                      a.get("ws", P), a.get("size", 1 << 30), None)
-    for bad in (dict(dq=heads(lib, heads=3)), dict(dw=None), dict(ws=None), dict(size=64), dict(ws=P + 8)):
-        assert back(**bad) == ARG, bad
 
 
 def test_nothing_to_do(lib):
-    L, p = lib.load(), plan(lib, positions=None)
-    q, k = heads(lib, data=None), heads(lib, data=None, heads=0)
-    assert L.aeth_rotary(p, q, k, 0, 64, 2, 0, None, None, None) == 0
-    assert L.aeth_qk_norm_rotary(p, q, k, P, None, 2, 1e-6, 0, 64, 2, None, None, None) == 0
+    for which in ("turn", "norm"):
+        assert rotary(lib, which, tokens=0, positions=None, q=None, k=None, qo=None, ko=None) == 0
 
 
 def step(lib, p=(P, 1 << 20), n=(100, 5), g=(P, P), pd=(0, 1), gd=(0, 2), count=2, **kw):
