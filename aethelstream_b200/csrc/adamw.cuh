@@ -64,45 +64,95 @@ struct AdamwArgs {
 };
 static_assert(sizeof(AdamwArgs<kAdamwTensors>) <= 32764, "a launch's parameters");
 
-// N elements (4 or 8) of any type, the first `have` of which exist; whole: they
-// start on as many bytes as they take, 16 at most.
+// N 16-bit elements as floats, and back
 template <int N>
-__device__ __forceinline__ void adamw_load(const void* p, int dtype, bool whole, int64_t i, int have, float (&v)[N]) {
-    if (dtype == AETH_DTYPE_F32) {
-        const float* q = static_cast<const float*>(p) + i;
-        if (whole && have >= N) {
+__device__ __forceinline__ void adamw_floats(const uint32_t (&w)[N / 2], int dtype, float (&v)[N]) {
+    if (dtype == AETH_DTYPE_F16) {
 #pragma unroll
-            for (int k = 0; k < N; k += 4) {
-                const float4 a = *reinterpret_cast<const float4*>(q + k);
-                v[k] = a.x; v[k + 1] = a.y; v[k + 2] = a.z; v[k + 3] = a.w;
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < N; ++k) v[k] = k < have ? q[k] : 0.0f;
-        }
-        return;
-    }
-    const uint16_t* q = static_cast<const uint16_t*>(p) + i;
-    uint32_t w[N / 2];
-    if (whole && have >= N) {
-        if constexpr (N == 8) {
-            const uint4 x = *reinterpret_cast<const uint4*>(q);
-            w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
-        } else {
-            const uint2 x = *reinterpret_cast<const uint2*>(q);
-            w[0] = x.x; w[1] = x.y;
+        for (int k = 0; k < N; k += 2) {
+            const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[k / 2]));
+            v[k] = x.x;
+            v[k + 1] = x.y;
         }
     } else {
 #pragma unroll
-        for (int k = 0; k < N; k += 2)
-            w[k / 2] = (k < have ? (uint32_t)q[k] : 0u) | (k + 1 < have ? (uint32_t)q[k + 1] << 16 : 0u);
+        for (int k = 0; k < N; k += 2) {
+            v[k] = __uint_as_float(w[k / 2] << 16);
+            v[k + 1] = __uint_as_float(w[k / 2] & 0xffff0000u);
+        }
     }
+}
+template <int N>
+__device__ __forceinline__ void adamw_words(const float (&v)[N], int dtype, uint32_t (&w)[N / 2]) {
+    if (dtype == AETH_DTYPE_F16) {
 #pragma unroll
-    for (int k = 0; k < N; k += 2) {
-        const float2 x = dtype == AETH_DTYPE_F16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[k / 2]))
-                                                 : make_float2(__uint_as_float(w[k / 2] << 16), __uint_as_float(w[k / 2] & 0xffff0000u));
-        v[k] = x.x;
-        v[k + 1] = x.y;
+        for (int k = 0; k < N; k += 2) w[k / 2] = ck_pack2<__half>(v[k], v[k + 1]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; k += 2) w[k / 2] = ck_pack2<__nv_bfloat16>(v[k], v[k + 1]);
+    }
+}
+
+// N elements (4 or 8) of any type as they lie in memory, the first `have` of which
+// exist; whole: they start on as many bytes as they take, 16 at most.  Read and
+// turned into floats apart, so that no read waits for another.
+template <int N>
+struct AdamwRaw {
+    uint32_t w[N];
+    __device__ __forceinline__ void load(const void* p, int dtype, bool whole, int64_t i, int have) {
+        if (dtype == AETH_DTYPE_F32) {
+            const uint32_t* q = static_cast<const uint32_t*>(p) + i;
+            if (whole && have >= N) {
+#pragma unroll
+                for (int k = 0; k < N; k += 4) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(q + k);
+                    w[k] = x.x; w[k + 1] = x.y; w[k + 2] = x.z; w[k + 3] = x.w;
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < N; ++k) w[k] = k < have ? q[k] : 0u;
+            }
+            return;
+        }
+        const uint16_t* q = static_cast<const uint16_t*>(p) + i;
+        if (whole && have >= N) {
+            if constexpr (N == 8) {
+                const uint4 x = *reinterpret_cast<const uint4*>(q);
+                w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+            } else {
+                const uint2 x = *reinterpret_cast<const uint2*>(q);
+                w[0] = x.x; w[1] = x.y;
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < N; k += 2)
+                w[k / 2] = (k < have ? (uint32_t)q[k] : 0u) | (k + 1 < have ? (uint32_t)q[k + 1] << 16 : 0u);
+        }
+    }
+    __device__ __forceinline__ void floats(int dtype, float (&v)[N]) const {
+        if (dtype == AETH_DTYPE_F32) {
+#pragma unroll
+            for (int k = 0; k < N; ++k) v[k] = __uint_as_float(w[k]);
+        } else {
+            uint32_t x[N / 2];
+#pragma unroll
+            for (int k = 0; k < N / 2; ++k) x[k] = w[k];
+            adamw_floats<N>(x, dtype, v);
+        }
+    }
+};
+template <int N>
+__device__ __forceinline__ void adamw_load(const void* p, int dtype, bool whole, int64_t i, int have, float (&v)[N]) {
+    AdamwRaw<N> r;
+    if (dtype == AETH_DTYPE_F32) {
+        r.load(p, AETH_DTYPE_F32, whole, i, have);
+        r.floats(AETH_DTYPE_F32, v);
+    } else {
+        r.load(p, AETH_DTYPE_F16, whole, i, have);
+        uint32_t x[N / 2];
+#pragma unroll
+        for (int k = 0; k < N / 2; ++k) x[k] = r.w[k];
+        adamw_floats<N>(x, dtype, v);
     }
 }
 template <int N>
@@ -120,9 +170,7 @@ __device__ __forceinline__ void adamw_store(void* p, int dtype, bool whole, int6
         return;
     }
     uint32_t w[N / 2];
-#pragma unroll
-    for (int k = 0; k < N; k += 2)
-        w[k / 2] = dtype == AETH_DTYPE_F16 ? ck_pack2<__half>(v[k], v[k + 1]) : ck_pack2<__nv_bfloat16>(v[k], v[k + 1]);
+    adamw_words<N>(v, dtype, w);
     uint16_t* q = static_cast<uint16_t*>(p) + i;
     if (whole && have >= N) {
         if constexpr (N == 8) *reinterpret_cast<uint4*>(q) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -207,14 +255,12 @@ __device__ __forceinline__ float adamw_scale(float x, float eps) {
     }
     return r;
 }
-// New moments from the old ones, and the parameters, of N elements in pairs: the
-// products of two in one instruction, the sums one by one (common.cuh, add2_sep).
+// New moments from the old ones of N elements, in pairs: the products of two in
+// one instruction, the sums one by one (common.cuh, add2_sep).
 template <int N>
-__device__ __forceinline__ void adamw_update(const AdamwScalars& s, float decay, const float (&g)[N], float (&p)[N], float (&m)[N],
-                                             float (&v)[N]) {
+__device__ __forceinline__ void adamw_moments(const AdamwScalars& s, const float (&g)[N], float (&m)[N], float (&v)[N]) {
     const float2 clip = make_float2(s.clip, s.clip), b1 = make_float2(s.b1, s.b1), b2 = make_float2(s.b2, s.b2);
     const float2 omb1 = make_float2(s.omb1, s.omb1), omb2 = make_float2(s.omb2, s.omb2);
-    const float2 first = make_float2(s.first, s.first), second = make_float2(s.second, s.second);
 #pragma unroll
     for (int k = 0; k < N; k += 2) {
         const float2 gg = mul2_rn(make_float2(g[k], g[k + 1]), clip);
@@ -225,6 +271,12 @@ __device__ __forceinline__ void adamw_update(const AdamwScalars& s, float decay,
         v[k] = vv.x;
         v[k + 1] = vv.y;
     }
+}
+// The parameters' step from the new moments
+template <int N>
+__device__ __forceinline__ void adamw_params(const AdamwScalars& s, float decay, const float (&m)[N], const float (&v)[N],
+                                             float (&p)[N]) {
+    const float2 first = make_float2(s.first, s.first), second = make_float2(s.second, s.second);
     auto params = [&](auto flush) {
 #pragma unroll
         for (int k = 0; k < N; k += 2) {
@@ -249,41 +301,49 @@ __global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ Adam
         const AdamwTensor& t = a.t[i];
         const int64_t e0 = (int64_t)(b - t.first) * kAdamwBlock + threadIdx.x * 4;
         const int64_t o0 = ((int64_t)a.at[i] + (b - t.first)) * kAdamwBlock + threadIdx.x * 4;
-        float p[2][4], g[2][4], m[2][4], v[2][4];
+        AdamwRaw<4> p[2], g[2], m[2], v[2];
         int have[2];
+        const int p_dtype = a.master ? AETH_DTYPE_F32 : t.p_dtype;
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
             const int64_t e = e0 + q * (kAdamwBlock / 2), o = o0 + q * (kAdamwBlock / 2);
             have[q] = (int)min(t.n - e, (int64_t)4);
             if (have[q] <= 0) continue;
-            adamw_load<4>(a.m, AETH_DTYPE_F32, true, o, 4, m[q]);
-            adamw_load<4>(a.v, AETH_DTYPE_F32, true, o, 4, v[q]);
-            if (a.master) adamw_load<4>(a.master, AETH_DTYPE_F32, true, o, 4, p[q]);
-            else adamw_load<4>(t.p, t.p_dtype, t.whole, e, have[q], p[q]);
-            adamw_load<4>(t.g, t.g_dtype, t.whole, e, have[q], g[q]);
+            m[q].load(a.m, AETH_DTYPE_F32, true, o, 4);
+            v[q].load(a.v, AETH_DTYPE_F32, true, o, 4);
+            p[q].load(a.master ? a.master : t.p, p_dtype, a.master || t.whole, a.master ? o : e, a.master ? 4 : have[q]);
+            g[q].load(t.g, t.g_dtype, t.whole, e, have[q]);
         }
         const float decay = t.decay ? s.decay : 0.0f;
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
             const int64_t e = e0 + q * (kAdamwBlock / 2), o = o0 + q * (kAdamwBlock / 2);
             if (have[q] <= 0) continue;
-            adamw_update<4>(s, decay, g[q], p[q], m[q], v[q]);
-            if (a.master) adamw_store<4>(a.master, AETH_DTYPE_F32, true, o, have[q], p[q]);
-            adamw_store<4>(t.p, t.p_dtype, t.whole, e, have[q], p[q]);
-            adamw_store<4>(a.m, AETH_DTYPE_F32, true, o, have[q], m[q]);
-            adamw_store<4>(a.v, AETH_DTYPE_F32, true, o, have[q], v[q]);
+            float pf[4], gf[4], mf[4], vf[4];
+            g[q].floats(t.g_dtype, gf);
+            m[q].floats(AETH_DTYPE_F32, mf);
+            v[q].floats(AETH_DTYPE_F32, vf);
+            p[q].floats(p_dtype, pf);
+            adamw_moments<4>(s, gf, mf, vf);
+            adamw_params<4>(s, decay, mf, vf, pf);
+            if (a.master) adamw_store<4>(a.master, AETH_DTYPE_F32, true, o, have[q], pf);
+            adamw_store<4>(t.p, t.p_dtype, t.whole, e, have[q], pf);
+            adamw_store<4>(a.m, AETH_DTYPE_F32, true, o, have[q], mf);
+            adamw_store<4>(a.v, AETH_DTYPE_F32, true, o, have[q], vf);
         }
     }
     adamw_count(a);
 }
 
-// Moments in 8 bits.  A CTA is four groups of 256 threads that share the maps
-// and the encode's tables (the layout of b2_adam_dyn_kernel: each map entry in
-// 32 copies, so that no lookup of a warp meets a bank conflict); a group takes a
-// block, a thread eight of its elements.
-constexpr int kAdamw8Threads = 1024;
+// Moments in 8 bits.  A CTA is five groups of 128 threads that share the maps and
+// the encode's tables (the layout of b2_adam_dyn_kernel: each map entry in 32
+// copies, so that no lookup of a warp meets a bank conflict); a group takes a
+// block, a thread eight elements of each of its halves.  A block's 16-bit gradients
+// and parameters and its codes are fetched while the one before it is encoded.
+constexpr int kAdamw8Groups = 5, kAdamw8Threads = 128 * kAdamw8Groups;
 constexpr int kAdamw8Dec = 256 * 256;
 constexpr int kAdamw8Shared = kAdamw8Dec + (2 * kDmapLutEntries + kDmapLutUEntries) * 4;
+constexpr int kAdamwHalf = kAdamwBlock / 2;
 
 template <int CAP>
 __global__ void __launch_bounds__(kAdamw8Threads, 1) adamw8_kernel(const __grid_constant__ AdamwArgs<CAP> a) {
@@ -292,57 +352,100 @@ __global__ void __launch_bounds__(kAdamw8Threads, 1) adamw8_kernel(const __grid_
     uint32_t* lut_s = reinterpret_cast<uint32_t*>(adamw_smem + kAdamw8Dec);
     uint32_t* lut_u = lut_s + 2 * kDmapLutEntries;
     __shared__ float corr[2];
-    __shared__ uint32_t red[4][2][2][8];  // [group][block parity][m, v][warp]: maxima, NaN above all
+    __shared__ uint32_t red[kAdamw8Groups][2][2][4];  // [group][block parity][m, v][warp]: maxima, NaN above all
     for (int i = threadIdx.x; i < 256 * 64; i += blockDim.x)
         dec[i] = (i & 63) < 32 ? c_dmap_signed[i >> 6] : c_dmap_unsigned[i >> 6];
     for (int i = threadIdx.x; i < 2 * kDmapLutEntries; i += blockDim.x) lut_s[i] = g_dmap_lut4_s[i];
     for (int i = threadIdx.x; i < kDmapLutUEntries; i += blockDim.x) lut_u[i] = g_dmap_lut4_u[i];
     const AdamwScalars s = adamw_scalars(a, corr);
-    const int grp = threadIdx.x >> 8, tid = threadIdx.x & 255, lane = tid & 31, warp = tid >> 5;
+    const int grp = threadIdx.x >> 7, tid = threadIdx.x & 127, lane = tid & 31, warp = tid >> 5;
     const uint32_t m1 = a.one << 1, m8 = a.one << 8, m15 = a.one << 15, m16 = a.one << 16;
     const uint32_t dec_base = smem_u32_addr(dec), off_m = (uint32_t)lane * 4u, off_v = off_m + 128u;
     const uint32_t adj_s = smem_u32_addr(lut_s) - (uint32_t)(kDmapLutExpLo << kDmapLutLog2P) * 4u;
     const uint32_t adj_u = smem_u32_addr(lut_u) - (uint32_t)(kDmapLutExpLo << kDmapLutULog2P) * 4u;
     int8_t *m_all = static_cast<int8_t*>(a.m), *v_all = static_cast<int8_t*>(a.v);
-    const int walker = blockIdx.x * 4 + grp;
-    int par = 0, i = a.start[walker];
-    for (int b = walker; b < a.blocks; b += gridDim.x * 4, par ^= 1) {
+    const int walker = blockIdx.x * kAdamw8Groups + grp, step = gridDim.x * kAdamw8Groups;
+    int i = a.start[walker], par = 0;
+    int64_t e = 0, o = 0, blk = 0;  // this thread's first element, in its tensor and among the moments; its block
+    bool p16 = false, g16 = false;  // fetched ahead
+    uint4 pw[2], gw[2];
+    uint2 qm[2], qv[2];
+    float sm = 0.0f, sv = 0.0f;
+    auto fetch = [&](int b) {
         if (b != walker) i = adamw_tensor(a, b, i);
         const AdamwTensor& t = a.t[i];
-        const int64_t blk = (int64_t)a.at[i] + (b - t.first);
-        const int64_t e = (int64_t)(b - t.first) * kAdamwBlock + tid * 8, o = blk * kAdamwBlock + tid * 8;
-        const int have = (int)max(min(t.n - e, (int64_t)8), (int64_t)0);
-        const float sm = a.m_scales[blk], sv = a.v_scales[blk];
-        const uint2 qm = *reinterpret_cast<const uint2*>(m_all + o), qv = *reinterpret_cast<const uint2*>(v_all + o);
-        float p[8], g[8], m[8], v[8], am = 0.0f, av = 0.0f;
-        adamw_load<8>(t.g, t.g_dtype, t.whole, e, have, g);
-        if (a.master) adamw_load<8>(a.master, AETH_DTYPE_F32, true, o, 8, p);
-        else adamw_load<8>(t.p, t.p_dtype, t.whole, e, have, p);
+        const int64_t at = (int64_t)(b - t.first);
+        blk = a.at[i] + at;
+        e = at * kAdamwBlock + tid * 8;
+        o = blk * kAdamwBlock + tid * 8;
+        const bool whole = t.whole && e + kAdamwHalf + 8 <= t.n;
+        p16 = whole && t.p_dtype != AETH_DTYPE_F32 && !a.master;
+        g16 = whole && t.g_dtype != AETH_DTYPE_F32;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            if (g16) gw[q] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(t.g) + e + q * kAdamwHalf);
+            if (p16) pw[q] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(t.p) + e + q * kAdamwHalf);
+            qm[q] = *reinterpret_cast<const uint2*>(m_all + o + q * kAdamwHalf);
+            qv[q] = *reinterpret_cast<const uint2*>(v_all + o + q * kAdamwHalf);
+        }
+        sm = a.m_scales[blk];
+        sv = a.v_scales[blk];
+    };
+    if (walker < a.blocks) fetch(walker);
+    for (int b = walker; b < a.blocks; b += step, par ^= 1) {
+        const AdamwTensor& t = a.t[i];
+        const int64_t oo = o, bb = blk;
+        float m[2][8], v[2][8], am = 0.0f, av = 0.0f;
         const float2 sm2 = make_float2(sm, sm), sv2 = make_float2(sv, sv);
+        const float decay = t.decay ? s.decay : 0.0f;
 #pragma unroll
-        for (int k = 0; k < 8; k += 2) {
-            const uint32_t sel = 0x5504u | ((uint32_t)(k & 3) << 4), wm = k < 4 ? qm.x : qm.y, wv = k < 4 ? qv.x : qv.y;
-            const float2 mm = mul2_rn(make_float2(__uint_as_float(lds_u32(dec_base + prmt(wm, off_m, sel))),
-                                                  __uint_as_float(lds_u32(dec_base + prmt(wm, off_m, sel + 0x10u)))), sm2);
-            const float2 vv = mul2_rn(make_float2(__uint_as_float(lds_u32(dec_base + prmt(wv, off_v, sel))),
-                                                  __uint_as_float(lds_u32(dec_base + prmt(wv, off_v, sel + 0x10u)))), sv2);
-            m[k] = mm.x;
-            m[k + 1] = mm.y;
-            v[k] = vv.x;
-            v[k + 1] = vv.y;
+        for (int q = 0; q < 2; ++q) {
+            const int64_t eq = e + q * kAdamwHalf;
+            const int have = (int)max(min(t.n - eq, (int64_t)8), (int64_t)0);
+            float g[8], p[8];
+            if (g16) {
+                const uint32_t w[4] = {gw[q].x, gw[q].y, gw[q].z, gw[q].w};
+                adamw_floats<8>(w, t.g_dtype, g);
+            } else {
+                adamw_load<8>(t.g, t.g_dtype, t.whole, eq, have, g);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k += 2) {
+                const uint32_t sel = 0x5504u | ((uint32_t)(k & 3) << 4), wm = k < 4 ? qm[q].x : qm[q].y, wv = k < 4 ? qv[q].x : qv[q].y;
+                const float2 mm = mul2_rn(make_float2(__uint_as_float(lds_u32(dec_base + prmt(wm, off_m, sel))),
+                                                      __uint_as_float(lds_u32(dec_base + prmt(wm, off_m, sel + 0x10u)))), sm2);
+                const float2 vv = mul2_rn(make_float2(__uint_as_float(lds_u32(dec_base + prmt(wv, off_v, sel))),
+                                                      __uint_as_float(lds_u32(dec_base + prmt(wv, off_v, sel + 0x10u)))), sv2);
+                m[q][k] = mm.x;
+                m[q][k + 1] = mm.y;
+                v[q][k] = vv.x;
+                v[q][k + 1] = vv.y;
+            }
+            adamw_moments<8>(s, g, m[q], v[q]);
+            if (p16) {
+                uint32_t w[4] = {pw[q].x, pw[q].y, pw[q].z, pw[q].w};
+                adamw_floats<8>(w, t.p_dtype, p);
+                adamw_params<8>(s, decay, m[q], v[q], p);
+                adamw_words<8>(p, t.p_dtype, w);
+                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(t.p) + eq) = make_uint4(w[0], w[1], w[2], w[3]);
+            } else {
+                if (a.master) adamw_load<8>(a.master, AETH_DTYPE_F32, true, o + q * kAdamwHalf, 8, p);
+                else adamw_load<8>(t.p, t.p_dtype, t.whole, eq, have, p);
+                adamw_params<8>(s, decay, m[q], v[q], p);
+                if (a.master) adamw_store<8>(a.master, AETH_DTYPE_F32, true, o + q * kAdamwHalf, have, p);
+                adamw_store<8>(t.p, t.p_dtype, t.whole, eq, have, p);
+            }
+            if (have < 8)  // past the tensor's end: codes of zero
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (k >= have) m[q][k] = v[q][k] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; k += 2) {
+                am = fmax3_nan(am, fabsf(m[q][k]), fabsf(m[q][k + 1]));
+                av = fmax3_nan(av, v[q][k], v[q][k + 1]);
+            }
         }
-        adamw_update<8>(s, t.decay ? s.decay : 0.0f, g, p, m, v);
-        if (a.master) adamw_store<8>(a.master, AETH_DTYPE_F32, true, o, have, p);
-        adamw_store<8>(t.p, t.p_dtype, t.whole, e, have, p);
-        if (have < 8)  // past the tensor's end: codes of zero
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (k >= have) m[k] = v[k] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 8; k += 2) {
-            am = fmax3_nan(am, fabsf(m[k]), fabsf(m[k + 1]));
-            av = fmax3_nan(av, v[k], v[k + 1]);
-        }
+        if (b + step < a.blocks) fetch(b + step);
         // non-negative or NaN (0x7fffffff): their bits order as they do
         const uint32_t wm = __reduce_max_sync(0xffffffffu, __float_as_uint(am));
         const uint32_t wv = __reduce_max_sync(0xffffffffu, __float_as_uint(av));
@@ -350,34 +453,39 @@ __global__ void __launch_bounds__(kAdamw8Threads, 1) adamw8_kernel(const __grid_
             red[grp][par][0][warp] = wm;
             red[grp][par][1][warp] = wv;
         }
-        group_bar(1 + grp);  // the parity's slots are written again two blocks later
-        const uint32_t bm = __reduce_max_sync(0xffffffffu, red[grp][par][0][lane & 7]);
-        const uint32_t bv = __reduce_max_sync(0xffffffffu, red[grp][par][1][lane & 7]);
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + grp) : "memory");  // the parity's slots are written again two blocks later
+        const uint32_t* rm = red[grp][par][0];
+        const uint32_t* rv = red[grp][par][1];
+        const uint32_t bm = max(max(rm[0], rm[1]), max(rm[2], rm[3])), bv = max(max(rv[0], rv[1]), max(rv[2], rv[3]));
         const bool bad_m = bm >= 0x7f800000u, bad_v = bv >= 0x7f800000u;
         const float nm = bad_m || bm < 0x00800000u ? 0.0f : __uint_as_float(bm);
         const float nv = bad_v || bv < 0x00800000u ? 0.0f : __uint_as_float(bv);
+        // 0: codes of zero (of NaN too: the scale says NaN)
         const float im = dyn_inv(nm), iv = dyn_inv(nv);
-        // im = 0: codes of zero (of NaN too: the scale says NaN)
-        uint32_t cm[8], cv[8];
         const float2 im2 = make_float2(im, im), iv2 = make_float2(iv, iv);
 #pragma unroll
-        for (int k = 0; k < 8; k += 2) {
-            const float2 mm = mul2_rn(make_float2(m[k], m[k + 1]), im2), vv = mul2_rn(make_float2(v[k], v[k + 1]), iv2);
-            cm[k] = dmap_enc4_s(adj_s, mm.x, m1, m8, m15);
-            cm[k + 1] = dmap_enc4_s(adj_s, mm.y, m1, m8, m15);
-            cv[k] = dmap_enc4_u(adj_u, vv.x, m8, m16);
-            cv[k + 1] = dmap_enc4_u(adj_u, vv.y, m8, m16);
+        for (int q = 0; q < 2; ++q) {
+            uint32_t cm[8], cv[8];
+#pragma unroll
+            for (int k = 0; k < 8; k += 2) {
+                const float2 mm = mul2_rn(make_float2(m[q][k], m[q][k + 1]), im2);
+                const float2 vv = mul2_rn(make_float2(v[q][k], v[q][k + 1]), iv2);
+                cm[k] = dmap_enc4_s(adj_s, mm.x, m1, m8, m15);
+                cm[k + 1] = dmap_enc4_s(adj_s, mm.y, m1, m8, m15);
+                cv[k] = dmap_enc4_u(adj_u, vv.x, m8, m16);
+                cv[k + 1] = dmap_enc4_u(adj_u, vv.y, m8, m16);
+            }
+            uint2 om, ov;
+            om.x = prmt(prmt(cm[0], cm[1], 0x3340u), prmt(cm[2], cm[3], 0x3340u), 0x5410u);
+            om.y = prmt(prmt(cm[4], cm[5], 0x3340u), prmt(cm[6], cm[7], 0x3340u), 0x5410u);
+            ov.x = prmt(prmt(cv[0], cv[1], 0x3340u), prmt(cv[2], cv[3], 0x3340u), 0x5410u);
+            ov.y = prmt(prmt(cv[4], cv[5], 0x3340u), prmt(cv[6], cv[7], 0x3340u), 0x5410u);
+            *reinterpret_cast<uint2*>(m_all + oo + q * kAdamwHalf) = om;
+            *reinterpret_cast<uint2*>(v_all + oo + q * kAdamwHalf) = ov;
         }
-        uint2 om, ov;
-        om.x = prmt(prmt(cm[0], cm[1], 0x3340u), prmt(cm[2], cm[3], 0x3340u), 0x5410u);
-        om.y = prmt(prmt(cm[4], cm[5], 0x3340u), prmt(cm[6], cm[7], 0x3340u), 0x5410u);
-        ov.x = prmt(prmt(cv[0], cv[1], 0x3340u), prmt(cv[2], cv[3], 0x3340u), 0x5410u);
-        ov.y = prmt(prmt(cv[4], cv[5], 0x3340u), prmt(cv[6], cv[7], 0x3340u), 0x5410u);
-        *reinterpret_cast<uint2*>(m_all + o) = om;
-        *reinterpret_cast<uint2*>(v_all + o) = ov;
         if (tid == 0) {
-            a.m_scales[blk] = bad_m ? __int_as_float(0x7fc00000) : nm;
-            a.v_scales[blk] = bad_v ? __int_as_float(0x7fc00000) : nv;
+            a.m_scales[bb] = bad_m ? __int_as_float(0x7fc00000) : nm;
+            a.v_scales[bb] = bad_v ? __int_as_float(0x7fc00000) : nv;
         }
     }
     adamw_count(a);

@@ -2433,9 +2433,9 @@ namespace {
 
 template <int CAP>
 int adamw_launch(AdamwArgs<CAP>& a, int bits, cudaStream_t st) {
-    const int ctas = std::max(bits == 8 ? std::min((a.blocks + 3) / 4, std::min(num_sms(), kAdamwStarts / 4))
-                                        : std::min(a.blocks, std::min(6 * num_sms(), kAdamwStarts)), 1);
-    for (int w = 0, i = 0; w < ctas * (bits == 8 ? 4 : 1); ++w) {
+    const int walkers = bits == 8 ? kAdamw8Groups : 1, per_sm = bits == 8 ? 1 : 6;  // of a CTA, CTAs of an SM
+    const int ctas = std::max(std::min((a.blocks + walkers - 1) / walkers, std::min(per_sm * num_sms(), kAdamwStarts / walkers)), 1);
+    for (int w = 0, i = 0; w < ctas * walkers; ++w) {
         while (i + 1 < a.count && a.t[i + 1].first <= w) ++i;
         a.start[w] = (uint16_t)i;
     }
