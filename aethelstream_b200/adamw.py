@@ -25,8 +25,8 @@ ADAMW_BLOCK = 2048  # elements that share a scale; a tensor's moments start on a
 _lib = L.load()
 
 
-_numel, _data_ptr, _contiguous = torch.Tensor.numel, torch.Tensor.data_ptr, torch.Tensor.is_contiguous
-_inference, _get_device, _shape, _dtype = torch.Tensor.is_inference, torch.Tensor.get_device, attrgetter("shape"), attrgetter("dtype")
+_data_ptr, _contiguous, _get_device = torch.Tensor.data_ptr, torch.Tensor.is_contiguous, torch.Tensor.get_device
+_shape, _dtype = attrgetter("shape"), attrgetter("dtype")
 
 
 def _kinds(what: str, tensors, dev: int) -> bytes:
@@ -132,7 +132,8 @@ def adamw_step(params, grads, state: AdamWState, config: AdamWConfig | None = No
     gkinds = _kinds(what, there, dev)
     if not all(map(_contiguous, params)):
         raise ValueError(f"{what}: the tensors must be contiguous")
-    if list(map(_shape, here)) != list(map(_shape, there)):
+    shapes = list(map(_shape, params))
+    if (list(map(_shape, here)) if some else shapes) != list(map(_shape, there)):
         raise ValueError(f"{what}: a gradient must have its tensor's shape")
     if not all(map(_contiguous, there)):
         there = [g.contiguous() for g in there]
@@ -141,7 +142,7 @@ def adamw_step(params, grads, state: AdamWState, config: AdamWConfig | None = No
         left = iter(zip(g_ptr, gkinds))
         each = [(0, 0) if g is None else next(left) for g in grads]
         g_ptr, gkinds = array("Q", [x for x, _ in each]), bytes(k for _, k in each)
-    p_ptr, sizes = array("Q", map(_data_ptr, params)), array("q", map(_numel, params))
+    p_ptr, sizes = array("Q", map(_data_ptr, params)), array("q", map(torch.Size.numel, shapes))
     blocks = sum([-(-n // ADAMW_BLOCK) for n in sizes])
     c = _state(what, state, dev)
     if blocks != c.blocks:
@@ -155,8 +156,7 @@ def adamw_step(params, grads, state: AdamWState, config: AdamWConfig | None = No
         raise ValueError(f"{what}: tensors that the step writes share memory")
     if st:
         L.check(st, "aeth_adamw_step")
-    torch.autograd.graph.increment_version(params if not any(map(_inference, params)) else
-                                           [p for p in params if not p.is_inference()])
+    torch.autograd.graph.increment_version(params)  # a backward pass that saved one of them is told
 
 
 def adamw_moments(state: AdamWState) -> tuple[torch.Tensor, torch.Tensor]:

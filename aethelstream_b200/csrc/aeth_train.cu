@@ -292,15 +292,15 @@ struct ProbsPlan {
     }
 };
 
-// A CTA's logits beside the hidden states in shared memory.
+// A CTA's logits, and two bytes for each, beside the hidden states in shared memory.
 constexpr int kVecLogitShared = 96 * 1024;
 int vec_slots(int64_t vocab) {
     const int each = 2 * kHeadVecThreads / 32;
     return (int)((vocab + each * num_sms() - 1) / (each * num_sms())) * each;
 }
 bool vec_probs_fits(int64_t n, int64_t d, int64_t vocab) {
-    return head_vec_fits(n, d) && vocab <= (int64_t)num_sms() * (kVecLogitShared / (4 * kHeadVecTokens)) &&
-           n * vec_slots(vocab) * 4 <= kVecLogitShared;
+    return head_vec_fits(n, d) && num_sms() <= kHeadVecJoin && vocab <= (int64_t)num_sms() * kVecLogitShared / 8 &&
+           n * vec_slots(vocab) * 6 <= kVecLogitShared;
 }
 
 struct ProbsWork {
@@ -330,12 +330,12 @@ int vec_probs(const HeadVecProbs& a, int64_t n, int ctas, const HeadProbsOut& ou
     AETH_TRY(runtime_for_current(&rt));
     auto kern = n == 1 ? head_vec_probs_kernel<BF16, 1> : n == 2 ? head_vec_probs_kernel<BF16, 2>
               : n == 3 ? head_vec_probs_kernel<BF16, 3> : head_vec_probs_kernel<BF16, 4>;
-    const int smem = (int)(n * (up(a.v.d, 8) * 2 + a.slots * 4));
+    const int smem = (int)(n * (up(a.v.d, 8) * 2 + a.slots * 6));
     static std::atomic<bool> allowed[kHeadVecTokens][kMaxDevices] = {};
     AETH_TRY(allow_shared(kern, kHeadVecShared + kVecLogitShared, allowed[n - 1]));
     kern<<<ctas, kHeadVecThreads, smem, st>>>(a);
     AETH_LAUNCH_CHECK();
-    AETH_CUDA(launch_after(head_vec_probs_join_kernel, dim3((unsigned)n), dim3(32), 0, st, 1, a, ctas, out, rt->err_word));
+    AETH_CUDA(launch_after(head_vec_probs_join_kernel, dim3((unsigned)n), dim3(kHeadVecJoin), 0, st, 1, a, ctas, out, rt->err_word));
     return AETH_OK;
 }
 

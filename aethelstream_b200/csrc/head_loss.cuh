@@ -508,8 +508,9 @@ __device__ __forceinline__ float2 head_pair(uint32_t w) {
 }
 
 // Stages the hidden states ([token][eight of features]), calls begin() behind a
-// barrier and then logit(token, entry, its logit) with all lanes of a warp, for
-// the entries that are the warp's: two in turn, from 2 (CTA's warps + warp) on.
+// barrier and then logit(token, entry, its place, its logit) with all lanes of a
+// warp, for the entries that are the warp's: two in turn, from 2 (CTA's warps +
+// warp) on.  place: the entry's among the CTA's.
 template <bool BF16, int NT, typename Begin, typename Logit>
 __device__ __forceinline__ void head_vec_walk(const HeadVec& a, uint4* head_sh, Begin begin, Logit logit) {
     constexpr int R = 2, U = 8;  // entries a warp, loads in flight an entry
@@ -528,7 +529,8 @@ __device__ __forceinline__ void head_vec_walk(const HeadVec& a, uint4* head_sh, 
     __syncthreads();
     pdl_trigger();
     const int warps = gridDim.x * (kHeadVecThreads / 32);
-    for (int64_t v0 = first; v0 < a.vocab; v0 += (int64_t)R * warps) {
+    int place = R * warp;
+    for (int64_t v0 = first; v0 < a.vocab; v0 += (int64_t)R * warps, place += R * kHeadVecThreads / 32) {
         const uint16_t* row[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) row[r] = a.weight + min(v0 + r, (int64_t)a.vocab - 1) * a.ld_w;
@@ -578,7 +580,7 @@ __device__ __forceinline__ void head_vec_walk(const HeadVec& a, uint4* head_sh, 
                 float x = acc[r][t].x + acc[r][t].y;
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-                if (v0 + r < a.vocab) logit(t, (int)(v0 + r), x);
+                if (v0 + r < a.vocab) logit(t, (int)(v0 + r), place + r, x);
             }
     }
 }
@@ -604,7 +606,7 @@ __global__ void __launch_bounds__(kHeadVecThreads, 1) head_vec_kernel(const Head
                 st[t] = make_float2(-INFINITY, 0.0f);
             }
         },
-        [&](int t, int entry, float x) {
+        [&](int t, int entry, int, float x) {
             st[t] = head_join(st[t], make_float2(x * kLog2e, 1.0f));
             if (lab[t] == entry && lane == 0) a.label_logit[t] = x;
         });
