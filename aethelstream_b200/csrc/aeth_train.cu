@@ -287,7 +287,7 @@ struct ProbsPlan {
         const int64_t tiles = (vocab + 255) / 256, fit = std::max<int64_t>(kHeadPieceBytes / (1024 * head.n_pad), 1);
         const int64_t pieces = (tiles + fit - 1) / fit;
         piece = std::min(256 * ((tiles + pieces - 1) / pieces), vocab);
-        ld = up(piece, 4);
+        ld = up(piece, 8);
         ranges = 2 * (int)tiles;
     }
 };
@@ -319,7 +319,8 @@ struct ProbsWork {
         part = c.take<HeadSums>(vec ? (int64_t)num_sms() * n : p.head.n_pad * p.ranges);
         cand = c.take<float2>(vec ? (int64_t)num_sms() * n * p.top : 0);
         best = c.take<float2>(p.top > 0 ? p.head.n_pad * 32 : 0);
-        logits = c.take<float>(p.top > 0 ? p.head.n_pad * p.ld : 0);
+        const uintptr_t at = reinterpret_cast<uintptr_t>(c.take<float>(p.top > 0 ? p.head.n_pad * p.ld + 8 : 0));
+        logits = reinterpret_cast<float*>((at + 31) & ~(uintptr_t)31);  // rows are written in sectors; a workspace starts on 16 bytes
         bytes = c.used;
     }
 };

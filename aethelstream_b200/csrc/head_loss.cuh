@@ -299,8 +299,13 @@ struct HeadLossSums {
     float2* part;  // [range][row]
     int64_t ld_part;
     __device__ static Sum none() { return make_float2(-INFINITY, 0.0f); }
+    // what a row's 128 logits are added to, the first `left` of which exist
+    __device__ static Sum before(const float (&)[128], int) { return none(); }
+    // whether a row's sums are good, or its logits are added once more the other way
+    __device__ static bool good(Sum) { return true; }
     __device__ static Sum join(Sum a, Sum b) { return head_join(a, b); }
     __device__ __forceinline__ static void add32(const float (&v)[32], int left, Sum& st) { head_stats32(v, left, st); }
+    __device__ __forceinline__ static void again32(const float (&v)[32], int left, Sum& st) { head_stats32(v, left, st); }
     __device__ __forceinline__ void put(int range, int row, Sum x) const { part[(int64_t)range * ld_part + row] = x; }
     // 32 columns of the warp's rows, and 32 entries of a token (none of them kept)
     __device__ __forceinline__ void rows(const PairTile&, const float (&)[32], int) const {}
@@ -322,10 +327,11 @@ struct HeadStats {
         const int row = t.row0 + t.lane;
         const bool in = row < t.M;
         const int at = in ? lab[row] - v0 - t.col0 - t.c_begin : -1;
-        typename Sums::Sum st = Sums::none();
+        const int all = min(t.c_end, t.N - t.col0) - t.c_begin;  // columns that exist
+        typename Sums::Sum st = Sums::before(acc, all);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            const int left = min(t.c_end, t.N - t.col0) - t.c_begin - 32 * c;  // columns of this chunk that exist
+            const int left = all - 32 * c;
             if (left > 0) {
                 float v[32];
                 head_slice(acc, c, v);
@@ -333,6 +339,17 @@ struct HeadStats {
                 head_label32(v, at - 32 * c, label_logit + row);
                 sums.rows(t, v, t.c_begin + 32 * c);
             }
+        }
+        if (__any_sync(0xffffffffu, !Sums::good(st))) {
+            typename Sums::Sum other = Sums::none();
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (all - 32 * c > 0) {
+                    float v[32];
+                    head_slice(acc, c, v);
+                    Sums::again32(v, all - 32 * c, other);
+                }
+            if (!Sums::good(st)) st = other;
         }
         if (in) sums.put(2 * t.n_tile + t.half, row, st);
     }
@@ -368,7 +385,7 @@ struct HeadStatsT {
                 float v[32];
                 head_slice(acc, c, v);
                 pair_transpose(t, v);
-                Sums::add32(v, left, st[c]);
+                Sums::again32(v, left, st[c]);
                 const int k = token < t.N ? lab[token] - v0 - t.row0 : -1;
                 head_label32(v, k < left ? k : -1, label_logit + token);
                 if (token < t.N) sums.token(token, t.row0, left, v);

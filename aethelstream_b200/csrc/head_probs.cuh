@@ -15,9 +15,9 @@
 // entries each) whose maxima are the best, the lower range before the other on
 // equal ones: each of these holds an entry before any of another range.  The
 // product therefore leaves its logits in fp32, a piece of the vocabulary at a time
-// (256 MiB), and a warp a row reads the maxima of a piece and then those ranges
-// alone.  It keeps the best so far in its lanes, one each, which bounds k by 32.
-// Equal logits: the lower entry first.
+// (256 MiB), and a warp a row reads the maxima of a piece and then such ranges
+// alone (head_top).  The best so far lie in its lanes, one each, which bounds k by
+// 32.  Equal logits: the lower entry first.
 //
 // Gradient of a log p_y + b entropy, with q = log p:
 //   G_v = a 1[v = y] - p_v (a + b (q_v + entropy))
@@ -60,7 +60,7 @@ __device__ __forceinline__ HeadSums head_shuffle(const HeadSums& a, int o) {
 __device__ __forceinline__ float head_lse3(const HeadSums& a) { return head_base(a.m) + logf(a.s); }
 __device__ __forceinline__ float head_entropy(const HeadSums& a) { return logf(a.s) - kLn2 * (a.u / a.s); }
 
-// Joins 32 logits, the first `left` of them.
+// Joins 32 logits, the first `left` of them, whatever they are.
 __device__ __forceinline__ void head_sums32(const float (&v)[32], int left, HeadSums& st) {
     float m = st.m;
 #pragma unroll
@@ -84,6 +84,37 @@ __device__ __forceinline__ void head_sums32(const float (&v)[32], int left, Head
     }
     st = {m, s0 + s1, u0 + u1, 0.0f};
 }
+// The same in two and a half instructions a logit, against a maximum that is known
+// (`unused` holds it in units of log2): fused multiply-adds of pairs.  Its rounding
+// is one factor of all sums, which head_fast_end takes out.  A logit of -infinity
+// makes u NaN and one above 2^127 / log2 e the maximum infinite; those rows go the
+// other way.
+__device__ __forceinline__ void head_fast32(const float (&v)[32], int left, HeadSums& st) {
+    const float2 l2 = make_float2(kLog2e, kLog2e), nb = make_float2(-st.unused, -st.unused);
+    float2 s = make_float2(st.s, 0.0f), u = make_float2(st.u, 0.0f);
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+        const float2 x = fma2_rn(make_float2(v[i], v[i + 1]), l2, nb);
+        const float2 e = make_float2(left >= 32 || i < left ? ex2(x.x) : 0.0f, left >= 32 || i + 1 < left ? ex2(x.y) : 0.0f);
+        s = add2_rn(s, e);
+        u = fma2_rn(e, x, u);
+    }
+    st.s = s.x + s.y;
+    st.u = u.x + u.y;
+}
+__device__ __forceinline__ HeadSums head_fast_begin(const float (&acc)[128], int left) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 128; i += 2)
+        m = left >= 128 ? fmax3(m, acc[i], acc[i + 1]) : fmaxf(i < left ? fmaxf(m, acc[i]) : m, i + 1 < left ? acc[i + 1] : m);
+    return {m, 0.0f, 0.0f, m * kLog2e};
+}
+__device__ __forceinline__ bool head_fast_good(const HeadSums& st) { return fabsf(st.unused) < 1e38f && st.u == st.u; }
+// Takes the base's rounding d = m log2 e - base out: s 2^-d and, of x - d, u.
+__device__ __forceinline__ HeadSums head_fast_end(const HeadSums& st) {
+    const float d = fmaf(st.m, kLog2e, -st.unused), w = fmaf(-d, kLn2, 1.0f);
+    return {st.m, st.s * w, fmaf(-st.s, d, st.u) * w, 0.0f};
+}
 
 // What the product's epilogues (HeadStats, HeadStatsT) keep: the sums and, with
 // TOP, the logits.
@@ -92,22 +123,34 @@ struct HeadProbsSums {
     using Sum = HeadSums;
     HeadSums* part;  // [row][range]; TOP: ranges of 128 entries, of all pieces
     int ranges, first;
-    float* logits;  // [row][entry of the piece], a multiple of 4 of them
+    float* logits;  // [row][entry of the piece], a multiple of 8 of them
     int64_t ld;
     __device__ static Sum none() { return head_no_sums(); }
     __device__ static Sum join(const Sum& a, const Sum& b) { return head_join3(a, b); }
-    __device__ __forceinline__ static void add32(const float (&v)[32], int left, Sum& st) { head_sums32(v, left, st); }
-    __device__ __forceinline__ void put(int range, int row, const Sum& x) const { part[(int64_t)row * ranges + first + range] = x; }
+    __device__ __forceinline__ static Sum before(const float (&acc)[128], int left) { return head_fast_begin(acc, left); }
+    __device__ __forceinline__ static void add32(const float (&v)[32], int left, Sum& st) { head_fast32(v, left, st); }
+    __device__ static bool good(const Sum& st) { return head_fast_good(st); }
+    __device__ __forceinline__ static void again32(const float (&v)[32], int left, Sum& st) { head_sums32(v, left, st); }
+    __device__ __forceinline__ void put(int range, int row, const Sum& x) const {
+        part[(int64_t)row * ranges + first + range] = x.unused != 0.0f ? head_fast_end(x) : x;
+    }
+    // A row's 32 logits go out from their thread, a sector (eight) at a time: through
+    // shared memory, in whole lines, they took the epilogue so long that the products
+    // waited for it.
+    __device__ __forceinline__ void store(float* o, const float (&v)[32], int left) const {
+#pragma unroll
+        for (int i = 0; i < 32; i += 8)
+            if (i < left)  // ld is a multiple of 8
+                asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(o + i), "f"(v[i]), "f"(v[i + 1]),
+                             "f"(v[i + 2]), "f"(v[i + 3]), "f"(v[i + 4]), "f"(v[i + 5]), "f"(v[i + 6]), "f"(v[i + 7])
+                             : "memory");
+    }
     __device__ __forceinline__ void rows(const PairTile& t, const float (&v)[32], int c) const {
-        if (TOP && t.row0 < t.M)
-            pair_store32(t, v, c, logits + (int64_t)t.row0 * ld + t.col0, ld, t.M - t.row0, (int)min((int64_t)256, ld - t.col0), true);
+        const int row = t.row0 + t.lane, col = t.col0 + c;
+        if (TOP && row < t.M) store(logits + (int64_t)row * ld + col, v, t.N - col);
     }
     __device__ __forceinline__ void token(int token, int entry, int left, const float (&v)[32]) const {
-        if (!TOP) return;
-        float4* o = reinterpret_cast<float4*>(logits + (int64_t)token * ld + entry);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (4 * i < left) o[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        if (TOP) store(logits + (int64_t)token * ld + entry, v, left);
     }
 };
 
@@ -183,53 +226,31 @@ __device__ __forceinline__ void head_probs_write(const HeadProbsOut& a, int64_t 
     }
 }
 
-template <bool TOP>
-__global__ void __launch_bounds__(256) head_probs_kernel(const HeadProbsOut a) {
+// Joins a row's ranges, by a warp: eight loads of a lane in flight, each brought to
+// the largest maximum so far.
+__device__ __forceinline__ HeadSums head_join_ranges(const HeadSums* p, int ranges) {
     const int lane = threadIdx.x & 31;
-    pdl_wait();
-    pdl_trigger();
-    for (int64_t t = blockIdx.x * 8ll + (threadIdx.x >> 5); t < a.n; t += gridDim.x * 8ll) {
-        const int row = a.pos[t];
-        HeadBest best = HeadBest::none();
-        if (TOP && row >= 0) {
-            if (!a.is_first) {
-                const float2 b = a.best[(int64_t)row * 32 + lane];
-                best = {b.x, __float_as_int(b.y)};
-            }
-            // the ranges whose maxima are the best, and then their entries
-            HeadBest at = HeadBest::none();
-            const HeadSums* p = a.part + (int64_t)row * a.ranges + a.first;
-            for (int r0 = 0; r0 < a.count; r0 += 32) {
-                const int r = r0 + lane;
-                const float m = r < a.count ? p[r].m : -INFINITY;
-                at.offer(m, r < a.count ? r : 0x7fffffff, a.top);
-            }
-            const float* s = a.logits + (int64_t)row * a.ld;
-            for (int k = 0; k < a.top; ++k) {
-                const float m = __shfl_sync(0xffffffffu, at.v, k);
-                const int r = __shfl_sync(0xffffffffu, at.i, k);
-                const float worst = __shfl_sync(0xffffffffu, best.v, a.top - 1);
-                const int worst_at = __shfl_sync(0xffffffffu, best.i, a.top - 1);
-                if (r == 0x7fffffff || !HeadBest::before(m, a.v0 + r * kHeadRange, worst, worst_at)) break;
-                const int e0 = r * kHeadRange + 4 * lane;
-                const float4 v = e0 < a.vp ? *reinterpret_cast<const float4*>(s + e0) : make_float4(0, 0, 0, 0);
-                const float x[4] = {v.x, v.y, v.z, v.w};
+    HeadSums x = head_no_sums();
+    for (int r0 = 0; r0 < ranges; r0 += 256) {
+        HeadSums y[8];
+        float m = x.m;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    best.offer(e0 + i < a.vp ? x[i] : -INFINITY, e0 + i < a.vp ? a.v0 + e0 + i : 0x7fffffff, a.top);
-            }
-            if (!a.is_last) a.best[(int64_t)row * 32 + lane] = make_float2(best.v, __int_as_float(best.i));
+        for (int j = 0; j < 8; ++j) {
+            const int r = r0 + 32 * j + lane;
+            y[j] = r < ranges ? p[r] : head_no_sums();
         }
-        if (TOP && !a.is_last) continue;
-        HeadSums x = head_no_sums();
-        if (row >= 0) {
-            const HeadSums* p = a.part + (int64_t)row * a.ranges;
-            for (int r = lane; r < a.ranges; r += 32) x = head_join3(x, p[r]);
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) x = head_join3(x, head_shuffle(x, o));
-        }
-        head_probs_write(a, t, lane, row == kHeadBad, row >= 0, x, row >= 0 ? a.label_logit[row] : 0.0f, best);
+        for (int j = 0; j < 8; ++j) m = fmaxf(m, y[j].m);
+        const float base = head_base(m);
+        float s = 0.0f, u = 0.0f;
+        head_rebase(x, base, s, u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) head_rebase(y[j], base, s, u);
+        x = {m, s, u, 0.0f};
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x = head_join3(x, head_shuffle(x, o));
+    return x;
 }
 
 // The place of (x, i) among values in shared memory: how many come before it.
@@ -242,6 +263,182 @@ __device__ __forceinline__ int head_place(float x, int i, int count, At at) {
         place += HeadBest::before(y.x, __float_as_int(y.y), x, i) ? 1 : 0;
     }
     return place;
+}
+
+// A float's place in the order of floats
+__device__ __forceinline__ uint32_t head_key(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float head_unkey(uint32_t k) { return __uint_as_float(k ^ ((uint32_t)((int32_t)~k >> 31) | 0x80000000u)); }
+
+// What a warp needs to take a row's best entries of a piece.
+constexpr int kTopRanges = 256, kTopList = 128;
+struct HeadTopShared {
+    float2 list[kTopList], out[kHeadTop];
+    uint16_t ranges[kTopRanges];
+    int count;
+};
+
+// The slow way, whatever the logits: one range and one entry after the other.
+__device__ __noinline__ HeadBest head_top_slow(const HeadProbsOut& a, const HeadSums* p, const float* s, HeadBest best) {
+    const int lane = threadIdx.x & 31;
+    HeadBest at = HeadBest::none();
+    for (int r0 = 0; r0 < a.count; r0 += 32) {
+        const int r = r0 + lane;
+        at.offer(r < a.count ? p[r].m : -INFINITY, r < a.count ? r : 0x7fffffff, a.top);
+    }
+    for (int k = 0; k < a.top; ++k) {
+        const float m = __shfl_sync(0xffffffffu, at.v, k);
+        const int r = __shfl_sync(0xffffffffu, at.i, k);
+        if (r == 0x7fffffff || !HeadBest::before(m, a.v0 + r * kHeadRange, __shfl_sync(0xffffffffu, best.v, a.top - 1),
+                                                 __shfl_sync(0xffffffffu, best.i, a.top - 1)))
+            break;
+        const int e0 = r * kHeadRange + 4 * lane;
+        const float4 v = e0 < a.vp ? *reinterpret_cast<const float4*>(s + e0) : make_float4(0, 0, 0, 0);
+        const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            best.offer(e0 + i < a.vp ? x[i] : -INFINITY, e0 + i < a.vp ? a.v0 + e0 + i : 0x7fffffff, a.top);
+    }
+    return best;
+}
+
+// A row's best entries, of a piece and those before it: a warp, lane i gets the
+// i-th.  A bound that `top` entries reach comes from the maxima of 256 groups (of
+// ranges, or of entries where there are few ranges), by halving the interval that
+// it lies in; the ranges whose maxima reach it are read, eight at a time, and the
+// entries that do are counted into their places.  With equal logits by the hundred,
+// which a bound cannot part, the slow way.
+__device__ __forceinline__ HeadBest head_top(const HeadProbsOut& a, int row, HeadBest best, HeadTopShared& sh) {
+    const int lane = threadIdx.x & 31;
+    const HeadSums* p = a.part + (int64_t)row * a.ranges + a.first;
+    const float* s = a.logits + (int64_t)row * a.ld;
+    const bool few = 2 * a.count < 3 * a.top;
+    uint32_t key[8] = {};
+    if (few) {
+        for (int e0 = 0; e0 < a.vp; e0 += 1024)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int e = e0 + 128 * j + 4 * lane;
+                if (e >= a.vp) continue;
+                const float4 v = *reinterpret_cast<const float4*>(s + e);
+                float m = fmaxf(-INFINITY, v.x);
+                if (e + 1 < a.vp) m = fmaxf(m, v.y);
+                if (e + 2 < a.vp) m = fmaxf(m, v.z);
+                if (e + 3 < a.vp) m = fmaxf(m, v.w);
+                key[j] = max(key[j], head_key(m));
+            }
+    } else {
+        for (int r0 = 0; r0 < a.count; r0 += 256)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int r = r0 + 32 * j + lane;
+                if (r < a.count) key[j] = max(key[j], head_key(p[r].m));
+            }
+    }
+    uint32_t most = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) most = max(most, key[j]);
+    // the least of the lanes' maxima is reached by 32 of them
+    uint32_t lo = __reduce_min_sync(0xffffffffu, most), hi = __reduce_max_sync(0xffffffffu, most);
+    for (int i = 0; i < 14 && lo < hi; ++i) {
+        const uint32_t mid = hi - (hi - lo) / 2;
+        int n = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) n += key[j] >= mid ? 1 : 0;
+        n = __reduce_add_sync(0xffffffffu, n);
+        if (n >= a.top) lo = mid;
+        else hi = mid - 1;
+        if (n == a.top) break;
+    }
+    const int last = __shfl_sync(0xffffffffu, best.i, a.top - 1);
+    const float last_v = __shfl_sync(0xffffffffu, best.v, a.top - 1);
+    if (last != 0x7fffffff) lo = max(lo, head_key(last_v));
+    const float bound = lo <= head_key(-INFINITY) ? -INFINITY : head_unkey(lo);  // below: no float, and no group either
+    int count = a.count;
+    if (!few) {
+        count = 0;
+        for (int r0 = 0; r0 < a.count; r0 += 256) {
+            bool in[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int r = r0 + 32 * j + lane;
+                in[j] = r < a.count && (a.count <= 256 ? head_unkey(key[j]) : p[r].m) >= bound;  // 256: a group is a range
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t who = __ballot_sync(0xffffffffu, in[j]);
+                const int at = count + __popc(who & ((1u << lane) - 1));
+                if (in[j] && at < kTopRanges) sh.ranges[at] = (uint16_t)(r0 + 32 * j + lane);
+                count += __popc(who);
+            }
+        }
+        if (count > kTopRanges) return head_top_slow(a, p, s, best);
+    }
+    sh.out[lane] = make_float2(-INFINITY, __int_as_float(0x7fffffff));
+    if (lane == 0) sh.count = 0;
+    __syncwarp();
+    auto take = [&](float x, int i) {
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < kTopList) sh.list[at] = make_float2(x, __int_as_float(i));
+    };
+    for (int q0 = 0; q0 < count; q0 += 8) {
+        float4 v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const int e = q0 + q < count ? (few ? q0 + q : (int)sh.ranges[q0 + q]) * kHeadRange + 4 * lane : a.vp;
+            v[q] = e < a.vp ? *reinterpret_cast<const float4*>(s + e) : make_float4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            if (q0 + q >= count) break;
+            const int e = (few ? q0 + q : (int)sh.ranges[q0 + q]) * kHeadRange + 4 * lane;
+            const float x[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (x[i] >= bound && e + i < a.vp) take(x[i], a.v0 + e + i);
+        }
+    }
+    if (lane < a.top && best.i != 0x7fffffff && best.v >= bound) take(best.v, best.i);
+    __syncwarp();
+    const int n = sh.count;
+    if (n > kTopList) return head_top_slow(a, p, s, best);
+    for (int q = lane; q < n; q += 32) {
+        const float2 x = sh.list[q];
+        const int place = head_place(x.x, __float_as_int(x.y), n, [&](int j) { return sh.list[j]; });
+        if (place < kHeadTop) sh.out[place] = x;
+    }
+    __syncwarp();
+    const float2 x = sh.out[lane];
+    __syncwarp();
+    return {x.x, __float_as_int(x.y)};
+}
+
+template <bool TOP>
+__global__ void __launch_bounds__(256) head_probs_kernel(const HeadProbsOut a) {
+    __shared__ HeadTopShared sh[TOP ? 8 : 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    pdl_wait();
+    pdl_trigger();
+    for (int64_t t = blockIdx.x * 8ll + warp; t < a.n; t += gridDim.x * 8ll) {
+        const int row = a.pos[t];
+        HeadBest best = HeadBest::none();
+        if (TOP && row >= 0) {
+            if (!a.is_first) {
+                const float2 b = a.best[(int64_t)row * 32 + lane];
+                best = {b.x, __float_as_int(b.y)};
+            }
+            best = head_top(a, row, best, sh[TOP ? warp : 0]);
+            if (!a.is_last) a.best[(int64_t)row * 32 + lane] = make_float2(best.v, __int_as_float(best.i));
+        }
+        if (TOP && !a.is_last) continue;
+        HeadSums x = head_no_sums();
+        if (row >= 0) {
+            x = head_join_ranges(a.part + (int64_t)row * a.ranges, a.ranges);
+        }
+        head_probs_write(a, t, lane, row == kHeadBad, row >= 0, x, row >= 0 ? a.label_logit[row] : 0.0f, best);
+    }
 }
 
 // One to four tokens: the weight by rows, as head_vec_kernel.  A CTA keeps its
@@ -364,10 +561,7 @@ __global__ void __launch_bounds__(kHeadVecJoin)
     if (a.top > 0)
         for (int i = tid; i < ctas; i += kHeadVecJoin) heads[i] = cand[(int64_t)i * a.top];
     if (tid >= kHeadVecJoin - 32) {
-        HeadSums x = head_no_sums();
-        for (int r = lane; r < ctas; r += 32) x = head_join3(x, a.part[(int64_t)t * ctas + r]);
-#pragma unroll
-        for (int s = 16; s > 0; s >>= 1) x = head_join3(x, head_shuffle(x, s));
+        const HeadSums x = head_join_ranges(a.part + (int64_t)t * ctas, ctas);
         if (lane == 0) sums = x;
     }
     __syncthreads();
