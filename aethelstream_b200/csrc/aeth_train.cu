@@ -188,10 +188,12 @@ int head_rows(HeadRows a, const int64_t* labels, int64_t n, int64_t d, int64_t v
     a.ldo = p.dp;
     const unsigned ctas = (unsigned)std::min<int64_t>(n, num_sms());
     if (n <= kHeadScan) {
-        head_rows_kernel<true><<<ctas, 1024, 0, st>>>(a, rt->err_word);
+        auto kern = a.row ? head_rows_kernel<true, true> : head_rows_kernel<true, false>;
+        kern<<<ctas, 1024, 0, st>>>(a, rt->err_word);
         AETH_LAUNCH_CHECK();
     } else {
-        head_rows_kernel<false><<<1, 1024, 0, st>>>(a, rt->err_word);
+        auto kern = a.row ? head_rows_kernel<false, true> : head_rows_kernel<false, false>;
+        kern<<<1, 1024, 0, st>>>(a, rt->err_word);
         AETH_LAUNCH_CHECK();
         AETH_CUDA(launch_after(head_pack_kernel, dim3(ctas), dim3(1024), 0, st, 1, a));
     }
@@ -681,10 +683,19 @@ int aeth_token_log_probs_backward(const void* hidden, int64_t ld_hidden, const v
     c.used = w.bytes;
     float4* row = c.take<float4>(p.n_pad);
     if (workspace_bytes < c.used || !aligned16(workspace)) return set_err(AETH_ERR_ARG);
-    AETH_TRY(head_rows({}, labels, n, d, vocab, ignore_index, hidden, ld_hidden, p, w, st));
-    const HeadProbsRows a{w.rows, w.count, lse, entropy, grad_log_probs, grad_entropy, 0.25f * logf((float)vocab) + 0.5f,
-                          head_g_bits(bf16), head_g_scale(bf16), w.lse2, w.out_scale, w.row_scale, row};
-    AETH_CUDA(launch_after(head_probs_rows_kernel, dim3(1), dim3(1024), 0, st, 1, a));
+    HeadRows a = {};
+    a.lse = lse;
+    a.entropy = entropy;
+    a.grad = grad_log_probs;
+    a.grad_entropy = grad_entropy;
+    a.bound = 0.25f * logf((float)vocab) + 0.5f;
+    a.g_bits = head_g_bits(bf16);
+    a.g_scale = head_g_scale(bf16);
+    a.lse2 = w.lse2;
+    a.out_scale = w.out_scale;
+    a.row_scale = w.row_scale;
+    a.row = row;
+    AETH_TRY(head_rows(a, labels, n, d, vocab, ignore_index, hidden, ld_hidden, p, w, st));
     auto run = bf16 ? head_backward<true, false, true> : unit ? head_backward<false, true, true> : head_backward<false, false, true>;
     return run(p, w, weight, ld_weight, n, d, vocab, row, d_hidden, ld_dh, d_weight, ld_dw, st);
 }

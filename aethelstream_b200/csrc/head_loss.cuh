@@ -65,6 +65,10 @@ struct HeadRows {
     float* lse2;       // live row -> lse * log2(e) - g_bits
     float* out_scale;  // max|g| / g_scale
     float* row_scale;  // live row -> |g_t| / g_scale
+    // the gradient of log probabilities and entropies in its place (head_probs.cuh; row != null)
+    const float *entropy, *grad_entropy;
+    float bound;  // of |p (log p + entropy)|
+    float4* row;
     // the live rows of H, gathered to a pitch that TMA takes
     const uint16_t* h;
     int64_t ld;
@@ -113,13 +117,27 @@ __device__ __forceinline__ int64_t head_padded(int live, int64_t n) {
     return min((int64_t)max((live + 255) / 256 * 256, 256), n);
 }
 
+// A live row of the gradient of a log p_y + b entropy: its weight w = |a| + c |b|
+// (returned, and for now in row[].w) and, of a / w and b / w, what an entry takes
+// (HeadRowGrad).
+__device__ __forceinline__ float head_probs_row(const HeadRows& a, int64_t t, int i) {
+    const float ga = a.grad ? a.grad[t] : 0.0f, gb = a.grad_entropy ? a.grad_entropy[t] : 0.0f;
+    const float w = fmaf(a.bound, fabsf(gb), fabsf(ga));
+    const float ua = w == 0.0f ? 0.0f : ga / w, ub = w == 0.0f ? 0.0f : gb / w, gamma = ub * kLn2;
+    a.lse2[i] = a.lse[t];
+    a.row_scale[i] = w / a.g_scale;
+    a.row[i] = make_float4(ua * a.g_scale, fmaf(-gamma, a.g_bits, fmaf(ub, a.entropy[t], ua)), gamma, w);
+    return w;
+}
+
 // Numbers the live tokens in order (a scan over the labels, 8192 at a time, so
 // that their loads are in flight together) and gathers what the epilogues need
-// per live row.  CTA 0 writes that.  PACK (up to 8192 tokens): every CTA makes
+// per live row.  CTA 0 writes that.  PROBS: for a gradient of log probabilities and
+// entropies (head_probs_row).  PACK (up to 8192 tokens): every CTA makes
 // the scan for itself and then gathers its share of H's rows; more tokens take
 // one CTA and head_pack_kernel behind it.
 constexpr int kHeadScan = 8192;
-template <bool PACK>
+template <bool PACK, bool PROBS>
 __global__ void __launch_bounds__(1024) head_rows_kernel(const __grid_constant__ HeadRows a, uint32_t* err) {
     constexpr int kItems = kHeadScan / 1024;
     __shared__ int wsum[kItems * 32];
@@ -185,7 +203,10 @@ __global__ void __launch_bounds__(1024) head_rows_kernel(const __grid_constant__
             a.pos[t] = i;
             a.rows[i] = (int)t;
             a.lab[i] = (int)lab[k];
-            if (a.coef) {
+            if (PROBS) {
+                const float w = head_probs_row(a, t, i);
+                if (w <= 3.402823466e38f) gmax = fmaxf(gmax, w);
+            } else if (a.coef) {
                 a.lse2[i] = fmaf(lse[k], kLog2e, -a.g_bits);
                 if (a.grad) {
                     const float g = grad[k] * a.scale;
@@ -211,6 +232,18 @@ __global__ void __launch_bounds__(1024) head_rows_kernel(const __grid_constant__
     if (tid == 0) {
         *a.count = base;
         *a.done = 0;
+    }
+    if (PROBS) {
+        gmax = warp_max(gmax);
+        if (lane == 0) wmax[warp] = gmax;
+        __syncthreads();
+        gmax = warp_max(wmax[lane]);
+        for (int i = tid; i < base; i += 1024) {
+            const float w = a.row[i].w;
+            a.row[i].w = w == 0.0f ? 0.0f : w / gmax;
+        }
+        if (tid == 0) *a.out_scale = gmax / a.g_scale;
+        return;
     }
     if (!a.coef) return;
     if (a.grad) {

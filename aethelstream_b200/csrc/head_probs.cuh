@@ -598,42 +598,4 @@ __global__ void __launch_bounds__(kHeadVecJoin)
                      HeadBest{top[lane].x, __float_as_int(top[lane].y)});
 }
 
-// The gradient's rows: a token's weight w = |a| + c |b| and, of a / w and b / w,
-// what an entry of its row takes (HeadRowGrad).  One CTA; what is not finite
-// stays its token's.
-struct HeadProbsRows {
-    const int *rows, *count;
-    const float *lse, *entropy, *grad, *grad_entropy;  // per token; the gradients may be null: 0
-    float c, g_bits, g_scale;
-    float *lse_row, *out_scale, *row_scale;
-    float4* row;
-};
-__global__ void __launch_bounds__(1024) head_probs_rows_kernel(const HeadProbsRows a) {
-    __shared__ float wmax[32];
-    pdl_wait();
-    pdl_trigger();
-    const int live = *a.count, lane = threadIdx.x & 31;
-    float top = 0.0f;
-    for (int i = threadIdx.x; i < live; i += 1024) {
-        const int t = a.rows[i];
-        const float ga = a.grad ? a.grad[t] : 0.0f, gb = a.grad_entropy ? a.grad_entropy[t] : 0.0f;
-        const float w = fmaf(a.c, fabsf(gb), fabsf(ga));
-        if (w <= 3.402823466e38f) top = fmaxf(top, w);
-    }
-    top = warp_max(top);
-    if (lane == 0) wmax[threadIdx.x >> 5] = top;
-    __syncthreads();
-    top = warp_max(wmax[lane]);
-    for (int i = threadIdx.x; i < live; i += 1024) {
-        const int t = a.rows[i];
-        const float ga = a.grad ? a.grad[t] : 0.0f, gb = a.grad_entropy ? a.grad_entropy[t] : 0.0f;
-        const float w = fmaf(a.c, fabsf(gb), fabsf(ga));
-        const float ua = w == 0.0f ? 0.0f : ga / w, ub = w == 0.0f ? 0.0f : gb / w, gamma = ub * kLn2;
-        a.lse_row[i] = a.lse[t];
-        a.row_scale[i] = w / a.g_scale;
-        a.row[i] = make_float4(ua * a.g_scale, fmaf(-gamma, a.g_bits, fmaf(ub, a.entropy[t], ua)), gamma, w == 0.0f ? 0.0f : w / top);
-    }
-    if (threadIdx.x == 0) *a.out_scale = top / a.g_scale;
-}
-
 }  // namespace aeth
