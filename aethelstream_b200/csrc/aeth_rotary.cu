@@ -91,6 +91,8 @@ void rot_grid(RotaryArgs& a, int64_t tokens, int step, int most) {
 // SM: 126 registers) 92, 102 and 110 in one, two and three.
 template <int OP>
 constexpr int rot_per_sm() { return OP == ROT_NORM_BACK ? 2 : 3; }
+// A CTA of more than one wave has eight passes (of all its groups) at least.
+constexpr int kRotPasses = 8;
 template <int OP>
 constexpr int rot_waves() { return OP == ROT_TURN ? 3 : OP == ROT_NORM ? 2 : 1; }
 int rot_back_ctas() { return rot_per_sm<ROT_NORM_BACK>() * num_sms(); }  // each leaves sums of the gains'
@@ -103,7 +105,8 @@ int rot_launch(RotaryArgs& a, int64_t tokens, bool whole, cudaStream_t st) {
         while (lanes < a.D / 16) lanes *= 2;
         const int groups = kRotThreads / lanes, held = kRotTableBytes / (4 * a.R);
         const int64_t rows = std::max(a.s[0].rows, a.s[1].rows);
-        const unsigned ctas = (unsigned)std::min<int64_t>((rows + groups - 1) / groups, (int64_t)rot_waves<OP>() * rot_per_sm<OP>() * num_sms());
+        const int64_t passes = (rows + groups - 1) / groups, wave = (int64_t)rot_per_sm<OP>() * num_sms();
+        const unsigned ctas = (unsigned)std::min(passes, std::max(wave, std::min(rot_waves<OP>() * wave, passes / kRotPasses)));
         int64_t most = 0;  // tokens that a CTA's rows have, and one more
         for (RotaryRows& s : a.s) {
             s.ctas = s.rows > 0 ? ctas : 0;
