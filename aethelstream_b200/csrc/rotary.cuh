@@ -82,7 +82,7 @@ __device__ __forceinline__ int rot_quotient(int n, int heads, uint32_t magic) {
     return heads == 1 ? n : heads > 32768 ? (n >= heads ? 1 : 0) : (int)__umulhi((uint32_t)n, magic);
 }
 __device__ __forceinline__ int64_t rot_position(const RotaryArgs& a, int64_t token) {
-    const int64_t i = a.period == 1 ? 0 : token % a.period;
+    const int64_t i = token < a.period ? token : token % a.period;
     return a.pos32 ? (int64_t)static_cast<const int*>(a.pos)[i] : static_cast<const int64_t*>(a.pos)[i];
 }
 

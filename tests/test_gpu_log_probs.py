@@ -199,6 +199,13 @@ def test_a_large_vocabulary_of_few_tokens():
         close(r.log_probs, s.gather(1, lab[:, None])[:, 0] - lse, 2.0 ** -18 * (1 + lse.abs()))
 
 
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_more_tokens_than_a_scan(dt):
+    """The live tokens are numbered 8192 at a time."""
+    check(*make(9001, 64, 300, dt, seed=16, masked=0.3), top=4)
+    check(*make(16385, 40, 70, dt, seed=17), top=2)
+
+
 @pytest.mark.parametrize("masked", [0.3, 0.9, 1.0])
 @pytest.mark.parametrize("n", [1, 3, 40, 300, 700])
 def test_masked_tokens_take_no_part(n, masked):

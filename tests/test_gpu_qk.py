@@ -259,6 +259,25 @@ def test_stretches_of_many_rows(A):
     assert all(torch.equal(a, b) for a, b in zip(got, again))
 
 
+@pytest.mark.parametrize("heads", [511, 512, 513, 32768, 32769, 40000])
+def test_many_heads(A, heads):
+    """Heads in the thousands, whose rows' tokens come by a product or a comparison."""
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    for d, r in ((16, 16), (6, 4)):
+        plan = A.RotaryPlan(r, device="cuda")
+        pos = torch.tensor([3, 70000, 12], device="cuda")
+        q, dq = (torch.randn(3, heads, d, generator=gen, device="cuda") for _ in range(2))
+        w = 1 + 0.1 * torch.randn(d, generator=gen, device="cuda")
+        close(A.rotary(q, q[:, :5], pos, plan)[0], *turn(plan, q.double(), pos), (heads, d))
+        dx, _, dw, _ = A.qk_norm_rotary_backward(dq, None, q, None, w, None, pos, plan)
+        g, _ = turn(plan, dq.double(), pos, -1.0)
+        x = q.double()
+        rr = 1 / torch.sqrt(x.square().mean(-1, keepdim=True) + 1e-6)
+        want = rr * w * g - x * rr ** 3 * (w * g * x).mean(-1, keepdim=True)
+        # of sizes of 1 to 10 in fp32: far below 1e-4
+        assert (dx.double() - want).abs().max() < 1e-4 and (dw.double() - (g * x * rr).sum((0, 1))).abs().max() < 3 * heads * 1e-6
+
+
 def test_captured(A):
     gen = torch.Generator(device="cuda").manual_seed(8)
     plan = A.RotaryPlan(64, device="cuda")
