@@ -273,20 +273,22 @@ __device__ __forceinline__ void adamw_moments(const AdamwScalars& s, const float
     }
 }
 // The parameters' step from the new moments
-template <int N>
+template <int N, bool FLUSH>
 __device__ __forceinline__ void adamw_params(const AdamwScalars& s, float decay, const float (&m)[N], const float (&v)[N],
                                              float (&p)[N]) {
     const float2 first = make_float2(s.first, s.first), second = make_float2(s.second, s.second);
-    auto params = [&](auto flush) {
 #pragma unroll
-        for (int k = 0; k < N; k += 2) {
-            const float2 mm = mul2_rn(make_float2(m[k], m[k + 1]), first), vv = mul2_rn(make_float2(v[k], v[k + 1]), second);
-            p[k] -= s.lr * fmaf(mm.x, adamw_scale<flush.value>(vv.x, s.eps), decay * p[k]);
-            p[k + 1] -= s.lr * fmaf(mm.y, adamw_scale<flush.value>(vv.y, s.eps), decay * p[k + 1]);
-        }
-    };
-    if (s.flush) params(std::true_type());
-    else params(std::false_type());
+    for (int k = 0; k < N; k += 2) {
+        const float2 mm = mul2_rn(make_float2(m[k], m[k + 1]), first), vv = mul2_rn(make_float2(v[k], v[k + 1]), second);
+        p[k] -= s.lr * fmaf(mm.x, adamw_scale<FLUSH>(vv.x, s.eps), decay * p[k]);
+        p[k + 1] -= s.lr * fmaf(mm.y, adamw_scale<FLUSH>(vv.y, s.eps), decay * p[k + 1]);
+    }
+}
+template <int N>
+__device__ __forceinline__ void adamw_params(const AdamwScalars& s, float decay, const float (&m)[N], const float (&v)[N],
+                                             float (&p)[N]) {
+    if (s.flush) adamw_params<N, true>(s, decay, m, v, p);
+    else adamw_params<N, false>(s, decay, m, v, p);
 }
 
 // Moments in 32 bits: a CTA takes blocks, a thread four elements of each half of
@@ -335,18 +337,26 @@ __global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ Adam
     adamw_count(a);
 }
 
-// Moments in 8 bits.  A CTA is five groups of 128 threads that share the maps and
+// Moments in 8 bits.  A CTA is some groups of 128 threads that share the maps and
 // the encode's tables (the layout of b2_adam_dyn_kernel: each map entry in 32
 // copies, so that no lookup of a warp meets a bank conflict); a group takes a
 // block, a thread eight elements of each of its halves.  A block's 16-bit gradients
 // and parameters and its codes are fetched while the one before it is encoded.
-constexpr int kAdamw8Groups = 5, kAdamw8Threads = 128 * kAdamw8Groups;
+// FAST, where all parameters and gradients of the launch are bf16, without a master
+// copy: whole blocks go without a branch on types and ends for every eight elements,
+// in four groups, whose registers that takes.  Else five, for what is not fetched
+// ahead.  2^27 elements: bf16 288 us (4.66 TB/s) fast, 316 in the other; f32 498 in
+// the other, 553 in four groups.  Bound by instructions (some 60 an element, issue
+// slots 75 % taken), most of them for the two encodes.
+template <bool FAST>
+constexpr int adamw8_groups() { return FAST ? 4 : 5; }
 constexpr int kAdamw8Dec = 256 * 256;
 constexpr int kAdamw8Shared = kAdamw8Dec + (2 * kDmapLutEntries + kDmapLutUEntries) * 4;
 constexpr int kAdamwHalf = kAdamwBlock / 2;
 
-template <int CAP>
-__global__ void __launch_bounds__(kAdamw8Threads, 1) adamw8_kernel(const __grid_constant__ AdamwArgs<CAP> a) {
+template <int CAP, bool FAST>
+__global__ void __launch_bounds__(128 * adamw8_groups<FAST>(), 1) adamw8_kernel(const __grid_constant__ AdamwArgs<CAP> a) {
+    constexpr int kAdamw8Groups = adamw8_groups<FAST>();
     extern __shared__ __align__(16) uint8_t adamw_smem[];
     float* dec = reinterpret_cast<float*>(adamw_smem);
     uint32_t* lut_s = reinterpret_cast<uint32_t*>(adamw_smem + kAdamw8Dec);
@@ -367,7 +377,7 @@ __global__ void __launch_bounds__(kAdamw8Threads, 1) adamw8_kernel(const __grid_
     const int walker = blockIdx.x * kAdamw8Groups + grp, step = gridDim.x * kAdamw8Groups;
     int i = a.start[walker], par = 0;
     int64_t e = 0, o = 0, blk = 0;  // this thread's first element, in its tensor and among the moments; its block
-    bool p16 = false, g16 = false;  // fetched ahead
+    bool p16 = false, g16 = false, fast16 = false;  // fetched ahead; both, by the whole warp, and both bf16
     uint4 pw[2], gw[2];
     uint2 qm[2], qv[2];
     float sm = 0.0f, sv = 0.0f;
@@ -381,6 +391,7 @@ __global__ void __launch_bounds__(kAdamw8Threads, 1) adamw8_kernel(const __grid_
         const bool whole = t.whole && e + kAdamwHalf + 8 <= t.n;
         p16 = whole && t.p_dtype != AETH_DTYPE_F32 && !a.master;
         g16 = whole && t.g_dtype != AETH_DTYPE_F32;
+        if (FAST) fast16 = __all_sync(0xffffffffu, p16 && g16 && s.flush && t.p_dtype == AETH_DTYPE_BF16 && t.g_dtype == AETH_DTYPE_BF16);
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
             if (g16) gw[q] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(t.g) + e + q * kAdamwHalf);
@@ -398,53 +409,60 @@ __global__ void __launch_bounds__(kAdamw8Threads, 1) adamw8_kernel(const __grid_
         float m[2][8], v[2][8], am = 0.0f, av = 0.0f;
         const float2 sm2 = make_float2(sm, sm), sv2 = make_float2(sv, sv);
         const float decay = t.decay ? s.decay : 0.0f;
+        auto update = [&](auto fast) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            const int64_t eq = e + q * kAdamwHalf;
-            const int have = (int)max(min(t.n - eq, (int64_t)8), (int64_t)0);
-            float g[8], p[8];
-            if (g16) {
-                const uint32_t w[4] = {gw[q].x, gw[q].y, gw[q].z, gw[q].w};
-                adamw_floats<8>(w, t.g_dtype, g);
-            } else {
-                adamw_load<8>(t.g, t.g_dtype, t.whole, eq, have, g);
-            }
+            for (int q = 0; q < 2; ++q) {
+                const int64_t eq = e + q * kAdamwHalf;
+                const int have = fast.value ? 8 : (int)max(min(t.n - eq, (int64_t)8), (int64_t)0);
+                float g[8], p[8];
+                if (fast.value || g16) {
+                    const uint32_t w[4] = {gw[q].x, gw[q].y, gw[q].z, gw[q].w};
+                    adamw_floats<8>(w, fast.value ? (int)AETH_DTYPE_BF16 : t.g_dtype, g);
+                } else {
+                    adamw_load<8>(t.g, t.g_dtype, t.whole, eq, have, g);
+                }
 #pragma unroll
-            for (int k = 0; k < 8; k += 2) {
-                const uint32_t sel = 0x5504u | ((uint32_t)(k & 3) << 4), wm = k < 4 ? qm[q].x : qm[q].y, wv = k < 4 ? qv[q].x : qv[q].y;
-                const float2 mm = mul2_rn(make_float2(__uint_as_float(lds_u32(dec_base + prmt(wm, off_m, sel))),
-                                                      __uint_as_float(lds_u32(dec_base + prmt(wm, off_m, sel + 0x10u)))), sm2);
-                const float2 vv = mul2_rn(make_float2(__uint_as_float(lds_u32(dec_base + prmt(wv, off_v, sel))),
-                                                      __uint_as_float(lds_u32(dec_base + prmt(wv, off_v, sel + 0x10u)))), sv2);
-                m[q][k] = mm.x;
-                m[q][k + 1] = mm.y;
-                v[q][k] = vv.x;
-                v[q][k + 1] = vv.y;
-            }
-            adamw_moments<8>(s, g, m[q], v[q]);
-            if (p16) {
-                uint32_t w[4] = {pw[q].x, pw[q].y, pw[q].z, pw[q].w};
-                adamw_floats<8>(w, t.p_dtype, p);
-                adamw_params<8>(s, decay, m[q], v[q], p);
-                adamw_words<8>(p, t.p_dtype, w);
-                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(t.p) + eq) = make_uint4(w[0], w[1], w[2], w[3]);
-            } else {
-                if (a.master) adamw_load<8>(a.master, AETH_DTYPE_F32, true, o + q * kAdamwHalf, 8, p);
-                else adamw_load<8>(t.p, t.p_dtype, t.whole, eq, have, p);
-                adamw_params<8>(s, decay, m[q], v[q], p);
-                if (a.master) adamw_store<8>(a.master, AETH_DTYPE_F32, true, o + q * kAdamwHalf, have, p);
-                adamw_store<8>(t.p, t.p_dtype, t.whole, eq, have, p);
-            }
-            if (have < 8)  // past the tensor's end: codes of zero
+                for (int k = 0; k < 8; k += 2) {
+                    const uint32_t sel = 0x5504u | ((uint32_t)(k & 3) << 4);
+                    const uint32_t wm = k < 4 ? qm[q].x : qm[q].y, wv = k < 4 ? qv[q].x : qv[q].y;
+                    const float2 mm = mul2_rn(make_float2(__uint_as_float(lds_u32(dec_base + prmt(wm, off_m, sel))),
+                                                          __uint_as_float(lds_u32(dec_base + prmt(wm, off_m, sel + 0x10u)))), sm2);
+                    const float2 vv = mul2_rn(make_float2(__uint_as_float(lds_u32(dec_base + prmt(wv, off_v, sel))),
+                                                          __uint_as_float(lds_u32(dec_base + prmt(wv, off_v, sel + 0x10u)))), sv2);
+                    m[q][k] = mm.x;
+                    m[q][k + 1] = mm.y;
+                    v[q][k] = vv.x;
+                    v[q][k + 1] = vv.y;
+                }
+                adamw_moments<8>(s, g, m[q], v[q]);
+                if (fast.value || p16) {
+                    const int dtype = fast.value ? (int)AETH_DTYPE_BF16 : t.p_dtype;
+                    uint32_t w[4] = {pw[q].x, pw[q].y, pw[q].z, pw[q].w};
+                    adamw_floats<8>(w, dtype, p);
+                    if (fast.value) adamw_params<8, true>(s, decay, m[q], v[q], p);
+                    else adamw_params<8>(s, decay, m[q], v[q], p);
+                    adamw_words<8>(p, dtype, w);
+                    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(t.p) + eq) = make_uint4(w[0], w[1], w[2], w[3]);
+                } else {
+                    if (a.master) adamw_load<8>(a.master, AETH_DTYPE_F32, true, o + q * kAdamwHalf, 8, p);
+                    else adamw_load<8>(t.p, t.p_dtype, t.whole, eq, have, p);
+                    adamw_params<8>(s, decay, m[q], v[q], p);
+                    if (a.master) adamw_store<8>(a.master, AETH_DTYPE_F32, true, o + q * kAdamwHalf, have, p);
+                    adamw_store<8>(t.p, t.p_dtype, t.whole, eq, have, p);
+                }
+                if (!fast.value && have < 8)  // past the tensor's end: codes of zero
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (k >= have) m[q][k] = v[q][k] = 0.0f;
+                    for (int k = 0; k < 8; ++k)
+                        if (k >= have) m[q][k] = v[q][k] = 0.0f;
 #pragma unroll
-            for (int k = 0; k < 8; k += 2) {
-                am = fmax3_nan(am, fabsf(m[q][k]), fabsf(m[q][k + 1]));
-                av = fmax3_nan(av, v[q][k], v[q][k + 1]);
+                for (int k = 0; k < 8; k += 2) {
+                    am = fmax3_nan(am, fabsf(m[q][k]), fabsf(m[q][k + 1]));
+                    av = fmax3_nan(av, v[q][k], v[q][k + 1]);
+                }
             }
-        }
+        };
+        if (FAST && fast16) update(std::true_type());
+        else update(std::false_type());
         if (b + step < a.blocks) fetch(b + step);
         // non-negative or NaN (0x7fffffff): their bits order as they do
         const uint32_t wm = __reduce_max_sync(0xffffffffu, __float_as_uint(am));

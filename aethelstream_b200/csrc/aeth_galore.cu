@@ -2433,17 +2433,19 @@ namespace {
 
 template <int CAP>
 int adamw_launch(AdamwArgs<CAP>& a, int bits, cudaStream_t st) {
-    const int walkers = bits == 8 ? kAdamw8Groups : 1, per_sm = bits == 8 ? 1 : 6;  // of a CTA, CTAs of an SM
+    bool fast = bits == 8 && !a.master;
+    for (int i = 0; i < a.count && fast; ++i) fast = a.t[i].p_dtype == AETH_DTYPE_BF16 && a.t[i].g_dtype == AETH_DTYPE_BF16;
+    const int walkers = bits != 8 ? 1 : fast ? adamw8_groups<true>() : adamw8_groups<false>(), per_sm = bits == 8 ? 1 : 6;
     const int ctas = std::max(std::min((a.blocks + walkers - 1) / walkers, std::min(per_sm * num_sms(), kAdamwStarts / walkers)), 1);
     for (int w = 0, i = 0; w < ctas * walkers; ++w) {
         while (i + 1 < a.count && a.t[i + 1].first <= w) ++i;
         a.start[w] = (uint16_t)i;
     }
     if (bits == 8) {
-        auto kern = adamw8_kernel<CAP>;
-        static std::atomic<bool> allowed[kMaxDevices] = {};
-        AETH_TRY(allow_shared(kern, kAdamw8Shared, allowed));
-        kern<<<ctas, kAdamw8Threads, kAdamw8Shared, st>>>(a);
+        auto kern = fast ? adamw8_kernel<CAP, true> : adamw8_kernel<CAP, false>;
+        static std::atomic<bool> allowed[2][kMaxDevices] = {};
+        AETH_TRY(allow_shared(kern, kAdamw8Shared, allowed[fast]));
+        kern<<<ctas, 128 * walkers, kAdamw8Shared, st>>>(a);
     } else {
         adamw_kernel<CAP><<<ctas, 256, 0, st>>>(a);
     }
