@@ -280,26 +280,36 @@ struct HeadTopShared {
     int count;
 };
 
+// A row's ranges of a piece, or some of them
+struct HeadPiece {
+    const HeadSums* p;
+    const float* s;
+    int count, v0, vp;  // ranges, first entry, entries
+    __device__ HeadPiece(const HeadProbsOut& a, int row, int from, int to)
+        : p(a.part + (int64_t)row * a.ranges + a.first + from), s(a.logits + (int64_t)row * a.ld + from * kHeadRange),
+          count(to - from), v0(a.v0 + from * kHeadRange), vp(min(a.vp, to * kHeadRange) - from * kHeadRange) {}
+};
+
 // The slow way, whatever the logits: one range and one entry after the other.
-__device__ __noinline__ HeadBest head_top_slow(const HeadProbsOut& a, const HeadSums* p, const float* s, HeadBest best) {
+__device__ __noinline__ HeadBest head_top_slow(const HeadPiece& a, int top, HeadBest best) {
     const int lane = threadIdx.x & 31;
     HeadBest at = HeadBest::none();
     for (int r0 = 0; r0 < a.count; r0 += 32) {
         const int r = r0 + lane;
-        at.offer(r < a.count ? p[r].m : -INFINITY, r < a.count ? r : 0x7fffffff, a.top);
+        at.offer(r < a.count ? a.p[r].m : -INFINITY, r < a.count ? r : 0x7fffffff, top);
     }
-    for (int k = 0; k < a.top; ++k) {
+    for (int k = 0; k < top; ++k) {
         const float m = __shfl_sync(0xffffffffu, at.v, k);
         const int r = __shfl_sync(0xffffffffu, at.i, k);
-        if (r == 0x7fffffff || !HeadBest::before(m, a.v0 + r * kHeadRange, __shfl_sync(0xffffffffu, best.v, a.top - 1),
-                                                 __shfl_sync(0xffffffffu, best.i, a.top - 1)))
+        if (r == 0x7fffffff || !HeadBest::before(m, a.v0 + r * kHeadRange, __shfl_sync(0xffffffffu, best.v, top - 1),
+                                                 __shfl_sync(0xffffffffu, best.i, top - 1)))
             break;
         const int e0 = r * kHeadRange + 4 * lane;
-        const float4 v = e0 < a.vp ? *reinterpret_cast<const float4*>(s + e0) : make_float4(0, 0, 0, 0);
+        const float4 v = e0 < a.vp ? *reinterpret_cast<const float4*>(a.s + e0) : make_float4(0, 0, 0, 0);
         const float x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            best.offer(e0 + i < a.vp ? x[i] : -INFINITY, e0 + i < a.vp ? a.v0 + e0 + i : 0x7fffffff, a.top);
+            best.offer(e0 + i < a.vp ? x[i] : -INFINITY, e0 + i < a.vp ? a.v0 + e0 + i : 0x7fffffff, top);
     }
     return best;
 }
@@ -310,11 +320,11 @@ __device__ __noinline__ HeadBest head_top_slow(const HeadProbsOut& a, const Head
 // it lies in; the ranges whose maxima reach it are read, eight at a time, and the
 // entries that do are counted into their places.  With equal logits by the hundred,
 // which a bound cannot part, the slow way.
-__device__ __forceinline__ HeadBest head_top(const HeadProbsOut& a, int row, HeadBest best, HeadTopShared& sh) {
+__device__ __forceinline__ HeadBest head_top(const HeadPiece& a, int top, HeadBest best, HeadTopShared& sh) {
     const int lane = threadIdx.x & 31;
-    const HeadSums* p = a.part + (int64_t)row * a.ranges + a.first;
-    const float* s = a.logits + (int64_t)row * a.ld;
-    const bool few = 2 * a.count < 3 * a.top;
+    const HeadSums* p = a.p;
+    const float* s = a.s;
+    const bool few = 2 * a.count < 3 * top;
     uint32_t key[8] = {};
     if (few) {
         for (int e0 = 0; e0 < a.vp; e0 += 1024)
@@ -348,12 +358,12 @@ __device__ __forceinline__ HeadBest head_top(const HeadProbsOut& a, int row, Hea
 #pragma unroll
         for (int j = 0; j < 8; ++j) n += key[j] >= mid ? 1 : 0;
         n = __reduce_add_sync(0xffffffffu, n);
-        if (n >= a.top) lo = mid;
+        if (n >= top) lo = mid;
         else hi = mid - 1;
-        if (n == a.top) break;
+        if (n == top) break;
     }
-    const int last = __shfl_sync(0xffffffffu, best.i, a.top - 1);
-    const float last_v = __shfl_sync(0xffffffffu, best.v, a.top - 1);
+    const int last = __shfl_sync(0xffffffffu, best.i, top - 1);
+    const float last_v = __shfl_sync(0xffffffffu, best.v, top - 1);
     if (last != 0x7fffffff) lo = max(lo, head_key(last_v));
     const float bound = lo <= head_key(-INFINITY) ? -INFINITY : head_unkey(lo);  // below: no float, and no group either
     int count = a.count;
@@ -374,7 +384,7 @@ __device__ __forceinline__ HeadBest head_top(const HeadProbsOut& a, int row, Hea
                 count += __popc(who);
             }
         }
-        if (count > kTopRanges) return head_top_slow(a, p, s, best);
+        if (count > kTopRanges) return head_top_slow(a, top, best);
     }
     sh.out[lane] = make_float2(-INFINITY, __int_as_float(0x7fffffff));
     if (lane == 0) sh.count = 0;
@@ -400,10 +410,10 @@ __device__ __forceinline__ HeadBest head_top(const HeadProbsOut& a, int row, Hea
                 if (x[i] >= bound && e + i < a.vp) take(x[i], a.v0 + e + i);
         }
     }
-    if (lane < a.top && best.i != 0x7fffffff && best.v >= bound) take(best.v, best.i);
+    if (lane < top && best.i != 0x7fffffff && best.v >= bound) take(best.v, best.i);
     __syncwarp();
     const int n = sh.count;
-    if (n > kTopList) return head_top_slow(a, p, s, best);
+    if (n > kTopList) return head_top_slow(a, top, best);
     for (int q = lane; q < n; q += 32) {
         const float2 x = sh.list[q];
         const int place = head_place(x.x, __float_as_int(x.y), n, [&](int j) { return sh.list[j]; });
@@ -415,29 +425,54 @@ __device__ __forceinline__ HeadBest head_top(const HeadProbsOut& a, int row, Hea
     return {x.x, __float_as_int(x.y)};
 }
 
-template <bool TOP>
+// A warp a token, or with SPLIT the eight warps of a CTA: each takes an eighth of
+// the ranges, and their best entries are counted into their places.
+template <bool TOP, bool SPLIT>
 __global__ void __launch_bounds__(256) head_probs_kernel(const HeadProbsOut a) {
     __shared__ HeadTopShared sh[TOP ? 8 : 1];
+    __shared__ float2 all[SPLIT && TOP ? 8 * kHeadTop : 1], out[SPLIT && TOP ? kHeadTop : 1];
+    __shared__ HeadSums sums[SPLIT ? 8 : 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     pdl_wait();
     pdl_trigger();
-    for (int64_t t = blockIdx.x * 8ll + warp; t < a.n; t += gridDim.x * 8ll) {
+    for (int64_t t = SPLIT ? blockIdx.x : blockIdx.x * 8ll + warp; t < a.n; t += gridDim.x * (SPLIT ? 1ll : 8ll)) {
         const int row = a.pos[t];
         HeadBest best = HeadBest::none();
         if (TOP && row >= 0) {
-            if (!a.is_first) {
+            if (!a.is_first && (!SPLIT || warp == 0)) {
                 const float2 b = a.best[(int64_t)row * 32 + lane];
                 best = {b.x, __float_as_int(b.y)};
             }
-            best = head_top(a, row, best, sh[TOP ? warp : 0]);
-            if (!a.is_last) a.best[(int64_t)row * 32 + lane] = make_float2(best.v, __int_as_float(best.i));
+            const int from = SPLIT ? a.count * warp / 8 : 0, to = SPLIT ? a.count * (warp + 1) / 8 : a.count;
+            if (from < to) best = head_top(HeadPiece(a, row, from, to), a.top, best, sh[TOP ? warp : 0]);
+            if (SPLIT) {
+                if (lane < a.top) all[warp * a.top + lane] = make_float2(best.v, __int_as_float(best.i));
+                if (warp == 0) out[lane] = make_float2(-INFINITY, __int_as_float(0x7fffffff));
+                __syncthreads();
+                if (lane < a.top && best.i != 0x7fffffff) {
+                    const int place = head_place(best.v, best.i, 8 * a.top, [&](int j) { return all[j]; });
+                    if (place < a.top) out[place] = make_float2(best.v, __int_as_float(best.i));
+                }
+                __syncthreads();
+                best = {out[lane].x, __float_as_int(out[lane].y)};
+            }
+            if (!a.is_last && (!SPLIT || warp == 0)) a.best[(int64_t)row * 32 + lane] = make_float2(best.v, __int_as_float(best.i));
         }
-        if (TOP && !a.is_last) continue;
         HeadSums x = head_no_sums();
-        if (row >= 0) {
-            x = head_join_ranges(a.part + (int64_t)row * a.ranges, a.ranges);
+        if (row >= 0 && (!TOP || a.is_last)) {
+            const int from = SPLIT ? a.ranges * warp / 8 : 0, to = SPLIT ? a.ranges * (warp + 1) / 8 : a.ranges;
+            x = head_join_ranges(a.part + (int64_t)row * a.ranges + from, to - from);
+            if (SPLIT) {
+                if (lane == 0) sums[warp] = x;
+                __syncthreads();
+                x = sums[lane & 7];
+#pragma unroll
+                for (int o = 1; o < 8; o <<= 1) x = head_join3(x, head_shuffle(x, o));
+            }
         }
-        head_probs_write(a, t, lane, row == kHeadBad, row >= 0, x, row >= 0 ? a.label_logit[row] : 0.0f, best);
+        if (SPLIT) __syncthreads();  // the shared places are the next token's
+        if ((!TOP || a.is_last) && (!SPLIT || warp == 0))
+            head_probs_write(a, t, lane, row == kHeadBad, row >= 0, x, row >= 0 ? a.label_logit[row] : 0.0f, best);
     }
 }
 

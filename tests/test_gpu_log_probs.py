@@ -190,7 +190,7 @@ def test_a_large_vocabulary_of_few_tokens():
     """Pieces with tokens as the products' columns, and past what one to four keep."""
     import aethelstream_b200 as A
     v = 1000003
-    for n in (1, 4, 300):
+    for n in (1, 4, 60, 300):
         h, w, lab = grid(n, 16, v, torch.bfloat16, n, 16)
         r = A.token_log_probs(h, w, lab, top_k=8)
         s = h.double() @ w.double().T
@@ -204,6 +204,31 @@ def test_more_tokens_than_a_scan(dt):
     """The live tokens are numbered 8192 at a time."""
     check(*make(9001, 64, 300, dt, seed=16, masked=0.3), top=4)
     check(*make(16385, 40, 70, dt, seed=17), top=2)
+
+
+@pytest.mark.parametrize("top", [0, 1, 20, 32])
+@pytest.mark.parametrize("n", [5, 40, 296, 297])
+def test_few_tokens_of_many_ranges(n, top):
+    """Eight warps a token, or one: masks, a NaN, a label outside, equal logits."""
+    import aethelstream_b200 as A
+    v = 66001
+    h, w, lab = grid(n, 64, v, torch.bfloat16, n, 2)
+    w[20000:60000] = w[7]
+    h[1, 3], lab[2], lab[3] = float("nan"), IGNORE, v
+    r = A.token_log_probs(h, w, lab, top_k=top)
+    A._lib.device_error_bits(0)
+    s = h.double() @ w.double().T
+    logs = torch.log_softmax(s, 1)
+    good = torch.ones(n, dtype=torch.bool, device="cuda")
+    good[1:4] = False
+    bound = 2.0 ** -18 * (1 + torch.logsumexp(s, 1).abs())
+    close(r.log_probs[good], logs.gather(1, lab.clamp(0, v - 1)[:, None])[:, 0][good], bound[good])
+    close(r.entropy[good], -(logs.exp() * logs).sum(1)[good], bound[good] * 12)
+    assert r.log_probs[1].isnan() and r.log_probs[2] == 0 and r.log_probs[3].isnan()
+    if top:
+        want = torch.argsort(s, dim=1, descending=True, stable=True)[:, :top]
+        assert torch.equal(r.top_ids[good], want[good]) and (r.top_ids[1:4] == -1).all()
+        close(r.top_log_probs[good], logs.gather(1, want)[good], bound[good, None].expand(-1, top))
 
 
 @pytest.mark.parametrize("masked", [0.3, 0.9, 1.0])
