@@ -107,8 +107,9 @@ def adamw_step(params, grads, state: AdamWState, config: AdamWConfig | None = No
     g = clip * gradient,
       m = beta1 m + (1 - beta1) g, v = beta2 v + (1 - beta2) g^2,
       p -= lr (m / (1 - beta1^t) / (sqrt(v / (1 - beta2^t)) + eps) + weight_decay p).
-    `grads`: one for each tensor, of its shape and any of the three types; None
-    leaves the tensor and its moments as they are.  clip: a float32 on the device
+    `grads`: one for each tensor, of its shape and any of the three types, and not
+    in the memory of another tensor; None leaves the tensor and its moments as they
+    are.  clip: a float32 on the device
     (what ``GaLoreOptimizer.finish_step`` leaves in its clip_out).  decay: a truth
     value for each tensor, whether weight_decay applies to it (None: to all).
     lr: a float32 on the device in config.lr's place, for a captured step."""
@@ -156,7 +157,7 @@ def adamw_step(params, grads, state: AdamWState, config: AdamWConfig | None = No
         raise ValueError(f"{what}: tensors that the step writes share memory")
     if st:
         L.check(st, "aeth_adamw_step")
-    torch.autograd.graph.increment_version(params)  # a backward pass that saved one of them is told
+    torch.autograd.graph.increment_version(here)  # a backward pass that saved one of them is told
 
 
 def adamw_moments(state: AdamWState) -> tuple[torch.Tensor, torch.Tensor]:

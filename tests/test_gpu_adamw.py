@@ -198,6 +198,25 @@ def test_many_blocks(A, maps, bits):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
+def test_more_elements_than_32_bits_count(A, bits):
+    """Blocks on both sides of element 2^31, and a tensor behind them: as alone."""
+    n = 2 ** 31 + 3 * BLOCK + 77
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    big, grad = (torch.empty(n, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    big.normal_(generator=gen)
+    grad.normal_(generator=gen)
+    small, small_grad = tensors(gen, [700, 700], [torch.bfloat16] * 2)
+    at = 2 ** 31 - 2 * BLOCK
+    alone, alone_grad = [big[at:].clone(), small.clone()], [grad[at:], small_grad]
+    state, other = A.AdamWState.zeros([big, small], bits=bits), A.AdamWState.zeros(alone, bits=bits)
+    for _ in range(2):
+        A.adamw_step([big, small], [grad, small_grad], state)
+        A.adamw_step(alone, alone_grad, other)
+    assert torch.equal(big[at:], alone[0]) and torch.equal(small, alone[1])
+    assert torch.equal(state.m[at:], other.m) and torch.equal(state.v[at:], other.v)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
 def test_gradients_at_the_edges(A, maps, bits):
     """Zeros, numbers whose squares vanish, the largest ones, infinities and NaN:
     what is not finite stays in its tensor (with 8 bits: in its block)."""
@@ -262,6 +281,15 @@ def test_saved_tensors_know(A):
     A.adamw_step([p], [torch.ones(8, device="cuda")], A.AdamWState.zeros([p]))
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+def test_a_tensor_left_out_is_not_marked(A):
+    """One without a gradient is as it was, for a backward pass that saved it too."""
+    p, q = (torch.ones(8, device="cuda", requires_grad=True) for _ in range(2))
+    y = (q * q).sum()
+    A.adamw_step([p, q], [torch.ones(8, device="cuda"), None], A.AdamWState.zeros([p, q]))
+    y.backward()
+    assert (q.grad == 2).all() and (p != 1).all()
 
 
 def test_refusals(A):
