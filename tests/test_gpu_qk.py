@@ -259,6 +259,22 @@ def test_stretches_of_many_rows(A):
     assert all(torch.equal(a, b) for a, b in zip(got, again))
 
 
+@pytest.mark.parametrize("d, heads", [(128, 64), (33, 200)])
+def test_more_features_than_32_bits_count(A, d, heads):
+    """Tokens on both sides of feature 2^31: as alone."""
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    plan = A.RotaryPlan(32, device="cuda")
+    n = 2 ** 31 // (heads * d) + 37
+    q, dq = (torch.empty(n, heads, d, dtype=torch.bfloat16, device="cuda").normal_(generator=gen) for _ in range(2))
+    w = torch.randn(d, generator=gen, device="cuda")
+    pos = torch.arange(n, device="cuda")
+    s = slice(n - 80, n)
+    assert torch.equal(A.rotary(q, None, pos, plan)[0][s], A.rotary(q[s], None, pos[s], plan)[0])
+    assert torch.equal(A.qk_norm_rotary(q, None, w, None, pos, plan)[0][s], A.qk_norm_rotary(q[s], None, w, None, pos[s], plan)[0])
+    assert torch.equal(A.qk_norm_rotary_backward(dq, None, q, None, w, None, pos, plan)[0][s],
+                       A.qk_norm_rotary_backward(dq[s], None, q[s], None, w, None, pos[s], plan)[0])
+
+
 @pytest.mark.parametrize("heads", [511, 512, 513, 32768, 32769, 40000])
 def test_many_heads(A, heads):
     """Heads in the thousands, whose rows' tokens come by a product or a comparison."""

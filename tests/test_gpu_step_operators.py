@@ -189,3 +189,43 @@ def test_one_token_after_the_other(A):
         assert (one.log_probs - r.log_probs[0, t]).abs().max() < 1e-4 and (one.entropy - r.entropy[0, t]).abs().max() < 1e-4
         if labels[0, t] >= 0:
             assert (one.top_log_probs - r.top_log_probs[0, t]).abs().max() < 1e-4
+
+
+def test_two_streams_at_once(A):
+    """Calls that run beside one another give what they give alone."""
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    plan = A.RotaryPlan(HD, device="cuda")
+    w = torch.randn(HD, device="cuda", generator=gen)
+    head = (0.05 * torch.randn(5000, D, device="cuda", generator=gen)).bfloat16()
+
+    def case(n):
+        q, dq = (torch.randn(n, H, HD, device="cuda", generator=gen).bfloat16() for _ in range(2))
+        h = torch.randn(n, D, device="cuda", generator=gen).bfloat16()
+        labels = torch.randint(0, 5000, (n,), device="cuda", generator=gen)
+        params, grads = [[torch.randn(x, device="cuda", generator=gen).bfloat16() for x in (50000, 77)] for _ in range(2)]
+        return q, dq, h, labels, torch.arange(n, device="cuda"), params, grads
+
+    def run(c):
+        q, dq, h, labels, pos, params, grads = c
+        params = [p.clone() for p in params]
+        states = [A.AdamWState.zeros(params, bits=bits) for bits in (8, 32)]
+        out = []
+        for _ in range(5):
+            out += A.qk_norm_rotary_backward(dq, None, q, None, w, None, pos, plan)[::2]
+            r = A.token_log_probs(h, head, labels, top_k=6)
+            out += [r.log_probs, r.entropy, r.top_ids, *A.token_log_probs_backward(h, head, labels, r, r.entropy, r.lse)]
+            for state in states:
+                A.adamw_step(params, grads, state)
+        return out + params + [states[0].m, states[0].v_scales, states[1].v]
+
+    cases = [case(n) for n in (3, 300, 1111)]
+    alone = [run(c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    both = []
+    for c, s in zip(cases, streams):
+        with torch.cuda.stream(s):
+            both.append(run(c))
+    torch.cuda.synchronize()
+    for x, y in zip(alone, both):
+        assert all(torch.equal(a, b) for a, b in zip(x, y))
