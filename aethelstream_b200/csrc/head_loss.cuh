@@ -69,6 +69,7 @@ struct HeadRows {
     const float *entropy, *grad_entropy;
     float bound;  // of |p (log p + entropy)|
     float4* row;
+    int twice;  // 1: live row i comes as rows 2 i and 2 i + 1 (head_round_twice); 0
     // the live rows of H, gathered to a pitch that TMA takes
     const uint16_t* h;
     int64_t ld;
@@ -120,13 +121,16 @@ __device__ __forceinline__ int64_t head_padded(int live, int64_t n) {
 // A live row of the gradient of a log p_y + b entropy: its weight w = |a| + c |b|
 // (returned, and for now in row[].w) and, of a / w and b / w, what an entry takes
 // (HeadRowGrad).
-__device__ __forceinline__ float head_probs_row(const HeadRows& a, int64_t t, int i) {
+__device__ __forceinline__ float head_probs_row(const HeadRows& a, int64_t t, int i, int lab) {
     const float ga = a.grad ? a.grad[t] : 0.0f, gb = a.grad_entropy ? a.grad_entropy[t] : 0.0f;
     const float w = fmaf(a.bound, fabsf(gb), fabsf(ga));
     const float ua = w == 0.0f ? 0.0f : ga / w, ub = w == 0.0f ? 0.0f : gb / w, gamma = ub * kLn2;
-    a.lse2[i] = a.lse[t];
-    a.row_scale[i] = w / a.g_scale;
-    a.row[i] = make_float4(ua * a.g_scale, fmaf(-gamma, a.g_bits, fmaf(ub, a.entropy[t], ua)), gamma, w);
+    for (int r = i << a.twice; r < (i + 1) << a.twice; ++r) {
+        a.lab[r] = lab;
+        a.lse2[r] = a.lse[t];
+        a.row_scale[r] = w / a.g_scale;
+        a.row[r] = make_float4(ua * a.g_scale, fmaf(-gamma, a.g_bits, fmaf(ub, a.entropy[t], ua)), gamma, w);
+    }
     return w;
 }
 
@@ -200,11 +204,11 @@ __global__ void __launch_bounds__(1024) head_rows_kernel(const __grid_constant__
                 a.pos[t] = bad ? kHeadBad : kHeadIgnored;
                 continue;
             }
-            a.pos[t] = i;
-            a.rows[i] = (int)t;
-            a.lab[i] = (int)lab[k];
+            a.pos[t] = PROBS ? i << a.twice : i;
+            a.rows[i] = (int)t;  // read where a token has one row
+            if (!PROBS) a.lab[i] = (int)lab[k];
             if (PROBS) {
-                const float w = head_probs_row(a, t, i);
+                const float w = head_probs_row(a, t, i, (int)lab[k]);
                 if (w <= 3.402823466e38f) gmax = fmaxf(gmax, w);
             } else if (a.coef) {
                 a.lse2[i] = fmaf(lse[k], kLog2e, -a.g_bits);
@@ -220,10 +224,14 @@ __global__ void __launch_bounds__(1024) head_rows_kernel(const __grid_constant__
         __syncthreads();
     }
     if (PACK) {
+        if (PROBS) base <<= a.twice;
         const int64_t g = gridDim.x, b = blockIdx.x, first = base + b;
-        head_copy_rows(a, (a.n - b + g - 1) / g, [&](int64_t r) { return b + r * g; },
-                       [&](int64_t r) { return (int64_t)spos[b + r * g]; });
-        const int64_t padded = head_padded(base, a.n);
+        for (int h = 0; h <= (PROBS ? a.twice : 0); ++h)
+            head_copy_rows(a, (a.n - b + g - 1) / g, [&](int64_t r) { return b + r * g; }, [&](int64_t r) {
+                const int64_t to = spos[b + r * g];
+                return PROBS && to >= 0 ? (to << a.twice) + h : to;
+            });
+        const int64_t padded = head_padded(base, PROBS ? a.n << a.twice : a.n);
         if (first < padded)
             head_copy_rows(a, (padded - first + g - 1) / g, [](int64_t) { return (int64_t)-1; },
                            [&](int64_t r) { return first + r * g; });
@@ -671,7 +679,6 @@ __global__ void __launch_bounds__(kHeadVecThreads, 1) head_vec_kernel(const Head
     }
 }
 
-
 // One warp a token joins the CTAs' pairs; then losses and mean.
 __global__ void __launch_bounds__(32 * kHeadVecTokens)
     head_vec_loss_kernel(const HeadVec a, int n, int ctas, float* losses, float* lse, float* loss, uint32_t* err) {
@@ -754,6 +761,25 @@ struct HeadRowGrad {
     }
 };
 
+// N numbers, times f, in 16 bits.  Where tokens are few a row of G comes twice, as
+// its rounding and as what that `left`, so that their sum is good to 2^-16 (f16: 2^-22).
+template <bool BF16, int N>
+__device__ __forceinline__ void head_round(const float (&v)[N], float f, uint32_t* w) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) w[i] = pack16<BF16>(v[2 * i] * f, v[2 * i + 1] * f);
+}
+template <bool BF16, int N>
+__device__ __forceinline__ void head_round_twice(const float (&v)[N], float f, bool left, uint32_t* w) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+        const float x = v[2 * i] * f, y = v[2 * i + 1] * f;
+        const uint32_t near = pack16<BF16>(x, y);
+        const float2 r = BF16 ? make_float2(__uint_as_float(near << 16), __uint_as_float(near & 0xffff0000u))
+                              : __half22float2(*reinterpret_cast<const __half2*>(&near));
+        w[i] = left ? pack16<BF16>(x - r.x, y - r.y) : near;
+    }
+}
+
 // Epilogue of the backward's product: G of the piece in 16 bits, as the tensor
 // cores take it for dW and dH.  G is rounded once, from fp32, which a sum over many
 // tokens or entries evens out (against 64 bits 1.9e-3 in bf16, 1.7e-3 of it the
@@ -767,7 +793,7 @@ struct HeadRowGrad {
 // UNIT (f16): the G without token weights, beside the other where that is wanted
 // (3584 x 4096 x 32000 with weights: 2.26 -> 2.42 ms, 64 tokens 178 -> 183 us).
 // PROBS: the gradient of log probability and entropy (head_probs.cuh), whose rows
-// have coefficients of their own in `row`.
+// have coefficients of their own in `row`, and where tokens are few come twice.
 template <bool BF16, bool UNIT, bool PROBS>
 struct HeadGrad {
     static constexpr int kChunk = 8;
@@ -781,6 +807,7 @@ struct HeadGrad {
     int n;   // rows of g: the tokens
     int v0;  // first vocabulary entry of the piece
     const float4* row;  // with PROBS
+    int twice;          // with PROBS: odd rows are what the rows before them left
     __device__ static void give_up(const PairTile&) {}
     __device__ __forceinline__ void finish(const PairTile& t, const float (&acc)[128]) const {
         const int r = t.row0 + t.lane;
@@ -797,10 +824,12 @@ struct HeadGrad {
                     float v[32];
                     head_slice(acc, 2 * b + h, v);
                     a.values(v, lab_c - 64 * b - 32 * h);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        w[16 * h + i] = pack16<BF16>(v[2 * i] * a.f, v[2 * i + 1] * a.f);
-                        if (UNIT) w1[16 * h + i] = pack16<BF16>(v[2 * i] * a.u, v[2 * i + 1] * a.u);
+                    if (PROBS && twice) {
+                        head_round_twice<BF16>(v, a.f, r & 1, w + 16 * h);
+                        if (UNIT) head_round_twice<BF16>(v, a.u, r & 1, w1 + 16 * h);
+                    } else {
+                        head_round<BF16>(v, a.f, w + 16 * h);
+                        if (UNIT) head_round<BF16>(v, a.u, w1 + 16 * h);
                     }
                 }
                 const int cols = min(t.N, t.col0 + t.c_end);
@@ -826,6 +855,7 @@ struct HeadGradT {
     int n;
     int v0;
     const float4* row;
+    int twice;
     __device__ static void give_up(const PairTile&) {}
     __device__ __forceinline__ void finish(const PairTile& t, const float (&acc)[128]) const {
 #pragma unroll
@@ -840,10 +870,12 @@ struct HeadGradT {
             const HeadRowGrad<BF16, PROBS> a(in, token, coef, lse2, row);
             a.values(v, in ? lab[token] - v0 - t.row0 : -1);
             uint32_t w[16], w1[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                w[i] = pack16<BF16>(v[2 * i] * a.f, v[2 * i + 1] * a.f);
-                if (UNIT) w1[i] = pack16<BF16>(v[2 * i] * a.u, v[2 * i + 1] * a.u);
+            if (PROBS && twice) {
+                head_round_twice<BF16>(v, a.f, token & 1, w);
+                if (UNIT) head_round_twice<BF16>(v, a.u, token & 1, w1);
+            } else {
+                head_round<BF16>(v, a.f, w);
+                if (UNIT) head_round<BF16>(v, a.u, w1);
             }
             if (!UNIT || g) store(t, w, c, g);
             if (UNIT) store(t, w1, c, g_unit);
@@ -881,7 +913,8 @@ struct HeadGradT {
 
 // dH of every token in 16 bits: the slab's row, plus the further K ranges of
 // the tail's tiles in their order; zero for the tokens that took no part.  A
-// CTA takes 1024 columns of tokens, TOKENS of them in flight.
+// CTA takes 1024 columns of tokens, TOKENS of them in flight.  TWICE: a token's
+// two rows, added up.
 struct HeadDh {
     const float* slab;
     int64_t ld;
@@ -895,7 +928,7 @@ struct HeadDh {
     uint16_t* out;
     int64_t ldo;
 };
-template <bool BF16, int TOKENS>
+template <bool BF16, int TOKENS, bool TWICE>
 __global__ void __launch_bounds__(128) head_dh_kernel(const HeadDh a) {
     __shared__ int sh[5];
     pdl_wait();
@@ -916,15 +949,16 @@ __global__ void __launch_bounds__(128) head_dh_kernel(const HeadDh a) {
     if (c >= a.d) return;
     const bool whole = (a.ldo % 8) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && c + 8 <= a.d;
     for (int64_t t0 = blockIdx.x; t0 < a.n; t0 += TOKENS * (int64_t)gridDim.x) {
-        float4 v[TOKENS][2];
+        constexpr int R = TWICE ? 2 : 1;
+        float4 v[TOKENS][2 * R];
         int p[TOKENS];
 #pragma unroll
         for (int k = 0; k < TOKENS; ++k) {
             const int64_t t = t0 + (int64_t)k * gridDim.x;
             p[k] = t < a.n ? a.pos[t] : kHeadIgnored;
 #pragma unroll
-            for (int h = 0; h < 2; ++h)  // ld is a multiple of 8
-                v[k][h] = p[k] >= 0 ? *reinterpret_cast<const float4*>(a.slab + p[k] * a.ld + c + 4 * h)
+            for (int h = 0; h < 2 * R; ++h)  // ld is a multiple of 8
+                v[k][h] = p[k] >= 0 ? *reinterpret_cast<const float4*>(a.slab + (p[k] + h / 2) * a.ld + c + 4 * (h & 1))
                                     : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
 #pragma unroll
@@ -934,17 +968,23 @@ __global__ void __launch_bounds__(128) head_dh_kernel(const HeadDh a) {
             if (p[k] >= 0) {
                 const int i = (a.live_n ? pair_tile_index(c / 256, p[k] / bt, tiles_d, tiles_t)
                                         : pair_tile_index(p[k] / bt, c / 256, tiles_t, tiles_d)) - full;
-                if (i >= 0) {
+                if (i >= 0) {  // of two rows too: they are in one tile, whose width is even
                     const float* e = a.extra + ((int64_t)i * 256 + p[k] % bt) * 256 + c % 256;
 #pragma unroll(TOKENS == 1 ? 12 : 4)
                     for (int s = 0; s + 1 < splits; ++s)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const float4 x = *reinterpret_cast<const float4*>(e + (int64_t)s * rest * 65536 + 4 * h);
+                        for (int h = 0; h < 2 * R; ++h) {
+                            const float4 x = *reinterpret_cast<const float4*>(e + (int64_t)s * rest * 65536 + 256 * (h / 2) + 4 * (h & 1));
                             v[k][h] = make_float4(v[k][h].x + x.x, v[k][h].y + x.y, v[k][h].z + x.z, v[k][h].w + x.w);
                         }
                 }
             }
+            if (TWICE)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float4 x = v[k][2 * R - 2 + h];
+                    v[k][h] = make_float4(v[k][h].x + x.x, v[k][h].y + x.y, v[k][h].z + x.z, v[k][h].w + x.w);
+                }
             uint32_t w[4] = {0, 0, 0, 0};
             const float scale = a.scale || p[k] < 0 ? scale_all : a.row_scale[p[k]];
             if (p[k] >= 0)

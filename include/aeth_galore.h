@@ -557,7 +557,8 @@ int aeth_cut_ce_backward(const void* hidden, int64_t ld_hidden, const void* weig
  *   256 entries where these take more), else not at all.
  *   backward: of sum_t grad_log_probs[t] log_probs[t] + grad_entropy[t] entropy[t]
  *   (either may be NULL: 0), lse and entropy being the forward's; G as the loss's,
- *   in F16 twice where d_hidden is wanted. */
+ *   in F16 twice where d_hidden is wanted, and up to 128 tokens as its rounding and
+ *   what that left, good to 2^-16 (F16: 2^-22). */
 int aeth_token_log_probs_workspace(int64_t n, int64_t d, int64_t vocab, int top, int backward, size_t* bytes);
 int aeth_token_log_probs(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, int dtype,
                          const int64_t* labels, int64_t n, int64_t d, int64_t vocab, int64_t ignore_index, int top,
@@ -667,8 +668,9 @@ int aeth_qk_norm_rotary_backward(const AethRotaryPlan* plan, const void* positio
  *     holds a NaN or an infinity).  master (or NULL): fp32 parameters laid out as
  *     the moments, which the step is taken on; p gets their rounding.
  *     m, v and master 16-byte aligned.  Parameters that overlap one another:
- *     AETH_ERR_ARG.  Nothing synchronises; with bits 32 nothing allocates, with
- *     bits 8 the library's first call on a device uploads its maps.
+ *     AETH_ERR_ARG; a gradient must not overlap another tensor's parameter.
+ *     Nothing synchronises; with bits 32 nothing allocates, with bits 8 the
+ *     library's first call on a device uploads its maps.
  * ====================================================================== */
 typedef struct {
     int bits; /* 32 or 8 */

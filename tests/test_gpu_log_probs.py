@@ -8,7 +8,8 @@ Tolerances (u = 2^-8 for bf16, 2^-11 for f16, half a step relative):
     and the logarithm;
   entropy: d entropy / d s_v = -p_v (q_v + entropy), whose sizes add up to 2 entropy
     at most: e_s twice of that, and the same 2^-18 (1 + |lse| + entropy);
-  G = a 1[y] - p (a + b (q + entropy)): relative u (rounded once), the error of its
+  G = a 1[y] - p (a + b (q + entropy)): relative u (rounded once; up to 128 tokens
+    u^2: kept as its rounding and the rounding of what that left), the error of its
     exponent, those of q and of the entropy times p |b|, and f16's spacing beside
     the largest weight; times |W| or |H| and summed;
   outputs: rounded once more.
@@ -55,7 +56,7 @@ def reference(h, w, lab, a, b):
     e_s = (hd.abs() @ wd.abs().T).amax(1) * (2 * d * 2.0 ** -24)
     e_lp = 2 * e_s + 2.0 ** -18 * (1 + lse.abs())
     e_ent = 4 * e_s * ent + 2.0 ** -18 * (1 + lse.abs() + ent)
-    e_g = G.abs() * (U[dt] + 2.0 ** -20) + p * slope.abs() * e_lp[:, None] + p * (b.abs() * (e_lp + e_ent))[:, None]
+    e_g = G.abs() * ((U[dt] if n > 128 else U[dt] ** 2) + 2.0 ** -20) + p * slope.abs() * e_lp[:, None] + p * (b.abs() * (e_lp + e_ent))[:, None]
     if dt is torch.float16:
         e_g += 2.0 ** -40 * (a.abs() + (math.log(v) / 4 + 0.5) * b.abs()).max()
     dh, dw = G @ wd, G.T @ hd
@@ -396,6 +397,36 @@ def test_strides_shapes_and_label_types():
     for x, y in ((r2.log_probs, r.log_probs), (r2.entropy, r.entropy), (r2.top_log_probs, r.top_log_probs), (r2.top_ids, r.top_ids)):
         assert torch.equal(x.flatten(0, 1), y)
     assert torch.equal(dh2.view(24, 64), dh) and torch.equal(dw2, dw)
+
+
+@pytest.mark.parametrize("n", [1, 2, 5, 33, 127, 128, 129])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_gradients_of_few_tokens(dt, n):
+    """Weights just above powers of two, which 16 bits round the most: nothing evens
+    that out where a token or two make up a row."""
+    h, w, lab = make(n, 264, 1200, dt, seed=18, masked=0.3 if n > 5 else 0.0)
+    a, b = grads(n, 19)
+    a = a.sign() * (1.0 + 0.9 * U[dt])
+    check(h, w, lab, a=a, b=1e-3 * b)
+
+
+@pytest.mark.parametrize("n", [3, 40, 600])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_without_gradients_and_an_entry_as_the_ignored(dt, n):
+    import aethelstream_b200 as A
+    h, w, lab = make(n, 72, 900, dt, seed=16, masked=0.4)
+    r = A.token_log_probs(h, w, lab, top_k=2)
+    dh, dw = A.token_log_probs_backward(h, w, lab, r)
+    assert (dh == 0).all() and (dw == 0).all()
+    a, b = grads(n, 17)
+    lab = torch.where(lab == 5, 6, lab)
+    r = A.token_log_probs(h, w, lab, top_k=2)
+    want = A.token_log_probs_backward(h, w, lab, r, grad_log_probs=a, grad_entropy=b)
+    other = torch.where(lab == IGNORE, 5, lab)
+    s = A.token_log_probs(h, w, other, top_k=2, ignore_index=5)
+    got = A.token_log_probs_backward(h, w, other, s, grad_log_probs=a, grad_entropy=b, ignore_index=5)
+    for x, y in ((r.log_probs, s.log_probs), (r.entropy, s.entropy), (r.lse, s.lse), (r.top_ids, s.top_ids), *zip(want, got)):
+        assert torch.equal(x, y)
 
 
 def test_nothing_to_do():
