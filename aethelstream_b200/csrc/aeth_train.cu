@@ -79,9 +79,15 @@ struct HeadPlan {
     int tail_kb;    // k-blocks of a piece's dH product
     int64_t extra;  // buffers of its tail
     int gs;         // G's of a piece: a second one without the token weights (head_loss.cuh)
+    int64_t g_rows;  // of a G
 
-    HeadPlan(int64_t n, int64_t d, int64_t vocab, int gs_ = 1) : gs(gs_) {
+    // probs: the gradient of log probabilities, whose G has no rows but the tokens' (what
+    // TMA reads past them is zero) and whose pieces are as good as equal where that
+    // takes no more waves: a small last one leaves CTA pairs idle (311 tokens, 155 of
+    // them live, x 2048 x 131071 f16: 482 us with rows and pieces as the loss's, 395)
+    HeadPlan(int64_t n, int64_t d, int64_t vocab, int gs_ = 1, bool probs = false) : gs(gs_) {
         n_pad = up(std::max<int64_t>(n, 1), 256);
+        g_rows = probs ? std::max<int64_t>(n, 1) : n_pad;
         dp = up(d, 8);
         live_n = head_tokens_as_columns(n);
         bn = head_bn(n_pad / 256, vocab);
@@ -93,9 +99,14 @@ struct HeadPlan {
         // a piece is a number of 256-entry tiles whose G's fit beside them; of those, from the
         // largest down to half of it (64 are looked at), the one with the fewest waves of tiles over all pieces
         const int64_t all = (vocab + 255) / 256;
-        const int64_t fit = std::max<int64_t>((kHeadPieceBytes - extra * 262144) / (512 * n_pad * gs), 1);
+        const int64_t fit = std::max<int64_t>((kHeadPieceBytes - extra * 262144) / (512 * g_rows * gs), 1);
         int64_t best = fit, least = INT64_MAX;
         auto waves = [&](int64_t tiles) { return (tiles * tiles_m + pairs - 1) / pairs; };
+        if (probs && fit < all) {
+            const int64_t count = (all + fit - 1) / fit;
+            best = (all + count - 1) / count;
+            least = all / best * waves(best) + waves(all % best);
+        }
         for (int64_t p = fit; p >= std::max((fit + 1) / 2, fit - 64) && fit < all; --p) {
             const int64_t cost = all / p * waves(p) + waves(all % p);
             if (cost < least) {
@@ -145,8 +156,8 @@ struct HeadWork {
             lse2 = c.take<float>(p.n_pad);
             row_scale = c.take<float>(p.n_pad);
             out_scale = c.take<float>(1);
-            g = c.take<uint16_t>(p.n_pad * p.ldg);
-            g_unit = p.gs > 1 ? c.take<uint16_t>(p.n_pad * p.ldg) : g;
+            g = c.take<uint16_t>(p.g_rows * p.ldg);
+            g_unit = p.gs > 1 ? c.take<uint16_t>(p.g_rows * p.ldg) : g;
             slab = c.take<float>(p.n_pad * p.dp);
             extra = c.take<float>(p.extra * 65536);
         }
@@ -628,9 +639,9 @@ int aeth_token_log_probs_workspace(int64_t n, int64_t d, int64_t vocab, int top,
     if (n < 0 || d <= 0 || vocab <= 0 || top < 0 || !bytes) return set_err(AETH_ERR_ARG);
     if (n > kHeadMaxDim || d > kHeadMaxDim || vocab > kHeadMaxDim || top > kHeadTop) return set_err(AETH_ERR_UNSUPPORTED);
     if (backward) {
-        const int64_t rows = n << probs_twice(n);
-        AETH_TRY(aeth_cut_ce_workspace(rows, d, vocab, 1, bytes));
-        *bytes += (size_t)up(HeadPlan(rows, d, vocab).n_pad * (int64_t)sizeof(float4), 256);
+        const HeadPlan one(n << probs_twice(n), d, vocab, 1, true), two(n << probs_twice(n), d, vocab, 2, true);
+        *bytes = std::max(HeadWork(one, n, true, nullptr).bytes, HeadWork(two, n, true, nullptr).bytes) +
+                 (size_t)up(one.n_pad * (int64_t)sizeof(float4), 256);
     } else {
         *bytes = ProbsWork(ProbsPlan(n, d, vocab, top), n, d, vocab, nullptr).bytes;
     }
@@ -693,7 +704,7 @@ int aeth_token_log_probs_backward(const void* hidden, int64_t ld_hidden, const v
     }
     const bool bf16 = dtype == AETH_DTYPE_BF16, unit = !bf16 && d_hidden;
     const int twice = probs_twice(n);
-    const HeadPlan p(n << twice, d, vocab, unit ? 2 : 1);
+    const HeadPlan p(n << twice, d, vocab, unit ? 2 : 1, true);
     const HeadWork w(p, n, true, workspace);
     Carver c(workspace);
     c.used = w.bytes;
