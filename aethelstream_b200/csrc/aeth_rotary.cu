@@ -60,7 +60,7 @@ bool rot_whole(const RotaryCall& c) {
            reinterpret_cast<uintptr_t>(c.k_out) % 16 == 0;
 }
 
-// Rows of a stretch and CTAs of rotary_any_kernel's grid.  A stretch is what gives
+// Rows of a stretch and CTAs of rotary_any_kernel's and rotary_pairs_kernel's grid.  A stretch is what gives
 // every SM six CTAs, 512 rows at most and what the table of its tokens holds;
 // `most`: CTAs that q and k may have together (0: one for each stretch).
 void rot_grid(RotaryArgs& a, int64_t tokens, int step, int most) {
@@ -95,11 +95,13 @@ constexpr int rot_per_sm() { return OP == ROT_NORM_BACK ? 2 : 3; }
 constexpr int kRotPasses = 8;
 template <int OP>
 constexpr int rot_waves() { return OP == ROT_TURN ? 3 : OP == ROT_NORM ? 2 : 1; }
-int rot_back_ctas() { return rot_per_sm<ROT_NORM_BACK>() * num_sms(); }  // each leaves sums of the gains'
+// CTAs of the gradient, each of which leaves sums of the gains', at most: rotary_kernel
+// has two an SM, the others four
+int rot_back_ctas() { return 4 * num_sms(); }
 
 template <typename T, bool INTER, int OP>
 int rot_launch(RotaryArgs& a, int64_t tokens, bool whole, cudaStream_t st) {
-    static std::atomic<bool> allowed[2][kMaxDevices] = {};
+    static std::atomic<bool> allowed[4][kMaxDevices] = {};
     if (whole && a.D % 16 == 0 && a.R % 16 == 0 && a.D <= 512) {
         int lanes = 1;
         while (lanes < a.D / 16) lanes *= 2;
@@ -121,7 +123,13 @@ int rot_launch(RotaryArgs& a, int64_t tokens, bool whole, cudaStream_t st) {
         rot_grid(a, tokens, kRotThreads / 32, OP == ROT_NORM_BACK ? rot_back_ctas() : 0);
         const int smem = a.table_bytes + (OP == ROT_NORM_BACK ? kRotThreads / 32 * a.D * 4 : 0);
         auto kern = rotary_any_kernel<T, INTER, OP>;
-        AETH_TRY(allow_shared(kern, 2 * kRotTableBytes, allowed[1]));
+        int one = 1;
+        if constexpr (OP != ROT_TURN)
+            if (a.D <= 256) {
+                kern = a.D <= 128 ? rotary_pairs_kernel<T, INTER, OP, 2> : rotary_pairs_kernel<T, INTER, OP, 4>;
+                one = a.D <= 128 ? 2 : 3;
+            }
+        AETH_TRY(allow_shared(kern, 2 * kRotTableBytes, allowed[one]));
         kern<<<a.s[0].ctas + a.s[1].ctas, kRotThreads, smem, st>>>(a);
     }
     AETH_LAUNCH_CHECK();

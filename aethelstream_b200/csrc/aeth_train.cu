@@ -82,7 +82,7 @@ struct HeadPlan {
     int64_t g_rows;  // of a G
 
     // probs: the gradient of log probabilities, whose G has no rows but the tokens' (what
-    // TMA reads past them is zero) and whose pieces are as good as equal where that
+    // TMA reads past them is zero) and whose pieces are equal where that
     // takes no more waves: a small last one leaves CTA pairs idle (311 tokens, 155 of
     // them live, x 2048 x 131071 f16: 482 us with rows and pieces as the loss's, 395)
     HeadPlan(int64_t n, int64_t d, int64_t vocab, int gs_ = 1, bool probs = false) : gs(gs_) {

@@ -23,8 +23,8 @@
 // memory first, each for all the heads of q and k.  A lane's rows to come are on
 // their way to shared memory by asynchronous copies of its own, which it alone
 // reads: bytes in flight without registers, and no barrier.  8192 tokens x (64 + 8)
-// heads x 128 bf16: rotation 56 us (5.4 TB/s), with the norm 62 (4.9), the gradient
-// 92 (4.9), where a copy of as many bytes takes 50, 50 and 73.  What is left is
+// heads x 128 bf16: rotation 52 us (5.8 TB/s), with the norm 58 (5.2), the gradient
+// 86 (5.3), where a copy of as many bytes takes 50, 50 and 73.  What is left is
 // the instructions of a row (issue slots half taken) and a CTA's first microsecond,
 // its table; with rows straight from global memory to registers it took 66, 82 and
 // 162 us, with q's rows and k's in CTAs of their own 72, 78 and 123.
@@ -50,8 +50,8 @@ struct RotaryRows {  // one of q and k
     int heads;
     uint32_t magic;  // of rot_quotient
     int64_t rows;    // tokens x heads
-    int stretch;     // rotary_any_kernel: rows of a stretch, of which a CTA takes every ctas-th
-    unsigned ctas;   // CTAs that have rows of it (rotary_any_kernel: for it alone)
+    int stretch;     // not rotary_kernel: rows of a stretch, of which a CTA takes every ctas-th
+    unsigned ctas;   // CTAs that have rows of it (not rotary_kernel: for it alone)
 };
 struct RotaryArgs {
     RotaryRows s[2];  // q, k
@@ -63,7 +63,7 @@ struct RotaryArgs {
     int flip;              // the other way round
     int D, R, gain_dtype;
     float eps;
-    int table_bytes;  // rotary_any_kernel: shared memory before the sums
+    int table_bytes;  // not rotary_kernel: shared memory before the sums
 };
 
 __device__ __forceinline__ float2 rot_angle(uint64_t t, float amp, bool flip) {
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(kRotThreads, CTAS) rotary_kernel(const __grid_
 
 // Heads that 16 features or 16 bytes do not divide: a warp takes a row, a lane
 // every 32nd pair and feature of the rest, one element at a time.  The second
-// pass over a row finds it in L1.
+// pass over a row finds it in L1.  For the rotation and heads above 256 features.
 template <typename T, bool INTER, int OP>
 __global__ void __launch_bounds__(kRotThreads) rotary_any_kernel(const __grid_constant__ RotaryArgs a) {
     extern __shared__ float4 rot_sh[];
@@ -463,6 +463,130 @@ __global__ void __launch_bounds__(kRotThreads) rotary_any_kernel(const __grid_co
         }
     }
     if (OP == ROT_NORM_BACK) {
+        __syncthreads();
+        for (int d = threadIdx.x; d < a.D; d += kRotThreads) {
+            float t = 0.0f;
+            for (int w = 0; w < kWarps; ++w) t += sums[w * a.D + d];
+            s.part[(int64_t)cta * a.D + d] = t;
+        }
+    }
+}
+
+// The norms of such heads up to 256 features and their gradients: a lane has NP pairs
+// at most, whose gains and sums of the gains' gradient stay in registers, and the row
+// after is on its way meanwhile.  Features that do not turn make pairs of neighbours;
+// the last may lack its second.  2047 x (32 + 8) x 80, 40 turning, bf16: norm 24 us,
+// gradient 44 (rotary_any_kernel 29 and 91); 8192 x (32 + 32) x 80, 20 turning: 126 and
+// 208 (202 and 793).  The rotation alone is no faster so (19 us, 18; 106, 98), nor is
+// the norm of 513 features with nine pairs a lane (63, 39).
+template <typename T, bool INTER, int OP, int NP>
+__global__ void __launch_bounds__(kRotThreads) rotary_pairs_kernel(const __grid_constant__ RotaryArgs a) {
+    extern __shared__ float4 rot_sh[];
+    float* table = reinterpret_cast<float*>(rot_sh);
+    constexpr int kWarps = kRotThreads / 32;
+    constexpr bool kBack = OP == ROT_NORM_BACK;
+    float* sums = table + a.table_bytes / 4;  // [warp][D]
+    const int which = blockIdx.x >= a.s[0].ctas ? 1 : 0;
+    const RotaryRows& s = a.s[which];
+    const unsigned cta = blockIdx.x - (which ? a.s[0].ctas : 0);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = a.R / 2, pairs = half + (a.D - a.R + 1) / 2;
+    auto each = [&](auto f) {  // f(j, its features, whether both are there) of the lane's pairs
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            const int p = 32 * j + lane;
+            const int d = p >= half ? a.R + 2 * (p - half) : INTER ? 2 * p : p, e = p >= half || INTER ? d + 1 : d + half;
+            if (p < pairs) f(j, d, e, e < a.D);
+        }
+    };
+    float gu[NP], gv[NP], wu[NP], wv[NP];
+#pragma unroll
+    for (int j = 0; j < NP; ++j) gu[j] = gv[j] = wu[j] = wv[j] = 0.0f;
+    each([&](int j, int d, int e, bool both) {
+        gu[j] = load_as_f32(s.gain, d, a.gain_dtype);
+        gv[j] = both ? load_as_f32(s.gain, e, a.gain_dtype) : 0.0f;
+    });
+    auto load = [&](const T* x, T (&u)[NP], T (&v)[NP]) {
+#pragma unroll
+        for (int j = 0; j < NP; ++j) u[j] = v[j] = T(0.0f);
+        each([&](int j, int d, int e, bool both) {
+            u[j] = x[d];
+            if (both) v[j] = x[e];
+        });
+    };
+    for (int64_t r0 = (int64_t)cta * s.stretch; r0 < s.rows; r0 += (int64_t)s.ctas * s.stretch) {
+        const int64_t t0 = r0 / s.heads;
+        const int h0 = (int)(r0 - t0 * s.heads), count = (int)min((int64_t)s.stretch, s.rows - r0);
+        __syncthreads();
+        rot_table(a, table, t0, (h0 + count - 1) / s.heads + 1, [](int p) { return p; });
+        __syncthreads();
+        T xu[NP], xv[NP], du[NP], dv[NP];
+        auto fetch = [&](int i) {  // row i of the stretch
+            if (i >= count) return;
+            const int tok = rot_quotient(h0 + i, s.heads, s.magic), h = h0 + i - tok * s.heads;
+            load(static_cast<const T*>(s.x) + (t0 + tok) * s.ld_t + h * s.ld_h, xu, xv);
+            if (kBack) load(static_cast<const T*>(s.dy) + (t0 + tok) * s.ld_dt + h * s.ld_dh, du, dv);
+        };
+        fetch(warp);
+        for (int i = warp; i < count; i += kWarps) {
+            T* o = static_cast<T*>(s.out) + (r0 + i) * a.D;
+            const float* cs = table + rot_quotient(h0 + i, s.heads, s.magic) * a.R;
+            float u[NP], v[NP], eu[NP], ev[NP], sq = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NP; ++j) {
+                u[j] = (float)xu[j];
+                v[j] = (float)xv[j];
+                eu[j] = kBack ? (float)du[j] : 0.0f;
+                ev[j] = kBack ? (float)dv[j] : 0.0f;
+                sq = fmaf(v[j], v[j], fmaf(u[j], u[j], sq));
+            }
+            fetch(i + kWarps);
+            const float r = rsqrtf(rot_sum(sq, 32) / (float)a.D + a.eps);
+            auto turn = [&](float (&x)[NP], float (&y)[NP]) {
+#pragma unroll
+                for (int j = 0; j < NP; ++j) {
+                    const int p = 32 * j + lane;
+                    if (p >= half) continue;
+                    const float co = cs[p], si = cs[half + p], was = x[j];
+                    x[j] = x[j] * co - y[j] * si;
+                    y[j] = y[j] * co + was * si;
+                }
+            };
+            if (kBack) {
+                float dot = 0.0f;
+                turn(eu, ev);
+#pragma unroll
+                for (int j = 0; j < NP; ++j) {
+                    wu[j] = fmaf(eu[j], u[j] * r, wu[j]);
+                    wv[j] = fmaf(ev[j], v[j] * r, wv[j]);
+                    eu[j] *= gu[j];
+                    ev[j] *= gv[j];
+                    dot = fmaf(ev[j], v[j], fmaf(eu[j], u[j], dot));
+                }
+                dot = rot_sum(dot, 32) / (float)a.D * (r * r * r);
+#pragma unroll
+                for (int j = 0; j < NP; ++j) {
+                    u[j] = r * eu[j] - u[j] * dot;
+                    v[j] = r * ev[j] - v[j] * dot;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < NP; ++j) {
+                    u[j] = u[j] * r * gu[j];
+                    v[j] = v[j] * r * gv[j];
+                }
+                turn(u, v);
+            }
+            each([&](int j, int d, int e, bool both) {
+                o[d] = (T)u[j];
+                if (both) o[e] = (T)v[j];
+            });
+        }
+    }
+    if (kBack) {
+        each([&](int j, int d, int e, bool both) {
+            sums[warp * a.D + d] = wu[j];
+            if (both) sums[warp * a.D + e] = wv[j];
+        });
         __syncthreads();
         for (int d = threadIdx.x; d < a.D; d += kRotThreads) {
             float t = 0.0f;

@@ -74,7 +74,8 @@ def rows(gen, shape, dtype, how):
 SHAPES = [  # tokens, heads of q and k, features, those that turn
     (1, 1, 1, 2, 2), (1, 64, 8, 128, 128), (3, 5, 1, 16, 16), (77, 8, 2, 128, 128), (33, 3, 1, 96, 64), (65, 4, 4, 80, 80),
     (21, 6, 2, 80, 40), (130, 2, 1, 64, 32), (9, 3, 2, 18, 6), (12, 2, 1, 256, 256), (7, 2, 1, 512, 128), (5, 1, 1, 1024, 1024),
-    (6, 2, 1, 513, 512), (700, 1, 1, 32, 32), (4, 71, 1, 192, 96)]
+    (6, 2, 1, 513, 512), (700, 1, 1, 32, 32), (4, 71, 1, 192, 96),
+    (9, 3, 2, 33, 32), (11, 2, 1, 129, 2), (50, 2, 3, 255, 250), (13, 4, 1, 256, 24)]
 
 
 @pytest.mark.parametrize("how", ["whole", "fused", "off"])
