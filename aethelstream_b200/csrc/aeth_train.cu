@@ -199,7 +199,7 @@ int head_rows(HeadRows a, const int64_t* labels, int64_t n, int64_t d, int64_t v
     a.ldo = p.dp;
     const unsigned ctas = (unsigned)std::min<int64_t>(n, num_sms());
     if (n <= kHeadScan) {
-        auto kern = a.row ? head_rows_kernel<true, true> : head_rows_kernel<true, false>;
+        auto kern = !a.row ? head_rows_kernel<true, false> : a.twice ? head_rows_kernel<true, true, true> : head_rows_kernel<true, true>;
         kern<<<ctas, 1024, 0, st>>>(a, rt->err_word);
         AETH_LAUNCH_CHECK();
     } else {
@@ -228,28 +228,28 @@ int head_vec(const HeadVec& a, int64_t n, int ctas, float* losses, float* lse, f
 }
 
 // UNIT: d_hidden comes from a G without the token weights.  PROBS: the gradient of
-// log probabilities and entropies, its rows' coefficients in `row`, and where `twice`
-// is 1 two rows for a token (rows of G: n << twice)
-template <bool BF16, bool UNIT, bool PROBS = false>
+// log probabilities and entropies, its rows' coefficients in `row`; TWICE: two rows
+// of G for a token
+template <bool BF16, bool UNIT, bool PROBS = false, bool TWICE = false>
 int head_backward(const HeadPlan& p, const HeadWork& w, const void* weight, int64_t ld_weight, int64_t n, int64_t d,
-                  int64_t vocab, const float4* row, int twice, void* d_hidden, int64_t ld_dh, void* d_weight, int64_t ld_dw,
+                  int64_t vocab, const float4* row, void* d_hidden, int64_t ld_dh, void* d_weight, int64_t ld_dw,
                   cudaStream_t st) {
     const uint16_t* W = static_cast<const uint16_t*>(weight);
     const int64_t tokens = n;
-    n <<= twice;
+    if (TWICE) n *= 2;
     uint16_t *g = UNIT && !d_weight ? nullptr : w.g, *g_unit = UNIT ? w.g_unit : nullptr;
     for (int64_t v0 = 0; v0 < vocab; v0 += p.piece) {
         const int64_t vp = std::min(p.piece, vocab - v0);
         const PairOperand H{w.h, p.dp, n, d}, Wp{W + v0 * ld_weight, ld_weight, vp, d};
         const PairOperand G{w.g, p.ldg, n, vp}, Gh{UNIT ? w.g_unit : w.g, p.ldg, n, vp};
         if (p.live_n) {
-            using Epi = HeadGradT<BF16, UNIT, PROBS>;
-            const Epi eg{w.lab, w.coef, w.lse2, g, g_unit, p.ldg, (int)n, (int)v0, row, twice};
+            using Epi = HeadGradT<BF16, UNIT, PROBS, TWICE>;
+            const Epi eg{w.lab, w.coef, w.lse2, g, g_unit, p.ldg, (int)n, (int)v0, row};
             AETH_TRY((pair_gemm_launch<Epi, false, false>(Wp, H, (int)vp, (int)n, (int)d, w.count, PAIR_LIVE_N, 256, 0, BF16,
                                                           eg, st)));
         } else {
-            using Epi = HeadGrad<BF16, UNIT, PROBS>;
-            const Epi eg{w.lab, w.coef, w.lse2, g, g_unit, p.ldg, (int)n, (int)v0, row, twice};
+            using Epi = HeadGrad<BF16, UNIT, PROBS, TWICE>;
+            const Epi eg{w.lab, w.coef, w.lse2, g, g_unit, p.ldg, (int)n, (int)v0, row};
             AETH_TRY((pair_gemm_launch<Epi, false, false>(H, Wp, (int)n, (int)vp, (int)d, w.count, PAIR_LIVE_M,
                                                           head_bn(p.n_pad / 256, vp), 0, BF16, eg, st)));
         }
@@ -276,7 +276,7 @@ int head_backward(const HeadPlan& p, const HeadWork& w, const void* weight, int6
         const unsigned cols = (unsigned)((d + 1023) / 1024);
         const int64_t rows = std::max<int64_t>(16 * num_sms() / cols, 1);
         // few tokens: one at a time, and more of its parts
-        if (twice) AETH_CUDA(launch_after(head_dh_kernel<BF16, 1, PROBS>, dim3((unsigned)tokens, cols), dim3(128), 0, st, 1, a));
+        if (TWICE) AETH_CUDA(launch_after(head_dh_kernel<BF16, 1, TWICE>, dim3((unsigned)tokens, cols), dim3(128), 0, st, 1, a));
         else if (n <= rows) AETH_CUDA(launch_after(head_dh_kernel<BF16, 1, false>, dim3((unsigned)n, cols), dim3(128), 0, st, 1, a));
         else AETH_CUDA(launch_after(head_dh_kernel<BF16, 4, false>, dim3((unsigned)std::min((n + 3) / 4, rows), cols), dim3(128), 0,
                                     st, 1, a));
@@ -309,12 +309,12 @@ struct ProbsPlan {
     }
 };
 
-// Whether the gradient takes two rows for a token (1 or 0): where few terms make up
+// Whether the gradient takes two rows for a token: where few terms make up
 // a sum, the rounding of G stands beside the result's own (for a token alone up to
 // twice of it). 4096 x 32000 bf16, one row and two: one token 188 and 190 us, 64
 // 190 and 207, 128 199 and 229; 256 (where 512 rows take 317) 223 with one, and sums
 // of so many labels' terms are even.
-int probs_twice(int64_t n) { return n <= 128; }
+bool probs_twice(int64_t n) { return n <= 128; }
 
 // A CTA's logits, and two bytes for each, beside the hidden states in shared memory.
 constexpr int kVecLogitShared = 96 * 1024;
@@ -632,7 +632,7 @@ int aeth_cut_ce_backward(const void* hidden, int64_t ld_hidden, const void* weig
     a.row_scale = w.row_scale;
     AETH_TRY(head_rows(a, labels, n, d, vocab, ignore_index, hidden, ld_hidden, p, w, st));
     auto run = bf16 ? head_backward<true, false> : unit ? head_backward<false, true> : head_backward<false, false>;
-    return run(p, w, weight, ld_weight, n, d, vocab, nullptr, 0, d_hidden, ld_dh, d_weight, ld_dw, st);
+    return run(p, w, weight, ld_weight, n, d, vocab, nullptr, d_hidden, ld_dh, d_weight, ld_dw, st);
 }
 
 int aeth_token_log_probs_workspace(int64_t n, int64_t d, int64_t vocab, int top, int backward, size_t* bytes) {
@@ -703,7 +703,7 @@ int aeth_token_log_probs_backward(const void* hidden, int64_t ld_hidden, const v
         return AETH_OK;
     }
     const bool bf16 = dtype == AETH_DTYPE_BF16, unit = !bf16 && d_hidden;
-    const int twice = probs_twice(n);
+    const bool twice = probs_twice(n);
     const HeadPlan p(n << twice, d, vocab, unit ? 2 : 1, true);
     const HeadWork w(p, n, true, workspace);
     Carver c(workspace);
@@ -724,8 +724,11 @@ int aeth_token_log_probs_backward(const void* hidden, int64_t ld_hidden, const v
     a.row = row;
     a.twice = twice;
     AETH_TRY(head_rows(a, labels, n, d, vocab, ignore_index, hidden, ld_hidden, p, w, st));
-    auto run = bf16 ? head_backward<true, false, true> : unit ? head_backward<false, true, true> : head_backward<false, false, true>;
-    return run(p, w, weight, ld_weight, n, d, vocab, row, twice, d_hidden, ld_dh, d_weight, ld_dw, st);
+    auto run = twice ? (bf16   ? head_backward<true, false, true, true>
+                        : unit ? head_backward<false, true, true, true> : head_backward<false, false, true, true>)
+                     : (bf16   ? head_backward<true, false, true>
+                        : unit ? head_backward<false, true, true> : head_backward<false, false, true>);
+    return run(p, w, weight, ld_weight, n, d, vocab, row, d_hidden, ld_dh, d_weight, ld_dw, st);
 }
 
 int aeth_rms_norm_checkpoint(const void* x, int64_t ld_x, const void* residual, int64_t ld_residual, const void* gain,

@@ -69,7 +69,7 @@ struct HeadRows {
     const float *entropy, *grad_entropy;
     float bound;  // of |p (log p + entropy)|
     float4* row;
-    int twice;  // 1: live row i comes as rows 2 i and 2 i + 1 (head_round_twice); 0
+    bool twice;  // live row i comes as rows 2 i and 2 i + 1 (head_round_twice)
     // the live rows of H, gathered to a pitch that TMA takes
     const uint16_t* h;
     int64_t ld;
@@ -120,12 +120,14 @@ __device__ __forceinline__ int64_t head_padded(int live, int64_t n) {
 
 // A live row of the gradient of a log p_y + b entropy: its weight w = |a| + c |b|
 // (returned, and for now in row[].w) and, of a / w and b / w, what an entry takes
-// (HeadRowGrad).
+// (HeadRowGrad).  TWICE: the row and the one after it.
+template <bool TWICE>
 __device__ __forceinline__ float head_probs_row(const HeadRows& a, int64_t t, int i, int lab) {
     const float ga = a.grad ? a.grad[t] : 0.0f, gb = a.grad_entropy ? a.grad_entropy[t] : 0.0f;
     const float w = fmaf(a.bound, fabsf(gb), fabsf(ga));
     const float ua = w == 0.0f ? 0.0f : ga / w, ub = w == 0.0f ? 0.0f : gb / w, gamma = ub * kLn2;
-    for (int r = i << a.twice; r < (i + 1) << a.twice; ++r) {
+#pragma unroll
+    for (int r = i; r <= i + (TWICE ? 1 : 0); ++r) {
         a.lab[r] = lab;
         a.lse2[r] = a.lse[t];
         a.row_scale[r] = w / a.g_scale;
@@ -139,9 +141,9 @@ __device__ __forceinline__ float head_probs_row(const HeadRows& a, int64_t t, in
 // per live row.  CTA 0 writes that.  PROBS: for a gradient of log probabilities and
 // entropies (head_probs_row).  PACK (up to 8192 tokens): every CTA makes
 // the scan for itself and then gathers its share of H's rows; more tokens take
-// one CTA and head_pack_kernel behind it.
+// one CTA and head_pack_kernel behind it.  TWICE: two rows for a token.
 constexpr int kHeadScan = 8192;
-template <bool PACK, bool PROBS>
+template <bool PACK, bool PROBS, bool TWICE = false>
 __global__ void __launch_bounds__(1024) head_rows_kernel(const __grid_constant__ HeadRows a, uint32_t* err) {
     constexpr int kItems = kHeadScan / 1024;
     __shared__ int wsum[kItems * 32];
@@ -204,11 +206,11 @@ __global__ void __launch_bounds__(1024) head_rows_kernel(const __grid_constant__
                 a.pos[t] = bad ? kHeadBad : kHeadIgnored;
                 continue;
             }
-            a.pos[t] = PROBS ? i << a.twice : i;
+            a.pos[t] = TWICE ? 2 * i : i;
             a.rows[i] = (int)t;  // read where a token has one row
             if (!PROBS) a.lab[i] = (int)lab[k];
             if (PROBS) {
-                const float w = head_probs_row(a, t, i, (int)lab[k]);
+                const float w = head_probs_row<TWICE>(a, t, TWICE ? 2 * i : i, (int)lab[k]);
                 if (w <= 3.402823466e38f) gmax = fmaxf(gmax, w);
             } else if (a.coef) {
                 a.lse2[i] = fmaf(lse[k], kLog2e, -a.g_bits);
@@ -224,14 +226,19 @@ __global__ void __launch_bounds__(1024) head_rows_kernel(const __grid_constant__
         __syncthreads();
     }
     if (PACK) {
-        if (PROBS) base <<= a.twice;
+        if (TWICE) base *= 2;
         const int64_t g = gridDim.x, b = blockIdx.x, first = base + b;
-        for (int h = 0; h <= (PROBS ? a.twice : 0); ++h)
-            head_copy_rows(a, (a.n - b + g - 1) / g, [&](int64_t r) { return b + r * g; }, [&](int64_t r) {
-                const int64_t to = spos[b + r * g];
-                return PROBS && to >= 0 ? (to << a.twice) + h : to;
+        const int64_t mine = (a.n - b + g - 1) / g;
+        auto from = [&](int64_t r) { return b + r * g; };
+        if (TWICE) {
+            head_copy_rows(a, 2 * mine, [&](int64_t r) { return from(r / 2); }, [&](int64_t r) {
+                const int64_t to = spos[from(r / 2)];
+                return to >= 0 ? 2 * to + r % 2 : to;
             });
-        const int64_t padded = head_padded(base, PROBS ? a.n << a.twice : a.n);
+        } else {
+            head_copy_rows(a, mine, from, [&](int64_t r) { return (int64_t)spos[from(r)]; });
+        }
+        const int64_t padded = head_padded(base, TWICE ? 2 * a.n : a.n);
         if (first < padded)
             head_copy_rows(a, (padded - first + g - 1) / g, [](int64_t) { return (int64_t)-1; },
                            [&](int64_t r) { return first + r * g; });
@@ -793,8 +800,9 @@ __device__ __forceinline__ void head_round_twice(const float (&v)[N], float f, b
 // UNIT (f16): the G without token weights, beside the other where that is wanted
 // (3584 x 4096 x 32000 with weights: 2.26 -> 2.42 ms, 64 tokens 178 -> 183 us).
 // PROBS: the gradient of log probability and entropy (head_probs.cuh), whose rows
-// have coefficients of their own in `row`, and where tokens are few come twice.
-template <bool BF16, bool UNIT, bool PROBS>
+// have coefficients of their own in `row`, and with TWICE come twice: odd rows are
+// what those before them left.
+template <bool BF16, bool UNIT, bool PROBS, bool TWICE>
 struct HeadGrad {
     static constexpr int kChunk = 8;
     static constexpr bool kLiveN = false;
@@ -807,7 +815,6 @@ struct HeadGrad {
     int n;   // rows of g: the tokens
     int v0;  // first vocabulary entry of the piece
     const float4* row;  // with PROBS
-    int twice;          // with PROBS: odd rows are what the rows before them left
     __device__ static void give_up(const PairTile&) {}
     __device__ __forceinline__ void finish(const PairTile& t, const float (&acc)[128]) const {
         const int r = t.row0 + t.lane;
@@ -824,7 +831,7 @@ struct HeadGrad {
                     float v[32];
                     head_slice(acc, 2 * b + h, v);
                     a.values(v, lab_c - 64 * b - 32 * h);
-                    if (PROBS && twice) {
+                    if (TWICE) {
                         head_round_twice<BF16>(v, a.f, r & 1, w + 16 * h);
                         if (UNIT) head_round_twice<BF16>(v, a.u, r & 1, w1 + 16 * h);
                     } else {
@@ -842,7 +849,7 @@ struct HeadGrad {
 
 // The same with tokens as the tile's columns: each 32 x 32 block is turned over,
 // so that a thread has a token and 32 entries.
-template <bool BF16, bool UNIT, bool PROBS>
+template <bool BF16, bool UNIT, bool PROBS, bool TWICE>
 struct HeadGradT {
     static constexpr int kChunk = 8;
     static constexpr bool kLiveN = true;
@@ -855,7 +862,6 @@ struct HeadGradT {
     int n;
     int v0;
     const float4* row;
-    int twice;
     __device__ static void give_up(const PairTile&) {}
     __device__ __forceinline__ void finish(const PairTile& t, const float (&acc)[128]) const {
 #pragma unroll
@@ -870,7 +876,7 @@ struct HeadGradT {
             const HeadRowGrad<BF16, PROBS> a(in, token, coef, lse2, row);
             a.values(v, in ? lab[token] - v0 - t.row0 : -1);
             uint32_t w[16], w1[16];
-            if (PROBS && twice) {
+            if (TWICE) {
                 head_round_twice<BF16>(v, a.f, token & 1, w);
                 if (UNIT) head_round_twice<BF16>(v, a.u, token & 1, w1);
             } else {
