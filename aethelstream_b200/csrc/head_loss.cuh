@@ -779,11 +779,10 @@ template <bool BF16, int N>
 __device__ __forceinline__ void head_round_twice(const float (&v)[N], float f, bool left, uint32_t* w) {
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
-        const float x = v[2 * i] * f, y = v[2 * i + 1] * f;
-        const uint32_t near = pack16<BF16>(x, y);
+        const uint32_t near = pack16<BF16>(v[2 * i] * f, v[2 * i + 1] * f);
         const float2 r = BF16 ? make_float2(__uint_as_float(near << 16), __uint_as_float(near & 0xffff0000u))
                               : __half22float2(*reinterpret_cast<const __half2*>(&near));
-        w[i] = left ? pack16<BF16>(x - r.x, y - r.y) : near;
+        w[i] = left ? pack16<BF16>(fmaf(v[2 * i], f, -r.x), fmaf(v[2 * i + 1], f, -r.y)) : near;
     }
 }
 

@@ -189,6 +189,12 @@ struct PairShape {
             bn = pair_live_bn(N);
         }
         tiles_m = max((M + 255) / 256, 1);
+        // Few tiles: narrower ones, where a wave takes them all (they too cover N
+        // rounded up to 64; 300 x 4096 x 2000 bf16, log probabilities and their gradient
+        // 35 + 56 -> 27 + 48 us).  A split product's stay as its reader knows them.
+        if (g.live_dim == PAIR_LIVE_N && g.tail_kb == 0)
+            for (int narrow = 64; narrow < bn; narrow += 64)
+                if (tiles_m * ((N + narrow - 1) / narrow) <= (int)gridDim.x / 2) bn = narrow;
         tiles_n = max((N + bn - 1) / bn, 1);
         kb = max((K + 63) / 64, 1);
         group = pair_group(tiles_m);
