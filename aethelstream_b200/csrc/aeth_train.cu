@@ -314,7 +314,7 @@ struct ProbsPlan {
 // Whether the gradient takes two rows for a token: where few terms make up
 // a sum, the rounding of G stands beside the result's own (for a token alone up to
 // twice of it). 4096 x 32000 bf16, one row and two: one token 188 and 190 us, 64
-// 190 and 207, 128 199 and 229; 256 (where 512 rows take 317) 223 with one, and sums
+// 190 and 203, 128 199 and 225; 256 (where 512 rows take 317) 223 with one, and sums
 // of so many labels' terms are even.
 bool probs_twice(int64_t n) { return n <= 128; }
 
