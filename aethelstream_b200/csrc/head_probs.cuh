@@ -57,7 +57,6 @@ __device__ __forceinline__ HeadSums head_join3(const HeadSums& a, const HeadSums
 __device__ __forceinline__ HeadSums head_shuffle(const HeadSums& a, int o) {
     return {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.u, o), 0.0f};
 }
-__device__ __forceinline__ float head_lse3(const HeadSums& a) { return head_base(a.m) + logf(a.s); }
 __device__ __forceinline__ float head_entropy(const HeadSums& a) { return logf(a.s) - kLn2 * (a.u / a.s); }
 
 // Joins 32 logits, the first `left` of them, whatever they are.
@@ -85,10 +84,11 @@ __device__ __forceinline__ void head_sums32(const float (&v)[32], int left, Head
     st = {m, s0 + s1, u0 + u1, 0.0f};
 }
 // The same in two and a half instructions a logit, against a maximum that is known
-// (`unused` holds it in units of log2): fused multiply-adds of pairs.  Its rounding
-// is one factor of all sums, which head_fast_end takes out.  A logit of -infinity
-// makes u NaN and one above 2^127 / log2 e the maximum infinite; those rows go the
-// other way.
+// (`unused` holds it in units of log2): fused multiply-adds of pairs.  The maximum's
+// rounding in those units, half a step of it, is one factor of all sums, which
+// head_fast_end takes out; up to 2^24 that is 2^0.5 at most.  Rows beyond, whose
+// sums it could overflow, and those with a logit of -infinity, which makes u NaN, go
+// the other way.
 __device__ __forceinline__ void head_fast32(const float (&v)[32], int left, HeadSums& st) {
     const float2 l2 = make_float2(kLog2e, kLog2e), nb = make_float2(-st.unused, -st.unused);
     float2 s = make_float2(st.s, 0.0f), u = make_float2(st.u, 0.0f);
@@ -109,10 +109,10 @@ __device__ __forceinline__ HeadSums head_fast_begin(const float (&acc)[128], int
         m = left >= 128 ? fmax3(m, acc[i], acc[i + 1]) : fmaxf(i < left ? fmaxf(m, acc[i]) : m, i + 1 < left ? acc[i + 1] : m);
     return {m, 0.0f, 0.0f, m * kLog2e};
 }
-__device__ __forceinline__ bool head_fast_good(const HeadSums& st) { return fabsf(st.unused) < 1e38f && st.u == st.u; }
+__device__ __forceinline__ bool head_fast_good(const HeadSums& st) { return fabsf(st.unused) < 0x1p24f && st.u == st.u; }
 // Takes the base's rounding d = m log2 e - base out: s 2^-d and, of x - d, u.
 __device__ __forceinline__ HeadSums head_fast_end(const HeadSums& st) {
-    const float d = fmaf(st.m, kLog2e, -st.unused), w = fmaf(-d, kLn2, 1.0f);
+    const float d = fmaf(st.m, kLog2e, -st.unused), w = ex2(-d);
     return {st.m, st.s * w, fmaf(-st.s, d, st.u) * w, 0.0f};
 }
 
@@ -213,15 +213,18 @@ __device__ __forceinline__ void head_probs_write(const HeadProbsOut& a, int64_t 
                                                  float label_logit, const HeadBest& best) {
     const float nan = __int_as_float(0x7fc00000);
     // one lane's: in the others the same sums were added the other way round
-    const float lse = __shfl_sync(0xffffffffu, bad ? nan : live ? head_lse3(x) : 0.0f, 0);
+    const float m = __shfl_sync(0xffffffffu, bad ? nan : live ? head_base(x.m) : 0.0f, 0);
+    const float log_s = __shfl_sync(0xffffffffu, live ? logf(x.s) : 0.0f, 0), lse = m + log_s;
+    // from a logit's distance to the maximum: without the rounding of a large lse
+    auto log_prob = [&](float v) { return (v - m) - log_s; };
     if (lane == 0) {
         a.lse[t] = lse;
-        a.log_probs[t] = bad ? nan : live ? label_logit - lse : 0.0f;
+        a.log_probs[t] = bad ? nan : live ? log_prob(label_logit) : 0.0f;
         a.entropy[t] = bad ? nan : live ? head_entropy(x) : 0.0f;
     }
     if (lane < a.top) {
         const bool known = live && !isnan(lse) && best.i != 0x7fffffff;
-        a.top_log_probs[t * a.top + lane] = known ? best.v - lse : bad || live ? nan : 0.0f;
+        a.top_log_probs[t * a.top + lane] = known ? log_prob(best.v) : bad || live ? nan : 0.0f;
         a.top_ids[t * a.top + lane] = known ? best.i : -1;
     }
 }

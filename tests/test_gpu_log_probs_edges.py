@@ -1,0 +1,33 @@
+"""Log probabilities at the head where their arithmetic has an edge."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("top", [0, 3])
+@pytest.mark.parametrize("n", [2, 40, 256, 1100])
+@pytest.mark.parametrize("power,sign", [(16, 1), (20, 1), (25, -1), (25, 1), (27, 1), (31, 1), (60, -1), (100, 1)])
+def test_logits_of_any_finite_size(power, sign, n, top):
+    """Half of the vocabulary has the largest logit, the other half less by
+    2^(power - 20), all around +-2^power.  The logits are exact in fp32, and so is
+    their distance from the maximum; what is left is the error of 1500 exponentials
+    of 2^-21 each, their sum and its logarithm: 2^-18 of 1 + the result covers these."""
+    import aethelstream_b200 as A
+    v = 1500
+    h, w = torch.zeros(n, 64, device="cuda"), torch.zeros(v, 64, device="cuda")
+    h[:, 0], w[:, 0] = 2.0 ** (power - power // 2), sign * 2.0 ** (power // 2)
+    h[:, 1], w[1::2, 1] = 2.0 ** (power - 20), 1.0
+    lab = torch.arange(n, device="cuda") % v
+    r = A.token_log_probs(h.bfloat16(), w.bfloat16(), lab, top_k=top)
+    s = h[:1].double() @ w.double().T
+    q = torch.log_softmax(s, 1)[0]
+    entropy = -(q.exp() * torch.where(q > -700, q, 0.0)).sum()
+    assert ((r.entropy.double() - entropy).abs() <= 2.0 ** -18 * (1 + entropy)).all()
+    assert ((r.log_probs.double() - q[lab]).abs() <= 2.0 ** -18 * (1 + q[lab].abs())).all()
+    assert ((r.lse.double() - torch.logsumexp(s, 1)).abs() <= 2.0 ** -18 + 2.0 ** -23 * 2.0 ** power).all()
+    if top:
+        assert torch.equal(r.top_ids, torch.tensor([1, 3, 5], device="cuda").expand(n, 3))
+        assert ((r.top_log_probs.double() - q[1]).abs() <= 2.0 ** -18 * (1 + q[1].abs())).all()
