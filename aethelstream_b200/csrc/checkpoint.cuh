@@ -702,10 +702,6 @@ __device__ __forceinline__ void ck_back_sums(uint2 q, const Pack8<T>& dy, const 
     xx += (float)__dp4a((int)q.y, (int)q.y, __dp4a((int)q.x, (int)q.x, 0)) * s * s;  // in this order: s * s may leave fp32's range
     xd += (dd.x + dd.y) * s;
 }
-// -r^3 mean(dy gain x^), what x^ is taken times in dx.  r |mean| is at most the root
-// mean square of dy gain, so that one factor of r at a time stays in fp32's range as long
-// as r^2 does (r^3 leaves it where activations reach 1e13, or 1e-13 without eps).
-__device__ __forceinline__ float ck_back_factor(float r, float mean) { return -(r * (r * (r * mean))); }
 // dx of eight features (dy gain r + x^ f + the residual's) and their addends
 // to d_gain's sums.
 template <typename T>

@@ -73,4 +73,9 @@ __device__ __forceinline__ uint2 ck_stream(const uint2* p) {
     return v;
 }
 
+// -r^3 mean(dy gain x), what x is taken times in a norm's dx.  r |mean| is at most the root
+// mean square of dy gain, so that one factor of r at a time stays in fp32's range as long
+// as r^2 does (r^3 leaves it where activations reach 1e13, or 1e-13 without eps).
+__device__ __forceinline__ float ck_back_factor(float r, float mean) { return -(r * (r * (r * mean))); }
+
 }  // namespace aeth

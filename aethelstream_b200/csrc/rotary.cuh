@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(kRotThreads, CTAS) rotary_kernel(const __grid_
                         }
                     }
                 }
-                const float dot = -(rot_sum(dot2.x + dot2.y, lanes) / (float)a.D * (rinv * rinv * rinv));
+                const float dot = ck_back_factor(rinv, rot_sum(dot2.x + dot2.y, lanes) / (float)a.D);
                 const float2 nd = make_float2(dot, dot);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(kRotThreads) rotary_any_kernel(const __grid_co
                     sums[warp * a.D + d] += (float)dy[d] * ((float)x[d] * r);
                     dot += gain(d) * (float)dy[d] * (float)x[d];
                 }
-                dot = rot_sum(dot, 32) / (float)a.D * (r * r * r);
+                dot = ck_back_factor(r, rot_sum(dot, 32) / (float)a.D);
             }
             for (int p = lane; p < half; p += 32) {
                 int u, v;
@@ -449,8 +449,8 @@ __global__ void __launch_bounds__(kRotThreads) rotary_any_kernel(const __grid_co
                 }
                 float yu = xu * cs[p] - xv * sn[p], yv = xv * cs[p] + xu * sn[p];
                 if (OP == ROT_NORM_BACK) {
-                    yu = r * (yu * gain(u)) - (float)x[u] * dot;
-                    yv = r * (yv * gain(v)) - (float)x[v] * dot;
+                    yu = r * (yu * gain(u)) + (float)x[u] * dot;
+                    yv = r * (yv * gain(v)) + (float)x[v] * dot;
                 }
                 o[u] = (T)yu;
                 o[v] = (T)yv;
@@ -458,7 +458,7 @@ __global__ void __launch_bounds__(kRotThreads) rotary_any_kernel(const __grid_co
             for (int d = a.R + lane; d < a.D; d += 32) {
                 if (OP == ROT_TURN) o[d] = x[d];
                 else if (OP == ROT_NORM) o[d] = (T)((float)x[d] * r * gain(d));
-                else o[d] = (T)(r * ((float)dy[d] * gain(d)) - (float)x[d] * dot);
+                else o[d] = (T)(r * ((float)dy[d] * gain(d)) + (float)x[d] * dot);
             }
         }
     }
@@ -562,11 +562,11 @@ __global__ void __launch_bounds__(kRotThreads) rotary_pairs_kernel(const __grid_
                     ev[j] *= gv[j];
                     dot = fmaf(ev[j], v[j], fmaf(eu[j], u[j], dot));
                 }
-                dot = rot_sum(dot, 32) / (float)a.D * (r * r * r);
+                dot = ck_back_factor(r, rot_sum(dot, 32) / (float)a.D);
 #pragma unroll
                 for (int j = 0; j < NP; ++j) {
-                    u[j] = r * eu[j] - u[j] * dot;
-                    v[j] = r * ev[j] - v[j] * dot;
+                    u[j] = r * eu[j] + u[j] * dot;
+                    v[j] = r * ev[j] + v[j] * dot;
                 }
             } else {
 #pragma unroll
