@@ -184,8 +184,8 @@ __device__ __forceinline__ void adamw_store(void* p, int dtype, bool whole, int6
 
 // What a step's elements share.
 struct AdamwScalars {
-    float clip, lr, b1, b2, omb1, omb2, first, second, eps, decay;
-    bool flush;  // eps is so large that a root below 2^-63 does not count beside it (2^-20 of it)
+    float clip, lr, b1, b2, omb1, omb2, first, root, eps, decay;  // root: of v's correction
+    bool flush;  // eps is so large that root times 2^-63 does not count beside it (2^-23 of it)
 };
 // 1 / (1 - b^t), b^t by squaring
 __device__ __forceinline__ float adamw_correction(double b, int64_t t) {
@@ -210,10 +210,10 @@ __device__ __forceinline__ AdamwScalars adamw_scalars(const AdamwArgs<CAP>& a, f
     s.omb2 = (float)(1.0 - a.beta2);
     s.eps = a.eps;
     s.decay = a.decay;
-    s.flush = a.eps >= 1e-12f;
     __syncthreads();
     s.first = shared2[0];
-    s.second = shared2[1];
+    s.root = sqrtf(shared2[1]);
+    s.flush = a.eps >= 1e-12f * s.root;
     return s;
 }
 // The CTA that ends last counts the step.  Every CTA has read the step's low
@@ -240,18 +240,25 @@ __device__ __forceinline__ int adamw_tensor(const AdamwArgs<CAP>& a, int block, 
     return lo;
 }
 
-// 1 / (sqrt(x) + eps), subnormal numbers flushed to 0 or not
+// 1 / (root sqrt(v) + eps) of two, subnormal numbers flushed to 0 or not.  The correction's
+// root, since the corrected v may lie past the largest float, or among the subnormal ones.
 template <bool FLUSH>
-__device__ __forceinline__ float adamw_scale(float x, float eps) {
-    float r;
+__device__ __forceinline__ float2 adamw_scale(float x, float y, float2 root, float2 eps) {
+    float a, b;
     if (FLUSH) {
-        asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-        r += eps;
-        asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(r));
+        asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(x));
+        asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(y));
     } else {
-        asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
-        r += eps;
-        asm("rcp.approx.f32 %0, %0;" : "+f"(r));
+        asm("sqrt.approx.f32 %0, %1;" : "=f"(a) : "f"(x));
+        asm("sqrt.approx.f32 %0, %1;" : "=f"(b) : "f"(y));
+    }
+    float2 r = fma2_rn(make_float2(a, b), root, eps);
+    if (FLUSH) {
+        asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(r.x));
+        asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(r.y));
+    } else {
+        asm("rcp.approx.f32 %0, %0;" : "+f"(r.x));
+        asm("rcp.approx.f32 %0, %0;" : "+f"(r.y));
     }
     return r;
 }
@@ -276,12 +283,13 @@ __device__ __forceinline__ void adamw_moments(const AdamwScalars& s, const float
 template <int N, bool FLUSH>
 __device__ __forceinline__ void adamw_params(const AdamwScalars& s, float decay, const float (&m)[N], const float (&v)[N],
                                              float (&p)[N]) {
-    const float2 first = make_float2(s.first, s.first), second = make_float2(s.second, s.second);
+    const float2 first = make_float2(s.first, s.first), root = make_float2(s.root, s.root), eps = make_float2(s.eps, s.eps);
 #pragma unroll
     for (int k = 0; k < N; k += 2) {
-        const float2 mm = mul2_rn(make_float2(m[k], m[k + 1]), first), vv = mul2_rn(make_float2(v[k], v[k + 1]), second);
-        p[k] -= s.lr * fmaf(mm.x, adamw_scale<FLUSH>(vv.x, s.eps), decay * p[k]);
-        p[k + 1] -= s.lr * fmaf(mm.y, adamw_scale<FLUSH>(vv.y, s.eps), decay * p[k + 1]);
+        const float2 mm = mul2_rn(make_float2(m[k], m[k + 1]), first);
+        const float2 x = adamw_scale<FLUSH>(v[k], v[k + 1], root, eps);
+        p[k] -= s.lr * fmaf(mm.x, x.x, decay * p[k]);
+        p[k + 1] -= s.lr * fmaf(mm.y, x.y, decay * p[k + 1]);
     }
 }
 template <int N>
