@@ -109,7 +109,8 @@ def adamw_step(params, grads, state: AdamWState, config: AdamWConfig | None = No
       p -= lr (m / (1 - beta1^t) / (sqrt(v / (1 - beta2^t)) + eps) + weight_decay p).
     `grads`: one for each tensor, of its shape and any of the three types, and not
     in the memory of another tensor; None leaves the tensor and its moments as they
-    are.  clip: a float32 on the device
+    are.  Tensors that share memory are refused where two of them have gradients.
+    clip: a float32 on the device
     (what ``GaLoreOptimizer.finish_step`` leaves in its clip_out).  decay: a truth
     value for each tensor, whether weight_decay applies to it (None: to all).
     lr: a float32 on the device in config.lr's place, for a captured step."""

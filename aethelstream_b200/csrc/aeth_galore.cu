@@ -2527,7 +2527,7 @@ bool adamw_overlap(const AdamwList& l) {
     std::vector<std::pair<uintptr_t, uintptr_t>> r;
     r.reserve((size_t)l.count);
     for (int i = 0; i < l.count; ++i)
-        if (l.n[i] > 0) {
+        if (l.n[i] > 0 && l.g[i]) {
             const uintptr_t a = reinterpret_cast<uintptr_t>(l.p[i]);
             r.emplace_back(a, a + (uintptr_t)l.n[i] * (l.p_dtype[i] == AETH_DTYPE_F32 ? 4 : 2));
         }

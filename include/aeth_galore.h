@@ -667,8 +667,9 @@ int aeth_qk_norm_rotary_backward(const AethRotaryPlan* plan, const void* positio
  *     block's largest magnitude (0 where that is below 2^-126; NaN where the block
  *     holds a NaN or an infinity).  master (or NULL): fp32 parameters laid out as
  *     the moments, which the step is taken on; p gets their rounding.
- *     m, v and master 16-byte aligned.  Parameters that overlap one another:
- *     AETH_ERR_ARG; a gradient must not overlap another tensor's parameter.
+ *     m, v and master 16-byte aligned.  Parameters that overlap one another, those
+ *     left out apart: AETH_ERR_ARG; a gradient must not overlap another tensor's
+ *     parameter.
  *     Nothing synchronises; with bits 32 nothing allocates, with bits 8 the
  *     library's first call on a device uploads its maps.
  * ====================================================================== */

@@ -40,3 +40,22 @@ def test_any_eps(A, maps, monkeypatch, kind, master, bits, eps):  # noqa: F811
     c = Check(A, params, state, A.AdamWConfig(beta1=0.9, beta2=0.999, eps=eps, lr=1e-3, weight_decay=0.1), maps)
     for _ in range(3):
         c.step([(s * torch.randn(n, generator=gen, device="cuda")).to(gk) for n, s in zip(sizes, (1e-3, 1e-19, 1e-20, 1e-22, 1e-18))])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_tied_tensor_that_is_left_out(A, bits):  # noqa: F811
+    """The same tensor twice, one of them without a gradient, which is not written."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    p, other, g = tensors(gen, [5000] * 3, [torch.bfloat16] * 3)
+    for grads in ([g, None, None], [None, g, None]):
+        both, alone = [p.clone()] * 2 + [other.clone()], p.clone()
+        s, t = A.AdamWState.zeros(both, bits=bits), A.AdamWState.zeros([alone], bits=bits)
+        for _ in range(2):
+            A.adamw_step(both, grads, s)
+            A.adamw_step([alone], [g], t)
+        at = 0 if grads[0] is not None else 3
+        assert torch.equal(both[0], alone) and torch.equal(both[2], other)
+        assert torch.equal(s.m.view(-1, 2048)[at:at + 3], t.m.view(-1, 2048)) and int(s.step) == 2
+        with pytest.raises(ValueError, match="share memory"):
+            A.adamw_step(both, [g, g, None], s)
+        assert int(s.step) == 2
