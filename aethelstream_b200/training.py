@@ -204,7 +204,7 @@ def token_log_probs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Te
         raise ValueError(f"{what}: top_k must be 0 to {min(MAX_ALTERNATIVES, v)}, got {top_k}")
     h, n, ld_h = _rows(hidden, d)
     w, _, ld_w = _tma_rows(weight, d)
-    lp, entropy, lse = lab.new_empty((3, *labels.shape), dtype=torch.float32).unbind(0)
+    lp, entropy, lse = (lab.new_empty(labels.shape, dtype=torch.float32) for _ in range(3))
     top = ids = None
     if top_k:
         top, ids = (lab.new_empty((*labels.shape, top_k), dtype=t) for t in (torch.float32, torch.int64))

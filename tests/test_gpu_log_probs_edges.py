@@ -31,3 +31,32 @@ def test_logits_of_any_finite_size(power, sign, n, top):
     if top:
         assert torch.equal(r.top_ids, torch.tensor([1, 3, 5], device="cuda").expand(n, 3))
         assert ((r.top_log_probs.double() - q[1]).abs() <= 2.0 ** -18 * (1 + q[1].abs())).all()
+
+
+def test_results_are_tensors_of_their_own():
+    """Log probabilities changed in place (for a ratio to older ones, say) leave what the
+    backward pass saved as it is, and torch agrees."""
+    import aethelstream_b200 as A
+
+    class LogProbs(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, h, w, lab):
+            r = A.token_log_probs(h, w, lab)
+            ctx.save_for_backward(h, w, lab, r.lse, r.entropy)
+            ctx.result = r
+            return r.log_probs
+
+        @staticmethod
+        def backward(ctx, g):
+            h, w, lab, lse, entropy = ctx.saved_tensors
+            r = A.TokenLogProbs(None, entropy, lse, None, None)
+            return *A.token_log_probs_backward(h, w, lab, r, grad_log_probs=g.contiguous()), None
+
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    h, w = (torch.randn(n, 64, generator=gen, device="cuda").bfloat16().requires_grad_() for n in (20, 300))
+    lab = torch.arange(20, device="cuda")
+    old = torch.randn(20, generator=gen, device="cuda")
+    LogProbs.apply(h, w, lab).sub_(old).sum().backward()
+    r = A.token_log_probs(h.detach(), w.detach(), lab)
+    dh, dw = A.token_log_probs_backward(h.detach(), w.detach(), lab, r, grad_log_probs=torch.ones(20, device="cuda"))
+    assert torch.equal(h.grad, dh) and torch.equal(w.grad, dw)
