@@ -2460,8 +2460,8 @@ struct AdamwList {
     const uint8_t *p_dtype, *g_dtype, *decay;
     int count;
 };
-// Launches for the tensors from `i` on that have a gradient: as many as a table
-// takes.  `block`: the first block of tensor i's moments.
+// A launch for the tensors from `i` on that have a gradient: as many as a table
+// takes (2^30 blocks at most: adamw_state_check).  `block`: the first block of tensor i's moments.
 template <int CAP>
 int adamw_some(const AdamwList& l, int& i, int64_t& block, AdamwArgs<CAP>& a, int bits, cudaStream_t st) {
     a.count = 0;
@@ -2469,7 +2469,6 @@ int adamw_some(const AdamwList& l, int& i, int64_t& block, AdamwArgs<CAP>& a, in
     for (; i < l.count && a.count < CAP; ++i) {
         const int64_t nb = (l.n[i] + kAdamwBlock - 1) / kAdamwBlock;
         if (l.g[i] && nb > 0) {
-            if (blocks + nb > (1 << 30)) break;  // one tensor alone has fewer (aeth_adamw_step)
             AdamwTensor& t = a.t[a.count];
             t.p = l.p[i];
             t.g = l.g[i];

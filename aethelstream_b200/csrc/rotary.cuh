@@ -19,8 +19,8 @@
 // D / 16 lanes (a power of two; lanes past it idle): a lane holds eight features
 // at 8 c and the eight R / 2 further on, which are eight pairs in either layout,
 // so a row needs no exchange but the norm's sums.  A CTA takes a stretch of the
-// (token, head) rows, all SMs one wave of them; its tokens' cosines go to shared
-// memory first, each for all the heads of q and k.  A lane's rows to come are on
+// (token, head) rows, all SMs one to three waves of them (rot_waves); its tokens'
+// cosines go to shared memory first, each for all the heads of q and k.  A lane's rows to come are on
 // their way to shared memory by asynchronous copies of its own, which it alone
 // reads: bytes in flight without registers, and no barrier.  8192 tokens x (64 + 8)
 // heads x 128 bf16: rotation 52 us (5.8 TB/s), with the norm 58 (5.2), the gradient
