@@ -82,12 +82,15 @@ struct HeadPlan {
     int64_t g_rows;  // of a G
 
     // probs: the gradient of log probabilities, whose G has no rows but the tokens' (what
-    // TMA reads past them is zero) and whose pieces are equal where that
-    // takes no more waves: a small last one leaves CTA pairs idle (311 tokens, 155 of
-    // them live, x 2048 x 131071 f16: 482 us with rows and pieces as the loss's, 395)
+    // TMA reads past them is zero; two for each up to kHeadTwice of them) and whose pieces
+    // are equal where that takes no more waves: a small last one leaves CTA pairs idle (311
+    // tokens, 155 of them live, x 2048 x 131071 f16: 482 us with rows and pieces as the
+    // loss's, 395)
     HeadPlan(int64_t n, int64_t d, int64_t vocab, int gs_ = 1, bool probs = false) : gs(gs_) {
+        const bool few = probs && n <= kHeadTwice;
+        if (few) n *= 2;
         n_pad = up(std::max<int64_t>(n, 1), 256);
-        g_rows = probs ? std::max<int64_t>(n, 1) : n_pad;
+        g_rows = few ? std::max<int64_t>(n, 1) : probs ? std::max<int64_t>(n, 2 * kHeadTwice) : n_pad;
         dp = up(d, 8);
         live_n = head_tokens_as_columns(n);
         bn = head_bn(n_pad / 256, vocab);
@@ -141,7 +144,7 @@ struct HeadWork {
         rows = c.take<int>(p.n_pad);
         pos = c.take<int>(std::max<int64_t>(n, 1));
         lab = c.take<int>(p.n_pad);
-        count = c.take<int>(1);
+        count = c.take<int>(2);
         done = c.take<unsigned>(1);
         h = c.take<uint16_t>(p.n_pad * p.dp);
         label_logit = nullptr;
@@ -197,9 +200,10 @@ int head_rows(HeadRows a, const int64_t* labels, int64_t n, int64_t d, int64_t v
     a.d = (int)d;
     a.out = w.h;
     a.ldo = p.dp;
+    a.room = a.row ? p.g_rows : n;
     const unsigned ctas = (unsigned)std::min<int64_t>(n, num_sms());
     if (n <= kHeadScan) {
-        auto kern = !a.row ? head_rows_kernel<true, false> : a.twice ? head_rows_kernel<true, true, true> : head_rows_kernel<true, true>;
+        auto kern = a.row ? head_rows_kernel<true, true> : head_rows_kernel<true, false>;
         kern<<<ctas, 1024, 0, st>>>(a, rt->err_word);
         AETH_LAUNCH_CHECK();
     } else {
@@ -228,28 +232,26 @@ int head_vec(const HeadVec& a, int64_t n, int ctas, float* losses, float* lse, f
 }
 
 // UNIT: d_hidden comes from a G without the token weights.  PROBS: the gradient of
-// log probabilities and entropies, its rows' coefficients in `row`; TWICE: two rows
-// of G for a token
-template <bool BF16, bool UNIT, bool PROBS = false, bool TWICE = false>
-int head_backward(const HeadPlan& p, const HeadWork& w, const void* weight, int64_t ld_weight, int64_t n, int64_t d,
+// log probabilities and entropies, its rows' coefficients in `row`
+template <bool BF16, bool UNIT, bool PROBS = false>
+int head_backward(const HeadPlan& p, const HeadWork& w, const void* weight, int64_t ld_weight, int64_t tokens, int64_t d,
                   int64_t vocab, const float4* row, void* d_hidden, int64_t ld_dh, void* d_weight, int64_t ld_dw,
                   cudaStream_t st) {
     const uint16_t* W = static_cast<const uint16_t*>(weight);
-    const int64_t tokens = n;
-    if (TWICE) n *= 2;
+    const int64_t n = PROBS ? p.g_rows : tokens;
     uint16_t *g = UNIT && !d_weight ? nullptr : w.g, *g_unit = UNIT ? w.g_unit : nullptr;
     for (int64_t v0 = 0; v0 < vocab; v0 += p.piece) {
         const int64_t vp = std::min(p.piece, vocab - v0);
         const PairOperand H{w.h, p.dp, n, d}, Wp{W + v0 * ld_weight, ld_weight, vp, d};
         const PairOperand G{w.g, p.ldg, n, vp}, Gh{UNIT ? w.g_unit : w.g, p.ldg, n, vp};
         if (p.live_n) {
-            using Epi = HeadGradT<BF16, UNIT, PROBS, TWICE>;
-            const Epi eg{w.lab, w.coef, w.lse2, g, g_unit, p.ldg, (int)n, (int)v0, row};
+            using Epi = HeadGradT<BF16, UNIT, PROBS>;
+            const Epi eg{w.lab, w.coef, w.lse2, g, g_unit, p.ldg, (int)n, (int)v0, row, w.count + 1};
             AETH_TRY((pair_gemm_launch<Epi, false, false>(Wp, H, (int)vp, (int)n, (int)d, w.count, PAIR_LIVE_N, 256, 0, BF16,
                                                           eg, st)));
         } else {
-            using Epi = HeadGrad<BF16, UNIT, PROBS, TWICE>;
-            const Epi eg{w.lab, w.coef, w.lse2, g, g_unit, p.ldg, (int)n, (int)v0, row};
+            using Epi = HeadGrad<BF16, UNIT, PROBS>;
+            const Epi eg{w.lab, w.coef, w.lse2, g, g_unit, p.ldg, (int)n, (int)v0, row, w.count + 1};
             AETH_TRY((pair_gemm_launch<Epi, false, false>(H, Wp, (int)n, (int)vp, (int)d, w.count, PAIR_LIVE_M,
                                                           head_bn(p.n_pad / 256, vp), 0, BF16, eg, st)));
         }
@@ -272,15 +274,14 @@ int head_backward(const HeadPlan& p, const HeadWork& w, const void* weight, int6
             }
         }
     }
-    if (d_hidden && n > 0) {
+    if (d_hidden && tokens > 0) {
         const HeadDh a{w.slab, p.dp, w.extra, pair_count(), p.tail_kb, p.live_n, w.pos, w.count, tokens, (int)d,
                        UNIT ? nullptr : w.out_scale, w.row_scale, static_cast<uint16_t*>(d_hidden), ld_dh};
         const unsigned cols = (unsigned)((d + 1023) / 1024);
         const int64_t rows = std::max<int64_t>(16 * num_sms() / cols, 1);
         // few tokens: one at a time, and more of its parts
-        if (TWICE) AETH_CUDA(launch_after(head_dh_kernel<BF16, 1, TWICE>, dim3((unsigned)tokens, cols), dim3(128), 0, st, 1, a));
-        else if (n <= rows) AETH_CUDA(launch_after(head_dh_kernel<BF16, 1, false>, dim3((unsigned)n, cols), dim3(128), 0, st, 1, a));
-        else AETH_CUDA(launch_after(head_dh_kernel<BF16, 4, false>, dim3((unsigned)std::min((n + 3) / 4, rows), cols), dim3(128), 0,
+        if (tokens <= rows) AETH_CUDA(launch_after(head_dh_kernel<BF16, 1, PROBS>, dim3((unsigned)tokens, cols), dim3(128), 0, st, 1, a));
+        else AETH_CUDA(launch_after(head_dh_kernel<BF16, 4, PROBS>, dim3((unsigned)std::min((tokens + 3) / 4, rows), cols), dim3(128), 0,
                                     st, 1, a));
     }
     return AETH_OK;
@@ -310,13 +311,6 @@ struct ProbsPlan {
         ranges = 2 * (int)tiles;
     }
 };
-
-// Whether the gradient takes two rows for a token: where few terms make up
-// a sum, the rounding of G stands beside the result's own (for a token alone up to
-// twice of it). 4096 x 32000 bf16, one row and two: one token 188 and 190 us, 64
-// 190 and 203, 128 199 and 225; 256 (where 512 rows take 317) 223 with one, and sums
-// of so many labels' terms are even.
-bool probs_twice(int64_t n) { return n <= 128; }
 
 // A CTA's logits, and two bytes for each, beside the hidden states in shared memory.
 constexpr int kVecLogitShared = 96 * 1024;
@@ -641,7 +635,7 @@ int aeth_token_log_probs_workspace(int64_t n, int64_t d, int64_t vocab, int top,
     if (n < 0 || d <= 0 || vocab <= 0 || top < 0 || !bytes) return set_err(AETH_ERR_ARG);
     if (n > kHeadMaxDim || d > kHeadMaxDim || vocab > kHeadMaxDim || top > kHeadTop) return set_err(AETH_ERR_UNSUPPORTED);
     if (backward) {
-        const HeadPlan one(n << probs_twice(n), d, vocab, 1, true), two(n << probs_twice(n), d, vocab, 2, true);
+        const HeadPlan one(n, d, vocab, 1, true), two(n, d, vocab, 2, true);
         *bytes = std::max(HeadWork(one, n, true, nullptr).bytes, HeadWork(two, n, true, nullptr).bytes) +
                  (size_t)up(one.n_pad * (int64_t)sizeof(float4), 256);
     } else {
@@ -705,8 +699,7 @@ int aeth_token_log_probs_backward(const void* hidden, int64_t ld_hidden, const v
         return AETH_OK;
     }
     const bool bf16 = dtype == AETH_DTYPE_BF16, unit = !bf16 && d_hidden;
-    const bool twice = probs_twice(n);
-    const HeadPlan p(n << twice, d, vocab, unit ? 2 : 1, true);
+    const HeadPlan p(n, d, vocab, unit ? 2 : 1, true);
     const HeadWork w(p, n, true, workspace);
     Carver c(workspace);
     c.used = w.bytes;
@@ -724,12 +717,8 @@ int aeth_token_log_probs_backward(const void* hidden, int64_t ld_hidden, const v
     a.out_scale = w.out_scale;
     a.row_scale = w.row_scale;
     a.row = row;
-    a.twice = twice;
     AETH_TRY(head_rows(a, labels, n, d, vocab, ignore_index, hidden, ld_hidden, p, w, st));
-    auto run = twice ? (bf16   ? head_backward<true, false, true, true>
-                        : unit ? head_backward<false, true, true, true> : head_backward<false, false, true, true>)
-                     : (bf16   ? head_backward<true, false, true>
-                        : unit ? head_backward<false, true, true> : head_backward<false, false, true>);
+    auto run = bf16 ? head_backward<true, false, true> : unit ? head_backward<false, true, true> : head_backward<false, false, true>;
     return run(p, w, weight, ld_weight, n, d, vocab, row, d_hidden, ld_dh, d_weight, ld_dw, st);
 }
 

@@ -55,7 +55,7 @@ struct HeadRows {
     int* rows;   // live row -> token
     int* pos;    // token -> live row, kHeadIgnored or kHeadBad
     int* lab;    // live row -> label
-    int* count;  // live rows
+    int* count;  // live rows; of the gradient of log probabilities also, after it, rows that a token has
     unsigned* done;  // zeroed: CTAs of head_loss_kernel that have finished
     // backward only (coef != null)
     const float* lse;   // per token
@@ -69,7 +69,7 @@ struct HeadRows {
     const float *entropy, *grad_entropy;
     float bound;  // of |p (log p + entropy)|
     float4* row;
-    bool twice;  // live row i comes as rows 2 i and 2 i + 1 (head_round_twice)
+    int64_t room;  // rows of G (the loss: tokens)
     // the live rows of H, gathered to a pitch that TMA takes
     const uint16_t* h;
     int64_t ld;
@@ -120,30 +120,32 @@ __device__ __forceinline__ int64_t head_padded(int live, int64_t n) {
 
 // A live row of the gradient of a log p_y + b entropy: its weight w = |a| + c |b|
 // (returned, and for now in row[].w) and, of a / w and b / w, what an entry takes
-// (HeadRowGrad).  TWICE: the row and the one after it.
-template <bool TWICE>
+// (HeadRowGrad).
 __device__ __forceinline__ float head_probs_row(const HeadRows& a, int64_t t, int i, int lab) {
     const float ga = a.grad ? a.grad[t] : 0.0f, gb = a.grad_entropy ? a.grad_entropy[t] : 0.0f;
     const float w = fmaf(a.bound, fabsf(gb), fabsf(ga));
     const float ua = w == 0.0f ? 0.0f : ga / w, ub = w == 0.0f ? 0.0f : gb / w, gamma = ub * kLn2;
-#pragma unroll
-    for (int r = i; r <= i + (TWICE ? 1 : 0); ++r) {
-        a.lab[r] = lab;
-        a.lse2[r] = a.lse[t];
-        a.row_scale[r] = w / a.g_scale;
-        a.row[r] = make_float4(ua * a.g_scale, fmaf(-gamma, a.g_bits, fmaf(ub, a.entropy[t], ua)), gamma, w);
-    }
+    a.lab[i] = lab;
+    a.lse2[i] = a.lse[t];
+    a.row_scale[i] = w / a.g_scale;
+    a.row[i] = make_float4(ua * a.g_scale, fmaf(-gamma, a.g_bits, fmaf(ub, a.entropy[t], ua)), gamma, w);
     return w;
 }
+
+// Up to how many live tokens the gradient of log probabilities has two rows of G for
+// each (HeadGrad says what that gives and costs).  By the live ones, whose number is
+// known on the device alone, so that a padded batch has the gradient of its tokens.
+constexpr int kHeadTwice = 128;
 
 // Numbers the live tokens in order (a scan over the labels, 8192 at a time, so
 // that their loads are in flight together) and gathers what the epilogues need
 // per live row.  CTA 0 writes that.  PROBS: for a gradient of log probabilities and
 // entropies (head_probs_row).  PACK (up to 8192 tokens): every CTA makes
 // the scan for itself and then gathers its share of H's rows; more tokens take
-// one CTA and head_pack_kernel behind it.  TWICE: two rows for a token.
+// one CTA and head_pack_kernel behind it.  Live token i has row i of what it writes,
+// or rows 2 i and 2 i + 1 (kHeadTwice).
 constexpr int kHeadScan = 8192;
-template <bool PACK, bool PROBS, bool TWICE = false>
+template <bool PACK, bool PROBS>
 __global__ void __launch_bounds__(1024) head_rows_kernel(const __grid_constant__ HeadRows a, uint32_t* err) {
     constexpr int kItems = kHeadScan / 1024;
     __shared__ int wsum[kItems * 32];
@@ -206,11 +208,11 @@ __global__ void __launch_bounds__(1024) head_rows_kernel(const __grid_constant__
                 a.pos[t] = bad ? kHeadBad : kHeadIgnored;
                 continue;
             }
-            a.pos[t] = TWICE ? 2 * i : i;
-            a.rows[i] = (int)t;  // read where a token has one row
+            a.pos[t] = i;
+            a.rows[i] = (int)t;
             if (!PROBS) a.lab[i] = (int)lab[k];
             if (PROBS) {
-                const float w = head_probs_row<TWICE>(a, t, TWICE ? 2 * i : i, (int)lab[k]);
+                const float w = head_probs_row(a, t, i, (int)lab[k]);
                 if (w <= 3.402823466e38f) gmax = fmaxf(gmax, w);
             } else if (a.coef) {
                 a.lse2[i] = fmaf(lse[k], kLog2e, -a.g_bits);
@@ -225,12 +227,13 @@ __global__ void __launch_bounds__(1024) head_rows_kernel(const __grid_constant__
         base += base_s;
         __syncthreads();
     }
+    const bool twice = PROBS && base <= kHeadTwice;
+    const int count = twice ? 2 * base : base;
     if (PACK) {
-        if (TWICE) base *= 2;
-        const int64_t g = gridDim.x, b = blockIdx.x, first = base + b;
+        const int64_t g = gridDim.x, b = blockIdx.x, first = count + b;
         const int64_t mine = (a.n - b + g - 1) / g;
         auto from = [&](int64_t r) { return b + r * g; };
-        if (TWICE) {
+        if (twice) {
             head_copy_rows(a, 2 * mine, [&](int64_t r) { return from(r / 2); }, [&](int64_t r) {
                 const int64_t to = spos[from(r / 2)];
                 return to >= 0 ? 2 * to + r % 2 : to;
@@ -238,14 +241,15 @@ __global__ void __launch_bounds__(1024) head_rows_kernel(const __grid_constant__
         } else {
             head_copy_rows(a, mine, from, [&](int64_t r) { return (int64_t)spos[from(r)]; });
         }
-        const int64_t padded = head_padded(base, TWICE ? 2 * a.n : a.n);
+        const int64_t padded = head_padded(count, a.room);
         if (first < padded)
             head_copy_rows(a, (padded - first + g - 1) / g, [](int64_t) { return (int64_t)-1; },
                            [&](int64_t r) { return first + r * g; });
     }
     if (!writes) return;
     if (tid == 0) {
-        *a.count = base;
+        a.count[0] = count;
+        if (PROBS) a.count[1] = twice ? 2 : 1;
         *a.done = 0;
     }
     if (PROBS) {
@@ -253,11 +257,29 @@ __global__ void __launch_bounds__(1024) head_rows_kernel(const __grid_constant__
         if (lane == 0) wmax[warp] = gmax;
         __syncthreads();
         gmax = warp_max(wmax[lane]);
-        for (int i = tid; i < base; i += 1024) {
-            const float w = a.row[i].w;
-            a.row[i].w = w == 0.0f ? 0.0f : w / gmax;
-        }
         if (tid == 0) *a.out_scale = gmax / a.g_scale;
+        if (!twice) {
+            for (int i = tid; i < base; i += 1024) {
+                const float w = a.row[i].w;
+                a.row[i].w = w == 0.0f ? 0.0f : w / gmax;
+            }
+            return;
+        }
+        const bool mine = tid < base;  // base <= kHeadTwice < 1024
+        float4 row = mine ? a.row[tid] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const int label = mine ? a.lab[tid] : 0;
+        const float row_lse = mine ? a.lse2[tid] : 0.0f, scale = mine ? a.row_scale[tid] : 0.0f;
+        row.w = row.w == 0.0f ? 0.0f : row.w / gmax;
+        __syncthreads();
+        if (mine) {
+            a.pos[a.rows[tid]] = 2 * tid;
+            for (int r = 2 * tid; r < 2 * tid + 2; ++r) {
+                a.row[r] = row;
+                a.lab[r] = label;
+                a.lse2[r] = row_lse;
+                a.row_scale[r] = scale;
+            }
+        }
         return;
     }
     if (!a.coef) return;
@@ -282,11 +304,11 @@ __global__ void __launch_bounds__(1024) head_rows_kernel(const __grid_constant__
 __global__ void __launch_bounds__(1024) head_pack_kernel(const __grid_constant__ HeadRows a) {
     pdl_wait();
     pdl_trigger();
-    const int live = *a.count;
-    const int64_t padded = head_padded(live, a.n), g = gridDim.x, b = blockIdx.x;
+    const int live = *a.count, half = a.row && a.count[1] == 2 ? 1 : 0;
+    const int64_t padded = head_padded(live, a.room), g = gridDim.x, b = blockIdx.x;
     if (b < padded)
         head_copy_rows(a, (padded - b + g - 1) / g,
-                       [&](int64_t r) { return b + r * g < live ? (int64_t)a.rows[b + r * g] : -1; },
+                       [&](int64_t r) { return b + r * g < live ? (int64_t)a.rows[(b + r * g) >> half] : -1; },
                        [&](int64_t r) { return b + r * g; });
 }
 
@@ -768,29 +790,27 @@ struct HeadRowGrad {
     }
 };
 
-// N numbers, times f, in 16 bits.  Where tokens are few a row of G comes twice, as
-// its rounding and as what that `left`, so that their sum is good to 2^-16 (f16: 2^-22).
+// N numbers, times f, in 16 bits; `left`: what that rounding leaves, in 16 bits.
 template <bool BF16, int N>
-__device__ __forceinline__ void head_round(const float (&v)[N], float f, uint32_t* w) {
+__device__ __forceinline__ void head_round(const float (&v)[N], float f, bool left, uint32_t* w) {
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) w[i] = pack16<BF16>(v[2 * i] * f, v[2 * i + 1] * f);
-}
-template <bool BF16, int N>
-__device__ __forceinline__ void head_round_twice(const float (&v)[N], float f, bool left, uint32_t* w) {
+    if (!left) return;
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
-        const uint32_t near = pack16<BF16>(v[2 * i] * f, v[2 * i + 1] * f);
-        const float2 r = BF16 ? make_float2(__uint_as_float(near << 16), __uint_as_float(near & 0xffff0000u))
-                              : __half22float2(*reinterpret_cast<const __half2*>(&near));
-        w[i] = left ? pack16<BF16>(fmaf(v[2 * i], f, -r.x), fmaf(v[2 * i + 1], f, -r.y)) : near;
+        const float2 r = BF16 ? make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u))
+                              : __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        w[i] = pack16<BF16>(fmaf(v[2 * i], f, -r.x), fmaf(v[2 * i + 1], f, -r.y));
     }
 }
 
 // Epilogue of the backward's product: G of the piece in 16 bits, as the tensor
-// cores take it for dW and dH.  G is rounded once, from fp32, which a sum over many
-// tokens or entries evens out (against 64 bits 1.9e-3 in bf16, 1.7e-3 of it the
-// output's own rounding); in dW of one token, all but an outer product, it stands
-// beside that rounding.  Rows from the count to the tile's end (or n) become zero.  The
+// cores take it for dW and dH.  G is rounded once, from fp32, which stands beside
+// the outputs' own rounding whatever the number of terms (a sum's error grows as the
+// sum does, and a label's entry is most of a row): with token weights 2.4e-3 against
+// 64 bits in both gradients where the outputs' rounding makes 1.7e-3 (f16 2.3e-4 to
+// 3.1e-4 and 2.1e-4), with 129 tokens as with 4096.  Without them a label's entry of
+// the loss's is a power of two but for p: 1.7e-3.  Rows from the count to the tile's end (or n) become zero.  The
 // logits are added up as in the forward, so that they are those that lse came
 // from: taken whole, one of 30 made of 8192 products is 2.3e-4 too small, which
 // is all of p - 1 for a label known with p = 0.9998.  That costs 1.4 to 2.4 % of a
@@ -799,9 +819,13 @@ __device__ __forceinline__ void head_round_twice(const float (&v)[N], float f, b
 // UNIT (f16): the G without token weights, beside the other where that is wanted
 // (3584 x 4096 x 32000 with weights: 2.26 -> 2.42 ms, 64 tokens 178 -> 183 us).
 // PROBS: the gradient of log probability and entropy (head_probs.cuh), whose rows
-// have coefficients of their own in `row`, and with TWICE come twice: odd rows are
-// what those before them left.
-template <bool BF16, bool UNIT, bool PROBS, bool TWICE>
+// have coefficients of their own in `row`.  Up to kHeadTwice live tokens each has two
+// rows: G's rounding and, in the odd ones, what that left, good together to 2^-16 (f16:
+// to 2^-20, and to 2^-40 of the largest weight), so that the outputs' rounding
+// alone is left.  All products have twice the rows: at 4096 x 32000 bf16, one row and
+// two, one token 188 and 190 us, 64 190 and 203, 128 199 and 225, 256 216 and 331, 1024
+// 570 and 1170, 4096 2620 and 5250.
+template <bool BF16, bool UNIT, bool PROBS>
 struct HeadGrad {
     static constexpr int kChunk = 8;
     static constexpr bool kLiveN = false;
@@ -811,14 +835,16 @@ struct HeadGrad {
     uint16_t* g;       // with UNIT: or null
     uint16_t* g_unit;  // with UNIT
     int64_t ldg;
-    int n;   // rows of g: the tokens
+    int n;   // rows of g
     int v0;  // first vocabulary entry of the piece
     const float4* row;  // with PROBS
+    const int* each;    // with PROBS: rows that a token has
     __device__ static void give_up(const PairTile&) {}
     __device__ __forceinline__ void finish(const PairTile& t, const float (&acc)[128]) const {
         const int r = t.row0 + t.lane;
         const bool in = r < t.M;
         const HeadRowGrad<BF16, PROBS> a(in, r, coef, lse2, row);
+        const bool left = PROBS && *each == 2 && (r & 1);
         const int lab_c = in ? lab[r] - v0 - t.col0 - t.c_begin : -1;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
@@ -830,13 +856,8 @@ struct HeadGrad {
                     float v[32];
                     head_slice(acc, 2 * b + h, v);
                     a.values(v, lab_c - 64 * b - 32 * h);
-                    if (TWICE) {
-                        head_round_twice<BF16>(v, a.f, r & 1, w + 16 * h);
-                        if (UNIT) head_round_twice<BF16>(v, a.u, r & 1, w1 + 16 * h);
-                    } else {
-                        head_round<BF16>(v, a.f, w + 16 * h);
-                        if (UNIT) head_round<BF16>(v, a.u, w1 + 16 * h);
-                    }
+                    head_round<BF16>(v, a.f, left, w + 16 * h);
+                    if (UNIT) head_round<BF16>(v, a.u, left, w1 + 16 * h);
                 }
                 const int cols = min(t.N, t.col0 + t.c_end);
                 if (!UNIT || g) pair_store16(t, w, c, g, ldg, n, cols);
@@ -848,7 +869,7 @@ struct HeadGrad {
 
 // The same with tokens as the tile's columns: each 32 x 32 block is turned over,
 // so that a thread has a token and 32 entries.
-template <bool BF16, bool UNIT, bool PROBS, bool TWICE>
+template <bool BF16, bool UNIT, bool PROBS>
 struct HeadGradT {
     static constexpr int kChunk = 8;
     static constexpr bool kLiveN = true;
@@ -861,8 +882,10 @@ struct HeadGradT {
     int n;
     int v0;
     const float4* row;
+    const int* each;
     __device__ static void give_up(const PairTile&) {}
     __device__ __forceinline__ void finish(const PairTile& t, const float (&acc)[128]) const {
+        const bool twice = PROBS && *each == 2;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
             const int c = t.c_begin + 32 * b;
@@ -875,13 +898,8 @@ struct HeadGradT {
             const HeadRowGrad<BF16, PROBS> a(in, token, coef, lse2, row);
             a.values(v, in ? lab[token] - v0 - t.row0 : -1);
             uint32_t w[16], w1[16];
-            if (TWICE) {
-                head_round_twice<BF16>(v, a.f, token & 1, w);
-                if (UNIT) head_round_twice<BF16>(v, a.u, token & 1, w1);
-            } else {
-                head_round<BF16>(v, a.f, w);
-                if (UNIT) head_round<BF16>(v, a.u, w1);
-            }
+            head_round<BF16>(v, a.f, twice && (token & 1), w);
+            if (UNIT) head_round<BF16>(v, a.u, twice && (token & 1), w1);
             if (!UNIT || g) store(t, w, c, g);
             if (UNIT) store(t, w1, c, g_unit);
         }
@@ -918,8 +936,8 @@ struct HeadGradT {
 
 // dH of every token in 16 bits: the slab's row, plus the further K ranges of
 // the tail's tiles in their order; zero for the tokens that took no part.  A
-// CTA takes 1024 columns of tokens, TOKENS of them in flight.  TWICE: a token's
-// two rows, added up.
+// CTA takes 1024 columns of tokens, TOKENS of them in flight.  PROBS: or one, where
+// tokens have two rows, which are added up.
 struct HeadDh {
     const float* slab;
     int64_t ld;
@@ -934,9 +952,7 @@ struct HeadDh {
     int64_t ldo;
 };
 template <bool BF16, int TOKENS, bool TWICE>
-__global__ void __launch_bounds__(128) head_dh_kernel(const HeadDh a) {
-    __shared__ int sh[5];
-    pdl_wait();
+__device__ __forceinline__ void head_dh(const HeadDh& a, int* sh) {
     if (threadIdx.x < 32) {
         const int count = *a.count, tiles_d = (a.d + 255) / 256;
         const int bt = a.live_n ? pair_live_bn(count) : 256, tiles_t = max((count + bt - 1) / bt, 1);
@@ -1008,6 +1024,13 @@ __global__ void __launch_bounds__(128) head_dh_kernel(const HeadDh a) {
             }
         }
     }
+}
+template <bool BF16, int TOKENS, bool PROBS>
+__global__ void __launch_bounds__(128) head_dh_kernel(const HeadDh a) {
+    __shared__ int sh[5];
+    pdl_wait();
+    if (PROBS && a.count[1] == 2) head_dh<BF16, 1, true>(a, sh);
+    else head_dh<BF16, TOKENS, false>(a, sh);
 }
 
 }  // namespace aeth

@@ -557,8 +557,10 @@ int aeth_cut_ce_backward(const void* hidden, int64_t ld_hidden, const void* weig
  *   256 entries where these take more), else not at all.
  *   backward: of sum_t grad_log_probs[t] log_probs[t] + grad_entropy[t] entropy[t]
  *   (either may be NULL: 0), lse and entropy being the forward's; G as the loss's,
- *   in F16 twice where d_hidden is wanted, and up to 128 tokens as its rounding and
- *   what that left, good to 2^-16 (F16: 2^-22). */
+ *   in F16 twice where d_hidden is wanted.  Up to 128 tokens that take part (whatever
+ *   n is) G is kept as its rounding and what that left, good to 2^-16 (F16: to 2^-20,
+ *   and to 2^-40 of the largest weight); with more it is rounded once, which makes the
+ *   gradients' error 1.4 times that of their own rounding. */
 int aeth_token_log_probs_workspace(int64_t n, int64_t d, int64_t vocab, int top, int backward, size_t* bytes);
 int aeth_token_log_probs(const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, int dtype,
                          const int64_t* labels, int64_t n, int64_t d, int64_t vocab, int64_t ignore_index, int top,

@@ -60,3 +60,32 @@ def test_results_are_tensors_of_their_own():
     r = A.token_log_probs(h.detach(), w.detach(), lab)
     dh, dw = A.token_log_probs_backward(h.detach(), w.detach(), lab, r, grad_log_probs=torch.ones(20, device="cuda"))
     assert torch.equal(h.grad, dh) and torch.equal(w.grad, dw)
+
+
+@pytest.mark.parametrize("live", [1, 2, 40, 128, 129])
+@pytest.mark.parametrize("n", [129, 200, 256, 300, 700, 1100, 8192, 9001])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_a_padded_batch_has_the_gradient_of_its_tokens(dt, n, live):
+    """As test_gradients_of_few_tokens, within its bounds (u^2 for G up to 128 tokens),
+    with the tokens anywhere among others that take no part."""
+    import aethelstream_b200 as A
+    from test_gpu_log_probs import IGNORE, U, close, grads, make, reference
+    h, w, lab = make(n, 264, 1200, dt, seed=n + live)
+    a, b = grads(n, 19)
+    a, b = a.sign() * (1.0 + 0.9 * U[dt]), 1e-3 * b
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    keep = torch.zeros(n, dtype=torch.bool, device="cuda")
+    keep[torch.randperm(n, generator=gen, device="cuda")[:live]] = True
+    e = reference(h[keep], w, lab[keep], a[keep], b[keep])
+    lab[~keep], h[~keep], a[~keep] = IGNORE, float("nan"), float("inf")
+    r = A.token_log_probs(h, w, lab)
+    close(r.entropy[keep], e["ent"], e["e_ent"])
+    dh, dw = A.token_log_probs_backward(h, w, lab, r, grad_log_probs=a, grad_entropy=b)
+    close(dh[keep], e["dh"], e["b_h"])
+    close(dw, e["dw"], e["b_w"])
+    assert (dh[~keep] == 0).all()
+    # the same where only one of the two is wanted
+    one = A.token_log_probs_backward(h, w, lab, r, grad_log_probs=a, grad_entropy=b, need_weight=False)[0]
+    two = A.token_log_probs_backward(h, w, lab, r, grad_log_probs=a, grad_entropy=b, need_hidden=False)[1]
+    assert torch.equal(one, dh)
+    close(two, e["dw"], e["b_w"])
