@@ -41,6 +41,9 @@ class RotaryPlan:
                 `original_length` positions stay, those below `beta_slow` turn
                 1 / factor as fast, between them a mixture that is linear in the
                 turns; cosines and sines are multiplied by 0.1 ln(factor) + 1.
+                Some programs mix linearly in the pair's index instead, between
+                the pairs at the two borders; their pairs in between turn at other
+                speeds, which a model trained so needs as `inv_freq`.
     `inv_freq` (rotary_dim / 2 numbers, radians a position) replaces the formula,
     `amplitude` the factor of cosines and sines."""
 
