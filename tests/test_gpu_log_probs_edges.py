@@ -89,3 +89,48 @@ def test_a_padded_batch_has_the_gradient_of_its_tokens(dt, n, live):
     two = A.token_log_probs_backward(h, w, lab, r, grad_log_probs=a, grad_entropy=b, need_hidden=False)[1]
     assert torch.equal(one, dh)
     close(two, e["dw"], e["b_w"])
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,live", [(3, 3), (20, 15), (300, 290)])
+@pytest.mark.parametrize("of", ["both", "log probabilities", "entropy"])
+def test_gradients_against_differences_in_64_bits(of, dt, n, live):
+    """Slopes of sum(a logp + b entropy) from values on both sides, in 64 bits: along
+    random directions and along the gradients themselves, where no sum cancels.
+
+    Half steps of 2^-12 of directions of length 1: the third derivative's part is below
+    1e-6 of a slope (logits change by 2^-12 |W| = 1e-3 at most), 64 bits' own rounding
+    below 1e-9.  A gradient's element is off by its rounding u and as much again where G
+    is rounded once (129 tokens on), which adds up along a direction z to 2 u sum |g z|
+    at most where all of G's error goes one way: along the gradient 2 u of the slope."""
+    import aethelstream_b200 as A
+    from test_gpu_log_probs import IGNORE, U, grads, make
+    h, w, lab = make(n, 64, 300, dt, seed=13)
+    lab[live:] = IGNORE
+    a, b = grads(n, 5)
+    r = A.token_log_probs(h, w, lab)
+    got = A.token_log_probs_backward(h, w, lab, r, grad_log_probs=None if of == "entropy" else a,
+                                     grad_entropy=None if of == "log probabilities" else b)
+    a, b = a * (of != "entropy"), b * (of != "log probabilities")
+
+    def value(x, y):
+        q = torch.log_softmax(x[:live] @ y.T, 1)
+        lp = q.gather(1, lab[:live, None])[:, 0]
+        return (lp * a[:live].double() - b[:live].double() * (q.exp() * q).sum(1)).sum().item()
+
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    for which, x in enumerate((h, w)):
+        g = got[which].double()
+        for along in (False, False, False, True):
+            z = g.clone() if along else torch.randn(x.shape, generator=gen, device="cuda", dtype=torch.float64)
+            z /= z.norm()
+            at = [h.double(), w.double()]
+            ends = []
+            for sign in (1, -1):
+                at[which] = x.double() + sign * 2.0 ** -12 * z
+                ends.append(value(*at))
+            slope = (ends[0] - ends[1]) * 2.0 ** 11
+            slack = 2.2 * U[dt] * (g * z).abs().sum().item() + 1e-5 * abs(slope) + 1e-8
+            assert abs(slope - (g * z).sum().item()) <= slack, (which, along)
+            assert not along or slack < abs(slope) / 50
+    assert (got[0][live:] == 0).all()
