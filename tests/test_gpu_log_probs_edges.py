@@ -134,3 +134,14 @@ def test_gradients_against_differences_in_64_bits(of, dt, n, live):
             assert abs(slope - (g * z).sum().item()) <= slack, (which, along)
             assert not along or slack < abs(slope) / 50
     assert (got[0][live:] == 0).all()
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,d,v", [(1, 1, 1), (1, 3, 2), (3, 1, 2), (4, 33, 129), (5, 3, 1), (40, 7, 600), (129, 1, 3), (130, 65, 257), (257, 5, 2),
+                                   (300, 129, 1001), (513, 31, 40), (1100, 13, 300)])
+def test_odd_features_and_single_entries(dt, n, d, v):
+    from test_gpu_log_probs import check, make
+    for masked in (0.0, 0.6):
+        h, w, lab = make(n, d, v, dt, seed=n + d + v, masked=masked)
+        check(h, w, lab, top=min(3, v))
+        check(h.view(1, n, 1, d).expand(2, n, 1, d)[1, :, 0], w.repeat(1, 2)[:, d:], lab)  # rows off 16 bytes
