@@ -91,8 +91,12 @@ void rot_grid(RotaryArgs& a, int64_t tokens, int step, int most) {
 // SM: 126 registers) 92, 102 and 110 in one, two and three.
 template <int OP>
 constexpr int rot_per_sm() { return OP == ROT_NORM_BACK ? 2 : 3; }
-// A CTA of more than one wave has eight passes (of all its groups) at least.
-constexpr int kRotPasses = 8;
+// Whole waves, whose CTAs have twelve passes (of all their groups) at least where there
+// are several: with 18 passes of one wave's CTAs, 8192 x (32 + 8) x 128 bf16, one wave takes
+// 32 and 34 us (rotation, norm), 2.3 and 2 waves 33 and 39, 1.15 waves 35 and 41; with
+// 9 and 13 passes (4096 and 6000 tokens) one wave 15 and 21, 21 and 27, two of half as
+// many 18 and 24, 25 and 33; with 37 (8192 x (64 + 8)) three waves 52, 1.15 waves 58.
+constexpr int kRotPasses = 12;
 template <int OP>
 constexpr int rot_waves() { return OP == ROT_TURN ? 3 : OP == ROT_NORM ? 2 : 1; }
 // CTAs of the gradient, each of which leaves sums of the gains', at most: rotary_kernel
@@ -108,7 +112,8 @@ int rot_launch(RotaryArgs& a, int64_t tokens, bool whole, cudaStream_t st) {
         const int groups = kRotThreads / lanes, held = kRotTableBytes / (4 * a.R);
         const int64_t rows = std::max(a.s[0].rows, a.s[1].rows);
         const int64_t passes = (rows + groups - 1) / groups, wave = (int64_t)rot_per_sm<OP>() * num_sms();
-        const unsigned ctas = (unsigned)std::min(passes, std::max(wave, std::min(rot_waves<OP>() * wave, passes / kRotPasses)));
+        const int64_t waves = std::clamp<int64_t>(passes / (kRotPasses * wave), 1, rot_waves<OP>());
+        const unsigned ctas = (unsigned)std::min(passes, waves * wave);
         int64_t most = 0;  // tokens that a CTA's rows have, and one more
         for (RotaryRows& s : a.s) {
             s.ctas = s.rows > 0 ? ctas : 0;
