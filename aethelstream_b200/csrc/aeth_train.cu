@@ -364,9 +364,13 @@ template <bool TOP>
 int probs_tiles(const ProbsPlan& p, const ProbsWork& w, HeadProbsOut out, const void* weight, int64_t ld_weight, int64_t n,
                 int64_t d, int64_t vocab, bool bf16, cudaStream_t st) {
     const PairOperand H{w.head.h, p.head.dp, n, d};
-    // Eight warps a token where tokens are few and ranges many: after the product, 155 tokens
-    // with five alternatives of 1024 ranges take 14 us for 27, 64 with twenty of 250 take 26 for 15.
-    const bool split = n <= 2 * num_sms() && p.ranges >= 512;
+    // Eight warps a token where tokens are few and ranges many, the more of these the more
+    // alternatives are wanted, since each warp takes as many.  Calls of 64 tokens (d 1024)
+    // with 1, 5, 20 and 32, eight warps a token and one: 250 ranges 30, 32, 44, 56 and 27, 28, 34,
+    // 39 us; 516 ranges 51, 53, 64, 74 and 55, 55, 60, 64; 1024 ranges 72, 74, 84, 94 and 81, 82, 89,
+    // 95; 2048 ranges 118, 120, 131, 140 and 143, 145, 151, 158.  Without alternatives, of 516 ranges,
+    // 36 and 38.5.  Eight tokens lose with twenty of 1024 (76 and 69).
+    const bool split = n <= 2 * num_sms() && p.ranges >= std::max(512, 32 * p.top);
     const unsigned ctas = (unsigned)std::min<int64_t>(split ? n : (n + 7) / 8, 8 * num_sms());
     for (int64_t v0 = 0; v0 < vocab; v0 += p.piece) {
         const int64_t vp = std::min(p.piece, vocab - v0);

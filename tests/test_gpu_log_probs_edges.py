@@ -145,3 +145,25 @@ def test_odd_features_and_single_entries(dt, n, d, v):
         h, w, lab = make(n, d, v, dt, seed=n + d + v, masked=masked)
         check(h, w, lab, top=min(3, v))
         check(h.view(1, n, 1, d).expand(2, n, 1, d)[1, :, 0], w.repeat(1, 2)[:, d:], lab)  # rows off 16 bytes
+
+
+@pytest.mark.parametrize("top", [16, 20, 32])
+@pytest.mark.parametrize("n", [5, 40, 296, 297])
+def test_many_alternatives_of_many_ranges(n, top):
+    """Eight warps a token with as many alternatives as there are, or one: equal logits
+    by the thousand, masks, a NaN; indices and their order exact."""
+    import aethelstream_b200 as A
+    from test_gpu_log_probs import IGNORE, close, grid
+    v = 140001
+    h, w, lab = grid(n, 64, v, torch.bfloat16, n, 2)
+    w[20000:60000] = w[7]
+    h[1, 3], lab[2] = float("nan"), IGNORE
+    r = A.token_log_probs(h, w, lab, top_k=top)
+    good = torch.ones(n, dtype=torch.bool, device="cuda")
+    good[1:3] = False
+    logs = torch.log_softmax(h.double() @ w.double().T, 1)
+    want = torch.argsort(logs, dim=1, descending=True, stable=True)[:, :top]
+    assert torch.equal(r.top_ids[good], want[good]) and (r.top_ids[1:3] == -1).all()
+    assert r.top_log_probs[1].isnan().all() and (r.top_log_probs[2] == 0).all()
+    bound = 2.0 ** -18 * (20 + logs.gather(1, want).abs())
+    close(r.top_log_probs[good], logs.gather(1, want)[good], bound[good])
