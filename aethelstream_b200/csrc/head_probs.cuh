@@ -57,7 +57,14 @@ __device__ __forceinline__ HeadSums head_join3(const HeadSums& a, const HeadSums
 __device__ __forceinline__ HeadSums head_shuffle(const HeadSums& a, int o) {
     return {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.u, o), 0.0f};
 }
-__device__ __forceinline__ float head_entropy(const HeadSums& a) { return logf(a.s) - kLn2 * (a.u / a.s); }
+// ln s and the entropy.  A whole row's s is 1 at least (the maximum's own term) and its
+// entropy 0, but for rounding, which may not make a log probability positive or an
+// entropy negative; s = 0 is a row of -infinity alone.
+__device__ __forceinline__ float head_log_sum(const HeadSums& a) { return a.s < 1.0f && a.s > 0.5f ? 0.0f : logf(a.s); }
+__device__ __forceinline__ float head_entropy(const HeadSums& a) {
+    const float e = head_log_sum(a) - kLn2 * (a.u / a.s);
+    return e < 0.0f ? 0.0f : e;
+}
 
 // Joins 32 logits, the first `left` of them, whatever they are.
 __device__ __forceinline__ void head_sums32(const float (&v)[32], int left, HeadSums& st) {
@@ -214,7 +221,7 @@ __device__ __forceinline__ void head_probs_write(const HeadProbsOut& a, int64_t 
     const float nan = __int_as_float(0x7fc00000);
     // one lane's: in the others the same sums were added the other way round
     const float m = __shfl_sync(0xffffffffu, bad ? nan : live ? head_base(x.m) : 0.0f, 0);
-    const float log_s = __shfl_sync(0xffffffffu, live ? logf(x.s) : 0.0f, 0), lse = m + log_s;
+    const float log_s = __shfl_sync(0xffffffffu, live ? head_log_sum(x) : 0.0f, 0), lse = m + log_s;
     // from a logit's distance to the maximum: without the rounding of a large lse
     auto log_prob = [&](float v) { return (v - m) - log_s; };
     if (lane == 0) {

@@ -167,3 +167,19 @@ def test_many_alternatives_of_many_ranges(n, top):
     assert r.top_log_probs[1].isnan().all() and (r.top_log_probs[2] == 0).all()
     bound = 2.0 ** -18 * (20 + logs.gather(1, want).abs())
     close(r.top_log_probs[good], logs.gather(1, want)[good], bound[good])
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [1, 4, 40, 256, 1100])
+def test_no_log_probability_above_zero_and_no_entropy_below(dt, n):
+    """Distributions of one entry, and nearly so, where a sum's rounding is all there is."""
+    import aethelstream_b200 as A
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    for v, scale in ((1, 1.0), (1, 100.0), (2, 8.0), (129, 8.0), (5000, 12.0)):
+        h = (scale * torch.randn(n, 64, generator=gen, device="cuda")).to(dt)
+        w = torch.randn(v, 64, generator=gen, device="cuda").to(dt)
+        lab = (h.float() @ w.float().T).argmax(1)
+        top = min(3, v)
+        for r in (A.token_log_probs(h, w, lab), A.token_log_probs(h, w, lab, top_k=top)):
+            assert (r.log_probs <= 0).all() and (r.entropy >= 0).all(), (v, r.log_probs.max().item(), r.entropy.min().item())
+        assert (r.top_log_probs <= 0).all()
