@@ -257,7 +257,8 @@ int head_backward(const HeadPlan& p, const HeadWork& w, const void* weight, int6
         }
         if (d_weight) {
             PairOut16<BF16> ew{static_cast<uint16_t*>(d_weight) + v0 * ld_dw, ld_dw, w.out_scale};
-            // half as wide where a wave takes them all (300 x 1272 x 686 39.7 -> 38.2 us, 1000 44.5 -> 42.4)
+            // half as wide where a wave takes them all (300 x 1272 x 686 39.7 -> 38.2 us, 1000 44.5 -> 42.4; with the
+            // narrower tiles of few tokens the loss's 58 -> 48 and 45 -> 43.5)
             const int bn = (vp + 255) / 256 * ((d + 127) / 128) <= pair_count() ? 128 : 256;
             AETH_TRY((pair_gemm_launch<PairOut16<BF16>, true, true>(G, H, (int)vp, (int)d, (int)n, w.count, PAIR_LIVE_K,
                                                                     bn, 0, BF16, ew, st)));

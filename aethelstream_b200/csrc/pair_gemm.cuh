@@ -191,7 +191,8 @@ struct PairShape {
         tiles_m = max((M + 255) / 256, 1);
         // Few tiles: narrower ones, where a wave takes them all (they too cover N
         // rounded up to 64; 300 x 4096 x 2000 bf16, log probabilities and their gradient
-        // 35 + 56 -> 27 + 48 us).  A split product's stay as its reader knows them.
+        // 35 + 56 -> 27 + 48 us, the loss and its 32 to 38 + 57 to 69 -> 27 to 31 + 50 to 63;
+        // 64 and 300 x 4096 x 32000 as before).  A split product's stay as its reader knows them.
         if (g.live_dim == PAIR_LIVE_N && g.tail_kb == 0)
             for (int narrow = 64; narrow < bn; narrow += 64)
                 if (tiles_m * ((N + narrow - 1) / narrow) <= (int)gridDim.x / 2) bn = narrow;

@@ -547,7 +547,8 @@ int aeth_cut_ce_backward(const void* hidden, int64_t ld_hidden, const void* weig
 /* Log probabilities of given tokens under softmax(hidden weight^T), with the
  * distributions' entropies and the likeliest entries; arguments as above.
  *   log_probs[t] = s_t,label - lse_t, entropy[t] = lse_t - sum_v p_tv s_tv (n
- *   floats each; lse too, for the backward).  top: the number of likeliest entries
+ *   floats each, taken against the largest logit; lse too, for the backward, where a
+ *   probability is good to 2^-24 of |lse|).  top: the number of likeliest entries
  *   wanted, 0 to 32 and at most vocab: their log probabilities, the largest first,
  *   and their indices (n x top; the lower index first among equal logits).
  *   Tokens with ignore_index get 0, and indices -1.  A label outside the vocabulary
